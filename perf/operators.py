@@ -12,6 +12,7 @@ pass cannot do without and ``exact`` evaluates a case in 64 bits.  With ``own``
 false ``run`` computes in elementary torch operations in 32 bits.
 """
 
+import functools
 import math
 import pathlib
 import sys
@@ -27,6 +28,7 @@ BYTES = {"bf16": 2, "fp16": 2, "fp32": 4}
 MAX_NODES = 64
 
 
+@functools.lru_cache(maxsize=None)
 def _package():
     pkg = str(pathlib.Path(__file__).resolve().parents[1] / "magenta-realtime-mlx-cpp_amd")
     if pkg not in sys.path:
