@@ -586,6 +586,92 @@ int mrt_coca_embed_time(mrt_coca* h, float* ms);
 /* Copy of an intermediate of the last embed_text (MRT_COCA_BUF_*); bytes must match. */
 int mrt_coca_read(mrt_coca* h, int which, void* dst, size_t bytes);
 
+/* ------------------------------------------------------------------------
+ * Operators for drafting decode over caches and weights of the caller's own.
+ * No counterpart in the reference, whose speculative path verifies one chain
+ * of drafts against no cache (decode.cpp:150-237).  A drafting step proposes a
+ * tree of tokens for each sequence, verifies all of them in one pass
+ * (mrt_tree_attention over the layer's cache).
+ *
+ * All pointers are DEVICE pointers on `device`; work is enqueued on
+ * `hip_stream` (a hipStream_t of that device; NULL = the null stream) and the
+ * call returns without waiting.  Nothing is allocated: a workspace, where an
+ * operator wants one, is the caller's, needs no initial contents, is aligned
+ * to 16 bytes and serves one call at a time (calls that may overlap, two
+ * captured graphs among them, take one each).  The calls may be captured into
+ * a HIP graph.  Sums, softmax statistics and scores are fp32 in every dtype;
+ * outputs are rounded to the dtype once.
+ * ------------------------------------------------------------------------ */
+
+/* The K/V of one layer for `rows` sequences.  k and v: (rows, kv_heads,
+ * capacity, d) in `dtype` -- the layout of MRT_BUF_TEMPORAL_K -- with element
+ * strides row_stride, head_stride and slot_stride (those of both; multiples of
+ * 16 bytes) and d contiguous; d a multiple of 8, at most 256.  Sequence b has
+ * length[b] entries, in slots 0 .. length[b] - 1 of every head (a length
+ * outside [0, capacity] is taken as the nearest bound); what the other slots
+ * hold is never looked at.  pos: NULL where an entry's slot is its position
+ * (the next token's is then length[b]); else (rows, kv_heads, capacity) int32
+ * positions, in any order, and next_pos (rows) the next token's.  score
+ * (rows, kv_heads, capacity) fp32: accumulated attention weights, or NULL. */
+typedef struct mrt_kv_cache {
+  void* k;
+  void* v;
+  int64_t row_stride;
+  int64_t head_stride;
+  int64_t slot_stride;
+  const int32_t* length;
+  int32_t* pos;
+  const int32_t* next_pos;
+  const float* score;
+  int32_t rows;
+  int32_t kv_heads;
+  int32_t capacity;
+  int32_t d;
+  int32_t dtype;
+} mrt_kv_cache;
+
+/* A (rows, nodes, heads, d) operand in the cache's dtype: element strides
+ * (multiples of 16 bytes), d contiguous, 16-byte aligned. */
+typedef struct mrt_node_rows {
+  void* data;
+  int64_t row_stride;
+  int64_t node_stride;
+  int64_t head_stride;
+} mrt_node_rows;
+
+/* Drafted tokens (nodes) a sequence may have in one call. */
+#define MRT_MAX_NODES 64
+
+typedef struct mrt_tree_attention_args {
+  mrt_node_rows q;        /* heads query heads */
+  mrt_node_rows k_new;    /* kv_heads heads: the nodes' own keys and values, which */
+  mrt_node_rows v_new;    /*   are not in the cache */
+  mrt_node_rows out;      /* heads heads */
+  const int32_t* parents; /* (rows, nodes) */
+  int64_t parents_stride; /* elements between sequences' parents; 0: one tree for all */
+  float* lse;             /* (rows, nodes, heads) fp32 log-sum-exp of the logits, or NULL */
+  const float* bias;      /* (heads, buckets) fp32 logit bias by distance, or NULL */
+  int32_t buckets;
+  int32_t nodes;          /* 1 .. MRT_MAX_NODES */
+  int32_t heads;          /* a multiple of kv_heads: heads / kv_heads query heads share a K/V head */
+  float scale;            /* 1 in this model (no 1/sqrt(d)) */
+} mrt_tree_attention_args;
+
+/* Attention of a tree of drafted tokens over the cache.  parents[b][t] is -1
+ * (node t follows the cache) or an earlier node of the sequence (< t); any
+ * other value means that node t is not there, as are its descendants: their
+ * outputs are 0, their lse -inf, and no other node is touched by them.  Node t
+ * attends every entry of the cache, its ancestors and itself:
+ *   logit(t, j) = scale * q_t . k_j + bias[h][min(max(p_t - p_j, 0), buckets - 1)]
+ * with p_t the next position plus the node's depth (0 under -1).  One node is
+ * an ordinary decode step.  K/V of a node that t does not see have no effect on
+ * t, whatever they hold.  Does not write the cache: mrt_cache_commit takes the
+ * accepted nodes into it.  mrt_tree_attention_workspace gives the workspace
+ * bytes for these sizes (0: none; workspace may then be NULL). */
+int mrt_tree_attention_workspace(const mrt_kv_cache* cache, int heads, int nodes, size_t* bytes);
+int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args* args, void* workspace,
+                       size_t workspace_bytes, int device, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

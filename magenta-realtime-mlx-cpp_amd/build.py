@@ -28,6 +28,7 @@ SOURCES = [
     "stream_kernels.hip",
     "batch_kernels.hip",
     "spec_kernels.hip",
+    "tree_attn.hip",
     "codec_kernels.hip",
     "conv_split.hip",
     "coca_kernels.hip",

@@ -10,6 +10,7 @@
 #include "coca.hpp"
 #include "codec.hpp"
 #include "kernels.hpp"
+#include "kv_cache.hpp"
 #include "model.hpp"
 #include "split_gemm.hpp"
 #include "stream.hpp"
@@ -167,6 +168,81 @@ mrt::CocaConfig to_coca_config(const mrt_coca_config* c) {
 mrt::Codec& CC(mrt_codec* c) {
   if (!c || !c->codec) throw mrt::Error(MRT_ERR_INVALID, "null codec handle");
   return *c->codec;
+}
+
+// ---- operators over caller-owned caches ---------------------------------------
+
+void require(bool ok, const char* msg) {
+  if (!ok) throw mrt::Error(MRT_ERR_INVALID, msg);
+}
+
+bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+// Makes `device` the calling thread's current one for the scope.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    MRT_HIP_CHECK(hipGetDevice(&before_));
+    if (before_ != device) MRT_HIP_CHECK(hipSetDevice(device));
+    changed_ = before_ != device;
+  }
+  ~OnDevice() {
+    if (changed_) (void)hipSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+};
+
+// Sizes and strides; the pointers only with `data`.
+mrt::KvCache to_cache(const mrt_kv_cache* c, bool data = true) {
+  require(c != nullptr, "null cache");
+  mrt::KvCache k;
+  k.dt = to_dtype(c->dtype);
+  require(c->rows >= 0 && c->kv_heads >= 1 && c->capacity >= 1, "cache: rows >= 0, kv_heads >= 1 and capacity >= 1");
+  require(c->d >= 8 && c->d <= mrt::kMaxHeadDim && c->d % 8 == 0, "cache: d must be a multiple of 8, 8..256");
+  require(static_cast<int64_t>(c->rows) * c->kv_heads <= (1 << 20), "cache: more than 2^20 (row, head) pairs");
+  if (data) {
+    require(c->k && c->v && c->length, "cache: null k, v or length");
+    require(aligned(c->k, 16) && aligned(c->v, 16), "cache: k and v must be 16-byte aligned");
+    const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(k.dt));
+    require(c->row_stride >= 0 && c->head_stride >= 0 && c->slot_stride >= 0, "cache: negative stride");
+    require(c->row_stride % unit == 0 && c->head_stride % unit == 0 && c->slot_stride % unit == 0,
+            "cache: strides must be multiples of 16 bytes");
+    require(c->capacity == 1 || c->slot_stride >= c->d, "cache: slots overlap");
+    require(c->pos == nullptr || c->next_pos != nullptr, "cache: pos without next_pos");
+  }
+  k.k = c->k, k.v = c->v;
+  k.row_stride = c->row_stride, k.head_stride = c->head_stride, k.slot_stride = c->slot_stride;
+  k.length = c->length, k.pos = c->pos, k.next_pos = c->next_pos, k.score = c->score;
+  k.rows = c->rows, k.kv_heads = c->kv_heads, k.capacity = c->capacity, k.d = c->d;
+  return k;
+}
+
+mrt::NodeRows to_nodes(const mrt_node_rows& r, const mrt::KvCache& c, const char* null_msg) {
+  require(r.data != nullptr, null_msg);
+  const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(c.dt));
+  require(aligned(r.data, 16), "nodes: operands must be 16-byte aligned");
+  require(r.row_stride >= 0 && r.node_stride >= 0 && r.head_stride >= 0, "nodes: negative stride");
+  require(r.row_stride % unit == 0 && r.node_stride % unit == 0 && r.head_stride % unit == 0,
+          "nodes: strides must be multiples of 16 bytes");
+  mrt::NodeRows n;
+  n.p = r.data, n.row_stride = r.row_stride, n.node_stride = r.node_stride, n.head_stride = r.head_stride;
+  return n;
+}
+
+void check_heads(const mrt::KvCache& c, int heads, int nodes) {
+  require(heads >= 1 && heads % c.kv_heads == 0, "heads must be a multiple of kv_heads");
+  require(heads <= 4096, "at most 4096 heads");
+  require(nodes >= 1 && nodes <= mrt::kMaxNodes, "nodes must be in 1..64");
+}
+
+void check_bias(const float* bias, int buckets) {
+  require(bias == nullptr || buckets >= 1, "bias without buckets");
+  require(bias == nullptr || aligned(bias, 4), "bias must be 4-byte aligned");
 }
 
 mrt::CodecConfig to_codec_config(const mrt_codec_config* c, int* max_frames) {
@@ -874,6 +950,43 @@ int mrt_coca_read(mrt_coca* h, int which, void* dst, size_t bytes) {
     if (bytes != n) throw mrt::Error(MRT_ERR_INVALID, "coca_read: size mismatch (" + std::to_string(n) + " bytes)");
     MRT_HIP_CHECK(hipMemcpyAsync(dst, src, n, hipMemcpyDefault, CO(h).stream));
     MRT_HIP_CHECK(hipStreamSynchronize(CO(h).stream));
+  });
+}
+
+int mrt_tree_attention_workspace(const mrt_kv_cache* cache, int heads, int nodes, size_t* bytes) {
+  return guarded([&] {
+    require(bytes != nullptr, "null argument");
+    const mrt::KvCache c = to_cache(cache, false);
+    check_heads(c, heads, nodes);
+    *bytes = mrt::tree_attention_workspace(c, heads, nodes);
+  });
+}
+
+int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args* args, void* workspace,
+                       size_t workspace_bytes, int device, void* hip_stream) {
+  return guarded([&] {
+    require(args != nullptr, "null argument");
+    const mrt::KvCache c = to_cache(cache);
+    check_heads(c, args->heads, args->nodes);
+    check_bias(args->bias, args->buckets);
+    mrt::TreeAttnArgs a;
+    a.q = to_nodes(args->q, c, "tree_attention: null q");
+    a.k_new = to_nodes(args->k_new, c, "tree_attention: null k_new");
+    a.v_new = to_nodes(args->v_new, c, "tree_attention: null v_new");
+    a.out = to_nodes(args->out, c, "tree_attention: null out");
+    require((c.rows <= 1 || a.out.row_stride > 0) && (args->nodes == 1 || a.out.node_stride >= c.d) &&
+                (args->heads == 1 || a.out.head_stride >= c.d),
+            "tree_attention: out overlaps itself");
+    require(args->parents != nullptr && args->parents_stride >= 0, "tree_attention: null parents or negative stride");
+    a.parents = args->parents, a.parents_stride = args->parents_stride;
+    a.lse = args->lse, a.bias = args->bias, a.buckets = args->bias ? args->buckets : 0;
+    a.nodes = args->nodes, a.heads = args->heads, a.scale = args->scale;
+    const size_t want = mrt::tree_attention_workspace(c, a.heads, a.nodes);
+    require(want == 0 || (workspace != nullptr && workspace_bytes >= want && aligned(workspace, 16)),
+            "tree_attention: workspace too small, misaligned or null");
+    if (c.rows == 0) return;
+    OnDevice on(device);
+    mrt::tree_attention(c, a, workspace, static_cast<hipStream_t>(hip_stream));
   });
 }
 

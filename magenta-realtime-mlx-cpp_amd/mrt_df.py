@@ -11,9 +11,11 @@ from __future__ import annotations
 
 import ctypes
 import dataclasses
+import functools
 import os
 import pathlib
 import re
+import struct
 from typing import Dict, Optional, Sequence
 
 import numpy as np
@@ -311,6 +313,8 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "mrt_df_batch_stream": (i32, [vp, ctypes.POINTER(vp)]),
         "mrt_df_batch_decode_time": (i32, [vp, ctypes.POINTER(ctypes.c_float)]),
         "mrt_df_batch_read_enc_out": (i32, [vp, vp, sz]),
+        "mrt_tree_attention_workspace": (i32, [vp, i32, i32, ctypes.POINTER(sz)]),
+        "mrt_tree_attention": (i32, [vp, vp, vp, sz, i32, vp]),
         "mrt_codec_config_default": (None, [ctypes.POINTER(_CodecConfig)]),
         "mrt_codec_create": (i32, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_CodecConfig), i32,
                                    ctypes.POINTER(vp)]),
@@ -1104,3 +1108,141 @@ class StyleModel:
             self.close()
         except Exception:  # noqa: BLE001
             pass
+
+
+# ---- operators for drafting decode over the caller's own tensors --------------------
+#
+# A small call takes the GPU a few microseconds, so the binding keeps its own share
+# low: structures are packed in one go, messages are built when a check fails, the
+# current stream is taken as a raw handle.
+
+MAX_NODES = 64
+_CACHE_STRUCT = struct.Struct("PPqqqPPPPiiiiixxxx")           # mrt_kv_cache
+_TREE_STRUCT = struct.Struct("PqqqPqqqPqqqPqqqPqPPiiif")  # mrt_tree_attention_args
+
+
+def _dtype_code(torch_dtype) -> int:
+    if not _TORCH_CODE:
+        torch = _torch()
+        _TORCH_CODE.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16})
+    return _TORCH_CODE.get(torch_dtype, -1)
+
+
+_TORCH_CODE: Dict = {}
+
+
+class KVCache:
+    """One layer's K/V of ``rows`` sequences in the caller's tensors (mrt_kv_cache).
+
+    k, v: (rows, kv_heads, capacity, d) of one dtype and the same strides, d
+    contiguous; length (rows) int32, the entries in use.  After evictions also
+    pos (rows, kv_heads, capacity) int32, each entry's position, and next_pos
+    (rows) int32, the next token's; score (rows, kv_heads, capacity) fp32 holds
+    the attention weights accumulated by ``cache_commit``.  The tensors are
+    kept, not copied.
+    """
+
+    __slots__ = ("k", "v", "length", "pos", "next_pos", "score", "index", "dtype", "shape", "_c")
+
+    def __init__(self, k, v, length, pos=None, next_pos=None, score=None):
+        code, shape, stride, index = _dtype_code(k.dtype), k.shape, k.stride(), k.get_device()
+        if code < 0 or len(shape) != 4 or stride[3] != 1:
+            raise ValueError("cache: k must be (rows, kv_heads, capacity, d) fp32, bf16 or fp16, d contiguous")
+        if v.shape != shape or v.dtype is not k.dtype or v.stride() != stride or v.get_device() != index:
+            raise ValueError("cache: v must have k's shape, dtype, strides and device")
+        if index < 0:
+            raise ValueError("cache: the tensors must be on a GPU")
+        slots = shape[:3]
+        self.index, self.dtype, self.shape = index, k.dtype, shape
+        lp = _ints(length, shape[:1], index, "length")
+        pp = np_ = sp = None
+        if pos is not None or next_pos is not None:
+            if pos is None or next_pos is None:
+                raise ValueError("cache: pos and next_pos go together")
+            pp, np_ = _ints(pos, slots, index, "pos"), _ints(next_pos, shape[:1], index, "next_pos")
+        if score is not None:
+            sp = _floats(score, slots, index, "score")
+        self.k, self.v, self.length, self.pos, self.next_pos, self.score = k, v, length, pos, next_pos, score
+        self._c = _CACHE_STRUCT.pack(k.data_ptr(), v.data_ptr(), stride[0], stride[1], stride[2], lp, pp or 0, np_ or 0,
+                                     sp or 0, shape[0], shape[1], shape[2], shape[3], code)
+
+
+def _ints(t, shape, index, what) -> int:
+    """Pointer of a contiguous int32 tensor of this shape on GPU ``index``."""
+    if t.shape != shape or t.dtype is not _torch().int32 or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous int32 {tuple(shape)} on GPU {index}")
+    return t.data_ptr()
+
+
+def _floats(t, shape, index, what) -> int:
+    if t.shape != shape or t.dtype is not _torch().float32 or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous fp32 {tuple(shape)} on GPU {index}")
+    return t.data_ptr()
+
+
+def _nodes(t, shape, cache, what):
+    """Pointer and strides of a (rows, nodes, heads, d) operand."""
+    s = t.stride()
+    if t.shape != shape or t.dtype is not cache.dtype or t.get_device() != cache.index or s[3] != 1:
+        raise ValueError(f"{what} must be {tuple(shape)} in the cache's dtype, on its GPU, d contiguous")
+    return t.data_ptr(), s[0], s[1], s[2]
+
+
+def _bias_table(bias, heads, cache):
+    if bias is None:
+        return 0, 0
+    if bias.dim() != 2:
+        raise ValueError("bias must be (heads, buckets)")
+    return _floats(bias, (heads, bias.shape[1]), cache.index, "bias"), bias.shape[1]
+
+
+def _raw_stream(index: int) -> int:
+    """torch's current stream on GPU ``index``, as a hipStream_t."""
+    return _torch()._C._cuda_getCurrentRawStream(index)
+
+
+@functools.lru_cache(maxsize=1024)
+def _tree_workspace(rows, kv_heads, capacity, d, dtype, heads, nodes) -> int:
+    lib, size = load_library(), ctypes.c_size_t()
+    c = _CACHE_STRUCT.pack(0, 0, 0, 0, 0, 0, 0, 0, 0, rows, kv_heads, capacity, d, _dtype_code(dtype))
+    _check(lib, lib.mrt_tree_attention_workspace(c, heads, nodes, ctypes.byref(size)))
+    return size.value
+
+
+def tree_attention(q, k_new, v_new, cache: KVCache, parents, scale: float = 1.0, bias=None, out=None, lse=None):
+    """Attention of a tree of drafted tokens over ``cache`` (mrt_tree_attention).
+
+    q (rows, nodes, heads, d), k_new / v_new (rows, nodes, kv_heads, d); parents
+    int32 (rows, nodes), or (nodes,) for one tree: -1 follows the cache, an
+    earlier node is that node's child, anything else is not there.  bias: fp32
+    (heads, buckets) by distance.  Returns (out (rows, nodes, heads, d), lse
+    (rows, nodes, heads) fp32), new tensors unless given, enqueued on torch's
+    current stream.  One node is an ordinary decode step.
+    """
+    torch, lib, index = _torch(), load_library(), cache.index
+    shape = q.shape
+    if len(shape) != 4:
+        raise ValueError("q must be (rows, nodes, heads, d)")
+    rows, nodes, heads, d = shape
+    _, kv_heads, capacity, _ = cache.shape
+    if rows != cache.shape[0] or d != cache.shape[3]:
+        raise ValueError("q must have the cache's rows and d")
+    qp = _nodes(q, shape, cache, "q")
+    new = (rows, nodes, kv_heads, d)
+    kp, vp = _nodes(k_new, new, cache, "k_new"), _nodes(v_new, new, cache, "v_new")
+    if out is None:
+        out = torch.empty(shape, dtype=q.dtype, device=q.device)
+    op = _nodes(out, shape, cache, "out")
+    if lse is None:
+        lse = torch.empty((rows, nodes, heads), dtype=torch.float32, device=q.device)
+    one = parents.dim() == 1
+    tp = _ints(parents, (nodes,) if one else (rows, nodes), index, "parents")
+    table, buckets = _bias_table(bias, heads, cache)
+    args = _TREE_STRUCT.pack(*qp, *kp, *vp, *op, tp, 0 if one else nodes,
+                             _floats(lse, (rows, nodes, heads), index, "lse"), table, buckets, nodes, heads, scale)
+    size = _tree_workspace(rows, kv_heads, capacity, d, cache.dtype, heads, nodes)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    code = lib.mrt_tree_attention(cache._c, args, ws.data_ptr() if size else None, size, index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+    return out, lse
