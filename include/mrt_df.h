@@ -590,8 +590,10 @@ int mrt_coca_read(mrt_coca* h, int which, void* dst, size_t bytes);
  * Operators for drafting decode over caches and weights of the caller's own.
  * No counterpart in the reference, whose speculative path verifies one chain
  * of drafts against no cache (decode.cpp:150-237).  A drafting step proposes a
- * tree of tokens for each sequence, verifies all of them in one pass
- * (mrt_tree_attention over the layer's cache).
+ * tree of tokens for each sequence (its products may come from 4-bit weights:
+ * mrt_q4_matmul), verifies all of them in one pass (mrt_tree_attention over
+ * each layer's cache), takes the accepted path into the cache
+ * (mrt_cache_commit) and holds the cache to a budget (mrt_cache_evict).
  *
  * All pointers are DEVICE pointers on `device`; work is enqueued on
  * `hip_stream` (a hipStream_t of that device; NULL = the null stream) and the
@@ -671,6 +673,72 @@ typedef struct mrt_tree_attention_args {
 int mrt_tree_attention_workspace(const mrt_kv_cache* cache, int heads, int nodes, size_t* bytes);
 int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args* args, void* workspace,
                        size_t workspace_bytes, int device, void* hip_stream);
+
+typedef struct mrt_cache_commit_args {
+  mrt_node_rows k_new;     /* kv_heads heads: as given to mrt_tree_attention */
+  mrt_node_rows v_new;
+  mrt_node_rows q;         /* heads heads; data NULL: commit without weights */
+  const int32_t* accepted; /* (rows, accepted_n) node ids, ascending */
+  int64_t accepted_stride; /* elements between sequences */
+  const float* lse;        /* (rows, nodes, heads) of mrt_tree_attention; with q */
+  const float* bias;       /* as there */
+  float* score_out;        /* (rows, kv_heads, capacity); with q; may be cache->score */
+  int32_t* length_out;     /* (rows), not cache->length */
+  int32_t* next_out;       /* (rows), not cache->next_pos; with cache->pos */
+  int32_t accepted_n;      /* 1 .. MRT_MAX_NODES */
+  int32_t nodes;
+  int32_t heads;
+  int32_t buckets;
+  float scale;
+} mrt_cache_commit_args;
+
+/* Takes the accepted path of a drafted tree into the cache.  Of accepted[b] the
+ * longest prefix of ascending node ids in [0, nodes) counts that the cache has
+ * room for: n tokens (a negative id ends it).  Token i's key and value go to
+ * slot length + i, its position next + i to pos; length_out = length + n and
+ * next_out = next + n.  With q, the attention weights that these tokens gave to
+ * each entry, summed over the query heads that share a K/V head, are added up:
+ *   score_out[j] = score[j] (0 for the n new entries and where score is NULL)
+ *     + sum over i, h of [j <= length + i] * exp(logit(i, j) - lse[accepted_i][h])
+ * for the length + n entries; what score_out holds past them stays.  A token
+ * whose lse is -inf gives no weight. */
+int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* args, int device, void* hip_stream);
+
+typedef struct mrt_cache_evict_args {
+  float* score_out;    /* (rows, kv_heads, capacity); may be cache->score */
+  int32_t* pos_out;    /* (rows, kv_heads, capacity); may be cache->pos */
+  int32_t* length_out; /* (rows), not cache->length */
+  int32_t keep;        /* entries a sequence keeps, >= 1 */
+  int32_t recent;      /* the entries of the last `recent` positions stay, */
+  int32_t sinks;       /*   and those of the first `sinks`; recent + sinks <= keep */
+} mrt_cache_evict_args;
+
+/* Evicts the entries with the least accumulated attention weight, per sequence
+ * and K/V head, down to length_out = min(length, keep).  Entries at positions
+ * >= next_pos - recent or < sinks stay; of the others those with the highest
+ * score, equal ones by the lower slot (a NaN score counts as -inf).  Kept
+ * entries below length_out stay in their slots; those at or above it move into
+ * the evicted slots, the lower into the lower: pos is what tells an entry's
+ * place, not its slot.  Rows of k and v move in place; score_out and pos_out
+ * receive the entries' scores and positions; nothing past length_out is
+ * written.  Needs pos, next_pos and score. */
+int mrt_cache_evict_workspace(const mrt_kv_cache* cache, int keep, size_t* bytes);
+int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args, void* workspace,
+                    size_t workspace_bytes, int device, void* hip_stream);
+
+/* out (rows, n) = x (rows, k) W^T with 4-bit weights: W[n][k] = scales[n][g] *
+ * code + biases[n][g], codes 0..15, eight to a 32-bit word of w (n, k / 8), the
+ * first in the low bits; scales and biases (n, k / group), g = k / group, group
+ * 32, 64 or 128, a divisor of k.  x, scales, biases and out in `dtype`, row
+ * strides ldx (a multiple of 16 bytes) and ldo in elements; w and x 16-byte
+ * aligned.  Meant for few rows: each 64 rows read the weights again.  Weights
+ * are multiplied exactly and summed in fp32; a row of x that is not
+ * finite gives outputs that are not.  mrt_q4_quantize makes the codes of src (n, k), row
+ * stride ld: bias the group's least weight, scale a 15th of its range. */
+int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const void* scales, const void* biases,
+                  int n, int k, int group, int dtype, void* out, int64_t ldo, int device, void* hip_stream);
+int mrt_q4_quantize(const void* src, int64_t ld, int n, int k, int group, int dtype, uint32_t* w, void* scales,
+                    void* biases, int device, void* hip_stream);
 
 #ifdef __cplusplus
 }

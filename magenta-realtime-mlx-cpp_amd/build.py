@@ -29,6 +29,8 @@ SOURCES = [
     "batch_kernels.hip",
     "spec_kernels.hip",
     "tree_attn.hip",
+    "cache_ops.hip",
+    "q4.hip",
     "codec_kernels.hip",
     "conv_split.hip",
     "coca_kernels.hip",

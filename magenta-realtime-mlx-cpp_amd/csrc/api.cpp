@@ -12,6 +12,7 @@
 #include "kernels.hpp"
 #include "kv_cache.hpp"
 #include "model.hpp"
+#include "q4.hpp"
 #include "split_gemm.hpp"
 #include "stream.hpp"
 
@@ -178,6 +179,9 @@ void require(bool ok, const char* msg) {
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// The stride of a dimension of `size` entries (that of a single entry is never used).
+bool stride_ok(int64_t stride, int size, int64_t unit) { return size <= 1 || (stride >= 0 && stride % unit == 0); }
+
 // Makes `device` the calling thread's current one for the scope.
 class OnDevice {
  public:
@@ -209,9 +213,9 @@ mrt::KvCache to_cache(const mrt_kv_cache* c, bool data = true) {
     require(c->k && c->v && c->length, "cache: null k, v or length");
     require(aligned(c->k, 16) && aligned(c->v, 16), "cache: k and v must be 16-byte aligned");
     const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(k.dt));
-    require(c->row_stride >= 0 && c->head_stride >= 0 && c->slot_stride >= 0, "cache: negative stride");
-    require(c->row_stride % unit == 0 && c->head_stride % unit == 0 && c->slot_stride % unit == 0,
-            "cache: strides must be multiples of 16 bytes");
+    require(stride_ok(c->row_stride, c->rows, unit) && stride_ok(c->head_stride, c->kv_heads, unit) &&
+                stride_ok(c->slot_stride, c->capacity, unit),
+            "cache: strides must be multiples of 16 bytes, not negative");
     require(c->capacity == 1 || c->slot_stride >= c->d, "cache: slots overlap");
     require(c->pos == nullptr || c->next_pos != nullptr, "cache: pos without next_pos");
   }
@@ -222,13 +226,13 @@ mrt::KvCache to_cache(const mrt_kv_cache* c, bool data = true) {
   return k;
 }
 
-mrt::NodeRows to_nodes(const mrt_node_rows& r, const mrt::KvCache& c, const char* null_msg) {
+mrt::NodeRows to_nodes(const mrt_node_rows& r, const mrt::KvCache& c, int nodes, int heads, const char* null_msg) {
   require(r.data != nullptr, null_msg);
   const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(c.dt));
   require(aligned(r.data, 16), "nodes: operands must be 16-byte aligned");
-  require(r.row_stride >= 0 && r.node_stride >= 0 && r.head_stride >= 0, "nodes: negative stride");
-  require(r.row_stride % unit == 0 && r.node_stride % unit == 0 && r.head_stride % unit == 0,
-          "nodes: strides must be multiples of 16 bytes");
+  require(stride_ok(r.row_stride, c.rows, unit) && stride_ok(r.node_stride, nodes, unit) &&
+              stride_ok(r.head_stride, heads, unit),
+          "nodes: strides must be multiples of 16 bytes, not negative");
   mrt::NodeRows n;
   n.p = r.data, n.row_stride = r.row_stride, n.node_stride = r.node_stride, n.head_stride = r.head_stride;
   return n;
@@ -238,6 +242,12 @@ void check_heads(const mrt::KvCache& c, int heads, int nodes) {
   require(heads >= 1 && heads % c.kv_heads == 0, "heads must be a multiple of kv_heads");
   require(heads <= 4096, "at most 4096 heads");
   require(nodes >= 1 && nodes <= mrt::kMaxNodes, "nodes must be in 1..64");
+}
+
+void check_q4(int n, int k, int group) {
+  require(group == 32 || group == 64 || group == 128, "4-bit weights: group must be 32, 64 or 128");
+  require(n >= 1 && n <= (1 << 28) && k >= group && k <= (1 << 20) && k % group == 0,
+          "4-bit weights: n in 1..2^28 and k a multiple of group, at most 2^20");
 }
 
 void check_bias(const float* bias, int buckets) {
@@ -970,10 +980,10 @@ int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args*
     check_heads(c, args->heads, args->nodes);
     check_bias(args->bias, args->buckets);
     mrt::TreeAttnArgs a;
-    a.q = to_nodes(args->q, c, "tree_attention: null q");
-    a.k_new = to_nodes(args->k_new, c, "tree_attention: null k_new");
-    a.v_new = to_nodes(args->v_new, c, "tree_attention: null v_new");
-    a.out = to_nodes(args->out, c, "tree_attention: null out");
+    a.q = to_nodes(args->q, c, args->nodes, args->heads, "tree_attention: null q");
+    a.k_new = to_nodes(args->k_new, c, args->nodes, c.kv_heads, "tree_attention: null k_new");
+    a.v_new = to_nodes(args->v_new, c, args->nodes, c.kv_heads, "tree_attention: null v_new");
+    a.out = to_nodes(args->out, c, args->nodes, args->heads, "tree_attention: null out");
     require((c.rows <= 1 || a.out.row_stride > 0) && (args->nodes == 1 || a.out.node_stride >= c.d) &&
                 (args->heads == 1 || a.out.head_stride >= c.d),
             "tree_attention: out overlaps itself");
@@ -987,6 +997,99 @@ int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args*
     if (c.rows == 0) return;
     OnDevice on(device);
     mrt::tree_attention(c, a, workspace, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* args, int device, void* hip_stream) {
+  return guarded([&] {
+    require(args != nullptr, "null argument");
+    const mrt::KvCache c = to_cache(cache);
+    check_heads(c, args->heads, args->nodes);
+    check_bias(args->bias, args->buckets);
+    mrt::CommitArgs a;
+    a.k_new = to_nodes(args->k_new, c, args->nodes, c.kv_heads, "cache_commit: null k_new");
+    a.v_new = to_nodes(args->v_new, c, args->nodes, c.kv_heads, "cache_commit: null v_new");
+    if (args->q.data != nullptr) {
+      a.q = to_nodes(args->q, c, args->nodes, args->heads, "cache_commit: null q");
+      require(args->lse != nullptr && args->score_out != nullptr, "cache_commit: q without lse or score_out");
+    }
+    require(args->accepted != nullptr && args->accepted_stride >= 0, "cache_commit: null accepted or negative stride");
+    require(args->accepted_n >= 1 && args->accepted_n <= mrt::kMaxNodes, "cache_commit: accepted_n must be in 1..64");
+    require(args->length_out != nullptr && args->length_out != c.length,
+            "cache_commit: length_out must be an array of its own");
+    require(c.pos == nullptr || (args->next_out != nullptr && args->next_out != c.next_pos),
+            "cache_commit: next_out must be an array of its own");
+    a.accepted = args->accepted, a.accepted_stride = args->accepted_stride, a.lse = args->lse, a.bias = args->bias;
+    a.score_out = args->score_out, a.length_out = args->length_out, a.next_out = args->next_out;
+    a.accepted_n = args->accepted_n, a.nodes = args->nodes, a.heads = args->heads;
+    a.buckets = args->bias ? args->buckets : 0, a.scale = args->scale;
+    if (c.rows == 0) return;
+    OnDevice on(device);
+    mrt::cache_commit(c, a, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_cache_evict_workspace(const mrt_kv_cache* cache, int keep, size_t* bytes) {
+  return guarded([&] {
+    require(bytes != nullptr, "null argument");
+    const mrt::KvCache c = to_cache(cache, false);
+    require(keep >= 1, "cache_evict: keep must be >= 1");
+    *bytes = mrt::cache_evict_workspace(c, keep);
+  });
+}
+
+int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args, void* workspace,
+                    size_t workspace_bytes, int device, void* hip_stream) {
+  return guarded([&] {
+    require(args != nullptr, "null argument");
+    const mrt::KvCache c = to_cache(cache);
+    require(c.pos != nullptr && c.score != nullptr, "cache_evict: the cache needs pos, next_pos and score");
+    require(args->score_out != nullptr && args->pos_out != nullptr, "cache_evict: null score_out or pos_out");
+    require(args->length_out != nullptr && args->length_out != c.length,
+            "cache_evict: length_out must be an array of its own");
+    require(args->keep >= 1 && args->recent >= 0 && args->sinks >= 0 &&
+                static_cast<int64_t>(args->recent) + args->sinks <= args->keep,
+            "cache_evict: keep >= 1, recent >= 0, sinks >= 0 and recent + sinks <= keep");
+    const size_t want = mrt::cache_evict_workspace(c, args->keep);
+    require(want == 0 || (workspace != nullptr && workspace_bytes >= want && aligned(workspace, 16)),
+            "cache_evict: workspace too small, misaligned or null");
+    mrt::EvictArgs a;
+    a.score_out = args->score_out, a.pos_out = args->pos_out, a.length_out = args->length_out;
+    a.keep = args->keep, a.recent = args->recent, a.sinks = args->sinks;
+    if (c.rows == 0) return;
+    OnDevice on(device);
+    mrt::cache_evict(c, a, workspace, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const void* scales, const void* biases,
+                  int n, int k, int group, int dtype, void* out, int64_t ldo, int device, void* hip_stream) {
+  return guarded([&] {
+    const mrt::DType dt = to_dtype(dtype);
+    const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(dt));
+    check_q4(n, k, group);
+    require(rows >= 0 && rows <= (1 << 20), "q4_matmul: rows must be in 0..2^20");
+    require(x && w && scales && biases && out, "q4_matmul: null argument");
+    require(aligned(x, 16) && aligned(w, 16), "q4_matmul: x and w must be 16-byte aligned");
+    require(rows <= 1 || (ldx >= k && ldx % unit == 0), "q4_matmul: ldx must be >= k, a multiple of 16 bytes");
+    require(rows <= 1 || ldo >= n, "q4_matmul: ldo must be >= n");
+    if (rows == 0) return;
+    mrt::Q4Weights q;
+    q.w = w, q.scales = scales, q.biases = biases, q.n = n, q.k = k, q.group = group;
+    OnDevice on(device);
+    mrt::q4_matmul(dt, q, x, ldx, rows, out, ldo, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_q4_quantize(const void* src, int64_t ld, int n, int k, int group, int dtype, uint32_t* w, void* scales,
+                    void* biases, int device, void* hip_stream) {
+  return guarded([&] {
+    const mrt::DType dt = to_dtype(dtype);
+    check_q4(n, k, group);
+    require(src && w && scales && biases, "q4_quantize: null argument");
+    require(ld >= k || n == 1, "q4_quantize: ld must be >= k");
+    OnDevice on(device);
+    mrt::q4_quantize(dt, src, ld, n, k, group, w, scales, biases, static_cast<hipStream_t>(hip_stream));
   });
 }
 

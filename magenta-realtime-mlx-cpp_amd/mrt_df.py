@@ -315,6 +315,11 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "mrt_df_batch_read_enc_out": (i32, [vp, vp, sz]),
         "mrt_tree_attention_workspace": (i32, [vp, i32, i32, ctypes.POINTER(sz)]),
         "mrt_tree_attention": (i32, [vp, vp, vp, sz, i32, vp]),
+        "mrt_cache_commit": (i32, [vp, vp, i32, vp]),
+        "mrt_cache_evict_workspace": (i32, [vp, i32, ctypes.POINTER(sz)]),
+        "mrt_cache_evict": (i32, [vp, vp, vp, sz, i32, vp]),
+        "mrt_q4_matmul": (i32, [vp, ctypes.c_int64, i32, vp, vp, vp, i32, i32, i32, i32, vp, ctypes.c_int64, i32, vp]),
+        "mrt_q4_quantize": (i32, [vp, ctypes.c_int64, i32, i32, i32, i32, vp, vp, vp, i32, vp]),
         "mrt_codec_config_default": (None, [ctypes.POINTER(_CodecConfig)]),
         "mrt_codec_create": (i32, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_CodecConfig), i32,
                                    ctypes.POINTER(vp)]),
@@ -1117,8 +1122,10 @@ class StyleModel:
 # current stream is taken as a raw handle.
 
 MAX_NODES = 64
-_CACHE_STRUCT = struct.Struct("PPqqqPPPPiiiiixxxx")           # mrt_kv_cache
-_TREE_STRUCT = struct.Struct("PqqqPqqqPqqqPqqqPqPPiiif")  # mrt_tree_attention_args
+_CACHE_STRUCT = struct.Struct("PPqqqPPPPiiiiixxxx")             # mrt_kv_cache
+_TREE_STRUCT = struct.Struct("PqqqPqqqPqqqPqqqPqPPiiif")      # mrt_tree_attention_args
+_COMMIT_STRUCT = struct.Struct("PqqqPqqqPqqqPqPPPPPiiiifxxxx")  # mrt_cache_commit_args
+_EVICT_STRUCT = struct.Struct("PPPiiixxxx")                     # mrt_cache_evict_args
 
 
 def _dtype_code(torch_dtype) -> int:
@@ -1246,3 +1253,114 @@ def tree_attention(q, k_new, v_new, cache: KVCache, parents, scale: float = 1.0,
     if code:
         _check(lib, code)
     return out, lse
+
+
+def cache_commit(cache: KVCache, k_new, v_new, accepted, length_out, next_out=None, q=None, lse=None, score_out=None,
+                 scale: float = 1.0, bias=None) -> None:
+    """Takes the accepted path of a drafted tree into ``cache`` (mrt_cache_commit).
+
+    accepted int32 (rows, n <= 64): ascending node ids of k_new / v_new (rows,
+    nodes, kv_heads, d), ended by a negative one.  length_out and, where the
+    cache has positions, next_out receive the new lengths and next positions
+    (tensors of their own).  With q and lse as in ``tree_attention`` the
+    attention weights of the accepted tokens are added to the cache's scores
+    into score_out (which may be the cache's).
+    """
+    lib, index = load_library(), cache.index
+    rows, kv_heads, capacity, d = cache.shape
+    new = k_new.shape
+    if len(new) != 4 or new[0] != rows or new[2] != kv_heads or new[3] != d:
+        raise ValueError("k_new must be (rows, nodes, kv_heads, d)")
+    nodes, heads, qp, lp, sp, table, buckets = new[1], kv_heads, (0, 0, 0, 0), 0, 0, 0, 0
+    if q is not None:
+        if lse is None or score_out is None or q.dim() != 4:
+            raise ValueError("q (rows, nodes, heads, d) needs lse and score_out")
+        heads = q.shape[2]
+        qp = _nodes(q, (rows, nodes, heads, d), cache, "q")
+        lp = _floats(lse, (rows, nodes, heads), index, "lse")
+        sp = _floats(score_out, (rows, kv_heads, capacity), index, "score_out")
+        table, buckets = _bias_table(bias, heads, cache)
+    if accepted.dim() != 2:
+        raise ValueError("accepted must be (rows, n)")
+    n = accepted.shape[1]
+    ap = _ints(accepted, (rows, n), index, "accepted")
+    op = _ints(length_out, (rows,), index, "length_out")
+    np_ = 0 if next_out is None else _ints(next_out, (rows,), index, "next_out")
+    args = _COMMIT_STRUCT.pack(*_nodes(k_new, new, cache, "k_new"), *_nodes(v_new, new, cache, "v_new"), *qp, ap, n, lp,
+                               table, sp, op, np_, n, nodes, heads, buckets, scale)
+    code = lib.mrt_cache_commit(cache._c, args, index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+
+
+@functools.lru_cache(maxsize=1024)
+def _evict_workspace(rows, kv_heads, capacity, d, dtype, keep) -> int:
+    lib, size = load_library(), ctypes.c_size_t()
+    c = _CACHE_STRUCT.pack(0, 0, 0, 0, 0, 0, 0, 0, 0, rows, kv_heads, capacity, d, _dtype_code(dtype))
+    _check(lib, lib.mrt_cache_evict_workspace(c, keep, ctypes.byref(size)))
+    return size.value
+
+
+def cache_evict(cache: KVCache, keep: int, length_out, score_out, pos_out, recent: int = 0, sinks: int = 0) -> None:
+    """Evicts the entries with the least accumulated attention weight (mrt_cache_evict).
+
+    Each sequence keeps ``keep`` entries of every K/V head: those of the last
+    ``recent`` positions and the first ``sinks``, then the highest scores.  K
+    and V rows move in place; length_out (a tensor of its own), score_out and
+    pos_out (which may be the cache's) receive the new state.
+    """
+    lib, index, slots = load_library(), cache.index, cache.shape[:3]
+    if cache.score is None or cache.pos is None:
+        raise ValueError("eviction needs the cache's pos, next_pos and score")
+    args = _EVICT_STRUCT.pack(_floats(score_out, slots, index, "score_out"), _ints(pos_out, slots, index, "pos_out"),
+                              _ints(length_out, slots[:1], index, "length_out"), keep, recent, sinks)
+    size = _evict_workspace(*cache.shape, cache.dtype, keep)
+    torch = _torch()
+    ws = torch.empty(size, dtype=torch.uint8, device=cache.k.device) if size else None
+    code = lib.mrt_cache_evict(cache._c, args, ws.data_ptr() if size else None, size, index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+
+
+def q4_matmul(x, w, scales, biases, out=None):
+    """x (rows, k) times 4-bit weights (mrt_q4_matmul): (rows, n) in x's dtype.
+
+    w int32 (n, k / 8), eight codes a word from the low bits; scales, biases
+    (n, k / group) in x's dtype, group 32, 64 or 128: weight = scale * code +
+    bias.  ``q4_quantize`` makes them.
+    """
+    lib, torch, index = load_library(), _torch(), x.get_device()
+    if x.dim() != 2 or w.dim() != 2 or scales.dim() != 2:
+        raise ValueError("x, w and scales must be matrices")
+    (rows, k), (n, words), dt = x.shape, w.shape, x.dtype
+    groups = scales.shape[1]
+    if index < 0 or words * 8 != k or k == 0 or groups == 0 or k % groups or scales.shape[0] != n:
+        raise ValueError("w must be (n, k / 8) and scales (n, k / group) for x (rows, k) on a GPU")
+    wp = _ints(w, (n, words), index, "w")
+    if (biases.shape != scales.shape or scales.dtype is not dt or biases.dtype is not dt or x.stride(1) != 1
+            or not scales.is_contiguous() or not biases.is_contiguous() or scales.get_device() != index
+            or biases.get_device() != index):
+        raise ValueError("scales and biases must be contiguous, in x's dtype and on its GPU, x's rows contiguous")
+    if out is None:
+        out = torch.empty((rows, n), dtype=dt, device=x.device)
+    elif out.shape != (rows, n) or out.dtype is not dt or out.get_device() != index or out.stride(1) != 1:
+        raise ValueError("out must be (rows, n) in x's dtype, on its GPU, rows contiguous")
+    code = lib.mrt_q4_matmul(x.data_ptr(), x.stride(0), rows, wp, scales.data_ptr(), biases.data_ptr(), n, k, k // groups,
+                             _dtype_code(dt), out.data_ptr(), out.stride(0), index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+    return out
+
+
+def q4_quantize(weight, group: int = 64):
+    """4-bit codes of weight (n, k) (mrt_q4_quantize): (w int32 (n, k / 8), scales, biases (n, k / group))."""
+    lib, torch, index = load_library(), _torch(), weight.get_device()
+    if weight.dim() != 2 or index < 0 or weight.stride(1) != 1 or group not in (32, 64, 128) or weight.shape[1] % group:
+        raise ValueError("weight must be (n, k) on a GPU, rows contiguous, k a multiple of group 32, 64 or 128")
+    n, k = weight.shape
+    w = torch.empty((n, k // 8), dtype=torch.int32, device=weight.device)
+    scales = torch.empty((n, k // group), dtype=weight.dtype, device=weight.device)
+    biases = torch.empty_like(scales)
+    _check(lib, lib.mrt_q4_quantize(weight.data_ptr(), weight.stride(0), n, k, group, _dtype_code(weight.dtype),
+                                    w.data_ptr(), scales.data_ptr(), biases.data_ptr(), index, _raw_stream(index)))
+    return w, scales, biases

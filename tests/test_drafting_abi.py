@@ -90,3 +90,98 @@ def test_binding_refuses_cpu_tensors_and_wrong_shapes():
         mrt_df.KVCache(k, k[:, :, :8], n)                  # v unlike k
     with pytest.raises(ValueError):
         mrt_df.KVCache(k.transpose(2, 3), k.transpose(2, 3), n)  # d not contiguous
+
+
+def commit(k=P, v=P, q=P, lse=P, score_out=P, accepted=P, astride=4, length_out=P + 64, next_out=0, accepted_n=4, nodes=4,
+           heads=4, bias=0, buckets=0):
+    qs = (4 * 256, 256, 64)
+    return mrt_df._COMMIT_STRUCT.pack(k, 512, 128, 64, v, 512, 128, 64, q, *qs, accepted, astride, lse, bias, score_out,
+                                      length_out, next_out, accepted_n, nodes, heads, buckets, 1.0)
+
+
+BAD_COMMITS = {
+    "null k": dict(k=0), "null v": dict(v=0), "misaligned k": dict(k=P + 2), "null accepted": dict(accepted=0),
+    "accepted stride": dict(astride=-1), "null length_out": dict(length_out=0), "length_out in place": dict(length_out=P),
+    "no lse": dict(lse=0), "no score_out": dict(score_out=0), "nothing accepted": dict(accepted_n=0),
+    "many accepted": dict(accepted_n=65), "no nodes": dict(nodes=0), "many nodes": dict(nodes=65), "heads": dict(heads=5),
+    "bias without buckets": dict(bias=P),
+}
+
+
+@pytest.mark.parametrize("bad", BAD_COMMITS)
+def test_commit_refuses(lib, bad):
+    refused(lib, lib.mrt_cache_commit(cache(), commit(**BAD_COMMITS[bad]), 0, None))
+
+
+def test_commit_refuses_caches(lib):
+    for bad in BAD_CACHES.values():
+        refused(lib, lib.mrt_cache_commit(cache(**bad), commit(), 0, None))
+    refused(lib, lib.mrt_cache_commit(None, commit(), 0, None))
+    refused(lib, lib.mrt_cache_commit(cache(), None, 0, None))
+    positions = dict(pos=P, next_pos=P + 128)
+    refused(lib, lib.mrt_cache_commit(cache(**positions), commit(), 0, None))                     # no next_out
+    refused(lib, lib.mrt_cache_commit(cache(**positions), commit(next_out=P + 128), 0, None))     # in place
+    assert lib.mrt_cache_commit(cache(rows=0), commit(), 0, None) == 0
+
+
+def evict(score_out=P, pos_out=P, length_out=P + 64, keep=8, recent=0, sinks=0):
+    return mrt_df._EVICT_STRUCT.pack(score_out, pos_out, length_out, keep, recent, sinks)
+
+
+BAD_EVICTS = {
+    "null score_out": dict(score_out=0), "null pos_out": dict(pos_out=0), "null length_out": dict(length_out=0),
+    "length_out in place": dict(length_out=P), "keep": dict(keep=0), "recent": dict(recent=-1), "sinks": dict(sinks=-1),
+    "more fixed than kept": dict(recent=5, sinks=4), "overflow": dict(recent=2 ** 31 - 1, sinks=2 ** 31 - 1),
+}
+
+
+@pytest.mark.parametrize("bad", BAD_EVICTS)
+def test_evict_refuses(lib, bad):
+    full = cache(pos=P, next_pos=P, score=P)
+    refused(lib, lib.mrt_cache_evict(full, evict(**BAD_EVICTS[bad]), P, 1 << 20, 0, None))
+
+
+def test_evict_refuses_caches_and_workspaces(lib):
+    for bad in BAD_CACHES.values():
+        refused(lib, lib.mrt_cache_evict(cache(**{**dict(pos=P, next_pos=P, score=P), **bad, **({"next_pos": 0} if "pos" in bad else {})}),
+                                         evict(), P, 1 << 20, 0, None))
+    refused(lib, lib.mrt_cache_evict(cache(score=P), evict(), P, 1 << 20, 0, None))
+    refused(lib, lib.mrt_cache_evict(cache(pos=P, next_pos=P), evict(), P, 1 << 20, 0, None))
+    refused(lib, lib.mrt_cache_evict(None, evict(), P, 1 << 20, 0, None))
+    refused(lib, lib.mrt_cache_evict(cache(pos=P, next_pos=P, score=P), None, P, 1 << 20, 0, None))
+    size = ctypes.c_size_t()
+    refused(lib, lib.mrt_cache_evict_workspace(cache(), 0, ctypes.byref(size)))
+    refused(lib, lib.mrt_cache_evict_workspace(cache(), 4, None))
+    long = cache(pos=P, next_pos=P, score=P, cap=100000, hs=6400000, rs=12800000)
+    assert lib.mrt_cache_evict_workspace(long, 50000, ctypes.byref(size)) == 0 and size.value > 0
+    refused(lib, lib.mrt_cache_evict(long, evict(keep=50000), None, 0, 0, None))
+    refused(lib, lib.mrt_cache_evict(long, evict(keep=50000), P, size.value - 1, 0, None))
+    assert lib.mrt_cache_evict(cache(rows=0, pos=P, next_pos=P, score=P), evict(), None, 0, 0, None) == 0
+
+
+Q4 = dict(x=P, ldx=128, rows=2, w=P, scales=P, biases=P, n=16, k=128, group=64, dtype=1, out=P, ldo=16)
+BAD_Q4 = {
+    "null x": dict(x=None), "null w": dict(w=None), "null scales": dict(scales=None), "null biases": dict(biases=None),
+    "null out": dict(out=None), "misaligned x": dict(x=P + 8), "misaligned w": dict(w=P + 4), "rows": dict(rows=-1),
+    "n": dict(n=0), "k": dict(k=0), "k and group": dict(k=96), "group": dict(group=16), "dtype": dict(dtype=7),
+    "narrow ldx": dict(ldx=64), "odd ldx": dict(ldx=132), "narrow ldo": dict(ldo=8),
+}
+
+
+@pytest.mark.parametrize("bad", BAD_Q4)
+def test_q4_matmul_refuses(lib, bad):
+    a = {**Q4, **BAD_Q4[bad]}
+    refused(lib, lib.mrt_q4_matmul(a["x"], a["ldx"], a["rows"], a["w"], a["scales"], a["biases"], a["n"], a["k"], a["group"],
+                                   a["dtype"], a["out"], a["ldo"], 0, None))
+
+
+def test_q4_no_rows_and_quantize_refusals(lib):
+    assert lib.mrt_q4_matmul(P, 128, 0, P, P, P, 16, 128, 64, 1, P, 16, 0, None) == 0
+    for a in ((None, 128, 16, 128, 64, 1, P, P, P), (P, 128, 16, 128, 48, 1, P, P, P), (P, 64, 16, 128, 64, 1, P, P, P),
+              (P, 128, 0, 128, 64, 1, P, P, P), (P, 128, 16, 128, 64, 9, P, P, P), (P, 128, 16, 128, 64, 1, None, P, P),
+              (P, 128, 16, 128, 64, 1, P, None, P), (P, 128, 16, 128, 64, 1, P, P, None)):
+        refused(lib, lib.mrt_q4_quantize(*a, 0, None))
+    with pytest.raises(ValueError):
+        mrt_df.q4_matmul(torch.zeros(2, 64), torch.zeros(4, 8, dtype=torch.int32), torch.zeros(4, 1), torch.zeros(4, 1))
+    with pytest.raises(ValueError):
+        mrt_df.q4_quantize(torch.zeros(4, 64), 64)
