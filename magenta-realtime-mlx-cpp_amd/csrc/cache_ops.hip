@@ -159,12 +159,14 @@ void launch_commit(const CommitK& a, int rows, int nr, hipStream_t s) {
 
 // ---- eviction -------------------------------------------------------------------
 //
-// A block a (sequence, head) finds the `keep` best of its entries by radix selection on
-// ordered keys (8 bits a pass, highest first), then moves the kept entries that lie at
-// or above the new length into the evicted slots below it, in order: no row is read
-// that another move writes, so the moves of a head need no order among themselves.
-// Each wave owns a run of consecutive slots, so that ranks are a count per wave, a sum
-// over the waves before and a ballot, and the result is the same on every run.
+// For each (sequence, head): the `keep` best entries by radix selection on ordered keys,
+// then the kept entries at or above the new length go to the evicted slots below it, in
+// order: no row is read that another move writes, so the moves need no order among
+// themselves.  Ranks come from ballots over consecutive slots, so the result is the same
+// on every run.  Short caches (k_evict_short): one wave holds a head's keys in registers
+// and finds the threshold by ballots, a bit at a time, with no barrier.  Long ones
+// (k_evict_select): a block a head, 11 bits a pass through LDS histograms until the keys
+// that are left fit LDS.
 
 constexpr uint32_t kLowest = 0x007fffffu;  // of -inf; a NaN counts as that
 constexpr uint32_t kFixed = 0xffffffffu;   // entries that stay
@@ -175,10 +177,16 @@ struct EvictK {
   const float* score;
   float* score_out;
   int *pos_out, *length_out;
+  uint32_t* keys;               // (rows * kv_heads, capacity): k_evict_select
   int *holes, *movers, *count;  // (rows * kv_heads, list), (rows * kv_heads): for k_evict_move, or nullptr
   int64_t c_row, c_head, c_slot;
   int capacity, kv_heads, keep, recent, sinks, list, row_bytes, esz;
 };
+
+__device__ __forceinline__ uint32_t evict_key(int p, float f, int64_t recent_from, int sinks) {
+  if (p >= recent_from || p < sinks) return kFixed;
+  return f != f ? kLowest : float_key(f + 0.f);  // -0 counts as 0
+}
 
 __device__ __forceinline__ void move_row(const EvictK& a, int64_t base, int from, int to, int piece) {
   const int64_t e = a.c_slot * a.esz;
@@ -189,10 +197,135 @@ __device__ __forceinline__ void move_row(const EvictK& a, int64_t base, int from
   *reinterpret_cast<uint4*>(vp + to * e) = y;
 }
 
-// Threads a block, keys a thread held in registers (0: read again in every pass).
-template <int THREADS, int KPT>
-__global__ __launch_bounds__(THREADS) void k_evict_select(const EvictK a) {
-  constexpr int W = THREADS / 64, kRep = 16;
+constexpr int kShortSlots = 2048;  // capacity up to which k_evict_short serves
+constexpr int kShortList = 1024;   // rows that it moves itself
+
+// Four waves load and move; the first finds the threshold from KPT keys a lane, slot 64 t
+// + lane in key t, so that ballots are in slot order.
+template <int KPT>
+__global__ __launch_bounds__(256) void k_evict_short(const EvictK a) {
+  constexpr int W = 4, PER = (KPT + W - 1) / W;
+  const int bg = blockIdx.x, b = bg / a.kv_heads, kvh = bg - b * a.kv_heads;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int64_t at = (int64_t)bg * a.capacity;
+  __shared__ uint32_t keys[KPT * 64];
+  __shared__ uint32_t few[64];
+  __shared__ uint64_t kept_of[KPT];
+  __shared__ int hole_base[KPT + 1], mover_base[KPT];
+  __shared__ int hole_at[kShortList], mover_at[kShortList];
+  float f[PER];
+  int p[PER];
+#pragma unroll
+  for (int z = 0; z < PER; ++z) {
+    const int j = (z * W + wid) * 64 + lane;
+    f[z] = j < a.capacity ? ld_g(a.score + at + j) : 0.f;
+    p[z] = j < a.capacity ? ld_g(a.pos + at + j) : 0;
+  }
+  const int len = min(max(a.length[b], 0), a.capacity), m = min(len, a.keep);
+  const int64_t recent_from = (int64_t)a.next_pos[b] - a.recent;
+  if (kvh == 0 && tid == 0) a.length_out[b] = m;
+#pragma unroll
+  for (int z = 0; z < PER; ++z) {
+    const int t = z * W + wid, j = t * 64 + lane;
+    if (t < KPT) keys[j] = j < len ? evict_key(p[z], f[z], recent_from, a.sinks) : 0u;  // 0: no entry's key
+  }
+  __syncthreads();
+  const uint64_t below = (1ull << lane) - 1;
+  if (wid == 0) {
+    uint32_t key[KPT];
+#pragma unroll
+    for (int t = 0; t < KPT; ++t) key[t] = keys[t * 64 + lane];
+    // The largest threshold `low` that at least m keys reach, a bit at a time; once no
+    // more than 64 keys share the bits found, one key a lane is enough.
+    uint32_t low = m < len ? 0 : 1;
+    int reach = len, over = 0;  // keys >= low; keys beyond those that share its bits
+    int bit = m < len ? 31 : -1;
+    for (; bit >= 0; --bit) {
+      const uint32_t x = low | (1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int t = 0; t < KPT; ++t) c += __popcll(__ballot(key[t] >= x));
+      if (c >= m) low = x, reach = c;
+      else over = c;
+      if (reach - over <= 64) break;
+    }
+    if (bit > 0) {
+      int n = 0;
+#pragma unroll
+      for (int t = 0; t < KPT; ++t) {
+        const bool in = key[t] != 0 && (key[t] >> bit) == (low >> bit);
+        const uint64_t who = __ballot(in);
+        if (in) few[n + __popcll(who & below)] = key[t];
+        n += __popcll(who);
+      }
+      __builtin_amdgcn_wave_barrier();
+      const uint32_t one = lane < n ? few[lane] : 0u;
+      const int beyond = over;
+      for (--bit; bit >= 0; --bit) {
+        const uint32_t x = low | (1u << bit);
+        const int c = beyond + __popcll(__ballot(one >= x));
+        if (c >= m) low = x;
+        else over = c;
+      }
+    }
+    // Every key above `low` is kept (`over` of them), and the first ties.
+    const int ties = m < len ? m - over : 0;
+    int seen = 0, holes = 0, movers = 0;
+#pragma unroll
+    for (int t = 0; t < KPT; ++t) {
+      const int j = t * 64 + lane;
+      const uint64_t eq = __ballot(key[t] == low);
+      const bool k = m < len ? key[t] > low || (key[t] == low && seen + __popcll(eq & below) < ties) : j < len;
+      seen += __popcll(eq);
+      const uint64_t who = __ballot(k);
+      if (lane == 0) kept_of[t] = who, hole_base[t] = holes, mover_base[t] = movers;
+      const int inside = min(max(m - t * 64, 0), 64);  // slots of these below m
+      const uint64_t head = inside == 64 ? ~0ull : (1ull << inside) - 1;
+      holes += inside - __popcll(who & head), movers += __popcll(who & ~head);
+    }
+    if (lane == 0) hole_base[KPT] = holes;
+  }
+  __syncthreads();
+  int* hl = a.holes != nullptr ? a.holes + (int64_t)bg * a.list : hole_at;
+  int* ml = a.holes != nullptr ? a.movers + (int64_t)bg * a.list : mover_at;
+#pragma unroll
+  for (int z = 0; z < PER; ++z) {
+    const int t = z * W + wid, j = t * 64 + lane;
+    if (t >= KPT) continue;
+    const uint64_t who = kept_of[t];
+    const int inside = min(max(m - t * 64, 0), 64);
+    const uint64_t head = inside == 64 ? ~0ull : (1ull << inside) - 1;
+    const bool k = (who >> lane) & 1;
+    if (j < m && k) a.score_out[at + j] = f[z], a.pos_out[at + j] = p[z];
+    if (j < m && !k) hl[hole_base[t] + __popcll(~who & head & below)] = j;
+    if (j >= m && k) ml[mover_base[t] + __popcll(who & ~head & below)] = j;
+  }
+  const int total = hole_base[KPT];
+  if (a.holes != nullptr) __threadfence_block();
+  __syncthreads();
+  if (a.count != nullptr) {
+    if (tid == 0) a.count[bg] = total;
+    for (int x = tid; x < total; x += 256) {
+      const int to = hl[x], from = ml[x];
+      a.score_out[at + to] = ld_g(a.score + at + from), a.pos_out[at + to] = ld_g(a.pos + at + from);
+    }
+    return;
+  }
+  const int64_t base = (b * a.c_row + kvh * a.c_head) * a.esz;
+  const int pieces = a.row_bytes / 16;
+#pragma unroll 2
+  for (int x = tid; x < total * pieces; x += 256) {
+    const int r = x / pieces, piece = x - r * pieces, from = ml[r], to = hl[r];
+    move_row(a, base, from, to, piece);
+    if (piece == 0) a.score_out[at + to] = ld_g(a.score + at + from), a.pos_out[at + to] = ld_g(a.pos + at + from);
+  }
+}
+
+constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBatch = 16;
+constexpr int kDigit = 11, kBins = 1 << kDigit, kFew = 8192;  // bins of a pass; keys that LDS takes for the rest
+
+__global__ __launch_bounds__(kSelThreads) void k_evict_select(const EvictK a) {
+  constexpr int W = kSelWaves, kRep = 4;
   const int bg = blockIdx.x, b = bg / a.kv_heads, kvh = bg - b * a.kv_heads;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int len = min(max(a.length[b], 0), a.capacity), m = min(len, a.keep);
@@ -201,98 +334,154 @@ __global__ __launch_bounds__(THREADS) void k_evict_select(const EvictK a) {
   const int* pos = a.pos + at;
   float* score_out = a.score_out + at;
   int* pos_out = a.pos_out + at;
+  uint32_t* keys = a.keys + at;
   if (kvh == 0 && tid == 0) a.length_out[b] = m;
-  if (a.count != nullptr && tid == 0) a.count[bg] = 0;
   if (m == len) {
-    for (int j = tid; j < len; j += THREADS) score_out[j] = score[j], pos_out[j] = pos[j];
+    for (int j = tid; j < len; j += kSelThreads) score_out[j] = score[j], pos_out[j] = pos[j];
+    if (tid == 0) a.count[bg] = 0;
     return;
   }
   const int64_t recent_from = (int64_t)a.next_pos[b] - a.recent;
-  // wave w owns slots [w run, (w + 1) run), 64 a turn
-  const int turns = (len + 64 * W - 1) / (64 * W), run = turns * 64;
-  const int lo = wid * run + lane;
-  auto key_at = [&](int t) -> uint32_t {
-    const int j = lo + t * 64;
-    if (j >= len) return 0u;
-    const int p = ld_g(pos + j);
-    const float f = ld_g(score + j);
-    if (p >= recent_from || p < a.sinks) return kFixed;
-    return f != f ? kLowest : float_key(f + 0.f);  // -0 counts as 0
-  };
-  constexpr int kHeld = KPT > 0 ? KPT : 1;
-  uint32_t held[kHeld];
-  if constexpr (KPT > 0) {
+  // Wave w owns slots [w run, (w + 1) run), 64 a turn.  f(slot, key, in use) in slot
+  // order, a batch of keys loaded ahead; only the owner reads what it wrote.
+  const int turns = (len + 64 * W - 1) / (64 * W), lo = wid * turns * 64 + lane;
+  auto each = [&](auto&& f) {
+    for (int t0 = 0; t0 < turns; t0 += kSelBatch) {
+      uint32_t k[kSelBatch];
 #pragma unroll
-    for (int t = 0; t < KPT; ++t) held[t] = t < turns ? key_at(t) : 0u;
-  }
-  auto each = [&](auto&& f) {  // f(turn, key) in slot order
-    if constexpr (KPT > 0) {
+      for (int t = 0; t < kSelBatch; ++t) {
+        const int j = lo + (t0 + t) * 64;
+        k[t] = t0 + t < turns && j < len ? ld_g(keys + j) : 0u;
+      }
 #pragma unroll
-      for (int t = 0; t < KPT; ++t)
-        if (t < turns) f(t, held[t]);
-    } else {
-      for (int t = 0; t < turns; ++t) f(t, key_at(t));
+      for (int t = 0; t < kSelBatch; ++t) {
+        const int j = lo + (t0 + t) * 64;
+        if (t0 + t < turns) f(j, k[t], j < len);
+      }
     }
   };
 
-  __shared__ uint32_t hist[256 * kRep];
-  __shared__ uint32_t bins[256];
-  __shared__ uint32_t picked[2];
+  __shared__ uint32_t hist[kBins * kRep];  // then the few keys that are left
+  __shared__ uint32_t total_of[W];
+  __shared__ uint32_t picked[4];           // digit, of its keys how many are kept, how many there are; the few's count
   __shared__ int tally[3][W];
   uint32_t prefix = 0, mask = 0, want = m;  // of the keys with this prefix, `want` are kept
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int x = tid; x < 256 * kRep; x += THREADS) hist[x] = 0;
+  // Picks the digit at `shift` from the histogram: thread t holds bins 2 t, 2 t + 1, and
+  // counts from the top.
+  auto pick = [&](int shift, int bits) {
     __syncthreads();
-    each([&](int t, uint32_t key) {
-      if (lo + t * 64 < len && (key & mask) == prefix) atomicAdd(&hist[((key >> shift) & 255) * kRep + (lane & (kRep - 1))], 1u);
-    });
-    __syncthreads();
-    for (int x = tid; x < 256; x += THREADS) {
-      uint32_t c = 0;
+    uint32_t c[2] = {0, 0};
 #pragma unroll
-      for (int r = 0; r < kRep; ++r) c += hist[x * kRep + ((r + x) & (kRep - 1))];
-      bins[x] = c;
+    for (int r = 0; r < kRep; ++r) {
+      c[0] += hist[(2 * tid) * kRep + ((r + tid) & (kRep - 1))];
+      c[1] += hist[(2 * tid + 1) * kRep + ((r + tid) & (kRep - 1))];
     }
+    uint32_t above = c[0] + c[1];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t x = __shfl_down(above, o, 64);
+      if (lane + o < 64) above += x;
+    }
+    if (lane == 0) total_of[wid] = above;
     __syncthreads();
-    if (wid == 0) {  // lane l: bins 4 l .. 4 l + 3; counts from the top
-      const uint32_t c0 = bins[4 * lane], c1 = bins[4 * lane + 1], c2 = bins[4 * lane + 2], c3 = bins[4 * lane + 3];
-      uint32_t above = c0 + c1 + c2 + c3;
+    above -= c[0] + c[1];
+    for (int w = wid + 1; w < W; ++w) above += total_of[w];
 #pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t x = __shfl_down(above, o, 64);
-        if (lane + o < 64) above += x;
-      }
-      above -= c0 + c1 + c2 + c3;  // in the lanes above
-      const uint32_t c[4] = {c0, c1, c2, c3};
-#pragma unroll
-      for (int j = 3; j >= 0; --j) {
-        if (above < want && want <= above + c[j]) picked[0] = 4 * lane + j, picked[1] = want - above;
-        above += c[j];
-      }
+    for (int j = 1; j >= 0; --j) {
+      if (above < want && want <= above + c[j]) picked[0] = 2 * tid + j, picked[1] = want - above, picked[2] = c[j];
+      above += c[j];
     }
     __syncthreads();
     prefix |= picked[0] << shift;
-    mask |= 255u << shift;
+    mask |= ((1u << bits) - 1) << shift;
     want = picked[1];
+  };
+  auto clear = [&] {
+    for (int x = tid; x < kBins * kRep; x += kSelThreads) hist[x] = 0;
+    __syncthreads();
+  };
+  auto count = [&](uint32_t digit) { atomicAdd(&hist[digit * kRep + (lane & (kRep - 1))], 1u); };
+  clear();
+  for (int t0 = 0; t0 < turns; t0 += kSelBatch) {
+    float f[kSelBatch];
+    int p[kSelBatch];
+#pragma unroll
+    for (int t = 0; t < kSelBatch; ++t) {
+      const int j = lo + (t0 + t) * 64;
+      const bool in = t0 + t < turns && j < len;
+      f[t] = in ? ld_g(score + j) : 0.f;
+      p[t] = in ? ld_g(pos + j) : 0;
+    }
+#pragma unroll
+    for (int t = 0; t < kSelBatch; ++t) {
+      const int j = lo + (t0 + t) * 64;
+      if (t0 + t >= turns || j >= len) continue;
+      const uint32_t key = evict_key(p[t], f[t], recent_from, a.sinks);
+      keys[j] = key;
+      if (j < m) score_out[j] = f[t], pos_out[j] = p[t];  // k_evict_move overwrites the evicted ones
+      count(key >> 21);
+    }
+  }
+  pick(21, kDigit);
+  int shift = 21;
+  while (shift > 0 && picked[2] > kFew) {  // crowded: another pass over all keys
+    const int bits = shift > kDigit ? kDigit : shift;
+    __syncthreads();  // picked has been read
+    clear();
+    each([&](int, uint32_t key, bool in) {
+      if (in && (key & mask) == prefix) count((key >> (shift - bits)) & ((1u << bits) - 1));
+    });
+    shift -= bits;
+    pick(shift, bits);
+  }
+  if (shift > 0) {  // the rest from LDS, a bit at a time
+    if (tid == 0) picked[3] = 0;
+    __syncthreads();
+    each([&](int, uint32_t key, bool in) {
+      const bool mine = in && (key & mask) == prefix;
+      const uint64_t who = __ballot(mine);
+      uint32_t first = 0;
+      if (who != 0 && lane == 0) first = atomicAdd(&picked[3], (uint32_t)__popcll(who));
+      first = __builtin_amdgcn_readfirstlane(first);
+      if (mine) hist[first + __popcll(who & ((1ull << lane) - 1))] = key;
+    });
+    __syncthreads();
+    const int n = picked[3];
+    uint32_t k[kFew / kSelThreads];
+#pragma unroll
+    for (int z = 0; z < kFew / kSelThreads; ++z) k[z] = tid + z * kSelThreads < n ? hist[tid + z * kSelThreads] : 0u;
+    for (int bit = shift - 1; bit >= 0; --bit) {
+      const uint32_t x = prefix | (1u << bit);
+      int c = 0;
+#pragma unroll
+      for (int z = 0; z < kFew / kSelThreads; ++z) c += __popcll(__ballot(k[z] >= x && k[z] >> bit == x >> bit));
+      if (lane == 0) tally[bit & 1][wid] = c;
+      __syncthreads();
+      int sum = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) sum += tally[bit & 1][w];
+      if (sum >= (int)want) prefix = x;
+      else want -= sum;
+    }
+    __syncthreads();
   }
   // Kept: keys above prefix, and the first `want` slots with it.
   int equal = 0;
-  each([&](int t, uint32_t key) { equal += __popcll(__ballot(lo + t * 64 < len && key == prefix)); });
+  each([&](int, uint32_t key, bool in) { equal += __popcll(__ballot(in && key == prefix)); });
   if (lane == 0) tally[0][wid] = equal;
   __syncthreads();
   int ties = 0;
   for (int w = 0; w < wid; ++w) ties += tally[0][w];
   const uint64_t below = (1ull << lane) - 1;
-  auto kept_of = [&](int t, uint32_t key, int& seen) -> bool {
-    const uint64_t eq = __ballot(lo + t * 64 < len && key == prefix);
-    const bool k = lo + t * 64 < len && (key > prefix || (key == prefix && seen + __popcll(eq & below) < (int)want));
+  auto kept_of = [&](uint32_t key, bool in, int& seen) -> bool {
+    const uint64_t eq = __ballot(in && key == prefix);
+    const bool k = in && (key > prefix || (key == prefix && seen + __popcll(eq & below) < (int)want));
     seen += __popcll(eq);
     return k;
   };
   int seen = ties, holes = 0, movers = 0;
-  each([&](int t, uint32_t key) {
-    const bool k = kept_of(t, key, seen);
-    const int j = lo + t * 64;
+  each([&](int j, uint32_t key, bool in) {
+    const bool k = kept_of(key, in, seen);
     holes += __popcll(__ballot(j < m && !k));
     movers += __popcll(__ballot(j >= m && k));
   });
@@ -303,53 +492,40 @@ __global__ __launch_bounds__(THREADS) void k_evict_select(const EvictK a) {
     if (w < wid) hole += tally[1][w], mover += tally[2][w];
     total += tally[1][w];
   }
-  extern __shared__ int lists[];  // holes, movers, where they are not in memory
-  int* hl = a.holes != nullptr ? a.holes + (int64_t)bg * a.list : lists;
-  int* ml = a.holes != nullptr ? a.movers + (int64_t)bg * a.list : lists + a.list;
+  int* hl = a.holes + (int64_t)bg * a.list;
+  int* ml = a.movers + (int64_t)bg * a.list;
   seen = ties;
-  each([&](int t, uint32_t key) {
-    const bool k = kept_of(t, key, seen);
-    const int j = lo + t * 64;
+  each([&](int j, uint32_t key, bool in) {
+    const bool k = kept_of(key, in, seen);
     const uint64_t h = __ballot(j < m && !k), v = __ballot(j >= m && k);
     if (j < m && !k) hl[hole + __popcll(h & below)] = j;
     if (j >= m && k) ml[mover + __popcll(v & below)] = j;
     hole += __popcll(h), mover += __popcll(v);
-    if (j < m && k) score_out[j] = score[j], pos_out[j] = pos[j];
   });
-  if (a.holes != nullptr) __threadfence_block();
-  __syncthreads();
-  for (int x = tid; x < total; x += THREADS) {
-    const int to = hl[x], from = ml[x];
-    score_out[to] = score[from], pos_out[to] = pos[from];
-  }
-  if (a.count != nullptr) {
-    if (tid == 0) a.count[bg] = total;
-    return;
-  }
-  const int64_t base = (b * a.c_row + kvh * a.c_head) * a.esz;
-  const int pieces = a.row_bytes / 16;
-  for (int x = tid; x < total * pieces; x += THREADS) {
-    const int r = x / pieces;
-    move_row(a, base, ml[r], hl[r], x - r * pieces);
-  }
+  if (tid == 0) a.count[bg] = total;
 }
 
-// Rows of the long lists, `blocks` blocks a (sequence, head).
-__global__ __launch_bounds__(256) void k_evict_move(const EvictK a, int blocks) {
-  const int bg = blockIdx.x / blocks, part = blockIdx.x - bg * blocks, b = bg / a.kv_heads, kvh = bg - b * a.kv_heads, pieces = a.row_bytes / 16;
+// Rows of the lists, `blocks` blocks a (sequence, head); with `entries`, their scores and
+// positions too.
+__global__ __launch_bounds__(256) void k_evict_move(const EvictK a, int blocks, bool entries) {
+  const int bg = blockIdx.x / blocks, part = blockIdx.x - bg * blocks, b = bg / a.kv_heads, kvh = bg - b * a.kv_heads;
+  const int pieces = a.row_bytes / 16;
   const int64_t total = (int64_t)a.count[bg] * pieces, base = (b * a.c_row + kvh * a.c_head) * a.esz;
+  const int64_t at = (int64_t)bg * a.capacity;
   const int* hl = a.holes + (int64_t)bg * a.list;
   const int* ml = a.movers + (int64_t)bg * a.list;
   for (int64_t x = part * 256 + threadIdx.x; x < total; x += (int64_t)blocks * 256) {
-    const int r = (int)(x / pieces);
-    move_row(a, base, ml[r], hl[r], (int)(x - (int64_t)r * pieces));
+    const int r = (int)(x / pieces), piece = (int)(x - (int64_t)r * pieces), from = ml[r], to = hl[r];
+    move_row(a, base, from, to, piece);
+    if (entries && piece == 0) a.score_out[at + to] = a.score[at + from], a.pos_out[at + to] = a.pos[at + from];
   }
 }
 
-// Most rows that a head can move, and whether its block moves them itself.
+// Most rows that a head can move; whether k_evict_short serves, and moves them itself.
 int most_moves(const KvCache& c, int keep) { return std::max(0, std::min(keep, c.capacity - keep)); }
+bool is_short(const KvCache& c) { return c.capacity <= kShortSlots; }
 bool moves_within(const KvCache& c, int keep) {
-  return (size_t)most_moves(c, keep) * c.d * dtype_size(c.dt) <= 64 * 1024;
+  return is_short(c) && (size_t)most_moves(c, keep) * c.d * dtype_size(c.dt) <= 16 * 1024;
 }
 
 }  // namespace
@@ -386,7 +562,7 @@ void cache_commit(const KvCache& c, const CommitArgs& t, hipStream_t s) {
 size_t cache_evict_workspace(const KvCache& c, int keep) {
   if (moves_within(c, keep)) return 0;
   const size_t heads = (size_t)c.rows * c.kv_heads;
-  return heads * (2 * (size_t)most_moves(c, keep) + 1) * 4;
+  return heads * (2 * (size_t)most_moves(c, keep) + 1 + (is_short(c) ? 0 : (size_t)c.capacity)) * 4;
 }
 
 void cache_evict(const KvCache& c, const EvictArgs& t, void* ws, hipStream_t s) {
@@ -397,22 +573,21 @@ void cache_evict(const KvCache& c, const EvictArgs& t, void* ws, hipStream_t s) 
   a.capacity = c.capacity, a.kv_heads = c.kv_heads, a.keep = t.keep, a.recent = t.recent, a.sinks = t.sinks;
   a.esz = (int)dtype_size(c.dt), a.row_bytes = c.d * a.esz, a.list = most_moves(c, t.keep);
   const int heads = c.rows * c.kv_heads;
-  size_t lds = (size_t)a.list * 8;
   if (!moves_within(c, t.keep)) {
     a.holes = static_cast<int*>(ws);
     a.movers = a.holes + (size_t)heads * a.list;
     a.count = a.movers + (size_t)heads * a.list;
-    lds = 0;
+    a.keys = reinterpret_cast<uint32_t*>(a.count + heads);
   }
-  if (c.capacity <= 256 * 8) hipLaunchKernelGGL((k_evict_select<256, 8>), dim3(heads), dim3(256), lds, s, a);
-  else if (c.capacity <= 1024 * 16) hipLaunchKernelGGL((k_evict_select<1024, 16>), dim3(heads), dim3(1024), lds, s, a);
-  else if (c.capacity <= 1024 * 72) hipLaunchKernelGGL((k_evict_select<1024, 72>), dim3(heads), dim3(1024), lds, s, a);
-  else hipLaunchKernelGGL((k_evict_select<1024, 0>), dim3(heads), dim3(1024), lds, s, a);
+  if (c.capacity <= 8 * 64) hipLaunchKernelGGL(k_evict_short<8>, dim3(heads), dim3(256), 0, s, a);
+  else if (c.capacity <= 18 * 64) hipLaunchKernelGGL(k_evict_short<18>, dim3(heads), dim3(256), 0, s, a);
+  else if (is_short(c)) hipLaunchKernelGGL(k_evict_short<32>, dim3(heads), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(k_evict_select, dim3(heads), dim3(kSelThreads), 0, s, a);
   MRT_HIP_CHECK(hipGetLastError());
-  if (a.holes != nullptr) {
+  if (a.holes != nullptr && a.list > 0) {
     const int64_t pieces = (int64_t)a.list * (a.row_bytes / 16);
     const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>((pieces + 1023) / 1024, 8192 / heads));
-    hipLaunchKernelGGL(k_evict_move, dim3(blocks * heads), dim3(256), 0, s, a, blocks);
+    hipLaunchKernelGGL(k_evict_move, dim3(blocks * heads), dim3(256), 0, s, a, blocks, !is_short(c));
     MRT_HIP_CHECK(hipGetLastError());
   }
 }

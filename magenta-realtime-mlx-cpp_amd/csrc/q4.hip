@@ -16,8 +16,10 @@
 // exchanges between lane halves and two between quarters turn that into the operand
 // order in which each instruction's 32 k are consecutive, so within one group.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_frag.hpp"
+#include "mfma_ring.hpp"
 #include "q4.hpp"
 
 namespace mrt {
@@ -25,6 +27,9 @@ namespace {
 
 constexpr int kQ4Waves = 8;
 constexpr int kChunk = 128;
+constexpr int kSlab = kQ4Waves * kChunk;      // k in LDS at a time: a chunk a wave
+constexpr size_t kTwoSlabs = 80 * 1024;       // LDS up to which a second slab saves a barrier
+constexpr int kFill = 256;                    // blocks that fill the card
 
 struct Q4Args {
   const uint32_t* w;
@@ -32,6 +37,7 @@ struct Q4Args {
   void* y;
   int64_t ldx, ldy;
   int n, k, groups, rows;
+  int bufs;   // slabs of x in LDS
   bool wide;  // y rows take 4-element stores
 };
 
@@ -41,21 +47,30 @@ template <typename T>
 struct Q4Op {
   static constexpr int kParts = 1;
   static constexpr uint32_t kOnes = sizeof(T) == 2 && std::is_same_v<T, f16> ? 0x3c003c00u : 0x3f803f80u;
-  typedef T Raw;
+  typedef uint4 Raw;  // eight values of x as they are in memory
   using M = Mma<T>;
   struct X {
     uint4 part[1];
   };
-  __device__ __forceinline__ static uint4 codes(uint32_t w) {
-    if constexpr (std::is_same_v<T, f16>)
-      return make_uint4(((w << 6) & 0x03c003c0u) | 0x4c004c00u, ((w << 2) & 0x03c003c0u) | 0x4c004c00u,
-                        ((w >> 2) & 0x03c003c0u) | 0x4c004c00u, ((w >> 6) & 0x03c003c0u) | 0x4c004c00u);
-    else
-      return make_uint4(((w << 3) & 0x00780078u) | 0x41804180u, ((w >> 1) & 0x00780078u) | 0x41804180u,
-                        ((w >> 5) & 0x00780078u) | 0x41804180u, ((w >> 9) & 0x00780078u) | 0x41804180u);
+  // 16 in both halves, in a register: one and-or instead of two instructions with literals.
+  __device__ __forceinline__ static uint32_t offset() {
+    uint32_t v = std::is_same_v<T, f16> ? 0x4c004c00u : 0x41804180u;
+    asm("" : "+v"(v));
+    return v;
   }
-  __device__ __forceinline__ static X load(const T* p, bool in) {
-    const uint4 v = in ? ld_g16(p) : make_uint4(0, 0, 0, 0);
+  __device__ __forceinline__ static uint4 codes(uint32_t w, uint32_t o) {
+    if constexpr (std::is_same_v<T, f16>) {
+      uint32_t m = 0x03c003c0u;
+      asm("" : "+s"(m));
+      return make_uint4(((w << 6) & m) | o, ((w << 2) & m) | o, ((w >> 2) & m) | o, ((w >> 6) & m) | o);
+    } else {
+      uint32_t m = 0x00780078u;
+      asm("" : "+s"(m));
+      return make_uint4(((w << 3) & m) | o, ((w >> 1) & m) | o, ((w >> 5) & m) | o, ((w >> 9) & m) | o);
+    }
+  }
+  __device__ __forceinline__ static Raw raw(const T* p, bool in) { return in ? ld_g16(p) : make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ static X split(const Raw& v) {
     X x;
     x.part[0] = make_uint4(__builtin_amdgcn_perm(v.z, v.x, 0x05040100u), __builtin_amdgcn_perm(v.z, v.x, 0x07060302u),
                            __builtin_amdgcn_perm(v.w, v.y, 0x05040100u), __builtin_amdgcn_perm(v.w, v.y, 0x07060302u));
@@ -66,13 +81,20 @@ template <>
 struct Q4Op<float> {
   static constexpr int kParts = 3;
   static constexpr uint32_t kOnes = 0x3f803f80u;
+  struct Raw {
+    uint4 a, b;
+  };
   using M = Mma<bf16>;
   struct X {
     uint4 part[3];
   };
-  __device__ __forceinline__ static uint4 codes(uint32_t w) { return Q4Op<bf16>::codes(w); }
-  __device__ __forceinline__ static X load(const float* p, bool in) {
-    const uint4 a = in ? ld_g16(p) : make_uint4(0, 0, 0, 0), b = in ? ld_g16(p + 4) : make_uint4(0, 0, 0, 0);
+  __device__ __forceinline__ static uint32_t offset() { return Q4Op<bf16>::offset(); }
+  __device__ __forceinline__ static uint4 codes(uint32_t w, uint32_t o) { return Q4Op<bf16>::codes(w, o); }
+  __device__ __forceinline__ static Raw raw(const float* p, bool in) {
+    return {in ? ld_g16(p) : make_uint4(0, 0, 0, 0), in ? ld_g16(p + 4) : make_uint4(0, 0, 0, 0)};
+  }
+  __device__ __forceinline__ static X split(const Raw& r) {
+    const uint4 a = r.a, b = r.b;
     const uint32_t lo[4] = {a.x, a.y, a.z, a.w}, hi[4] = {b.x, b.y, b.z, b.w};
     uint32_t out[3][4];
 #pragma unroll
@@ -85,10 +107,10 @@ struct Q4Op<float> {
         x -= bf2f(u), y -= bf2f(v);
       }
     }
-    X r;
+    X o;
 #pragma unroll
-    for (int c = 0; c < 3; ++c) r.part[c] = make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
-    return r;
+    for (int c = 0; c < 3; ++c) o.part[c] = make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
+    return o;
   }
 };
 
@@ -101,28 +123,58 @@ __device__ __forceinline__ void swap16(uint32_t& a, uint32_t& b) {
   a = r[0], b = r[1];
 }
 
+// What a thread loads for a slab, a slab ahead: its lane's codes (16 bytes of row l / 4,
+// so that four lanes share 64 consecutive bytes), and its shares of the scales, biases and
+// x, which the block puts into LDS.
+template <typename T, int MT, int G, int NT>
+struct Q4Load {
+  static constexpr int S = (16 * NT * kQ4Waves * G + 64 * kQ4Waves - 1) / (64 * kQ4Waves);
+  static constexpr int X = MT * 16 * (kSlab / 8) / (64 * kQ4Waves);
+  uint4 w[NT];
+  T s[S], b[S];
+  typename Q4Op<T>::Raw x[X];
+};
+
 // GT: instructions (32 k) a group.  MT: 16-row tiles of x.
 template <typename T, int MT, int GT, int NT>
 __global__ __launch_bounds__(64 * kQ4Waves) void k_q4(const Q4Args a) {
   using Op = Q4Op<T>;
-  constexpr int G = 4 / GT;  // groups of a chunk
+  constexpr int G = 4 / GT, P = Op::kParts;  // groups of a chunk; parts of x
+  constexpr int kThreads = 64 * kQ4Waves, kRows = 16 * NT;
+  using Load = Q4Load<T, MT, G, NT>;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 64;
-  const int words = a.k / 8, chunks = (a.k + kChunk - 1) / kChunk;
-  __shared__ float2 sc[kQ4Waves][NT][4][16];  // scale and offset of a wave's chunk: group, row
-  __shared__ f32x4_t buf[kQ4Waves][NT][MT][64];
+  const int i = lane & 15, g = lane >> 4, n0 = blockIdx.x * kRows, m0 = blockIdx.y * 16 * MT;
+  const int words = a.k / 8, chunks = (a.k + kChunk - 1) / kChunk, cols = min(a.rows - m0, 16 * MT);
+  const int slab_chunks = min(kQ4Waves, chunks), pieces = slab_chunks * kChunk / 8;
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  // LDS, `bufs` times: x as operands, 16 bytes of (instruction, part, row, lane group);
+  // scale and offset of (group of the slab, row).
+  const int x16 = pieces / 4 * P * cols * 4, buf16 = x16 + kQ4Waves * G * kRows / 2;
 
   const uint32_t* wrow[NT];
-  const T *srow[NT], *brow[NT], *xrow[MT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t) {
-    const int64_t row = min(n0 + t * 16 + i, a.n - 1);
-    wrow[t] = a.w + row * words + g * 4;
-    srow[t] = static_cast<const T*>(a.scales) + row * a.groups;
-    brow[t] = static_cast<const T*>(a.biases) + row * a.groups;
-  }
+  for (int t = 0; t < NT; ++t) wrow[t] = a.w + (int64_t)min(n0 + t * 16 + (lane >> 2), a.n - 1) * words;
+  auto load = [&](int c0) {
+    Load l;
+    // past the end: the row's last codes, against zeros of x
+    const int at = min((c0 + wid) * 16 + (lane & 3) * 4, words - 4);
 #pragma unroll
-  for (int t = 0; t < MT; ++t) xrow[t] = static_cast<const T*>(a.x) + (int64_t)min(m0 + t * 16 + i, a.rows - 1) * a.ldx + g * 8;
+    for (int z = 0; z < Load::S; ++z) {
+      const int e = tid + z * kThreads, row = e / (slab_chunks * G), gi = c0 * G + e - row * (slab_chunks * G);
+      const int64_t from = (int64_t)min(n0 + min(row, kRows - 1), a.n - 1) * a.groups + min(gi, a.groups - 1);
+      l.s[z] = ld_g(static_cast<const T*>(a.scales) + from);
+      l.b[z] = ld_g(static_cast<const T*>(a.biases) + from);
+    }
+#pragma unroll
+    for (int z = 0; z < Load::X; ++z) {
+      const int e = tid + z * kThreads, m = e / pieces, k = c0 * kChunk + (e - m * pieces) * 8;
+      l.x[z] = Op::raw(static_cast<const T*>(a.x) + (int64_t)(m0 + m) * a.ldx + k, m < cols && k < a.k);
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) l.w[t] = ld_nt16(wrow[t] + at);
+    return l;
+  };
+  Load next = load(0);
 
   f32x4_t y[NT][MT];
 #pragma unroll
@@ -130,76 +182,99 @@ __global__ __launch_bounds__(64 * kQ4Waves) void k_q4(const Q4Args a) {
 #pragma unroll
     for (int m = 0; m < MT; ++m) y[t][m] = {0.f, 0.f, 0.f, 0.f};
   const uint4 ones = make_uint4(Op::kOnes, Op::kOnes, Op::kOnes, Op::kOnes);
+  const uint32_t offset = Op::offset();
+  const int pull = (i * 4 + g) * 4;  // the lane with row i's codes of lane group g
 
-  for (int c = wid; c < chunks; c += kQ4Waves) {
-    const int k0 = c * kChunk;
-    uint4 w[NT];
+  int buf = 0;
+  for (int c0 = 0; c0 < chunks; c0 += kQ4Waves) {
+    uint4* xl = reinterpret_cast<uint4*>(lds) + buf * buf16;
+    float2* sc = reinterpret_cast<float2*>(xl + x16);
+    if (c0 > 0 && a.bufs == 1) ring_barrier();
 #pragma unroll
-    for (int t = 0; t < NT; ++t) w[t] = k0 + g * 32 < a.k ? ld_nt16(wrow[t] + k0 / 8) : make_uint4(0, 0, 0, 0);
-    __builtin_amdgcn_wave_barrier();
-    const int gi = min(k0 / 32 / GT + min(g, G - 1), a.groups - 1);
-#pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      const float s = St<T>::ld(ld_g(srow[t] + gi)), b = St<T>::ld(ld_g(brow[t] + gi));
-      sc[wid][t][g][i] = make_float2(s, fmaf(-16.f, s, b));
+    for (int z = 0; z < Load::S; ++z) {
+      const int e = tid + z * kThreads, row = e / (slab_chunks * G), q = e - row * (slab_chunks * G);
+      const float s = St<T>::ld(next.s[z]), b = St<T>::ld(next.b[z]);
+      if (row < kRows) sc[q * kRows + row] = make_float2(s, fmaf(-16.f, s, b));
     }
-    // the wave's own LDS, which serves it in order: only the compiler is held
-    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int z = 0; z < Load::X; ++z) {
+      const int e = tid + z * kThreads, m = e / pieces, p = e - m * pieces;
+      const typename Op::X x = Op::split(next.x[z]);
+      if (m < cols) {
+#pragma unroll
+        for (int c = 0; c < P; ++c) xl[((p / 4 * P + c) * cols + m) * 4 + (p & 3)] = x.part[c];
+      }
+    }
     uint32_t wd[NT][4];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-      wd[t][0] = w[t].x, wd[t][1] = w[t].y, wd[t][2] = w[t].z, wd[t][3] = w[t].w;
-      swap32(wd[t][0], wd[t][2]);
-      swap32(wd[t][1], wd[t][3]);
-      swap16(wd[t][0], wd[t][1]);
-      swap16(wd[t][2], wd[t][3]);
-    }
-#pragma unroll
-    for (int q = 0; q < G; ++q) {
-      f32x4_t p[NT][MT], sum[MT];
-#pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        sum[m] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int t = 0; t < NT; ++t) p[t][m] = {0.f, 0.f, 0.f, 0.f};
-      }
-#pragma unroll
-      for (int z = 0; z < GT; ++z) {
-        const int step = q * GT + z, k = k0 + step * 32;
-#pragma unroll
-        for (int m = 0; m < MT; ++m) {
-          const typename Op::X x = Op::load(xrow[m] + k, k + g * 8 < a.k);
-#pragma unroll
-          for (int c3 = 0; c3 < Op::kParts; ++c3) {
-            sum[m] = Op::M::mma(ones, x.part[c3], sum[m]);
-#pragma unroll
-            for (int t = 0; t < NT; ++t) p[t][m] = Op::M::mma(Op::codes(wd[t][step]), x.part[c3], p[t][m]);
-          }
-        }
-      }
+    for (int t = 0; t < NT; ++t) wd[t][0] = next.w[t].x, wd[t][1] = next.w[t].y, wd[t][2] = next.w[t].z, wd[t][3] = next.w[t].w;
+    if (c0 + kQ4Waves < chunks) next = load(c0 + kQ4Waves);
+    ring_barrier();
+    if (c0 + wid < chunks) {
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
-        const float4 u = *reinterpret_cast<const float4*>(&sc[wid][t][q][g * 4]);
-        const float4 v = *reinterpret_cast<const float4*>(&sc[wid][t][q][g * 4 + 2]);
-        const float s[4] = {u.x, u.z, v.x, v.z}, o[4] = {u.y, u.w, v.y, v.w};
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
+        for (int z = 0; z < 4; ++z) wd[t][z] = __builtin_amdgcn_ds_bpermute(pull, wd[t][z]);
+        swap32(wd[t][0], wd[t][2]);
+        swap32(wd[t][1], wd[t][3]);
+        swap16(wd[t][0], wd[t][1]);
+        swap16(wd[t][2], wd[t][3]);
+      }
+      const uint4* xw[MT];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) y[t][m][r] += fmaf(s[r], p[t][m][r], o[r] * sum[m][r]);
+      for (int m = 0; m < MT; ++m) xw[m] = xl + wid * 4 * P * cols * 4 + min(m * 16 + i, cols - 1) * 4 + g;
+#pragma unroll
+      for (int q = 0; q < G; ++q) {
+        f32x4_t p[NT][MT], sum[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          sum[m] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int t = 0; t < NT; ++t) p[t][m] = {0.f, 0.f, 0.f, 0.f};
+        }
+#pragma unroll
+        for (int z = 0; z < GT; ++z) {
+          const int step = q * GT + z;
+          uint4 code[NT];
+#pragma unroll
+          for (int t = 0; t < NT; ++t) code[t] = Op::codes(wd[t][step], offset);
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int c3 = 0; c3 < P; ++c3) {
+              const uint4 x = xw[m][(step * P + c3) * cols * 4];
+              sum[m] = Op::M::mma(ones, x, sum[m]);
+#pragma unroll
+              for (int t = 0; t < NT; ++t) p[t][m] = Op::M::mma(code[t], x, p[t][m]);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          const float4* at = reinterpret_cast<const float4*>(sc + (wid * G + q) * kRows + t * 16 + g * 4);
+          const float4 u = at[0], v = at[1];
+          const float s[4] = {u.x, u.z, v.x, v.z}, o[4] = {u.y, u.w, v.y, v.w};
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[t][m][r] += fmaf(s[r], p[t][m][r], o[r] * sum[m][r]);
+        }
       }
     }
+    buf ^= a.bufs - 1;
   }
 
+  ring_barrier();
+  f32x4_t* sums = reinterpret_cast<f32x4_t*>(lds);
 #pragma unroll
   for (int t = 0; t < NT; ++t)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) buf[wid][t][m][lane] = y[t][m];
-  __syncthreads();
+    for (int m = 0; m < MT; ++m) sums[((wid * NT + t) * MT + m) * 64 + lane] = y[t][m];
+  ring_barrier();
   for (int z = wid; z < NT * MT; z += kQ4Waves) {
     const int t = z / MT, m = z - t * MT, row = m0 + m * 16 + i, col = n0 + t * 16 + g * 4;
-    f32x4_t v = buf[0][t][m][lane];
+    f32x4_t v = sums[z * 64 + lane];
 #pragma unroll
-    for (int w = 1; w < kQ4Waves; ++w) v += buf[w][t][m][lane];
+    for (int w = 1; w < kQ4Waves; ++w) v += sums[(w * NT * MT + z) * 64 + lane];
     if (row >= a.rows) continue;
     T* dst = static_cast<T*>(a.y) + row * a.ldy + col;
     union {
@@ -220,12 +295,31 @@ __global__ __launch_bounds__(64 * kQ4Waves) void k_q4(const Q4Args a) {
   }
 }
 
+template <typename T, int MT, int GT, int NT>
+void launch(Q4Args a, hipStream_t s) {
+  const size_t slab = (size_t)std::min(kSlab, (a.k + kChunk - 1) / kChunk * kChunk) * std::min(a.rows, 16 * MT) * 2 * Q4Op<T>::kParts +
+                      (size_t)kQ4Waves * (4 / GT) * 16 * NT * 8;
+  a.bufs = a.k > kSlab && 2 * slab <= kTwoSlabs ? 2 : 1;
+  const size_t lds = std::max((size_t)kQ4Waves * NT * MT * 64 * 16, slab * a.bufs);
+  const dim3 grid((a.n + 16 * NT - 1) / (16 * NT), (a.rows + 16 * MT - 1) / (16 * MT));
+  allow_dynamic_lds(reinterpret_cast<const void*>(&k_q4<T, MT, GT, NT>), 160 * 1024);
+  hipLaunchKernelGGL((k_q4<T, MT, GT, NT>), grid, dim3(64 * kQ4Waves), lds, s, a);
+}
+
 template <typename T, int MT, int NT>
-void launch(const Q4Args& a, int group, hipStream_t s) {
-  const dim3 grid((a.n + 16 * NT - 1) / (16 * NT), (a.rows + 63) / 64), block(64 * kQ4Waves);
-  if (group == 32) hipLaunchKernelGGL((k_q4<T, MT, 1, NT>), grid, block, 0, s, a);
-  else if (group == 64) hipLaunchKernelGGL((k_q4<T, MT, 2, NT>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((k_q4<T, MT, 4, NT>), grid, block, 0, s, a);
+void launch_group(const Q4Args& a, int group, hipStream_t s) {
+  if (group == 32) launch<T, MT, 1, NT>(a, s);
+  else if (group == 64) launch<T, MT, 2, NT>(a, s);
+  else launch<T, MT, 4, NT>(a, s);
+}
+
+template <typename T, int MT>
+void launch_tiles(const Q4Args& a, int group, hipStream_t s) {
+  const int tiles = (a.n + 15) / 16;
+  if constexpr (MT == 1)
+    if (tiles >= 4 * kFill) return launch_group<T, MT, 4>(a, group, s);
+  if (tiles >= 2 * kFill) launch_group<T, MT, 2>(a, group, s);
+  else launch_group<T, MT, 1>(a, group, s);
 }
 
 // Eight weights a thread, group / 8 threads a group: bias = least weight, scale = a
@@ -268,11 +362,14 @@ void q4_matmul(DType dt, const Q4Weights& w, const void* x, int64_t ldx, int row
   a.n = w.n, a.k = w.k, a.groups = w.k / w.group, a.rows = rows;
   const size_t unit = 4 * dtype_size(dt);
   a.wide = reinterpret_cast<uintptr_t>(y) % unit == 0 && ldy % 4 == 0;
-  const int mt = (std::min(rows, 64) + 15) / 16;
   MRT_DTYPE_DISPATCH(dt, {
-    if (mt == 1) launch<T, 1, 1>(a, w.group, s);
-    else if (mt == 2) launch<T, 2, 1>(a, w.group, s);
-    else launch<T, 4, 1>(a, w.group, s);
+    if constexpr (std::is_same_v<T, float>) {
+      launch_tiles<T, 1>(a, w.group, s);
+    } else {
+      if (rows <= 16) launch_tiles<T, 1>(a, w.group, s);
+      else if (rows <= 32) launch_tiles<T, 2>(a, w.group, s);
+      else launch_tiles<T, 4>(a, w.group, s);
+    }
   });
   MRT_HIP_CHECK(hipGetLastError());
 }
