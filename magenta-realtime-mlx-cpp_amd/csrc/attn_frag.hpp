@@ -3,10 +3,10 @@
 //
 // A wave holds scores transposed, S^T = K Q^T (keys down, query rows across), so
 // that lane (i, g), i = lane & 15, g = lane >> 4, of the two 16-key tiles of a step
-// has the scores of query row i with keys 8g + 0..3 (first tile) and 8g + 4..7
-// (second): tile row 4g + r is key 8g + r or 8g + 4 + r.  These eight are just what
-// the second product O^T = V^T P^T reads from that lane for the 32 keys, in every
-// type, so P never moves between lanes.  V's operand wants eight keys of one
+// has the scores of query row i with keys 4g .. 4g + 3 (first tile) and 16 + 4g .. 16 +
+// 4g + 3 (second).  These eight are just what the second product O^T = V^T P^T reads
+// from that lane for the 32 keys, in every type, so P never moves between lanes: the
+// order of keys inside that product is free.  V's operand wants eight keys of one
 // dimension in a lane; lane (i, g) loads dimensions i E .. i E + E - 1 (E = DP / 16)
 // of its eight keys and pairs them with one byte permutation a register: output
 // tile t then has dimension i E + t in row i.
@@ -210,7 +210,36 @@ struct AttnFrag {
   }
 };
 
-// Key of row `i` of a step's first (half 0) or second (half 1) 16-key tile.
-__device__ __forceinline__ int step_key(int i, int half) { return ((i >> 2) << 3) + half * 4 + (i & 3); }
+// Key (of a step's 32) of row i of its first (half 0) or second 16-key tile, and of
+// element j of lane group g's eight scores.
+__device__ __forceinline__ int step_key(int i, int half) { return i + 16 * half; }
+__device__ __forceinline__ int lane_key(int g, int j) { return 4 * g + (j & 3) + (j >> 2) * 16; }
+
+// One step of the running softmax of NR row tiles: s, the logits in log2 units (-inf
+// where masked), become weights exp2(s - m); m, l and o follow.  m is the maximum less
+// `shift`, uniform over the lanes of a row; l stays a sum of the lane's own keys.
+template <int NR, int E>
+__device__ __forceinline__ void running_softmax(float (&s)[NR][8], float (&m)[NR], float (&l)[NR], f32x4_t (&o)[NR][E],
+                                                float shift) {
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    float top = s[t][0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) top = fmaxf(top, s[t][j]);
+    top = max_over_groups(top) - shift;
+    if (__any(top > m[t])) {
+      const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
+      m[t] = mn;
+      l[t] *= f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[t][e] *= f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      s[t][j] = __builtin_amdgcn_exp2f(s[t][j] - m[t]);
+      l[t] += s[t][j];
+    }
+  }
+}
 
 }  // namespace mrt

@@ -110,21 +110,22 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
         const int key = min(base + step_key(i, h), end - 1);
         F::load_row(fresh ? kn + acc[key] * a.kn_node : kc + (int64_t)key * a.c_slot, g, D, kf[h]);
       }
-      // the running sum of key base + 8 g + i, by lane i < 8
-      const int key = base + 8 * g + (i & 7), slot = (fresh ? len : 0) + key;
+      // the running sum of the group's key i, by lane i < 8
+      const int key = base + lane_key(g, i & 7), slot = (fresh ? len : 0) + key;
       float sum = 0.f;
       if (i < 8 && key < end) sum = row0 > 0 ? score_out[slot] : fresh || score == nullptr ? 0.f : score[slot];
       int kpos[8];
       if (a.bias != nullptr) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int kj = min(base + 8 * g + j, end - 1);
+          const int kj = min(base + lane_key(g, j), end - 1);
           kpos[j] = fresh ? first + kj : pos != nullptr ? pos[kj] : kj;
         }
       }
       float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
+        if (row0 + t * 16 >= R) continue;
         const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
         const float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
@@ -133,7 +134,7 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
           if (a.bias != nullptr)
             z = a.bias[(size_t)head[t] * a.buckets + min(max(first + tok[t] - kpos[j], 0), a.buckets - 1)];
           z = __builtin_amdgcn_exp2f((fmaf(s[j], a.scale, z) - lse[t]) * kLog2e);
-          w[j] += on[t] && !(fresh && base + 8 * g + j > tok[t]) ? z : 0.f;
+          w[j] += on[t] && !(fresh && base + lane_key(g, j) > tok[t]) ? z : 0.f;
         }
       }
 #pragma unroll

@@ -5,13 +5,18 @@
 //   s_tj = scale q_t . k_j + bias[h, min(distance, M - 1)],  out_t = softmax(s_t) V.
 // One pass over the keys with the running maximum and sum of the softmax.
 //
-// Work split: the n = heads / kv_heads query heads of a KV head share its keys, so a
-// KV head's rows are r = t n + hq, R = nodes n of them, 16 NR to a block; the keys are
-// cut into splits, a block each, whose four waves take steps of 32 keys in turn, each
-// with its own maximum, sum and output in registers (attn_frag.hpp).  The drafted
-// nodes are the last steps of a sequence.  Blocks of one split write the output; with
-// more, each leaves (maximum, sum, output) in fp32 and k_tree_join sums them in order,
-// so a result does not depend on timing.
+// Work: the n = heads / kv_heads query heads of a K/V head share its keys, so a K/V head
+// (a unit) has R = nodes n rows r = t n + hq; its keys are taken in steps of 32, the
+// drafted nodes the last ones.  Two kernels:
+//   k_tree_few (up to 16 rows, fp32, odd head sizes): the four waves of a block take
+//   steps in turn, straight from memory to registers, each with its own maximum, sum and
+//   output; joined through LDS at the end.  What such rows cost is reading the keys.
+//   k_tree_many (16-bit, d 64 or 128): eight waves, WR of them on different rows and
+//   8 / WR on different steps, share K and V through a ring of LDS stages that loads
+//   fill while products run.
+// A unit's steps are cut where the card needs more blocks (Share); parts leave (maximum,
+// sum, output) in fp32 and k_tree_join sums them in order, so a result does not depend
+// on timing.  The cut is made on the device, from the lengths, which the host never sees.
 #include <algorithm>
 #include <type_traits>
 
@@ -24,7 +29,7 @@ namespace {
 
 constexpr int kWaves = 4;
 constexpr float kNone = -1e30f;  // running maximum before any key: finite, so exp2(-inf - kNone) is 0
-constexpr int kBiasLds = 8192;   // floats of the bias by distance kept in LDS
+constexpr int kBiasLds = 4096;   // floats of the bias by distance kept in LDS
 
 struct TreeArgs {
   const void *q, *k_new, *v_new, *k, *v;
@@ -32,14 +37,76 @@ struct TreeArgs {
   const int *parents, *length, *pos, *next_pos;
   const float* bias;
   float* lse;
-  float* part;        // (rows * kv_heads, splits, R, D) outputs of the splits
-  float2* part_ml;    // (rows * kv_heads, splits, R) maximum (in log2 units) and sum
+  float* part;     // (slots, R, D) outputs of the parts
+  float2* part_ml; // (slots, R) maximum (in log2 units) and sum
   uint64_t* present;  // (rows) mask of the nodes that are there
   int64_t q_row, q_node, q_head, kn_row, kn_node, kn_head, vn_row, vn_node, vn_head, o_row, o_node, o_head;
   int64_t c_row, c_head, c_slot, parents_stride;
-  int capacity, kv_heads, heads, nodes, D, buckets, splits, split_steps, row_blocks, units;
+  int rows, capacity, kv_heads, heads, nodes, D, buckets;
+  int teams;       // parts of the whole work wanted; 0: a unit is never cut
+  int least;       // steps that a part has at least
+  int row_blocks;
   float scale;
 };
+
+__device__ __forceinline__ int steps_of(const TreeArgs& a, int b) {
+  const int len = min(max(a.length[b], 0), a.capacity);
+  return (len + kStepKeys - 1) / kStepKeys + (a.nodes + kStepKeys - 1) / kStepKeys;
+}
+
+// How the steps of all units (b, K/V head), in order, are cut into parts.  Long work
+// (16 least a team): team t has the steps [t total / teams, (t + 1) total / teams), which
+// may end and begin inside units; part t of unit u leaves its result in slot u + t.
+// Short work: each unit is cut into parts of `chunk` steps, part t of all in slot t.
+// Either way there are at most teams + units slots.
+struct Share {
+  int64_t total;
+  int chunk;  // 0: by teams
+};
+// A value that all lanes hold, in scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return uniform(v);
+}
+__device__ __forceinline__ Share share_of(const TreeArgs& a, int lane) {
+  int64_t sum = 0;
+  for (int b = lane; b < a.rows; b += 64) sum += steps_of(a, b);
+  Share s;
+  s.total = wave_sum64(sum) * a.kv_heads;
+  s.chunk = s.total >= (int64_t)a.teams * a.least * 2 ? 0 : max(a.least, (int)((s.total + a.teams - 1) / a.teams));
+  return s;
+}
+// The sequence whose units hold position `at` of the running sum of count(b) kv_heads,
+// and the sum before it; rows if there is none.
+template <class Count>
+__device__ __forceinline__ int find_row(const TreeArgs& a, int lane, int64_t at, int64_t* before, Count&& count) {
+  int64_t base = 0;
+  for (int b0 = 0; b0 < a.rows; b0 += 64) {
+    int64_t incl = b0 + lane < a.rows ? (int64_t)count(b0 + lane) * a.kv_heads : 0;
+    const int64_t own = incl;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += x;
+    }
+    const uint64_t past = __ballot(base + incl > at);
+    if (past != 0) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      *before = uniform((int64_t)(base + __shfl(incl - own, l, 64)));
+      return uniform(b0 + l);
+    }
+    base += uniform((int64_t)__shfl(incl, 63, 64));
+  }
+  return a.rows;
+}
+__device__ __forceinline__ int64_t team_of(const Share& s, int teams, int64_t at) {
+  return ((at + 1) * teams + s.total - 1) / s.total - 1;
+}
 
 // Ancestor masks (own bit among them; 0: not there) of a sequence's nodes, by one wave:
 // six doublings reach all 63 ancestors.
@@ -62,28 +129,73 @@ __device__ __forceinline__ uint64_t ancestors(const int* parents, int nodes, int
   return bad ? 0ull : mask;
 }
 
+// E consecutive outputs of row r from dimension d on: to `out`, or, of a part, to its slot.
+template <typename T, int E>
+__device__ __forceinline__ void emit(const TreeArgs& a, bool whole, int64_t slot, int b, int kvh, int r, int d,
+                                     const float (&v)[E], float top, float sum, bool there) {
+  const int n = a.heads / a.kv_heads, node = r / n, h = kvh * n + r - node * n;
+  if (whole) {
+    const float inv = there ? 1.f / sum : 0.f;
+    T* dst = static_cast<T*>(a.out) + b * a.o_row + node * a.o_node + h * a.o_head + d;
+    union {
+      T x[E];
+      uint4 w4[(E * sizeof(T) + 15) / 16];
+      uint2 w2;
+      uint32_t w1;
+    } u;
+#pragma unroll
+    for (int e = 0; e < E; ++e) u.x[e] = St<T>::st(there ? v[e] * inv : 0.f);
+    if constexpr (E * sizeof(T) >= 16) {
+#pragma unroll
+      for (int w = 0; w < (int)(E * sizeof(T) / 16); ++w)
+        if (d + w * (int)(16 / sizeof(T)) < a.D) reinterpret_cast<uint4*>(dst)[w] = u.w4[w];
+    } else if (d < a.D) {
+      if constexpr (E * sizeof(T) == 8) *reinterpret_cast<uint2*>(dst) = u.w2;
+      else *reinterpret_cast<uint32_t*>(dst) = u.w1;
+    }
+    if (a.lse != nullptr && d == 0)
+      a.lse[((size_t)b * a.nodes + node) * a.heads + h] = there ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
+  } else {
+    const size_t at = slot * (size_t)(a.nodes * n) + r;
+    float* dst = a.part + at * a.D + d;
+#pragma unroll
+    for (int e = 0; e < E; e += 2)
+      if (d + e < a.D) *reinterpret_cast<float2*>(dst + e) = make_float2(v[e], v[e + 1]);
+    if (d == 0) a.part_ml[at] = make_float2(top, sum);
+  }
+}
+
 template <typename T, int DP, int NR>
-__global__ __launch_bounds__(64 * kWaves, 1) void k_tree(const TreeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
   using F = AttnFrag<T, DP>;
   constexpr int E = F::E, VW = F::VW, KC = F::KC;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, D = a.D;
-  // Row blocks of the same keys follow each other on one XCD, whose L2 they share.
-  const int id = blockIdx.x >> 3, unit = (id / a.row_blocks) * 8 + (blockIdx.x & 7);
-  if (unit >= a.units) return;
-  const int row0 = (id % a.row_blocks) * (16 * NR);
-  const int bg = unit / a.splits, split = unit - bg * a.splits;
-  const int b = bg / a.kv_heads, kvh = bg - b * a.kv_heads, n = a.heads / a.kv_heads, R = a.nodes * n;
-  const int len = min(max(a.length[b], 0), a.capacity);
-  const int old_steps = (len + kStepKeys - 1) / kStepKeys;
-  const int steps = old_steps + (a.nodes + kStepKeys - 1) / kStepKeys;
-  const int s0 = split * a.split_steps, s1 = min(steps, s0 + a.split_steps);
-  if (s0 >= steps) return;
+  const int id = blockIdx.x / a.row_blocks, row0 = (blockIdx.x - id * a.row_blocks) * (16 * NR);
+  int b, kvh, s0, s1, steps;
+  if (a.teams == 0) {
+    b = id / a.kv_heads, kvh = id - b * a.kv_heads;
+    s0 = 0, s1 = steps = steps_of(a, b);
+  } else {
+    const Share sh = share_of(a, lane);
+    const int chunk = sh.chunk > 0 ? sh.chunk : (int)((sh.total + a.teams - 1) / a.teams);
+    auto parts = [&](int x) { return (steps_of(a, x) + chunk - 1) / chunk; };
+    int64_t before = 0;
+    b = find_row(a, lane, id, &before, parts);
+    if (b >= a.rows) return;
+    const int n = parts(b), at = (int)(id - before);
+    kvh = at / n;
+    steps = steps_of(a, b);
+    s0 = (at - kvh * n) * chunk, s1 = min(steps, s0 + chunk);
+  }
+  const int n = a.heads / a.kv_heads, R = a.nodes * n;
+  const int len = min(max(a.length[b], 0), a.capacity), old_steps = (len + kStepKeys - 1) / kStepKeys;
+  const bool all = s0 == 0 && s1 == steps;
 
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ uint64_t sees[kMaxNodes];
   __shared__ float2 ml[kWaves][16 * NR];
-  float* btab = reinterpret_cast<float*>(lds);  // the bias of this KV head's heads, until the waves join
+  float* btab = reinterpret_cast<float*>(lds);  // the bias of this K/V head's heads, until the waves join
   const bool bias_in_lds = n * a.buckets <= kBiasLds;
 
   uint4 q[NR][KC];
@@ -100,7 +212,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree(const TreeArgs a) {
 
   const T* kc = static_cast<const T*>(a.k) + b * a.c_row + kvh * a.c_head;
   const T* vc = static_cast<const T*>(a.v) + b * a.c_row + kvh * a.c_head;
-  const int* pos = a.pos == nullptr ? nullptr : a.pos + (size_t)bg * a.capacity;
+  const int* pos = a.pos == nullptr ? nullptr : a.pos + (size_t)(b * a.kv_heads + kvh) * a.capacity;
   int qpos[NR];
   const float* brow[NR];
   if (a.bias != nullptr) {
@@ -122,8 +234,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree(const TreeArgs a) {
     for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
   }
   const float scale2 = a.scale * kLog2e;
-  // m is the maximum less kShift: fp16 weights reach up to 2^15, so that those far
-  // below the maximum keep their bits.
+  // fp16 weights reach up to 2^15, so that those far below the maximum keep their bits.
   constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;
 
   for (int st = s0 + wid; st < s1; st += kWaves) {
@@ -139,60 +250,46 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree(const TreeArgs a) {
     for (int h = 0; h < 2; ++h)
       F::load_row(kb + (int64_t)min(base + step_key(i, h), end - 1) * kstep, g, D, kf[h]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) F::load_v(vb + (int64_t)min(base + 8 * g + j, end - 1) * vstep, i, D, vf[j]);
+    for (int j = 0; j < 8; ++j) F::load_v(vb + (int64_t)min(base + lane_key(g, j), end - 1) * vstep, i, D, vf[j]);
     if (!whole) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int w = 0; w < VW; ++w) vf[j][w] = base + 8 * g + j < end ? vf[j][w] : 0u;
+        for (int w = 0; w < VW; ++w) vf[j][w] = base + lane_key(g, j) < end ? vf[j][w] : 0u;
     }
     float p[NR][8];
     int kpos[8];
     if (a.bias != nullptr) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const int key = min(base + 8 * g + j, end - 1);
+        const int key = min(base + lane_key(g, j), end - 1);
         kpos[j] = fresh ? __popcll(sees[key]) - 1 : pos != nullptr ? pos[key] : key;
       }
     }
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
       const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
-      float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      const float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      const int node = min(row0 + t * 16 + i, R - 1) / n;
       if (a.bias != nullptr) {
-        const int at = fresh ? __popcll(sees[min(row0 + t * 16 + i, R - 1) / n]) - 1 : qpos[t];
+        const int at = fresh ? __popcll(sees[node]) - 1 : qpos[t];
 #pragma unroll
         for (int j = 0; j < 8; ++j)
-          s[j] = fmaf(s[j], scale2, brow[t][min(max(at - kpos[j], 0), a.buckets - 1)] * kLog2e);
+          p[t][j] = fmaf(s[j], scale2, brow[t][min(max(at - kpos[j], 0), a.buckets - 1)] * kLog2e);
       } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] *= scale2;
+        for (int j = 0; j < 8; ++j) p[t][j] = s[j] * scale2;
       }
       if (fresh) {
-        const uint64_t see = sees[min(row0 + t * 16 + i, R - 1) / n] >> base;
+        const uint64_t see = sees[node] >> base;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = (see >> (8 * g + j)) & 1 ? s[j] : -INFINITY;
+        for (int j = 0; j < 8; ++j) p[t][j] = (see >> lane_key(g, j)) & 1 ? p[t][j] : -INFINITY;
       } else if (!whole) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = base + 8 * g + j < end ? s[j] : -INFINITY;
-      }
-      float top = s[0];
-#pragma unroll
-      for (int j = 1; j < 8; ++j) top = fmaxf(top, s[j]);
-      top = max_over_groups(top) - kShift;
-      if (__any(top > m[t])) {
-        const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
-        m[t] = mn;
-        l[t] *= f;
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[t][e] *= f;
-      }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        p[t][j] = __builtin_amdgcn_exp2f(s[j] - m[t]);
-        l[t] += p[t][j];
+        for (int j = 0; j < 8; ++j) p[t][j] = base + lane_key(g, j) < end ? p[t][j] : -INFINITY;
       }
     }
+    running_softmax<NR, E>(p, m, l, o, kShift);
     if (!fresh) {
       F::template add_pv<NR>(vf, p, o);
     } else {
@@ -211,7 +308,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree(const TreeArgs a) {
       if (__any(diff != 0)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int key = base + 8 * g + j;
+          const int key = base + lane_key(g, j);
           F::load_v(vb + (int64_t)min(key, end - 1) * vstep, i, D, vf[j]);
 #pragma unroll
           for (int w = 0; w < VW; ++w) vf[j][w] = key < end ? F::classes(vf[j][w]) : 0u;
@@ -221,7 +318,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree(const TreeArgs a) {
           const uint64_t see = sees[min(row0 + t * 16 + i, R - 1) / n] >> base;
           float one[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) one[j] = (see >> (8 * g + j)) & 1 ? 1.f : 0.f;
+          for (int j = 0; j < 8; ++j) one[j] = (see >> lane_key(g, j)) & 1 ? 1.f : 0.f;
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             const f32x4_t c = F::count(vf, one, e);
@@ -252,6 +349,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree(const TreeArgs a) {
   }
   __syncthreads();
   // Thread (lane, r = wid): dimensions (4 g + r) E .. + E - 1 of row i of each tile.
+  const int64_t slot = id;
 #pragma unroll
   for (int t = 0; t < NR; ++t) {
     const int r = row0 + t * 16 + i, d = (4 * g + wid) * E;
@@ -268,75 +366,403 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree(const TreeArgs a) {
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) v[e] += reinterpret_cast<const float*>(&buf[((w * NR + t) * E + e) * 64 + lane])[wid];
     }
-    const int node = r / n, h = kvh * n + r - node * n;
-    if (a.splits == 1) {
-      const bool there = sees[node] != 0;
-      const float inv = there ? 1.f / sum : 0.f;
-      T* dst = static_cast<T*>(a.out) + b * a.o_row + node * a.o_node + h * a.o_head + d;
-      union {
-        T x[E];
-        uint4 w4[(E * sizeof(T) + 15) / 16];
-        uint2 w2;
-        uint32_t w1;
-      } u;
-#pragma unroll
-      for (int e = 0; e < E; ++e) u.x[e] = St<T>::st(there ? v[e] * inv : 0.f);
-      if constexpr (E * sizeof(T) >= 16) {
-#pragma unroll
-        for (int w = 0; w < (int)(E * sizeof(T) / 16); ++w)
-          if (d + w * (int)(16 / sizeof(T)) < D) reinterpret_cast<uint4*>(dst)[w] = u.w4[w];
-      } else if (d < D) {
-        if constexpr (E * sizeof(T) == 8) *reinterpret_cast<uint2*>(dst) = u.w2;
-        else *reinterpret_cast<uint32_t*>(dst) = u.w1;
-      }
-      if (a.lse != nullptr && d == 0)
-        a.lse[((size_t)b * a.nodes + node) * a.heads + h] = there ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
-    } else {
-      const size_t at = ((size_t)bg * a.splits + split) * R + r;
-      float* dst = a.part + at * D + d;
-#pragma unroll
-      for (int e = 0; e < E; e += 2)
-        if (d + e < D) *reinterpret_cast<float2*>(dst + e) = make_float2(v[e], v[e + 1]);
-      if (d == 0) a.part_ml[at] = make_float2(top, sum);
-    }
+    emit<T, E>(a, all, slot, b, kvh, r, d, v, top, sum, sees[r / n] != 0);
   }
-  if (a.splits > 1 && s1 > old_steps && kvh == 0 && row0 == 0 && wid == 0) {
+  if (!all && s1 == steps && row0 == 0 && wid == 0) {  // the same from every K/V head
     const uint64_t there = __ballot(sees[lane] != 0);
     if (lane == 0) a.present[b] = there;
   }
 }
 
-// Sums the splits of one row: a wave a row, each lane some of its dimensions.
-template <typename T>
-__global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a) {
-  const int lane = threadIdx.x & 63, n = a.heads / a.kv_heads, R = a.nodes * n;
-  const int blocks = (R + 3) / 4, bg = blockIdx.x / blocks;
-  const int r = (blockIdx.x - bg * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (r >= R) return;
-  const int b = bg / a.kv_heads, kvh = bg - b * a.kv_heads, node = r / n, h = kvh * n + r - node * n;
-  const int len = min(max(a.length[b], 0), a.capacity);
-  const int steps = (len + kStepKeys - 1) / kStepKeys + (a.nodes + kStepKeys - 1) / kStepKeys;
-  const int splits = (steps + a.split_steps - 1) / a.split_steps;
-  const float2* ml = a.part_ml + (size_t)bg * a.splits * R + r;
-  float top = kNone;
-  for (int s = lane; s < splits; s += 64) top = fmaxf(top, ml[(size_t)s * R].x);
-  top = wave_max(top);
-  const float* part = a.part + ((size_t)bg * a.splits * R + r) * a.D;
-  float sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  const int d = lane * 4;
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float2 x = ml[(size_t)s * R];
-    const float f = __builtin_amdgcn_exp2f(x.x - top);
-    sum = fmaf(x.y, f, sum);
-    if (d < a.D) {
-      const float4 y = *reinterpret_cast<const float4*>(part + (size_t)s * R * a.D + d);
-      v[0] = fmaf(y.x, f, v[0]), v[1] = fmaf(y.y, f, v[1]), v[2] = fmaf(y.z, f, v[2]), v[3] = fmaf(y.w, f, v[3]);
+// ---- many rows ---------------------------------------------------------------------
+
+template <int DP, int WR, int NR>
+struct Many {
+  static constexpr int kWaves = 8, WK = kWaves / WR, kKeys = 32 * WK;  // keys of a stage
+  static constexpr int kRow = 2 * DP, kStage = 2 * kKeys * kRow;       // bytes: a key, K and V of a stage
+  static constexpr int S = kStage >= 64 * 1024 ? 2 : kStage >= 32 * 1024 ? 4 : 6;  // stages
+  static constexpr int kLoads = kStage / 1024 / kWaves;  // 1 KB loads of a wave and stage
+  static constexpr int kPieces = kRow / 16, kRowsLoad = 1024 / kRow;
+  static constexpr size_t kRing = (size_t)S * kStage, kJoin = WK > 1 ? (size_t)kWaves * NR * (DP / 16) * 1024 : 0;
+  static constexpr size_t kLds = kRing > kJoin ? kRing : kJoin;
+  // 16-byte piece p of key row r lies at place p ^ swz(r): the 16 keys of a fragment read
+  // fall in distinct banks.
+  __device__ static int swz(int r) { return DP == 128 ? r & 15 : (r >> 1) & 7; }
+};
+
+// Fragments of one step from LDS.  Written out, since the compiler waits for every load
+// into LDS that is in flight before any read of LDS, which would empty the ring; each
+// block waits for its own reads.  k: rows i and i + 16 at one address per column chunk;
+// v: keys 4g + j and 16 + 4g + j at one address.
+template <int ROW>
+__device__ __forceinline__ void read_k(const uint32_t (&at)[4], uint32_t base, u32x4_t (&f)[2][4]) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:%12\n\tds_read_b128 %2, %9\n\tds_read_b128 %3, %9 offset:%12\n\t"
+      "ds_read_b128 %4, %10\n\tds_read_b128 %5, %10 offset:%12\n\tds_read_b128 %6, %11\n\t"
+      "ds_read_b128 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0][0]), "=&v"(f[1][0]), "=&v"(f[0][1]), "=&v"(f[1][1]), "=&v"(f[0][2]), "=&v"(f[1][2]), "=&v"(f[0][3]),
+        "=&v"(f[1][3])
+      : "v"(at[0] + base), "v"(at[1] + base), "v"(at[2] + base), "v"(at[3] + base), "n"(16 * ROW)
+      : "memory");
+}
+template <int ROW>
+__device__ __forceinline__ void read_k(const uint32_t (&at)[2], uint32_t base, u32x4_t (&f)[2][2]) {
+  asm volatile(
+      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %5\n\tds_read_b128 %3, %5 offset:%6\n\t"
+      "s_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0][0]), "=&v"(f[1][0]), "=&v"(f[0][1]), "=&v"(f[1][1])
+      : "v"(at[0] + base), "v"(at[1] + base), "n"(16 * ROW)
+      : "memory");
+}
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+template <int ROW>
+__device__ __forceinline__ void read_v(uint32_t at, u32x4_t (&f)[8]) {
+  asm volatile(
+      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:%9\n\tds_read_b128 %2, %8 offset:%10\n\t"
+      "ds_read_b128 %3, %8 offset:%11\n\tds_read_b128 %4, %8 offset:%12\n\tds_read_b128 %5, %8 offset:%13\n\t"
+      "ds_read_b128 %6, %8 offset:%14\n\tds_read_b128 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7])
+      : "v"(at), "n"(ROW), "n"(2 * ROW), "n"(3 * ROW), "n"(16 * ROW), "n"(17 * ROW), "n"(18 * ROW), "n"(19 * ROW)
+      : "memory");
+}
+template <int ROW>
+__device__ __forceinline__ void read_v(uint32_t at, u32x2_t (&f)[8]) {
+  asm volatile(
+      "ds_read_b64 %0, %8\n\tds_read_b64 %1, %8 offset:%9\n\tds_read_b64 %2, %8 offset:%10\n\t"
+      "ds_read_b64 %3, %8 offset:%11\n\tds_read_b64 %4, %8 offset:%12\n\tds_read_b64 %5, %8 offset:%13\n\t"
+      "ds_read_b64 %6, %8 offset:%14\n\tds_read_b64 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7])
+      : "v"(at), "n"(ROW), "n"(2 * ROW), "n"(3 * ROW), "n"(16 * ROW), "n"(17 * ROW), "n"(18 * ROW), "n"(19 * ROW)
+      : "memory");
+}
+
+template <typename T, int DP, int WR, int NR, bool BIAS>
+__global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
+  using F = AttnFrag<T, DP>;
+  using M = Many<DP, WR, NR>;
+  constexpr int E = F::E, VW = F::VW, KC = F::KC, WK = M::WK, S = M::S;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
+  // The row blocks of a team share keys: they follow each other on one XCD.
+  const int id = blockIdx.x >> 3, rb = id % a.row_blocks;
+  const int64_t team = (int64_t)(id / a.row_blocks) * 8 + (blockIdx.x & 7);
+  const int n = a.heads / a.kv_heads, R = a.nodes * n, row0 = (rb * WR + wr) * (16 * NR);
+  const float scale2 = a.scale * kLog2e;
+  constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;  // as above
+
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ uint64_t sees[kMaxNodes];
+  __shared__ float2 ml[WK][16 * NR * WR];
+  float* btab = reinterpret_cast<float*>(lds + M::kLds);
+  const uint32_t ring = (uint32_t)(uintptr_t)(MRT_LDS char*)lds;  // LDS address of the ring
+  uint32_t k_at[KC];  // of this lane's key row and chunk, V row, in a stage
+#pragma unroll
+  for (int c = 0; c < KC; ++c) k_at[c] = wk * 32 * M::kRow + i * M::kRow + ((c * 4 + g) ^ M::swz(i)) * 16;
+  const uint32_t v_at = M::kKeys * M::kRow + wk * 32 * M::kRow + 4 * g * M::kRow + i * (2 * E);
+  const bool bias_in_lds = n * a.buckets <= kBiasLds;
+
+  // This block's part of the work: steps [at, stop) of the running order, from unit
+  // (b, kvh) whose first step is at `unit_at`.
+  int b, kvh;
+  int64_t at, stop, unit_at;
+  Share sh{0, 0};
+  if (a.teams == 0) {
+    if (team >= (int64_t)a.rows * a.kv_heads) return;
+    b = (int)(team / a.kv_heads), kvh = (int)(team - (int64_t)b * a.kv_heads);
+    at = unit_at = 0, stop = steps_of(a, b);
+  } else {
+    sh = share_of(a, lane);
+    int64_t before = 0;
+    if (sh.chunk > 0) {
+      auto parts = [&](int x) { return (steps_of(a, x) + sh.chunk - 1) / sh.chunk; };
+      b = find_row(a, lane, team, &before, parts);
+      if (b >= a.rows) return;
+      const int np = parts(b), x = (int)(team - before);
+      kvh = x / np;
+      unit_at = 0, at = (int64_t)(x - kvh * np) * sh.chunk, stop = min((int64_t)steps_of(a, b), at + sh.chunk);
+    } else {
+      if (team >= a.teams) return;
+      at = team * sh.total / a.teams, stop = (team + 1) * sh.total / a.teams;
+      b = find_row(a, lane, at, &before, [&](int x) { return steps_of(a, x); });
+      const int per = steps_of(a, b);
+      kvh = (int)((at - before) / per);
+      unit_at = before + (int64_t)kvh * per;
     }
+  }
+
+  while (at < stop) {
+    const int len = min(max(a.length[b], 0), a.capacity), old_steps = (len + kStepKeys - 1) / kStepKeys;
+    const int steps = steps_of(a, b), s0 = (int)(at - unit_at), s1 = (int)min((int64_t)steps, stop - unit_at);
+    const bool all = s0 == 0 && s1 == steps;
+    const T* kc = static_cast<const T*>(a.k) + b * a.c_row + kvh * a.c_head;
+    const T* vc = static_cast<const T*>(a.v) + b * a.c_row + kvh * a.c_head;
+    const T* kn = static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head;
+    const T* vn = static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
+    const int* pos = a.pos == nullptr ? nullptr : a.pos + (size_t)(b * a.kv_heads + kvh) * a.capacity;
+    const int stages = (s1 - s0 + WK - 1) / WK;
+
+    // Requests stage s (past the end: its last step again): K rows, then V rows.
+    auto issue = [&](int s) {
+      char* to = lds + (s % S) * M::kStage;
+#pragma unroll
+      for (int x = 0; x < M::kLoads; ++x) {
+        const int t = x * M::kWaves + wid, half = M::kLoads * M::kWaves / 2, u = t < half ? t : t - half;
+        const int row = u * M::kRowsLoad + lane / M::kPieces, place = lane % M::kPieces;
+        const int st = min(s0 + s * WK + u * M::kRowsLoad / 32, s1 - 1);
+        const bool fresh = st >= old_steps;
+        const int key = min((fresh ? st - old_steps : st) * kStepKeys + (row & 31), (fresh ? a.nodes : len) - 1);
+        const T* from = t < half ? (fresh ? kn + key * a.kn_node : kc + key * a.c_slot) + (place ^ M::swz(row)) * 8
+                                 : (fresh ? vn + key * a.vn_node : vc + key * a.c_slot) + place * 8;
+        __builtin_amdgcn_global_load_lds((const MRT_GLOBAL void*)from, (MRT_LDS void*)(to + t * 1024), 16, 0, 0);
+      }
+    };
+    uint4 q[NR][KC];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      const int r = min(row0 + t * 16 + i, R - 1), node = r / n;
+      F::load_row(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + r - node * n) * a.q_head,
+                  g, DP, q[t]);
+    }
+    if (wid == 0) sees[lane] = ancestors(a.parents + b * a.parents_stride, a.nodes, lane);
+    if (BIAS && bias_in_lds)
+      for (int x = tid; x < n * a.buckets; x += 512) btab[x] = a.bias[(size_t)kvh * n * a.buckets + x];
+    const int first = BIAS && a.next_pos != nullptr ? a.next_pos[b] : len;
+    // From here on the only vector memory operations are the stages' (but for a bias
+    // with positions or too large for LDS, whose loads make waits longer, not shorter).
+#pragma unroll
+    for (int s = 0; s < S - 1; ++s) issue(s);
+
+    f32x4_t o[NR][E];
+    float m[NR], l[NR];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      m[t] = kNone, l[t] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
+    }
+
+    for (int s = 0; s < stages; ++s) {
+      __builtin_amdgcn_s_waitcnt(vm_wait_imm((S - 2) * M::kLoads));  // this wave's part of stage s is in LDS
+      ring_barrier();                                                // everyone's is, and stage s - 1 has been read
+      issue(s + S - 1);
+      const int st = s0 + s * WK + wk;
+      if (st >= s1 || row0 >= R) continue;
+      const uint32_t stage = ring + (s % S) * M::kStage;
+      const bool fresh = st >= old_steps;
+      const int base = (fresh ? st - old_steps : st) * kStepKeys, end = fresh ? a.nodes : len;
+      const bool whole = base + kStepKeys <= end;
+      u32x4_t kx[2][KC];
+      read_k<M::kRow>(k_at, stage, kx);
+      uint4 kf[2][KC];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kf[h][c] = __builtin_bit_cast(uint4, kx[h][c]);
+      float p[NR][8];
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
+        const float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[t][j] = z[j] * scale2;
+      }
+      if constexpr (BIAS) {
+        int kpos[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int key = min(base + lane_key(g, j), end - 1);
+          kpos[j] = fresh ? __popcll(sees[key]) - 1 : pos != nullptr ? pos[key] : key;
+        }
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+          const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
+          const int qp = (fresh ? 0 : first) + max(__popcll(sees[node]) - 1, 0);
+          const float* row = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[t][j] = fmaf(row[min(max(qp - kpos[j], 0), a.buckets - 1)], kLog2e, p[t][j]);
+        }
+      }
+      if (fresh || !whole) {
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+          const uint64_t see = fresh ? sees[min(row0 + t * 16 + i, R - 1) / n] >> base : ~0ull;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            p[t][j] = base + lane_key(g, j) < end && (see >> lane_key(g, j)) & 1 ? p[t][j] : -INFINITY;
+        }
+      }
+      typename std::conditional<VW == 4, u32x4_t, u32x2_t>::type vx[8];
+      read_v<M::kRow>(v_at + stage, vx);
+      uint32_t vf[8][VW];
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vf[j][w] = vx[j][w];
+      running_softmax<NR, E>(p, m, l, o, kShift);
+      if (!fresh && whole) {
+        F::template add_pv<NR>(vf, p, o);
+        continue;
+      }
+      // Rows past the end are zeros; nodes' infinities and NaN go by class (as above).
+      uint32_t diff = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int w = 0; w < VW; ++w) {
+          const uint32_t v = base + lane_key(g, j) < end ? vf[j][w] : 0u, x = fresh ? F::finite_part(v) : v;
+          diff |= x ^ v;
+          vf[j][w] = x;
+        }
+      F::template add_pv<NR>(vf, p, o);
+      if (__any(diff != 0)) {
+        read_v<M::kRow>(v_at + stage, vx);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vf[j][w] = base + lane_key(g, j) < end ? F::classes(vx[j][w]) : 0u;
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+          const uint64_t see = sees[min(row0 + t * 16 + i, R - 1) / n] >> base;
+          float one[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) one[j] = (see >> lane_key(g, j)) & 1 ? 1.f : 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const f32x4_t c = F::count(vf, one, e);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(c[r]);
+          }
+        }
+      }
+    }
+
+    const int64_t slot = sh.chunk > 0 ? team : (int64_t)b * a.kv_heads + kvh + team;
+    // every load into LDS has landed and every stage been read
+    __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));
+#pragma unroll
+    for (int t = 0; t < NR; ++t) l[t] = sum_over_groups(l[t]);
+    if constexpr (WK == 1) {
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        const int row = row0 + t * 16 + i;
+        if (row >= R) continue;
+        const bool there = sees[row / n] != 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          float v[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) v[e] = o[t][e][r];
+          emit<T, E>(a, all, slot, b, kvh, row, (4 * g + r) * E, v, m[t], l[t], there);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < NR; ++t)
+        if (g == 0) ml[wk][(wr * NR + t) * 16 + i] = make_float2(m[t], l[t]);
+      __syncthreads();
+      f32x4_t* buf = reinterpret_cast<f32x4_t*>(lds);
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        const int x = (wr * NR + t) * 16 + i;
+        float top = ml[0][x].x;
+#pragma unroll
+        for (int w = 1; w < WK; ++w) top = fmaxf(top, ml[w][x].x);
+        const float f = __builtin_amdgcn_exp2f(m[t] - top);
+#pragma unroll
+        for (int e = 0; e < E; ++e) buf[((wid * NR + t) * E + e) * 64 + lane] = o[t][e] * f;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        const int row = row0 + t * 16 + i, x = (wr * NR + t) * 16 + i;
+        if (row >= R) continue;
+        float top = ml[0][x].x, sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < WK; ++w) top = fmaxf(top, ml[w][x].x);
+#pragma unroll
+        for (int w = 0; w < WK; ++w) sum = fmaf(ml[w][x].y, __builtin_amdgcn_exp2f(ml[w][x].x - top), sum);
+#pragma unroll
+        for (int r0 = 0; r0 < 4; r0 += WK) {
+          const int r = r0 + wk;
+          float v[E];
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            v[e] = 0.f;
+#pragma unroll
+            for (int w = 0; w < WK; ++w)
+              v[e] += reinterpret_cast<const float*>(&buf[(((w * WR + wr) * NR + t) * E + e) * 64 + lane])[r];
+          }
+          emit<T, E>(a, all, slot, b, kvh, row, (4 * g + r) * E, v, top, sum, sees[row / n] != 0);
+        }
+      }
+    }
+    if (!all && s1 == steps && rb == 0 && wid == 0) {  // the same from every K/V head
+      const uint64_t there = __ballot(sees[lane] != 0);
+      if (lane == 0) a.present[b] = there;
+    }
+    at = unit_at + s1;
+    if (s1 == steps) {
+      unit_at += steps;
+      if (++kvh == a.kv_heads) kvh = 0, ++b;
+    }
+    __syncthreads();  // LDS may be written again
+  }
+}
+
+// Sums the parts of one row, a wave a row: `cols` lanes share the dimensions, the others
+// further parts.
+template <typename T>
+__global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, bool many, int cols) {
+  const int lane = threadIdx.x & 63, n = a.heads / a.kv_heads, R = a.nodes * n;
+  const int blocks = (R + 3) / 4, unit = blockIdx.x / blocks;
+  const int r = (blockIdx.x - unit * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (r >= R) return;
+  const int b = unit / a.kv_heads, kvh = unit - b * a.kv_heads, node = r / n, h = kvh * n + r - node * n;
+  const Share sh = share_of(a, lane);
+  int64_t first = 0;
+  int parts = 0;
+  const int steps = steps_of(a, b);
+  const int chunk = sh.chunk > 0 ? sh.chunk : many ? 0 : (int)((sh.total + a.teams - 1) / a.teams);
+  int64_t before = 0;  // parts, or steps, of the sequences before
+  for (int x = lane; x < b; x += 64) before += chunk > 0 ? (steps_of(a, x) + chunk - 1) / chunk : steps_of(a, x);
+  before = wave_sum64(before) * a.kv_heads;
+  if (chunk > 0) {
+    parts = (steps + chunk - 1) / chunk;
+    first = before + (int64_t)kvh * parts;
+  } else {
+    const int64_t at = before + (int64_t)kvh * steps, t0 = team_of(sh, a.teams, at);
+    parts = (int)(team_of(sh, a.teams, at + steps - 1) - t0) + 1;
+    first = unit + t0;
+  }
+  if (parts == 1) return;  // written by its block
+  const float2* ml = a.part_ml + first * R + r;
+  const float* part = a.part + (first * R + r) * a.D;
+  const int d = lane % cols * 4, from = lane / cols, every = 64 / cols;
+  float top = kNone, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < parts; s0 += 64) {
+    const float2 x = s0 + lane < parts ? ml[(size_t)(s0 + lane) * R] : make_float2(kNone, 0.f);
+    const float to = fmaxf(top, wave_max(x.x)), f = __builtin_amdgcn_exp2f(top - to);
+    top = to;
+    const float w = s0 + lane < parts ? __builtin_amdgcn_exp2f(x.x - top) : 0.f;
+    sum = fmaf(sum, f, wave_sum(x.y * w));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= f;
+    const int end = min(64, parts - s0);
+    for (int s = from; s < ((end + every - 1) / every) * every; s += every) {
+      const float ws = __shfl(w, s, 64);
+      if (s < end && d < a.D) {
+        const float4 y = *reinterpret_cast<const float4*>(part + (size_t)(s0 + s) * R * a.D + d);
+        v[0] = fmaf(y.x, ws, v[0]), v[1] = fmaf(y.y, ws, v[1]), v[2] = fmaf(y.z, ws, v[2]), v[3] = fmaf(y.w, ws, v[3]);
+      }
+    }
+  }
+  for (int o = cols; o < 64; o <<= 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], o, 64);
   }
   const bool there = (a.present[b] >> node) & 1;
   const float inv = 1.f / sum;
-  if (d < a.D) {
+  if (d < a.D && from == 0) {
     T* dst = static_cast<T*>(a.out) + b * a.o_row + node * a.o_node + h * a.o_head + d;
     union {
       T x[4];
@@ -352,56 +778,81 @@ __global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a) {
     a.lse[((size_t)b * a.nodes + node) * a.heads + h] = there ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
 }
 
-// Row tiles that a wave's registers hold: the output takes dp / 4 a tile, queries as
-// much again in 16-bit types (twice that in fp32), a step's keys and values dp / 2.
+// Row tiles that a wave of k_tree_few holds: the output takes dp / 4 registers a tile,
+// queries as much again in 16-bit types (twice that in fp32), a step's keys and values dp / 2.
 constexpr int row_tiles(size_t elt, int dp) {
   return dp == 256 ? 1 : elt == 4 || dp == 128 ? 2 : 4;
 }
 
 struct Plan {
-  int nr, splits, split_steps, row_blocks;
+  bool many;
+  int tiles;  // row tiles of a block
+  int row_blocks, teams, least;
 };
 
 Plan plan(const KvCache& c, int heads, int nodes) {
   const int R = nodes * (heads / c.kv_heads), dp = c.d <= 32 ? 32 : c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
-  const int most = row_tiles(dtype_size(c.dt), dp);
   Plan p;
-  p.nr = std::min(most, R <= 16 ? 1 : R <= 32 ? 2 : 4);
-  p.row_blocks = (R + 16 * p.nr - 1) / (16 * p.nr);
-  const int steps = (c.capacity + kStepKeys - 1) / kStepKeys + (nodes + kStepKeys - 1) / kStepKeys;
-  const int units = std::max(1, c.rows * c.kv_heads * p.row_blocks);
-  const int want = std::max(1, 1024 / units);
-  p.split_steps = std::max(2 * kWaves, (steps + want - 1) / want);
-  p.splits = (steps + p.split_steps - 1) / p.split_steps;
-  if (p.splits == 1) p.split_steps = steps;
+  p.many = R > 16 && c.dt != DType::F32 && (c.d == 64 || c.d == 128);
+  p.tiles = p.many ? (R <= 32 ? 2 : R <= 64 ? 4 : R <= 128 || c.d == 128 ? 8 : 16)
+                   : std::min(row_tiles(dtype_size(c.dt), dp), R <= 16 ? 1 : R <= 32 ? 2 : 4);
+  p.row_blocks = (R + 16 * p.tiles - 1) / (16 * p.tiles);
+  const int64_t steps = (c.capacity + kStepKeys - 1) / kStepKeys + (nodes + kStepKeys - 1) / kStepKeys;
+  // k_tree_many fills a CU with a block; of the others a CU holds a few at a time, and
+  // more of them even out the lengths.
+  p.least = 8;
+  p.teams = std::max(8, (p.many ? 256 : 1024) / p.row_blocks / 8 * 8);
+  if (steps <= p.least) p.teams = 0;
   return p;
 }
 
+size_t slots(const KvCache& c, const Plan& p) { return p.teams == 0 ? 0 : (size_t)p.teams + (size_t)c.rows * c.kv_heads; }
+
 template <typename T, int DP, int NR>
-void launch(const TreeArgs& a, hipStream_t s) {
+void launch_few(const TreeArgs& a, int blocks, hipStream_t s) {
   const size_t join = (size_t)kWaves * NR * AttnFrag<T, DP>::E * 64 * 16;
   const size_t lds = std::max(join, a.bias != nullptr ? (size_t)kBiasLds * 4 : size_t{0});
-  allow_dynamic_lds(reinterpret_cast<const void*>(&k_tree<T, DP, NR>), std::max(join, (size_t)kBiasLds * 4));
-  const int grid = (a.units + 7) / 8 * 8 * a.row_blocks;
-  hipLaunchKernelGGL((k_tree<T, DP, NR>), dim3(grid), dim3(64 * kWaves), lds, s, a);
+  allow_dynamic_lds(reinterpret_cast<const void*>(&k_tree_few<T, DP, NR>), std::max(join, (size_t)kBiasLds * 4));
+  hipLaunchKernelGGL((k_tree_few<T, DP, NR>), dim3(blocks * a.row_blocks), dim3(64 * kWaves), lds, s, a);
 }
 
 template <typename T, int DP>
-void launch_nr(const TreeArgs& a, int nr, hipStream_t s) {
+void launch_few(const TreeArgs& a, int blocks, int nr, hipStream_t s) {
   constexpr int most = row_tiles(sizeof(T), DP);
-  if (nr == 1) return launch<T, DP, 1>(a, s);
+  if (nr == 1) return launch_few<T, DP, 1>(a, blocks, s);
   if constexpr (most >= 2)
-    if (nr == 2) return launch<T, DP, 2>(a, s);
-  if constexpr (most >= 4) launch<T, DP, 4>(a, s);
+    if (nr == 2) return launch_few<T, DP, 2>(a, blocks, s);
+  if constexpr (most >= 4) launch_few<T, DP, 4>(a, blocks, s);
+}
+
+template <typename T, int DP, int WR, int NR>
+void launch_many(const TreeArgs& a, int blocks, hipStream_t s) {
+  using M = Many<DP, WR, NR>;
+  const dim3 grid((blocks + 7) / 8 * 8 * a.row_blocks);
+  if (a.bias != nullptr) {
+    const size_t lds = M::kLds + (size_t)kBiasLds * 4;
+    allow_dynamic_lds(reinterpret_cast<const void*>(&k_tree_many<T, DP, WR, NR, true>), lds);
+    hipLaunchKernelGGL((k_tree_many<T, DP, WR, NR, true>), grid, dim3(512), lds, s, a);
+  } else {
+    allow_dynamic_lds(reinterpret_cast<const void*>(&k_tree_many<T, DP, WR, NR, false>), M::kLds);
+    hipLaunchKernelGGL((k_tree_many<T, DP, WR, NR, false>), grid, dim3(512), M::kLds, s, a);
+  }
+}
+
+template <typename T, int DP>
+void launch_many(const TreeArgs& a, int blocks, int tiles, hipStream_t s) {
+  if (tiles == 2) launch_many<T, DP, 2, 1>(a, blocks, s);
+  else if (tiles == 4) launch_many<T, DP, 4, 1>(a, blocks, s);
+  else if (tiles == 8) launch_many<T, DP, 8, 1>(a, blocks, s);
+  else if constexpr (DP == 64) launch_many<T, DP, 8, 2>(a, blocks, s);
 }
 
 }  // namespace
 
 size_t tree_attention_workspace(const KvCache& c, int heads, int nodes) {
   const Plan p = plan(c, heads, nodes);
-  if (p.splits == 1) return 0;
-  const size_t rows = (size_t)c.rows * heads * nodes * p.splits;
-  return rows * (c.d + 2) * 4 + (size_t)c.rows * 8;
+  if (p.teams == 0) return 0;
+  return slots(c, p) * (size_t)(heads / c.kv_heads * nodes) * (c.d + 2) * 4 + (size_t)c.rows * 8;
 }
 
 void tree_attention(const KvCache& c, const TreeAttnArgs& t, void* ws, hipStream_t s) {
@@ -415,27 +866,38 @@ void tree_attention(const KvCache& c, const TreeAttnArgs& t, void* ws, hipStream
   a.vn_row = t.v_new.row_stride, a.vn_node = t.v_new.node_stride, a.vn_head = t.v_new.head_stride;
   a.o_row = t.out.row_stride, a.o_node = t.out.node_stride, a.o_head = t.out.head_stride;
   a.c_row = c.row_stride, a.c_head = c.head_stride, a.c_slot = c.slot_stride, a.parents_stride = t.parents_stride;
-  a.capacity = c.capacity, a.kv_heads = c.kv_heads, a.heads = t.heads, a.nodes = t.nodes, a.D = c.d;
-  a.buckets = t.buckets, a.splits = p.splits, a.split_steps = p.split_steps, a.row_blocks = p.row_blocks;
-  a.units = c.rows * c.kv_heads * p.splits;
+  a.rows = c.rows, a.capacity = c.capacity, a.kv_heads = c.kv_heads, a.heads = t.heads, a.nodes = t.nodes, a.D = c.d;
+  a.buckets = t.buckets, a.teams = p.teams, a.least = p.least, a.row_blocks = p.row_blocks;
   a.scale = t.scale;
-  if (p.splits > 1) {
-    const size_t rows = (size_t)c.rows * t.heads * t.nodes * p.splits;
+  const int R = t.nodes * (t.heads / c.kv_heads);
+  if (p.teams > 0) {
+    const size_t rows = slots(c, p) * R;
     a.part = static_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(a.part + rows * c.d);
     a.present = reinterpret_cast<uint64_t*>(a.part_ml + rows);
   }
-  MRT_DTYPE_DISPATCH(c.dt, {
-    if (c.d <= 32) launch_nr<T, 32>(a, p.nr, s);
-    else if (c.d <= 64) launch_nr<T, 64>(a, p.nr, s);
-    else if (c.d <= 128) launch_nr<T, 128>(a, p.nr, s);
-    else launch_nr<T, 256>(a, p.nr, s);
-  });
+  const int blocks = p.teams > 0 ? (int)slots(c, p) : c.rows * c.kv_heads;
+  if (p.many) {
+    auto go = [&](auto x) {
+      using T = decltype(x);
+      if (c.d == 64) launch_many<T, 64>(a, blocks, p.tiles, s);
+      else launch_many<T, 128>(a, blocks, p.tiles, s);
+    };
+    if (c.dt == DType::BF16) go(bf16{});
+    else go(f16{});
+  } else {
+    MRT_DTYPE_DISPATCH(c.dt, {
+      if (c.d <= 32) launch_few<T, 32>(a, blocks, p.tiles, s);
+      else if (c.d <= 64) launch_few<T, 64>(a, blocks, p.tiles, s);
+      else if (c.d <= 128) launch_few<T, 128>(a, blocks, p.tiles, s);
+      else launch_few<T, 256>(a, blocks, p.tiles, s);
+    });
+  }
   MRT_HIP_CHECK(hipGetLastError());
-  if (p.splits > 1) {
-    const int R = t.nodes * (t.heads / c.kv_heads);
+  if (p.teams > 0) {
     const dim3 grid(c.rows * c.kv_heads * ((R + 3) / 4));
-    MRT_DTYPE_DISPATCH(c.dt, hipLaunchKernelGGL(k_tree_join<T>, grid, dim3(256), 0, s, a));
+    const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64;
+    MRT_DTYPE_DISPATCH(c.dt, hipLaunchKernelGGL(k_tree_join<T>, grid, dim3(256), 0, s, a, p.many, cols));
     MRT_HIP_CHECK(hipGetLastError());
   }
 }

@@ -115,6 +115,19 @@ CASES = [
     (1, 2, 1, 200, 20, [130]),
     (1, 8, 1, 256, 4, [777]),
     (5, 2, 1, 32, 2, [5, 0, 200, 32, 96]),
+    (2, 8, 4, 64, 15, [900, 260]),             # 30 rows: two row tiles, four key groups
+    (2, 8, 4, 128, 16, [900, 260]),
+    (2, 4, 2, 64, 31, [900, 260]),             # 62 rows: four row tiles
+    (2, 4, 2, 128, 20, [300, 1100]),
+    (1, 16, 4, 64, 30, [513]),                 # 120 rows: eight
+    (1, 8, 2, 128, 29, [1025]),
+    (1, 12, 2, 64, 50, [333]),                 # 300 rows: two blocks of sixteen
+    (2, 9, 1, 128, 33, [100, 640]),
+    # work enough that parts are cut by equal shares, across sequences and heads
+    (4, 16, 8, 64, 9, [7000, 5000, 31, 6200]),
+    (3, 32, 16, 128, 17, [6000, 3333, 1]),
+    (70, 8, 4, 64, 20, [700 + 13 * b for b in range(70)]),
+    (2, 16, 2, 64, 20, [9000, 30000]),
 ]
 
 
