@@ -53,6 +53,15 @@ struct Mma<bf16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
   static constexpr uint32_t kExp = 0x7f80u;  // all ones: infinite or NaN
+  // Two values to the type and back, the first in the low half.
+  __device__ __forceinline__ static uint32_t pack(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    const f2 v = {x, y};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2));
+  }
+  __device__ __forceinline__ static float low(uint32_t w) { return __uint_as_float(w << 16); }
+  __device__ __forceinline__ static float high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 };
 template <>
 struct Mma<f16> {
@@ -61,6 +70,18 @@ struct Mma<f16> {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
   }
   static constexpr uint32_t kExp = 0x7c00u;
+  __device__ __forceinline__ static uint32_t pack(float x, float y) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    const f2 v = {x, y};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2));
+  }
+  __device__ __forceinline__ static float low(uint32_t w) {
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)(w & 0xffffu));
+  }
+  __device__ __forceinline__ static float high(uint32_t w) {
+    return (float)__builtin_bit_cast(_Float16, (unsigned short)(w >> 16));
+  }
 };
 template <>
 struct Mma<float> {
@@ -114,6 +135,17 @@ struct AttnFrag {
       f[0] = D == DP || i * E < D ? ld_g(reinterpret_cast<const uint32_t*>(p)) : 0u;
     }
   }
+  // Eight weights as a high and a low operand.
+  __device__ __forceinline__ static void split(const float (&p)[8], uint4& h, uint4& l) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      hi[j] = Mma<T>::pack(p[2 * j], p[2 * j + 1]);
+      lo[j] = Mma<T>::pack(p[2 * j] - Mma<T>::low(hi[j]), p[2 * j + 1] - Mma<T>::high(hi[j]));
+    }
+    h = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    l = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
   // o[r][t] += V^T P^T of the lane's eight keys, for every row tile r.  16-bit types:
   // P in two parts, high and low, since rounding P alone to 16 bits would add as much
   // error as the output's own rounding; the parts' sum is within 2^-17 (bf16) of P.
@@ -129,21 +161,9 @@ struct AttnFrag {
           for (int r = 0; r < NR; ++r)
             o[r][t] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v[j][t]), p[r][j], o[r][t], 0, 0, 0);
     } else {
-      using S = St<T>;
       uint4 ph[NR], pl[NR];
 #pragma unroll
-      for (int r = 0; r < NR; ++r) {
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = p[r][2 * j], y = p[r][2 * j + 1];
-          const uint32_t a = S::bits(x), b = S::bits(y);
-          hi[j] = a | (b << 16);
-          lo[j] = S::bits(x - S::unbits(a)) | (S::bits(y - S::unbits(b)) << 16);
-        }
-        ph[r] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-        pl[r] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
-      }
+      for (int r = 0; r < NR; ++r) split(p[r], ph[r], pl[r]);
 #pragma unroll
       for (int t = 0; t < E; ++t) {
         const uint4 a = v_operand(v, t);

@@ -158,9 +158,13 @@ __device__ __forceinline__ void emit(const TreeArgs& a, bool whole, int64_t slot
   } else {
     const size_t at = slot * (size_t)(a.nodes * n) + r;
     float* dst = a.part + at * a.D + d;
+    if constexpr (E % 4 == 0) {
 #pragma unroll
-    for (int e = 0; e < E; e += 2)
-      if (d + e < a.D) *reinterpret_cast<float2*>(dst + e) = make_float2(v[e], v[e + 1]);
+      for (int e = 0; e < E; e += 4)
+        if (d + e < a.D) *reinterpret_cast<float4*>(dst + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else if (d < a.D) {
+      *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
+    }
     if (d == 0) a.part_ml[at] = make_float2(top, sum);
   }
 }
@@ -380,20 +384,20 @@ template <int DP, int WR, int NR>
 struct Many {
   static constexpr int kWaves = 8, WK = kWaves / WR, kKeys = 32 * WK;  // keys of a stage
   static constexpr int kRow = 2 * DP, kStage = 2 * kKeys * kRow;       // bytes: a key, K and V of a stage
-  static constexpr int S = kStage >= 64 * 1024 ? 2 : kStage >= 32 * 1024 ? 4 : 6;  // stages
+  static constexpr int S = kStage >= 64 * 1024 ? 2 : 4;                // stages
   static constexpr int kLoads = kStage / 1024 / kWaves;  // 1 KB loads of a wave and stage
   static constexpr int kPieces = kRow / 16, kRowsLoad = 1024 / kRow;
   static constexpr size_t kRing = (size_t)S * kStage, kJoin = WK > 1 ? (size_t)kWaves * NR * (DP / 16) * 1024 : 0;
   static constexpr size_t kLds = kRing > kJoin ? kRing : kJoin;
-  // 16-byte piece p of key row r lies at place p ^ swz(r): the 16 keys of a fragment read
-  // fall in distinct banks.
-  __device__ static int swz(int r) { return DP == 128 ? r & 15 : (r >> 1) & 7; }
+  // 16-byte piece p of row r lies at place p ^ swz(r), so that what is read together falls
+  // in distinct banks: of K the same piece of 16 keys, of V 32 bytes of 4 keys.
+  __device__ static int swz_k(int r) { return DP == 128 ? r & 15 : (r >> 1) & 7; }
+  __device__ static int swz_v(int r) { return DP == 128 ? (r & 3) * 2 : ((r >> 1) & 1) * 2; }
 };
 
 // Fragments of one step from LDS.  Written out, since the compiler waits for every load
 // into LDS that is in flight before any read of LDS, which would empty the ring; each
-// block waits for its own reads.  k: rows i and i + 16 at one address per column chunk;
-// v: keys 4g + j and 16 + 4g + j at one address.
+// block waits for its own reads.  K: rows i and i + 16 at one address per column chunk.
 template <int ROW>
 __device__ __forceinline__ void read_k(const uint32_t (&at)[4], uint32_t base, u32x4_t (&f)[2][4]) {
   asm volatile(
@@ -414,25 +418,35 @@ __device__ __forceinline__ void read_k(const uint32_t (&at)[2], uint32_t base, u
       : "v"(at[0] + base), "v"(at[1] + base), "n"(16 * ROW)
       : "memory");
 }
+// V, transposed as it is read: of 16 lanes, lane 4 r + c gives the address of columns 4 c ..
+// 4 c + 3 of row r, and lane i receives column i of rows 0..3.  f[e][h]: keys 16 h + 4 g ..
+// + 3 of dimension 16 e + i.  Tiles e and e + 4 share an address (128 bytes apart).
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 template <int ROW>
-__device__ __forceinline__ void read_v(uint32_t at, u32x4_t (&f)[8]) {
+__device__ __forceinline__ void read_v(const uint32_t (&at)[4], uint32_t base, u32x2_t (&f)[4][2]) {
   asm volatile(
-      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:%9\n\tds_read_b128 %2, %8 offset:%10\n\t"
-      "ds_read_b128 %3, %8 offset:%11\n\tds_read_b128 %4, %8 offset:%12\n\tds_read_b128 %5, %8 offset:%13\n\t"
-      "ds_read_b128 %6, %8 offset:%14\n\tds_read_b128 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7])
-      : "v"(at), "n"(ROW), "n"(2 * ROW), "n"(3 * ROW), "n"(16 * ROW), "n"(17 * ROW), "n"(18 * ROW), "n"(19 * ROW)
+      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %9\n\t"
+      "ds_read_b64_tr_b16 %3, %9 offset:%12\n\tds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1]), "=&v"(f[2][0]), "=&v"(f[2][1]), "=&v"(f[3][0]),
+        "=&v"(f[3][1])
+      : "v"(at[0] + base), "v"(at[1] + base), "v"(at[2] + base), "v"(at[3] + base), "n"(16 * ROW)
       : "memory");
 }
 template <int ROW>
-__device__ __forceinline__ void read_v(uint32_t at, u32x2_t (&f)[8]) {
+__device__ __forceinline__ void read_v(const uint32_t (&at)[4], uint32_t base, u32x2_t (&f)[8][2]) {
   asm volatile(
-      "ds_read_b64 %0, %8\n\tds_read_b64 %1, %8 offset:%9\n\tds_read_b64 %2, %8 offset:%10\n\t"
-      "ds_read_b64 %3, %8 offset:%11\n\tds_read_b64 %4, %8 offset:%12\n\tds_read_b64 %5, %8 offset:%13\n\t"
-      "ds_read_b64 %6, %8 offset:%14\n\tds_read_b64 %7, %8 offset:%15\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0]), "=&v"(f[1]), "=&v"(f[2]), "=&v"(f[3]), "=&v"(f[4]), "=&v"(f[5]), "=&v"(f[6]), "=&v"(f[7])
-      : "v"(at), "n"(ROW), "n"(2 * ROW), "n"(3 * ROW), "n"(16 * ROW), "n"(17 * ROW), "n"(18 * ROW), "n"(19 * ROW)
+      "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:%20\n\tds_read_b64_tr_b16 %2, %17\n\t"
+      "ds_read_b64_tr_b16 %3, %17 offset:%20\n\tds_read_b64_tr_b16 %4, %18\n\tds_read_b64_tr_b16 %5, %18 offset:%20\n\t"
+      "ds_read_b64_tr_b16 %6, %19\n\tds_read_b64_tr_b16 %7, %19 offset:%20\n\tds_read_b64_tr_b16 %8, %16 offset:128\n\t"
+      "ds_read_b64_tr_b16 %9, %16 offset:%21\n\tds_read_b64_tr_b16 %10, %17 offset:128\n\t"
+      "ds_read_b64_tr_b16 %11, %17 offset:%21\n\tds_read_b64_tr_b16 %12, %18 offset:128\n\t"
+      "ds_read_b64_tr_b16 %13, %18 offset:%21\n\tds_read_b64_tr_b16 %14, %19 offset:128\n\t"
+      "ds_read_b64_tr_b16 %15, %19 offset:%21\n\ts_waitcnt lgkmcnt(0)"
+      : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1]), "=&v"(f[2][0]), "=&v"(f[2][1]), "=&v"(f[3][0]),
+        "=&v"(f[3][1]), "=&v"(f[4][0]), "=&v"(f[4][1]), "=&v"(f[5][0]), "=&v"(f[5][1]), "=&v"(f[6][0]), "=&v"(f[6][1]),
+        "=&v"(f[7][0]), "=&v"(f[7][1])
+      : "v"(at[0] + base), "v"(at[1] + base), "v"(at[2] + base), "v"(at[3] + base), "n"(16 * ROW), "n"(16 * ROW + 128)
       : "memory");
 }
 
@@ -440,14 +454,17 @@ template <typename T, int DP, int WR, int NR, bool BIAS>
 __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   using F = AttnFrag<T, DP>;
   using M = Many<DP, WR, NR>;
-  constexpr int E = F::E, VW = F::VW, KC = F::KC, WK = M::WK, S = M::S;
+  constexpr int E = F::E, KC = F::KC, WK = M::WK, S = M::S;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, wr = wid % WR, wk = wid / WR;
   // The row blocks of a team share keys: they follow each other on one XCD.
   const int id = blockIdx.x >> 3, rb = id % a.row_blocks;
   const int64_t team = (int64_t)(id / a.row_blocks) * 8 + (blockIdx.x & 7);
   const int n = a.heads / a.kv_heads, R = a.nodes * n, row0 = (rb * WR + wr) * (16 * NR);
-  const float scale2 = a.scale * kLog2e;
+  // Logits in log2 units are mult z: z the products themselves, whose sign q takes on, or
+  // with a bias the finished logits.
+  const float scale2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f), mult = BIAS ? 1.f : scale2;
+  const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
   constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;  // as above
 
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -455,10 +472,23 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   __shared__ float2 ml[WK][16 * NR * WR];
   float* btab = reinterpret_cast<float*>(lds + M::kLds);
   const uint32_t ring = (uint32_t)(uintptr_t)(MRT_LDS char*)lds;  // LDS address of the ring
-  uint32_t k_at[KC];  // of this lane's key row and chunk, V row, in a stage
+  uint32_t k_at[KC], v_at[4];  // in a stage: this lane's key row and chunk; V row and columns
 #pragma unroll
-  for (int c = 0; c < KC; ++c) k_at[c] = wk * 32 * M::kRow + i * M::kRow + ((c * 4 + g) ^ M::swz(i)) * 16;
-  const uint32_t v_at = M::kKeys * M::kRow + wk * 32 * M::kRow + 4 * g * M::kRow + i * (2 * E);
+  for (int c = 0; c < KC; ++c) k_at[c] = (wk * 32 + i) * M::kRow + ((c * 4 + g) ^ M::swz_k(i)) * 16;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const int row = 4 * g + (i >> 2), piece = 2 * e + ((i >> 1) & 1);
+    v_at[e] = (M::kKeys + wk * 32 + row) * M::kRow + (piece ^ M::swz_v(row)) * 16 + (i & 1) * 8;
+  }
+  // Where this lane's part of each load lies behind a stage's first key (whole stages).
+  uint32_t src[M::kLoads];
+  const bool near = a.c_slot < (1 << 23);
+#pragma unroll
+  for (int x = 0; x < M::kLoads; ++x) {
+    const int t = x * M::kWaves + wid, half = M::kLoads * M::kWaves / 2, u = t < half ? t : t - half;
+    const int row = u * M::kRowsLoad + lane / M::kPieces, place = lane % M::kPieces;
+    src[x] = ((uint32_t)row * (uint32_t)a.c_slot + (place ^ (t < half ? M::swz_k(row & 31) : M::swz_v(row))) * 8) * 2;
+  }
   const bool bias_in_lds = n * a.buckets <= kBiasLds;
 
   // This block's part of the work: steps [at, stop) of the running order, from unit
@@ -489,30 +519,43 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       unit_at = before + (int64_t)kvh * per;
     }
   }
+  b = uniform(b), kvh = uniform(kvh), at = uniform(at), stop = uniform(stop), unit_at = uniform(unit_at);
 
   while (at < stop) {
-    const int len = min(max(a.length[b], 0), a.capacity), old_steps = (len + kStepKeys - 1) / kStepKeys;
-    const int steps = steps_of(a, b), s0 = (int)(at - unit_at), s1 = (int)min((int64_t)steps, stop - unit_at);
+    const int len = uniform(min(max(a.length[b], 0), a.capacity)), old_steps = (len + kStepKeys - 1) / kStepKeys;
+    const int steps = old_steps + (a.nodes + kStepKeys - 1) / kStepKeys;
+    const int s0 = (int)(at - unit_at), s1 = (int)min((int64_t)steps, stop - unit_at);
     const bool all = s0 == 0 && s1 == steps;
     const T* kc = static_cast<const T*>(a.k) + b * a.c_row + kvh * a.c_head;
     const T* vc = static_cast<const T*>(a.v) + b * a.c_row + kvh * a.c_head;
-    const T* kn = static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head;
-    const T* vn = static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
-    const int* pos = a.pos == nullptr ? nullptr : a.pos + (size_t)(b * a.kv_heads + kvh) * a.capacity;
     const int stages = (s1 - s0 + WK - 1) / WK;
 
     // Requests stage s (past the end: its last step again): K rows, then V rows.
     auto issue = [&](int s) {
       char* to = lds + (s % S) * M::kStage;
+      const int first = s0 + s * WK;
+      if (near && first + WK <= s1 && (first + WK) * kStepKeys <= len) {
+        const char* kb = reinterpret_cast<const char*>(kc + (int64_t)first * kStepKeys * a.c_slot);
+        const char* vb = reinterpret_cast<const char*>(vc + (int64_t)first * kStepKeys * a.c_slot);
+#pragma unroll
+        for (int x = 0; x < M::kLoads; ++x) {
+          const int t = x * M::kWaves + wid;
+          const char* from = (x < M::kLoads / 2 || (M::kLoads == 1 && wid < M::kWaves / 2) ? kb : vb) + src[x];
+          __builtin_amdgcn_global_load_lds((const MRT_GLOBAL void*)from, (MRT_LDS void*)(to + t * 1024), 16, 0, 0);
+        }
+        return;
+      }
+      const T* kn = static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head;
+      const T* vn = static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
 #pragma unroll
       for (int x = 0; x < M::kLoads; ++x) {
         const int t = x * M::kWaves + wid, half = M::kLoads * M::kWaves / 2, u = t < half ? t : t - half;
         const int row = u * M::kRowsLoad + lane / M::kPieces, place = lane % M::kPieces;
-        const int st = min(s0 + s * WK + u * M::kRowsLoad / 32, s1 - 1);
+        const int st = min(first + u * M::kRowsLoad / 32, s1 - 1);
         const bool fresh = st >= old_steps;
         const int key = min((fresh ? st - old_steps : st) * kStepKeys + (row & 31), (fresh ? a.nodes : len) - 1);
-        const T* from = t < half ? (fresh ? kn + key * a.kn_node : kc + key * a.c_slot) + (place ^ M::swz(row)) * 8
-                                 : (fresh ? vn + key * a.vn_node : vc + key * a.c_slot) + place * 8;
+        const T* from = t < half ? (fresh ? kn + key * a.kn_node : kc + key * a.c_slot) + (place ^ M::swz_k(row & 31)) * 8
+                                 : (fresh ? vn + key * a.vn_node : vc + key * a.c_slot) + (place ^ M::swz_v(row)) * 8;
         __builtin_amdgcn_global_load_lds((const MRT_GLOBAL void*)from, (MRT_LDS void*)(to + t * 1024), 16, 0, 0);
       }
     };
@@ -523,16 +566,20 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       F::load_row(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + r - node * n) * a.q_head,
                   g, DP, q[t]);
     }
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+#pragma unroll
+      for (int c = 0; c < KC; ++c) q[t][c].x ^= flip, q[t][c].y ^= flip, q[t][c].z ^= flip, q[t][c].w ^= flip;
     if (wid == 0) sees[lane] = ancestors(a.parents + b * a.parents_stride, a.nodes, lane);
     if (BIAS && bias_in_lds)
       for (int x = tid; x < n * a.buckets; x += 512) btab[x] = a.bias[(size_t)kvh * n * a.buckets + x];
-    const int first = BIAS && a.next_pos != nullptr ? a.next_pos[b] : len;
+    const int first_pos = BIAS && a.next_pos != nullptr ? a.next_pos[b] : len;
     // From here on the only vector memory operations are the stages' (but for a bias
     // with positions or too large for LDS, whose loads make waits longer, not shorter).
 #pragma unroll
     for (int s = 0; s < S - 1; ++s) issue(s);
 
-    f32x4_t o[NR][E];
+    f32x4_t o[NR][E];  // [t][e][r]: dimension 16 e + 4 g + r of row i of tile t
     float m[NR], l[NR];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
@@ -553,20 +600,25 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       const bool whole = base + kStepKeys <= end;
       u32x4_t kx[2][KC];
       read_k<M::kRow>(k_at, stage, kx);
-      uint4 kf[2][KC];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int c = 0; c < KC; ++c) kf[h][c] = __builtin_bit_cast(uint4, kx[h][c]);
-      float p[NR][8];
+      f32x4_t x[NR], y[NR];
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
-        const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
-        const float z[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        x[t] = {0.f, 0.f, 0.f, 0.f}, y[t] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[t][j] = z[j] * scale2;
+        for (int c = 0; c < KC; ++c) {
+          x[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[0][c]), q[t][c], x[t]);
+          y[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[1][c]), q[t][c], y[t]);
+        }
       }
+      u32x2_t vx[E][2];
+      read_v<M::kRow>(v_at, stage, vx);
+      float z[NR][8];
+#pragma unroll
+      for (int t = 0; t < NR; ++t)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) z[t][j] = x[t][j], z[t][4 + j] = y[t][j];
       if constexpr (BIAS) {
+        const int* pos = a.pos == nullptr ? nullptr : a.pos + (size_t)(b * a.kv_heads + kvh) * a.capacity;
         int kpos[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -576,61 +628,95 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
           const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
-          const int qp = (fresh ? 0 : first) + max(__popcll(sees[node]) - 1, 0);
+          const int qp = (fresh ? 0 : first_pos) + max(__popcll(sees[node]) - 1, 0);
           const float* row = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) p[t][j] = fmaf(row[min(max(qp - kpos[j], 0), a.buckets - 1)], kLog2e, p[t][j]);
+          for (int j = 0; j < 8; ++j)
+            z[t][j] = fmaf(z[t][j], scale2, row[min(max(qp - kpos[j], 0), a.buckets - 1)] * kLog2e);
         }
       }
-      if (fresh || !whole) {
+      const bool plain = !fresh && whole;
+      if (!plain) {
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
           const uint64_t see = fresh ? sees[min(row0 + t * 16 + i, R - 1) / n] >> base : ~0ull;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
-            p[t][j] = base + lane_key(g, j) < end && (see >> lane_key(g, j)) & 1 ? p[t][j] : -INFINITY;
+            z[t][j] = base + lane_key(g, j) < end && (see >> lane_key(g, j)) & 1 ? z[t][j] : -INFINITY;
         }
       }
-      typename std::conditional<VW == 4, u32x4_t, u32x2_t>::type vx[8];
-      read_v<M::kRow>(v_at + stage, vx);
-      uint32_t vf[8][VW];
+      uint4 ph[NR], pl[NR];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+      for (int t = 0; t < NR; ++t) {
+        const float top = max_over_groups(fmaxf(fmaxf(fmaxf(z[t][0], z[t][1]), fmaxf(z[t][2], z[t][3])),
+                                                fmaxf(fmaxf(z[t][4], z[t][5]), fmaxf(z[t][6], z[t][7])))) *
+                              mult -
+                          kShift;
+        if (__any(top > m[t])) {
+          const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
+          m[t] = mn;
+          l[t] *= f;
 #pragma unroll
-        for (int w = 0; w < VW; ++w) vf[j][w] = vx[j][w];
-      running_softmax<NR, E>(p, m, l, o, kShift);
-      if (!fresh && whole) {
-        F::template add_pv<NR>(vf, p, o);
-        continue;
+          for (int e = 0; e < E; ++e) o[t][e] *= f;
+        }
+        float p[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[j] = __builtin_amdgcn_exp2f(fmaf(z[t][j], mult, -m[t]));
+        l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+        F::split(p, ph[t], pl[t]);
       }
-      // Rows past the end are zeros; nodes' infinities and NaN go by class (as above).
       uint32_t diff = 0;
+      if (!plain) {
+        // Rows past the end are zeros; a node's infinities and NaN belong to those who see
+        // it and go by class (as above).
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+        for (int h = 0; h < 2; ++h) {
+          const int key = base + 16 * h + 4 * g;
+          const uint32_t in[2] = {(key < end ? 0xffffu : 0u) | (key + 1 < end ? 0xffff0000u : 0u),
+                                  (key + 2 < end ? 0xffffu : 0u) | (key + 3 < end ? 0xffff0000u : 0u)};
 #pragma unroll
-        for (int w = 0; w < VW; ++w) {
-          const uint32_t v = base + lane_key(g, j) < end ? vf[j][w] : 0u, x = fresh ? F::finite_part(v) : v;
-          diff |= x ^ v;
-          vf[j][w] = x;
+          for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const uint32_t v = vx[e][h][w] & in[w], u = fresh ? F::finite_part(v) : v;
+              diff |= u ^ v;
+              vx[e][h][w] = u;
+            }
         }
-      F::template add_pv<NR>(vf, p, o);
-      if (__any(diff != 0)) {
-        read_v<M::kRow>(v_at + stage, vx);
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+      for (int e0 = 0; e0 < E; e0 += 4) {
 #pragma unroll
-          for (int w = 0; w < VW; ++w) vf[j][w] = base + lane_key(g, j) < end ? F::classes(vx[j][w]) : 0u;
+        for (int part = 0; part < 2; ++part)
+#pragma unroll
+          for (int e = e0; e < e0 + 4; ++e)
+#pragma unroll
+            for (int t = 0; t < NR; ++t)
+              o[t][e] = Mma<T>::mma(make_uint4(vx[e][0].x, vx[e][0].y, vx[e][1].x, vx[e][1].y), part == 0 ? ph[t] : pl[t],
+                                    o[t][e]);
+      }
+      if (!plain && __any(diff != 0)) {
+        read_v<M::kRow>(v_at, stage, vx);
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
           const uint64_t see = sees[min(row0 + t * 16 + i, R - 1) / n] >> base;
-          float one[8];
+          uint32_t one[4];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) one[j] = (see >> lane_key(g, j)) & 1 ? 1.f : 0.f;
+          for (int j = 0; j < 4; ++j)
+            one[j] = Mma<T>::pack((see >> lane_key(g, 2 * j)) & 1 ? 1.f : 0.f, (see >> lane_key(g, 2 * j + 1)) & 1 ? 1.f : 0.f);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            const f32x4_t c = F::count(vf, one, e);
+            uint32_t c[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(c[r]);
+            for (int w = 0; w < 4; ++w) {
+              const int key = base + 16 * (w >> 1) + 4 * g + 2 * (w & 1);
+              const uint32_t in = (key < end ? 0xffffu : 0u) | (key + 1 < end ? 0xffff0000u : 0u);
+              c[w] = F::classes(vx[e][w >> 1][w & 1]) & in;
+            }
+            const f32x4_t sum = Mma<T>::mma(make_uint4(c[0], c[1], c[2], c[3]), make_uint4(one[0], one[1], one[2], one[3]),
+                                            f32x4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(sum[r]);
           }
         }
       }
@@ -648,11 +734,9 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         if (row >= R) continue;
         const bool there = sees[row / n] != 0;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          float v[E];
-#pragma unroll
-          for (int e = 0; e < E; ++e) v[e] = o[t][e][r];
-          emit<T, E>(a, all, slot, b, kvh, row, (4 * g + r) * E, v, m[t], l[t], there);
+        for (int e = 0; e < E; ++e) {
+          const float v[4] = {o[t][e][0], o[t][e][1], o[t][e][2], o[t][e][3]};
+          emit<T, 4>(a, all, slot, b, kvh, row, 16 * e + 4 * g, v, m[t], l[t], there);
         }
       }
     } else {
@@ -681,18 +765,13 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         for (int w = 1; w < WK; ++w) top = fmaxf(top, ml[w][x].x);
 #pragma unroll
         for (int w = 0; w < WK; ++w) sum = fmaf(ml[w][x].y, __builtin_amdgcn_exp2f(ml[w][x].x - top), sum);
+        const bool there = sees[row / n] != 0;
+        for (int e = wk; e < E; e += WK) {
+          f32x4_t u = buf[((wr * NR + t) * E + e) * 64 + lane];
 #pragma unroll
-        for (int r0 = 0; r0 < 4; r0 += WK) {
-          const int r = r0 + wk;
-          float v[E];
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            v[e] = 0.f;
-#pragma unroll
-            for (int w = 0; w < WK; ++w)
-              v[e] += reinterpret_cast<const float*>(&buf[(((w * WR + wr) * NR + t) * E + e) * 64 + lane])[r];
-          }
-          emit<T, E>(a, all, slot, b, kvh, row, (4 * g + r) * E, v, top, sum, sees[row / n] != 0);
+          for (int w = 1; w < WK; ++w) u += buf[(((w * WR + wr) * NR + t) * E + e) * 64 + lane];
+          const float v[4] = {u[0], u[1], u[2], u[3]};
+          emit<T, 4>(a, all, slot, b, kvh, row, 16 * e + 4 * g, v, top, sum, there);
         }
       }
     }
@@ -709,15 +788,17 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   }
 }
 
-// Sums the parts of one row, a wave a row: `cols` lanes share the dimensions, the others
-// further parts.
+// Sums the parts of the rows of units that were cut, kJoinRows rows a wave: `cols` lanes
+// share the dimensions, the others further parts.
+constexpr int kJoinRows = 4;
+
 template <typename T>
 __global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, bool many, int cols) {
   const int lane = threadIdx.x & 63, n = a.heads / a.kv_heads, R = a.nodes * n;
-  const int blocks = (R + 3) / 4, unit = blockIdx.x / blocks;
-  const int r = (blockIdx.x - unit * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (r >= R) return;
-  const int b = unit / a.kv_heads, kvh = unit - b * a.kv_heads, node = r / n, h = kvh * n + r - node * n;
+  const int blocks = (R + 4 * kJoinRows - 1) / (4 * kJoinRows), unit = blockIdx.x / blocks;
+  const int r0 = ((blockIdx.x - unit * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kJoinRows;
+  if (r0 >= R) return;
+  const int b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
   const Share sh = share_of(a, lane);
   int64_t first = 0;
   int parts = 0;
@@ -735,47 +816,54 @@ __global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, bool many, 
     first = unit + t0;
   }
   if (parts == 1) return;  // written by its block
-  const float2* ml = a.part_ml + first * R + r;
-  const float* part = a.part + (first * R + r) * a.D;
+  const uint64_t present = a.present[b];
   const int d = lane % cols * 4, from = lane / cols, every = 64 / cols;
-  float top = kNone, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < parts; s0 += 64) {
-    const float2 x = s0 + lane < parts ? ml[(size_t)(s0 + lane) * R] : make_float2(kNone, 0.f);
-    const float to = fmaxf(top, wave_max(x.x)), f = __builtin_amdgcn_exp2f(top - to);
-    top = to;
-    const float w = s0 + lane < parts ? __builtin_amdgcn_exp2f(x.x - top) : 0.f;
-    sum = fmaf(sum, f, wave_sum(x.y * w));
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= f;
-    const int end = min(64, parts - s0);
-    for (int s = from; s < ((end + every - 1) / every) * every; s += every) {
-      const float ws = __shfl(w, s, 64);
-      if (s < end && d < a.D) {
-        const float4 y = *reinterpret_cast<const float4*>(part + (size_t)(s0 + s) * R * a.D + d);
-        v[0] = fmaf(y.x, ws, v[0]), v[1] = fmaf(y.y, ws, v[1]), v[2] = fmaf(y.z, ws, v[2]), v[3] = fmaf(y.w, ws, v[3]);
+  for (int x = 0; x < kJoinRows; ++x) {
+    const int r = r0 + x;
+    if (r >= R) break;
+    const float2* ml = a.part_ml + first * R + r;
+    const float* part = a.part + (first * R + r) * a.D;
+    float top = kNone, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s0 = 0; s0 < parts; s0 += 64) {
+      const float2 y = s0 + lane < parts ? ml[(size_t)(s0 + lane) * R] : make_float2(kNone, 0.f);
+      const float to = fmaxf(top, wave_max(y.x)), f = __builtin_amdgcn_exp2f(top - to);
+      top = to;
+      const float w = s0 + lane < parts ? __builtin_amdgcn_exp2f(y.x - top) : 0.f;
+      sum = fmaf(sum, f, wave_sum(y.y * w));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] *= f;
+      const int end = min(64, parts - s0);
+      for (int s = from; s < ((end + every - 1) / every) * every; s += every) {
+        const float ws = __shfl(w, s, 64);
+        if (s < end && d < a.D) {
+          const float4 z = *reinterpret_cast<const float4*>(part + (size_t)(s0 + s) * R * a.D + d);
+          v[0] = fmaf(z.x, ws, v[0]), v[1] = fmaf(z.y, ws, v[1]), v[2] = fmaf(z.z, ws, v[2]), v[3] = fmaf(z.w, ws, v[3]);
+        }
       }
     }
-  }
-  for (int o = cols; o < 64; o <<= 1) {
+    for (int o = cols; o < 64; o <<= 1) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], o, 64);
-  }
-  const bool there = (a.present[b] >> node) & 1;
-  const float inv = 1.f / sum;
-  if (d < a.D && from == 0) {
-    T* dst = static_cast<T*>(a.out) + b * a.o_row + node * a.o_node + h * a.o_head + d;
-    union {
-      T x[4];
-      uint4 w4;
-      uint2 w2;
-    } u;
+      for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], o, 64);
+    }
+    const int node = r / n, h = kvh * n + r - node * n;
+    const bool there = (present >> node) & 1;
+    const float inv = 1.f / sum;
+    if (d < a.D && from == 0) {
+      T* dst = static_cast<T*>(a.out) + b * a.o_row + node * a.o_node + h * a.o_head + d;
+      union {
+        T x[4];
+        uint4 w4;
+        uint2 w2;
+      } u;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) u.x[e] = St<T>::st(there ? v[e] * inv : 0.f);
-    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = u.w4;
-    else *reinterpret_cast<uint2*>(dst) = u.w2;
+      for (int e = 0; e < 4; ++e) u.x[e] = St<T>::st(there ? v[e] * inv : 0.f);
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = u.w4;
+      else *reinterpret_cast<uint2*>(dst) = u.w2;
+    }
+    if (a.lse != nullptr && lane == 0)
+      a.lse[((size_t)b * a.nodes + node) * a.heads + h] = there ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
   }
-  if (a.lse != nullptr && lane == 0)
-    a.lse[((size_t)b * a.nodes + node) * a.heads + h] = there ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
 }
 
 // Row tiles that a wave of k_tree_few holds: the output takes dp / 4 registers a tile,
@@ -895,7 +983,7 @@ void tree_attention(const KvCache& c, const TreeAttnArgs& t, void* ws, hipStream
   }
   MRT_HIP_CHECK(hipGetLastError());
   if (p.teams > 0) {
-    const dim3 grid(c.rows * c.kv_heads * ((R + 3) / 4));
+    const dim3 grid(c.rows * c.kv_heads * ((R + 4 * kJoinRows - 1) / (4 * kJoinRows)));
     const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64;
     MRT_DTYPE_DISPATCH(c.dt, hipLaunchKernelGGL(k_tree_join<T>, grid, dim3(256), 0, s, a, p.many, cols));
     MRT_HIP_CHECK(hipGetLastError());
