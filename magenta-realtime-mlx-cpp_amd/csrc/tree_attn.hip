@@ -7,7 +7,7 @@
 //
 // Work: the n = heads / kv_heads query heads of a K/V head share its keys, so a K/V head
 // (a unit) has R = nodes n rows r = t n + hq; its keys are taken in steps of 32, the
-// drafted nodes the last ones.  Two kernels:
+// drafted nodes the first ones.  Two kernels:
 //   k_tree_few (up to 16 rows, fp32, odd head sizes): the four waves of a block take
 //   steps in turn, straight from memory to registers, each with its own maximum, sum and
 //   output; joined through LDS at the end.  What such rows cost is reading the keys.
@@ -43,7 +43,8 @@ struct TreeArgs {
   int64_t q_row, q_node, q_head, kn_row, kn_node, kn_head, vn_row, vn_node, vn_head, o_row, o_node, o_head;
   int64_t c_row, c_head, c_slot, parents_stride;
   int rows, capacity, kv_heads, heads, nodes, D, buckets;
-  int teams;       // parts of the whole work wanted; 0: a unit is never cut
+  int teams;       // parts of the whole work wanted, cut by all lengths; 0: each unit by itself,
+  int splits;      //   into at most this many
   int least;       // steps that a part has at least
   int row_blocks;
   float scale;
@@ -52,6 +53,13 @@ struct TreeArgs {
 __device__ __forceinline__ int steps_of(const TreeArgs& a, int b) {
   const int len = min(max(a.length[b], 0), a.capacity);
   return (len + kStepKeys - 1) / kStepKeys + (a.nodes + kStepKeys - 1) / kStepKeys;
+}
+
+// Work too small to be shared evenly: parts of a unit have max(least, ceil(steps /
+// splits)) steps, part x of unit u leaves its result in slot u splits + x.  No block
+// needs another sequence's length.
+__device__ __forceinline__ int own_chunk(const TreeArgs& a, int steps) {
+  return max(a.least, (steps + a.splits - 1) / a.splits);
 }
 
 // How the steps of all units (b, K/V head), in order, are cut into parts.  Long work
@@ -176,10 +184,12 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, D = a.D;
   const int id = blockIdx.x / a.row_blocks, row0 = (blockIdx.x - id * a.row_blocks) * (16 * NR);
+  const int new_steps = (a.nodes + kStepKeys - 1) / kStepKeys;
   int b, kvh, s0, s1, steps;
   if (a.teams == 0) {
-    b = id / a.kv_heads, kvh = id - b * a.kv_heads;
-    s0 = 0, s1 = steps = steps_of(a, b);
+    const int unit = id / a.splits;
+    b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
+    s0 = 0;
   } else {
     const Share sh = share_of(a, lane);
     const int chunk = sh.chunk > 0 ? sh.chunk : (int)((sh.total + a.teams - 1) / a.teams);
@@ -192,8 +202,37 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
     steps = steps_of(a, b);
     s0 = (at - kvh * n) * chunk, s1 = min(steps, s0 + chunk);
   }
+  if (a.teams == 0 && a.splits > 1) {
+    const int part = id - (b * a.kv_heads + kvh) * a.splits;
+    steps = steps_of(a, b);
+    const int chunk = own_chunk(a, steps);
+    s0 = part * chunk, s1 = min(steps, s0 + chunk);
+    if (s0 >= steps) return;
+  }
   const int n = a.heads / a.kv_heads, R = a.nodes * n;
+  const T* kc = static_cast<const T*>(a.k) + b * a.c_row + kvh * a.c_head;
+  const T* vc = static_cast<const T*>(a.v) + b * a.c_row + kvh * a.c_head;
+
+  // Keys and values of a step.  Nothing here needs the length (rows past it are masked,
+  // those past the capacity are read from its last slot), so a wave's first step is
+  // requested before anything else.
+  uint4 kf[2][KC];
+  uint32_t vf[8][VW];
+  auto load = [&](int st) {
+    const bool fresh = st < new_steps;  // drafted nodes
+    const int base = (fresh ? st : st - new_steps) * kStepKeys, last = (fresh ? a.nodes : a.capacity) - 1;
+    const T* kb = fresh ? static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head : kc;
+    const T* vb = fresh ? static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head : vc;
+    const int64_t kstep = fresh ? a.kn_node : a.c_slot, vstep = fresh ? a.vn_node : a.c_slot;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) F::load_row(kb + (int64_t)min(base + step_key(i, h), last) * kstep, g, D, kf[h]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) F::load_v(vb + (int64_t)min(base + lane_key(g, j), last) * vstep, i, D, vf[j]);
+  };
+  load(s0 + wid);
+
   const int len = min(max(a.length[b], 0), a.capacity), old_steps = (len + kStepKeys - 1) / kStepKeys;
+  if (a.teams == 0 && a.splits == 1) s1 = steps = new_steps + old_steps;
   const bool all = s0 == 0 && s1 == steps;
 
   extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -212,10 +251,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
   if (wid == 0) sees[lane] = ancestors(a.parents + b * a.parents_stride, a.nodes, lane);
   if (a.bias != nullptr && bias_in_lds)
     for (int x = tid; x < n * a.buckets; x += 64 * kWaves) btab[x] = a.bias[(size_t)kvh * n * a.buckets + x];
-  __syncthreads();
+  ring_barrier();  // does not wait for the loads of the first step
 
-  const T* kc = static_cast<const T*>(a.k) + b * a.c_row + kvh * a.c_head;
-  const T* vc = static_cast<const T*>(a.v) + b * a.c_row + kvh * a.c_head;
   const int* pos = a.pos == nullptr ? nullptr : a.pos + (size_t)(b * a.kv_heads + kvh) * a.capacity;
   int qpos[NR];
   const float* brow[NR];
@@ -242,19 +279,9 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
   constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;
 
   for (int st = s0 + wid; st < s1; st += kWaves) {
-    const bool fresh = st >= old_steps;  // drafted nodes
-    const int base = (fresh ? st - old_steps : st) * kStepKeys, end = fresh ? a.nodes : len;
-    const T* kb = fresh ? static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head : kc;
-    const T* vb = fresh ? static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head : vc;
-    const int64_t kstep = fresh ? a.kn_node : a.c_slot, vstep = fresh ? a.vn_node : a.c_slot;
+    const bool fresh = st < new_steps;
+    const int base = (fresh ? st : st - new_steps) * kStepKeys, end = fresh ? a.nodes : len;
     const bool whole = base + kStepKeys <= end;
-    uint4 kf[2][KC];
-    uint32_t vf[8][VW];
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      F::load_row(kb + (int64_t)min(base + step_key(i, h), end - 1) * kstep, g, D, kf[h]);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) F::load_v(vb + (int64_t)min(base + lane_key(g, j), end - 1) * vstep, i, D, vf[j]);
     if (!whole) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -313,7 +340,8 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = base + lane_key(g, j);
-          F::load_v(vb + (int64_t)min(key, end - 1) * vstep, i, D, vf[j]);
+          F::load_v(static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head + (int64_t)min(key, end - 1) * a.vn_node, i,
+                    D, vf[j]);
 #pragma unroll
           for (int w = 0; w < VW; ++w) vf[j][w] = key < end ? F::classes(vf[j][w]) : 0u;
         }
@@ -332,6 +360,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
         }
       }
     }
+    if (st + kWaves < s1) load(st + kWaves);
   }
 
   // Join the waves: outputs at the common maximum, summed through LDS.
@@ -372,7 +401,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
     }
     emit<T, E>(a, all, slot, b, kvh, r, d, v, top, sum, sees[r / n] != 0);
   }
-  if (!all && s1 == steps && row0 == 0 && wid == 0) {  // the same from every K/V head
+  if (!all && s0 == 0 && row0 == 0 && wid == 0) {  // the same from every K/V head
     const uint64_t there = __ballot(sees[lane] != 0);
     if (lane == 0) a.present[b] = there;
   }
@@ -390,27 +419,16 @@ struct Many {
   static constexpr size_t kRing = (size_t)S * kStage, kJoin = WK > 1 ? (size_t)kWaves * NR * (DP / 16) * 1024 : 0;
   static constexpr size_t kLds = kRing > kJoin ? kRing : kJoin;
   // 16-byte piece p of row r lies at place p ^ swz(r), so that what is read together falls
-  // in distinct banks: of K the same piece of 16 keys, of V 32 bytes of 4 keys.
+  // in distinct banks: of K the same piece of 16 keys, of V 32 bytes of 8 keys.
   __device__ static int swz_k(int r) { return DP == 128 ? r & 15 : (r >> 1) & 7; }
-  __device__ static int swz_v(int r) { return DP == 128 ? (r & 3) * 2 : ((r >> 1) & 1) * 2; }
+  __device__ static int swz_v(int r) { return DP == 128 ? (r & 7) * 2 : ((r >> 1) & 3) * 2; }
 };
 
 // Fragments of one step from LDS.  Written out, since the compiler waits for every load
 // into LDS that is in flight before any read of LDS, which would empty the ring; each
-// block waits for its own reads.  K: rows i and i + 16 at one address per column chunk.
+// block waits for its own reads.  K: rows i and i + 16 of two column chunks.
 template <int ROW>
-__device__ __forceinline__ void read_k(const uint32_t (&at)[4], uint32_t base, u32x4_t (&f)[2][4]) {
-  asm volatile(
-      "ds_read_b128 %0, %8\n\tds_read_b128 %1, %8 offset:%12\n\tds_read_b128 %2, %9\n\tds_read_b128 %3, %9 offset:%12\n\t"
-      "ds_read_b128 %4, %10\n\tds_read_b128 %5, %10 offset:%12\n\tds_read_b128 %6, %11\n\t"
-      "ds_read_b128 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0][0]), "=&v"(f[1][0]), "=&v"(f[0][1]), "=&v"(f[1][1]), "=&v"(f[0][2]), "=&v"(f[1][2]), "=&v"(f[0][3]),
-        "=&v"(f[1][3])
-      : "v"(at[0] + base), "v"(at[1] + base), "v"(at[2] + base), "v"(at[3] + base), "n"(16 * ROW)
-      : "memory");
-}
-template <int ROW>
-__device__ __forceinline__ void read_k(const uint32_t (&at)[2], uint32_t base, u32x4_t (&f)[2][2]) {
+__device__ __forceinline__ void read_k(const uint32_t* at, uint32_t base, u32x4_t (&f)[2][2]) {
   asm volatile(
       "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %5\n\tds_read_b128 %3, %5 offset:%6\n\t"
       "s_waitcnt lgkmcnt(0)"
@@ -420,10 +438,10 @@ __device__ __forceinline__ void read_k(const uint32_t (&at)[2], uint32_t base, u
 }
 // V, transposed as it is read: of 16 lanes, lane 4 r + c gives the address of columns 4 c ..
 // 4 c + 3 of row r, and lane i receives column i of rows 0..3.  f[e][h]: keys 16 h + 4 g ..
-// + 3 of dimension 16 e + i.  Tiles e and e + 4 share an address (128 bytes apart).
+// + 3 of dimension 16 e + i, for four e.
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 template <int ROW>
-__device__ __forceinline__ void read_v(const uint32_t (&at)[4], uint32_t base, u32x2_t (&f)[4][2]) {
+__device__ __forceinline__ void read_v(const uint32_t* at, uint32_t base, u32x2_t (&f)[4][2]) {
   asm volatile(
       "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %9\n\t"
       "ds_read_b64_tr_b16 %3, %9 offset:%12\n\tds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
@@ -433,23 +451,6 @@ __device__ __forceinline__ void read_v(const uint32_t (&at)[4], uint32_t base, u
       : "v"(at[0] + base), "v"(at[1] + base), "v"(at[2] + base), "v"(at[3] + base), "n"(16 * ROW)
       : "memory");
 }
-template <int ROW>
-__device__ __forceinline__ void read_v(const uint32_t (&at)[4], uint32_t base, u32x2_t (&f)[8][2]) {
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %16\n\tds_read_b64_tr_b16 %1, %16 offset:%20\n\tds_read_b64_tr_b16 %2, %17\n\t"
-      "ds_read_b64_tr_b16 %3, %17 offset:%20\n\tds_read_b64_tr_b16 %4, %18\n\tds_read_b64_tr_b16 %5, %18 offset:%20\n\t"
-      "ds_read_b64_tr_b16 %6, %19\n\tds_read_b64_tr_b16 %7, %19 offset:%20\n\tds_read_b64_tr_b16 %8, %16 offset:128\n\t"
-      "ds_read_b64_tr_b16 %9, %16 offset:%21\n\tds_read_b64_tr_b16 %10, %17 offset:128\n\t"
-      "ds_read_b64_tr_b16 %11, %17 offset:%21\n\tds_read_b64_tr_b16 %12, %18 offset:128\n\t"
-      "ds_read_b64_tr_b16 %13, %18 offset:%21\n\tds_read_b64_tr_b16 %14, %19 offset:128\n\t"
-      "ds_read_b64_tr_b16 %15, %19 offset:%21\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1]), "=&v"(f[2][0]), "=&v"(f[2][1]), "=&v"(f[3][0]),
-        "=&v"(f[3][1]), "=&v"(f[4][0]), "=&v"(f[4][1]), "=&v"(f[5][0]), "=&v"(f[5][1]), "=&v"(f[6][0]), "=&v"(f[6][1]),
-        "=&v"(f[7][0]), "=&v"(f[7][1])
-      : "v"(at[0] + base), "v"(at[1] + base), "v"(at[2] + base), "v"(at[3] + base), "n"(16 * ROW), "n"(16 * ROW + 128)
-      : "memory");
-}
-
 template <typename T, int DP, int WR, int NR, bool BIAS>
 __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   using F = AttnFrag<T, DP>;
@@ -472,11 +473,11 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   __shared__ float2 ml[WK][16 * NR * WR];
   float* btab = reinterpret_cast<float*>(lds + M::kLds);
   const uint32_t ring = (uint32_t)(uintptr_t)(MRT_LDS char*)lds;  // LDS address of the ring
-  uint32_t k_at[KC], v_at[4];  // in a stage: this lane's key row and chunk; V row and columns
+  uint32_t k_at[KC], v_at[E];  // in a stage: this lane's key row and chunk; V row and columns
 #pragma unroll
   for (int c = 0; c < KC; ++c) k_at[c] = (wk * 32 + i) * M::kRow + ((c * 4 + g) ^ M::swz_k(i)) * 16;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
+  for (int e = 0; e < E; ++e) {
     const int row = 4 * g + (i >> 2), piece = 2 * e + ((i >> 1) & 1);
     v_at[e] = (M::kKeys + wk * 32 + row) * M::kRow + (piece ^ M::swz_v(row)) * 16 + (i & 1) * 8;
   }
@@ -497,9 +498,11 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   int64_t at, stop, unit_at;
   Share sh{0, 0};
   if (a.teams == 0) {
-    if (team >= (int64_t)a.rows * a.kv_heads) return;
-    b = (int)(team / a.kv_heads), kvh = (int)(team - (int64_t)b * a.kv_heads);
-    at = unit_at = 0, stop = steps_of(a, b);
+    const int unit = (int)team / a.splits, part = (int)team - unit * a.splits;
+    if (unit >= a.rows * a.kv_heads) return;
+    b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
+    const int steps = steps_of(a, b), chunk = a.splits > 1 ? own_chunk(a, steps) : steps;
+    unit_at = 0, at = (int64_t)part * chunk, stop = min((int64_t)steps, at + chunk);
   } else {
     sh = share_of(a, lane);
     int64_t before = 0;
@@ -523,41 +526,47 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
 
   while (at < stop) {
     const int len = uniform(min(max(a.length[b], 0), a.capacity)), old_steps = (len + kStepKeys - 1) / kStepKeys;
-    const int steps = old_steps + (a.nodes + kStepKeys - 1) / kStepKeys;
+    const int new_steps = (a.nodes + kStepKeys - 1) / kStepKeys, steps = new_steps + old_steps;
     const int s0 = (int)(at - unit_at), s1 = (int)min((int64_t)steps, stop - unit_at);
     const bool all = s0 == 0 && s1 == steps;
     const T* kc = static_cast<const T*>(a.k) + b * a.c_row + kvh * a.c_head;
     const T* vc = static_cast<const T*>(a.v) + b * a.c_row + kvh * a.c_head;
     const int stages = (s1 - s0 + WK - 1) / WK;
 
-    // Requests stage s (past the end: its last step again): K rows, then V rows.
-    auto issue = [&](int s) {
-      char* to = lds + (s % S) * M::kStage;
-      const int first = s0 + s * WK;
-      if (near && first + WK <= s1 && (first + WK) * kStepKeys <= len) {
-        const char* kb = reinterpret_cast<const char*>(kc + (int64_t)first * kStepKeys * a.c_slot);
-        const char* vb = reinterpret_cast<const char*>(vc + (int64_t)first * kStepKeys * a.c_slot);
+    // Requests the next stage (past the end: the last step again): K rows, then V rows.
+    const int64_t stride = (int64_t)M::kKeys * a.c_slot * 2;  // bytes of a stage's keys
+    const char* kb = reinterpret_cast<const char*>(kc + (int64_t)(s0 - new_steps) * kStepKeys * a.c_slot);
+    const char* vb = reinterpret_cast<const char*>(vc + (int64_t)(s0 - new_steps) * kStepKeys * a.c_slot);
+    int ahead = s0, to_slot = 0;
+    const int plain_to = near ? min(s1, new_steps + len / kStepKeys) : 0;  // whole cached steps end here
+    auto issue = [&] {
+      char* to = lds + to_slot * M::kStage;
+      to_slot = to_slot + 1 == S ? 0 : to_slot + 1;
+      const int first = ahead;
+      ahead += WK;
+      if (first >= new_steps && ahead <= plain_to) {
 #pragma unroll
         for (int x = 0; x < M::kLoads; ++x) {
           const int t = x * M::kWaves + wid;
           const char* from = (x < M::kLoads / 2 || (M::kLoads == 1 && wid < M::kWaves / 2) ? kb : vb) + src[x];
           __builtin_amdgcn_global_load_lds((const MRT_GLOBAL void*)from, (MRT_LDS void*)(to + t * 1024), 16, 0, 0);
         }
-        return;
-      }
-      const T* kn = static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head;
-      const T* vn = static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
+      } else {
+        const T* kn = static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head;
+        const T* vn = static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
 #pragma unroll
-      for (int x = 0; x < M::kLoads; ++x) {
-        const int t = x * M::kWaves + wid, half = M::kLoads * M::kWaves / 2, u = t < half ? t : t - half;
-        const int row = u * M::kRowsLoad + lane / M::kPieces, place = lane % M::kPieces;
-        const int st = min(first + u * M::kRowsLoad / 32, s1 - 1);
-        const bool fresh = st >= old_steps;
-        const int key = min((fresh ? st - old_steps : st) * kStepKeys + (row & 31), (fresh ? a.nodes : len) - 1);
-        const T* from = t < half ? (fresh ? kn + key * a.kn_node : kc + key * a.c_slot) + (place ^ M::swz_k(row & 31)) * 8
-                                 : (fresh ? vn + key * a.vn_node : vc + key * a.c_slot) + (place ^ M::swz_v(row)) * 8;
-        __builtin_amdgcn_global_load_lds((const MRT_GLOBAL void*)from, (MRT_LDS void*)(to + t * 1024), 16, 0, 0);
+        for (int x = 0; x < M::kLoads; ++x) {
+          const int t = x * M::kWaves + wid, half = M::kLoads * M::kWaves / 2, u = t < half ? t : t - half;
+          const int row = u * M::kRowsLoad + lane / M::kPieces, place = lane % M::kPieces;
+          const int st = min(first + u * M::kRowsLoad / 32, s1 - 1);
+          const bool fresh = st < new_steps;
+          const int key = min((fresh ? st : st - new_steps) * kStepKeys + (row & 31), (fresh ? a.nodes : len) - 1);
+          const T* from = t < half ? (fresh ? kn + key * a.kn_node : kc + key * a.c_slot) + (place ^ M::swz_k(row & 31)) * 8
+                                   : (fresh ? vn + key * a.vn_node : vc + key * a.c_slot) + (place ^ M::swz_v(row)) * 8;
+          __builtin_amdgcn_global_load_lds((const MRT_GLOBAL void*)from, (MRT_LDS void*)(to + t * 1024), 16, 0, 0);
+        }
       }
+      kb += stride, vb += stride;
     };
     uint4 q[NR][KC];
 #pragma unroll
@@ -577,7 +586,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
     // From here on the only vector memory operations are the stages' (but for a bias
     // with positions or too large for LDS, whose loads make waits longer, not shorter).
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) issue(s);
+    for (int s = 0; s < S - 1; ++s) issue();
 
     f32x4_t o[NR][E];  // [t][e][r]: dimension 16 e + 4 g + r of row i of tile t
     float m[NR], l[NR];
@@ -588,30 +597,33 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
     }
 
+    int slot_now = 0;
     for (int s = 0; s < stages; ++s) {
       __builtin_amdgcn_s_waitcnt(vm_wait_imm((S - 2) * M::kLoads));  // this wave's part of stage s is in LDS
       ring_barrier();                                                // everyone's is, and stage s - 1 has been read
-      issue(s + S - 1);
+      issue();
+      const uint32_t stage = ring + slot_now * M::kStage;
+      slot_now = slot_now + 1 == S ? 0 : slot_now + 1;
       const int st = s0 + s * WK + wk;
       if (st >= s1 || row0 >= R) continue;
-      const uint32_t stage = ring + (s % S) * M::kStage;
-      const bool fresh = st >= old_steps;
-      const int base = (fresh ? st - old_steps : st) * kStepKeys, end = fresh ? a.nodes : len;
+      const bool fresh = st < new_steps;
+      const int base = (fresh ? st : st - new_steps) * kStepKeys, end = fresh ? a.nodes : len;
       const bool whole = base + kStepKeys <= end;
-      u32x4_t kx[2][KC];
-      read_k<M::kRow>(k_at, stage, kx);
       f32x4_t x[NR], y[NR];
 #pragma unroll
-      for (int t = 0; t < NR; ++t) {
-        x[t] = {0.f, 0.f, 0.f, 0.f}, y[t] = {0.f, 0.f, 0.f, 0.f};
+      for (int t = 0; t < NR; ++t) x[t] = {0.f, 0.f, 0.f, 0.f}, y[t] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          x[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[0][c]), q[t][c], x[t]);
-          y[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[1][c]), q[t][c], y[t]);
-        }
+      for (int c0 = 0; c0 < KC; c0 += 2) {
+        u32x4_t kx[2][2];
+        read_k<M::kRow>(k_at + c0, stage, kx);
+#pragma unroll
+        for (int c = 0; c < 2; ++c)
+#pragma unroll
+          for (int t = 0; t < NR; ++t) {
+            x[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[0][c]), q[t][c0 + c], x[t]);
+            y[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[1][c]), q[t][c0 + c], y[t]);
+          }
       }
-      u32x2_t vx[E][2];
-      read_v<M::kRow>(v_at, stage, vx);
       float z[NR][8];
 #pragma unroll
       for (int t = 0; t < NR; ++t)
@@ -665,38 +677,43 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         F::split(p, ph[t], pl[t]);
       }
-      uint32_t diff = 0;
-      if (!plain) {
-        // Rows past the end are zeros; a node's infinities and NaN belong to those who see
-        // it and go by class (as above).
+      // Rows past the end are zeros; a node's infinities and NaN belong to those who see it
+      // and go by class (as above).
+      uint32_t in[2][2], diff = 0;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int key = base + 16 * h + 4 * g;
-          const uint32_t in[2] = {(key < end ? 0xffffu : 0u) | (key + 1 < end ? 0xffff0000u : 0u),
-                                  (key + 2 < end ? 0xffffu : 0u) | (key + 3 < end ? 0xffff0000u : 0u)};
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {
-              const uint32_t v = vx[e][h][w] & in[w], u = fresh ? F::finite_part(v) : v;
-              diff |= u ^ v;
-              vx[e][h][w] = u;
-            }
-        }
+      for (int h = 0; h < 2; ++h) {
+        const int key = base + 16 * h + 4 * g;
+        in[h][0] = (key < end ? 0xffffu : 0u) | (key + 1 < end ? 0xffff0000u : 0u);
+        in[h][1] = (key + 2 < end ? 0xffffu : 0u) | (key + 3 < end ? 0xffff0000u : 0u);
       }
 #pragma unroll
       for (int e0 = 0; e0 < E; e0 += 4) {
+        u32x2_t vx[4][2];
+        read_v<M::kRow>(v_at + e0, stage, vx);
+        if (!plain) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int w = 0; w < 2; ++w) {
+                const uint32_t v = vx[e][h][w] & in[h][w], u = fresh ? F::finite_part(v) : v;
+                diff |= u ^ v;
+                vx[e][h][w] = u;
+              }
+        }
 #pragma unroll
         for (int part = 0; part < 2; ++part)
 #pragma unroll
-          for (int e = e0; e < e0 + 4; ++e)
+          for (int e = 0; e < 4; ++e)
 #pragma unroll
             for (int t = 0; t < NR; ++t)
-              o[t][e] = Mma<T>::mma(make_uint4(vx[e][0].x, vx[e][0].y, vx[e][1].x, vx[e][1].y), part == 0 ? ph[t] : pl[t],
-                                    o[t][e]);
+              o[t][e0 + e] = Mma<T>::mma(make_uint4(vx[e][0].x, vx[e][0].y, vx[e][1].x, vx[e][1].y), part == 0 ? ph[t] : pl[t],
+                                         o[t][e0 + e]);
       }
       if (!plain && __any(diff != 0)) {
-        read_v<M::kRow>(v_at, stage, vx);
+        // rare, so from memory
+        const uint16_t* vn = static_cast<const uint16_t*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
           const uint64_t see = sees[min(row0 + t * 16 + i, R - 1) / n] >> base;
@@ -704,25 +721,28 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             one[j] = Mma<T>::pack((see >> lane_key(g, 2 * j)) & 1 ? 1.f : 0.f, (see >> lane_key(g, 2 * j + 1)) & 1 ? 1.f : 0.f);
-#pragma unroll
           for (int e = 0; e < E; ++e) {
             uint32_t c[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
               const int key = base + 16 * (w >> 1) + 4 * g + 2 * (w & 1);
-              const uint32_t in = (key < end ? 0xffffu : 0u) | (key + 1 < end ? 0xffff0000u : 0u);
-              c[w] = F::classes(vx[e][w >> 1][w & 1]) & in;
+              c[w] = (key < end ? ld_g(vn + key * a.vn_node + 16 * e + i) : 0u) |
+                     (key + 1 < end ? (uint32_t)ld_g(vn + (key + 1) * a.vn_node + 16 * e + i) << 16 : 0u);
+              c[w] = F::classes(c[w]);
             }
             const f32x4_t sum = Mma<T>::mma(make_uint4(c[0], c[1], c[2], c[3]), make_uint4(one[0], one[1], one[2], one[3]),
                                             f32x4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(sum[r]);
+            for (int u = 0; u < E; ++u)
+              if (u == e)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) o[t][u][r] += F::class_value(sum[r]);
           }
         }
       }
     }
 
-    const int64_t slot = sh.chunk > 0 ? team : (int64_t)b * a.kv_heads + kvh + team;
+    const int64_t slot = sh.chunk > 0 || a.teams == 0 ? team : (int64_t)b * a.kv_heads + kvh + team;
     // every load into LDS has landed and every stage been read
     __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));
 #pragma unroll
@@ -775,7 +795,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         }
       }
     }
-    if (!all && s1 == steps && rb == 0 && wid == 0) {  // the same from every K/V head
+    if (!all && s0 == 0 && rb == 0 && wid == 0) {  // the same from every K/V head
       const uint64_t there = __ballot(sees[lane] != 0);
       if (lane == 0) a.present[b] = there;
     }
@@ -788,32 +808,37 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   }
 }
 
-// Sums the parts of the rows of units that were cut, kJoinRows rows a wave: `cols` lanes
+// Sums the parts of the rows of units that were cut, kJoinRows rows a wave (one where
+// there are few: then the latency of a row counts): `cols` lanes
 // share the dimensions, the others further parts.
-constexpr int kJoinRows = 4;
-
-template <typename T>
+template <typename T, int kJoinRows>
 __global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, bool many, int cols) {
   const int lane = threadIdx.x & 63, n = a.heads / a.kv_heads, R = a.nodes * n;
   const int blocks = (R + 4 * kJoinRows - 1) / (4 * kJoinRows), unit = blockIdx.x / blocks;
   const int r0 = ((blockIdx.x - unit * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kJoinRows;
   if (r0 >= R) return;
   const int b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
-  const Share sh = share_of(a, lane);
   int64_t first = 0;
   int parts = 0;
   const int steps = steps_of(a, b);
-  const int chunk = sh.chunk > 0 ? sh.chunk : many ? 0 : (int)((sh.total + a.teams - 1) / a.teams);
-  int64_t before = 0;  // parts, or steps, of the sequences before
-  for (int x = lane; x < b; x += 64) before += chunk > 0 ? (steps_of(a, x) + chunk - 1) / chunk : steps_of(a, x);
-  before = wave_sum64(before) * a.kv_heads;
-  if (chunk > 0) {
+  if (a.teams == 0) {
+    const int chunk = own_chunk(a, steps);
     parts = (steps + chunk - 1) / chunk;
-    first = before + (int64_t)kvh * parts;
+    first = (int64_t)unit * a.splits;
   } else {
-    const int64_t at = before + (int64_t)kvh * steps, t0 = team_of(sh, a.teams, at);
-    parts = (int)(team_of(sh, a.teams, at + steps - 1) - t0) + 1;
-    first = unit + t0;
+    const Share sh = share_of(a, lane);
+    const int chunk = sh.chunk > 0 ? sh.chunk : many ? 0 : (int)((sh.total + a.teams - 1) / a.teams);
+    int64_t before = 0;  // parts, or steps, of the sequences before
+    for (int x = lane; x < b; x += 64) before += chunk > 0 ? (steps_of(a, x) + chunk - 1) / chunk : steps_of(a, x);
+    before = wave_sum64(before) * a.kv_heads;
+    if (chunk > 0) {
+      parts = (steps + chunk - 1) / chunk;
+      first = before + (int64_t)kvh * parts;
+    } else {
+      const int64_t at = before + (int64_t)kvh * steps, t0 = team_of(sh, a.teams, at);
+      parts = (int)(team_of(sh, a.teams, at + steps - 1) - t0) + 1;
+      first = unit + t0;
+    }
   }
   if (parts == 1) return;  // written by its block
   const uint64_t present = a.present[b];
@@ -875,26 +900,35 @@ constexpr int row_tiles(size_t elt, int dp) {
 struct Plan {
   bool many;
   int tiles;  // row tiles of a block
-  int row_blocks, teams, least;
+  int row_blocks, teams, splits, least;
 };
 
 Plan plan(const KvCache& c, int heads, int nodes) {
   const int R = nodes * (heads / c.kv_heads), dp = c.d <= 32 ? 32 : c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
   Plan p;
   p.many = R > 16 && c.dt != DType::F32 && (c.d == 64 || c.d == 128);
-  p.tiles = p.many ? (R <= 32 ? 2 : R <= 64 ? 4 : R <= 128 || c.d == 128 ? 8 : 16)
+  p.tiles = p.many ? (R <= 32 ? 2 : R <= 64 ? 4 : R <= 128 ? 8 : 16)
                    : std::min(row_tiles(dtype_size(c.dt), dp), R <= 16 ? 1 : R <= 32 ? 2 : 4);
   p.row_blocks = (R + 16 * p.tiles - 1) / (16 * p.tiles);
   const int64_t steps = (c.capacity + kStepKeys - 1) / kStepKeys + (nodes + kStepKeys - 1) / kStepKeys;
+  const int64_t units = std::max<int64_t>(1, (int64_t)c.rows * c.kv_heads);
   // k_tree_many fills a CU with a block; of the others a CU holds a few at a time, and
   // more of them even out the lengths.
   p.least = 8;
+  p.splits = 1;
   p.teams = std::max(8, (p.many ? 256 : 1024) / p.row_blocks / 8 * 8);
-  if (steps <= p.least) p.teams = 0;
+  if (steps * units <= (int64_t)p.teams * p.least * 2) {
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((steps + p.least - 1) / p.least, p.teams / units));
+    p.teams = 0;
+  }
   return p;
 }
 
-size_t slots(const KvCache& c, const Plan& p) { return p.teams == 0 ? 0 : (size_t)p.teams + (size_t)c.rows * c.kv_heads; }
+bool cuts(const Plan& p) { return p.teams > 0 || p.splits > 1; }
+size_t blocks_of(const KvCache& c, const Plan& p) {  // and slots, where units are cut
+  const size_t units = (size_t)c.rows * c.kv_heads;
+  return p.teams > 0 ? p.teams + units : units * p.splits;
+}
 
 template <typename T, int DP, int NR>
 void launch_few(const TreeArgs& a, int blocks, hipStream_t s) {
@@ -932,15 +966,15 @@ void launch_many(const TreeArgs& a, int blocks, int tiles, hipStream_t s) {
   if (tiles == 2) launch_many<T, DP, 2, 1>(a, blocks, s);
   else if (tiles == 4) launch_many<T, DP, 4, 1>(a, blocks, s);
   else if (tiles == 8) launch_many<T, DP, 8, 1>(a, blocks, s);
-  else if constexpr (DP == 64) launch_many<T, DP, 8, 2>(a, blocks, s);
+  else launch_many<T, DP, 8, 2>(a, blocks, s);
 }
 
 }  // namespace
 
 size_t tree_attention_workspace(const KvCache& c, int heads, int nodes) {
   const Plan p = plan(c, heads, nodes);
-  if (p.teams == 0) return 0;
-  return slots(c, p) * (size_t)(heads / c.kv_heads * nodes) * (c.d + 2) * 4 + (size_t)c.rows * 8;
+  if (!cuts(p)) return 0;
+  return blocks_of(c, p) * (size_t)(heads / c.kv_heads * nodes) * (c.d + 2) * 4 + (size_t)c.rows * 8;
 }
 
 void tree_attention(const KvCache& c, const TreeAttnArgs& t, void* ws, hipStream_t s) {
@@ -955,16 +989,16 @@ void tree_attention(const KvCache& c, const TreeAttnArgs& t, void* ws, hipStream
   a.o_row = t.out.row_stride, a.o_node = t.out.node_stride, a.o_head = t.out.head_stride;
   a.c_row = c.row_stride, a.c_head = c.head_stride, a.c_slot = c.slot_stride, a.parents_stride = t.parents_stride;
   a.rows = c.rows, a.capacity = c.capacity, a.kv_heads = c.kv_heads, a.heads = t.heads, a.nodes = t.nodes, a.D = c.d;
-  a.buckets = t.buckets, a.teams = p.teams, a.least = p.least, a.row_blocks = p.row_blocks;
+  a.buckets = t.buckets, a.teams = p.teams, a.splits = p.splits, a.least = p.least, a.row_blocks = p.row_blocks;
   a.scale = t.scale;
   const int R = t.nodes * (t.heads / c.kv_heads);
-  if (p.teams > 0) {
-    const size_t rows = slots(c, p) * R;
+  if (cuts(p)) {
+    const size_t rows = blocks_of(c, p) * R;
     a.part = static_cast<float*>(ws);
     a.part_ml = reinterpret_cast<float2*>(a.part + rows * c.d);
     a.present = reinterpret_cast<uint64_t*>(a.part_ml + rows);
   }
-  const int blocks = p.teams > 0 ? (int)slots(c, p) : c.rows * c.kv_heads;
+  const int blocks = (int)blocks_of(c, p);
   if (p.many) {
     auto go = [&](auto x) {
       using T = decltype(x);
@@ -982,10 +1016,14 @@ void tree_attention(const KvCache& c, const TreeAttnArgs& t, void* ws, hipStream
     });
   }
   MRT_HIP_CHECK(hipGetLastError());
-  if (p.teams > 0) {
-    const dim3 grid(c.rows * c.kv_heads * ((R + 4 * kJoinRows - 1) / (4 * kJoinRows)));
-    const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64;
-    MRT_DTYPE_DISPATCH(c.dt, hipLaunchKernelGGL(k_tree_join<T>, grid, dim3(256), 0, s, a, p.many, cols));
+  if (cuts(p)) {
+    const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64, units = c.rows * c.kv_heads;
+    MRT_DTYPE_DISPATCH(c.dt, {
+      if ((int64_t)units * R < 16384)
+        hipLaunchKernelGGL((k_tree_join<T, 1>), dim3(units * ((R + 3) / 4)), dim3(256), 0, s, a, p.many, cols);
+      else
+        hipLaunchKernelGGL((k_tree_join<T, 4>), dim3(units * ((R + 15) / 16)), dim3(256), 0, s, a, p.many, cols);
+    });
     MRT_HIP_CHECK(hipGetLastError());
   }
 }
