@@ -413,7 +413,8 @@ template <int DP, int WR, int NR>
 struct Many {
   static constexpr int kWaves = 8, WK = kWaves / WR, kKeys = 32 * WK;  // keys of a stage
   static constexpr int kRow = 2 * DP, kStage = 2 * kKeys * kRow;       // bytes: a key, K and V of a stage
-  static constexpr int S = kStage >= 64 * 1024 ? 2 : 4;                // stages
+  static constexpr bool kHalves = WR == 8;                             // two halves of the waves, half a step apart
+  static constexpr int S = kStage >= 64 * 1024 ? 2 : kHalves ? 5 : 4;  // stages
   static constexpr int kLoads = kStage / 1024 / kWaves;  // 1 KB loads of a wave and stage
   static constexpr int kPieces = kRow / 16, kRowsLoad = 1024 / kRow;
   static constexpr size_t kRing = (size_t)S * kStage, kJoin = WK > 1 ? (size_t)kWaves * NR * (DP / 16) * 1024 : 0;
@@ -586,7 +587,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
     // From here on the only vector memory operations are the stages' (but for a bias
     // with positions or too large for LDS, whose loads make waits longer, not shorter).
 #pragma unroll
-    for (int s = 0; s < S - 1; ++s) issue();
+    for (int s = 0; s < (M::kHalves ? S - 2 : S - 1); ++s) issue();
 
     f32x4_t o[NR][E];  // [t][e][r]: dimension 16 e + 4 g + r of row i of tile t
     float m[NR], l[NR];
@@ -597,19 +598,29 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
     }
 
+    // A step: where its keys are, whether they are nodes, and whether all 32 count for all.
+    struct Step {
+      uint32_t stage;
+      int base, end;
+      bool on, fresh, plain;
+    };
     int slot_now = 0;
-    for (int s = 0; s < stages; ++s) {
-      __builtin_amdgcn_s_waitcnt(vm_wait_imm((S - 2) * M::kLoads));  // this wave's part of stage s is in LDS
-      ring_barrier();                                                // everyone's is, and stage s - 1 has been read
-      issue();
-      const uint32_t stage = ring + slot_now * M::kStage;
+    auto step_of = [&](int s) {
+      Step p;
+      p.stage = ring + slot_now * M::kStage;
       slot_now = slot_now + 1 == S ? 0 : slot_now + 1;
       const int st = s0 + s * WK + wk;
-      if (st >= s1 || row0 >= R) continue;
-      const bool fresh = st < new_steps;
-      const int base = (fresh ? st : st - new_steps) * kStepKeys, end = fresh ? a.nodes : len;
-      const bool whole = base + kStepKeys <= end;
-      f32x4_t x[NR], y[NR];
+      p.on = st < s1 && row0 < R;
+      p.fresh = st < new_steps;
+      p.base = (p.fresh ? st : st - new_steps) * kStepKeys, p.end = p.fresh ? a.nodes : len;
+      p.plain = !p.fresh && p.base + kStepKeys <= len;
+      return p;
+    };
+    f32x4_t x[NR], y[NR];  // Q K^T of a step
+    uint4 ph[NR], pl[NR];  // its weights
+    uint32_t left_out = 0;  // nonzero: infinities or NaN among the nodes' values
+    auto scores = [&](const Step& p) {
+      const uint32_t stage = p.stage;
 #pragma unroll
       for (int t = 0; t < NR; ++t) x[t] = {0.f, 0.f, 0.f, 0.f}, y[t] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -624,6 +635,10 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
             y[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[1][c]), q[t][c0 + c], y[t]);
           }
       }
+    };
+    auto weights = [&](const Step& w) {
+      const bool fresh = w.fresh, plain = w.plain;
+      const int base = w.base, end = w.end;
       float z[NR][8];
 #pragma unroll
       for (int t = 0; t < NR; ++t)
@@ -647,7 +662,6 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
             z[t][j] = fmaf(z[t][j], scale2, row[min(max(qp - kpos[j], 0), a.buckets - 1)] * kLog2e);
         }
       }
-      const bool plain = !fresh && whole;
       if (!plain) {
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
@@ -657,7 +671,6 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
             z[t][j] = base + lane_key(g, j) < end && (see >> lane_key(g, j)) & 1 ? z[t][j] : -INFINITY;
         }
       }
-      uint4 ph[NR], pl[NR];
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
         const float top = max_over_groups(fmaxf(fmaxf(fmaxf(z[t][0], z[t][1]), fmaxf(z[t][2], z[t][3])),
@@ -677,9 +690,14 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         l[t] += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
         F::split(p, ph[t], pl[t]);
       }
+    };
+    auto values = [&](const Step& p) {
+      const uint32_t stage = p.stage;
+      const bool fresh = p.fresh, plain = p.plain;
+      const int base = p.base, end = p.end;
       // Rows past the end are zeros; a node's infinities and NaN belong to those who see it
-      // and go by class (as above).
-      uint32_t in[2][2], diff = 0;
+      // and are added in the end.
+      uint32_t in[2][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int key = base + 16 * h + 4 * g;
@@ -698,7 +716,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
 #pragma unroll
               for (int w = 0; w < 2; ++w) {
                 const uint32_t v = vx[e][h][w] & in[h][w], u = fresh ? F::finite_part(v) : v;
-                diff |= u ^ v;
+                left_out |= u ^ v;
                 vx[e][h][w] = u;
               }
         }
@@ -711,9 +729,53 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
               o[t][e0 + e] = Mma<T>::mma(make_uint4(vx[e][0].x, vx[e][0].y, vx[e][1].x, vx[e][1].y), part == 0 ? ph[t] : pl[t],
                                          o[t][e0 + e]);
       }
-      if (!plain && __any(diff != 0)) {
-        // rare, so from memory
-        const uint16_t* vn = static_cast<const uint16_t*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
+    };
+
+    if constexpr (M::kHalves) {
+      // Two halves of the block, a wave of each on every SIMD, half a step apart: while one
+      // multiplies (Q K^T of step s, P V of step s - 1), the other has its softmax.  Every
+      // wave passes 2 stages + 1 barriers; barrier 2 s comes after everyone's loads of
+      // stage s and the last read of stage s - 2.
+      constexpr int kWait = (S - 3) * M::kLoads;
+      const bool second = wid >= M::kWaves / 2;
+      if (second) {
+        __builtin_amdgcn_s_waitcnt(vm_wait_imm(kWait));
+        ring_barrier();
+        issue();
+      }
+      Step prev{0, 0, 0, false, false, false};
+      for (int s = 0; s < stages; ++s) {
+        if (!second) __builtin_amdgcn_s_waitcnt(vm_wait_imm(kWait));
+        ring_barrier();
+        if (!second) issue();
+        const Step now = step_of(s);
+        if (now.on) scores(now);
+        if (prev.on) values(prev);
+        if (second) __builtin_amdgcn_s_waitcnt(vm_wait_imm(kWait));
+        ring_barrier();
+        if (second) issue();
+        if (now.on) weights(now);
+        prev = now;
+      }
+      if (!second) ring_barrier();
+      if (prev.on) values(prev);
+    } else {
+      for (int s = 0; s < stages; ++s) {
+        __builtin_amdgcn_s_waitcnt(vm_wait_imm((S - 2) * M::kLoads));  // this wave's part of stage s is in LDS
+        ring_barrier();                                                // everyone's is, and stage s - 1 has been read
+        issue();
+        const Step now = step_of(s);
+        if (!now.on) continue;
+        scores(now);
+        weights(now);
+        values(now);
+      }
+    }
+
+    if (__any(left_out != 0)) {  // rare, so from memory; by class as above
+      const uint16_t* vn = static_cast<const uint16_t*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
+      for (int st = s0 + wk; st < min(s1, new_steps); st += WK) {
+        const int base = st * kStepKeys;
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
           const uint64_t see = sees[min(row0 + t * 16 + i, R - 1) / n] >> base;
@@ -721,27 +783,23 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
 #pragma unroll
           for (int j = 0; j < 4; ++j)
             one[j] = Mma<T>::pack((see >> lane_key(g, 2 * j)) & 1 ? 1.f : 0.f, (see >> lane_key(g, 2 * j + 1)) & 1 ? 1.f : 0.f);
+#pragma unroll
           for (int e = 0; e < E; ++e) {
             uint32_t c[4];
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-              const int key = base + 16 * (w >> 1) + 4 * g + 2 * (w & 1);
-              c[w] = (key < end ? ld_g(vn + key * a.vn_node + 16 * e + i) : 0u) |
-                     (key + 1 < end ? (uint32_t)ld_g(vn + (key + 1) * a.vn_node + 16 * e + i) << 16 : 0u);
-              c[w] = F::classes(c[w]);
+              const int key = base + 16 * (w >> 1) + 4 * g + 2 * (w & 1), last = a.nodes - 1;
+              c[w] = F::classes(ld_g(vn + min(key, last) * a.vn_node + 16 * e + i) |
+                                (uint32_t)ld_g(vn + min(key + 1, last) * a.vn_node + 16 * e + i) << 16);
             }
             const f32x4_t sum = Mma<T>::mma(make_uint4(c[0], c[1], c[2], c[3]), make_uint4(one[0], one[1], one[2], one[3]),
                                             f32x4_t{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
-            for (int u = 0; u < E; ++u)
-              if (u == e)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) o[t][u][r] += F::class_value(sum[r]);
+            for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(sum[r]);
           }
         }
       }
     }
-
     const int64_t slot = sh.chunk > 0 || a.teams == 0 ? team : (int64_t)b * a.kv_heads + kvh + team;
     // every load into LDS has landed and every stage been read
     __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));
