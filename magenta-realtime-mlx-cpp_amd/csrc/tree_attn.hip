@@ -467,7 +467,9 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   // with a bias the finished logits.
   const float scale2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f), mult = BIAS ? 1.f : scale2;
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
-  constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;  // as above
+  // The maximum that the weights refer to follows only where a logit passes it by more
+  // than kSlack: most steps then leave the output alone.  fp16 weights stay below 2^15.
+  constexpr float kSlack = 8.f, kShift = std::is_same_v<T, f16> ? 15.f - kSlack : 0.f;
 
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ uint64_t sees[kMaxNodes];
@@ -677,7 +679,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
                                                 fmaxf(fmaxf(z[t][4], z[t][5]), fmaxf(z[t][6], z[t][7])))) *
                               mult -
                           kShift;
-        if (__any(top > m[t])) {
+        if (__any(top > m[t] + kSlack)) {
           const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
           m[t] = mn;
           l[t] *= f;
@@ -697,18 +699,19 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       const int base = p.base, end = p.end;
       // Rows past the end are zeros; a node's infinities and NaN belong to those who see it
       // and are added in the end.
-      uint32_t in[2][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int key = base + 16 * h + 4 * g;
-        in[h][0] = (key < end ? 0xffffu : 0u) | (key + 1 < end ? 0xffff0000u : 0u);
-        in[h][1] = (key + 2 < end ? 0xffffu : 0u) | (key + 3 < end ? 0xffff0000u : 0u);
-      }
 #pragma unroll
       for (int e0 = 0; e0 < E; e0 += 4) {
         u32x2_t vx[4][2];
         read_v<M::kRow>(v_at + e0, stage, vx);
         if (!plain) {
+          uint32_t in[2][2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {
+              const int key = base + 16 * h + 4 * g + 2 * w;
+              in[h][w] = (key < end ? 0xffffu : 0u) | (key + 1 < end ? 0xffff0000u : 0u);
+            }
 #pragma unroll
           for (int e = 0; e < 4; ++e)
 #pragma unroll
@@ -743,22 +746,22 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         ring_barrier();
         issue();
       }
-      Step prev{0, 0, 0, false, false, false};
+      Step prev{};  // each stage is a step here; waves without rows compute along and write nothing
       for (int s = 0; s < stages; ++s) {
         if (!second) __builtin_amdgcn_s_waitcnt(vm_wait_imm(kWait));
         ring_barrier();
         if (!second) issue();
         const Step now = step_of(s);
-        if (now.on) scores(now);
-        if (prev.on) values(prev);
+        scores(now);
+        if (s > 0) values(prev);
         if (second) __builtin_amdgcn_s_waitcnt(vm_wait_imm(kWait));
         ring_barrier();
         if (second) issue();
-        if (now.on) weights(now);
+        weights(now);
         prev = now;
       }
       if (!second) ring_barrier();
-      if (prev.on) values(prev);
+      values(prev);
     } else {
       for (int s = 0; s < stages; ++s) {
         __builtin_amdgcn_s_waitcnt(vm_wait_imm((S - 2) * M::kLoads));  // this wave's part of stage s is in LDS
