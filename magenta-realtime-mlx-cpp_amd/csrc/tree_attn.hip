@@ -425,33 +425,28 @@ struct Many {
   __device__ static int swz_v(int r) { return DP == 128 ? (r & 7) * 2 : ((r >> 1) & 3) * 2; }
 };
 
-// Fragments of one step from LDS.  Written out, since the compiler waits for every load
-// into LDS that is in flight before any read of LDS, which would empty the ring; each
-// block waits for its own reads.  K: rows i and i + 16 of two column chunks.
-template <int ROW>
-__device__ __forceinline__ void read_k(const uint32_t* at, uint32_t base, u32x4_t (&f)[2][2]) {
-  asm volatile(
-      "ds_read_b128 %0, %4\n\tds_read_b128 %1, %4 offset:%6\n\tds_read_b128 %2, %5\n\tds_read_b128 %3, %5 offset:%6\n\t"
-      "s_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0][0]), "=&v"(f[1][0]), "=&v"(f[0][1]), "=&v"(f[1][1])
-      : "v"(at[0] + base), "v"(at[1] + base), "n"(16 * ROW)
-      : "memory");
+// 1 KB of a stage: lane l's 16 bytes from `base` + `off` (or `from`) to LDS address `to` +
+// 16 l.  Written out, since before any read of LDS the compiler waits for every such load
+// that it knows of, which would empty the ring; the waits below count them.  No register
+// is written; m0, which nothing else here uses, is set in the same place.  What the
+// compiler counts itself only gets longer by these loads.
+__device__ __forceinline__ void load_lds(uint32_t to, const void* base, uint32_t off) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(to), "v"(off), "s"(base) : "memory");
+}
+__device__ __forceinline__ void load_lds(uint32_t to, const void* from) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(to), "v"(from) : "memory");
 }
 // V, transposed as it is read: of 16 lanes, lane 4 r + c gives the address of columns 4 c ..
-// 4 c + 3 of row r, and lane i receives column i of rows 0..3.  f[e][h]: keys 16 h + 4 g ..
-// + 3 of dimension 16 e + i, for four e.
+// 4 c + 3 of row r, and lane i receives column i of rows 0..3.
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-template <int ROW>
-__device__ __forceinline__ void read_v(const uint32_t* at, uint32_t base, u32x2_t (&f)[4][2]) {
-  asm volatile(
-      "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%12\n\tds_read_b64_tr_b16 %2, %9\n\t"
-      "ds_read_b64_tr_b16 %3, %9 offset:%12\n\tds_read_b64_tr_b16 %4, %10\n\tds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
-      "ds_read_b64_tr_b16 %6, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\ts_waitcnt lgkmcnt(0)"
-      : "=&v"(f[0][0]), "=&v"(f[0][1]), "=&v"(f[1][0]), "=&v"(f[1][1]), "=&v"(f[2][0]), "=&v"(f[2][1]), "=&v"(f[3][0]),
-        "=&v"(f[3][1])
-      : "v"(at[0] + base), "v"(at[1] + base), "v"(at[2] + base), "v"(at[3] + base), "n"(16 * ROW)
-      : "memory");
+__device__ __forceinline__ u32x2_t read_transposed(uint32_t at) {
+  typedef short s4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((MRT_LDS s4*)(uintptr_t)at));
 }
+__device__ __forceinline__ uint4 read_lds16(uint32_t at) {
+  return __builtin_bit_cast(uint4, *(const MRT_LDS u32x4_t*)(uintptr_t)at);
+}
+
 template <typename T, int DP, int WR, int NR, bool BIAS>
 __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   using F = AttnFrag<T, DP>;
@@ -543,7 +538,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
     int ahead = s0, to_slot = 0;
     const int plain_to = near ? min(s1, new_steps + len / kStepKeys) : 0;  // whole cached steps end here
     auto issue = [&] {
-      char* to = lds + to_slot * M::kStage;
+      const uint32_t to = ring + to_slot * M::kStage;
       to_slot = to_slot + 1 == S ? 0 : to_slot + 1;
       const int first = ahead;
       ahead += WK;
@@ -551,8 +546,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
 #pragma unroll
         for (int x = 0; x < M::kLoads; ++x) {
           const int t = x * M::kWaves + wid;
-          const char* from = (x < M::kLoads / 2 || (M::kLoads == 1 && wid < M::kWaves / 2) ? kb : vb) + src[x];
-          __builtin_amdgcn_global_load_lds((const MRT_GLOBAL void*)from, (MRT_LDS void*)(to + t * 1024), 16, 0, 0);
+          load_lds(to + t * 1024, x < M::kLoads / 2 || (M::kLoads == 1 && wid < M::kWaves / 2) ? kb : vb, src[x]);
         }
       } else {
         const T* kn = static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head;
@@ -566,7 +560,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
           const int key = min((fresh ? st : st - new_steps) * kStepKeys + (row & 31), (fresh ? a.nodes : len) - 1);
           const T* from = t < half ? (fresh ? kn + key * a.kn_node : kc + key * a.c_slot) + (place ^ M::swz_k(row & 31)) * 8
                                    : (fresh ? vn + key * a.vn_node : vc + key * a.c_slot) + (place ^ M::swz_v(row)) * 8;
-          __builtin_amdgcn_global_load_lds((const MRT_GLOBAL void*)from, (MRT_LDS void*)(to + t * 1024), 16, 0, 0);
+          load_lds(to + t * 1024, from);
         }
       }
       kb += stride, vb += stride;
@@ -627,14 +621,18 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       for (int t = 0; t < NR; ++t) x[t] = {0.f, 0.f, 0.f, 0.f}, y[t] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c0 = 0; c0 < KC; c0 += 2) {
-        u32x4_t kx[2][2];
-        read_k<M::kRow>(k_at + c0, stage, kx);
+        uint4 kx[2][2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          kx[0][c] = read_lds16(stage + k_at[c0 + c]);
+          kx[1][c] = read_lds16(stage + k_at[c0 + c] + 16 * M::kRow);
+        }
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int t = 0; t < NR; ++t) {
-            x[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[0][c]), q[t][c0 + c], x[t]);
-            y[t] = Mma<T>::mma(__builtin_bit_cast(uint4, kx[1][c]), q[t][c0 + c], y[t]);
+            x[t] = Mma<T>::mma(kx[0][c], q[t][c0 + c], x[t]);
+            y[t] = Mma<T>::mma(kx[1][c], q[t][c0 + c], y[t]);
           }
       }
     };
@@ -701,8 +699,12 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       // and are added in the end.
 #pragma unroll
       for (int e0 = 0; e0 < E; e0 += 4) {
-        u32x2_t vx[4][2];
-        read_v<M::kRow>(v_at + e0, stage, vx);
+        u32x2_t vx[4][2];  // keys 16 h + 4 g .. + 3 of dimension 16 e + i
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          vx[e][0] = read_transposed(stage + v_at[e0 + e]);
+          vx[e][1] = read_transposed(stage + v_at[e0 + e] + 16 * M::kRow);
+        }
         if (!plain) {
           uint32_t in[2][2];
 #pragma unroll
