@@ -1,6 +1,7 @@
 // Commit of an accepted path into a cache, and eviction by accumulated attention
 // weight.
 #include <algorithm>
+#include <utility>
 
 #include "attn_frag.hpp"
 #include "kv_cache.hpp"
@@ -165,9 +166,12 @@ void launch_commit(const CommitK& a, int rows, int nr, hipStream_t s) {
 // order: no row is read that another move writes, so the moves need no order among
 // themselves.  Ranks come from ballots over consecutive slots, so the result is the same
 // on every run.  Short caches (k_evict_short): one wave holds a head's keys in registers
-// and finds the threshold by ballots, a bit at a time, with no barrier.  Long ones
-// (k_evict_select): a block a head, 11 bits a pass through LDS histograms until the keys
-// that are left fit LDS.
+// and finds the threshold by ballots, a bit at a time, with no barrier.  Long ones: a head's
+// slots go to several blocks.  k_evict_keys counts each part's keys by their first 10 bits,
+// k_evict_collect finds the digit that the threshold has from all parts' counts and
+// collects its keys, k_evict_lists finds the other 22 bits from these in two passes, each
+// block by itself, and lists what moves: no block waits for another, and keys that are all
+// alike only make the collected ones more.
 
 constexpr uint32_t kLowest = 0x007fffffu;  // of -inf; a NaN counts as that
 constexpr uint32_t kFixed = 0xffffffffu;   // entries that stay
@@ -178,10 +182,13 @@ struct EvictK {
   const float* score;
   float* score_out;
   int *pos_out, *length_out;
-  uint32_t* keys;               // (rows * kv_heads, capacity): k_evict_select
   int *holes, *movers, *count;  // (rows * kv_heads, list), (rows * kv_heads): for k_evict_move, or nullptr
+  uint32_t *keys, *few;         // (rows * kv_heads, capacity): of long caches, and what follows
+  uint32_t* hist;               // (rows * kv_heads, parts, kBins1)
+  int2* part_of;                // (rows * kv_heads, parts): keys in few, keys of higher digits
+  uint2* digit;                 // (rows * kv_heads): of `few`, and how many of these are kept
   int64_t c_row, c_head, c_slot;
-  int capacity, kv_heads, keep, recent, sinks, list, row_bytes, esz;
+  int capacity, kv_heads, keep, recent, sinks, list, row_bytes, esz, parts, part_slots;
 };
 
 __device__ __forceinline__ uint32_t evict_key(int p, float f, int64_t recent_from, int sinks) {
@@ -289,6 +296,7 @@ __global__ __launch_bounds__(256) void k_evict_short(const EvictK a) {
   __syncthreads();
   int* hl = a.holes != nullptr ? a.holes + (int64_t)bg * a.list : hole_at;
   int* ml = a.holes != nullptr ? a.movers + (int64_t)bg * a.list : mover_at;
+  const int total = hole_base[KPT];
 #pragma unroll
   for (int z = 0; z < PER; ++z) {
     const int t = z * W + wid, j = t * 64 + lane;
@@ -299,15 +307,14 @@ __global__ __launch_bounds__(256) void k_evict_short(const EvictK a) {
     const bool k = (who >> lane) & 1;
     if (j < m && k) a.score_out[at + j] = f[z], a.pos_out[at + j] = p[z];
     if (j < m && !k) hl[hole_base[t] + __popcll(~who & head & below)] = j;
-    if (j >= m && k) ml[mover_base[t] + __popcll(who & ~head & below)] = j;
+    if (j >= m && k) ml[total - 1 - mover_base[t] - __popcll(who & ~head & below)] = j;
   }
-  const int total = hole_base[KPT];
   if (a.holes != nullptr) __threadfence_block();
   __syncthreads();
   if (a.count != nullptr) {
     if (tid == 0) a.count[bg] = total;
     for (int x = tid; x < total; x += 256) {
-      const int to = hl[x], from = ml[x];
+      const int to = hl[x], from = ml[total - 1 - x];
       a.score_out[at + to] = ld_g(a.score + at + from), a.pos_out[at + to] = ld_g(a.pos + at + from);
     }
     return;
@@ -316,194 +323,257 @@ __global__ __launch_bounds__(256) void k_evict_short(const EvictK a) {
   const int pieces = a.row_bytes / 16;
 #pragma unroll 2
   for (int x = tid; x < total * pieces; x += 256) {
-    const int r = x / pieces, piece = x - r * pieces, from = ml[r], to = hl[r];
+    const int r = x / pieces, piece = x - r * pieces, from = ml[total - 1 - r], to = hl[r];
     move_row(a, base, from, to, piece);
     if (piece == 0) a.score_out[at + to] = ld_g(a.score + at + from), a.pos_out[at + to] = ld_g(a.pos + at + from);
   }
 }
 
-constexpr int kSelThreads = 1024, kSelWaves = kSelThreads / 64, kSelBatch = 16;
-constexpr int kDigit = 11, kBins = 1 << kDigit, kFew = 8192;  // bins of a pass; keys that LDS takes for the rest
+constexpr int kSelThreads = 512, kSelWaves = kSelThreads / 64, kSelBatch = 8;
+constexpr int kPartSlots = kSelThreads * kSelBatch;  // slots of a part: a multiple of these
+constexpr int kMostParts = 32;
+constexpr int kBins1 = 1 << 10, kBins2 = 1 << 11;    // digits of 10, 11 and 11 bits
+constexpr int kRep = 4;                              // copies of a histogram, by lane
 
-__global__ __launch_bounds__(kSelThreads) void k_evict_select(const EvictK a) {
-  constexpr int W = kSelWaves, kRep = 4;
-  const int bg = blockIdx.x, b = bg / a.kv_heads, kvh = bg - b * a.kv_heads;
-  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int len = min(max(a.length[b], 0), a.capacity), m = min(len, a.keep);
-  const int64_t at = (int64_t)bg * a.capacity;
-  const float* score = a.score + at;
-  const int* pos = a.pos + at;
-  float* score_out = a.score_out + at;
-  int* pos_out = a.pos_out + at;
-  uint32_t* keys = a.keys + at;
-  if (kvh == 0 && tid == 0) a.length_out[b] = m;
-  if (m == len) {
-    for (int j = tid; j < len; j += kSelThreads) score_out[j] = score[j], pos_out[j] = pos[j];
-    if (tid == 0) a.count[bg] = 0;
-    return;
+// One more key of `digit`; lanes that share the first active lane's digit count as one.
+__device__ __forceinline__ void count_digit(uint32_t* hist, uint32_t digit, int lane) {
+  const uint32_t lead = __builtin_amdgcn_readfirstlane(digit);
+  const uint64_t who = __ballot(digit == lead);
+  if (digit != lead) atomicAdd(&hist[digit * kRep + (lane & (kRep - 1))], 1u);
+  else if (lane == __ffsll((unsigned long long)who) - 1) atomicAdd(&hist[digit * kRep], (uint32_t)__popcll(who));
+}
+
+// The digit with which the `want` highest of BINS counted digits end: thread t brings the
+// counts of digits PER t .. and counts from the top.  Returns it in `picked`: the digit,
+// and how many of its keys are among the `want`.
+template <int BINS>
+__device__ __forceinline__ void pick_digit(const uint32_t (&c)[BINS / kSelThreads], uint32_t want, uint32_t* total_of,
+                                           uint32_t* picked) {
+  constexpr int PER = BINS / kSelThreads;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  uint32_t own = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) own += c[j];
+  uint32_t above = own;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t x = __shfl_down(above, o, 64);
+    if (lane + o < 64) above += x;
   }
-  const int64_t recent_from = (int64_t)a.next_pos[b] - a.recent;
-  // Wave w owns slots [w run, (w + 1) run), 64 a turn.  f(slot, key, in use) in slot
-  // order, a batch of keys loaded ahead; only the owner reads what it wrote.
-  const int turns = (len + 64 * W - 1) / (64 * W), lo = wid * turns * 64 + lane;
-  auto each = [&](auto&& f) {
-    for (int t0 = 0; t0 < turns; t0 += kSelBatch) {
-      uint32_t k[kSelBatch];
+  if (lane == 0) total_of[wid] = above;
+  __syncthreads();
+  above -= own;
+  for (int w = wid + 1; w < kSelWaves; ++w) above += total_of[w];
 #pragma unroll
-      for (int t = 0; t < kSelBatch; ++t) {
-        const int j = lo + (t0 + t) * 64;
-        k[t] = t0 + t < turns && j < len ? ld_g(keys + j) : 0u;
-      }
-#pragma unroll
-      for (int t = 0; t < kSelBatch; ++t) {
-        const int j = lo + (t0 + t) * 64;
-        if (t0 + t < turns) f(j, k[t], j < len);
-      }
-    }
-  };
+  for (int j = PER - 1; j >= 0; --j) {
+    if (above < want && want <= above + c[j]) picked[0] = PER * tid + j, picked[1] = want - above;
+    above += c[j];
+  }
+  __syncthreads();
+}
 
-  __shared__ uint32_t hist[kBins * kRep];  // then the few keys that are left
-  __shared__ uint32_t total_of[W];
-  __shared__ uint32_t picked[4];           // digit, of its keys how many are kept, how many there are; the few's count
-  __shared__ int tally[3][W];
-  uint32_t prefix = 0, mask = 0, want = m;  // of the keys with this prefix, `want` are kept
-  // Picks the digit at `shift` from the histogram: thread t holds bins 2 t, 2 t + 1, and
-  // counts from the top.
-  auto pick = [&](int shift, int bits) {
-    __syncthreads();
-    uint32_t c[2] = {0, 0};
-#pragma unroll
-    for (int r = 0; r < kRep; ++r) {
-      c[0] += hist[(2 * tid) * kRep + ((r + tid) & (kRep - 1))];
-      c[1] += hist[(2 * tid + 1) * kRep + ((r + tid) & (kRep - 1))];
-    }
-    uint32_t above = c[0] + c[1];
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t x = __shfl_down(above, o, 64);
-      if (lane + o < 64) above += x;
-    }
-    if (lane == 0) total_of[wid] = above;
-    __syncthreads();
-    above -= c[0] + c[1];
-    for (int w = wid + 1; w < W; ++w) above += total_of[w];
-#pragma unroll
-    for (int j = 1; j >= 0; --j) {
-      if (above < want && want <= above + c[j]) picked[0] = 2 * tid + j, picked[1] = want - above, picked[2] = c[j];
-      above += c[j];
-    }
-    __syncthreads();
-    prefix |= picked[0] << shift;
-    mask |= ((1u << bits) - 1) << shift;
-    want = picked[1];
-  };
-  auto clear = [&] {
-    for (int x = tid; x < kBins * kRep; x += kSelThreads) hist[x] = 0;
-    __syncthreads();
-  };
-  auto count = [&](uint32_t digit) { atomicAdd(&hist[digit * kRep + (lane & (kRep - 1))], 1u); };
-  clear();
-  for (int t0 = 0; t0 < turns; t0 += kSelBatch) {
+// What a block of the three kernels works on.
+struct EvictPart {
+  int bg, part, parts, len, m, from, to;  // parts in use; slots [from, to)
+  int64_t at;
+};
+__device__ __forceinline__ EvictPart evict_part(const EvictK& a) {
+  EvictPart e;
+  e.bg = blockIdx.x / a.parts, e.part = blockIdx.x - e.bg * a.parts;
+  e.len = min(max(a.length[e.bg / a.kv_heads], 0), a.capacity), e.m = min(e.len, a.keep);
+  e.parts = (e.len + a.part_slots - 1) / a.part_slots;
+  e.from = min(e.part * a.part_slots, e.len), e.to = min(e.len, e.from + a.part_slots);
+  e.at = (int64_t)e.bg * a.capacity;
+  return e;
+}
+
+__global__ __launch_bounds__(kSelThreads) void k_evict_keys(const EvictK a) {
+  const EvictPart e = evict_part(a);
+  const int tid = threadIdx.x, lane = tid & 63, b = e.bg / a.kv_heads;
+  if (e.part == 0 && e.bg == b * a.kv_heads && tid == 0) a.length_out[b] = e.m;
+  if (e.from >= e.to) return;
+  __shared__ uint32_t hist[kBins1 * kRep];
+  for (int x = tid; x < kBins1 * kRep; x += kSelThreads) hist[x] = 0;
+  const int64_t recent_from = (int64_t)a.next_pos[b] - a.recent;
+  __syncthreads();
+  for (int j0 = e.from + tid; j0 < e.to; j0 += kPartSlots) {
     float f[kSelBatch];
     int p[kSelBatch];
 #pragma unroll
     for (int t = 0; t < kSelBatch; ++t) {
-      const int j = lo + (t0 + t) * 64;
-      const bool in = t0 + t < turns && j < len;
-      f[t] = in ? ld_g(score + j) : 0.f;
-      p[t] = in ? ld_g(pos + j) : 0;
+      const int j = j0 + t * kSelThreads;
+      f[t] = j < e.to ? ld_g(a.score + e.at + j) : 0.f;
+      p[t] = j < e.to ? ld_g(a.pos + e.at + j) : 0;
     }
 #pragma unroll
     for (int t = 0; t < kSelBatch; ++t) {
-      const int j = lo + (t0 + t) * 64;
-      if (t0 + t >= turns || j >= len) continue;
+      const int j = j0 + t * kSelThreads;
+      if (j >= e.to) continue;
+      if (j < e.m) a.score_out[e.at + j] = f[t], a.pos_out[e.at + j] = p[t];  // k_evict_move overwrites the evicted ones
+      if (e.m == e.len) continue;
       const uint32_t key = evict_key(p[t], f[t], recent_from, a.sinks);
-      keys[j] = key;
-      if (j < m) score_out[j] = f[t], pos_out[j] = p[t];  // k_evict_move overwrites the evicted ones
-      count(key >> 21);
+      a.keys[e.at + j] = key;
+      count_digit(hist, key >> 22, lane);
     }
   }
-  pick(21, kDigit);
-  int shift = 21;
-  while (shift > 0 && picked[2] > kFew) {  // crowded: another pass over all keys
-    const int bits = shift > kDigit ? kDigit : shift;
-    __syncthreads();  // picked has been read
-    clear();
-    each([&](int, uint32_t key, bool in) {
-      if (in && (key & mask) == prefix) count((key >> (shift - bits)) & ((1u << bits) - 1));
-    });
-    shift -= bits;
-    pick(shift, bits);
+  if (e.m == e.len) return;
+  __syncthreads();
+  uint32_t* out = a.hist + (size_t)blockIdx.x * kBins1;
+  for (int x = tid; x < kBins1; x += kSelThreads) {
+    const uint4 c = reinterpret_cast<const uint4*>(hist)[x];
+    out[x] = c.x + c.y + c.z + c.w;
   }
-  if (shift > 0) {  // the rest from LDS, a bit at a time
-    if (tid == 0) picked[3] = 0;
-    __syncthreads();
-    each([&](int, uint32_t key, bool in) {
-      const bool mine = in && (key & mask) == prefix;
-      const uint64_t who = __ballot(mine);
+}
+
+__global__ __launch_bounds__(kSelThreads) void k_evict_collect(const EvictK a) {
+  constexpr int PER = kBins1 / kSelThreads;
+  const EvictPart e = evict_part(a);
+  if (e.m == e.len || e.from >= e.to) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  __shared__ uint32_t total_of[kSelWaves], picked[2], left, beyond;
+  if (tid == 0) left = 0, beyond = 0;
+  const uint32_t* hist = a.hist + (size_t)e.bg * a.parts * kBins1 + PER * tid;
+  uint32_t c[PER] = {}, own[PER] = {};
+#pragma unroll 8
+  for (int p = 0; p < e.parts; ++p) {
+    const uint2 x = *reinterpret_cast<const uint2*>(hist + (size_t)p * kBins1);
+    c[0] += x.x, c[1] += x.y;
+    if (p == e.part) own[0] = x.x, own[1] = x.y;
+  }
+  static_assert(PER == 2);
+  pick_digit<kBins1>(c, e.m, total_of, picked);
+  const uint32_t digit = picked[0];
+  uint32_t above = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) above += (uint32_t)(PER * tid + j) > digit ? own[j] : 0u;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) above += __shfl_xor(above, o, 64);
+  if (lane == 0 && above > 0) atomicAdd(&beyond, above);
+  // The keys with that digit, in any order.
+  for (int j0 = e.from + tid; j0 < e.to; j0 += kPartSlots) {
+    uint32_t key[kSelBatch];
+#pragma unroll
+    for (int t = 0; t < kSelBatch; ++t) {
+      const int j = j0 + t * kSelThreads;
+      key[t] = j < e.to ? ld_g(a.keys + e.at + j) : 0u;
+    }
+#pragma unroll
+    for (int t = 0; t < kSelBatch; ++t) {
+      const bool in = j0 + t * kSelThreads < e.to && key[t] >> 22 == digit;
+      const uint64_t who = __ballot(in);
+      if (!in) continue;
+      const int lead = __ffsll((unsigned long long)who) - 1;
       uint32_t first = 0;
-      if (who != 0 && lane == 0) first = atomicAdd(&picked[3], (uint32_t)__popcll(who));
-      first = __builtin_amdgcn_readfirstlane(first);
-      if (mine) hist[first + __popcll(who & ((1ull << lane) - 1))] = key;
+      if (lane == lead) first = atomicAdd(&left, (uint32_t)__popcll(who));
+      first = __shfl(first, lead, 64);
+      a.few[e.at + e.from + first + __popcll(who & ((1ull << lane) - 1))] = key[t];
+    }
+  }
+  __syncthreads();
+  if (tid == 0) {
+    a.part_of[blockIdx.x] = make_int2((int)left, (int)beyond);
+    if (e.part == 0) a.digit[e.bg] = make_uint2(digit, picked[1]);
+  }
+}
+
+__global__ __launch_bounds__(kSelThreads) void k_evict_lists(const EvictK a) {
+  constexpr int W = kSelWaves, PER = kBins2 / kSelThreads;
+  const EvictPart e = evict_part(a);
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  if (e.m == e.len) {
+    if (e.part == 0 && tid == 0) a.count[e.bg] = 0;
+    return;
+  }
+  if (e.from >= e.to) return;
+  __shared__ uint32_t hist[kBins2 * kRep];
+  __shared__ uint32_t total_of[W], picked[2];
+  __shared__ int tally[3][W];
+  const uint2 first = a.digit[e.bg];
+  const int2* part_of = a.part_of + (size_t)e.bg * a.parts;
+  // f(key, part) for every key of the head that shares the digit.
+  auto each_few = [&](int parts, auto&& f) {
+    for (int p = wid; p < parts; p += W) {
+      const int n = __builtin_amdgcn_readfirstlane(part_of[p].x);
+      const uint32_t* few = a.few + e.at + (int64_t)p * a.part_slots;
+      for (int x0 = lane; x0 < n; x0 += 64 * kSelBatch) {
+        uint32_t key[kSelBatch];
+#pragma unroll
+        for (int t = 0; t < kSelBatch; ++t) key[t] = x0 + t * 64 < n ? ld_g(few + x0 + t * 64) : 0u;
+#pragma unroll
+        for (int t = 0; t < kSelBatch; ++t)
+          if (x0 + t * 64 < n) f(key[t]);
+      }
+    }
+  };
+  uint32_t prefix = first.x, want = first.y;
+#pragma unroll
+  for (int shift = 11; shift >= 0; shift -= 11) {
+    for (int x = tid; x < kBins2 * kRep; x += kSelThreads) hist[x] = 0;
+    __syncthreads();
+    each_few(e.parts, [&](uint32_t key) {
+      if (key >> (shift + 11) == prefix) count_digit(hist, (key >> shift) & (kBins2 - 1), lane);
     });
     __syncthreads();
-    const int n = picked[3];
-    uint32_t k[kFew / kSelThreads];
+    uint32_t c[PER];
 #pragma unroll
-    for (int z = 0; z < kFew / kSelThreads; ++z) k[z] = tid + z * kSelThreads < n ? hist[tid + z * kSelThreads] : 0u;
-    for (int bit = shift - 1; bit >= 0; --bit) {
-      const uint32_t x = prefix | (1u << bit);
-      int c = 0;
-#pragma unroll
-      for (int z = 0; z < kFew / kSelThreads; ++z) c += __popcll(__ballot(k[z] >= x && k[z] >> bit == x >> bit));
-      if (lane == 0) tally[bit & 1][wid] = c;
-      __syncthreads();
-      int sum = 0;
-#pragma unroll
-      for (int w = 0; w < W; ++w) sum += tally[bit & 1][w];
-      if (sum >= (int)want) prefix = x;
-      else want -= sum;
+    for (int j = 0; j < PER; ++j) {
+      const uint4 x = reinterpret_cast<const uint4*>(hist)[PER * tid + j];
+      c[j] = x.x + x.y + x.z + x.w;
     }
-    __syncthreads();
+    pick_digit<kBins2>(c, want, total_of, picked);
+    prefix = prefix << 11 | picked[0], want = picked[1];
+    __syncthreads();  // before `picked` and `hist` are written again
   }
-  // Kept: keys above prefix, and the first `want` slots with it.
-  int equal = 0;
-  each([&](int, uint32_t key, bool in) { equal += __popcll(__ballot(in && key == prefix)); });
-  if (lane == 0) tally[0][wid] = equal;
+  // Kept: keys above prefix, and the first `want` slots with it.  Those of earlier parts:
+  int above = 0, equal = 0;
+  each_few(e.part, [&](uint32_t key) { above += key > prefix, equal += key == prefix; });
+  for (int p = tid; p < e.part; p += kSelThreads) above += part_of[p].y;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) above += __shfl_xor(above, o, 64), equal += __shfl_xor(equal, o, 64);
+  if (lane == 0) tally[0][wid] = above, tally[1][wid] = equal;
   __syncthreads();
-  int ties = 0;
-  for (int w = 0; w < wid; ++w) ties += tally[0][w];
-  const uint64_t below = (1ull << lane) - 1;
-  auto kept_of = [&](uint32_t key, bool in, int& seen) -> bool {
-    const uint64_t eq = __ballot(in && key == prefix);
-    const bool k = in && (key > prefix || (key == prefix && seen + __popcll(eq & below) < (int)want));
-    seen += __popcll(eq);
-    return k;
+  int kept = 0, ties = 0;
+  for (int w = 0; w < W; ++w) kept += tally[0][w], ties += tally[1][w];
+  __syncthreads();
+  // Wave w owns `run` slots of the part, 64 a turn.
+  const int run = ((e.to - e.from + 64 * W - 1) / (64 * W)) * 64, lo = min(e.to, e.from + wid * run);
+  const int hi = min(e.to, lo + run);
+  auto each = [&](auto&& f) {
+    for (int j0 = lo; j0 < hi; j0 += 64 * kSelBatch) {
+      uint32_t key[kSelBatch];
+#pragma unroll
+      for (int t = 0; t < kSelBatch; ++t) {
+        const int j = j0 + t * 64 + lane;
+        key[t] = j < hi ? ld_g(a.keys + e.at + j) : 0u;
+      }
+#pragma unroll
+      for (int t = 0; t < kSelBatch; ++t)
+        if (j0 + t * 64 < hi) f(j0 + t * 64 + lane, key[t], j0 + t * 64 + lane < hi);
+    }
   };
-  int seen = ties, holes = 0, movers = 0;
-  each([&](int j, uint32_t key, bool in) {
-    const bool k = kept_of(key, in, seen);
-    holes += __popcll(__ballot(j < m && !k));
-    movers += __popcll(__ballot(j >= m && k));
+  above = 0, equal = 0;
+  each([&](int, uint32_t key, bool in) {
+    above += __popcll(__ballot(in && key > prefix)), equal += __popcll(__ballot(in && key == prefix));
   });
-  if (lane == 0) tally[1][wid] = holes, tally[2][wid] = movers;
+  if (lane == 0) tally[0][wid] = above, tally[1][wid] = equal;
   __syncthreads();
-  int hole = 0, mover = 0, total = 0;
-  for (int w = 0; w < W; ++w) {
-    if (w < wid) hole += tally[1][w], mover += tally[2][w];
-    total += tally[1][w];
-  }
-  int* hl = a.holes + (int64_t)bg * a.list;
-  int* ml = a.movers + (int64_t)bg * a.list;
-  seen = ties;
+  for (int w = 0; w < wid; ++w) kept += tally[0][w], ties += tally[1][w];
+  kept += min(ties, (int)want);
+  // A slot below m that is evicted comes after (its slot - kept before) others; the kept
+  // entries at or above m are listed from the last one down.
+  const uint64_t below = (1ull << lane) - 1;
+  int* hl = a.holes + (int64_t)e.bg * a.list;
+  int* ml = a.movers + (int64_t)e.bg * a.list;
   each([&](int j, uint32_t key, bool in) {
-    const bool k = kept_of(key, in, seen);
-    const uint64_t h = __ballot(j < m && !k), v = __ballot(j >= m && k);
-    if (j < m && !k) hl[hole + __popcll(h & below)] = j;
-    if (j >= m && k) ml[mover + __popcll(v & below)] = j;
-    hole += __popcll(h), mover += __popcll(v);
+    const uint64_t eq = __ballot(in && key == prefix);
+    const bool k = in && (key > prefix || (key == prefix && ties + __popcll(eq & below) < (int)want));
+    const uint64_t who = __ballot(k);
+    const int before = kept + __popcll(who & below);
+    if (in && j < e.m && !k) hl[j - before] = j;
+    if (j >= e.m && k) ml[e.m - 1 - before] = j;
+    if (in && j == e.m) a.count[e.bg] = e.m - before;
+    ties += __popcll(eq), kept += __popcll(who);
   });
-  if (tid == 0) a.count[bg] = total;
 }
 
 // Rows of the lists, `blocks` blocks a (sequence, head); with `entries`, their scores and
@@ -511,12 +581,13 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_select(const EvictK a) {
 __global__ __launch_bounds__(256) void k_evict_move(const EvictK a, int blocks, bool entries) {
   const int bg = blockIdx.x / blocks, part = blockIdx.x - bg * blocks, b = bg / a.kv_heads, kvh = bg - b * a.kv_heads;
   const int pieces = a.row_bytes / 16;
-  const int64_t total = (int64_t)a.count[bg] * pieces, base = (b * a.c_row + kvh * a.c_head) * a.esz;
+  const int n = a.count[bg];
+  const int64_t total = (int64_t)n * pieces, base = (b * a.c_row + kvh * a.c_head) * a.esz;
   const int64_t at = (int64_t)bg * a.capacity;
   const int* hl = a.holes + (int64_t)bg * a.list;
   const int* ml = a.movers + (int64_t)bg * a.list;
   for (int64_t x = part * 256 + threadIdx.x; x < total; x += (int64_t)blocks * 256) {
-    const int r = (int)(x / pieces), piece = (int)(x - (int64_t)r * pieces), from = ml[r], to = hl[r];
+    const int r = (int)(x / pieces), piece = (int)(x - (int64_t)r * pieces), from = ml[n - 1 - r], to = hl[r];
     move_row(a, base, from, to, piece);
     if (entries && piece == 0) a.score_out[at + to] = a.score[at + from], a.pos_out[at + to] = a.pos[at + from];
   }
@@ -528,6 +599,14 @@ bool is_short(const KvCache& c) { return c.capacity <= kShortSlots; }
 bool moves_within(const KvCache& c, int keep) {
   return is_short(c) && (size_t)most_moves(c, keep) * c.d * dtype_size(c.dt) <= 16 * 1024;
 }
+// Slots of a part of a long cache: the smallest that leave no more parts than the card
+// takes at once, nor more than each block's sums over the parts' counts are worth.
+int part_slots(const KvCache& c) {
+  const int heads = c.rows * c.kv_heads, parts = std::max(1, std::min(kMostParts, 1024 / std::max(1, heads)));
+  const int64_t units = (c.capacity + (int64_t)kPartSlots - 1) / kPartSlots;
+  return (int)((units + parts - 1) / parts * kPartSlots);
+}
+int parts_of(const KvCache& c) { return (int)((c.capacity + (int64_t)part_slots(c) - 1) / part_slots(c)); }
 
 }  // namespace
 
@@ -562,8 +641,9 @@ void cache_commit(const KvCache& c, const CommitArgs& t, hipStream_t s) {
 
 size_t cache_evict_workspace(const KvCache& c, int keep) {
   if (moves_within(c, keep)) return 0;
-  const size_t heads = (size_t)c.rows * c.kv_heads;
-  return heads * (2 * (size_t)most_moves(c, keep) + 1 + (is_short(c) ? 0 : (size_t)c.capacity)) * 4;
+  const size_t heads = (size_t)c.rows * c.kv_heads, parts = is_short(c) ? 0 : parts_of(c);
+  const size_t of_long = is_short(c) ? 0 : 2 * (size_t)c.capacity + parts * (kBins1 + 2) + 2;
+  return heads * (2 * (size_t)most_moves(c, keep) + 1 + of_long) * 4;
 }
 
 void cache_evict(const KvCache& c, const EvictArgs& t, void* ws, hipStream_t s) {
@@ -575,15 +655,29 @@ void cache_evict(const KvCache& c, const EvictArgs& t, void* ws, hipStream_t s) 
   a.esz = (int)dtype_size(c.dt), a.row_bytes = c.d * a.esz, a.list = most_moves(c, t.keep);
   const int heads = c.rows * c.kv_heads;
   if (!moves_within(c, t.keep)) {
-    a.holes = static_cast<int*>(ws);
-    a.movers = a.holes + (size_t)heads * a.list;
-    a.count = a.movers + (size_t)heads * a.list;
-    a.keys = reinterpret_cast<uint32_t*>(a.count + heads);
+    uint32_t* at = static_cast<uint32_t*>(ws);
+    auto take = [&](size_t n) { return std::exchange(at, at + n); };
+    if (!is_short(c)) {
+      a.parts = parts_of(c), a.part_slots = part_slots(c);
+      a.hist = take((size_t)heads * a.parts * kBins1);
+      a.part_of = reinterpret_cast<int2*>(take((size_t)heads * a.parts * 2));
+      a.digit = reinterpret_cast<uint2*>(take((size_t)heads * 2));
+      a.keys = take((size_t)heads * c.capacity);
+      a.few = take((size_t)heads * c.capacity);
+    }
+    a.holes = reinterpret_cast<int*>(take((size_t)heads * a.list));
+    a.movers = reinterpret_cast<int*>(take((size_t)heads * a.list));
+    a.count = reinterpret_cast<int*>(take(heads));
   }
   if (c.capacity <= 8 * 64) hipLaunchKernelGGL(k_evict_short<8>, dim3(heads), dim3(256), 0, s, a);
   else if (c.capacity <= 18 * 64) hipLaunchKernelGGL(k_evict_short<18>, dim3(heads), dim3(256), 0, s, a);
   else if (is_short(c)) hipLaunchKernelGGL(k_evict_short<32>, dim3(heads), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(k_evict_select, dim3(heads), dim3(kSelThreads), 0, s, a);
+  else {
+    const dim3 grid(heads * a.parts), block(kSelThreads);
+    hipLaunchKernelGGL(k_evict_keys, grid, block, 0, s, a);
+    hipLaunchKernelGGL(k_evict_collect, grid, block, 0, s, a);
+    hipLaunchKernelGGL(k_evict_lists, grid, block, 0, s, a);
+  }
   MRT_HIP_CHECK(hipGetLastError());
   if (a.holes != nullptr && a.list > 0) {
     const int64_t pieces = (int64_t)a.list * (a.row_bytes / 16);

@@ -113,13 +113,15 @@ def cache_evict(k, v, length, pos, next_pos, score, keep, recent, sinks):
         m = min(L, keep)
         out["length"].append(m)
         for g in range(kv_heads):
+            positions, scores = pos[b, g].tolist(), score[b, g].tolist()
+
             def rank(j):
-                p, s = int(pos[b, g, j]), float(score[b, g, j])
+                p, s = positions[j], scores[j]
                 stays = p >= int(next_pos[b]) - recent or p < sinks
                 return (not stays, math.inf if math.isnan(s) else -s, j)
             kept = sorted(sorted(range(L), key=rank)[:m])
-            src = list(range(m))
-            holes = [j for j in range(m) if j not in set(kept)]
+            src, stay = list(range(m)), set(kept)
+            holes = [j for j in range(m) if j not in stay]
             for to, at in zip(holes, [j for j in kept if j >= m]):
                 src[to] = at
             out["k"][b, g, :m], out["v"][b, g, :m] = k[b, g, src], v[b, g, src]

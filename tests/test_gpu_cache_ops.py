@@ -215,6 +215,20 @@ def test_evict_ties_and_special_scores():
         check_evict(s, evict(s, keep), keep)
 
 
+@pytest.mark.parametrize("length", [2900, 4096, 4097, 20000, 140000])
+def test_evict_long_ties_and_special_scores(length):
+    """The same where a head's slots go to several blocks: one score everywhere, few
+    scores, scores that differ in their last bits alone."""
+    s = make_evict(13, "bf16", 2, 2, 16, [length, length // 2 + 1], spread=False)
+    c = s["score"].shape[-1]
+    s["score"][0, 0] = 0.25
+    s["score"][0, 1] = torch.randint(0, 3, (c,)).float()
+    s["score"][1, 0] = torch.tensor([math.nan, -math.inf, 0.0, -0.0, 1e-42, -1e-42, math.inf, -3.0]).repeat(c // 8 + 1)[:c]
+    s["score"][1, 1] = torch.nextafter(torch.tensor(1.0), torch.tensor(2.0)) * (1 + torch.randint(0, 9, (c,)) * 2.0**-23)
+    for keep, recent, sinks in ((1, 0, 0), (length // 3, 5, 4), (length // 2 + 1, 0, 1), (length - 1, 700, 3)):
+        check_evict(s, evict(s, keep, recent, sinks), keep, recent, sinks)
+
+
 def test_evict_in_place_and_repeated():
     s = make_evict(7, "fp16", 2, 4, 128, [4000, 3000])
     for keep in (3500, 1000):
