@@ -372,14 +372,18 @@ __device__ __forceinline__ void pick_digit(const uint32_t (&c)[BINS / kSelThread
   __syncthreads();
 }
 
-// What a block of the three kernels works on.
+// What a block of the three kernels works on.  Blocks of one head are `heads` apart, so
+// that they share an L2 where the heads are a multiple of the XCDs.
 struct EvictPart {
   int bg, part, parts, len, m, from, to;  // parts in use; slots [from, to)
+  size_t id;
   int64_t at;
 };
 __device__ __forceinline__ EvictPart evict_part(const EvictK& a) {
   EvictPart e;
-  e.bg = blockIdx.x / a.parts, e.part = blockIdx.x - e.bg * a.parts;
+  const int heads = gridDim.x / a.parts;
+  e.part = blockIdx.x / heads, e.bg = blockIdx.x - e.part * heads;
+  e.id = (size_t)e.bg * a.parts + e.part;
   e.len = min(max(a.length[e.bg / a.kv_heads], 0), a.capacity), e.m = min(e.len, a.keep);
   e.parts = (e.len + a.part_slots - 1) / a.part_slots;
   e.from = min(e.part * a.part_slots, e.len), e.to = min(e.len, e.from + a.part_slots);
@@ -418,7 +422,7 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_keys(const EvictK a) {
   }
   if (e.m == e.len) return;
   __syncthreads();
-  uint32_t* out = a.hist + (size_t)blockIdx.x * kBins1;
+  uint32_t* out = a.hist + e.id * kBins1;
   for (int x = tid; x < kBins1; x += kSelThreads) {
     const uint4 c = reinterpret_cast<const uint4*>(hist)[x];
     out[x] = c.x + c.y + c.z + c.w;
@@ -471,7 +475,7 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_collect(const EvictK a) {
   }
   __syncthreads();
   if (tid == 0) {
-    a.part_of[blockIdx.x] = make_int2((int)left, (int)beyond);
+    a.part_of[e.id] = make_int2((int)left, (int)beyond);
     if (e.part == 0) a.digit[e.bg] = make_uint2(digit, picked[1]);
   }
 }
@@ -488,14 +492,42 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_lists(const EvictK a) {
   __shared__ uint32_t hist[kBins2 * kRep];
   __shared__ uint32_t total_of[W], picked[2];
   __shared__ int tally[3][W];
+  // What the first steps need is requested at once: the part's own keys, wave w's `run`
+  // slots, 64 a turn; the head's digit; its parts' counts.
+  const int run = ((e.to - e.from + 64 * W - 1) / (64 * W)) * 64, lo = min(e.to, e.from + wid * run);
+  const int hi = min(e.to, lo + run);
+  uint32_t own[kSelBatch];
+#pragma unroll
+  for (int t = 0; t < kSelBatch; ++t) {
+    const int j = lo + t * 64 + lane;
+    own[t] = j < hi ? ld_g(a.keys + e.at + j) : 0u;
+  }
   const uint2 first = a.digit[e.bg];
-  const int2* part_of = a.part_of + (size_t)e.bg * a.parts;
-  // f(key, part) for every key of the head that shares the digit.
+  const int2 mine = lane < e.parts ? a.part_of[(size_t)e.bg * a.parts + lane] : make_int2(0, 0);
+  // The keys of the head that share the digit: wave w has those of parts w, w + W, ..; the
+  // first 64 kHold of a part stay in registers, f(key) sees each.
+  constexpr int kHold = 10, kOwnParts = kMostParts / W;
+  uint32_t held[kOwnParts][kHold];
+  int held_n[kOwnParts];
+#pragma unroll
+  for (int z = 0; z < kOwnParts; ++z) {
+    const int p = z * W + wid;
+    held_n[z] = __builtin_amdgcn_readlane(mine.x, p);
+    const uint32_t* few = a.few + e.at + (int64_t)p * a.part_slots + lane;
+#pragma unroll
+    for (int t = 0; t < kHold; ++t)
+      if (t * 64 < held_n[z]) held[z][t] = t * 64 + lane < held_n[z] ? ld_g(few + t * 64) : 0u;
+  }
   auto each_few = [&](int parts, auto&& f) {
-    for (int p = wid; p < parts; p += W) {
-      const int n = __builtin_amdgcn_readfirstlane(part_of[p].x);
+#pragma unroll
+    for (int z = 0; z < kOwnParts; ++z) {
+      const int p = z * W + wid, n = held_n[z];
+      if (p >= parts) continue;
+#pragma unroll
+      for (int t = 0; t < kHold; ++t)
+        if (t * 64 + lane < n) f(held[z][t]);
       const uint32_t* few = a.few + e.at + (int64_t)p * a.part_slots;
-      for (int x0 = lane; x0 < n; x0 += 64 * kSelBatch) {
+      for (int x0 = kHold * 64 + lane; x0 < n; x0 += 64 * kSelBatch) {
         uint32_t key[kSelBatch];
 #pragma unroll
         for (int t = 0; t < kSelBatch; ++t) key[t] = x0 + t * 64 < n ? ld_g(few + x0 + t * 64) : 0u;
@@ -527,7 +559,7 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_lists(const EvictK a) {
   // Kept: keys above prefix, and the first `want` slots with it.  Those of earlier parts:
   int above = 0, equal = 0;
   each_few(e.part, [&](uint32_t key) { above += key > prefix, equal += key == prefix; });
-  for (int p = tid; p < e.part; p += kSelThreads) above += part_of[p].y;
+  if (wid == 0 && lane < e.part) above += mine.y;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) above += __shfl_xor(above, o, 64), equal += __shfl_xor(equal, o, 64);
   if (lane == 0) tally[0][wid] = above, tally[1][wid] = equal;
@@ -535,16 +567,13 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_lists(const EvictK a) {
   int kept = 0, ties = 0;
   for (int w = 0; w < W; ++w) kept += tally[0][w], ties += tally[1][w];
   __syncthreads();
-  // Wave w owns `run` slots of the part, 64 a turn.
-  const int run = ((e.to - e.from + 64 * W - 1) / (64 * W)) * 64, lo = min(e.to, e.from + wid * run);
-  const int hi = min(e.to, lo + run);
   auto each = [&](auto&& f) {
     for (int j0 = lo; j0 < hi; j0 += 64 * kSelBatch) {
       uint32_t key[kSelBatch];
 #pragma unroll
       for (int t = 0; t < kSelBatch; ++t) {
         const int j = j0 + t * 64 + lane;
-        key[t] = j < hi ? ld_g(a.keys + e.at + j) : 0u;
+        key[t] = j0 == lo ? own[t] : j < hi ? ld_g(a.keys + e.at + j) : 0u;
       }
 #pragma unroll
       for (int t = 0; t < kSelBatch; ++t)
