@@ -333,14 +333,15 @@ constexpr int kSelThreads = 512, kSelWaves = kSelThreads / 64, kSelBatch = 8;
 constexpr int kPartSlots = kSelThreads * kSelBatch;  // slots of a part: a multiple of these
 constexpr int kMostParts = 32;
 constexpr int kBins1 = 1 << 10, kBins2 = 1 << 11;    // digits of 10, 11 and 11 bits
-constexpr int kRep = 4;                              // copies of a histogram, by lane
 
-// One more key of `digit`; lanes that share the first active lane's digit count as one.
+// One more key of `digit`, in one of REP copies of the histogram by lane; lanes that share
+// the first active lane's digit count as one.
+template <int REP>
 __device__ __forceinline__ void count_digit(uint32_t* hist, uint32_t digit, int lane) {
   const uint32_t lead = __builtin_amdgcn_readfirstlane(digit);
   const uint64_t who = __ballot(digit == lead);
-  if (digit != lead) atomicAdd(&hist[digit * kRep + (lane & (kRep - 1))], 1u);
-  else if (lane == __ffsll((unsigned long long)who) - 1) atomicAdd(&hist[digit * kRep], (uint32_t)__popcll(who));
+  if (digit != lead) atomicAdd(&hist[digit * REP + (lane & (REP - 1))], 1u);
+  else if (lane == __ffsll((unsigned long long)who) - 1) atomicAdd(&hist[digit * REP], (uint32_t)__popcll(who));
 }
 
 // The digit with which the `want` highest of BINS counted digits end: thread t brings the
@@ -396,6 +397,7 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_keys(const EvictK a) {
   const int tid = threadIdx.x, lane = tid & 63, b = e.bg / a.kv_heads;
   if (e.part == 0 && e.bg == b * a.kv_heads && tid == 0) a.length_out[b] = e.m;
   if (e.from >= e.to) return;
+  constexpr int kRep = 4;  // exponents crowd
   __shared__ uint32_t hist[kBins1 * kRep];
   for (int x = tid; x < kBins1 * kRep; x += kSelThreads) hist[x] = 0;
   const int64_t recent_from = (int64_t)a.next_pos[b] - a.recent;
@@ -417,7 +419,7 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_keys(const EvictK a) {
       if (e.m == e.len) continue;
       const uint32_t key = evict_key(p[t], f[t], recent_from, a.sinks);
       a.keys[e.at + j] = key;
-      count_digit(hist, key >> 22, lane);
+      count_digit<kRep>(hist, key >> 22, lane);
     }
   }
   if (e.m == e.len) return;
@@ -489,7 +491,7 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_lists(const EvictK a) {
     return;
   }
   if (e.from >= e.to) return;
-  __shared__ uint32_t hist[kBins2 * kRep];
+  __shared__ uint32_t hist[kBins2];
   __shared__ uint32_t total_of[W], picked[2];
   __shared__ int tally[3][W];
   // What the first steps need is requested at once: the part's own keys, wave w's `run`
@@ -540,18 +542,15 @@ __global__ __launch_bounds__(kSelThreads) void k_evict_lists(const EvictK a) {
   uint32_t prefix = first.x, want = first.y;
 #pragma unroll
   for (int shift = 11; shift >= 0; shift -= 11) {
-    for (int x = tid; x < kBins2 * kRep; x += kSelThreads) hist[x] = 0;
+    reinterpret_cast<uint4*>(hist)[tid] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     each_few(e.parts, [&](uint32_t key) {
-      if (key >> (shift + 11) == prefix) count_digit(hist, (key >> shift) & (kBins2 - 1), lane);
+      if (key >> (shift + 11) == prefix) count_digit<1>(hist, (key >> shift) & (kBins2 - 1), lane);
     });
     __syncthreads();
-    uint32_t c[PER];
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const uint4 x = reinterpret_cast<const uint4*>(hist)[PER * tid + j];
-      c[j] = x.x + x.y + x.z + x.w;
-    }
+    static_assert(PER == 4);
+    const uint4 x = reinterpret_cast<const uint4*>(hist)[tid];
+    const uint32_t c[PER] = {x.x, x.y, x.z, x.w};
     pick_digit<kBins2>(c, want, total_of, picked);
     prefix = prefix << 11 | picked[0], want = picked[1];
     __syncthreads();  // before `picked` and `hist` are written again
