@@ -89,8 +89,8 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
       for (int j = s0 * kStepKeys + tid; j < min(len, s1 * kStepKeys); j += 64 * kCommitWaves) score_out[j] = score[j];
     return;
   }
+  __shared__ uint4 rows[NR][KC][64];  // q, as the lanes read it
   for (int row0 = 0; row0 < R; row0 += 16 * NR) {
-    uint4 q[NR][KC];
     float lse[NR];
     int tok[NR], head[NR];
     bool on[NR];
@@ -98,10 +98,16 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
     for (int t = 0; t < NR; ++t) {
       const int row = row0 + t * 16 + i, r = min(row, R - 1);
       tok[t] = r / nh, head[t] = kvh * nh + r - tok[t] * nh;
-      F::load_row(static_cast<const T*>(a.q) + b * a.q_row + acc[tok[t]] * a.q_node + head[t] * a.q_head, g, D, q[t]);
+      if (wid == t % kCommitWaves) {
+        uint4 x[KC];
+        F::load_row(static_cast<const T*>(a.q) + b * a.q_row + acc[tok[t]] * a.q_node + head[t] * a.q_head, g, D, x);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) rows[t][c][lane] = x[c];
+      }
       lse[t] = a.lse[((size_t)b * a.nodes + acc[tok[t]]) * a.heads + head[t]];
       on[t] = row < R && lse[t] > -INFINITY;
     }
+    __syncthreads();
     for (int st = s0 + wid; st < s1; st += kCommitWaves) {
       const bool fresh = st >= old_steps;
       const int base = (fresh ? st - old_steps : st) * kStepKeys, end = fresh ? n : len;
@@ -127,7 +133,10 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
         if (row0 + t * 16 >= R) continue;
-        const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
+        uint4 q[KC];
+#pragma unroll
+        for (int c = 0; c < KC; ++c) q[c] = rows[t][c][lane];
+        const f32x4_t x = F::scores(kf[0], q), y = F::scores(kf[1], q);
         const float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -145,6 +154,7 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
       }
       if (i < 8 && key < end) score_out[slot] = sum;
     }
+    if (row0 + 16 * NR < R) __syncthreads();  // before `rows` is written again
   }
 }
 
