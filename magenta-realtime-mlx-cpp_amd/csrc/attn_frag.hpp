@@ -111,6 +111,17 @@ struct AttnFrag {
       f[c] = (D == DP || d < D) ? ld_g16(row + d) : make_uint4(0, 0, 0, 0);
     }
   }
+  // 16 key rows as the cache's lines are read best, four lanes to 64 bytes of a row: lane l
+  // loads with load_row(row l / 4, l % 4), and spread() hands each lane (i, g) its part of
+  // row i.  Read as the lanes need them, each load asks the L1 for 64 lines instead of 16.
+  __device__ __forceinline__ static void spread(uint4 (&f)[KC], int lane) {
+    const int from = ((lane & 15) * 4 + (lane >> 4)) * 4;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      f[c].x = __builtin_amdgcn_ds_bpermute(from, f[c].x), f[c].y = __builtin_amdgcn_ds_bpermute(from, f[c].y);
+      f[c].z = __builtin_amdgcn_ds_bpermute(from, f[c].z), f[c].w = __builtin_amdgcn_ds_bpermute(from, f[c].w);
+    }
+  }
   __device__ __forceinline__ static f32x4_t scores(const uint4 (&k)[KC], const uint4 (&q)[KC]) {
     f32x4_t a = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll

@@ -114,8 +114,8 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
       uint4 kf[2][KC];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const int key = min(base + step_key(i, h), end - 1);
-        F::load_row(fresh ? kn + acc[key] * a.kn_node : kc + (int64_t)key * a.c_slot, g, D, kf[h]);
+        const int key = min(base + step_key(lane >> 2, h), end - 1);
+        F::load_row(fresh ? kn + acc[key] * a.kn_node : kc + (int64_t)key * a.c_slot, lane & 3, D, kf[h]);
       }
       // the running sum of the group's key i, by lane i < 8
       const int key = base + lane_key(g, i & 7), slot = (fresh ? len : 0) + key;
@@ -129,6 +129,8 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
           kpos[j] = fresh ? first + kj : pos != nullptr ? pos[kj] : kj;
         }
       }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) F::spread(kf[h], lane);
       float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int t = 0; t < NR; ++t) {

@@ -212,12 +212,14 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
   const int n = a.heads / a.kv_heads, R = a.nodes * n;
   const T* kc = static_cast<const T*>(a.k) + b * a.c_row + kvh * a.c_head;
   const T* vc = static_cast<const T*>(a.v) + b * a.c_row + kvh * a.c_head;
+  const int* pos = a.pos == nullptr ? nullptr : a.pos + (size_t)(b * a.kv_heads + kvh) * a.capacity;
 
-  // Keys and values of a step.  Nothing here needs the length (rows past it are masked,
+  // Keys, values and positions of a step.  Nothing here needs the length (rows past it are masked,
   // those past the capacity are read from its last slot), so a wave's first step is
   // requested before anything else.
   uint4 kf[2][KC];
   uint32_t vf[8][VW];
+  int kpos[8];
   auto load = [&](int st) {
     const bool fresh = st < new_steps;  // drafted nodes
     const int base = (fresh ? st : st - new_steps) * kStepKeys, last = (fresh ? a.nodes : a.capacity) - 1;
@@ -228,6 +230,10 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
     for (int h = 0; h < 2; ++h) F::load_row(kb + (int64_t)min(base + step_key(i, h), last) * kstep, g, D, kf[h]);
 #pragma unroll
     for (int j = 0; j < 8; ++j) F::load_v(vb + (int64_t)min(base + lane_key(g, j), last) * vstep, i, D, vf[j]);
+    if (a.bias != nullptr && pos != nullptr && !fresh) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) kpos[j] = ld_g(pos + min(base + lane_key(g, j), last));
+    }
   };
   load(s0 + wid);
 
@@ -253,7 +259,6 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
     for (int x = tid; x < n * a.buckets; x += 64 * kWaves) btab[x] = a.bias[(size_t)kvh * n * a.buckets + x];
   ring_barrier();  // does not wait for the loads of the first step
 
-  const int* pos = a.pos == nullptr ? nullptr : a.pos + (size_t)(b * a.kv_heads + kvh) * a.capacity;
   int qpos[NR];
   const float* brow[NR];
   if (a.bias != nullptr) {
@@ -289,12 +294,11 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
         for (int w = 0; w < VW; ++w) vf[j][w] = base + lane_key(g, j) < end ? vf[j][w] : 0u;
     }
     float p[NR][8];
-    int kpos[8];
-    if (a.bias != nullptr) {
+    if (a.bias != nullptr && (fresh || pos == nullptr)) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int key = min(base + lane_key(g, j), end - 1);
-        kpos[j] = fresh ? __popcll(sees[key]) - 1 : pos != nullptr ? pos[key] : key;
+        kpos[j] = fresh ? __popcll(sees[key]) - 1 : key;
       }
     }
 #pragma unroll
