@@ -611,7 +611,7 @@ int mrt_coca_read(mrt_coca* h, int which, void* dst, size_t bytes);
  * 16 bytes) and d contiguous; d a multiple of 8, at most 256.  Sequence b has
  * length[b] entries, in slots 0 .. length[b] - 1 of every head (a length
  * outside [0, capacity] is taken as the nearest bound); what the other slots
- * hold is never looked at.  pos: NULL where an entry's slot is its position
+ * hold has no effect.  capacity at most 2^30, rows * kv_heads 2^20.  pos: NULL where an entry's slot is its position
  * (the next token's is then length[b]); else (rows, kv_heads, capacity) int32
  * positions, in any order, and next_pos (rows) the next token's.  score
  * (rows, kv_heads, capacity) fp32: accumulated attention weights, or NULL. */
@@ -653,7 +653,7 @@ typedef struct mrt_tree_attention_args {
   int64_t parents_stride; /* elements between sequences' parents; 0: one tree for all */
   float* lse;             /* (rows, nodes, heads) fp32 log-sum-exp of the logits, or NULL */
   const float* bias;      /* (heads, buckets) fp32 logit bias by distance, or NULL */
-  int32_t buckets;
+  int32_t buckets;        /* with bias: 1 .. 2^18 */
   int32_t nodes;          /* 1 .. MRT_MAX_NODES */
   int32_t heads;          /* a multiple of kv_heads: heads / kv_heads query heads share a K/V head */
   float scale;            /* 1 in this model (no 1/sqrt(d)) */
@@ -665,8 +665,10 @@ typedef struct mrt_tree_attention_args {
  * outputs are 0, their lse -inf, and no other node is touched by them.  Node t
  * attends every entry of the cache, its ancestors and itself:
  *   logit(t, j) = scale * q_t . k_j + bias[h][min(max(p_t - p_j, 0), buckets - 1)]
- * with p_t the next position plus the node's depth (0 under -1).  One node is
- * an ordinary decode step.  K/V of a node that t does not see have no effect on
+ * with p_t the next position plus the node's depth (0 under -1).  A logit of
+ * -inf, or below -1e30 (a bias of the type's lowest value), is a mask; a row
+ * with nothing left has output 0 and lse -inf.  One node is an ordinary decode
+ * step.  K/V of a node that t does not see have no effect on
  * t, whatever they hold.  Does not write the cache: mrt_cache_commit takes the
  * accepted nodes into it.  mrt_tree_attention_workspace gives the workspace
  * bytes for these sizes (0: none; workspace may then be NULL). */
@@ -683,8 +685,8 @@ typedef struct mrt_cache_commit_args {
   const float* lse;        /* (rows, nodes, heads) of mrt_tree_attention; with q */
   const float* bias;       /* as there */
   float* score_out;        /* (rows, kv_heads, capacity); with q; may be cache->score */
-  int32_t* length_out;     /* (rows), not cache->length */
-  int32_t* next_out;       /* (rows), not cache->next_pos; with cache->pos */
+  int32_t* length_out;     /* (rows), an array of its own */
+  int32_t* next_out;       /* (rows), an array of its own; with cache->pos */
   int32_t accepted_n;      /* 1 .. MRT_MAX_NODES */
   int32_t nodes;
   int32_t heads;
@@ -707,7 +709,7 @@ int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* arg
 typedef struct mrt_cache_evict_args {
   float* score_out;    /* (rows, kv_heads, capacity); may be cache->score */
   int32_t* pos_out;    /* (rows, kv_heads, capacity); may be cache->pos */
-  int32_t* length_out; /* (rows), not cache->length */
+  int32_t* length_out; /* (rows), an array of its own */
   int32_t keep;        /* entries a sequence keeps, >= 1 */
   int32_t recent;      /* the entries of the last `recent` positions stay, */
   int32_t sinks;       /*   and those of the first `sinks`; recent + sinks <= keep */
@@ -731,7 +733,8 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
  * first in the low bits; scales and biases (n, k / group), g = k / group, group
  * 32, 64 or 128, a divisor of k.  x, scales, biases and out in `dtype`, row
  * strides ldx (a multiple of 16 bytes) and ldo in elements; w and x 16-byte
- * aligned.  Meant for few rows: each 64 rows read the weights again.  Weights
+ * aligned.  Meant for few rows (at most 2^19): each 64, in fp32 each 16, read the
+ * weights again.  Weights
  * are multiplied exactly and summed in fp32; a row of x that is not
  * finite gives outputs that are not.  mrt_q4_quantize makes the codes of src (n, k), row
  * stride ld: bias the group's least weight, scale a 15th of its range. */

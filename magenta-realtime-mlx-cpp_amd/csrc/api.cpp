@@ -208,6 +208,7 @@ mrt::KvCache to_cache(const mrt_kv_cache* c, bool data = true) {
   k.dt = to_dtype(c->dtype);
   require(c->rows >= 0 && c->kv_heads >= 1 && c->capacity >= 1, "cache: rows >= 0, kv_heads >= 1 and capacity >= 1");
   require(c->d >= 8 && c->d <= mrt::kMaxHeadDim && c->d % 8 == 0, "cache: d must be a multiple of 8, 8..256");
+  require(c->capacity <= (1 << 30), "cache: capacity must be at most 2^30");
   require(static_cast<int64_t>(c->rows) * c->kv_heads <= (1 << 20), "cache: more than 2^20 (row, head) pairs");
   if (data) {
     require(c->k && c->v && c->length, "cache: null k, v or length");
@@ -242,6 +243,7 @@ void check_heads(const mrt::KvCache& c, int heads, int nodes) {
   require(heads >= 1 && heads % c.kv_heads == 0, "heads must be a multiple of kv_heads");
   require(heads <= 4096, "at most 4096 heads");
   require(nodes >= 1 && nodes <= mrt::kMaxNodes, "nodes must be in 1..64");
+  require(static_cast<int64_t>(c.rows) * heads * nodes < (1ll << 31), "rows * heads * nodes must be below 2^31");
 }
 
 void check_q4(int n, int k, int group) {
@@ -252,6 +254,7 @@ void check_q4(int n, int k, int group) {
 
 void check_bias(const float* bias, int buckets) {
   require(bias == nullptr || buckets >= 1, "bias without buckets");
+  require(bias == nullptr || buckets <= (1 << 18), "bias: at most 2^18 buckets");
   require(bias == nullptr || aligned(bias, 4), "bias must be 4-byte aligned");
 }
 
@@ -1015,9 +1018,10 @@ int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* arg
     }
     require(args->accepted != nullptr && args->accepted_stride >= 0, "cache_commit: null accepted or negative stride");
     require(args->accepted_n >= 1 && args->accepted_n <= mrt::kMaxNodes, "cache_commit: accepted_n must be in 1..64");
-    require(args->length_out != nullptr && args->length_out != c.length,
+    require(args->length_out != nullptr && args->length_out != c.length && args->length_out != c.next_pos &&
+                args->length_out != args->next_out,
             "cache_commit: length_out must be an array of its own");
-    require(c.pos == nullptr || (args->next_out != nullptr && args->next_out != c.next_pos),
+    require(c.pos == nullptr || (args->next_out != nullptr && args->next_out != c.next_pos && args->next_out != c.length),
             "cache_commit: next_out must be an array of its own");
     a.accepted = args->accepted, a.accepted_stride = args->accepted_stride, a.lse = args->lse, a.bias = args->bias;
     a.score_out = args->score_out, a.length_out = args->length_out, a.next_out = args->next_out;
@@ -1045,7 +1049,7 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
     const mrt::KvCache c = to_cache(cache);
     require(c.pos != nullptr && c.score != nullptr, "cache_evict: the cache needs pos, next_pos and score");
     require(args->score_out != nullptr && args->pos_out != nullptr, "cache_evict: null score_out or pos_out");
-    require(args->length_out != nullptr && args->length_out != c.length,
+    require(args->length_out != nullptr && args->length_out != c.length && args->length_out != c.next_pos,
             "cache_evict: length_out must be an array of its own");
     require(args->keep >= 1 && args->recent >= 0 && args->sinks >= 0 &&
                 static_cast<int64_t>(args->recent) + args->sinks <= args->keep,
@@ -1068,7 +1072,7 @@ int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const
     const mrt::DType dt = to_dtype(dtype);
     const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(dt));
     check_q4(n, k, group);
-    require(rows >= 0 && rows <= (1 << 20), "q4_matmul: rows must be in 0..2^20");
+    require(rows >= 0 && rows <= (1 << 19), "q4_matmul: rows must be in 0..2^19");
     require(x && w && scales && biases && out, "q4_matmul: null argument");
     require(aligned(x, 16) && aligned(w, 16), "q4_matmul: x and w must be 16-byte aligned");
     require(rows <= 1 || (ldx >= k && ldx % unit == 0), "q4_matmul: ldx must be >= k, a multiple of 16 bytes");

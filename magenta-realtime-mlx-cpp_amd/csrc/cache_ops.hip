@@ -105,7 +105,7 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
         for (int c = 0; c < KC; ++c) rows[t][c][lane] = x[c];
       }
       lse[t] = a.lse[((size_t)b * a.nodes + acc[tok[t]]) * a.heads + head[t]];
-      on[t] = row < R && lse[t] > -INFINITY;
+      on[t] = row < R && lse[t] != -INFINITY;
     }
     __syncthreads();
     for (int st = s0 + wid; st < s1; st += kCommitWaves) {

@@ -28,7 +28,9 @@ namespace mrt {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr float kNone = -1e30f;  // running maximum before any key: finite, so exp2(-inf - kNone) is 0
+// Running maximum before any key: finite, so exp2(-inf - kNone) is 0.  Logits below it count
+// as masked, and a row whose sum is 0 has nothing left.
+constexpr float kNone = -1e30f;
 constexpr int kBiasLds = 4096;   // floats of the bias by distance kept in LDS
 
 struct TreeArgs {
@@ -143,6 +145,7 @@ __device__ __forceinline__ void emit(const TreeArgs& a, bool whole, int64_t slot
                                      const float (&v)[E], float top, float sum, bool there) {
   const int n = a.heads / a.kv_heads, node = r / n, h = kvh * n + r - node * n;
   if (whole) {
+    there = there && sum != 0.f;
     const float inv = there ? 1.f / sum : 0.f;
     T* dst = static_cast<T*>(a.out) + b * a.o_row + node * a.o_node + h * a.o_head + d;
     union {
@@ -939,7 +942,7 @@ __global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, bool many, 
       for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], o, 64);
     }
     const int node = r / n, h = kvh * n + r - node * n;
-    const bool there = (present >> node) & 1;
+    const bool there = ((present >> node) & 1) && sum != 0.f;
     const float inv = 1.f / sum;
     if (d < a.D && from == 0) {
       T* dst = static_cast<T*>(a.out) + b * a.o_row + node * a.o_node + h * a.o_head + d;

@@ -28,6 +28,7 @@ BAD_CACHES = {
     "negative rows": dict(rows=-1), "no heads": dict(kv=0), "no slots": dict(cap=0), "odd d": dict(d=60),
     "wide d": dict(d=264), "no d": dict(d=0), "dtype": dict(dtype=3), "stride": dict(ss=68), "negative stride": dict(hs=-1024),
     "overlapping slots": dict(ss=32), "pos alone": dict(pos=P), "too many heads": dict(rows=1 << 12, kv=1 << 9),
+    "too long": dict(cap=(1 << 30) + 1),
 }
 
 
@@ -42,6 +43,7 @@ BAD_TREES = {
     "misaligned q": dict(q=P + 4), "stride": dict(qs=(1024, 250, 64)), "negative stride": dict(qs=(1024, 256, -64)),
     "no nodes": dict(nodes=0), "many nodes": dict(nodes=65), "heads": dict(heads=3), "no heads": dict(heads=0),
     "bias without buckets": dict(bias=P), "overlapping out": dict(os=(1024, 256, 0)), "parents stride": dict(ps=-4),
+    "too many buckets": dict(bias=P, buckets=(1 << 18) + 1),
 }
 
 
@@ -71,6 +73,13 @@ def test_tree_attention_refuses_null_and_small_workspaces(lib):
     refused(lib, lib.mrt_tree_attention(long, tree(), P, size.value - 1, 0, None))
     refused(lib, lib.mrt_tree_attention(long, tree(), P + 4, size.value, 0, None))
     assert lib.mrt_tree_attention_workspace(cache(cap=64), 4, 4, ctypes.byref(size)) == 0 and size.value == 0
+
+
+def test_tree_attention_refuses_more_rows_than_it_counts(lib):
+    many = cache(rows=1 << 20, kv=1, rs=0, hs=0)
+    refused(lib, lib.mrt_tree_attention(many, tree(nodes=64, heads=64), P, 1 << 40, 0, None))
+    size = ctypes.c_size_t()
+    refused(lib, lib.mrt_tree_attention_workspace(many, 64, 64, ctypes.byref(size)))
 
 
 def test_no_rows_is_no_work(lib):

@@ -145,6 +145,33 @@ def test_commit_ignores_unused_slots_and_scores_in_place():
         assert torch.equal(d["score"][b, :, :n].cpu(), clean["score"][b, :, :n])
 
 
+@pytest.mark.parametrize("masked", [-math.inf, float(torch.finfo(torch.float32).min)], ids=["inf", "lowest"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_commit_masks_in_the_bias(dtype, masked):
+    """Masked distances add nothing, nor does a head for which nothing is left."""
+    s = make_commit(31, dtype, 2, 6, 2, 64, 9, [300, 37], [[0, 1, 5], [2]], buckets=16)
+    plain = s["bias"].clone()
+    s["bias"][0, 3:], s["bias"][4] = -math.inf, -math.inf
+    s["lse"] = O.tree_attention(**{n: s[n] for n in ("q", "k_new", "v_new", "k", "v", "length", "parents", "scale", "bias",
+                                                     "pos", "next_pos")})[1].float()
+    assert (s["lse"][:, :, 4] == -math.inf).all()
+    got = commit(dict(s, bias=s["bias"].clamp(min=masked)))
+    ref = O.cache_commit(s["k"], s["v"], s["length"], s["k_new"], s["v_new"], s["accepted"], q=s["q"], lse=s["lse"],
+                         score=s["score"], score_out=s["score_out"], scale=s["scale"], bias=s["bias"])
+    big = float(s["scale"] * s["q"].double().norm(dim=-1).max() * max(s[n].double().norm(dim=-1).max() for n in ("k", "k_new")))
+    big += float(plain.abs().max()) + float(s["lse"][s["lse"] > -math.inf].abs().max())
+    rel = (64 + 8) * 2.0 ** -24 * big + 2.0 ** -21 + 10 * 2.0 ** -24
+    assert ((got["score"].double() - ref["score"]).abs() <= rel * ref["score"].abs()).all()
+
+
+def test_commit_lse_that_is_not_a_number():
+    """It makes the scores of the entries that its token sees NaN, as the formula says."""
+    s = make_commit(33, "bf16", 1, 4, 2, 64, 6, [50], [[1, 2, 4]])
+    s["lse"][0, 2, 1] = math.nan
+    got = commit(s)["score"][0]
+    assert got[0, :52].isnan().all() and not got[0, 52:].isnan().any() and not got[1].isnan().any()
+
+
 def make_evict(seed, dtype, rows, kv_heads, d, lengths, capacity=None, spread=True):
     g = torch.Generator().manual_seed(seed)
     cap = capacity or max(lengths) + 3

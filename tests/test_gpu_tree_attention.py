@@ -282,3 +282,22 @@ def test_long_cache_offsets():
         assert (lse[2, t].cpu().double() - total.log()).abs().max() < 1e-4
         ref = (e @ vals[:40 + t + 1]) / total[:, None]
         assert (out[2, t].cpu().double() - ref).norm() <= 5e-3 * ref.norm()
+
+
+@pytest.mark.parametrize("masked", [-math.inf, float(torch.finfo(torch.float32).min)], ids=["inf", "lowest"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("nodes,heads,lengths", [(4, 4, [40, 3]), (33, 4, [40, 3]), (9, 8, [3000, 5000]), (40, 8, [9000, 0])])
+def test_masks_in_the_bias(nodes, heads, lengths, dtype, masked):
+    """Distances of 5 and more are masked for one head, all of them for another: what is
+    left is as if the rest were not there, and a row with nothing left is 0, its lse -inf."""
+    s = make(41, dtype, 2, heads, 2, 64, nodes, lengths, buckets=8)
+    plain = s["bias"].clone()
+    s["bias"][0, 5:], s["bias"][1] = -math.inf, -math.inf
+    ref, rlse = oracle(s)
+    out, lse = call(dict(s, bias=s["bias"].clamp(min=masked)))
+    assert (out[:, :, 1] == 0).all() and (lse[:, :, 1] == -math.inf).all()
+    tol, ltol = bounds(dict(s, bias=plain), dtype)
+    rest = [h for h in range(heads) if h != 1]
+    err = (out.double() - ref).abs()[:, :, rest]
+    assert (err <= tol + torch.finfo(out.dtype).eps / 2 * (ref.abs()[:, :, rest] + tol)).all()
+    assert ((lse.double() - rlse).abs()[:, :, rest] <= ltol).all()
