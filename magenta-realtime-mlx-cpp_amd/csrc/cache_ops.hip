@@ -666,7 +666,7 @@ void cache_commit(const KvCache& c, const CommitArgs& t, hipStream_t s) {
   if (t.q.p != nullptr) {
     const int steps = (c.capacity + kStepKeys - 1) / kStepKeys + (t.accepted_n + kStepKeys - 1) / kStepKeys;
     const int want = std::max(1, 2048 / std::max(1, c.rows * c.kv_heads));
-    a.split_steps = std::max(2 * kCommitWaves, (steps + want - 1) / want);
+    a.split_steps = std::max(kCommitWaves, (steps + want - 1) / want);
     a.splits = (steps + a.split_steps - 1) / a.split_steps;
   }
   const int nr = t.q.p == nullptr || t.accepted_n * (t.heads / c.kv_heads) <= 16 ? 1 : 4;

@@ -65,12 +65,14 @@ __device__ __forceinline__ int own_chunk(const TreeArgs& a, int steps) {
 }
 
 // How the steps of all units (b, K/V head), in order, are cut into parts.  Long work
-// (16 least a team): team t has the steps [t total / teams, (t + 1) total / teams), which
+// (16 least a team): each unit counts kUnitCost steps more, before its own, for beginning
+// and ending it, and team t has the steps [t total / teams, (t + 1) total / teams), which
 // may end and begin inside units; part t of unit u leaves its result in slot u + t.
 // Short work: each unit is cut into parts of `chunk` steps, part t of all in slot t.
 // Either way there are at most teams + units slots.
+constexpr int kUnitCost = 8;
 struct Share {
-  int64_t total;
+  int64_t total;  // kUnitCost among it where chunk is 0
   int chunk;  // 0: by teams
 };
 // A value that all lanes hold, in scalar registers.
@@ -89,6 +91,7 @@ __device__ __forceinline__ Share share_of(const TreeArgs& a, int lane) {
   Share s;
   s.total = wave_sum64(sum) * a.kv_heads;
   s.chunk = s.total >= (int64_t)a.teams * a.least * 2 ? 0 : max(a.least, (int)((s.total + a.teams - 1) / a.teams));
+  if (s.chunk == 0) s.total += (int64_t)kUnitCost * a.rows * a.kv_heads;
   return s;
 }
 // The sequence whose units hold position `at` of the running sum of count(b) kv_heads,
@@ -521,10 +524,10 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
     } else {
       if (team >= a.teams) return;
       at = team * sh.total / a.teams, stop = (team + 1) * sh.total / a.teams;
-      b = find_row(a, lane, at, &before, [&](int x) { return steps_of(a, x); });
-      const int per = steps_of(a, b);
+      b = find_row(a, lane, at, &before, [&](int x) { return kUnitCost + steps_of(a, x); });
+      const int per = kUnitCost + steps_of(a, b);
       kvh = (int)((at - before) / per);
-      unit_at = before + (int64_t)kvh * per;
+      unit_at = before + (int64_t)kvh * per + kUnitCost;
     }
   }
   b = uniform(b), kvh = uniform(kvh), at = uniform(at), stop = uniform(stop), unit_at = uniform(unit_at);
@@ -532,7 +535,8 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   while (at < stop) {
     const int len = uniform(min(max(a.length[b], 0), a.capacity)), old_steps = (len + kStepKeys - 1) / kStepKeys;
     const int new_steps = (a.nodes + kStepKeys - 1) / kStepKeys, steps = new_steps + old_steps;
-    const int s0 = (int)(at - unit_at), s1 = (int)min((int64_t)steps, stop - unit_at);
+    const int s0 = (int)max(at - unit_at, (int64_t)0), s1 = (int)min((int64_t)steps, stop - unit_at);
+    if (s1 <= 0) break;  // the next team begins this unit
     const bool all = s0 == 0 && s1 == steps;
     const T* kc = static_cast<const T*>(a.k) + b * a.c_row + kvh * a.c_head;
     const T* vc = static_cast<const T*>(a.v) + b * a.c_row + kvh * a.c_head;
@@ -871,7 +875,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
     }
     at = unit_at + s1;
     if (s1 == steps) {
-      unit_at += steps;
+      unit_at += steps + kUnitCost;
       if (++kvh == a.kv_heads) kvh = 0, ++b;
     }
     __syncthreads();  // LDS may be written again
@@ -899,13 +903,13 @@ __global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, bool many, 
     const Share sh = share_of(a, lane);
     const int chunk = sh.chunk > 0 ? sh.chunk : many ? 0 : (int)((sh.total + a.teams - 1) / a.teams);
     int64_t before = 0;  // parts, or steps, of the sequences before
-    for (int x = lane; x < b; x += 64) before += chunk > 0 ? (steps_of(a, x) + chunk - 1) / chunk : steps_of(a, x);
+    for (int x = lane; x < b; x += 64) before += chunk > 0 ? (steps_of(a, x) + chunk - 1) / chunk : kUnitCost + steps_of(a, x);
     before = wave_sum64(before) * a.kv_heads;
     if (chunk > 0) {
       parts = (steps + chunk - 1) / chunk;
       first = before + (int64_t)kvh * parts;
     } else {
-      const int64_t at = before + (int64_t)kvh * steps, t0 = team_of(sh, a.teams, at);
+      const int64_t at = before + (int64_t)kvh * (kUnitCost + steps) + kUnitCost, t0 = team_of(sh, a.teams, at);
       parts = (int)(team_of(sh, a.teams, at + steps - 1) - t0) + 1;
       first = unit + t0;
     }
@@ -986,8 +990,8 @@ Plan plan(const KvCache& c, int heads, int nodes) {
   // more of them even out the lengths.
   p.least = 8;
   p.splits = 1;
-  p.teams = std::max(8, (p.many ? 256 : 1024) / p.row_blocks / 8 * 8);
-  if (steps * units <= (int64_t)p.teams * p.least * 2) {
+  p.teams = std::max(8, (p.many ? 256 : 512) / p.row_blocks / 8 * 8);
+  if (steps * units * p.row_blocks <= 32768) {
     p.splits = (int)std::max<int64_t>(1, std::min<int64_t>((steps + p.least - 1) / p.least, p.teams / units));
     p.teams = 0;
   }
