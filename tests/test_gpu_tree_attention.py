@@ -301,3 +301,25 @@ def test_masks_in_the_bias(nodes, heads, lengths, dtype, masked):
     err = (out.double() - ref).abs()[:, :, rest]
     assert (err <= tol + torch.finfo(out.dtype).eps / 2 * (ref.abs()[:, :, rest] + tol)).all()
     assert ((lse.double() - rlse).abs()[:, :, rest] <= ltol).all()
+
+
+BIG = [
+    # rows heads kv d nodes capacity lengths   work that is shared out by all lengths
+    (4, 4, 4, 64, 17, 70000, [60000, 0, 100, 9000]),               # cut anywhere, whole sequences in one part
+    (4, 4, 4, 64, 17, 70000, [900, 0, 100, 3]),                    # far less than the caches hold
+    (17, 8, 1, 64, 9, 63000, [50000, 3, 50000, 1, 50000] + [40 * i for i in range(12)]),  # halves, 72 rows
+    (4, 4, 4, 64, 1, 140000, [60000, 0, 100, 9000]),               # few rows
+    (4, 4, 4, 64, 1, 140000, [900, 0, 100, 3]),
+    (300, 4, 1, 64, 5, 4000, [(37 * i) % 700 for i in range(299)] + [4000]),   # more sequences than blocks at a time
+    (300, 1, 1, 64, 1, 4000, [(37 * i) % 700 for i in range(299)] + [4000]),
+]
+
+
+@pytest.mark.parametrize("case", BIG, ids=[f"r{c[0]}h{c[1]}n{c[4]}l{max(c[6])}" for c in BIG])
+def test_work_shared_out_by_lengths(case):
+    rows, heads, kv, d, nodes, cap, lengths = case
+    s = make(43, "bf16", rows, heads, kv, d, nodes, lengths, capacity=cap)
+    got = call(s)
+    check(s, "bf16", got)
+    again = call(s)
+    assert torch.equal(got[0], again[0]) and torch.equal(got[1], again[1])
