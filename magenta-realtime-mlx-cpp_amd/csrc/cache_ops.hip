@@ -16,7 +16,10 @@ namespace {
 // exp(scale q_i . k_j + bias - lse_i), for the entries at or before the token.  Reads
 // every key once (values not at all): 32 keys a step as attention does (attn_frag.hpp),
 // each lane summing its eight keys over row tiles, 16 lanes a row tile at the end.  The
-// rows (token, head) beyond 16 NR take another turn over the keys.  Accepted rows are
+// rows (token, head) beyond 16 NR take another turn over the keys.  Query rows wait in LDS,
+// as the lanes read them: in registers they cost a third of the waves (65 us instead of
+// 62).  Bound by the keys: 5 caches of up to 40001, 8 K/V heads, d 128, fp16 (242 MB) 62 us,
+// 3.9 TB/s.  Accepted rows are
 // copied by the first block of a head; all keys they are scored against come from
 // k_new, so that no block waits for another.
 
@@ -184,6 +187,9 @@ void launch_commit(const CommitK& a, int rows, int nr, hipStream_t s) {
 // collects its keys, k_evict_lists finds the other 22 bits from these in two passes, each
 // block by itself, and lists what moves: no block waits for another, and keys that are all
 // alike only make the collected ones more.
+// Bound: 64 x 16 heads from 1056 to 1006 entries, d 64 (43 MB), 18 us, one round of blocks
+// with five dependent steps; 4 x 8 heads from 65536 to 32768, d 128 (570 MB), 151 us, of
+// which 115 move rows at the rate of a copy and 37 find them (one block a head: 111).
 
 constexpr uint32_t kLowest = 0x007fffffu;  // of -inf; a NaN counts as that
 constexpr uint32_t kFixed = 0xffffffffu;   // entries that stay
@@ -217,7 +223,9 @@ __device__ __forceinline__ void move_row(const EvictK& a, int64_t base, int from
   *reinterpret_cast<uint4*>(vp + to * e) = y;
 }
 
-constexpr int kShortSlots = 2048;  // capacity up to which k_evict_short serves
+// Capacity up to which k_evict_short serves (what a wave has registers for): 1024 heads from
+// 2048 to 1900 42 us, with the kernels of long caches 57; 32 heads to 1024 23 and 21.
+constexpr int kShortSlots = 2048;
 constexpr int kShortList = 1024;   // rows that it moves itself
 
 // Four waves load and move; the first finds the threshold from KPT keys a lane, slot 64 t
@@ -636,11 +644,14 @@ __global__ __launch_bounds__(256) void k_evict_move(const EvictK a, int blocks, 
 // Most rows that a head can move; whether k_evict_short serves, and moves them itself.
 int most_moves(const KvCache& c, int keep) { return std::max(0, std::min(keep, c.capacity - keep)); }
 bool is_short(const KvCache& c) { return c.capacity <= kShortSlots; }
+// Up to 16 KB of K rows a head: 1024 heads from 1056 to 1006, d 64, 18.3 us, with a kernel of
+// its own for the moves 20.3; to 928 28.3 and 29.0; 32 heads to 928 12.7 and 14.5.
 bool moves_within(const KvCache& c, int keep) {
   return is_short(c) && (size_t)most_moves(c, keep) * c.d * dtype_size(c.dt) <= 16 * 1024;
 }
 // Slots of a part of a long cache: the smallest that leave no more parts than the card
-// takes at once, nor more than each block's sums over the parts' counts are worth.
+// takes at once, nor more than each block's sums over the parts' counts are worth: 8 heads of
+// 131072 with 8 / 16 / 32 parts 83 / 67 / 60 us, 32 of 65536 with 8 / 17 169 / 166.
 int part_slots(const KvCache& c) {
   const int heads = c.rows * c.kv_heads, parts = std::max(1, std::min(kMostParts, 1024 / std::max(1, heads)));
   const int64_t units = (c.capacity + (int64_t)kPartSlots - 1) / kPartSlots;
@@ -665,10 +676,13 @@ void cache_commit(const KvCache& c, const CommitArgs& t, hipStream_t s) {
   a.splits = 1, a.split_steps = 1 << 30;
   if (t.q.p != nullptr) {
     const int steps = (c.capacity + kStepKeys - 1) / kStepKeys + (t.accepted_n + kStepKeys - 1) / kStepKeys;
+    // A step for each wave at least (2 x 16 heads of 2048, d 64: 5.4 us, with two 6.5, with
+    // eight 13.3), and about eight blocks a CU (four to sixteen are the same).
     const int want = std::max(1, 2048 / std::max(1, c.rows * c.kv_heads));
     a.split_steps = std::max(kCommitWaves, (steps + want - 1) / want);
     a.splits = (steps + a.split_steps - 1) / a.split_steps;
   }
+  // 4 x 8 heads of 16384, d 128: 32 rows 35.5 us with four tiles, 49 with one; 16 rows 34 and 32
   const int nr = t.q.p == nullptr || t.accepted_n * (t.heads / c.kv_heads) <= 16 ? 1 : 4;
   MRT_DTYPE_DISPATCH(c.dt, {
     if (c.d <= 32) launch_commit<T, 32>(a, c.rows, nr, s);

@@ -15,6 +15,9 @@
 // turn, summed through LDS in order.  A lane loads 32 codes (16 bytes) of one row; two
 // exchanges between lane halves and two between quarters turn that into the operand
 // order in which each instruction's 32 k are consecutive, so within one group.
+// Reached: 2 x 1024 by 5632 (3.3 MB, bf16) 5 us, most of it one trip to memory and the sums
+// of the waves; 5 x 1024 by 29824 in fp32 (23.5 MB) 12 us; 9 x 8192 by 28672 (125 MB) 38 us,
+// 3.3 TB/s, bound by turning codes into operands between the loads.
 #include <algorithm>
 #include <type_traits>
 
@@ -28,8 +31,13 @@ namespace {
 constexpr int kQ4Waves = 8;
 constexpr int kChunk = 128;
 constexpr int kSlab = kQ4Waves * kChunk;      // k in LDS at a time: a chunk a wave
-constexpr size_t kTwoSlabs = 80 * 1024;       // LDS up to which a second slab saves a barrier
-constexpr int kFill = 256;                    // blocks that fill the card
+// LDS up to which a second slab saves a barrier, two blocks to a CU: 9 x 8192 by 28672 38.3
+// us instead of 40.7, 16 x 4096 by 8192 9.1 instead of 10.0.
+constexpr size_t kTwoSlabs = 80 * 1024;
+// Blocks that fill the card; with more, a block takes two or four column tiles and x is
+// read less often: 2 x 1024 by 8192 with one / two / four tiles 4.9 / 4.4 / 5.7 us, by 29824
+// one / four 13.3 / 9.7, 9 x 8192 by 28672 47.7 / 38.8, 40 x 4096 by 16384 one / two 57 / 44.
+constexpr int kFill = 256;
 
 struct Q4Args {
   const uint32_t* w;

@@ -14,6 +14,13 @@
 //   k_tree_many (16-bit, d 64 or 128): eight waves, WR of them on different rows and
 //   8 / WR on different steps, share K and V through a ring of LDS stages that loads
 //   fill while products run.
+// What they reach (bf16; one pass of the call, the joining of parts among it): 3 sequences
+// of up to 65500 entries, 8 K/V heads, d 128, 60 rows (461 MB) 103 us, 4.5 TB/s, near the
+// rate of a large copy; 16 of up to 8191, 4 K/V heads, 512 rows (79 GFLOP, half as much again
+// for weights in two parts) 152 us, bound by the softmax between the products (187 vector
+// instructions a wave and step against 48 matrix ones); fp32, 4 of up to 4099, 12 heads, 7
+// rows (58 MB) 25 us, bound by a few dependent trips to memory; one node over 49 entries
+// 8 us of such trips.
 // A unit's steps are cut where the card needs more blocks (Share); parts leave (maximum,
 // sum, output) in fp32 and k_tree_join sums them in order, so a result does not depend
 // on timing.  The cut is made on the device, from the lengths, which the host never sees.
@@ -70,6 +77,8 @@ __device__ __forceinline__ int own_chunk(const TreeArgs& a, int steps) {
 // may end and begin inside units; part t of unit u leaves its result in slot u + t.
 // Short work: each unit is cut into parts of `chunk` steps, part t of all in slot t.
 // Either way there are at most teams + units slots.
+// Without that cost, 8 heads of 65500 entries beside 16 of 100 took 159 us (60 rows, d 128),
+// the last team beginning and ending most of the short ones; with it 85.
 constexpr int kUnitCost = 8;
 struct Share {
   int64_t total;  // kUnitCost among it where chunk is 0
@@ -980,14 +989,24 @@ struct Plan {
 Plan plan(const KvCache& c, int heads, int nodes) {
   const int R = nodes * (heads / c.kv_heads), dp = c.d <= 32 ? 32 : c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
   Plan p;
+  // Times in us, bf16, 4 sequences, 8 K/V heads, d 128 unless said otherwise.
+  // 24 rows, 16384 entries: 61 by k_tree_many, 103 by k_tree_few; 16 rows 61 and 58.
+  // Row tiles 2 / 4 / 8 / 16 over 8192 entries: 64 rows 47 / 41 / 49 / 69, 256 rows
+  // 111 / 85 / 84 / 79.
   p.many = R > 16 && c.dt != DType::F32 && (c.d == 64 || c.d == 128);
   p.tiles = p.many ? (R <= 32 ? 2 : R <= 64 ? 4 : R <= 128 ? 8 : 16)
                    : std::min(row_tiles(dtype_size(c.dt), dp), R <= 16 ? 1 : R <= 32 ? 2 : 4);
   p.row_blocks = (R + 16 * p.tiles - 1) / (16 * p.tiles);
   const int64_t steps = (c.capacity + kStepKeys - 1) / kStepKeys + (nodes + kStepKeys - 1) / kStepKeys;
   const int64_t units = std::max<int64_t>(1, (int64_t)c.rows * c.kv_heads);
-  // k_tree_many fills a CU with a block; of the others a CU holds a few at a time, and
-  // more of them even out the lengths.
+  // k_tree_many fills a CU with a block (128 / 256 / 512 teams for 64 rows, 16384 entries:
+  // 76 / 64 / 76), of k_tree_few a CU holds two (256 / 512 / 1024 parts for one node: 60 / 58 /
+  // 62).  Parts of 8 steps at least: one node over 1000 entries, d 64, with 4 / 8 / 16 / 32
+  // steps 11.5 / 11.6 / 13.3 / 19.1.
+  // Up to 32768 steps the units are cut by themselves: 300 sequences of 2048, one K/V head,
+  // 76 against 95 shared out by all lengths (k_tree_few), 51 against 58 (k_tree_many, d 64).
+  // Beyond, unequal lengths would cost more than that: 32 sequences of 100 and one of 8192,
+  // one node, 25 shared out and 71 by themselves (32 of 8192: 191 and 186).
   p.least = 8;
   p.splits = 1;
   p.teams = std::max(8, (p.many ? 256 : 512) / p.row_blocks / 8 * 8);
@@ -1093,6 +1112,7 @@ void tree_attention(const KvCache& c, const TreeAttnArgs& t, void* ws, hipStream
   if (cuts(p)) {
     const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64, units = c.rows * c.kv_heads;
     MRT_DTYPE_DISPATCH(c.dt, {
+      // one row a wave or four: 1056 rows 16.1 us and 21.2 with the attention, 32768 rows 232 and 228
       if ((int64_t)units * R < 16384)
         hipLaunchKernelGGL((k_tree_join<T, 1>), dim3(units * ((R + 3) / 4)), dim3(256), 0, s, a, p.many, cols);
       else
