@@ -210,7 +210,7 @@ mrt::KvCache to_cache(const mrt_kv_cache* c, bool data = true) {
   require(c->d >= 8 && c->d <= mrt::kMaxHeadDim && c->d % 8 == 0, "cache: d must be a multiple of 8, 8..256");
   require(c->capacity <= (1 << 30), "cache: capacity must be at most 2^30");
   require(static_cast<int64_t>(c->rows) * c->kv_heads <= (1 << 20), "cache: more than 2^20 (row, head) pairs");
-  if (data) {
+  if (data && c->rows > 0) {
     require(c->k && c->v && c->length, "cache: null k, v or length");
     require(aligned(c->k, 16) && aligned(c->v, 16), "cache: k and v must be 16-byte aligned");
     const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(k.dt));
@@ -237,6 +237,12 @@ mrt::NodeRows to_nodes(const mrt_node_rows& r, const mrt::KvCache& c, int nodes,
   mrt::NodeRows n;
   n.p = r.data, n.row_stride = r.row_stride, n.node_stride = r.node_stride, n.head_stride = r.head_stride;
   return n;
+}
+
+// Of a cache that is written.
+void check_own_slots(const mrt::KvCache& c) {
+  require((c.rows == 1 || c.row_stride > 0) && (c.kv_heads == 1 || c.head_stride > 0),
+          "cache: sequences or heads share their slots");
 }
 
 void check_heads(const mrt::KvCache& c, int heads, int nodes) {
@@ -980,6 +986,7 @@ int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args*
   return guarded([&] {
     require(args != nullptr, "null argument");
     const mrt::KvCache c = to_cache(cache);
+    if (c.rows == 0) return;
     check_heads(c, args->heads, args->nodes);
     check_bias(args->bias, args->buckets);
     mrt::TreeAttnArgs a;
@@ -997,7 +1004,6 @@ int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args*
     const size_t want = mrt::tree_attention_workspace(c, a.heads, a.nodes);
     require(want == 0 || (workspace != nullptr && workspace_bytes >= want && aligned(workspace, 16)),
             "tree_attention: workspace too small, misaligned or null");
-    if (c.rows == 0) return;
     OnDevice on(device);
     mrt::tree_attention(c, a, workspace, static_cast<hipStream_t>(hip_stream));
   });
@@ -1007,8 +1013,10 @@ int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* arg
   return guarded([&] {
     require(args != nullptr, "null argument");
     const mrt::KvCache c = to_cache(cache);
+    if (c.rows == 0) return;
     check_heads(c, args->heads, args->nodes);
     check_bias(args->bias, args->buckets);
+    check_own_slots(c);
     mrt::CommitArgs a;
     a.k_new = to_nodes(args->k_new, c, args->nodes, c.kv_heads, "cache_commit: null k_new");
     a.v_new = to_nodes(args->v_new, c, args->nodes, c.kv_heads, "cache_commit: null v_new");
@@ -1027,7 +1035,6 @@ int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* arg
     a.score_out = args->score_out, a.length_out = args->length_out, a.next_out = args->next_out;
     a.accepted_n = args->accepted_n, a.nodes = args->nodes, a.heads = args->heads;
     a.buckets = args->bias ? args->buckets : 0, a.scale = args->scale;
-    if (c.rows == 0) return;
     OnDevice on(device);
     mrt::cache_commit(c, a, static_cast<hipStream_t>(hip_stream));
   });
@@ -1047,6 +1054,8 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
   return guarded([&] {
     require(args != nullptr, "null argument");
     const mrt::KvCache c = to_cache(cache);
+    if (c.rows == 0) return;
+    check_own_slots(c);
     require(c.pos != nullptr && c.score != nullptr, "cache_evict: the cache needs pos, next_pos and score");
     require(args->score_out != nullptr && args->pos_out != nullptr, "cache_evict: null score_out or pos_out");
     require(args->length_out != nullptr && args->length_out != c.length && args->length_out != c.next_pos,
@@ -1060,7 +1069,6 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
     mrt::EvictArgs a;
     a.score_out = args->score_out, a.pos_out = args->pos_out, a.length_out = args->length_out;
     a.keep = args->keep, a.recent = args->recent, a.sinks = args->sinks;
-    if (c.rows == 0) return;
     OnDevice on(device);
     mrt::cache_evict(c, a, workspace, static_cast<hipStream_t>(hip_stream));
   });
@@ -1073,11 +1081,11 @@ int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const
     const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(dt));
     check_q4(n, k, group);
     require(rows >= 0 && rows <= (1 << 19), "q4_matmul: rows must be in 0..2^19");
+    if (rows == 0) return;
     require(x && w && scales && biases && out, "q4_matmul: null argument");
     require(aligned(x, 16) && aligned(w, 16), "q4_matmul: x and w must be 16-byte aligned");
     require(rows <= 1 || (ldx >= k && ldx % unit == 0), "q4_matmul: ldx must be >= k, a multiple of 16 bytes");
     require(rows <= 1 || ldo >= n, "q4_matmul: ldo must be >= n");
-    if (rows == 0) return;
     mrt::Q4Weights q;
     q.w = w, q.scales = scales, q.biases = biases, q.n = n, q.k = k, q.group = group;
     OnDevice on(device);

@@ -84,6 +84,26 @@ def test_tree_attention_refuses_more_rows_than_it_counts(lib):
 
 def test_no_rows_is_no_work(lib):
     assert lib.mrt_tree_attention(cache(rows=0), tree(), None, 0, 0, None) == 0
+    empty = cache(rows=0, k=0, v=0, length=0)  # as an empty tensor's pointers are
+    assert lib.mrt_tree_attention(empty, tree(q=0, k=0, v=0, out=0, parents=0, lse=0), None, 0, 0, None) == 0
+    assert lib.mrt_cache_commit(empty, commit(k=0, v=0, q=0, accepted=0, length_out=0), 0, None) == 0
+    assert lib.mrt_cache_evict(empty, evict(score_out=0, pos_out=0, length_out=0), None, 0, 0, None) == 0
+    assert lib.mrt_q4_matmul(None, 64, 0, None, None, None, 64, 64, 64, 1, None, 64, 0, None) == 0
+
+
+def test_writes_refuse_caches_that_share_slots(lib):
+    full = dict(pos=P, next_pos=P, score=P)
+    for bad in (dict(rs=0), dict(hs=0)):
+        refused(lib, lib.mrt_cache_commit(cache(**bad), commit(), 0, None))
+        refused(lib, lib.mrt_cache_evict(cache(**bad, **full), evict(), P, 1 << 20, 0, None))
+
+
+def test_outputs_of_their_own(lib):
+    positions = dict(pos=P, next_pos=P + 128)
+    refused(lib, lib.mrt_cache_commit(cache(**positions), commit(length_out=P + 128, next_out=P + 256), 0, None))
+    refused(lib, lib.mrt_cache_commit(cache(**positions), commit(length_out=P + 256, next_out=P + 256), 0, None))
+    refused(lib, lib.mrt_cache_commit(cache(**positions), commit(next_out=P), 0, None))
+    refused(lib, lib.mrt_cache_evict(cache(score=P, **positions), evict(length_out=P + 128), P, 1 << 20, 0, None))
 
 
 def test_binding_refuses_cpu_tensors_and_wrong_shapes():
