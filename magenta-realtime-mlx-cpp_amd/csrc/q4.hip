@@ -17,7 +17,8 @@
 // order in which each instruction's 32 k are consecutive, so within one group.
 // Reached: 2 x 1024 by 5632 (3.3 MB, bf16) 5 us, most of it one trip to memory and the sums
 // of the waves; 5 x 1024 by 29824 in fp32 (23.5 MB) 12 us; 9 x 8192 by 28672 (125 MB) 38 us,
-// 3.3 TB/s, bound by turning codes into operands between the loads.
+// 3.3 TB/s: a block a CU (its registers), whose loads and products take turns.  Two blocks
+// by fewer registers spill (47 us), codes two slabs ahead gain nothing (43).
 #include <algorithm>
 #include <type_traits>
 
