@@ -87,9 +87,10 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
   const int R = n * nh;
   const float* score = a.score == nullptr ? nullptr : a.score + (size_t)bg * a.capacity;
   float* score_out = a.score_out + (size_t)bg * a.capacity;
-  if (R == 0) {
-    if (score != nullptr && score != score_out)
-      for (int j = s0 * kStepKeys + tid; j < min(len, s1 * kStepKeys); j += 64 * kCommitWaves) score_out[j] = score[j];
+  if (R == 0) {  // nothing accepted: the scores stay, 0 where there were none
+    if (score != score_out)
+      for (int j = s0 * kStepKeys + tid; j < min(len, s1 * kStepKeys); j += 64 * kCommitWaves)
+        score_out[j] = score == nullptr ? 0.f : score[j];
     return;
   }
   __shared__ uint4 rows[NR][KC][64];  // q, as the lanes read it

@@ -104,6 +104,22 @@ def test_commit_without_weights_and_first_scores():
     check_commit(s, commit(s))
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("old_scores", [False, True], ids=["first", "later"])
+def test_commit_writes_the_scores_of_sequences_that_accept_nothing(dtype, old_scores):
+    """All drafts rejected, a full cache, an empty one: their scores are the old ones, 0 where
+    there were none, and not what score_out held."""
+    acc = [[], [0, 2], [3], [], [1, 4]]
+    s = make_commit(35, dtype, 5, 4, 2, 64, 5, [300, 7, 310, 0, 45], acc, capacity=310, old_scores=old_scores)
+    got = commit(s)
+    assert got["length"].tolist() == [300, 9, 310, 0, 47]
+    check_commit(s, got)
+    for b in (0, 2):
+        n = int(s["length"][b])
+        assert torch.equal(got["score"][b, :, :n], s["score"][b, :, :n] if old_scores else torch.zeros(2, n))
+        assert (got["score"][b, :, n:] == -7).all()
+
+
 def test_commit_stops_where_the_path_does():
     """Descending, repeated and foreign ids end the path, and so does a full cache."""
     acc = [[0, 3, 3, 4], [2, 1, 4, -1], [1, 5, -1, -1], [-1, 0, 1, 2], [1, 2, 4, -1], [0, 1, 2, 3]]
