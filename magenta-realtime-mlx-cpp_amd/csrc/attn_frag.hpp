@@ -246,6 +246,11 @@ struct AttnFrag {
 __device__ __forceinline__ int step_key(int i, int half) { return i + 16 * half; }
 __device__ __forceinline__ int lane_key(int g, int j) { return 4 * g + (j & 3) + (j >> 2) * 16; }
 
+// The factor 2^x, x <= 0, by which sums and outputs follow a larger maximum.  At least the
+// smallest normal number: 0 would make NaN of an infinite value, whose weight is small but
+// not 0; finite sums, of at least 2^-8, take in 2^-126 of others without a trace.
+__device__ __forceinline__ float fade(float x) { return fmaxf(__builtin_amdgcn_exp2f(x), 0x1p-126f); }
+
 // One step of the running softmax of NR row tiles: s, the logits in log2 units (-inf
 // where masked), become weights exp2(s - m); m, l and o follow.  m is the maximum less
 // `shift`, uniform over the lanes of a row; l stays a sum of the lane's own keys.
@@ -259,7 +264,7 @@ __device__ __forceinline__ void running_softmax(float (&s)[NR][8], float (&m)[NR
     for (int j = 1; j < 8; ++j) top = fmaxf(top, s[t][j]);
     top = max_over_groups(top) - shift;
     if (__any(top > m[t])) {
-      const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
+      const float mn = fmaxf(m[t], top), f = fade(m[t] - mn);
       m[t] = mn;
       l[t] *= f;
 #pragma unroll

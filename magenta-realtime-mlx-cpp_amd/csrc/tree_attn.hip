@@ -72,7 +72,7 @@ __device__ __forceinline__ int own_chunk(const TreeArgs& a, int steps) {
 }
 
 // How the steps of all units (b, K/V head), in order, are cut into parts.  Long work
-// (16 least a team): each unit counts kUnitCost steps more, before its own, for beginning
+// (2 least, 16 steps, a team): each unit counts kUnitCost steps more, before its own, for beginning
 // and ending it, and team t has the steps [t total / teams, (t + 1) total / teams), which
 // may end and begin inside units; part t of unit u leaves its result in slot u + t.
 // Short work: each unit is cut into parts of `chunk` steps, part t of all in slot t.
@@ -395,7 +395,7 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
     float top = ml[0][t * 16 + i].x;
 #pragma unroll
     for (int w = 1; w < kWaves; ++w) top = fmaxf(top, ml[w][t * 16 + i].x);
-    const float f = __builtin_amdgcn_exp2f(m[t] - top);
+    const float f = fade(m[t] - top);
 #pragma unroll
     for (int e = 0; e < E; ++e) buf[((wid * NR + t) * E + e) * 64 + lane] = o[t][e] * f;
   }
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
                               mult -
                           kShift;
         if (__any(top > m[t] + kSlack)) {
-          const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
+          const float mn = fmaxf(m[t], top), f = fade(m[t] - mn);
           m[t] = mn;
           l[t] *= f;
 #pragma unroll
@@ -854,7 +854,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         float top = ml[0][x].x;
 #pragma unroll
         for (int w = 1; w < WK; ++w) top = fmaxf(top, ml[w][x].x);
-        const float f = __builtin_amdgcn_exp2f(m[t] - top);
+        const float f = fade(m[t] - top);
 #pragma unroll
         for (int e = 0; e < E; ++e) buf[((wid * NR + t) * E + e) * 64 + lane] = o[t][e] * f;
       }
@@ -935,9 +935,9 @@ __global__ __launch_bounds__(256) void k_tree_join(const TreeArgs a, bool many, 
     float top = kNone, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
     for (int s0 = 0; s0 < parts; s0 += 64) {
       const float2 y = s0 + lane < parts ? ml[(size_t)(s0 + lane) * R] : make_float2(kNone, 0.f);
-      const float to = fmaxf(top, wave_max(y.x)), f = __builtin_amdgcn_exp2f(top - to);
+      const float to = fmaxf(top, wave_max(y.x)), f = fade(top - to);
       top = to;
-      const float w = s0 + lane < parts ? __builtin_amdgcn_exp2f(y.x - top) : 0.f;
+      const float w = s0 + lane < parts ? fade(y.x - top) : 0.f;
       sum = fmaf(sum, f, wave_sum(y.y * w));
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] *= f;

@@ -1,0 +1,75 @@
+"""Infinities, NaN and masks of tree attention, in every form of its kernels.
+
+What an output is follows from the definition, out = sum of w v over the entries that are
+not masked, each w > 0 however small: an infinite v makes it that infinity, two opposite
+ones or a NaN make it NaN, and what is masked has no part in it, whatever it holds.
+Finite outputs have the tolerances of test_gpu_tree_attention.
+"""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import mrt_df
+from oracle import drafting_oracle as O
+from test_gpu_tree_attention import DEV, DT, bounds, call, make, oracle
+
+pytestmark = pytest.mark.gpu
+
+FORMS = [
+    # heads kv d nodes lengths capacity   which kernel, and how its work is cut
+    (4, 4, 64, 1, [40], None),          # few rows, one block a unit
+    (4, 4, 64, 3, [3000], None),        # ... cut
+    (3, 1, 24, 7, [300], None),         # ... other head sizes
+    (2, 1, 128, 20, [700], None),       # two, four and eight row tiles (16-bit), d 128
+    (2, 1, 256, 9, [700], None),
+    (2, 2, 64, 25, [40], None),         # d 64: two, four, eight, sixteen row tiles; whole and cut
+    (2, 2, 64, 25, [3000], None),
+    (2, 1, 64, 25, [900], None),
+    (4, 1, 64, 25, [900], None),
+    (8, 1, 64, 25, [40], None),
+    (8, 1, 128, 25, [2000], None),
+    (8, 2, 128, 25, [900], None),
+    (4, 4, 64, 17, [9000, 0, 400], 70000),   # shared out by all lengths
+    (4, 4, 64, 1, [9000, 0, 400], 140000),
+]
+IDS = [f"h{f[0]}kv{f[1]}d{f[2]}n{f[3]}l{f[4][0]}c{f[5] or 0}" for f in FORMS]
+
+
+def form(seed, dtype, f, **kw):
+    heads, kv, d, nodes, lengths, cap = f
+    return make(seed, dtype, len(lengths), heads, kv, d, nodes, lengths, capacity=cap, **kw)
+
+
+def finite_check(s, dtype, out, ref, where):
+    tol, _ = bounds(s, dtype)
+    lim = tol + torch.finfo(out.dtype).eps / 2 * (ref.abs() + tol)
+    assert ((out.double() - ref).abs() <= lim)[where].all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("f", FORMS, ids=IDS)
+def test_infinite_nodes_stay_beside_a_dominating_entry(f, dtype):
+    """An ancestor's infinite value stays, though a cached key outweighs it by some 150 powers
+    of e, so that its weight beside the key's is far below what fp32 holds."""
+    s = form(51, dtype, f)
+    s["v_new"][0, 0, :, 3] = math.inf
+    s["v_new"][0, 0, :, 5] = -math.inf
+    s["parents"][0] = torch.arange(-1, f[3] - 1, dtype=torch.int32)  # a chain: all see node 0
+    s["q"][0] = s["q"][0].abs() * 0.5 + 0.5
+    big = 150 / (s["scale"] * f[2] * 0.5)  # every q is at least 0.5 in every dimension
+    s["k"][0, :, s["length"][0] - 1] = big
+    assert (s["scale"] * (s["q"][0].double().sum(-1) * big)).min() > 150
+    out, lse = call(s)
+    ref, rlse = oracle(s)
+    assert (out[0, :, :, 3] == math.inf).all() and (out[0, :, :, 5] == -math.inf).all()
+    fin = torch.ones(out.shape[-1], dtype=torch.bool)
+    fin[3], fin[5] = False, False
+    assert torch.isfinite(out[0][..., fin]).all() and torch.isfinite(lse[0]).all()
+    # the dominating entry's values, to the type's last digit and the logits' own
+    want = s["v"][0, :, s["length"][0] - 1].double().repeat_interleave(f[0] // f[1], 0)[None].expand_as(out[0])
+    err = (out[0].double() - want).abs()[..., fin]
+    assert (err <= (torch.finfo(out.dtype).eps / 2 + 2.0 ** -16) * want.abs()[..., fin]).all()
