@@ -670,7 +670,9 @@ typedef struct mrt_tree_attention_args {
  * -inf, or below -1e30 (a bias of the type's lowest value), is a mask; a row
  * with nothing left has output 0 and lse -inf.  One node is an ordinary decode
  * step.  K/V of a node that t does not see have no effect on
- * t, whatever they hold.  Does not write the cache: mrt_cache_commit takes the
+ * t, whatever they hold; an infinite value that t does see makes the output
+ * that infinity however small its weight, opposite ones or a NaN make it NaN.
+ * Does not write the cache: mrt_cache_commit takes the
  * accepted nodes into it.  mrt_tree_attention_workspace gives the workspace
  * bytes for these sizes (0: none; workspace may then be NULL). */
 int mrt_tree_attention_workspace(const mrt_kv_cache* cache, int heads, int nodes, size_t* bytes);

@@ -151,6 +151,17 @@ __device__ __forceinline__ uint64_t ancestors(const int* parents, int nodes, int
   return bad ? 0ull : mask;
 }
 
+// Whether a row's sum and outputs are numbers.
+template <int E>
+__device__ __forceinline__ bool all_finite(float l, const f32x4_t (&o)[E]) {
+  float top = fabsf(l);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) top = fmaf(0.f, o[e][r], top);  // NaN from either
+  return top < INFINITY;
+}
+
 // E consecutive outputs of row r from dimension d on: to `out`, or, of a part, to its slot.
 template <typename T, int E>
 __device__ __forceinline__ void emit(const TreeArgs& a, bool whole, int64_t slot, int b, int kvh, int r, int d,
@@ -192,8 +203,14 @@ __device__ __forceinline__ void emit(const TreeArgs& a, bool whole, int64_t slot
   }
 }
 
+// Blocks of k_tree_few that a CU holds at least: its registers without the rare second
+// round of steps would let it hold as many.
+constexpr int few_blocks(size_t elt, int dp, int nr) {
+  return elt == 4 ? 1 : dp == 32 ? (nr == 1 ? 4 : nr == 2 ? 3 : 2) : dp * nr <= 128 ? 2 : 1;
+}
+
 template <typename T, int DP, int NR>
-__global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
+__global__ __launch_bounds__(64 * kWaves, few_blocks(sizeof(T), DP, NR)) void k_tree_few(const TreeArgs a) {
   using F = AttnFrag<T, DP>;
   constexpr int E = F::E, VW = F::VW, KC = F::KC;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -251,6 +268,12 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
     }
   };
   load(s0 + wid);
+  // Of cached step `st` or the nodes', element j of V once more.
+  auto load_v = [&](bool fresh, int key, uint32_t (&f)[VW]) {
+    F::load_v(fresh ? static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head + (int64_t)key * a.vn_node
+                    : vc + (int64_t)key * a.c_slot,
+              i, D, f);
+  };
 
   const int len = min(max(a.length[b], 0), a.capacity), old_steps = (len + kStepKeys - 1) / kStepKeys;
   if (a.teams == 0 && a.splits == 1) s1 = steps = new_steps + old_steps;
@@ -288,17 +311,23 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
 
   f32x4_t o[NR][E];
   float m[NR], l[NR];
+  auto begin = [&] {
 #pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    m[t] = kNone, l[t] = 0.f;
+    for (int t = 0; t < NR; ++t) {
+      m[t] = kNone, l[t] = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
-  }
+      for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  begin();
   const float scale2 = a.scale * kLog2e;
   // fp16 weights reach up to 2^15, so that those far below the maximum keep their bits.
   constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;
 
-  for (int st = s0 + wid; st < s1; st += kWaves) {
+  // One step.  A matrix product makes NaN of 0 * inf, and of infinities whose weight is in
+  // two parts: a node's infinities and NaN, which others may not see, are left out of it and
+  // added by class; with `exact`, the cache's are too.
+  auto step = [&](int st, auto exact) {
     const bool fresh = st < new_steps;
     const int base = (fresh ? st : st - new_steps) * kStepKeys, end = fresh ? a.nodes : len;
     const bool whole = base + kStepKeys <= end;
@@ -339,12 +368,19 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
         for (int j = 0; j < 8; ++j) p[t][j] = base + lane_key(g, j) < end ? p[t][j] : -INFINITY;
       }
     }
+    uint32_t seen[NR];  // the keys that the row does not mask, a bit each
+    if (fresh || exact.value) {
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        seen[t] = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) seen[t] |= p[t][j] < kNone ? 0u : 1u << j;
+      }
+    }
     running_softmax<NR, E>(p, m, l, o, kShift);
-    if (!fresh) {
+    if (!fresh && !exact.value) {
       F::template add_pv<NR>(vf, p, o);
     } else {
-      // A node's infinities and NaN belong to those who see it: 0 * inf is NaN in a
-      // matrix product, so they are left out of it and added by class.
       uint32_t diff = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -355,21 +391,19 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
           vf[j][w] = x;
         }
       F::template add_pv<NR>(vf, p, o);
-      if (__any(diff != 0)) {
+      if (__builtin_expect(__any(diff != 0), 0)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int key = base + lane_key(g, j);
-          F::load_v(static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head + (int64_t)min(key, end - 1) * a.vn_node, i,
-                    D, vf[j]);
+          load_v(fresh, min(key, end - 1), vf[j]);
 #pragma unroll
           for (int w = 0; w < VW; ++w) vf[j][w] = key < end ? F::classes(vf[j][w]) : 0u;
         }
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
-          const uint64_t see = sees[min(row0 + t * 16 + i, R - 1) / n] >> base;
           float one[8];
 #pragma unroll
-          for (int j = 0; j < 8; ++j) one[j] = (see >> lane_key(g, j)) & 1 ? 1.f : 0.f;
+          for (int j = 0; j < 8; ++j) one[j] = (seen[t] >> j) & 1 ? 1.f : 0.f;
 #pragma unroll
           for (int e = 0; e < E; ++e) {
             const f32x4_t c = F::count(vf, one, e);
@@ -379,7 +413,21 @@ __global__ __launch_bounds__(64 * kWaves, 1) void k_tree_few(const TreeArgs a) {
         }
       }
     }
+  };
+  for (int st = s0 + wid; st < s1; st += kWaves) {
+    step(st, std::false_type{});
     if (st + kWaves < s1) load(st + kWaves);
+  }
+  bool odd = false;
+#pragma unroll
+  for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]);
+  if (__builtin_expect(__any(odd), 0)) {  // rare: this wave's steps once more
+    begin();
+#pragma unroll 1
+    for (int st = s0 + wid; st < s1; st += kWaves) {
+      load(st);
+      step(st, std::true_type{});
+    }
   }
 
   // Join the waves: outputs at the common maximum, summed through LDS.
@@ -607,12 +655,15 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
 
     f32x4_t o[NR][E];  // [t][e][r]: dimension 16 e + 4 g + r of row i of tile t
     float m[NR], l[NR];
+    auto begin = [&] {
 #pragma unroll
-    for (int t = 0; t < NR; ++t) {
-      m[t] = kNone, l[t] = 0.f;
+      for (int t = 0; t < NR; ++t) {
+        m[t] = kNone, l[t] = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
-    }
+        for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
+      }
+    };
+    begin();
 
     // A step: where its keys are, whether they are nodes, and whether all 32 count for all.
     struct Step {
@@ -634,6 +685,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
     };
     f32x4_t x[NR], y[NR];  // Q K^T of a step
     uint4 ph[NR], pl[NR];  // its weights
+    uint32_t seen[NR];     // with `exact`: the keys that the row does not mask, a bit each
     uint32_t left_out = 0;  // nonzero: infinities or NaN among the nodes' values
     auto scores = [&](const Step& p) {
       const uint32_t stage = p.stage;
@@ -656,12 +708,14 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
           }
       }
     };
-    auto weights = [&](const Step& w) {
+    auto weights = [&](const Step& w, auto only) {  // of all row tiles, or with `exact` of one
+      constexpr bool exact = only.value >= 0;
+      constexpr int t0 = exact ? only.value : 0, t1 = exact ? t0 + 1 : NR;
       const bool fresh = w.fresh, plain = w.plain;
       const int base = w.base, end = w.end;
       float z[NR][8];
 #pragma unroll
-      for (int t = 0; t < NR; ++t)
+      for (int t = t0; t < t1; ++t)
 #pragma unroll
         for (int j = 0; j < 4; ++j) z[t][j] = x[t][j], z[t][4 + j] = y[t][j];
       if constexpr (BIAS) {
@@ -673,7 +727,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
           kpos[j] = fresh ? __popcll(sees[key]) - 1 : pos != nullptr ? pos[key] : key;
         }
 #pragma unroll
-        for (int t = 0; t < NR; ++t) {
+        for (int t = t0; t < t1; ++t) {
           const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
           const int qp = (fresh ? 0 : first_pos) + max(__popcll(sees[node]) - 1, 0);
           const float* row = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
@@ -684,15 +738,23 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
       }
       if (!plain) {
 #pragma unroll
-        for (int t = 0; t < NR; ++t) {
+        for (int t = t0; t < t1; ++t) {
           const uint64_t see = fresh ? sees[min(row0 + t * 16 + i, R - 1) / n] >> base : ~0ull;
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             z[t][j] = base + lane_key(g, j) < end && (see >> lane_key(g, j)) & 1 ? z[t][j] : -INFINITY;
         }
       }
+      if constexpr (exact) {
 #pragma unroll
-      for (int t = 0; t < NR; ++t) {
+        for (int t = t0; t < t1; ++t) {
+          seen[t] = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) seen[t] |= z[t][j] * mult < kNone ? 0u : 1u << j;
+        }
+      }
+#pragma unroll
+      for (int t = t0; t < t1; ++t) {
         const float top = max_over_groups(fmaxf(fmaxf(fmaxf(z[t][0], z[t][1]), fmaxf(z[t][2], z[t][3])),
                                                 fmaxf(fmaxf(z[t][4], z[t][5]), fmaxf(z[t][6], z[t][7])))) *
                               mult -
@@ -779,7 +841,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         if (second) __builtin_amdgcn_s_waitcnt(vm_wait_imm(kWait));
         ring_barrier();
         if (second) issue();
-        weights(now);
+        weights(now, std::integral_constant<int, -1>{});
         prev = now;
       }
       if (!second) ring_barrier();
@@ -792,12 +854,12 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
         const Step now = step_of(s);
         if (!now.on) continue;
         scores(now);
-        weights(now);
+        weights(now, std::integral_constant<int, -1>{});
         values(now);
       }
     }
 
-    if (__any(left_out != 0)) {  // rare, so from memory; by class as above
+    if (__builtin_expect(__any(left_out != 0), 0)) {  // rare, so from memory; by class as above
       const uint16_t* vn = static_cast<const uint16_t*>(a.v_new) + b * a.vn_row + kvh * a.vn_head;
       for (int st = s0 + wk; st < min(s1, new_steps); st += WK) {
         const int base = st * kStepKeys;
@@ -824,6 +886,60 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
           }
         }
       }
+    }
+    // Where something did not stay finite (see k_tree_few), the wave takes its steps once
+    // more, from memory, with all infinities and NaN of V added by class.
+    bool odd = false;
+#pragma unroll
+    for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]);
+    if (__builtin_expect(row0 < R && __any(odd), 0)) {
+      begin();
+      // One row tile after the other, no loads ahead: what this takes in registers, the loops
+      // above would have to do without.
+      auto tile = [&](auto only) {
+        constexpr int t = only.value;
+#pragma unroll 1
+        for (int st = s0 + wk; st < s1; st += WK) {
+          const bool fresh = st < new_steps;
+          const int base = (fresh ? st : st - new_steps) * kStepKeys, end = fresh ? a.nodes : len;
+          const int64_t k_step = fresh ? a.kn_node : a.c_slot, v_step = fresh ? a.vn_node : a.c_slot;
+          const T* kf = fresh ? static_cast<const T*>(a.k_new) + b * a.kn_row + kvh * a.kn_head : kc;
+          const T* vf = fresh ? static_cast<const T*>(a.v_new) + b * a.vn_row + kvh * a.vn_head : vc;
+          x[t] = {0.f, 0.f, 0.f, 0.f}, y[t] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            __builtin_amdgcn_sched_barrier(0);
+            x[t] = Mma<T>::mma(ld_g16(kf + min(base + step_key(i, 0), end - 1) * k_step + (c * 4 + g) * 8), q[t][c], x[t]);
+            y[t] = Mma<T>::mma(ld_g16(kf + min(base + step_key(i, 1), end - 1) * k_step + (c * 4 + g) * 8), q[t][c], y[t]);
+          }
+          weights(Step{0, base, end, true, fresh, false}, only);
+          uint32_t one[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            one[j] = Mma<T>::pack((seen[t] >> (2 * j)) & 1 ? 1.f : 0.f, (seen[t] >> (2 * j + 1)) & 1 ? 1.f : 0.f);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            __builtin_amdgcn_sched_barrier(0);
+            const uint16_t* col = reinterpret_cast<const uint16_t*>(vf) + 16 * e + i;
+            uint32_t v[4], c[4];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+              const int key = base + 16 * (w >> 1) + 4 * g + 2 * (w & 1);
+              v[w] = (key < end ? ld_g(col + min(key, end - 1) * v_step) : 0u) |
+                     (key + 1 < end ? (uint32_t)ld_g(col + min(key + 1, end - 1) * v_step) << 16 : 0u);
+              c[w] = F::classes(v[w]), v[w] = F::finite_part(v[w]);
+            }
+            o[t][e] = Mma<T>::mma(make_uint4(v[0], v[1], v[2], v[3]), ph[t], o[t][e]);
+            o[t][e] = Mma<T>::mma(make_uint4(v[0], v[1], v[2], v[3]), pl[t], o[t][e]);
+            const f32x4_t sum = Mma<T>::mma(make_uint4(c[0], c[1], c[2], c[3]), make_uint4(one[0], one[1], one[2], one[3]),
+                                            f32x4_t{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(sum[r]);
+          }
+        }
+      };
+      tile(std::integral_constant<int, 0>{});
+      if constexpr (NR == 2) tile(std::integral_constant<int, 1>{});
     }
     const int64_t slot = sh.chunk > 0 || a.teams == 0 ? team : (int64_t)b * a.kv_heads + kvh + team;
     // every load into LDS has landed and every stage been read

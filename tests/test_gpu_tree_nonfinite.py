@@ -73,3 +73,79 @@ def test_infinite_nodes_stay_beside_a_dominating_entry(f, dtype):
     want = s["v"][0, :, s["length"][0] - 1].double().repeat_interleave(f[0] // f[1], 0)[None].expand_as(out[0])
     err = (out[0].double() - want).abs()[..., fin]
     assert (err <= (torch.finfo(out.dtype).eps / 2 + 2.0 ** -16) * want.abs()[..., fin]).all()
+
+
+def seen_values(s, j):
+    """Infinities and a NaN in cached entries of sequence 0, the columns that they reach."""
+    s["v"][0, :, j[0], 1] = math.inf
+    s["v"][0, :, j[1], 2] = -math.inf
+    s["v"][0, :, j[2], 3] = math.nan
+    s["v"][0, :, j[0], 4], s["v"][0, :, j[2], 4] = math.inf, -math.inf
+    s["v"][0, :, j[1], 6] = math.inf
+    s["v_new"][0, 0, :, 6] = math.inf
+    s["parents"][0] = torch.arange(-1, s["parents"].shape[1] - 1, dtype=torch.int32)
+    return {1: math.inf, 2: -math.inf, 3: math.nan, 4: math.nan, 6: math.inf}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("f", FORMS, ids=IDS)
+@pytest.mark.parametrize("buckets", [0, 16])
+def test_infinities_of_the_cache_stay(f, dtype, buckets):
+    """In its first, its last and another entry; other columns and sequences as without them."""
+    s = form(53, dtype, f, buckets=buckets)
+    ref, rlse = oracle(s)
+    L = int(s["length"][0])
+    s2 = {n: x.clone() if isinstance(x, torch.Tensor) else x for n, x in s.items()}
+    want = seen_values(s2, (0, L // 2 + 1, L - 1))
+    s["parents"][0] = s2["parents"][0]
+    ref, rlse = oracle(s)
+    out, lse = call(s2)
+    for col, v in want.items():
+        got = out[0, :, :, col]
+        assert (got.isnan() if math.isnan(v) else got == v).all(), (col, got)
+        ref[0, :, :, col], out[0, :, :, col] = 0, 0
+    finite_check(s, dtype, out, ref, torch.ones(out.shape, dtype=torch.bool))
+    assert (lse.double() - rlse).abs().max() <= bounds(s, dtype)[1]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("f", FORMS, ids=IDS)
+def test_infinities_of_the_cache_stay_beside_a_dominating_entry(f, dtype):
+    s = form(55, dtype, f)
+    L = int(s["length"][0])
+    want = seen_values(s, (0, L // 2 + 1, L - 2))
+    s["q"][0] = s["q"][0].abs() * 0.5 + 0.5
+    s["k"][0, :, L - 1] = 150 / (s["scale"] * f[2] * 0.5)
+    out, _ = call(s)
+    for col, v in want.items():
+        got = out[0, :, :, col]
+        assert (got.isnan() if math.isnan(v) else got == v).all(), (col, got)
+    rest = [c for c in range(f[2]) if c not in want]
+    assert torch.isfinite(out[0][..., rest]).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("f", FORMS, ids=IDS)
+def test_infinite_keys(f, dtype):
+    """A key with a logit of -inf is masked, of +inf or NaN makes its row NaN, and no other."""
+    s = form(57, dtype, f)
+    heads, kv, d, nodes = f[:4]
+    s["q"][0, :, :, 0] = 1.0
+    s["q"][0, 0, 0, 0] = -1.0       # one row for which the infinite key is +inf
+    s["k"][0, 0, 5, 0] = -math.inf
+    s["v"][0, 0, 5] = math.nan      # and whose value nobody else reads
+    clean = {n: x.clone() if isinstance(x, torch.Tensor) else x for n, x in s.items()}
+    clean["k"][0, 0, 5] = 0
+    clean["v"][0, 0, 5] = 0
+    ref, rlse = oracle(clean)
+    # without entry 5: its weight e^0 and value 0 taken out again
+    n = heads // kv
+    for h in range(n):
+        w = (-rlse[0, :, h]).exp()
+        ref[0, :, h] /= (1 - w)[:, None]
+        rlse[0, :, h] += torch.log1p(-w)
+    out, lse = call(s)
+    assert out[0, 0, 0].isnan().all() and lse[0, 0, 0].isnan()
+    out[0, 0, 0], lse[0, 0, 0], ref[0, 0, 0], rlse[0, 0, 0] = 0, 0, 0, 0
+    finite_check(clean, dtype, out, ref, torch.ones(out.shape, dtype=torch.bool))
+    assert (lse.double() - rlse).abs().max() <= bounds(clean, dtype)[1]
