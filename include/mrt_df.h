@@ -666,10 +666,11 @@ typedef struct mrt_tree_attention_args {
  * outputs are 0, their lse -inf, and no other node is touched by them.  Node t
  * attends every entry of the cache, its ancestors and itself:
  *   logit(t, j) = scale * q_t . k_j + bias[h][min(max(p_t - p_j, 0), buckets - 1)]
- * with p_t the next position plus the node's depth (0 under -1).  A logit of
- * -inf, or below -1e30 (a bias of the type's lowest value), is a mask; a row
- * with nothing left has output 0 and lse -inf.  One node is an ordinary decode
- * step.  K/V of a node that t does not see have no effect on
+ * with p_t the next position plus the node's depth (0 under -1).  A bias of
+ * -inf, or below -1e30 in powers of two (-6.9e29; so a bias of the type's lowest
+ * value is one), is a mask: the entry has no part in the row, whatever its key
+ * and value hold.  So is a logit as low.  A row with nothing left has output 0
+ * and lse -inf.  One node is an ordinary decode step.  K/V of a node that t does not see have no effect on
  * t, whatever they hold; an infinite value that t does see makes the output
  * that infinity however small its weight, opposite ones or a NaN make it NaN.
  * Does not write the cache: mrt_cache_commit takes the

@@ -35,8 +35,8 @@ namespace mrt {
 namespace {
 
 constexpr int kWaves = 4;
-// Running maximum before any key: finite, so exp2(-inf - kNone) is 0.  Logits below it count
-// as masked, and a row whose sum is 0 has nothing left.
+// Running maximum before any key, in log2 units: finite, so exp2(-inf - kNone) is 0.  Logits
+// below it count as masked, and a row whose sum is 0 has nothing left.
 constexpr float kNone = -1e30f;
 constexpr int kBiasLds = 4096;   // floats of the bias by distance kept in LDS
 
@@ -326,7 +326,7 @@ __global__ __launch_bounds__(64 * kWaves, few_blocks(sizeof(T), DP, NR)) void k_
 
   // One step.  A matrix product makes NaN of 0 * inf, and of infinities whose weight is in
   // two parts: a node's infinities and NaN, which others may not see, are left out of it and
-  // added by class; with `exact`, the cache's are too.
+  // added by class; with `exact`, the cache's are too, and masked entries' keys have no part.
   auto step = [&](int st, auto exact) {
     const bool fresh = st < new_steps;
     const int base = (fresh ? st : st - new_steps) * kStepKeys, end = fresh ? a.nodes : len;
@@ -353,8 +353,11 @@ __global__ __launch_bounds__(64 * kWaves, few_blocks(sizeof(T), DP, NR)) void k_
       if (a.bias != nullptr) {
         const int at = fresh ? __popcll(sees[node]) - 1 : qpos[t];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          p[t][j] = fmaf(s[j], scale2, brow[t][min(max(at - kpos[j], 0), a.buckets - 1)] * kLog2e);
+        for (int j = 0; j < 8; ++j) {
+          const float by = brow[t][min(max(at - kpos[j], 0), a.buckets - 1)] * kLog2e;
+          p[t][j] = fmaf(s[j], scale2, by);
+          if (exact.value && by < kNone) p[t][j] = -INFINITY;  // masked, whatever the key holds
+        }
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[t][j] = s[j] * scale2;
@@ -732,8 +735,11 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
           const int qp = (fresh ? 0 : first_pos) + max(__popcll(sees[node]) - 1, 0);
           const float* row = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            z[t][j] = fmaf(z[t][j], scale2, row[min(max(qp - kpos[j], 0), a.buckets - 1)] * kLog2e);
+          for (int j = 0; j < 8; ++j) {
+            const float by = row[min(max(qp - kpos[j], 0), a.buckets - 1)] * kLog2e;
+            z[t][j] = fmaf(z[t][j], scale2, by);
+            if (exact && by < kNone) z[t][j] = -INFINITY;  // masked, whatever the key holds
+          }
         }
       }
       if (!plain) {

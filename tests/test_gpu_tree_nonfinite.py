@@ -149,3 +149,50 @@ def test_infinite_keys(f, dtype):
     out[0, 0, 0], lse[0, 0, 0], ref[0, 0, 0], rlse[0, 0, 0] = 0, 0, 0, 0
     finite_check(clean, dtype, out, ref, torch.ones(out.shape, dtype=torch.bool))
     assert (lse.double() - rlse).abs().max() <= bounds(clean, dtype)[1]
+
+
+@pytest.mark.parametrize("lowest", [False, True], ids=["inf", "lowest"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("evicted", [False, True], ids=["slots", "pos"])
+@pytest.mark.parametrize("f", FORMS, ids=IDS)
+def test_masked_entries_may_hold_anything(f, evicted, dtype, lowest):
+    """Distances of 9 and more masked by the bias: infinities and NaN in the keys and values of
+    such entries change nothing."""
+    s = form(59, dtype, f, buckets=12, evicted=evicted)
+    heads, kv, d, nodes = f[:4]
+    plain = s["bias"].clone()
+    s["bias"][:, 9:] = -math.inf
+    ref, rlse = oracle(s)
+    run = dict(s, bias=s["bias"].clamp(min=float(torch.finfo(torch.float32).min))) if lowest else s
+    L, first = int(s["length"][0]), int(s["next_pos"][0]) if evicted else int(s["length"][0])
+    pos = s["pos"][0, :, :L] if evicted else torch.arange(L).expand(kv, L)
+    dirty = dict(run, k=s["k"].clone(), v=s["v"].clone())
+    for g in range(kv):
+        far = (first - pos[g] >= 9).nonzero()[:, 0]  # of every node: a node's position is first or later
+        for at, bad in zip((0, len(far) // 3, len(far) // 2, len(far) - 2, len(far) - 1),
+                           (math.nan, math.inf, -math.inf, math.nan, math.inf)):
+            dirty["k"][0, g, far[at], at % d] = bad
+            dirty["v"][0, g, far[at], (at + 1) % d] = bad
+            dirty["v"][0, g, far[at], d - 1] = -bad
+    out, lse = call(dirty)
+    finite_check(dict(s, bias=plain), dtype, out, ref, torch.ones(out.shape, dtype=torch.bool))
+    assert (lse.double() - rlse).abs().max() <= bounds(dict(s, bias=plain), dtype)[1]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("nodes", [3, 20, 60])
+def test_masked_nodes_may_hold_anything(nodes, dtype):
+    """The same of drafted nodes: ancestors from distance 2 on are masked."""
+    s = make(61, dtype, 2, 4, 2, 64, nodes, [30, 0], buckets=3)
+    s["parents"][:] = torch.arange(-1, nodes - 1, dtype=torch.int32)
+    plain = s["bias"].clone()
+    s["bias"][:, 2:] = -math.inf
+    ref, rlse = oracle(s)
+    dirty = dict(s, k_new=s["k_new"].clone(), v_new=s["v_new"].clone())
+    dirty["k_new"][:, 0], dirty["v_new"][:, 0] = math.nan, math.inf  # masked for nodes 2 and on
+    out, lse = call(dirty)
+    where = torch.zeros(out.shape, dtype=torch.bool)
+    where[:, 2:] = True
+    finite_check(dict(s, bias=plain), dtype, out, ref, where)
+    assert (lse.double() - rlse).abs()[:, 2:].max() <= bounds(dict(s, bias=plain), dtype)[1]
+    assert out[:, :2].isnan().all()
