@@ -707,7 +707,8 @@ typedef struct mrt_cache_commit_args {
  *   score_out[j] = score[j] (0 for the n new entries and where score is NULL)
  *     + sum over i, h of [j <= length + i] * exp(logit(i, j) - lse[accepted_i][h])
  * for the length + n entries; what score_out holds past them stays.  A token
- * whose lse is -inf gives no weight. */
+ * whose lse is -inf gives no weight, nor does an entry get any from a token for
+ * which the bias masks it. */
 int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* args, int device, void* hip_stream);
 
 typedef struct mrt_cache_evict_args {

@@ -22,6 +22,9 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kStepKeys = 32;
+// Running maximum before any key, in log2 units: finite, so exp2(-inf - kNone) is 0.  Logits
+// and biases below it count as masked, and a row whose sum is 0 has nothing left.
+constexpr float kNone = -1e30f;
 
 __device__ __forceinline__ float max_over_groups(float x) {  // of lanes i, i + 16, i + 32, i + 48
   auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);

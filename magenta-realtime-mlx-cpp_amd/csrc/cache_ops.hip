@@ -146,11 +146,12 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
         const float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          float z = 0.f;
+          float by = 0.f;
           if (a.bias != nullptr)
-            z = a.bias[(size_t)head[t] * a.buckets + min(max(first + tok[t] - kpos[j], 0), a.buckets - 1)];
-          z = __builtin_amdgcn_exp2f((fmaf(s[j], a.scale, z) - lse[t]) * kLog2e);
-          w[j] += on[t] && !(fresh && base + lane_key(g, j) > tok[t]) ? z : 0.f;
+            by = a.bias[(size_t)head[t] * a.buckets + min(max(first + tok[t] - kpos[j], 0), a.buckets - 1)];
+          const float z = __builtin_amdgcn_exp2f((fmaf(s[j], a.scale, by) - lse[t]) * kLog2e);
+          const bool masked = by * kLog2e < kNone;  // whatever the key holds
+          w[j] += on[t] && !masked && !(fresh && base + lane_key(g, j) > tok[t]) ? z : 0.f;
         }
       }
 #pragma unroll

@@ -35,9 +35,6 @@ namespace mrt {
 namespace {
 
 constexpr int kWaves = 4;
-// Running maximum before any key, in log2 units: finite, so exp2(-inf - kNone) is 0.  Logits
-// below it count as masked, and a row whose sum is 0 has nothing left.
-constexpr float kNone = -1e30f;
 constexpr int kBiasLds = 4096;   // floats of the bias by distance kept in LDS
 
 struct TreeArgs {

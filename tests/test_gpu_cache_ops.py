@@ -180,6 +180,29 @@ def test_commit_masks_in_the_bias(dtype, masked):
     assert ((got["score"].double() - ref["score"]).abs() <= rel * ref["score"].abs()).all()
 
 
+@pytest.mark.parametrize("masked", [-math.inf, float(torch.finfo(torch.float32).min)], ids=["inf", "lowest"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("evicted", [False, True], ids=["slots", "pos"])
+def test_commit_masked_entries_may_hold_anything(dtype, evicted, masked):
+    """Infinities and NaN in the keys of entries that the bias masks for every token: their
+    scores are the old ones, and all others as without them."""
+    s = make_commit(37, dtype, 2, 6, 2, 64, 9, [300, 37], [[0, 1, 5], [2]], buckets=12, evicted=evicted)
+    s["bias"][:, 9:] = -math.inf
+    s["lse"] = O.tree_attention(**{n: s[n] for n in ("q", "k_new", "v_new", "k", "v", "length", "parents", "scale", "bias",
+                                                     "pos", "next_pos")})[1].float()
+    s["bias"] = s["bias"].clamp(min=masked)
+    want = commit(s)["score"]
+    for b, L in enumerate((300, 37)):
+        first = int(s["next_pos"][b]) if evicted else L
+        for g in range(2):
+            pos = s["pos"][b, g, :L] if evicted else torch.arange(L)
+            far = (first - pos >= 9).nonzero()[:, 0]
+            for at, bad in zip((far[0], far[len(far) // 2], far[-1]), (math.nan, math.inf, -math.inf)):
+                s["k"][b, g, at, int(at) % 64] = bad
+                assert want[b, g, at] == s["score"][b, g, at]
+    assert torch.equal(commit(s)["score"], want)
+
+
 def test_commit_lse_that_is_not_a_number():
     """It makes the scores of the entries that its token sees NaN, as the formula says."""
     s = make_commit(33, "bf16", 1, 4, 2, 64, 6, [50], [[1, 2, 4]])
