@@ -526,8 +526,8 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
   const int64_t team = (int64_t)(id / a.row_blocks) * 8 + (blockIdx.x & 7);
   const int n = a.heads / a.kv_heads, R = a.nodes * n, row0 = (rb * WR + wr) * (16 * NR);
   // Logits in log2 units are mult z: z the products themselves, whose sign q takes on, or
-  // with a bias the finished logits.
-  const float scale2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f), mult = BIAS ? 1.f : scale2;
+  // with a bias the finished logits.  Not 0, which would make NaN of a masked -inf.
+  const float size = fabsf(a.scale) * kLog2e, scale2 = size < 1e-37f ? 1e-37f : size, mult = BIAS ? 1.f : scale2;
   const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
   // The maximum that the weights refer to follows only where a logit passes it by more
   // than kSlack: most steps then leave the output alone.  fp16 weights stay below 2^15.

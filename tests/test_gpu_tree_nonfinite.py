@@ -196,3 +196,27 @@ def test_masked_nodes_may_hold_anything(nodes, dtype):
     finite_check(dict(s, bias=plain), dtype, out, ref, where)
     assert (lse.double() - rlse).abs()[:, 2:].max() <= bounds(dict(s, bias=plain), dtype)[1]
     assert out[:, :2].isnan().all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("nodes", [1, 10, 25, 60])
+@pytest.mark.parametrize("buckets", [0, 16])
+def test_scales_of_every_kind(nodes, buckets, dtype):
+    """0, tiny and negative scales as the formula says; one that is NaN makes every row that is
+    there NaN, in every kernel, and an absent node's 0."""
+    s = make(63, dtype, 2, 4, 2, 64, nodes, [300, 0], buckets=buckets)
+    if nodes > 1:
+        s["parents"][:, 1:] = 0
+        s["parents"][:, nodes - 1] = -3
+    for scale in (0.0, 1e-42, -0.11):
+        run = dict(s, scale=scale)
+        out, lse = call(run)
+        ref, rlse = oracle(run)
+        tol, ltol = bounds(dict(s, scale=abs(scale)), dtype)
+        assert ((out.double() - ref).abs() <= tol + torch.finfo(out.dtype).eps / 2 * (ref.abs() + tol)).all()
+        there = torch.isfinite(rlse)
+        assert (lse.double() - rlse).abs()[there].max() <= ltol and torch.equal(there, torch.isfinite(lse))
+    out, lse = call(dict(s, scale=math.nan))
+    there = nodes - 1 if nodes > 1 else 1
+    assert out[:, :there].isnan().all() and lse[:, :there].isnan().all()
+    assert (out[:, there:] == 0).all() and (lse[:, there:] == -math.inf).all()
