@@ -739,9 +739,9 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
  * 32, 64 or 128, a divisor of k.  x, scales, biases and out in `dtype`, row
  * strides ldx (a multiple of 16 bytes) and ldo in elements; w and x 16-byte
  * aligned.  Meant for few rows (at most 2^19): each 64, in fp32 each 16, read the
- * weights again.  Weights
- * are multiplied exactly and summed in fp32; a row of x that is not
- * finite gives outputs that are not.  mrt_q4_quantize makes the codes of src (n, k), row
+ * weights again.  Codes are multiplied exactly and summed in fp32, those of fp32
+ * rows from the middle of their range, so that a mean of x costs no accuracy; a
+ * row of x that is not finite gives outputs that are not.  mrt_q4_quantize makes the codes of src (n, k), row
  * stride ld: bias the group's least weight, scale a 15th of its range. */
 int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const void* scales, const void* biases,
                   int n, int k, int group, int dtype, void* out, int64_t ldo, int device, void* hip_stream);

@@ -7,16 +7,23 @@
 // 16 + code is exact in bf16 and fp16 and costs one shift and one and-or for two codes
 // (in [16, 32) a step of 1 is the bits 3..6 of bf16, 6..9 of fp16), products with x
 // are exact in fp32, and a group's sum is scaled in fp32; the sums of x come from the
-// same instruction with an operand of ones, in the lanes that need them.  The offset
-// makes a group's sum about 5 times its part without it: 2 bits of the 24.
-// fp32 activations are split exactly into three bf16 parts.
+// same instruction with an operand of ones, in the lanes that need them.
+//
+// The two terms cancel where x has a mean: one as large as its deviation puts y off by 8e-6
+// (norm-wise; k 2048, groups of 128), a product with the weights in fp32 by 3e-7.  Rounding y
+// to bf16 takes 240 times that, to fp16 30 times, but fp32 results have codes around 0,
+//   y_n = sum_g s_g sum_k (code_k - 7.5) x_k + (b_g + 7.5 s_g) sum_k x_k
+// from tables of bytes (18 instructions for eight codes instead of 7), which puts y off by
+// 4e-7: 5 x 1024 by 29824 13.0 us instead of 12.2.  fp32 rows are split exactly into three bf16
+// parts.  In bf16 and fp32 the codes, and so all sums, are 2^-12 or 2^-11 of what they stand
+// for until the end, so that terms that cancel do not overflow where y does not.
 //
 // A block takes 16 NT output columns (matrix-core rows), its waves chunks of 128 k in
 // turn, summed through LDS in order.  A lane loads 32 codes (16 bytes) of one row; two
 // exchanges between lane halves and two between quarters turn that into the operand
 // order in which each instruction's 32 k are consecutive, so within one group.
 // Reached: 2 x 1024 by 5632 (3.3 MB, bf16) 5 us, most of it one trip to memory and the sums
-// of the waves; 5 x 1024 by 29824 in fp32 (23.5 MB) 12 us; 9 x 8192 by 28672 (125 MB) 38 us,
+// of the waves; 5 x 1024 by 29824 in fp32 (23.5 MB) 13 us; 9 x 8192 by 28672 (125 MB) 38 us,
 // 3.3 TB/s: a block a CU (its registers), whose loads and products take turns.  Two blocks
 // by fewer registers spill (47 us), codes two slabs ahead gain nothing (43).
 #include <algorithm>
@@ -51,19 +58,21 @@ struct Q4Args {
 };
 
 // Operands of the matrix instruction: parts of x (1, or 3 bf16 parts of fp32) in the
-// order of the codes: 0 4 1 5 2 6 3 7 of eight consecutive k.
+// order of the codes: 0 4 1 5 2 6 3 7 of eight consecutive k, in fp32 0 2 4 6 1 3 5 7.
 template <typename T>
 struct Q4Op {
   static constexpr int kParts = 1;
-  static constexpr uint32_t kOnes = sizeof(T) == 2 && std::is_same_v<T, f16> ? 0x3c003c00u : 0x3f803f80u;
+  static constexpr uint32_t kOnes = std::is_same_v<T, f16> ? 0x3c003c00u : 0x39803980u;  // 1, 2^-12
+  static constexpr float kUp = std::is_same_v<T, f16> ? 1.f : 4096.f;
+  static constexpr float kOffset = -16.f;  // of a code, from what its operand stands for
   typedef uint4 Raw;  // eight values of x as they are in memory
   using M = Mma<T>;
   struct X {
     uint4 part[1];
   };
-  // 16 in both halves, in a register: one and-or instead of two instructions with literals.
+  // 16 (in bf16 2^-8) in both halves, in a register: one and-or instead of two instructions with literals.
   __device__ __forceinline__ static uint32_t offset() {
-    uint32_t v = std::is_same_v<T, f16> ? 0x4c004c00u : 0x41804180u;
+    uint32_t v = std::is_same_v<T, f16> ? 0x4c004c00u : 0x3b803b80u;
     asm("" : "+v"(v));
     return v;
   }
@@ -89,7 +98,9 @@ struct Q4Op {
 template <>
 struct Q4Op<float> {
   static constexpr int kParts = 3;
-  static constexpr uint32_t kOnes = 0x3f803f80u;
+  static constexpr uint32_t kOnes = 0x3a003a00u;  // 2^-11
+  static constexpr float kUp = 2048.f;
+  static constexpr float kOffset = 7.5f;
   struct Raw {
     uint4 a, b;
   };
@@ -97,29 +108,40 @@ struct Q4Op<float> {
   struct X {
     uint4 part[3];
   };
-  __device__ __forceinline__ static uint32_t offset() { return Q4Op<bf16>::offset(); }
-  __device__ __forceinline__ static uint4 codes(uint32_t w, uint32_t o) { return Q4Op<bf16>::codes(w, o); }
+  __device__ __forceinline__ static uint32_t offset() { return 0; }
+  // (code - 7.5) 2^-11 = (2 code - 15) 2^-12 in bf16: sign, exponent and significant bits of the
+  // odd numbers 1 .. 15 from tables of their two bytes, by l = (magnitude - 1) / 2, which is the
+  // code's low three bits, and below 8 those inverted.
+  __device__ __forceinline__ static uint4 codes(uint32_t w, uint32_t) {
+    const uint32_t neg = ~w & 0x88888888u, l = w ^ (neg - (neg >> 3));
+    uint32_t v[4];
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const uint32_t at = (odd ? l >> 4 : l) & 0x07070707u;
+      const uint32_t high = __builtin_amdgcn_perm(0x3b3b3b3bu, 0x3a3a3a39u, at) | ((odd ? neg : neg << 4) & 0x80808080u);
+      const uint32_t low = __builtin_amdgcn_perm(0x70503010u, 0xe0a04080u, at);
+      v[2 * odd] = __builtin_amdgcn_perm(high, low, 0x05010400u);
+      v[2 * odd + 1] = __builtin_amdgcn_perm(high, low, 0x07030602u);
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+  }
   __device__ __forceinline__ static Raw raw(const float* p, bool in) {
     return {in ? ld_g16(p) : make_uint4(0, 0, 0, 0), in ? ld_g16(p + 4) : make_uint4(0, 0, 0, 0)};
   }
+  // Three times the upper 8 of the significant bits that are left.
   __device__ __forceinline__ static X split(const Raw& r) {
-    const uint4 a = r.a, b = r.b;
-    const uint32_t lo[4] = {a.x, a.y, a.z, a.w}, hi[4] = {b.x, b.y, b.z, b.w};
-    uint32_t out[3][4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float x = __uint_as_float(lo[j]), y = __uint_as_float(hi[j]);
-#pragma unroll
-      for (int c = 0; c < 3; ++c) {
-        const uint32_t u = f2bf(x), v = f2bf(y);
-        out[c][j] = u | (v << 16);
-        x -= bf2f(u), y -= bf2f(v);
-      }
-    }
+    uint4 a = r.a, b = r.b;
     X o;
 #pragma unroll
-    for (int c = 0; c < 3; ++c) o.part[c] = make_uint4(out[c][0], out[c][1], out[c][2], out[c][3]);
+    for (int c = 0; c < 3; ++c) {
+      o.part[c] = make_uint4(__builtin_amdgcn_perm(a.z, a.x, 0x07060302u), __builtin_amdgcn_perm(b.z, b.x, 0x07060302u),
+                             __builtin_amdgcn_perm(a.w, a.y, 0x07060302u), __builtin_amdgcn_perm(b.w, b.y, 0x07060302u));
+      a = make_uint4(rest(a.x), rest(a.y), rest(a.z), rest(a.w)), b = make_uint4(rest(b.x), rest(b.y), rest(b.z), rest(b.w));
+    }
     return o;
+  }
+  __device__ __forceinline__ static uint32_t rest(uint32_t x) {
+    return __float_as_uint(__uint_as_float(x) - __uint_as_float(x & 0xffff0000u));
   }
 };
 
@@ -203,7 +225,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void k_q4(const Q4Args a) {
     for (int z = 0; z < Load::S; ++z) {
       const int e = tid + z * kThreads, row = e / (slab_chunks * G), q = e - row * (slab_chunks * G);
       const float s = St<T>::ld(next.s[z]), b = St<T>::ld(next.b[z]);
-      if (row < kRows) sc[q * kRows + row] = make_float2(s, fmaf(-16.f, s, b));
+      if (row < kRows) sc[q * kRows + row] = make_float2(s, fmaf(Op::kOffset, s, b));
     }
 #pragma unroll
     for (int z = 0; z < Load::X; ++z) {
@@ -292,7 +314,7 @@ __global__ __launch_bounds__(64 * kQ4Waves) void k_q4(const Q4Args a) {
       uint2 w2;
     } u;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) u.x[r] = St<T>::st(v[r]);
+    for (int r = 0; r < 4; ++r) u.x[r] = St<T>::st(v[r] * Op::kUp);
     if (a.wide && col + 4 <= a.n) {
       if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = u.w4;
       else *reinterpret_cast<uint2*>(dst) = u.w2;

@@ -123,3 +123,57 @@ def test_quantize(dtype, group):
     assert ((back - w.double()).abs() <= lim).all()
     assert (back[3, :group] == 0.75).all()
     assert int(codes[3, 0]) == 0
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("mean", [0.0, 1.0, 30.0])
+@pytest.mark.parametrize("rows,k,n", [(4, 2048, 64), (5, 1024, 520), (3, 8192, 40)])
+def test_fp32_rows_with_a_mean(rows, k, n, mean, group):
+    """Codes count from their middle, so that a mean of x does not make large sums that cancel.
+    Per instruction (32 products of one of x's parts) two roundings or truncations, at most
+    2^-23 each, of the accumulator, whose values are computed here, and the 32 products;
+    then per group three roundings of its terms, and of the running sum: 2^-24 each."""
+    g = torch.Generator().manual_seed(17)
+    w, scales, biases = (t.cpu() for t in mrt_df.q4_quantize(torch.randn((n, k), generator=g).to(DEV), group))
+    x = torch.randn((rows, k), generator=g) + mean
+    got = mrt_df.q4_matmul(x.to(DEV), w.to(DEV), scales.to(DEV), biases.to(DEV)).cpu().double()
+    wd = O.q4_weights(w, scales, biases)
+    ref = x.double() @ wd.T
+    s = scales.double().repeat_interleave(group, 1)
+    b = biases.double().repeat_interleave(group, 1)
+    code = (wd - b) / s - 7.5
+    xs = x.double()[:, None, :] * (s * code)[None]                       # (rows, n, k)
+    step = xs.view(rows, n, k // group, group // 32, 32)
+    acc = step.sum(-1).cumsum(-1).abs()
+    inside = (acc + step.abs().sum(-1)).sum((-1, -2))
+    off = (b + 7.5 * s)[:, ::group][None] * x.double().view(rows, 1, k // group, group).sum(-1)
+    terms = acc[..., -1] + off.abs()
+    running = (step.sum((-1, -2)) + off).abs().cumsum(-1)
+    size = (x.double().abs()[:, None, :] * (b + 7.5 * s).abs()[None]).sum(-1)  # the sums of x, by the same instructions
+    tol = 2 * 2.0 ** -23 * (inside + size) + 2.0 ** -24 * (3 * terms.sum(-1) + running.sum(-1) / 8 + 8 * running[..., -1])
+    err = (got - ref).abs()
+    assert (err <= tol + 2.0 ** -24 * ref.abs()).all(), float((err / tol).max())
+    # As a whole, with roundings that do not depend on each other: 6 k / 32 of them (three parts),
+    # of sums of at most 128 + 32 products where the result is one of k, so
+    # sqrt(6 / 32 160) 2^-23 = 6.6e-7 of it.
+    assert err.norm() <= 1e-6 * ref.norm()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_large_rows(dtype, group):
+    """Finite x up to the type's largest values: a result within the type's range is right."""
+    x, w, s, b = make(19, dtype, 4, 512, 40, group)
+    big = torch.finfo(DT[dtype]).max
+    x[0] = torch.where(x[0].double() > 0, 1.0, -1.0).to(DT[dtype]) * big
+    x[1] = big
+    x[2] = (x[2].double() / x[2].double().abs().max() * big).to(DT[dtype])
+    s, b = s / 256, b / 256         # outputs stay in range
+    got = mrt_df.q4_matmul(x.to(DEV), w.to(DEV), s.to(DEV), b.to(DEV)).cpu()
+    ref = x.double() @ O.q4_weights(w, s, b).T
+    assert ref.abs().max() < big
+    assert torch.isfinite(got.double()).all()
+    group_size = (31 * s.double().abs() + b.double().abs() + 16 * s.double().abs()).repeat_interleave(group, 1)
+    tol = (64 + 512 / 32 + 8) * 2.0 ** -24 * (x.double().abs() @ group_size.T)
+    lim = tol + torch.finfo(got.dtype).eps / 2 * (ref.abs() + tol) + 2.0 ** -25
+    assert ((got.double() - ref).abs() <= lim).all()
