@@ -742,7 +742,8 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
  * weights again.  Codes are multiplied exactly and summed in fp32, those of fp32
  * rows from the middle of their range, so that a mean of x costs no accuracy; a
  * row of x that is not finite gives outputs that are not.  mrt_q4_quantize makes the codes of src (n, k), row
- * stride ld: bias the group's least weight, scale a 15th of its range. */
+ * stride ld: bias the group's least weight, scale a 15th of its range; a group
+ * with an infinite or NaN weight has NaN for both. */
 int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const void* scales, const void* biases,
                   int n, int k, int group, int dtype, void* out, int64_t ldo, int device, void* hip_stream);
 int mrt_q4_quantize(const void* src, int64_t ld, int n, int k, int group, int dtype, uint32_t* w, void* scales,

@@ -354,7 +354,8 @@ void launch_tiles(const Q4Args& a, int group, hipStream_t s) {
 }
 
 // Eight weights a thread, group / 8 threads a group: bias = least weight, scale = a
-// 15th of the range, both rounded to the type before the codes are taken.
+// 15th of the range, both rounded to the type before the codes are taken.  Codes cannot hold
+// infinities or NaN: a group with any is NaN.
 template <typename T>
 __global__ __launch_bounds__(256) void k_q4_quantize(const T* src, int64_t ld, int64_t total, int k, int group,
                                                      uint32_t* w, T* scales, T* biases) {
@@ -364,13 +365,15 @@ __global__ __launch_bounds__(256) void k_q4_quantize(const T* src, int64_t ld, i
   const int64_t at = min(word, total - 1), row = at / words;
   const int c = (int)(at - row * words);
   float v[8], lo = INFINITY, hi = -INFINITY;
+  int odd = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     v[j] = S::ld(src[row * ld + c * 8 + j]);
-    lo = fminf(lo, v[j]), hi = fmaxf(hi, v[j]);
+    lo = fminf(lo, v[j]), hi = fmaxf(hi, v[j]), odd |= !(fabsf(v[j]) < INFINITY);
   }
-  for (int o = 1; o < span; o <<= 1) lo = fminf(lo, __shfl_xor(lo, o, 64)), hi = fmaxf(hi, __shfl_xor(hi, o, 64));
-  const float scale = S::rnd((hi - lo) / 15.f), bias = S::rnd(lo);
+  for (int o = 1; o < span; o <<= 1)
+    lo = fminf(lo, __shfl_xor(lo, o, 64)), hi = fmaxf(hi, __shfl_xor(hi, o, 64)), odd |= __shfl_xor(odd, o, 64);
+  const float scale = odd ? NAN : S::rnd((hi - lo) / 15.f), bias = odd ? NAN : S::rnd(lo);
   uint32_t code = 0;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {

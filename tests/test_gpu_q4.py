@@ -177,3 +177,24 @@ def test_large_rows(dtype, group):
     tol = (64 + 512 / 32 + 8) * 2.0 ** -24 * (x.double().abs() @ group_size.T)
     lim = tol + torch.finfo(got.dtype).eps / 2 * (ref.abs() + tol) + 2.0 ** -25
     assert ((got.double() - ref).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_quantize_keeps_what_is_not_a_number(dtype, group, bad):
+    """A group with an infinite or NaN weight becomes NaN as a whole, the others as without it."""
+    g = torch.Generator().manual_seed(23)
+    w = torch.randn((6, 384), generator=g).to(DT[dtype])
+    clean = [t.cpu() for t in mrt_df.q4_quantize(w.to(DEV), group)]
+    w[1, 5], w[1, group - 1], w[4, 383] = bad, bad, bad
+    got = [t.cpu() for t in mrt_df.q4_quantize(w.to(DEV), group)]
+    hit = torch.zeros(got[1].shape, dtype=torch.bool)
+    hit[1, 0], hit[4, -1] = True, True
+    for t, c in zip(got[1:], clean[1:]):
+        assert t[hit].isnan().all() and torch.equal(t[~hit], c[~hit])
+    words = ~hit.repeat_interleave(group // 8, 1)
+    assert torch.equal(got[0][words], clean[0][words])
+    y = mrt_df.q4_matmul(torch.ones((2, 384), dtype=DT[dtype], device=DEV), *(t.to(DEV) for t in got)).cpu()
+    rows = torch.tensor([False, True, False, False, True, False])
+    assert y[:, rows].isnan().all() and torch.isfinite(y[:, ~rows]).all()
