@@ -3,6 +3,8 @@
 // thread-local message; nothing throws across the ABI.
 #include "../../include/mrt_df.h"
 
+#include <algorithm>
+#include <initializer_list>
 #include <memory>
 #include <string>
 
@@ -179,6 +181,11 @@ void require(bool ok, const char* msg) {
 
 bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
+// int32 and fp32 arrays.
+bool aligned4(std::initializer_list<const void*> ps) {
+  return std::all_of(ps.begin(), ps.end(), [](const void* p) { return aligned(p, 4); });
+}
+
 // The stride of a dimension of `size` entries (that of a single entry is never used).
 bool stride_ok(int64_t stride, int size, int64_t unit) { return size <= 1 || (stride >= 0 && stride % unit == 0); }
 
@@ -219,6 +226,7 @@ mrt::KvCache to_cache(const mrt_kv_cache* c, bool data = true) {
             "cache: strides must be multiples of 16 bytes, not negative");
     require(c->capacity == 1 || c->slot_stride >= c->d, "cache: slots overlap");
     require(c->pos == nullptr || c->next_pos != nullptr, "cache: pos without next_pos");
+    require(aligned4({c->length, c->pos, c->next_pos, c->score}), "cache: length, pos, next_pos and score must be 4-byte aligned");
   }
   k.k = c->k, k.v = c->v;
   k.row_stride = c->row_stride, k.head_stride = c->head_stride, k.slot_stride = c->slot_stride;
@@ -998,6 +1006,7 @@ int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args*
                 (args->heads == 1 || a.out.head_stride >= c.d),
             "tree_attention: out overlaps itself");
     require(args->parents != nullptr && args->parents_stride >= 0, "tree_attention: null parents or negative stride");
+    require(aligned4({args->parents, args->lse}), "tree_attention: parents and lse must be 4-byte aligned");
     a.parents = args->parents, a.parents_stride = args->parents_stride;
     a.lse = args->lse, a.bias = args->bias, a.buckets = args->bias ? args->buckets : 0;
     a.nodes = args->nodes, a.heads = args->heads, a.scale = args->scale;
@@ -1031,6 +1040,8 @@ int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* arg
             "cache_commit: length_out must be an array of its own");
     require(c.pos == nullptr || (args->next_out != nullptr && args->next_out != c.next_pos && args->next_out != c.length),
             "cache_commit: next_out must be an array of its own");
+    require(aligned4({args->accepted, args->lse, args->score_out, args->length_out, args->next_out}),
+            "cache_commit: accepted, lse and the outputs must be 4-byte aligned");
     a.accepted = args->accepted, a.accepted_stride = args->accepted_stride, a.lse = args->lse, a.bias = args->bias;
     a.score_out = args->score_out, a.length_out = args->length_out, a.next_out = args->next_out;
     a.accepted_n = args->accepted_n, a.nodes = args->nodes, a.heads = args->heads;
@@ -1063,6 +1074,7 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
     require(args->keep >= 1 && args->recent >= 0 && args->sinks >= 0 &&
                 static_cast<int64_t>(args->recent) + args->sinks <= args->keep,
             "cache_evict: keep >= 1, recent >= 0, sinks >= 0 and recent + sinks <= keep");
+    require(aligned4({args->score_out, args->pos_out, args->length_out}), "cache_evict: outputs must be 4-byte aligned");
     const size_t want = mrt::cache_evict_workspace(c, args->keep);
     require(want == 0 || (workspace != nullptr && workspace_bytes >= want && aligned(workspace, 16)),
             "cache_evict: workspace too small, misaligned or null");
@@ -1084,6 +1096,9 @@ int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const
     if (rows == 0) return;
     require(x && w && scales && biases && out, "q4_matmul: null argument");
     require(aligned(x, 16) && aligned(w, 16), "q4_matmul: x and w must be 16-byte aligned");
+    const size_t size = mrt::dtype_size(dt);
+    require(aligned(scales, size) && aligned(biases, size) && aligned(out, size),
+            "q4_matmul: scales, biases and out must be aligned to their elements");
     require(rows <= 1 || (ldx >= k && ldx % unit == 0), "q4_matmul: ldx must be >= k, a multiple of 16 bytes");
     require(rows <= 1 || ldo >= n, "q4_matmul: ldo must be >= n");
     mrt::Q4Weights q;
@@ -1099,6 +1114,9 @@ int mrt_q4_quantize(const void* src, int64_t ld, int n, int k, int group, int dt
     const mrt::DType dt = to_dtype(dtype);
     check_q4(n, k, group);
     require(src && w && scales && biases, "q4_quantize: null argument");
+    const size_t size = mrt::dtype_size(dt);
+    require(aligned(src, size) && aligned(w, 4) && aligned(scales, size) && aligned(biases, size),
+            "q4_quantize: operands must be aligned to their elements");
     require(ld >= k || n == 1, "q4_quantize: ld must be >= k");
     OnDevice on(device);
     mrt::q4_quantize(dt, src, ld, n, k, group, w, scales, biases, static_cast<hipStream_t>(hip_stream));

@@ -214,3 +214,43 @@ def test_q4_no_rows_and_quantize_refusals(lib):
         mrt_df.q4_matmul(torch.zeros(2, 64), torch.zeros(4, 8, dtype=torch.int32), torch.zeros(4, 1), torch.zeros(4, 1))
     with pytest.raises(ValueError):
         mrt_df.q4_quantize(torch.zeros(4, 64), 64)
+
+
+@pytest.mark.parametrize("name", ["length", "pos", "next_pos", "score"])
+def test_refuses_misaligned_arrays_of_caches(lib, name):
+    full = dict(pos=P, next_pos=P, score=P)
+    bad = cache(**{**full, name: P + 2})
+    refused(lib, lib.mrt_tree_attention(bad, tree(), P, 1 << 20, 0, None))
+    refused(lib, lib.mrt_cache_commit(bad, commit(next_out=P + 256), 0, None))
+    refused(lib, lib.mrt_cache_evict(bad, evict(), P, 1 << 20, 0, None))
+
+
+@pytest.mark.parametrize("bad", [dict(parents=P + 2), dict(lse=P + 1), dict(bias=P + 2, buckets=4)], ids=["parents", "lse", "bias"])
+def test_tree_attention_refuses_misaligned_arrays(lib, bad):
+    refused(lib, lib.mrt_tree_attention(cache(), tree(**bad), P, 1 << 20, 0, None))
+
+
+@pytest.mark.parametrize("name", ["accepted", "lse", "score_out", "length_out", "next_out"])
+def test_commit_refuses_misaligned_arrays(lib, name):
+    args = dict(length_out=P + 64, next_out=P + 256)
+    refused(lib, lib.mrt_cache_commit(cache(pos=P, next_pos=P), commit(**{**args, name: P + 514}), 0, None))
+
+
+@pytest.mark.parametrize("name", ["score_out", "pos_out", "length_out"])
+def test_evict_refuses_misaligned_arrays(lib, name):
+    refused(lib, lib.mrt_cache_evict(cache(pos=P, next_pos=P, score=P), evict(**{name: P + 66}), P, 1 << 20, 0, None))
+
+
+@pytest.mark.parametrize("dtype,off", [(0, 2), (1, 1), (2, 1)], ids=["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("name", ["scales", "biases", "out"])
+def test_q4_matmul_refuses_misaligned_arrays(lib, name, dtype, off):
+    a = {**Q4, "dtype": dtype, name: P + off}
+    refused(lib, lib.mrt_q4_matmul(a["x"], a["ldx"], a["rows"], a["w"], a["scales"], a["biases"], a["n"], a["k"], a["group"],
+                                   a["dtype"], a["out"], a["ldo"], 0, None))
+
+
+@pytest.mark.parametrize("at", [0, 6, 7, 8], ids=["src", "w", "scales", "biases"])
+def test_q4_quantize_refuses_misaligned_arrays(lib, at):
+    a = [P, 128, 16, 128, 64, 1, P, P, P]
+    a[at] = P + 1
+    refused(lib, lib.mrt_q4_quantize(*a, 0, None))
