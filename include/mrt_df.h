@@ -614,7 +614,8 @@ int mrt_coca_read(mrt_coca* h, int which, void* dst, size_t bytes);
  * hold has no effect.  capacity at most 2^30, rows * kv_heads 2^20.  pos: NULL where an entry's slot is its position
  * (the next token's is then length[b]); else (rows, kv_heads, capacity) int32
  * positions, in any order, and next_pos (rows) the next token's.  Sequences
- * and heads may share slots (stride 0) where the cache is only read.  score
+ * and heads may share slots (stride 0) where the cache is only read; where it is
+ * written, its slots and those of k and v lie apart.  score
  * (rows, kv_heads, capacity) fp32: accumulated attention weights, or NULL. */
 typedef struct mrt_kv_cache {
   void* k;

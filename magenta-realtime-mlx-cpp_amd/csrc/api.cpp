@@ -4,6 +4,7 @@
 #include "../../include/mrt_df.h"
 
 #include <algorithm>
+#include <array>
 #include <initializer_list>
 #include <memory>
 #include <string>
@@ -247,10 +248,44 @@ mrt::NodeRows to_nodes(const mrt_node_rows& r, const mrt::KvCache& c, int nodes,
   return n;
 }
 
+// An array of vectors of d elements: extents and strides of its dimensions, largest stride
+// first.
+struct Vectors {
+  struct Dim {
+    int64_t size, stride;
+  };
+  std::array<Dim, 3> dims;
+  int64_t d;
+  Vectors(int64_t d_, Dim a, Dim b, Dim c) : dims{a, b, c}, d(d_) {
+    for (Dim& x : dims)
+      if (x.size <= 1) x = {1, 0};
+    std::sort(dims.begin(), dims.end(), [](const Dim& x, const Dim& y) { return x.stride > y.stride; });
+  }
+  // Whether no two vectors share elements, by the dimensions lying one inside the other.
+  bool apart() const {
+    __int128 extent = d;
+    for (int i = 2; i >= 0; --i) {
+      if (dims[i].size > 1 && dims[i].stride < extent) return false;
+      extent += static_cast<__int128>(dims[i].size - 1) * dims[i].stride;
+    }
+    return true;
+  }
+  // Whether one of these vectors shares elements with one of the same array `by` elements on.
+  bool meets(__int128 by, int i = 0) const {
+    if (i == 3) return by > -d && by < d;
+    const __int128 most = dims[i].size - 1, at = dims[i].stride > 0 ? by / dims[i].stride : 0;
+    for (__int128 n = at - 1; n <= at + 1; ++n)  // further off than what lies inside can reach
+      if (n >= -most && n <= most && meets(by - n * dims[i].stride, i + 1)) return true;
+    return false;
+  }
+};
+
 // Of a cache that is written.
 void check_own_slots(const mrt::KvCache& c) {
-  require((c.rows == 1 || c.row_stride > 0) && (c.kv_heads == 1 || c.head_stride > 0),
-          "cache: sequences or heads share their slots");
+  const Vectors slots(c.d, {c.rows, c.row_stride}, {c.kv_heads, c.head_stride}, {c.capacity, c.slot_stride});
+  require(slots.apart(), "cache: sequences, heads or slots overlap");
+  const __int128 bytes = static_cast<__int128>(reinterpret_cast<uintptr_t>(c.v)) - reinterpret_cast<uintptr_t>(c.k);
+  require(!slots.meets(bytes / static_cast<int64_t>(mrt::dtype_size(c.dt))), "cache: k and v overlap");
 }
 
 void check_heads(const mrt::KvCache& c, int heads, int nodes) {
@@ -1002,8 +1037,7 @@ int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args*
     a.k_new = to_nodes(args->k_new, c, args->nodes, c.kv_heads, "tree_attention: null k_new");
     a.v_new = to_nodes(args->v_new, c, args->nodes, c.kv_heads, "tree_attention: null v_new");
     a.out = to_nodes(args->out, c, args->nodes, args->heads, "tree_attention: null out");
-    require((c.rows <= 1 || a.out.row_stride > 0) && (args->nodes == 1 || a.out.node_stride >= c.d) &&
-                (args->heads == 1 || a.out.head_stride >= c.d),
+    require(Vectors(c.d, {c.rows, a.out.row_stride}, {args->nodes, a.out.node_stride}, {args->heads, a.out.head_stride}).apart(),
             "tree_attention: out overlaps itself");
     require(args->parents != nullptr && args->parents_stride >= 0, "tree_attention: null parents or negative stride");
     require(aligned4({args->parents, args->lse}), "tree_attention: parents and lse must be 4-byte aligned");
@@ -1025,7 +1059,6 @@ int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* arg
     if (c.rows == 0) return;
     check_heads(c, args->heads, args->nodes);
     check_bias(args->bias, args->buckets);
-    check_own_slots(c);
     mrt::CommitArgs a;
     a.k_new = to_nodes(args->k_new, c, args->nodes, c.kv_heads, "cache_commit: null k_new");
     a.v_new = to_nodes(args->v_new, c, args->nodes, c.kv_heads, "cache_commit: null v_new");
@@ -1046,6 +1079,7 @@ int mrt_cache_commit(const mrt_kv_cache* cache, const mrt_cache_commit_args* arg
     a.score_out = args->score_out, a.length_out = args->length_out, a.next_out = args->next_out;
     a.accepted_n = args->accepted_n, a.nodes = args->nodes, a.heads = args->heads;
     a.buckets = args->bias ? args->buckets : 0, a.scale = args->scale;
+    check_own_slots(c);
     OnDevice on(device);
     mrt::cache_commit(c, a, static_cast<hipStream_t>(hip_stream));
   });
@@ -1066,7 +1100,6 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
     require(args != nullptr, "null argument");
     const mrt::KvCache c = to_cache(cache);
     if (c.rows == 0) return;
-    check_own_slots(c);
     require(c.pos != nullptr && c.score != nullptr, "cache_evict: the cache needs pos, next_pos and score");
     require(args->score_out != nullptr && args->pos_out != nullptr, "cache_evict: null score_out or pos_out");
     require(args->length_out != nullptr && args->length_out != c.length && args->length_out != c.next_pos,
@@ -1081,6 +1114,7 @@ int mrt_cache_evict(const mrt_kv_cache* cache, const mrt_cache_evict_args* args,
     mrt::EvictArgs a;
     a.score_out = args->score_out, a.pos_out = args->pos_out, a.length_out = args->length_out;
     a.keep = args->keep, a.recent = args->recent, a.sinks = args->sinks;
+    check_own_slots(c);
     OnDevice on(device);
     mrt::cache_evict(c, a, workspace, static_cast<hipStream_t>(hip_stream));
   });

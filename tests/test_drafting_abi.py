@@ -12,6 +12,7 @@ import mrt_df
 
 INVALID = 1
 P = 0x1000  # a pointer that no refused call follows
+V = 0x100000  # another, far from it
 
 
 @pytest.fixture(scope="module")
@@ -254,3 +255,49 @@ def test_q4_quantize_refuses_misaligned_arrays(lib, at):
     a = [P, 128, 16, 128, 64, 1, P, P, P]
     a[at] = P + 1
     refused(lib, lib.mrt_q4_quantize(*a, 0, None))
+
+
+OVERLAPS = {
+    "sequences share slots": dict(rs=0), "heads share slots": dict(hs=0), "sequences reach into heads": dict(rs=1024, hs=1024),
+    "sequences reach into slots": dict(rs=64, hs=1024), "heads reach into slots": dict(hs=1016), "heads among slots": dict(hs=64),
+    "sequences a slot short": dict(rs=1984), "slots reach into each other": dict(hs=64, ss=120, rs=2048),
+    "v is k": dict(v=P), "v a slot behind k": dict(v=P + 128), "v a sequence behind k": dict(v=P + 4096),
+    "v before k": dict(k=V + 1024, v=V), "v half a slot behind k": dict(v=P + 64),
+}
+
+
+@pytest.mark.parametrize("bad", OVERLAPS)
+def test_writes_refuse_caches_that_overlap(lib, bad):
+    c = cache(**{"v": V, "pos": P, "next_pos": P, "score": P, **OVERLAPS[bad]})
+    refused(lib, lib.mrt_cache_commit(c, commit(next_out=P + 256), 0, None))
+    assert b"overlap" in lib.mrt_last_error()
+    refused(lib, lib.mrt_cache_evict(c, evict(), P, 1 << 20, 0, None))
+    assert b"overlap" in lib.mrt_last_error()
+
+
+@pytest.mark.parametrize("strides", [(1024, 64, 64), (1024, 256, 256), (256, 256, 64), (1024, 256, 56), (1016, 256, 64), (0, 256, 64)])
+def test_tree_attention_refuses_out_that_overlaps(lib, strides):
+    refused(lib, lib.mrt_tree_attention(cache(), tree(os=strides), P, 1 << 20, 0, None))
+    assert b"out overlaps" in lib.mrt_last_error()
+
+
+NOWHERE = 1 << 20  # a device that there is not: a call that passes the checks ends there
+
+
+def test_tree_attention_takes_out_with_sequences_innermost(lib):
+    code = lib.mrt_tree_attention(cache(), tree(os=(64, 1024, 256)), P, 1 << 20, NOWHERE, None)
+    assert code not in (0, INVALID)
+
+
+@pytest.mark.parametrize("layout", [
+    dict(rs=2048, hs=1024, ss=64, v=P + 8192),                  # one array after the other
+    dict(rs=4096, hs=128, ss=256, k=P, v=P + 128),              # slots of k and v in turn: (rows, capacity, heads, 2, d)
+    dict(rs=4096, hs=64, ss=256, v=P + 256),                    # (rows, capacity, 2, heads, d)
+    dict(rs=1024, hs=8192, ss=64, v=P + (1 << 20)),               # heads outermost
+    dict(rs=64, hs=4096, ss=128, v=P + 2048 * 2),               # sequences innermost; v behind k's head
+    dict(rs=7, hs=1024, ss=64, rows=1, v=P + 4096),             # a single sequence's stride is not used
+    dict(rs=1 << 60, hs=1 << 59, ss=1 << 40, cap=1 << 18, v=V),  # extents past 64 bits
+])
+def test_writes_take_caches_whose_slots_lie_apart(lib, layout):
+    c = cache(**{"pos": P, "next_pos": P, **layout})
+    assert lib.mrt_cache_commit(c, commit(next_out=P + 256), NOWHERE, None) not in (0, INVALID)
