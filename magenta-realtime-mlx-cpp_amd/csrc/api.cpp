@@ -295,6 +295,8 @@ void check_heads(const mrt::KvCache& c, int heads, int nodes) {
   require(static_cast<int64_t>(c.rows) * heads * nodes < (1ll << 31), "rows * heads * nodes must be below 2^31");
 }
 
+constexpr char kTreeTooLarge[] = "tree_attention: too many sequences, heads and nodes for one call";
+
 void check_q4(int n, int k, int group) {
   require(group == 32 || group == 64 || group == 128, "4-bit weights: group must be 32, 64 or 128");
   require(n >= 1 && n <= (1 << 28) && k >= group && k <= (1 << 20) && k % group == 0,
@@ -1020,6 +1022,7 @@ int mrt_tree_attention_workspace(const mrt_kv_cache* cache, int heads, int nodes
     require(bytes != nullptr, "null argument");
     const mrt::KvCache c = to_cache(cache, false);
     check_heads(c, heads, nodes);
+    require(mrt::tree_attention_fits(c, heads, nodes), kTreeTooLarge);
     *bytes = mrt::tree_attention_workspace(c, heads, nodes);
   });
 }
@@ -1044,6 +1047,7 @@ int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args*
     a.parents = args->parents, a.parents_stride = args->parents_stride;
     a.lse = args->lse, a.bias = args->bias, a.buckets = args->bias ? args->buckets : 0;
     a.nodes = args->nodes, a.heads = args->heads, a.scale = args->scale;
+    require(mrt::tree_attention_fits(c, a.heads, a.nodes), kTreeTooLarge);
     const size_t want = mrt::tree_attention_workspace(c, a.heads, a.nodes);
     require(want == 0 || (workspace != nullptr && workspace_bytes >= want && aligned(workspace, 16)),
             "tree_attention: workspace too small, misaligned or null");
@@ -1128,6 +1132,8 @@ int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const
     check_q4(n, k, group);
     require(rows >= 0 && rows <= (1 << 19), "q4_matmul: rows must be in 0..2^19");
     if (rows == 0) return;
+    // 512 threads for 32 columns, for up to 16 rows for 64
+    require(rows <= 16 || n <= (1 << 28) - 64, "q4_matmul: n must be at most 2^28 - 64 for more than 16 rows");
     require(x && w && scales && biases && out, "q4_matmul: null argument");
     require(aligned(x, 16) && aligned(w, 16), "q4_matmul: x and w must be 16-byte aligned");
     const size_t size = mrt::dtype_size(dt);
@@ -1148,6 +1154,7 @@ int mrt_q4_quantize(const void* src, int64_t ld, int n, int k, int group, int dt
     const mrt::DType dt = to_dtype(dtype);
     check_q4(n, k, group);
     require(src && w && scales && biases, "q4_quantize: null argument");
+    require(static_cast<int64_t>(n) * (k / 8) <= (1ll << 32) - 256, "q4_quantize: more than 2^35 weights");  // a thread each 8
     const size_t size = mrt::dtype_size(dt);
     require(aligned(src, size) && aligned(w, 4) && aligned(scales, size) && aligned(biases, size),
             "q4_quantize: operands must be aligned to their elements");

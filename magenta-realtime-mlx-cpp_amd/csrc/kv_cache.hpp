@@ -41,6 +41,8 @@ struct TreeAttnArgs {
   int buckets = 0, nodes = 0, heads = 0;
   float scale = 1.f;
 };
+// Whether a launch has threads enough for these sizes.
+bool tree_attention_fits(const KvCache& c, int heads, int nodes);
 // Bytes of workspace that tree_attention wants (0: none).
 size_t tree_attention_workspace(const KvCache& c, int heads, int nodes);
 void tree_attention(const KvCache& c, const TreeAttnArgs& a, void* ws, hipStream_t s);

@@ -1142,6 +1142,10 @@ size_t blocks_of(const KvCache& c, const Plan& p) {  // and slots, where units a
   return p.teams > 0 ? p.teams + units : units * p.splits;
 }
 
+// Rows that a wave of k_tree_join takes: 1056 rows 16.1 us by ones and 21.2 by fours, with the
+// attention, 32768 rows 232 and 228.
+int join_rows(int64_t units, int R) { return units * R < 16384 ? 1 : 4; }
+
 template <typename T, int DP, int NR>
 void launch_few(const TreeArgs& a, int blocks, hipStream_t s) {
   const size_t join = (size_t)kWaves * NR * AttnFrag<T, DP>::E * 64 * 16;
@@ -1182,6 +1186,14 @@ void launch_many(const TreeArgs& a, int blocks, int tiles, hipStream_t s) {
 }
 
 }  // namespace
+
+bool tree_attention_fits(const KvCache& c, int heads, int nodes) {
+  const Plan p = plan(c, heads, nodes);
+  const int64_t units = (int64_t)c.rows * c.kv_heads, most = (1ll << 32) - 1;  // threads of a launch
+  const int R = nodes * (heads / c.kv_heads), per = 4 * join_rows(units, R);
+  const int64_t blocks = ((int64_t)blocks_of(c, p) + 7) / 8 * 8 * p.row_blocks;
+  return blocks * (p.many ? 512 : 64 * kWaves) <= most && units * ((R + per - 1) / per) * 256 <= most;
+}
 
 size_t tree_attention_workspace(const KvCache& c, int heads, int nodes) {
   const Plan p = plan(c, heads, nodes);
@@ -1231,8 +1243,7 @@ void tree_attention(const KvCache& c, const TreeAttnArgs& t, void* ws, hipStream
   if (cuts(p)) {
     const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64, units = c.rows * c.kv_heads;
     MRT_DTYPE_DISPATCH(c.dt, {
-      // one row a wave or four: 1056 rows 16.1 us and 21.2 with the attention, 32768 rows 232 and 228
-      if ((int64_t)units * R < 16384)
+      if (join_rows(units, R) == 1)
         hipLaunchKernelGGL((k_tree_join<T, 1>), dim3(units * ((R + 3) / 4)), dim3(256), 0, s, a, p.many, cols);
       else
         hipLaunchKernelGGL((k_tree_join<T, 4>), dim3(units * ((R + 15) / 16)), dim3(256), 0, s, a, p.many, cols);

@@ -301,3 +301,20 @@ def test_tree_attention_takes_out_with_sequences_innermost(lib):
 def test_writes_take_caches_whose_slots_lie_apart(lib, layout):
     c = cache(**{"pos": P, "next_pos": P, **layout})
     assert lib.mrt_cache_commit(c, commit(next_out=P + 256), NOWHERE, None) not in (0, INVALID)
+
+
+def test_refuses_what_a_launch_has_no_threads_for(lib):
+    size = ctypes.c_size_t()
+    for rows, heads, nodes, ok in ((1 << 20, 1, 64, True), (1 << 20, 16, 64, False), (1 << 16, 1024, 16, False), (1, 4096, 64, True),
+                                   (1 << 14, 64, 64, True)):
+        c = cache(rows=rows, kv=1, rs=0, hs=0)
+        assert (lib.mrt_tree_attention_workspace(c, heads, nodes, ctypes.byref(size)) == 0) == ok, (rows, heads, nodes)
+        if not ok:
+            wide = (heads * nodes * 64, heads * 64, 64)
+            refused(lib, lib.mrt_tree_attention(c, tree(nodes=nodes, heads=heads, os=wide), P, 1 << 60, NOWHERE, None))
+            assert b"too many" in lib.mrt_last_error()
+    a = {**Q4, "n": (1 << 28) - 63, "ldo": 1 << 28, "rows": 40}
+    refused(lib, lib.mrt_q4_matmul(a["x"], a["ldx"], a["rows"], a["w"], a["scales"], a["biases"], a["n"], a["k"], a["group"],
+                                   a["dtype"], a["out"], a["ldo"], NOWHERE, None))
+    refused(lib, lib.mrt_q4_quantize(P, 1 << 20, 1 << 15, 1 << 20, 64, 1, P, P, P, NOWHERE, None))
+    assert lib.mrt_q4_quantize(P, 1 << 20, (1 << 15) - 1, 1 << 20, 64, 1, P, P, P, NOWHERE, None) not in (0, INVALID)
