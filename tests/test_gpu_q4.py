@@ -198,3 +198,20 @@ def test_quantize_keeps_what_is_not_a_number(dtype, group, bad):
     y = mrt_df.q4_matmul(torch.ones((2, 384), dtype=DT[dtype], device=DEV), *(t.to(DEV) for t in got)).cpu()
     rows = torch.tensor([False, True, False, False, True, False])
     assert y[:, rows].isnan().all() and torch.isfinite(y[:, ~rows]).all()
+
+
+WIDE = [
+    # rows k n     column tiles of a block: two from n 8177 on, four for up to 16 rows from 16369 on
+    (1, 256, 8177), (16, 1152, 8200), (17, 1152, 8177), (32, 256, 8200), (33, 1152, 8177), (64, 1152, 8200),
+    (5, 1152, 16385), (16, 256, 16400), (1, 2304, 16385), (9, 128, 29824),
+]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("rows,k,n", WIDE)
+def test_many_columns(rows, k, n, group, dtype):
+    k -= 128 - group if k > 1024 else 0  # no whole chunk of 128 at the end
+    x, w, s, b = make(29, dtype, rows, k, n, group)
+    got = mrt_df.q4_matmul(x.to(DEV), w.to(DEV), s.to(DEV), b.to(DEV))
+    check(x, w, s, b, got.cpu())

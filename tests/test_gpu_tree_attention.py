@@ -124,6 +124,8 @@ CASES = [
     (1, 12, 2, 64, 50, [333]),                 # 300 rows: two blocks of sixteen
     (2, 9, 1, 128, 33, [100, 640]),
     # work enough that parts are cut by equal shares, across sequences and heads
+    # (where the caches have 32768 steps and less, as here, each unit is cut by itself; shared
+    # out by all lengths: BIG below and test_gpu_tree_forms.py)
     (4, 16, 8, 64, 9, [7000, 5000, 31, 6200]),
     (3, 32, 16, 128, 17, [6000, 3333, 1]),
     (70, 8, 4, 64, 20, [700 + 13 * b for b in range(70)]),
