@@ -420,7 +420,7 @@ __global__ __launch_bounds__(64 * kWaves, few_blocks(sizeof(T), DP, NR)) void k_
   }
   bool odd = false;
 #pragma unroll
-  for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]);
+  for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]) && sees[min(row0 + t * 16 + i, R - 1) / n] != 0;
   if (__builtin_expect(__any(odd), 0)) {  // rare: this wave's steps once more
     begin();
 #pragma unroll 1
@@ -894,7 +894,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
     // more, from memory, with all infinities and NaN of V added by class.
     bool odd = false;
 #pragma unroll
-    for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]);
+    for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]) && sees[min(row0 + t * 16 + i, R - 1) / n] != 0;
     if (__builtin_expect(row0 < R && __any(odd), 0)) {
       begin();
       // One row tile after the other, no loads ahead: what this takes in registers, the loops

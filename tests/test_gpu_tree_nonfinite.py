@@ -220,3 +220,19 @@ def test_scales_of_every_kind(nodes, buckets, dtype):
     there = nodes - 1 if nodes > 1 else 1
     assert out[:, :there].isnan().all() and lse[:, :there].isnan().all()
     assert (out[:, there:] == 0).all() and (lse[:, there:] == -math.inf).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("f", FORMS, ids=IDS)
+def test_absent_nodes_may_hold_anything(f, dtype):
+    """Padding: q, k_new and v_new of absent nodes that nobody wrote."""
+    s = form(65, dtype, f)
+    nodes = f[3]
+    s["parents"][:, (nodes + 1) // 2:] = -9
+    for n in ("q", "k_new", "v_new"):
+        s[n][:, (nodes + 1) // 2:] = 0
+    clean = call(s)
+    for n, bad in (("q", math.nan), ("k_new", math.inf), ("v_new", -math.inf)):
+        s[n][:, (nodes + 1) // 2:] = bad
+    got = call(s)
+    assert torch.equal(got[0], clean[0]) and torch.equal(got[1], clean[1])
