@@ -249,6 +249,11 @@ struct AttnFrag {
 __device__ __forceinline__ int step_key(int i, int half) { return i + 16 * half; }
 __device__ __forceinline__ int lane_key(int g, int j) { return 4 * g + (j & 3) + (j >> 2) * 16; }
 
+// Column of the bias by distance: positions may lie further apart than 31 bits count.
+__device__ __forceinline__ int bucket(int from, int to, int buckets) {
+  return min(max(__builtin_elementwise_sub_sat(from, to), 0), buckets - 1);
+}
+
 // The factor 2^x, x <= 0, by which sums and outputs follow a larger maximum.  At least the
 // smallest normal number: 0 would make NaN of an infinite value, whose weight is small but
 // not 0; finite sums, of at least 2^-8, take in 2^-126 of others without a trace.

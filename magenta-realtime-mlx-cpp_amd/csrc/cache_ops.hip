@@ -148,7 +148,7 @@ __global__ __launch_bounds__(64 * kCommitWaves) void k_commit(const CommitK a) {
         for (int j = 0; j < 8; ++j) {
           float by = 0.f;
           if (a.bias != nullptr)
-            by = a.bias[(size_t)head[t] * a.buckets + min(max(first + tok[t] - kpos[j], 0), a.buckets - 1)];
+            by = a.bias[(size_t)head[t] * a.buckets + bucket(first + tok[t], kpos[j], a.buckets)];
           const float z = __builtin_amdgcn_exp2f((fmaf(s[j], a.scale, by) - lse[t]) * kLog2e);
           const bool masked = by * kLog2e < kNone;  // whatever the key holds
           w[j] += on[t] && !masked && !(fresh && base + lane_key(g, j) > tok[t]) ? z : 0.f;

@@ -351,7 +351,7 @@ __global__ __launch_bounds__(64 * kWaves, few_blocks(sizeof(T), DP, NR)) void k_
         const int at = fresh ? __popcll(sees[node]) - 1 : qpos[t];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float by = brow[t][min(max(at - kpos[j], 0), a.buckets - 1)] * kLog2e;
+          const float by = brow[t][bucket(at, kpos[j], a.buckets)] * kLog2e;
           p[t][j] = fmaf(s[j], scale2, by);
           if (exact.value && by < kNone) p[t][j] = -INFINITY;  // masked, whatever the key holds
         }
@@ -733,7 +733,7 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
           const float* row = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const float by = row[min(max(qp - kpos[j], 0), a.buckets - 1)] * kLog2e;
+            const float by = row[bucket(qp, kpos[j], a.buckets)] * kLog2e;
             z[t][j] = fmaf(z[t][j], scale2, by);
             if (exact && by < kNone) z[t][j] = -INFINITY;  // masked, whatever the key holds
           }

@@ -13,9 +13,9 @@ import math
 import pytest
 import torch
 
-import mrt_df
 from oracle import drafting_oracle as O
-from test_gpu_tree_attention import DEV, DT, bounds, call, make, oracle
+from test_gpu_cache_ops import check_commit, commit, make_commit
+from test_gpu_tree_attention import bounds, call, make, oracle
 
 pytestmark = pytest.mark.gpu
 
@@ -242,3 +242,25 @@ def test_absent_nodes_may_hold_anything(f, dtype):
     finite_check(s, dtype, out, ref, torch.ones(out.shape, dtype=torch.bool))
     there = torch.isfinite(rlse)
     assert torch.equal(there, torch.isfinite(lse)) and (lse.double() - rlse).abs()[there].max() <= bounds(s, dtype)[1]
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("nodes", [1, 25])
+def test_positions_at_the_ends_of_their_type(nodes, dtype):
+    """Distances beyond 31 bits count as far, or where they are negative as 0."""
+    s = make(67, dtype, 2, 4, 2, 64, nodes, [90, 40], buckets=7, evicted=True)
+    s["pos"][:, :, ::3] = -(2 ** 31)
+    s["pos"][:, :, 1::3] = 2 ** 31 - 1
+    s["next_pos"] = torch.tensor([2 ** 31 - 100, -(2 ** 31) + 5], dtype=torch.int32)
+    ref, rlse = oracle(s)
+    out, lse = call(s)
+    finite_check(s, dtype, out, ref, torch.ones(out.shape, dtype=torch.bool))
+    there = torch.isfinite(rlse)
+    assert (lse.double() - rlse).abs()[there].max() <= bounds(s, dtype)[1]
+    c = make_commit(67, dtype, 2, 4, 2, 64, nodes, [90, 40], [[0], [nodes - 1]], buckets=7, evicted=True)
+    c["pos"][:, :, ::3] = -(2 ** 31)
+    c["pos"][:, :, 1::3] = 2 ** 31 - 1
+    c["next_pos"] = s["next_pos"].clone()
+    c["lse"] = O.tree_attention(**{n: c[n] for n in ("q", "k_new", "v_new", "k", "v", "length", "parents", "scale", "bias",
+                                                     "pos", "next_pos")})[1].float()
+    check_commit(c, commit(c))
