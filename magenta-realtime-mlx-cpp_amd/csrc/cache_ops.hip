@@ -643,6 +643,15 @@ __global__ __launch_bounds__(256) void k_evict_move(const EvictK a, int blocks, 
   }
 }
 
+// Keys a lane in steps of 4, 256 slots: the threshold's search and the lists take a ballot a
+// key.  1024 heads of 1200 slots with 20 / 24 / 32 keys 20.4 / 21.9 / 24.6 us.
+template <int KPT>
+void launch_short(const EvictK& a, int heads, hipStream_t s) {
+  if constexpr (KPT * 64 < kShortSlots)
+    if (a.capacity > KPT * 64) return launch_short<KPT + 4>(a, heads, s);
+  hipLaunchKernelGGL(k_evict_short<KPT>, dim3(heads), dim3(256), 0, s, a);
+}
+
 // Most rows that a head can move; whether k_evict_short serves, and moves them itself.
 int most_moves(const KvCache& c, int keep) { return std::max(0, std::min(keep, c.capacity - keep)); }
 bool is_short(const KvCache& c) { return c.capacity <= kShortSlots; }
@@ -725,9 +734,7 @@ void cache_evict(const KvCache& c, const EvictArgs& t, void* ws, hipStream_t s) 
     a.movers = reinterpret_cast<int*>(take((size_t)heads * a.list));
     a.count = reinterpret_cast<int*>(take(heads));
   }
-  if (c.capacity <= 8 * 64) hipLaunchKernelGGL(k_evict_short<8>, dim3(heads), dim3(256), 0, s, a);
-  else if (c.capacity <= 18 * 64) hipLaunchKernelGGL(k_evict_short<18>, dim3(heads), dim3(256), 0, s, a);
-  else if (is_short(c)) hipLaunchKernelGGL(k_evict_short<32>, dim3(heads), dim3(256), 0, s, a);
+  if (is_short(c)) launch_short<4>(a, heads, s);
   else {
     const dim3 grid(heads * a.parts), block(kSelThreads);
     hipLaunchKernelGGL(k_evict_keys, grid, block, 0, s, a);

@@ -271,6 +271,14 @@ def test_evict(case, dtype):
     check_evict(s, evict(s, keep, recent, sinks), keep, recent, sinks)
 
 
+@pytest.mark.parametrize("capacity", [200, 256, 257, 512, 513, 768, 769, 1024, 1025, 1280, 1281, 1536, 1537, 1792, 1793, 2048, 2049])
+def test_evict_at_the_capacities_where_kernels_change(capacity):
+    s = make_evict(17, "bf16", 2, 2, 16, [capacity, capacity - 70], capacity=capacity)
+    s["score"][1, 1] = torch.randint(0, 5, (capacity,)).float()  # ties
+    for keep in (capacity - 40, capacity // 3):
+        check_evict(s, evict(s, keep, 9, 4), keep, 9, 4)
+
+
 def test_evict_ties_and_special_scores():
     """Equal scores go by the lower slot; NaN and -inf last, +inf first, -0 is 0."""
     s = make_evict(5, "bf16", 2, 2, 64, [300, 300], spread=False)
