@@ -601,8 +601,12 @@ int mrt_coca_read(mrt_coca* h, int which, void* dst, size_t bytes);
  * operator wants one, is the caller's, needs no initial contents, is aligned
  * to 16 bytes and serves one call at a time (calls that may overlap, two
  * captured graphs among them, take one each).  The calls may be captured into
- * a HIP graph.  Sums, softmax statistics and scores are fp32 in every dtype;
- * outputs are rounded to the dtype once.
+ * a HIP graph.  What a call writes must not overlap what it reads, unless it is
+ * said that it may.  Sums, softmax statistics and scores are fp32 in every dtype;
+ * outputs are rounded to the dtype once.  16-bit attention weights enter the
+ * product with the values as two parts of that type, within 2^-17 (bf16) or 2^-22
+ * (fp16) of them.  Weighted values are summed before they are divided by the sum
+ * of the weights: finite values beyond some 2^100 may overflow.
  * ------------------------------------------------------------------------ */
 
 /* The K/V of one layer for `rows` sequences.  k and v: (rows, kv_heads,
@@ -611,12 +615,13 @@ int mrt_coca_read(mrt_coca* h, int which, void* dst, size_t bytes);
  * 16 bytes) and d contiguous; d a multiple of 8, at most 256.  Sequence b has
  * length[b] entries, in slots 0 .. length[b] - 1 of every head (a length
  * outside [0, capacity] is taken as the nearest bound); what the other slots
- * hold has no effect.  capacity at most 2^30, rows * kv_heads 2^20.  pos: NULL where an entry's slot is its position
- * (the next token's is then length[b]); else (rows, kv_heads, capacity) int32
- * positions, in any order, and next_pos (rows) the next token's.  Sequences
- * and heads may share slots (stride 0) where the cache is only read; where it is
- * written, its slots and those of k and v lie apart.  score
- * (rows, kv_heads, capacity) fp32: accumulated attention weights, or NULL. */
+ * hold has no effect.  capacity at most 2^30, rows * kv_heads 2^20.  pos: NULL
+ * where an entry's slot is its position (the next token's is then length[b]);
+ * else (rows, kv_heads, capacity) int32 positions, in any order, and next_pos
+ * (rows) the next token's.  Sequences and heads may share slots (stride 0) where
+ * the cache is only read; where it is written, its slots and those of k and v lie
+ * apart.  score (rows, kv_heads, capacity) fp32: accumulated attention weights, or
+ * NULL. */
 typedef struct mrt_kv_cache {
   void* k;
   void* v;
@@ -674,9 +679,9 @@ typedef struct mrt_tree_attention_args {
  * and lse -inf.  One node is an ordinary decode step.  K/V of a node that t does not see have no effect on
  * t, whatever they hold; an infinite value that t does see makes the output
  * that infinity however small its weight, opposite ones or a NaN make it NaN.
- * Does not write the cache: mrt_cache_commit takes the
- * accepted nodes into it.  mrt_tree_attention_workspace gives the workspace
- * bytes for these sizes (0: none; workspace may then be NULL). */
+ * Does not write the cache: mrt_cache_commit takes the accepted nodes into it.
+ * mrt_tree_attention_workspace gives the workspace bytes for these sizes (0: none;
+ * workspace may then be NULL). */
 int mrt_tree_attention_workspace(const mrt_kv_cache* cache, int heads, int nodes, size_t* bytes);
 int mrt_tree_attention(const mrt_kv_cache* cache, const mrt_tree_attention_args* args, void* workspace,
                        size_t workspace_bytes, int device, void* hip_stream);

@@ -189,7 +189,7 @@ void launch_commit(const CommitK& a, int rows, int nr, hipStream_t s) {
 // collects its keys, k_evict_lists finds the other 22 bits from these in two passes, each
 // block by itself, and lists what moves: no block waits for another, and keys that are all
 // alike only make the collected ones more.
-// Bound: 64 x 16 heads from 1056 to 1006 entries, d 64 (43 MB), 18 us, one round of blocks
+// Bound: 64 x 16 heads from 1056 to 1006 entries, d 64 (43 MB), 19 us, one round of blocks
 // with five dependent steps; 4 x 8 heads from 65536 to 32768, d 128 (570 MB), 151 us, of
 // which 115 move rows at the rate of a copy and 37 find them (one block a head: 111).
 
@@ -655,8 +655,8 @@ void launch_short(const EvictK& a, int heads, hipStream_t s) {
 // Most rows that a head can move; whether k_evict_short serves, and moves them itself.
 int most_moves(const KvCache& c, int keep) { return std::max(0, std::min(keep, c.capacity - keep)); }
 bool is_short(const KvCache& c) { return c.capacity <= kShortSlots; }
-// Up to 16 KB of K rows a head: 1024 heads from 1056 to 1006, d 64, 18.3 us, with a kernel of
-// its own for the moves 20.3; to 928 28.3 and 29.0; 32 heads to 928 12.7 and 14.5.
+// Up to 16 KB of K rows a head: 1024 heads from 1056 to 1006, d 64, 18.7 us, with a kernel of
+// its own for the moves 21.0; to 928 28.3 and 29.0; 32 heads to 928 12.7 and 14.5.
 bool moves_within(const KvCache& c, int keep) {
   return is_short(c) && (size_t)most_moves(c, keep) * c.d * dtype_size(c.dt) <= 16 * 1024;
 }

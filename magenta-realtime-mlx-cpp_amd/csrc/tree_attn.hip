@@ -15,12 +15,13 @@
 //   8 / WR on different steps, share K and V through a ring of LDS stages that loads
 //   fill while products run.
 // What they reach (bf16; one pass of the call, the joining of parts among it): 3 sequences
-// of up to 65500 entries, 8 K/V heads, d 128, 60 rows (461 MB) 103 us, 4.5 TB/s, near the
+// of up to 65500 entries, 8 K/V heads, d 128, 60 rows (461 MB) 101 us, 4.6 TB/s, near the
 // rate of a large copy; 16 of up to 8191, 4 K/V heads, 512 rows (79 GFLOP, half as much again
-// for weights in two parts) 152 us, bound by the softmax between the products (187 vector
-// instructions a wave and step against 48 matrix ones); fp32, 4 of up to 4099, 12 heads, 7
-// rows (58 MB) 25 us, bound by a few dependent trips to memory; one node over 49 entries
-// 8 us of such trips.
+// for weights in two parts) 153 us, matrix cores busy for 33 % of the SIMDs' cycles and vector
+// instructions (187 a wave and step against 48 matrix ones) for 42 %, which overlap little;
+// fp32, 4 of up to 4099, 12 heads, 7 rows (58 MB) 25 us, bound by a few dependent trips to
+// memory; one node over 49 entries 8 us of such trips.  Infinities among a cache's values cost
+// a second round of steps (16 K/V heads of 4000 entries, 512 rows: 387 us instead of 58).
 // A unit's steps are cut where the card needs more blocks (Share); parts leave (maximum,
 // sum, output) in fp32 and k_tree_join sums them in order, so a result does not depend
 // on timing.  The cut is made on the device, from the lengths, which the host never sees.

@@ -1117,6 +1117,9 @@ class StyleModel:
 
 # ---- operators for drafting decode over the caller's own tensors --------------------
 #
+# They serve: autograd does not see them.  Tensors that require gradients are taken as
+# any others, and what a call returns has none.
+#
 # A small call takes the GPU a few microseconds, so the binding keeps its own share
 # low: structures are packed in one go, messages are built when a check fails, the
 # current stream is taken as a raw handle.
@@ -1224,7 +1227,7 @@ def tree_attention(q, k_new, v_new, cache: KVCache, parents, scale: float = 1.0,
     earlier node is that node's child, anything else is not there.  bias: fp32
     (heads, buckets) by distance.  Returns (out (rows, nodes, heads, d), lse
     (rows, nodes, heads) fp32), new tensors unless given, enqueued on torch's
-    current stream.  One node is an ordinary decode step.
+    current stream, without gradients.  One node is an ordinary decode step.
     """
     torch, lib, index = _torch(), load_library(), cache.index
     shape = q.shape
@@ -1327,7 +1330,7 @@ def q4_matmul(x, w, scales, biases, out=None):
 
     w int32 (n, k / 8), eight codes a word from the low bits; scales, biases
     (n, k / group) in x's dtype, group 32, 64 or 128: weight = scale * code +
-    bias.  ``q4_quantize`` makes them.
+    bias.  ``q4_quantize`` makes them.  The result has no gradients.
     """
     lib, torch, index = load_library(), _torch(), x.get_device()
     if x.dim() != 2 or w.dim() != 2 or scales.dim() != 2:
