@@ -16,7 +16,8 @@
 // from tables of bytes (18 instructions for eight codes instead of 7), which puts y off by
 // 4e-7: 5 x 1024 by 29824 13.0 us instead of 12.2.  fp32 rows are split exactly into three bf16
 // parts.  In bf16 and fp32 the codes, and so all sums, are 2^-12 or 2^-11 of what they stand
-// for until the end, so that terms that cancel do not overflow where y does not.
+// for until the end, so that terms that cancel do not overflow where y does not (and y below
+// 2^-114 loses bits).
 //
 // A block takes 16 NT output columns (matrix-core rows), its waves chunks of 128 k in
 // turn, summed through LDS in order.  A lane loads 32 codes (16 bytes) of one row; two
