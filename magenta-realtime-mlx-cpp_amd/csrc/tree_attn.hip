@@ -763,8 +763,8 @@ __global__ __launch_bounds__(512) void k_tree_many(const TreeArgs a) {
                                                 fmaxf(fmaxf(z[t][4], z[t][5]), fmaxf(z[t][6], z[t][7])))) *
                               mult -
                           kShift;
-        if (__any(top > m[t] + kSlack)) {
-          const float mn = fmaxf(m[t], top), f = fade(m[t] - mn);
+        if (__any(top > m[t] + kSlack)) {  // each row by itself: its bits do not depend on the others'
+          const float mn = top > m[t] + kSlack ? top : m[t], f = fade(m[t] - mn);
           m[t] = mn;
           l[t] *= f;
 #pragma unroll

@@ -225,23 +225,36 @@ def test_scales_of_every_kind(nodes, buckets, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "fp16", "fp32"])
 @pytest.mark.parametrize("f", FORMS, ids=IDS)
 def test_absent_nodes_may_hold_anything(f, dtype):
-    """Padding: q, k_new and v_new of absent nodes that nobody wrote.  In 16 bits the reference
-    of a row's weights follows when any row of its tile asks for it, so other rows may move
-    its last bits: the oracle's tolerances, not the bits."""
+    """Padding: q, k_new and v_new of absent nodes that nobody wrote.  No bit of the others
+    depends on them."""
     s = form(65, dtype, f)
     nodes = f[3]
     s["parents"][:, (nodes + 1) // 2:] = -9
     for n in ("q", "k_new", "v_new"):
         s[n][:, (nodes + 1) // 2:] = 0
     ref, rlse = oracle(s)
-    dirty = dict(s)
-    for n, bad in (("q", math.nan), ("k_new", math.inf), ("v_new", -math.inf)):
-        dirty[n] = s[n].clone()
-        dirty[n][:, (nodes + 1) // 2:] = bad
-    out, lse = call(dirty)
-    finite_check(s, dtype, out, ref, torch.ones(out.shape, dtype=torch.bool))
     there = torch.isfinite(rlse)
-    assert torch.equal(there, torch.isfinite(lse)) and (lse.double() - rlse).abs()[there].max() <= bounds(s, dtype)[1]
+    clean = call(s)
+    for bad in ((math.nan, math.inf, -math.inf), (60.0, -60.0, 1e4)):
+        dirty = dict(s)
+        for n, x in zip(("q", "k_new", "v_new"), bad):
+            dirty[n] = s[n].clone()
+            dirty[n][:, (nodes + 1) // 2:] = x
+        out, lse = call(dirty)
+        finite_check(s, dtype, out, ref, torch.ones(out.shape, dtype=torch.bool))
+        assert torch.equal(there, torch.isfinite(lse)) and (lse.double() - rlse).abs()[there].max() <= bounds(s, dtype)[1]
+        assert torch.equal(out, clean[0]) and torch.equal(lse, clean[1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("f", FORMS, ids=IDS)
+def test_rows_do_not_depend_on_each_other(f, dtype):
+    """Other queries for one node: the other nodes' bits stay."""
+    s = form(69, dtype, f)
+    clean = call(s)
+    s["q"][:, -1] = s["q"][:, -1] * 7 + 1
+    got = call(s)
+    assert torch.equal(got[0][:, :-1], clean[0][:, :-1]) and torch.equal(got[1][:, :-1], clean[1][:, :-1])
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
