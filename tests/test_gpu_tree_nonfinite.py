@@ -249,12 +249,15 @@ def test_absent_nodes_may_hold_anything(f, dtype):
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 @pytest.mark.parametrize("f", FORMS, ids=IDS)
 def test_rows_do_not_depend_on_each_other(f, dtype):
-    """Other queries for one node: the other nodes' bits stay."""
+    """Other queries for one node, NaN too: the other nodes' bits stay."""
     s = form(69, dtype, f)
     clean = call(s)
-    s["q"][:, -1] = s["q"][:, -1] * 7 + 1
-    got = call(s)
-    assert torch.equal(got[0][:, :-1], clean[0][:, :-1]) and torch.equal(got[1][:, :-1], clean[1][:, :-1])
+    for q in (s["q"][:, -1] * 7 + 1, math.nan):
+        run = dict(s, q=s["q"].clone())
+        run["q"][:, -1] = q
+        got = call(run)
+        assert torch.equal(got[0][:, :-1], clean[0][:, :-1]) and torch.equal(got[1][:, :-1], clean[1][:, :-1])
+    assert got[0][:, -1].isnan().all() and got[1][:, -1].isnan().all()
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
