@@ -755,6 +755,164 @@ int mrt_q4_matmul(const void* x, int64_t ldx, int rows, const uint32_t* w, const
 int mrt_q4_quantize(const void* src, int64_t ld, int n, int k, int group, int dtype, uint32_t* w, void* scales,
                     void* biases, int device, void* hip_stream);
 
+/* ------------------------------------------------------------------------
+ * Operators of a server's step over caches in pages, in 8 bits.  No counterpart
+ * in the reference.  The conventions are those of the drafting operators above:
+ * device pointers, the caller's stream and workspace, no allocation, calls that
+ * may be captured, errors before any device work.  A step: products
+ * (mrt_i8_quantize, mrt_i8_matmul), the new tokens' keys and values into the
+ * pages (mrt_paged_write), their attention (mrt_paged_attention), and for
+ * drafted tokens which of them stand (mrt_draft_verify).
+ * ------------------------------------------------------------------------ */
+
+/* Pages of 8-bit codes: an entry's d values of a head are code * scale. */
+#define MRT_PAGES_I8 3
+
+/* The K/V of one layer for `rows` sequences, in pages of a pool.  k and v:
+ * (pages, kv_heads, page_size, d) with element strides page_stride, head_stride
+ * and slot_stride (those of both; multiples of 16 bytes) and d contiguous, in
+ * `dtype`: MRT_DTYPE_*, d a multiple of 8, or MRT_PAGES_I8, d a multiple of 16;
+ * at most 256.  With codes also k_scale and v_scale, (pages, kv_heads, page_size)
+ * fp32, 16-byte aligned, not negative.  page_size is a multiple of 16, at most
+ * 2^16.  table (rows, row_pages), table_stride elements between sequences: entries
+ * x page_size .. of sequence b are in page table[b][x]; an id outside [0, pages)
+ * means that there is no page, whose entries are neither seen, read nor written.
+ * Sequence b has length[b] entries (outside [0, row_pages * page_size], at most
+ * 2^30: the nearest bound).  Sequences may share pages as long as only one
+ * writes to them. */
+typedef struct mrt_paged_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* table;
+  const int32_t* length;
+  int64_t page_stride;
+  int64_t head_stride;
+  int64_t slot_stride;
+  int64_t table_stride;
+  int32_t pages;
+  int32_t rows;
+  int32_t row_pages;
+  int32_t kv_heads;
+  int32_t page_size;
+  int32_t d;
+  int32_t dtype;
+} mrt_paged_cache;
+
+typedef struct mrt_paged_store_args {
+  mrt_node_rows k;       /* (rows, tokens, kv_heads, d) of `dtype`; written by mrt_paged_read */
+  mrt_node_rows v;
+  const int32_t* fresh;  /* write: (rows) tokens that are there, 0 .. tokens; NULL: all */
+  const int32_t* start;  /* read: (rows) the first entry; NULL: 0 */
+  int32_t* length_out;   /* write: (rows), an array of its own, or NULL */
+  int32_t tokens;        /* >= 1 */
+  int32_t dtype;         /* of k and v: the pages' own, any of the three for codes */
+} mrt_paged_store_args;
+
+/* Writes the first fresh[b] of each sequence's tokens to its entries length[b] ..;
+ * what the pages have no room for is left out.  length_out = min(length + fresh,
+ * row_pages * page_size).  Codes: scale = max |x| * (1/127) of the d values of an
+ * entry and head, code = the quotient x / scale (fp32) to the nearest whole
+ * number; an entry that holds an infinity or NaN has scale NaN, and reads as NaN. */
+int mrt_paged_write(const mrt_paged_cache* cache, const mrt_paged_store_args* args, int device, void* hip_stream);
+/* Reads entries start[b] + t, t < tokens, of each sequence; what is at or past its
+ * length or in no page is left as it was in k and v. */
+int mrt_paged_read(const mrt_paged_cache* cache, const mrt_paged_store_args* args, int device, void* hip_stream);
+
+typedef struct mrt_paged_attention_args {
+  mrt_node_rows q;       /* (rows, tokens, heads, d) of `dtype` */
+  mrt_node_rows out;     /* the same */
+  const int32_t* fresh;  /* (rows) new tokens that are there; NULL: all */
+  float* lse;            /* (rows, tokens, heads) fp32 log-sum-exp of the logits, or NULL */
+  const float* bias;     /* (heads, buckets) fp32 logit bias by distance, or NULL */
+  int32_t buckets;       /* with bias: 1 .. 2^18 */
+  int32_t tokens;        /* 1 .. MRT_MAX_NODES */
+  int32_t heads;         /* a multiple of kv_heads */
+  int32_t dtype;         /* of q and out: the pages' own, any of the three for codes */
+  float scale;           /* 1 in this model (no 1/sqrt(d)) */
+} mrt_paged_attention_args;
+
+/* Attention of each sequence's newest tokens, whose keys and values are in the
+ * cache already (mrt_paged_write, the same length and fresh): token t sees entries
+ * 0 .. length[b] + t,
+ *   logit(t, j) = scale * q_t . k_j + bias[h][min(length + t - j, buckets - 1)].
+ * Tokens past fresh[b], and those that see nothing, have output 0 and lse -inf.
+ * Masks by the bias, and infinities and NaN in entries that a token does not
+ * see, are treated as in mrt_tree_attention.  Over codes a row of q that holds an
+ * infinity or NaN gives NaN; q is taken as whole multiples of 2^-22 (or up to 2^-21) of
+ * its largest magnitude, and weights times scales likewise among 64 entries, and
+ * what is below 2^-104 counts as 0. */
+int mrt_paged_attention_workspace(const mrt_paged_cache* cache, int heads, int tokens, size_t* bytes);
+int mrt_paged_attention(const mrt_paged_cache* cache, const mrt_paged_attention_args* args, void* workspace,
+                        size_t workspace_bytes, int device, void* hip_stream);
+
+typedef struct mrt_draft_verify_args {
+  const void* target;       /* (rows, nodes + 1, vocab) of `dtype` */
+  const void* draft;        /* (rows, nodes, vocab), or NULL: the tokens were not drawn */
+  int64_t target_row_stride;
+  int64_t target_slot_stride;
+  int64_t draft_row_stride;
+  int64_t draft_slot_stride;
+  const int32_t* tokens;    /* (rows, nodes) */
+  const int32_t* parents;   /* (rows, nodes) as in mrt_tree_attention; NULL: each follows the one before */
+  int64_t parents_stride;   /* elements between sequences' parents; 0: one tree for all */
+  const float* uniforms;    /* (rows, nodes + 1) random numbers in [0, 1): a node's, then the last draw's */
+  int32_t* accepted;        /* (rows, nodes): as mrt_cache_commit takes it */
+  int32_t* count;           /* (rows) accepted nodes */
+  int32_t* token;           /* (rows) the token after them */
+  int32_t rows;
+  int32_t nodes;            /* 1 .. MRT_MAX_NODES */
+  int32_t vocab;            /* 1 .. 2^24 */
+  int32_t dtype;
+} mrt_draft_verify_args;
+
+/* Which path of a drafted tree the target's probabilities accept, and the next
+ * token.  Slot 0 follows the cache, slot t + 1 node t: target[b][s] are the
+ * target's probabilities of the token at slot s, draft[b][s] those that the nodes
+ * at slot s (its children) were drawn from, each by itself.  From slot 0 on, with
+ * r = target[s], Z = 1, the children in order of their ids:
+ *   uniforms[child] * Z * draft[s][x] < r[x]: the child, of token x, is accepted,
+ *   and its own slot is next; else r = max(r - Z draft[s], 0), Z = sum of r.
+ * Where none is accepted the walk ends with a token from r: the least i with
+ * r[0] + .. + r[i] > uniforms[nodes] * sum of r; where nothing is left of r, from
+ * target[s]; -1 if that has nothing either.  The tokens so taken are distributed as
+ * the target's own draws.  Without draft: uniforms[child] * Z < r[x], else r[x] = 0
+ * and Z = Z - r[x].  In 64 bits; probabilities that are not positive finite
+ * numbers count as 0, nodes with a token outside the vocabulary as absent.
+ * accepted: the path's ids, ascending, then -1. */
+int mrt_draft_verify(const mrt_draft_verify_args* args, int device, void* hip_stream);
+
+/* 8-bit codes of the rows of src (rows, k), row stride ld, in `dtype`: scales (rows)
+ * and codes (rows, k), row stride ldc, as mrt_paged_write makes them; a row that
+ * holds an infinity or NaN has scale NaN.  k is a multiple of 16, below 2^17; row
+ * strides are multiples of 16 bytes, src and codes 16-byte aligned. */
+int mrt_i8_quantize(const void* src, int64_t ld, int rows, int k, int dtype, int8_t* codes, int64_t ldc, float* scales,
+                    int device, void* hip_stream);
+
+typedef struct mrt_i8_matmul_args {
+  const int8_t* x;       /* (rows, k), row stride ldx */
+  const float* x_scale;  /* (rows) */
+  const int8_t* w;       /* (n, k), row stride ldw */
+  const float* w_scale;  /* (n) */
+  const void* add;       /* (rows, n) of `dtype`, row stride lda, or NULL; may be out itself */
+  void* out;             /* (rows, n) of `dtype`, row stride ldo */
+  int64_t ldx;
+  int64_t ldw;
+  int64_t lda;
+  int64_t ldo;
+  int32_t rows;
+  int32_t n;
+  int32_t k;
+  int32_t dtype;
+} mrt_i8_matmul_args;
+
+/* out = (x w^T) x_scale w_scale + add: a scale for each row and each column.  The
+ * products are summed exactly; the sum is rounded to fp32, scaled and added to in
+ * fp32, and rounded to `dtype`.  k is a multiple of 16, below 2^17; ldx and ldw are
+ * multiples of 16, x and w 16-byte aligned. */
+int mrt_i8_matmul(const mrt_i8_matmul_args* args, int device, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -31,6 +31,10 @@ SOURCES = [
     "tree_attn.hip",
     "cache_ops.hip",
     "q4.hip",
+    "paged_attn.hip",
+    "paged_store.hip",
+    "verify.hip",
+    "i8.hip",
     "codec_kernels.hip",
     "conv_split.hip",
     "coca_kernels.hip",

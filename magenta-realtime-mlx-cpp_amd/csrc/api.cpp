@@ -12,12 +12,15 @@
 #include "batch.hpp"
 #include "coca.hpp"
 #include "codec.hpp"
+#include "i8.hpp"
 #include "kernels.hpp"
 #include "kv_cache.hpp"
 #include "model.hpp"
+#include "paged.hpp"
 #include "q4.hpp"
 #include "split_gemm.hpp"
 #include "stream.hpp"
+#include "verify.hpp"
 
 struct mrt_df {
   std::unique_ptr<mrt::Model> model;
@@ -236,16 +239,19 @@ mrt::KvCache to_cache(const mrt_kv_cache* c, bool data = true) {
   return k;
 }
 
-mrt::NodeRows to_nodes(const mrt_node_rows& r, const mrt::KvCache& c, int nodes, int heads, const char* null_msg) {
+mrt::NodeRows to_nodes(const mrt_node_rows& r, mrt::DType dt, int rows, int nodes, int heads, const char* null_msg) {
   require(r.data != nullptr, null_msg);
-  const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(c.dt));
+  const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(dt));
   require(aligned(r.data, 16), "nodes: operands must be 16-byte aligned");
-  require(stride_ok(r.row_stride, c.rows, unit) && stride_ok(r.node_stride, nodes, unit) &&
+  require(stride_ok(r.row_stride, rows, unit) && stride_ok(r.node_stride, nodes, unit) &&
               stride_ok(r.head_stride, heads, unit),
           "nodes: strides must be multiples of 16 bytes, not negative");
   mrt::NodeRows n;
   n.p = r.data, n.row_stride = r.row_stride, n.node_stride = r.node_stride, n.head_stride = r.head_stride;
   return n;
+}
+mrt::NodeRows to_nodes(const mrt_node_rows& r, const mrt::KvCache& c, int nodes, int heads, const char* null_msg) {
+  return to_nodes(r, c.dt, c.rows, nodes, heads, null_msg);
 }
 
 // An array of vectors of d elements: extents and strides of its dimensions, largest stride
@@ -288,12 +294,13 @@ void check_own_slots(const mrt::KvCache& c) {
   require(!slots.meets(bytes / static_cast<int64_t>(mrt::dtype_size(c.dt))), "cache: k and v overlap");
 }
 
-void check_heads(const mrt::KvCache& c, int heads, int nodes) {
-  require(heads >= 1 && heads % c.kv_heads == 0, "heads must be a multiple of kv_heads");
+void check_heads(int rows, int kv_heads, int heads, int nodes) {
+  require(heads >= 1 && heads % kv_heads == 0, "heads must be a multiple of kv_heads");
   require(heads <= 4096, "at most 4096 heads");
   require(nodes >= 1 && nodes <= mrt::kMaxNodes, "nodes must be in 1..64");
-  require(static_cast<int64_t>(c.rows) * heads * nodes < (1ll << 31), "rows * heads * nodes must be below 2^31");
+  require(static_cast<int64_t>(rows) * heads * nodes < (1ll << 31), "rows * heads * nodes must be below 2^31");
 }
+void check_heads(const mrt::KvCache& c, int heads, int nodes) { check_heads(c.rows, c.kv_heads, heads, nodes); }
 
 constexpr char kTreeTooLarge[] = "tree_attention: too many sequences, heads and nodes for one call";
 
@@ -307,6 +314,76 @@ void check_bias(const float* bias, int buckets) {
   require(bias == nullptr || buckets >= 1, "bias without buckets");
   require(bias == nullptr || buckets <= (1 << 18), "bias: at most 2^18 buckets");
   require(bias == nullptr || aligned(bias, 4), "bias must be 4-byte aligned");
+}
+
+// Sizes and strides; the pointers only with `data`.
+mrt::PagedCache to_pages(const mrt_paged_cache* c, bool data = true) {
+  require(c != nullptr, "null cache");
+  mrt::PagedCache k;
+  k.codes = c->dtype == MRT_PAGES_I8;
+  if (!k.codes) k.dt = to_dtype(c->dtype);
+  require(c->rows >= 0 && c->kv_heads >= 1 && c->pages >= 1 && c->row_pages >= 1,
+          "pages: rows >= 0, kv_heads >= 1, pages >= 1 and row_pages >= 1");
+  require(c->page_size >= mrt::kPageUnit && c->page_size <= (1 << 16) && c->page_size % mrt::kPageUnit == 0,
+          "pages: page_size must be a multiple of 16, at most 2^16");
+  const int unit = k.codes ? 16 : 8;
+  require(c->d >= unit && c->d <= mrt::kMaxHeadDim && c->d % unit == 0,
+          "pages: d must be a multiple of 8, with 8-bit codes of 16, and at most 256");
+  require(static_cast<int64_t>(c->row_pages) * c->page_size <= (1 << 30), "pages: at most 2^30 entries a sequence");
+  require(static_cast<int64_t>(c->rows) * c->kv_heads <= (1 << 20), "pages: more than 2^20 (row, head) pairs");
+  if (data && c->rows > 0) {
+    require(c->k && c->v && c->table && c->length, "pages: null k, v, table or length");
+    require(aligned(c->k, 16) && aligned(c->v, 16), "pages: k and v must be 16-byte aligned");
+    require(!k.codes || (c->k_scale && c->v_scale && aligned(c->k_scale, 16) && aligned(c->v_scale, 16)),
+            "pages: 8-bit codes need k_scale and v_scale, 16-byte aligned");
+    const int64_t step = k.codes ? 16 : 16 / static_cast<int64_t>(mrt::dtype_size(k.dt));
+    require(stride_ok(c->page_stride, c->pages, step) && stride_ok(c->head_stride, c->kv_heads, step) &&
+                stride_ok(c->slot_stride, c->page_size, step),
+            "pages: strides must be multiples of 16 bytes, not negative");
+    require(c->table_stride >= 0, "pages: negative table_stride");
+    require(aligned4({c->table, c->length}), "pages: table and length must be 4-byte aligned");
+  }
+  k.k = c->k, k.v = c->v, k.k_scale = c->k_scale, k.v_scale = c->v_scale, k.table = c->table, k.length = c->length;
+  k.page_stride = c->page_stride, k.head_stride = c->head_stride, k.slot_stride = c->slot_stride;
+  k.table_stride = c->table_stride, k.pages = c->pages, k.rows = c->rows, k.row_pages = c->row_pages;
+  k.kv_heads = c->kv_heads, k.page_size = c->page_size, k.d = c->d;
+  return k;
+}
+
+// The type of operands that go with these pages.
+mrt::DType operand_type(const mrt::PagedCache& c, int dtype) {
+  const mrt::DType dt = to_dtype(dtype);
+  require(c.codes || dt == c.dt, "pages: operands must be of the pages' type");
+  return dt;
+}
+
+mrt::PagedStoreArgs to_store(const mrt::PagedCache& c, const mrt_paged_store_args* args) {
+  mrt::PagedStoreArgs a;
+  a.dt = operand_type(c, args->dtype);
+  require(args->tokens >= 1, "pages: tokens must be >= 1");
+  require(static_cast<int64_t>(c.rows) * c.kv_heads * args->tokens <= (1 << 27), "pages: rows * kv_heads * tokens above 2^27");
+  a.k = to_nodes(args->k, a.dt, c.rows, args->tokens, c.kv_heads, "pages: null k rows");
+  a.v = to_nodes(args->v, a.dt, c.rows, args->tokens, c.kv_heads, "pages: null v rows");
+  require(aligned4({args->fresh, args->start, args->length_out}), "pages: fresh, start and length_out must be 4-byte aligned");
+  a.fresh = args->fresh, a.start = args->start, a.length_out = args->length_out, a.tokens = args->tokens;
+  return a;
+}
+
+// Two arrays of vectors that are written: neither overlaps itself, nor, where they are
+// laid out alike, the other.
+void check_apart(const Vectors& x, const Vectors& y, const void* px, const void* py, size_t size, const char* msg) {
+  require(x.apart() && y.apart(), msg);
+  bool alike = true;
+  for (int i = 0; i < 3; ++i) alike = alike && x.dims[i].size == y.dims[i].size && x.dims[i].stride == y.dims[i].stride;
+  const __int128 bytes = static_cast<__int128>(reinterpret_cast<uintptr_t>(py)) - reinterpret_cast<uintptr_t>(px);
+  require(alike ? !x.meets(bytes / static_cast<int64_t>(size)) : px != py, msg);
+}
+
+constexpr char kPagedTooLarge[] = "paged_attention: too many sequences, heads and tokens for one call";
+
+void check_i8(int rows, int k) {
+  require(rows >= 0 && rows <= (1 << 24), "8-bit products: rows must be in 0..2^24");
+  require(k >= 16 && k % 16 == 0 && k < (1 << 17), "8-bit products: k must be a multiple of 16, below 2^17");
 }
 
 mrt::CodecConfig to_codec_config(const mrt_codec_config* c, int* max_frames) {
@@ -1161,6 +1238,147 @@ int mrt_q4_quantize(const void* src, int64_t ld, int n, int k, int group, int dt
     require(ld >= k || n == 1, "q4_quantize: ld must be >= k");
     OnDevice on(device);
     mrt::q4_quantize(dt, src, ld, n, k, group, w, scales, biases, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_paged_write(const mrt_paged_cache* cache, const mrt_paged_store_args* args, int device, void* hip_stream) {
+  return guarded([&] {
+    require(args != nullptr, "null argument");
+    const mrt::PagedCache c = to_pages(cache);
+    if (c.rows == 0) return;
+    const mrt::PagedStoreArgs a = to_store(c, args);
+    require(a.length_out == nullptr || (a.length_out != c.length && a.length_out != a.fresh),
+            "paged_write: length_out must be an array of its own");
+    const Vectors slots(c.d, {c.pages, c.page_stride}, {c.kv_heads, c.head_stride}, {c.page_size, c.slot_stride});
+    check_apart(slots, slots, c.k, c.v, c.codes ? 1 : mrt::dtype_size(c.dt), "pages: pages, heads, slots or k and v overlap");
+    require(!c.codes || c.k_scale != c.v_scale, "pages: k_scale and v_scale overlap");
+    OnDevice on(device);
+    mrt::paged_write(c, a, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_paged_read(const mrt_paged_cache* cache, const mrt_paged_store_args* args, int device, void* hip_stream) {
+  return guarded([&] {
+    require(args != nullptr, "null argument");
+    const mrt::PagedCache c = to_pages(cache);
+    if (c.rows == 0) return;
+    const mrt::PagedStoreArgs a = to_store(c, args);
+    auto vectors = [&](const mrt::NodeRows& r) {
+      return Vectors(c.d, {c.rows, r.row_stride}, {a.tokens, r.node_stride}, {c.kv_heads, r.head_stride});
+    };
+    check_apart(vectors(a.k), vectors(a.v), a.k.p, a.v.p, mrt::dtype_size(a.dt), "paged_read: k or v overlaps itself or the other");
+    OnDevice on(device);
+    mrt::paged_read(c, a, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_paged_attention_workspace(const mrt_paged_cache* cache, int heads, int tokens, size_t* bytes) {
+  return guarded([&] {
+    require(bytes != nullptr, "null argument");
+    const mrt::PagedCache c = to_pages(cache, false);
+    check_heads(c.rows, c.kv_heads, heads, tokens);
+    require(mrt::paged_attention_fits(c, heads, tokens), kPagedTooLarge);
+    *bytes = mrt::paged_attention_workspace(c, heads, tokens);
+  });
+}
+
+int mrt_paged_attention(const mrt_paged_cache* cache, const mrt_paged_attention_args* args, void* workspace,
+                        size_t workspace_bytes, int device, void* hip_stream) {
+  return guarded([&] {
+    require(args != nullptr, "null argument");
+    const mrt::PagedCache c = to_pages(cache);
+    if (c.rows == 0) return;
+    check_heads(c.rows, c.kv_heads, args->heads, args->tokens);
+    check_bias(args->bias, args->buckets);
+    mrt::PagedAttnArgs a;
+    a.dt = operand_type(c, args->dtype);
+    a.q = to_nodes(args->q, a.dt, c.rows, args->tokens, args->heads, "paged_attention: null q");
+    a.out = to_nodes(args->out, a.dt, c.rows, args->tokens, args->heads, "paged_attention: null out");
+    require(Vectors(c.d, {c.rows, a.out.row_stride}, {args->tokens, a.out.node_stride}, {args->heads, a.out.head_stride}).apart(),
+            "paged_attention: out overlaps itself");
+    require(aligned4({args->fresh, args->lse}), "paged_attention: fresh and lse must be 4-byte aligned");
+    a.fresh = args->fresh, a.lse = args->lse, a.bias = args->bias, a.buckets = args->bias ? args->buckets : 0;
+    a.tokens = args->tokens, a.heads = args->heads, a.scale = args->scale;
+    require(mrt::paged_attention_fits(c, a.heads, a.tokens), kPagedTooLarge);
+    const size_t want = mrt::paged_attention_workspace(c, a.heads, a.tokens);
+    require(want == 0 || (workspace != nullptr && workspace_bytes >= want && aligned(workspace, 16)),
+            "paged_attention: workspace too small, misaligned or null");
+    OnDevice on(device);
+    mrt::paged_attention(c, a, workspace, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_draft_verify(const mrt_draft_verify_args* args, int device, void* hip_stream) {
+  return guarded([&] {
+    require(args != nullptr, "null argument");
+    const mrt::DType dt = to_dtype(args->dtype);
+    require(args->rows >= 0 && args->rows <= (1 << 20), "draft_verify: rows must be in 0..2^20");
+    if (args->rows == 0) return;
+    require(args->nodes >= 1 && args->nodes <= mrt::kMaxNodes, "draft_verify: nodes must be in 1..64");
+    require(args->vocab >= 1 && args->vocab <= (1 << 24), "draft_verify: vocab must be in 1..2^24");
+    require(args->target && args->tokens && args->uniforms && args->accepted && args->count && args->token,
+            "draft_verify: null argument");
+    const size_t size = mrt::dtype_size(dt);
+    require(aligned(args->target, size) && aligned(args->draft, size), "draft_verify: target and draft must be aligned to their elements");
+    require(args->target_row_stride >= 0 && args->target_slot_stride >= 0 && args->draft_row_stride >= 0 &&
+                args->draft_slot_stride >= 0 && args->parents_stride >= 0,
+            "draft_verify: negative stride");
+    require(aligned4({args->tokens, args->parents, args->uniforms, args->accepted, args->count, args->token}),
+            "draft_verify: int32 and fp32 arrays must be 4-byte aligned");
+    require(args->accepted != args->count && args->accepted != args->token && args->count != args->token,
+            "draft_verify: outputs must be arrays of their own");
+    mrt::VerifyArgs a;
+    a.target = args->target, a.draft = args->draft, a.t_row = args->target_row_stride, a.t_slot = args->target_slot_stride;
+    a.d_row = args->draft_row_stride, a.d_slot = args->draft_slot_stride, a.tokens = args->tokens;
+    a.parents = args->parents, a.parents_stride = args->parents_stride, a.uniforms = args->uniforms;
+    a.accepted = args->accepted, a.count = args->count, a.token = args->token;
+    a.rows = args->rows, a.nodes = args->nodes, a.vocab = args->vocab;
+    OnDevice on(device);
+    mrt::draft_verify(dt, a, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_i8_quantize(const void* src, int64_t ld, int rows, int k, int dtype, int8_t* codes, int64_t ldc, float* scales,
+                    int device, void* hip_stream) {
+  return guarded([&] {
+    const mrt::DType dt = to_dtype(dtype);
+    check_i8(rows, k);
+    if (rows == 0) return;
+    require(src && codes && scales, "i8_quantize: null argument");
+    require(aligned(src, 16) && aligned(codes, 16) && aligned(scales, 4), "i8_quantize: src and codes must be 16-byte aligned, scales 4");
+    const int64_t unit = 16 / static_cast<int64_t>(mrt::dtype_size(dt));
+    require(rows == 1 || (ld >= k && ld % unit == 0 && ldc >= k && ldc % 16 == 0),
+            "i8_quantize: row strides must be >= k, multiples of 16 bytes");
+    OnDevice on(device);
+    mrt::i8_quantize(dt, src, ld, rows, k, codes, ldc, scales, static_cast<hipStream_t>(hip_stream));
+  });
+}
+
+int mrt_i8_matmul(const mrt_i8_matmul_args* args, int device, void* hip_stream) {
+  return guarded([&] {
+    require(args != nullptr, "null argument");
+    const mrt::DType dt = to_dtype(args->dtype);
+    check_i8(args->rows, args->k);
+    require(args->n >= 1 && args->n <= (1 << 26), "i8_matmul: n must be in 1..2^26");
+    require((static_cast<int64_t>(args->rows) / 64 + 1) * (args->n / 64 + 1) < (1ll << 31), "i8_matmul: too many rows and columns");
+    if (args->rows == 0) return;
+    require(args->x && args->x_scale && args->w && args->w_scale && args->out, "i8_matmul: null argument");
+    require(aligned(args->x, 16) && aligned(args->w, 16), "i8_matmul: x and w must be 16-byte aligned");
+    const size_t size = mrt::dtype_size(dt);
+    require(aligned4({args->x_scale, args->w_scale}) && aligned(args->add, size) && aligned(args->out, size),
+            "i8_matmul: scales, add and out must be aligned to their elements");
+    require((args->rows == 1 || (args->ldx >= args->k && args->ldx % 16 == 0)) &&
+                (args->n == 1 || (args->ldw >= args->k && args->ldw % 16 == 0)),
+            "i8_matmul: ldx and ldw must be >= k, multiples of 16");
+    require(args->rows == 1 || (args->ldo >= args->n && (args->add == nullptr || args->lda >= 0)),
+            "i8_matmul: ldo must be >= n, lda not negative");
+    require(args->add != args->out || args->rows == 1 || args->lda == args->ldo, "i8_matmul: add in place needs out's row stride");
+    mrt::I8Args a;
+    a.x = args->x, a.x_scale = args->x_scale, a.w = args->w, a.w_scale = args->w_scale, a.add = args->add, a.out = args->out;
+    a.ldx = args->ldx, a.ldw = args->ldw, a.lda = args->lda, a.ldo = args->ldo;
+    a.rows = args->rows, a.n = args->n, a.k = args->k;
+    OnDevice on(device);
+    mrt::i8_matmul(dt, a, static_cast<hipStream_t>(hip_stream));
   });
 }
 

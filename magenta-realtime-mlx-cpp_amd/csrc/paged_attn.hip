@@ -1,0 +1,965 @@
+// Attention of a sequence's newest tokens over a cache in pages.
+//
+// Query t of a sequence's n new tokens sees the entries 0 .. length + t, its own among
+// them:
+//   s_tj = scale q_t . k_j + bias[h, min(length + t - j, M - 1)],  out_t = softmax(s_t) V.
+// One pass over the keys with the running maximum and sum of the softmax.  Few query rows
+// meet each key (a K/V head, a unit, has R = tokens heads / kv_heads of them), so reading the
+// keys is what it costs: straight from memory to registers, the waves of a block taking
+// steps in turn.  Pages are multiples of 16 entries, so the 16 keys of a matrix tile share a
+// page: a wave looks up its next 64 tiles in its lanes at once and then needs a scalar for
+// each.
+//
+// Pages of the operands' type: the fragments of attn_frag.hpp, 32 keys a step.
+//
+// Pages of 8-bit codes: 64 keys a step, and both products in integers.  Converting codes to
+// 16 bits would cost a vector instruction for two of them; instead the few query rows and
+// weights become three digits of 8 bits,
+//   x = f (65536 a + 256 b + c),  a, b, c in [-128, 127],
+// f a power of two for the row (of weights: for the row and step) by which its largest
+// magnitude is in [2^21, 2^22), so that x is within 2^-22 of that magnitude; sums of products
+// with codes are exact.  Scales of keys multiply scores, those of values the weights.  S^T = K Q^T leaves
+// lane (i, g) with keys 16 t + 4 g + r of the four tiles, just the 16 keys whose codes of one
+// dimension, transposed in registers by byte permutations, are its operand of
+// O^T = V^T P^T.
+//
+// A unit's steps are cut into parts of equal size where the card needs more blocks, on the
+// device, from the lengths, which the host never sees; parts leave (maximum, sum, output)
+// in fp32 and k_paged_join sums them in order, so a result does not depend on timing.
+#include <algorithm>
+#include <type_traits>
+
+#include "attn_frag.hpp"
+#include "mfma_ring.hpp"
+#include "paged.hpp"
+
+namespace mrt {
+namespace {
+
+constexpr int kBiasLds = 4096;  // floats of the bias by distance kept in LDS
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
+struct PageArgs {
+  const void *q, *k, *v;
+  void* out;
+  const float *k_scale, *v_scale, *bias;
+  const int *table, *length, *fresh;
+  float* lse;
+  float* part;      // (slots, R, D) outputs of the parts
+  float2* part_ml;  // (slots, R) maximum (in log2 units) and sum
+  int64_t q_row, q_node, q_head, o_row, o_node, o_head, page_stride, head_stride, slot_stride, table_stride;
+  Divide by_tiles;  // 16-key tiles of a page
+  int page_tiles, row_pages, pages, rows, kv_heads, heads, tokens, D, buckets;
+  int parts;   // wanted of the whole work; 0: units are not cut
+  int least;   // steps that a part has at least
+  int row_blocks;
+  float scale;
+};
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+  return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+
+// Entries before the new tokens, and new tokens, of sequence b.
+__device__ __forceinline__ int capacity_of(const PageArgs& a) { return a.row_pages * a.page_tiles * kPageUnit; }
+__device__ __forceinline__ int length_of(const PageArgs& a, int b) { return min(max(a.length[b], 0), capacity_of(a)); }
+__device__ __forceinline__ int fresh_of(const PageArgs& a, int b) {
+  return a.fresh != nullptr ? min(max(a.fresh[b], 0), a.tokens) : a.tokens;
+}
+// Steps of a unit of sequence b: none where it has no new token.
+template <int KEYS>
+__device__ __forceinline__ int steps_of(const PageArgs& a, int b) {
+  const int n = fresh_of(a, b);
+  return n == 0 ? 0 : (min(length_of(a, b) + n, capacity_of(a)) + KEYS - 1) / KEYS;
+}
+
+// Steps of a part, the same for all units: ceil(total / parts), at least `least`; the
+// last part of a unit may have fewer.  At most parts + units parts then.
+template <int KEYS>
+__device__ __forceinline__ int chunk_of(const PageArgs& a, int lane) {
+  int64_t sum = 0;
+  for (int b = lane; b < a.rows; b += 64) sum += steps_of<KEYS>(a, b);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
+  const int64_t total = uniform(sum) * a.kv_heads;
+  return max(a.least, (int)((total + a.parts - 1) / a.parts));
+}
+__device__ __forceinline__ int parts_of(int steps, int chunk) { return max(1, (steps + chunk - 1) / chunk); }
+
+// The sequence whose units hold part `at` of all, and the parts before it; rows if none.
+template <int KEYS>
+__device__ __forceinline__ int find_row(const PageArgs& a, int lane, int chunk, int64_t at, int64_t* before) {
+  int64_t base = 0;
+  for (int b0 = 0; b0 < a.rows; b0 += 64) {
+    const int64_t own = b0 + lane < a.rows ? (int64_t)parts_of(steps_of<KEYS>(a, b0 + lane), chunk) * a.kv_heads : 0;
+    int64_t incl = own;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t x = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += x;
+    }
+    const uint64_t past = __ballot(base + incl > at);
+    if (past != 0) {
+      const int l = __ffsll((unsigned long long)past) - 1;
+      *before = uniform((int64_t)(base + __shfl(incl - own, l, 64)));
+      return uniform(b0 + l);
+    }
+    base += uniform((int64_t)__shfl(incl, 63, 64));
+  }
+  return a.rows;
+}
+
+// The page and place in it of a wave's next tiles, one a lane.
+template <int TILES>
+struct TileLookup {
+  int page, place;  // page -1: not there
+  // lane l: tile l % TILES of the wave's step `first + every (l / TILES)`
+  __device__ __forceinline__ void fetch(const PageArgs& a, const int* table, int first, int every, int lane) {
+    const int tile = (first + every * (lane / TILES)) * TILES + lane % TILES, at = a.by_tiles(tile);
+    place = (tile - at * a.page_tiles) * kPageUnit;
+    page = -1;
+    if (at < a.row_pages) {
+      const int id = ld_g(table + at);
+      page = id >= 0 && id < a.pages ? id : -1;
+    }
+  }
+  static constexpr int kSteps = 64 / TILES;  // that a fetch is good for
+};
+
+// E consecutive outputs of row r from dimension d on: to `out`, or, of a part, to its slot.
+template <typename T, int E>
+__device__ __forceinline__ void emit(const PageArgs& a, bool whole, int64_t slot, int b, int kvh, int r, int d,
+                                     const float (&v)[E], float top, float sum, bool there) {
+  const int n = a.heads / a.kv_heads, node = r / n, h = kvh * n + r - node * n;
+  if (whole) {
+    there = there && sum != 0.f;
+    const float inv = there ? 1.f / sum : 0.f;
+    T* dst = static_cast<T*>(a.out) + b * a.o_row + node * a.o_node + h * a.o_head + d;
+    union {
+      T x[E];
+      uint4 w4[(E * sizeof(T) + 15) / 16];
+      uint2 w2;
+      uint32_t w1;
+    } u;
+#pragma unroll
+    for (int e = 0; e < E; ++e) u.x[e] = St<T>::st(there ? v[e] * inv : 0.f);
+    if constexpr (E * sizeof(T) >= 16) {
+#pragma unroll
+      for (int w = 0; w < (int)(E * sizeof(T) / 16); ++w)
+        if (d + w * (int)(16 / sizeof(T)) < a.D) reinterpret_cast<uint4*>(dst)[w] = u.w4[w];
+    } else if (d < a.D) {
+      if constexpr (E * sizeof(T) == 8) *reinterpret_cast<uint2*>(dst) = u.w2;
+      else *reinterpret_cast<uint32_t*>(dst) = u.w1;
+    }
+    if (a.lse != nullptr && d == 0)
+      a.lse[((size_t)b * a.tokens + node) * a.heads + h] = there ? fmaf(top, kLn2, logf(sum)) : -INFINITY;
+  } else {
+    const size_t at = slot * (size_t)(a.tokens * n) + r;
+    float* dst = a.part + at * a.D + d;
+    if constexpr (E % 4 == 0) {
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        if (d + e < a.D) *reinterpret_cast<float4*>(dst + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+    } else if (d < a.D) {
+      *reinterpret_cast<float2*>(dst) = make_float2(v[0], v[1]);
+    }
+    if (d == 0) a.part_ml[at] = make_float2(top, sum);
+  }
+}
+
+// Whether a row's sum and outputs are numbers.
+template <int E>
+__device__ __forceinline__ bool all_finite(float l, const f32x4_t (&o)[E]) {
+  float top = fabsf(l);
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) top = fmaf(0.f, o[e][r], top);  // NaN from either
+  return top < INFINITY;
+}
+
+// ---- fragments of 8-bit pages ----------------------------------------------------------
+
+// The power of two that brings a magnitude (as bits, finite) into [2^21, 2^22), and its
+// inverse.  Magnitudes below 2^-104, whose power would not be finite, count as 0.
+constexpr uint32_t kLeastBits = 23u << 23;
+__device__ __forceinline__ float to_digits(uint32_t size) {
+  return size >= kLeastBits ? __uint_as_float((275u << 23) - (size & 0x7f800000u)) : 0.f;
+}
+__device__ __forceinline__ float from_digits(uint32_t size) {  // NaN for what is not finite
+  return size >= 0x7f800000u ? NAN : size >= kLeastBits ? __uint_as_float((size & 0x7f800000u) - (21u << 23)) : 0.f;
+}
+
+// Bytes 0, 1 and 2 of four words.
+__device__ __forceinline__ void bytes_of(const uint32_t (&y)[4], uint32_t& b0, uint32_t& b1, uint32_t& b2) {
+  const uint32_t p = __builtin_amdgcn_perm(y[1], y[0], 0x05010400u), q = __builtin_amdgcn_perm(y[3], y[2], 0x05010400u);
+  b0 = __builtin_amdgcn_perm(q, p, 0x05040100u);
+  b1 = __builtin_amdgcn_perm(q, p, 0x07060302u);
+  b2 = __builtin_amdgcn_perm(__builtin_amdgcn_perm(y[3], y[2], 0x0c0c0602u), __builtin_amdgcn_perm(y[1], y[0], 0x0c0c0602u),
+                             0x05040100u);
+}
+
+__device__ __forceinline__ i32x4_t mma8(uint4 a, uint4 b, i32x4_t c) {
+  return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, a), __builtin_bit_cast(i32x4_t, b), c, 0, 0, 0);
+}
+// 65536 a + 256 b + c of three sums, each below 2^23.
+__device__ __forceinline__ float join_digits(int a, int b, int c) { return fmaf((float)a, 65536.f, (float)((b << 8) + c)); }
+
+__device__ __forceinline__ uint32_t max_bits_over_groups(uint32_t x) {  // of lanes i, i + 16, i + 32, i + 48
+  auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  x = max((uint32_t)r[0], (uint32_t)r[1]);
+  r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  return max((uint32_t)r[0], (uint32_t)r[1]);
+}
+
+// Fragments of head dimension DP (64, 128 or 256; D <= DP, a multiple of 16).
+template <int DP>
+struct CodeFrag {
+  static constexpr int KC = DP / 64;  // 16-byte loads of a key row, a lane
+  static constexpr int E = DP / 16;   // codes of a V row, a lane
+  static constexpr int VW = E / 4;    // the same in registers
+  __device__ __forceinline__ static void load_row(const char* row, int g, int D, uint4 (&f)[KC]) {
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      const int d = (c * 4 + g) * 16;
+      f[c] = (D == DP || d < D) ? ld_g16(row + d) : make_uint4(0, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ static void load_v(const char* row, int i, int D, uint32_t (&f)[VW]) {
+    const char* p = row + i * E;
+    const bool in = D == DP || i * E < D;
+    if constexpr (VW == 4) {
+      const uint4 x = in ? ld_g16(p) : make_uint4(0, 0, 0, 0);
+      f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
+    } else if constexpr (VW == 2) {
+      const uint64_t x = in ? ld_g(reinterpret_cast<const uint64_t*>(p)) : 0ull;
+      f[0] = (uint32_t)x, f[1] = (uint32_t)(x >> 32);
+    } else {
+      f[0] = in ? ld_g(reinterpret_cast<const uint32_t*>(p)) : 0u;
+    }
+  }
+  // One query row: the digits of lane group g's 16 KC values, and f.
+  template <typename T>
+  __device__ __forceinline__ static float digits(const T* row, int g, int D, uint4 (&a)[KC], uint4 (&b)[KC], uint4 (&c)[KC]) {
+    float x[KC][16];
+    uint32_t top = 0;
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      const int d = (k * 4 + g) * 16;
+      constexpr int kPer = 16 / sizeof(T);
+#pragma unroll
+      for (int w = 0; w < 16 / kPer; ++w) {
+        const uint4 u = d < D ? ld_g16(row + d + w * kPer) : make_uint4(0, 0, 0, 0);
+        const uint32_t r[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          if constexpr (sizeof(T) == 4) x[k][w * 4 + j] = __uint_as_float(r[j]);
+          else x[k][w * 8 + 2 * j] = Mma<T>::low(r[j]), x[k][w * 8 + 2 * j + 1] = Mma<T>::high(r[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(x[k][j]) & 0x7fffffffu);
+    }
+    top = max_bits_over_groups(top);
+    const float up = top < 0x7f800000u ? to_digits(top) : 0.f;
+#pragma unroll
+    for (int k = 0; k < KC; ++k) {
+      uint32_t q[3][4];
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          y[j] = (uint32_t)((int)rintf(x[k][w * 4 + j] * up) + 0x808080);  // each digit and 128
+        }
+        bytes_of(y, q[2][w], q[1][w], q[0][w]);
+      }
+      a[k] = make_uint4(q[0][0] ^ 0x80808080u, q[0][1] ^ 0x80808080u, q[0][2] ^ 0x80808080u, q[0][3] ^ 0x80808080u);
+      b[k] = make_uint4(q[1][0] ^ 0x80808080u, q[1][1] ^ 0x80808080u, q[1][2] ^ 0x80808080u, q[1][3] ^ 0x80808080u);
+      c[k] = make_uint4(q[2][0] ^ 0x80808080u, q[2][1] ^ 0x80808080u, q[2][2] ^ 0x80808080u, q[2][3] ^ 0x80808080u);
+    }
+    return from_digits(top);
+  }
+  // 16 weights, not negative and below 2^22 by `up`: the digits, in the order of the
+  // keys.  In [2^23, 2^24) a float's low bits count ones; 0x8080 adds 128 to two digits.
+  __device__ __forceinline__ static void digits(const float (&w)[16], float up, uint4& a, uint4& b, uint4& c) {
+    uint32_t q[3][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      uint32_t y[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) y[j] = __float_as_uint(fmaf(w[t * 4 + j], up, 8388608.f + 32896.f));
+      bytes_of(y, q[2][t], q[1][t], q[0][t]);
+    }
+    a = make_uint4(q[0][0], q[0][1], q[0][2], q[0][3]);
+    b = make_uint4(q[1][0] ^ 0x80808080u, q[1][1] ^ 0x80808080u, q[1][2] ^ 0x80808080u, q[1][3] ^ 0x80808080u);
+    c = make_uint4(q[2][0] ^ 0x80808080u, q[2][1] ^ 0x80808080u, q[2][2] ^ 0x80808080u, q[2][3] ^ 0x80808080u);
+  }
+  // Codes of dimensions 4 w .. 4 w + 3 of the lane, all 16 keys: operands of the four
+  // output tiles.  v[4 t + j]: key 16 t + 4 g + j.
+  __device__ __forceinline__ static void transpose(const uint32_t (&v)[16][VW], int w, uint4 (&out)[4]) {
+    uint32_t o[4][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t p = __builtin_amdgcn_perm(v[4 * t + 1][w], v[4 * t][w], 0x05010400u);
+      const uint32_t q = __builtin_amdgcn_perm(v[4 * t + 3][w], v[4 * t + 2][w], 0x05010400u);
+      const uint32_t r = __builtin_amdgcn_perm(v[4 * t + 1][w], v[4 * t][w], 0x07030602u);
+      const uint32_t s = __builtin_amdgcn_perm(v[4 * t + 3][w], v[4 * t + 2][w], 0x07030602u);
+      o[0][t] = __builtin_amdgcn_perm(q, p, 0x05040100u), o[1][t] = __builtin_amdgcn_perm(q, p, 0x07060302u);
+      o[2][t] = __builtin_amdgcn_perm(s, r, 0x05040100u), o[3][t] = __builtin_amdgcn_perm(s, r, 0x07060302u);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) out[e] = make_uint4(o[e][0], o[e][1], o[e][2], o[e][3]);
+  }
+};
+
+// ---- what both kernels share ------------------------------------------------------------
+
+struct Work {
+  int b, kvh, row0, s0, s1, steps, id;
+  bool all;
+};
+
+// The block's part; false: none.  Where units are not cut, s1 and steps are left for later,
+// since they depend on the length.
+template <int KEYS, int NR>
+__device__ __forceinline__ bool find_work(const PageArgs& a, int lane, Work& w) {
+  int64_t id = blockIdx.x;
+  int rb = 0;
+  if (a.row_blocks > 1) {  // the row blocks of a part share keys: they follow each other on one XCD
+    const int x = blockIdx.x >> 3;
+    rb = x % a.row_blocks;
+    id = (int64_t)(x / a.row_blocks) * 8 + (blockIdx.x & 7);
+  }
+  w.row0 = rb * (16 * NR);
+  w.id = (int)id;
+  if (a.parts == 0) {
+    if (id >= (int64_t)a.rows * a.kv_heads) return false;
+    w.b = w.id / a.kv_heads, w.kvh = w.id - w.b * a.kv_heads, w.s0 = 0, w.s1 = w.steps = 0, w.all = true;
+    return true;
+  }
+  const int chunk = chunk_of<KEYS>(a, lane);
+  int64_t before = 0;
+  w.b = find_row<KEYS>(a, lane, chunk, id, &before);
+  if (w.b >= a.rows) return false;
+  w.steps = steps_of<KEYS>(a, w.b);
+  const int n = parts_of(w.steps, chunk), at = (int)(id - before);
+  w.kvh = at / n;
+  w.s0 = (at - w.kvh * n) * chunk, w.s1 = min(w.steps, w.s0 + chunk);
+  w.all = n == 1;
+  return true;
+}
+
+// Joins the waves' outputs at the common maximum and stores the rows.  l: the lane's own
+// sums.  In two halves, so that the buffer holds half of the waves' outputs.
+template <typename T, int W, int NR, int E>
+__device__ __forceinline__ void join_waves(const PageArgs& a, const Work& w, int there_rows, char* lds, float2 (*ml)[16 * NR],
+                                           const float (&m)[NR], float (&l)[NR], f32x4_t (&o)[NR][E]) {
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
+  constexpr int H = W / 2;
+  f32x4_t* buf = reinterpret_cast<f32x4_t*>(lds);
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    l[t] = sum_over_groups(l[t]);
+    if (g == 0) ml[wid][t * 16 + i] = make_float2(m[t], l[t]);
+  }
+  __syncthreads();  // and the bias in LDS has been read
+  float top[NR], sum[NR];
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    top[t] = kNone, sum[t] = 0.f;
+#pragma unroll
+    for (int x = 0; x < W; ++x) top[t] = fmaxf(top[t], ml[x][t * 16 + i].x);
+#pragma unroll
+    for (int x = 0; x < W; ++x) sum[t] = fmaf(ml[x][t * 16 + i].y, fade(ml[x][t * 16 + i].x - top[t]), sum[t]);
+    const float f = fade(m[t] - top[t]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      o[t][e] *= f;
+      if (wid >= H) buf[((wid - H) * NR * E + t * E + e) * 64 + lane] = o[t][e];
+    }
+  }
+  __syncthreads();
+  if (wid < H) {
+#pragma unroll
+    for (int t = 0; t < NR; ++t)
+#pragma unroll
+      for (int e = 0; e < E; ++e) buf[(wid * NR * E + t * E + e) * 64 + lane] += o[t][e];
+  }
+  __syncthreads();
+  const int R = a.tokens * (a.heads / a.kv_heads);
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    if (wid / 4 != t % (W / 4)) continue;  // wave x: register x % 4 of every W / 4 th row tile
+    const int r = w.row0 + t * 16 + i, reg = wid & 3, d = (4 * g + reg) * E;
+    if (r >= R) continue;
+    float v[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      v[e] = 0.f;
+#pragma unroll
+      for (int x = 0; x < H; ++x) v[e] += reinterpret_cast<const float*>(&buf[(x * NR * E + t * E + e) * 64 + lane])[reg];
+    }
+    emit<T, E>(a, w.all, w.id, w.b, w.kvh, r, d, v, top[t], sum[t], r < there_rows);
+  }
+}
+
+template <typename T, int DP, int NR, int W>
+__global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
+  using F = AttnFrag<T, DP>;
+  constexpr int E = F::E, VW = F::VW, KC = F::KC, KEYS = 32;
+  using Lookup = TileLookup<2>;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4, D = a.D;
+  Work w;
+  if (!find_work<KEYS, NR>(a, lane, w)) return;
+  const int b = w.b, kvh = w.kvh, n = a.heads / a.kv_heads, R = a.tokens * n;
+  const int* table = a.table + b * a.table_stride;
+  const T* kc = static_cast<const T*>(a.k) + kvh * a.head_stride;
+  const T* vc = static_cast<const T*>(a.v) + kvh * a.head_stride;
+
+  // Nothing here needs the length: what lies past it is masked, and pages that are not
+  // there are not read.
+  Lookup look;
+  int looked = w.s0 + wid;  // the step of the lookup's first tile
+  look.fetch(a, table, looked, W, lane);
+  uint4 kf[2][KC];
+  uint32_t vf[8][VW];
+  int page[2], place[2];
+  auto find = [&](int st) {
+    const int x = (st - looked) / W * 2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      page[h] = __builtin_amdgcn_readlane(look.page, x + h);
+      place[h] = __builtin_amdgcn_readlane(look.place, x + h);
+    }
+  };
+  auto load_k = [&] {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (page[h] >= 0) {
+        F::load_row(kc + page[h] * a.page_stride + (int64_t)(place[h] + i) * a.slot_stride, g, D, kf[h]);
+      } else {
+#pragma unroll
+        for (int c = 0; c < KC; ++c) kf[h][c] = make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+  auto load_v = [&] {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const T* base = vc + (page[h] >= 0 ? page[h] * a.page_stride + (int64_t)place[h] * a.slot_stride : 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (page[h] >= 0) {
+          F::load_v(base + (4 * g + j) * a.slot_stride, i, D, vf[h * 4 + j]);
+        } else {
+#pragma unroll
+          for (int x = 0; x < VW; ++x) vf[h * 4 + j][x] = 0u;
+        }
+      }
+    }
+  };
+  find(w.s0 + wid);
+  load_k();
+  load_v();
+
+  const int len = length_of(a, b), fresh = fresh_of(a, b), end = min(len + fresh, capacity_of(a));
+  if (a.parts == 0) w.s1 = w.steps = steps_of<KEYS>(a, b);
+
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float2 ml[W][16 * NR];
+  float* btab = reinterpret_cast<float*>(lds);  // the bias of this K/V head's heads, until the waves join
+  const bool bias_in_lds = n * a.buckets <= kBiasLds;
+  uint4 q[NR][KC];
+  int last[NR];  // the newest entry that the row sees; -1: the row is not there
+  const float* brow[NR];
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    const int r = min(w.row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
+    F::load_row(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D, q[t]);
+    last[t] = node < fresh ? len + node : -1;
+    brow[t] = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
+  }
+  if (a.bias != nullptr && bias_in_lds) {
+    for (int x = tid; x < n * a.buckets; x += 64 * W) btab[x] = a.bias[(size_t)kvh * n * a.buckets + x];
+    ring_barrier();
+  }
+
+  f32x4_t o[NR][E];
+  float m[NR], l[NR];
+  auto begin = [&] {
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      m[t] = kNone, l[t] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
+    }
+  };
+  begin();
+  const float scale2 = a.scale * kLog2e;
+  // fp16 weights reach up to 2^15, so that those far below the maximum keep their bits.
+  constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;
+
+  // One step; next() requests the keys of the wave's next one.  A matrix product makes NaN
+  // of 0 * inf: infinities and NaN in values that some rows do not see (the new tokens', and
+  // with `exact` all) are left out of it and added by class.
+  auto step = [&](int st, auto exact, auto&& next) {
+    const int base = st * KEYS;
+    const bool whole = base + KEYS <= len + 1 && fresh > 0 && page[0] >= 0 && page[1] >= 0;
+    const bool apart = exact.value || (fresh > 1 && base + KEYS > len + 1);
+    const bool in[2] = {page[0] >= 0, page[1] >= 0};
+    const int page_v[2] = {page[0], page[1]}, place_v[2] = {place[0], place[1]};
+    if (!whole) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int x = 0; x < VW; ++x) vf[j][x] = base + lane_key(g, j) < end ? vf[j][x] : 0u;
+    }
+    float p[NR][8];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
+      const float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+      if (a.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float by = brow[t][bucket(last[t], base + lane_key(g, j), a.buckets)] * kLog2e;
+          p[t][j] = fmaf(s[j], scale2, by);
+          if (by < kNone) p[t][j] = -INFINITY;  // masked, whatever the key holds
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[t][j] = s[j] * scale2;
+      }
+      if (!whole) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) p[t][j] = in[j >> 2] && base + lane_key(g, j) <= last[t] ? p[t][j] : -INFINITY;
+      }
+    }
+    next();
+    uint32_t seen[NR];  // the keys that the row does not mask, a bit each
+    if (apart) {
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        seen[t] = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) seen[t] |= p[t][j] < kNone ? 0u : 1u << j;
+      }
+    }
+    running_softmax<NR, E>(p, m, l, o, kShift);
+    if (!apart) {
+      F::template add_pv<NR>(vf, p, o);
+    } else {
+      uint32_t diff = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+#pragma unroll
+        for (int x = 0; x < VW; ++x) {
+          const uint32_t y = F::finite_part(vf[j][x]);
+          diff |= y ^ vf[j][x];
+          vf[j][x] = y;
+        }
+      F::template add_pv<NR>(vf, p, o);
+      if (__builtin_expect(__any(diff != 0), 0)) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int h = j >> 2;
+          const bool have = page_v[h] >= 0 && base + lane_key(g, j) < end;
+          if (page_v[h] >= 0)
+            F::load_v(vc + page_v[h] * a.page_stride + (int64_t)(place_v[h] + 4 * g + (j & 3)) * a.slot_stride, i, D, vf[j]);
+#pragma unroll
+          for (int x = 0; x < VW; ++x) vf[j][x] = have ? F::classes(vf[j][x]) : 0u;
+        }
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+          float one[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) one[j] = (seen[t] >> j) & 1 ? 1.f : 0.f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            const f32x4_t c = F::count(vf, one, e);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(c[r]);
+          }
+        }
+      }
+    }
+  };
+  auto steps = [&](auto exact) {
+    for (int st = w.s0 + wid; st < w.s1; st += W) {
+      const bool more = st + W < w.s1;
+      step(st, exact, [&] {
+        if (!more) return;
+        if (st + W - looked >= Lookup::kSteps * W) {
+          looked = st + W;
+          look.fetch(a, table, looked, W, lane);
+        }
+        find(st + W);
+        load_k();
+      });
+      if (more) load_v();
+    }
+  };
+  steps(std::false_type{});
+  bool odd = false;
+#pragma unroll
+  for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]) && last[t] >= 0;
+  if (__builtin_expect(__any(odd), 0)) {  // rare: this wave's steps once more
+    begin();
+    looked = w.s0 + wid;
+    look.fetch(a, table, looked, W, lane);
+    find(looked);
+    load_k();
+    load_v();
+    steps(std::true_type{});
+  }
+  join_waves<T, W, NR, E>(a, w, fresh * n, lds, ml, m, l, o);
+}
+
+template <typename T, int DP, int NR, int W>
+__global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
+  using F = CodeFrag<DP>;
+  constexpr int E = F::E, VW = F::VW, KC = F::KC, KEYS = 64;
+  using Lookup = TileLookup<4>;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4, D = a.D;
+  Work w;
+  if (!find_work<KEYS, NR>(a, lane, w)) return;
+  const int b = w.b, kvh = w.kvh, n = a.heads / a.kv_heads, R = a.tokens * n, page_size = a.page_tiles * kPageUnit;
+  const int* table = a.table + b * a.table_stride;
+  const char* kc = static_cast<const char*>(a.k) + kvh * a.head_stride;
+  const char* vc = static_cast<const char*>(a.v) + kvh * a.head_stride;
+
+  Lookup look;
+  int looked = w.s0 + wid;
+  look.fetch(a, table, looked, W, lane);
+  uint4 kf[4][KC];
+  uint32_t vf[16][VW];
+  float ks, vs;  // the scales of key `lane` of the step, of K and of V
+  int page[4], place[4];
+  auto find = [&](int st) {
+    const int x = (st - looked) / W * 4;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      page[t] = __builtin_amdgcn_readlane(look.page, x + t);
+      place[t] = __builtin_amdgcn_readlane(look.place, x + t);
+    }
+  };
+  // Pages that are not there are not read: their keys are masked, whatever the registers hold.
+  auto load_k = [&](int st) {
+    const int x = (st - looked) / W * 4 + g;  // of the lane's own key, 16 g + i
+    const int pg = __shfl(look.page, x, 64), pl = __shfl(look.place, x, 64);
+    const int64_t at = ((int64_t)max(pg, 0) * a.kv_heads + kvh) * page_size + pl + i;
+    ks = pg >= 0 ? ld_g(a.k_scale + at) : 0.f;
+    vs = pg >= 0 ? ld_g(a.v_scale + at) : 0.f;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+      if (page[t] >= 0) F::load_row(kc + page[t] * a.page_stride + (int64_t)(place[t] + i) * a.slot_stride, g, D, kf[t]);
+  };
+  auto load_v = [&] {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      if (page[t] < 0) continue;
+      const char* base = vc + page[t] * a.page_stride + (int64_t)place[t] * a.slot_stride;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) F::load_v(base + (4 * g + j) * a.slot_stride, i, D, vf[4 * t + j]);
+    }
+  };
+#pragma unroll
+  for (int t = 0; t < 4; ++t)
+#pragma unroll
+    for (int c = 0; c < KC; ++c) kf[t][c] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+  for (int j = 0; j < 16; ++j)
+#pragma unroll
+    for (int x = 0; x < VW; ++x) vf[j][x] = 0u;
+  find(w.s0 + wid);
+  load_k(w.s0 + wid);
+  load_v();
+
+  const int len = length_of(a, b), fresh = fresh_of(a, b);
+  if (a.parts == 0) w.s1 = w.steps = steps_of<KEYS>(a, b);
+
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  __shared__ float2 ml[W][16 * NR];
+  __shared__ __attribute__((aligned(16))) float sc[W][128];  // the scales of a wave's step
+  float* btab = reinterpret_cast<float*>(lds);
+  const bool bias_in_lds = n * a.buckets <= kBiasLds;
+  uint4 qa[NR][KC], qb[NR][KC], qc[NR][KC];
+  float qf[NR];
+  int last[NR];
+  const float* brow[NR];
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    const int r = min(w.row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
+    qf[t] = F::digits(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D,
+                      qa[t], qb[t], qc[t]) * a.scale * kLog2e;
+    last[t] = node < fresh ? len + node : -1;
+    brow[t] = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
+  }
+  if (a.bias != nullptr && bias_in_lds) {
+    for (int x = tid; x < n * a.buckets; x += 64 * W) btab[x] = a.bias[(size_t)kvh * n * a.buckets + x];
+    ring_barrier();
+  }
+
+  f32x4_t o[NR][E];
+  float m[NR], l[NR];
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    m[t] = kNone, l[t] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
+  }
+  const i32x4_t zero = {0, 0, 0, 0};
+
+  for (int st = w.s0 + wid; st < w.s1; st += W) {
+    const int base = st * KEYS;
+    const bool there = page[0] >= 0 && page[1] >= 0 && page[2] >= 0 && page[3] >= 0;
+    const bool masks = a.bias != nullptr || !there || fresh == 0 || base + KEYS > len + 1;
+    const bool in[4] = {page[0] >= 0, page[1] >= 0, page[2] >= 0, page[3] >= 0};
+    const bool more = st + W < w.s1;
+    sc[wid][lane] = ks, sc[wid][64 + lane] = vs;  // read by the wave's lanes alone, in order
+    __builtin_amdgcn_wave_barrier();
+    float p[NR][16];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        i32x4_t x = zero, y = zero, z = zero;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          x = mma8(kf[k][c], qa[t][c], x);
+          y = mma8(kf[k][c], qb[t][c], y);
+          z = mma8(kf[k][c], qc[t][c], z);
+        }
+        const float4 s = *reinterpret_cast<const float4*>(&sc[wid][k * 16 + 4 * g]);
+        const float by_key[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[t][4 * k + r] = join_digits(x[r], y[r], z[r]) * qf[t] * by_key[r];
+      }
+    }
+    if (more) {
+      if (st + W - looked >= Lookup::kSteps * W) {
+        looked = st + W;
+        look.fetch(a, table, looked, W, lane);
+      }
+      find(st + W);
+      load_k(st + W);
+    }
+    uint4 wa[NR], wb[NR], wc[NR];
+    float wf[NR];
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      float sv[16];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float4 s = *reinterpret_cast<const float4*>(&sc[wid][64 + k * 16 + 4 * g]);
+        sv[4 * k] = s.x, sv[4 * k + 1] = s.y, sv[4 * k + 2] = s.z, sv[4 * k + 3] = s.w;
+      }
+      if (masks) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int key = base + (j >> 2) * 16 + 4 * g + (j & 3);
+          float by = 0.f;
+          if (a.bias != nullptr) by = brow[t][bucket(last[t], key, a.buckets)] * kLog2e;
+          const float x = p[t][j] + by;
+          const bool out = by < kNone || x < kNone || !in[j >> 2] || key > last[t];
+          p[t][j] = out ? -INFINITY : x;
+          sv[j] = out ? 0.f : sv[j];  // a masked entry's scale may be NaN
+        }
+      }
+      float top = p[t][0];
+#pragma unroll
+      for (int j = 1; j < 16; ++j) top = fmaxf(top, p[t][j]);
+      top = max_over_groups(top);
+      if (__any(top > m[t])) {
+        const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
+        m[t] = mn;
+        l[t] *= f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[t][e] *= f;
+      }
+      uint32_t size = 0;
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float x = __builtin_amdgcn_exp2f(p[t][j] - m[t]);
+        l[t] += x;
+        p[t][j] = x * sv[j];
+        size = max(size, __float_as_uint(p[t][j]));  // bits of what is not negative order as the values do, NaN above all
+      }
+      size = max_bits_over_groups(size);
+      F::digits(p[t], to_digits(size), wa[t], wb[t], wc[t]);
+      wf[t] = from_digits(size);
+    }
+#pragma unroll
+    for (int x = 0; x < VW; ++x) {
+      uint4 op[4];
+      F::transpose(vf, x, op);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int t = 0; t < NR; ++t) {
+          const i32x4_t u = mma8(op[e], wa[t], zero), v = mma8(op[e], wb[t], zero), y = mma8(op[e], wc[t], zero);
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[t][4 * x + e][r] = fmaf(join_digits(u[r], v[r], y[r]), wf[t], o[t][4 * x + e][r]);
+        }
+    }
+    if (more) load_v();
+  }
+  join_waves<T, W, NR, E>(a, w, fresh * n, lds, ml, m, l, o);
+}
+
+// ---- joining parts ------------------------------------------------------------------------
+
+// A wave a row: the row's parts at their common maximum, in order.  `cols` lanes (a power of
+// two, 4 cols >= D) take a part's outputs, four each, 64 / cols parts at a time.
+template <typename T, int KEYS>
+__global__ __launch_bounds__(256) void k_paged_join(const PageArgs a, int cols) {
+  const int lane = threadIdx.x & 63, n = a.heads / a.kv_heads, R = a.tokens * n;
+  const int blocks = (R + 3) / 4, unit = blockIdx.x / blocks;
+  const int r = (blockIdx.x - unit * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (r >= R) return;
+  const int b = unit / a.kv_heads, kvh = unit - b * a.kv_heads, steps = steps_of<KEYS>(a, b);
+  const int chunk = chunk_of<KEYS>(a, lane), parts = parts_of(steps, chunk);
+  if (parts == 1) return;  // written by its block
+  int64_t first = 0;
+  for (int x = lane; x < b; x += 64) first += parts_of(steps_of<KEYS>(a, x), chunk);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) first += __shfl_xor(first, o, 64);
+  first = uniform(first) * a.kv_heads + (int64_t)kvh * parts;
+  const int d = lane % cols * 4, from = lane / cols, every = 64 / cols;
+  const float2* ml = a.part_ml + first * R + r;
+  const float* part = a.part + (first * R + r) * a.D;
+  float top = kNone, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < parts; s0 += 64) {
+    const float2 y = s0 + lane < parts ? ml[(size_t)(s0 + lane) * R] : make_float2(kNone, 0.f);
+    const float to = fmaxf(top, wave_max(y.x)), f = fade(top - to);
+    top = to;
+    const float w = s0 + lane < parts ? fade(y.x - top) : 0.f;
+    sum = fmaf(sum, f, wave_sum(y.y * w));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] *= f;
+    const int end = min(64, parts - s0);
+    for (int s = from; s < (end + every - 1) / every * every; s += every) {
+      const float ws = __shfl(w, s, 64);
+      if (s < end && d < a.D) {
+        const float4 z = *reinterpret_cast<const float4*>(part + (size_t)(s0 + s) * R * a.D + d);
+        v[0] = fmaf(z.x, ws, v[0]), v[1] = fmaf(z.y, ws, v[1]), v[2] = fmaf(z.z, ws, v[2]), v[3] = fmaf(z.w, ws, v[3]);
+      }
+    }
+  }
+  for (int o = cols; o < 64; o <<= 1) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], o, 64);
+  }
+  if (from == 0 && d < a.D) emit<T, 4>(a, true, 0, b, kvh, r, d, v, top, sum, r / n < fresh_of(a, b));
+}
+
+// ---- host -----------------------------------------------------------------------------------
+
+struct Plan {
+  int keys, tiles, row_blocks, parts, least;
+};
+
+// Row tiles a wave holds at most, and waves of a block: registers allow two tiles and
+// eight waves (two a SIMD), of wide heads or fp32 values less.
+constexpr int row_tiles(size_t elt, int dp) { return dp == 256 ? 1 : 2; }
+constexpr int waves_of(size_t elt, int dp) { return dp == 256 || (elt == 4 && dp == 128) ? 4 : 8; }
+
+Plan plan(const PagedCache& c, int heads, int tokens) {
+  const int R = tokens * (heads / c.kv_heads), dp = c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
+  const size_t elt = c.codes ? 1 : dtype_size(c.dt);
+  Plan p;
+  p.keys = c.codes ? 64 : 32;
+  p.tiles = std::min(row_tiles(elt, dp), R <= 16 ? 1 : 2);
+  p.row_blocks = (R + 16 * p.tiles - 1) / (16 * p.tiles);
+  const int64_t units = std::max<int64_t>(1, (int64_t)c.rows * c.kv_heads);
+  const int64_t steps = ((int64_t)c.capacity() + p.keys - 1) / p.keys;
+  p.least = 2 * waves_of(elt, dp);
+  p.parts = std::max(8, 1024 / p.row_blocks);
+  if (steps <= p.least || units >= 4096) p.parts = 0;
+  return p;
+}
+
+size_t blocks_of(const PagedCache& c, const Plan& p) { return (size_t)p.parts + (size_t)c.rows * c.kv_heads; }
+
+template <typename K>
+void start(K kernel, int threads, size_t lds, const PageArgs& a, size_t blocks, hipStream_t s) {
+  lds = std::max(lds, a.bias != nullptr ? (size_t)kBiasLds * 4 : size_t{0});
+  allow_dynamic_lds(reinterpret_cast<const void*>(kernel), 96 * 1024);
+  const size_t grid = a.row_blocks > 1 ? (blocks + 7) / 8 * 8 * a.row_blocks : blocks;
+  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, s, a);
+}
+
+template <typename T, int DP, int NR>
+void launch(const PageArgs& a, bool codes, size_t blocks, hipStream_t s) {
+  if constexpr (NR <= row_tiles(sizeof(T), DP)) {
+    if (codes) {
+      if constexpr (DP >= 64) {
+        constexpr int W = waves_of(1, DP);
+        start(&k_paged_codes<T, DP, NR, W>, 64 * W, (size_t)W / 2 * NR * (DP / 16) * 1024, a, blocks, s);
+      }
+    } else {
+      constexpr int W = waves_of(sizeof(T), DP);
+      start(&k_paged<T, DP, NR, W>, 64 * W, (size_t)W / 2 * NR * (DP / 16) * 1024, a, blocks, s);
+    }
+  }
+}
+
+}  // namespace
+
+bool paged_attention_fits(const PagedCache& c, int heads, int tokens) {
+  const Plan p = plan(c, heads, tokens);
+  const int64_t units = (int64_t)c.rows * c.kv_heads, most = (1ll << 32) - 1;  // threads of a launch
+  const int R = tokens * (heads / c.kv_heads);
+  return ((int64_t)blocks_of(c, p) + 7) / 8 * 8 * p.row_blocks * 512 <= most && units * ((R + 3) / 4) * 256 <= most;
+}
+
+size_t paged_attention_workspace(const PagedCache& c, int heads, int tokens) {
+  const Plan p = plan(c, heads, tokens);
+  return p.parts == 0 ? 0 : blocks_of(c, p) * (size_t)(heads / c.kv_heads * tokens) * (c.d + 2) * 4;
+}
+
+void paged_attention(const PagedCache& c, const PagedAttnArgs& t, void* ws, hipStream_t s) {
+  const Plan p = plan(c, t.heads, t.tokens);
+  PageArgs a{};
+  a.q = t.q.p, a.k = c.k, a.v = c.v, a.out = t.out.p, a.k_scale = c.k_scale, a.v_scale = c.v_scale, a.bias = t.bias;
+  a.table = c.table, a.length = c.length, a.fresh = t.fresh, a.lse = t.lse;
+  a.q_row = t.q.row_stride, a.q_node = t.q.node_stride, a.q_head = t.q.head_stride;
+  a.o_row = t.out.row_stride, a.o_node = t.out.node_stride, a.o_head = t.out.head_stride;
+  a.page_stride = c.page_stride, a.head_stride = c.head_stride, a.slot_stride = c.slot_stride, a.table_stride = c.table_stride;
+  a.page_tiles = c.page_size / kPageUnit, a.by_tiles = Divide(a.page_tiles), a.row_pages = c.row_pages, a.pages = c.pages;
+  a.rows = c.rows, a.kv_heads = c.kv_heads, a.heads = t.heads, a.tokens = t.tokens, a.D = c.d, a.buckets = t.buckets;
+  a.parts = p.parts, a.least = p.least, a.row_blocks = p.row_blocks, a.scale = t.scale;
+  const int R = t.tokens * (t.heads / c.kv_heads);
+  const size_t blocks = blocks_of(c, p);
+  if (p.parts > 0) {
+    a.part = static_cast<float*>(ws);
+    a.part_ml = reinterpret_cast<float2*>(a.part + blocks * R * c.d);
+  }
+  MRT_DTYPE_DISPATCH(t.dt, {
+    auto tiles = [&](auto width) {
+      constexpr int DP = decltype(width)::value;
+      if (p.tiles == 1) launch<T, DP, 1>(a, c.codes, blocks, s);
+      else launch<T, DP, 2>(a, c.codes, blocks, s);
+    };
+    if (c.d <= 32 && !c.codes) tiles(std::integral_constant<int, 32>{});
+    else if (c.d <= 64) tiles(std::integral_constant<int, 64>{});
+    else if (c.d <= 128) tiles(std::integral_constant<int, 128>{});
+    else tiles(std::integral_constant<int, 256>{});
+  });
+  MRT_HIP_CHECK(hipGetLastError());
+  if (p.parts > 0) {
+    const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64;
+    const dim3 grid((unsigned)((size_t)c.rows * c.kv_heads * ((R + 3) / 4)));
+    MRT_DTYPE_DISPATCH(t.dt, {
+      if (c.codes) hipLaunchKernelGGL((k_paged_join<T, 64>), grid, dim3(256), 0, s, a, cols);
+      else hipLaunchKernelGGL((k_paged_join<T, 32>), grid, dim3(256), 0, s, a, cols);
+    });
+    MRT_HIP_CHECK(hipGetLastError());
+  }
+}
+
+}  // namespace mrt

@@ -42,6 +42,7 @@ struct Mfma<f16> {
 template <typename T>
 struct Core16 {
   typedef typename Mfma<T>::v8 v8;
+  typedef f32x16_t Acc;
   static constexpr int kChunks = 8, kSteps = 4, kParts = 1, kDepth = 64;
   __device__ static int swz(int r) { return (r ^ (r >> 3)) & 7; }
   __device__ static int place(int r, int chunk) { return chunk ^ swz(r); }
@@ -77,8 +78,8 @@ struct RingTile {
   __device__ static void load_b(unsigned char* stage, int q, const void* src) { load(stage + BM * kRow, q, src); }
 
   struct State {
-    f32x16_t acc[MI][NJ];  // (i, j), r: row 32 i + lane % 32, column 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4
-    f32x16_t low[Core::kFine ? MI : 1][Core::kFine ? NJ : 1];  // sums of all products but the last
+    typename Core::Acc acc[MI][NJ];  // (i, j), r: row 32 i + lane % 32, column 32 j + 8 (r / 4) + 4 (lane / 32) + r % 4
+    typename Core::Acc low[Core::kFine ? MI : 1][Core::kFine ? NJ : 1];  // sums of all products but the last
     v8 a[2][MI][Core::kParts], b[2][NJ][Core::kParts];
     int slot = 0;  // ring stage of the next k-tile
     __device__ void clear() {
@@ -88,8 +89,8 @@ struct RingTile {
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            acc[i][j][r] = 0.f;
-            if constexpr (Core::kFine) low[i][j][r] = 0.f;
+            acc[i][j][r] = 0;
+            if constexpr (Core::kFine) low[i][j][r] = 0;
           }
     }
     // acc the whole sums

@@ -73,6 +73,7 @@ __device__ __forceinline__ void store_split4(bf16* base, size_t idx, const float
 // 12 LDS reads of a 64 x 64 wave tile's 16-deep step).
 struct CoreSplit {
   typedef __bf16 v8 __attribute__((ext_vector_type(8)));
+  typedef f32x16_t Acc;
   static constexpr int kChunks = 12, kSteps = 2, kParts = 3, kDepth = 32;
   static constexpr int kProducts = 6;
   static constexpr bool kFine = false;

@@ -320,6 +320,13 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "mrt_cache_evict": (i32, [vp, vp, vp, sz, i32, vp]),
         "mrt_q4_matmul": (i32, [vp, ctypes.c_int64, i32, vp, vp, vp, i32, i32, i32, i32, vp, ctypes.c_int64, i32, vp]),
         "mrt_q4_quantize": (i32, [vp, ctypes.c_int64, i32, i32, i32, i32, vp, vp, vp, i32, vp]),
+        "mrt_paged_write": (i32, [vp, vp, i32, vp]),
+        "mrt_paged_read": (i32, [vp, vp, i32, vp]),
+        "mrt_paged_attention_workspace": (i32, [vp, i32, i32, ctypes.POINTER(sz)]),
+        "mrt_paged_attention": (i32, [vp, vp, vp, sz, i32, vp]),
+        "mrt_draft_verify": (i32, [vp, i32, vp]),
+        "mrt_i8_quantize": (i32, [vp, ctypes.c_int64, i32, i32, i32, vp, ctypes.c_int64, vp, i32, vp]),
+        "mrt_i8_matmul": (i32, [vp, i32, vp]),
         "mrt_codec_config_default": (None, [ctypes.POINTER(_CodecConfig)]),
         "mrt_codec_create": (i32, [ctypes.c_char_p, ctypes.c_char_p, ctypes.POINTER(_CodecConfig), i32,
                                    ctypes.POINTER(vp)]),
@@ -1367,3 +1374,230 @@ def q4_quantize(weight, group: int = 64):
     _check(lib, lib.mrt_q4_quantize(weight.data_ptr(), weight.stride(0), n, k, group, _dtype_code(weight.dtype),
                                     w.data_ptr(), scales.data_ptr(), biases.data_ptr(), index, _raw_stream(index)))
     return w, scales, biases
+
+
+# ---- operators of a server's step: caches in pages, 8-bit products, verification ------
+#
+# As the operators above: the caller's tensors, torch's current stream, no gradients.
+
+PAGES_I8 = 3
+_PAGES_STRUCT = struct.Struct("PPPPPPqqqqiiiiiiixxxx")      # mrt_paged_cache
+_STORE_STRUCT = struct.Struct("PqqqPqqqPPPii")              # mrt_paged_store_args
+_PAGED_STRUCT = struct.Struct("PqqqPqqqPPPiiiifxxxx")       # mrt_paged_attention_args
+_VERIFY_STRUCT = struct.Struct("PPqqqqPPqPPPPiiii")         # mrt_draft_verify_args
+_I8_STRUCT = struct.Struct("PPPPPPqqqqiiii")                # mrt_i8_matmul_args
+
+
+class PagedCache:
+    """One layer's K/V of ``rows`` sequences in pages of the caller's pool (mrt_paged_cache).
+
+    k, v: (pages, kv_heads, page_size, d) of one dtype and the same strides, d
+    contiguous, page_size a multiple of 16; fp32, bf16 or fp16, or int8 codes with
+    k_scale, v_scale (pages, kv_heads, page_size) fp32.  table int32 (rows,
+    row_pages): the page of each page_size entries of a sequence, an id outside
+    the pool where there is none; length int32 (rows), the entries in use.  The
+    tensors are kept, not copied.
+    """
+
+    __slots__ = ("k", "v", "table", "length", "k_scale", "v_scale", "index", "dtype", "codes", "shape", "rows", "row_pages",
+                 "_c")
+
+    def __init__(self, k, v, table, length, k_scale=None, v_scale=None):
+        torch = _torch()
+        shape, stride, index, self.codes = k.shape, k.stride(), k.get_device(), k.dtype is torch.int8
+        code = PAGES_I8 if self.codes else _dtype_code(k.dtype)
+        if code < 0 or len(shape) != 4 or stride[3] != 1:
+            raise ValueError("pages: k must be (pages, kv_heads, page_size, d) fp32, bf16, fp16 or int8, d contiguous")
+        if v.shape != shape or v.dtype is not k.dtype or v.stride() != stride or v.get_device() != index:
+            raise ValueError("pages: v must have k's shape, dtype, strides and device")
+        if index < 0:
+            raise ValueError("pages: the tensors must be on a GPU")
+        if table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != index or table.stride(1) != 1:
+            raise ValueError("pages: table must be int32 (rows, row_pages) on k's GPU, rows contiguous")
+        rows, row_pages = table.shape
+        lp, ks, vs = _ints(length, (rows,), index, "length"), 0, 0
+        if self.codes:
+            if k_scale is None or v_scale is None:
+                raise ValueError("pages: int8 codes need k_scale and v_scale")
+            ks, vs = _floats(k_scale, shape[:3], index, "k_scale"), _floats(v_scale, shape[:3], index, "v_scale")
+        elif k_scale is not None or v_scale is not None:
+            raise ValueError("pages: k_scale and v_scale go with int8 codes")
+        self.k, self.v, self.table, self.length, self.k_scale, self.v_scale = k, v, table, length, k_scale, v_scale
+        self.index, self.dtype, self.shape, self.rows, self.row_pages = index, k.dtype, shape, rows, row_pages
+        self._c = _PAGES_STRUCT.pack(k.data_ptr(), v.data_ptr(), ks, vs, table.data_ptr(), lp, stride[0], stride[1],
+                                     stride[2], table.stride(0), shape[0], rows, row_pages, shape[1], shape[2], shape[3],
+                                     code)
+
+
+def _page_rows(t, shape, dtype, cache, what):
+    """Pointer and strides of a 4-d operand of ``dtype``, which goes with the cache's pages."""
+    s = t.stride()
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != cache.index or s[3] != 1 or _dtype_code(dtype) < 0 or (
+            not cache.codes and dtype is not cache.dtype):
+        raise ValueError(f"{what} must be {tuple(shape)} of the pages' dtype, with int8 pages fp32, bf16 or fp16, on their GPU, "
+                         "d contiguous")
+    return t.data_ptr(), s[0], s[1], s[2]
+
+
+def paged_write(cache: PagedCache, k_new, v_new, fresh=None, length_out=None) -> None:
+    """Writes new tokens' keys and values into the pages (mrt_paged_write).
+
+    k_new, v_new (rows, tokens, kv_heads, d): sequence b's go to its entries
+    length[b] .., the first fresh[b] (int32 (rows); None: all) of them, quantised
+    where the pages hold codes.  length_out, a tensor of its own, receives the
+    new lengths.
+    """
+    lib, index = load_library(), cache.index
+    if k_new.dim() != 4:
+        raise ValueError("k_new must be (rows, tokens, kv_heads, d)")
+    tokens, dtype = k_new.shape[1], k_new.dtype
+    shape = (cache.rows, tokens, cache.shape[1], cache.shape[3])
+    args = _STORE_STRUCT.pack(*_page_rows(k_new, shape, dtype, cache, "k_new"), *_page_rows(v_new, shape, dtype, cache, "v_new"),
+                              0 if fresh is None else _ints(fresh, (cache.rows,), index, "fresh"), 0,
+                              0 if length_out is None else _ints(length_out, (cache.rows,), index, "length_out"), tokens,
+                              _dtype_code(dtype))
+    code = lib.mrt_paged_write(cache._c, args, index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+
+
+def paged_read(cache: PagedCache, k_out, v_out, start=None) -> None:
+    """Reads entries start[b] .. of each sequence back into k_out, v_out (mrt_paged_read).
+
+    k_out, v_out (rows, kv_heads, tokens, d), the layout of ``KVCache``; start
+    int32 (rows), None: 0.  Entries past a sequence's length are left as they are.
+    """
+    lib, index = load_library(), cache.index
+    if k_out.dim() != 4:
+        raise ValueError("k_out must be (rows, kv_heads, tokens, d)")
+    tokens, dtype = k_out.shape[2], k_out.dtype
+    shape = (cache.rows, cache.shape[1], tokens, cache.shape[3])
+    kp, vp = _page_rows(k_out, shape, dtype, cache, "k_out"), _page_rows(v_out, shape, dtype, cache, "v_out")
+    args = _STORE_STRUCT.pack(kp[0], kp[1], kp[3], kp[2], vp[0], vp[1], vp[3], vp[2], 0,
+                              0 if start is None else _ints(start, (cache.rows,), index, "start"), 0, tokens, _dtype_code(dtype))
+    code = lib.mrt_paged_read(cache._c, args, index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(rows, row_pages, pages, kv_heads, page_size, d, code, heads, tokens) -> int:
+    lib, size = load_library(), ctypes.c_size_t()
+    c = _PAGES_STRUCT.pack(0, 0, 0, 0, 0, 0, 0, 0, 0, 0, pages, rows, row_pages, kv_heads, page_size, d, code)
+    _check(lib, lib.mrt_paged_attention_workspace(c, heads, tokens, ctypes.byref(size)))
+    return size.value
+
+
+def paged_attention(q, cache: PagedCache, fresh=None, scale: float = 1.0, bias=None, out=None, lse=None):
+    """Attention of each sequence's newest tokens over its pages (mrt_paged_attention).
+
+    q (rows, tokens, heads, d); the tokens' own keys and values are in the cache
+    already (``paged_write`` with the same ``cache`` and ``fresh``): token t sees
+    entries 0 .. length + t.  bias: fp32 (heads, buckets) by distance.  Returns
+    (out (rows, tokens, heads, d), lse (rows, tokens, heads) fp32), new tensors
+    unless given; tokens past fresh[b] get 0 and -inf.
+    """
+    torch, lib, index = _torch(), load_library(), cache.index
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 4 or shape[0] != cache.rows or shape[3] != cache.shape[3]:
+        raise ValueError("q must be (rows, tokens, heads, d) with the cache's rows and d")
+    rows, tokens, heads, d = shape
+    qp = _page_rows(q, shape, dtype, cache, "q")
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=q.device)
+    op = _page_rows(out, shape, dtype, cache, "out")
+    if lse is None:
+        lse = torch.empty((rows, tokens, heads), dtype=torch.float32, device=q.device)
+    table, buckets = _bias_table(bias, heads, cache)
+    args = _PAGED_STRUCT.pack(*qp, *op, 0 if fresh is None else _ints(fresh, (rows,), index, "fresh"),
+                              _floats(lse, (rows, tokens, heads), index, "lse"), table, buckets, tokens, heads,
+                              _dtype_code(dtype), scale)
+    pages, kv_heads, page_size, _ = cache.shape
+    size = _paged_workspace(rows, cache.row_pages, pages, kv_heads, page_size, d,
+                            PAGES_I8 if cache.codes else _dtype_code(dtype), heads, tokens)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    code = lib.mrt_paged_attention(cache._c, args, ws.data_ptr() if size else None, size, index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+    return out, lse
+
+
+def draft_verify(target, draft, tokens, uniforms, parents=None):
+    """Which drafted tokens stand against the target's probabilities (mrt_draft_verify).
+
+    target (rows, nodes + 1, vocab): the target's probabilities after the cache
+    and after each node; draft (rows, nodes, vocab), those that the children of a
+    slot were drawn from, or None for drafts that were not drawn; tokens int32
+    (rows, nodes); uniforms fp32 (rows, nodes + 1) in [0, 1); parents as in
+    ``tree_attention``, None: a chain.  Returns int32 (accepted (rows, nodes), as
+    ``cache_commit`` takes it, count (rows), token (rows): the one that follows).
+    """
+    torch, lib, index = _torch(), load_library(), target.get_device()
+    if target.dim() != 3 or index < 0 or target.shape[1] < 2 or target.stride(2) != 1 or _dtype_code(target.dtype) < 0:
+        raise ValueError("target must be (rows, nodes + 1, vocab) fp32, bf16 or fp16 on a GPU, the vocabulary contiguous")
+    rows, nodes, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    dp = d_row = d_slot = 0
+    if draft is not None:
+        if draft.shape != (rows, nodes, vocab) or draft.dtype is not target.dtype or draft.get_device() != index or (
+                draft.stride(2) != 1):
+            raise ValueError("draft must be (rows, nodes, vocab) in target's dtype, on its GPU, the vocabulary contiguous")
+        dp, d_row, d_slot = draft.data_ptr(), draft.stride(0), draft.stride(1)
+    tp = pstride = 0
+    if parents is not None:
+        one = parents.dim() == 1
+        tp, pstride = _ints(parents, (nodes,) if one else (rows, nodes), index, "parents"), 0 if one else nodes
+    got = torch.empty(rows * (nodes + 2), dtype=torch.int32, device=target.device)
+    ap = got.data_ptr()
+    args = _VERIFY_STRUCT.pack(target.data_ptr(), dp, target.stride(0), target.stride(1), d_row, d_slot,
+                               _ints(tokens, (rows, nodes), index, "tokens"), tp, pstride,
+                               _floats(uniforms, (rows, nodes + 1), index, "uniforms"), ap, ap + 4 * rows * nodes,
+                               ap + 4 * rows * (nodes + 1), rows, nodes, vocab, _dtype_code(target.dtype))
+    code = lib.mrt_draft_verify(args, index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+    return got[:rows * nodes].view(rows, nodes), got[rows * nodes:rows * (nodes + 1)], got[rows * (nodes + 1):]
+
+
+def i8_quantize(x):
+    """8-bit codes of the rows of x (rows, k), k a multiple of 16 (mrt_i8_quantize): (int8 (rows, k), fp32 scales (rows))."""
+    lib, torch, index = load_library(), _torch(), x.get_device()
+    if x.dim() != 2 or index < 0 or x.stride(1) != 1 or _dtype_code(x.dtype) < 0:
+        raise ValueError("x must be (rows, k) fp32, bf16 or fp16 on a GPU, rows contiguous")
+    rows, k = x.shape
+    codes = torch.empty((rows, k), dtype=torch.int8, device=x.device)
+    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
+    code = lib.mrt_i8_quantize(x.data_ptr(), x.stride(0), rows, k, _dtype_code(x.dtype), codes.data_ptr(), k,
+                               scales.data_ptr(), index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+    return codes, scales
+
+
+def i8_matmul(x, x_scale, w, w_scale, dtype=None, add=None, out=None):
+    """Product of 8-bit codes with a scale for each row and column (mrt_i8_matmul): (rows, n) in ``dtype``.
+
+    x int8 (rows, k), x_scale fp32 (rows); w int8 (n, k), w_scale fp32 (n), as
+    ``i8_quantize`` makes them: out = (x w^T) x_scale w_scale + add, add (rows,
+    n) or None, which may be out.  dtype: that of out or add where given, else bf16.
+    """
+    lib, torch, index = load_library(), _torch(), x.get_device()
+    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype is not torch.int8 or w.dtype is not torch.int8:
+        raise ValueError("x and w must be int8 (rows, k) and (n, k)")
+    (rows, k), n = x.shape, w.shape[0]
+    if index < 0 or w.get_device() != index or x.stride(1) != 1 or w.stride(1) != 1:
+        raise ValueError("x and w must be on one GPU, rows contiguous")
+    if dtype is None:
+        dtype = out.dtype if out is not None else add.dtype if add is not None else torch.bfloat16
+    if out is None:
+        out = torch.empty((rows, n), dtype=dtype, device=x.device)
+    for t, what in ((out, "out"), (add, "add")):
+        if t is not None and (t.shape != (rows, n) or t.dtype is not dtype or t.get_device() != index or t.stride(1) != 1):
+            raise ValueError(f"{what} must be (rows, n) in dtype, on x's GPU, rows contiguous")
+    args = _I8_STRUCT.pack(x.data_ptr(), _floats(x_scale, (rows,), index, "x_scale"), w.data_ptr(),
+                           _floats(w_scale, (n,), index, "w_scale"), 0 if add is None else add.data_ptr(), out.data_ptr(),
+                           x.stride(0), w.stride(0), 0 if add is None else add.stride(0), out.stride(0), rows, n, k,
+                           _dtype_code(dtype))
+    code = lib.mrt_i8_matmul(args, index, _raw_stream(index))
+    if code:
+        _check(lib, code)
+    return out
