@@ -27,6 +27,7 @@
 // device, from the lengths, which the host never sees; parts leave (maximum, sum, output)
 // in fp32 and k_paged_join sums them in order, so a result does not depend on timing.
 #include <algorithm>
+#include <climits>
 #include <type_traits>
 
 #include "attn_frag.hpp"
@@ -219,24 +220,37 @@ struct CodeFrag {
   static constexpr int KC = DP / 64;  // 16-byte loads of a key row, a lane
   static constexpr int E = DP / 16;   // codes of a V row, a lane
   static constexpr int VW = E / 4;    // the same in registers
-  __device__ __forceinline__ static void load_row(const char* row, int g, int D, uint4 (&f)[KC]) {
+  // The lane's byte offsets from a tile's first row on, of K and of V (j: row 4 g + j).  What
+  // lies past D is read from the row's start: queries have digits 0 there, outputs no place.
+  struct Offsets {
+    uint32_t k[KC], v[4];
+    __device__ __forceinline__ Offsets(uint32_t slot, int i, int g, int D) {
 #pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      const int d = (c * 4 + g) * 16;
-      f[c] = (D == DP || d < D) ? ld_g16(row + d) : make_uint4(0, 0, 0, 0);
+      for (int c = 0; c < KC; ++c) k[c] = i * slot + ((c * 4 + g) * 16 < D ? (c * 4 + g) * 16 : 0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) v[j] = (4 * g + j) * slot + (i * E < D ? i * E : 0);
     }
+  };
+  // Widened where it is used, an offset needs no registers for 64 bits: the load adds it to
+  // the uniform base.
+  __device__ __forceinline__ static uint32_t here(uint32_t at) {
+    asm volatile("" : "+v"(at));
+    return at;
   }
-  __device__ __forceinline__ static void load_v(const char* row, int i, int D, uint32_t (&f)[VW]) {
-    const char* p = row + i * E;
-    const bool in = D == DP || i * E < D;
+  __device__ __forceinline__ static void load_row(const char* base, const Offsets& at, uint4 (&f)[KC]) {
+#pragma unroll
+    for (int c = 0; c < KC; ++c) f[c] = ld_g16(base + here(at.k[c]));
+  }
+  __device__ __forceinline__ static void load_v(const char* base, uint32_t at, uint32_t (&f)[VW]) {
+    at = here(at);
     if constexpr (VW == 4) {
-      const uint4 x = in ? ld_g16(p) : make_uint4(0, 0, 0, 0);
+      const uint4 x = ld_g16(base + at);
       f[0] = x.x, f[1] = x.y, f[2] = x.z, f[3] = x.w;
     } else if constexpr (VW == 2) {
-      const uint64_t x = in ? ld_g(reinterpret_cast<const uint64_t*>(p)) : 0ull;
+      const uint64_t x = ld_g(reinterpret_cast<const uint64_t*>(base + at));
       f[0] = (uint32_t)x, f[1] = (uint32_t)(x >> 32);
     } else {
-      f[0] = in ? ld_g(reinterpret_cast<const uint32_t*>(p)) : 0u;
+      f[0] = ld_g(reinterpret_cast<const uint32_t*>(base + at));
     }
   }
   // One query row: the digits of lane group g's 16 KC values, and f.
@@ -315,6 +329,34 @@ struct CodeFrag {
 };
 
 // ---- what both kernels share ------------------------------------------------------------
+
+// The bias by distance of a K/V head's heads: in LDS where it fits, else in memory.
+struct BiasTable {
+  const float* lds;
+  const float* mem;
+  int last;  // column of the furthest distances
+  bool small;
+  __device__ __forceinline__ BiasTable(const PageArgs& a, float* buf, int kvh, int n)
+      : lds(buf), mem(a.bias + (size_t)kvh * n * a.buckets), last(a.buckets - 1), small(n * a.buckets <= kBiasLds) {}
+  // By the whole block; true if a barrier is due.
+  __device__ __forceinline__ bool fill(float* buf, int n, int threads) const {
+    if (!small) return false;
+    for (int x = threadIdx.x; x < n * (last + 1); x += threads) buf[x] = mem[x];
+    return true;
+  }
+  // use(j, value, in log2 units) for the distances far - off(j), j < J, of query head hq.
+  template <int J, class Off, class Use>
+  __device__ __forceinline__ void each(int hq, int far, Off&& off, Use&& use) const {
+    const int row = hq * (last + 1);
+    if (small) {
+#pragma unroll
+      for (int j = 0; j < J; ++j) use(j, lds[row + min(max(far - off(j), 0), last)] * kLog2e);
+    } else {
+#pragma unroll
+      for (int j = 0; j < J; ++j) use(j, ld_g(mem + row + min(max(far - off(j), 0), last)) * kLog2e);
+    }
+  }
+};
 
 struct Work {
   int b, kvh, row0, s0, s1, steps, id;
@@ -419,8 +461,8 @@ __global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
   const T* kc = static_cast<const T*>(a.k) + kvh * a.head_stride;
   const T* vc = static_cast<const T*>(a.v) + kvh * a.head_stride;
 
-  // Nothing here needs the length: what lies past it is masked, and pages that are not
-  // there are not read.
+  // Nothing here needs the length: what lies past it is masked, and so is what has no page,
+  // which is read from page 0.
   Lookup look;
   int looked = w.s0 + wid;  // the step of the lookup's first tile
   look.fetch(a, table, looked, W, lane);
@@ -437,28 +479,15 @@ __global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
   };
   auto load_k = [&] {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (page[h] >= 0) {
-        F::load_row(kc + page[h] * a.page_stride + (int64_t)(place[h] + i) * a.slot_stride, g, D, kf[h]);
-      } else {
-#pragma unroll
-        for (int c = 0; c < KC; ++c) kf[h][c] = make_uint4(0, 0, 0, 0);
-      }
-    }
+    for (int h = 0; h < 2; ++h)
+      F::load_row(kc + max(page[h], 0) * a.page_stride + (int64_t)(place[h] + i) * a.slot_stride, g, D, kf[h]);
   };
   auto load_v = [&] {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const T* base = vc + (page[h] >= 0 ? page[h] * a.page_stride + (int64_t)place[h] * a.slot_stride : 0);
+      const T* base = vc + max(page[h], 0) * a.page_stride + (int64_t)place[h] * a.slot_stride;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (page[h] >= 0) {
-          F::load_v(base + (4 * g + j) * a.slot_stride, i, D, vf[h * 4 + j]);
-        } else {
-#pragma unroll
-          for (int x = 0; x < VW; ++x) vf[h * 4 + j][x] = 0u;
-        }
-      }
+      for (int j = 0; j < 4; ++j) F::load_v(base + (4 * g + j) * a.slot_stride, i, D, vf[h * 4 + j]);
     }
   };
   find(w.s0 + wid);
@@ -471,21 +500,16 @@ __global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float2 ml[W][16 * NR];
   float* btab = reinterpret_cast<float*>(lds);  // the bias of this K/V head's heads, until the waves join
-  const bool bias_in_lds = n * a.buckets <= kBiasLds;
+  const BiasTable table_of(a, btab, kvh, n);
   uint4 q[NR][KC];
-  int last[NR];  // the newest entry that the row sees; -1: the row is not there
-  const float* brow[NR];
+  int last[NR], head[NR];  // the newest entry that the row sees, -1: the row is not there; its query head of the K/V head's
 #pragma unroll
   for (int t = 0; t < NR; ++t) {
     const int r = min(w.row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
     F::load_row(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D, q[t]);
-    last[t] = node < fresh ? len + node : -1;
-    brow[t] = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
+    last[t] = node < fresh ? len + node : -1, head[t] = hq;
   }
-  if (a.bias != nullptr && bias_in_lds) {
-    for (int x = tid; x < n * a.buckets; x += 64 * W) btab[x] = a.bias[(size_t)kvh * n * a.buckets + x];
-    ring_barrier();
-  }
+  if (a.bias != nullptr && table_of.fill(btab, n, 64 * W)) ring_barrier();  // does not wait for the loads of the first step
 
   f32x4_t o[NR][E];
   float m[NR], l[NR];
@@ -507,15 +531,15 @@ __global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
   // with `exact` all) are left out of it and added by class.
   auto step = [&](int st, auto exact, auto&& next) {
     const int base = st * KEYS;
-    const bool whole = base + KEYS <= len + 1 && fresh > 0 && page[0] >= 0 && page[1] >= 0;
-    const bool apart = exact.value || (fresh > 1 && base + KEYS > len + 1);
     const bool in[2] = {page[0] >= 0, page[1] >= 0};
+    const bool whole = base + KEYS <= len + 1 && fresh > 0 && in[0] && in[1];
+    const bool apart = exact.value || (fresh > 1 && base + KEYS > len + 1);
     const int page_v[2] = {page[0], page[1]}, place_v[2] = {place[0], place[1]};
     if (!whole) {
 #pragma unroll
       for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int x = 0; x < VW; ++x) vf[j][x] = base + lane_key(g, j) < end ? vf[j][x] : 0u;
+        for (int x = 0; x < VW; ++x) vf[j][x] = in[j >> 2] && base + lane_key(g, j) < end ? vf[j][x] : 0u;
     }
     float p[NR][8];
 #pragma unroll
@@ -523,19 +547,17 @@ __global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
       const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
       const float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
       if (a.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float by = brow[t][bucket(last[t], base + lane_key(g, j), a.buckets)] * kLog2e;
-          p[t][j] = fmaf(s[j], scale2, by);
-          if (by < kNone) p[t][j] = -INFINITY;  // masked, whatever the key holds
-        }
+        table_of.template each<8>(head[t], last[t] - base - 4 * g, [](int j) { return lane_key(0, j); }, [&](int j, float by) {
+          p[t][j] = by < kNone ? -INFINITY : fmaf(s[j], scale2, by);  // a masked key may hold anything
+        });
       } else {
 #pragma unroll
         for (int j = 0; j < 8; ++j) p[t][j] = s[j] * scale2;
       }
       if (!whole) {
+        const int most[2] = {in[0] ? last[t] - base - 4 * g : -1, in[1] ? last[t] - base - 4 * g : -1};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) p[t][j] = in[j >> 2] && base + lane_key(g, j) <= last[t] ? p[t][j] : -INFINITY;
+        for (int j = 0; j < 8; ++j) p[t][j] = lane_key(0, j) <= most[j >> 2] ? p[t][j] : -INFINITY;
       }
     }
     next();
@@ -647,34 +669,25 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
       place[t] = __builtin_amdgcn_readlane(look.place, x + t);
     }
   };
-  // Pages that are not there are not read: their keys are masked, whatever the registers hold.
+  const typename F::Offsets at((uint32_t)a.slot_stride, i, g, D);
+  // Keys whose page is not there are read from page 0, and masked.
   auto load_k = [&](int st) {
     const int x = (st - looked) / W * 4 + g;  // of the lane's own key, 16 g + i
     const int pg = __shfl(look.page, x, 64), pl = __shfl(look.place, x, 64);
-    const int64_t at = ((int64_t)max(pg, 0) * a.kv_heads + kvh) * page_size + pl + i;
-    ks = pg >= 0 ? ld_g(a.k_scale + at) : 0.f;
-    vs = pg >= 0 ? ld_g(a.v_scale + at) : 0.f;
+    const int64_t own = ((int64_t)max(pg, 0) * a.kv_heads + kvh) * page_size + pl + i;
+    ks = ld_g(a.k_scale + own);
+    vs = ld_g(a.v_scale + own);
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
-      if (page[t] >= 0) F::load_row(kc + page[t] * a.page_stride + (int64_t)(place[t] + i) * a.slot_stride, g, D, kf[t]);
+    for (int t = 0; t < 4; ++t) F::load_row(kc + max(page[t], 0) * a.page_stride + place[t] * a.slot_stride, at, kf[t]);
   };
   auto load_v = [&] {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
-      if (page[t] < 0) continue;
-      const char* base = vc + page[t] * a.page_stride + (int64_t)place[t] * a.slot_stride;
+      const char* base = vc + max(page[t], 0) * a.page_stride + place[t] * a.slot_stride;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) F::load_v(base + (4 * g + j) * a.slot_stride, i, D, vf[4 * t + j]);
+      for (int j = 0; j < 4; ++j) F::load_v(base, at.v[j], vf[4 * t + j]);
     }
   };
-#pragma unroll
-  for (int t = 0; t < 4; ++t)
-#pragma unroll
-    for (int c = 0; c < KC; ++c) kf[t][c] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-  for (int j = 0; j < 16; ++j)
-#pragma unroll
-    for (int x = 0; x < VW; ++x) vf[j][x] = 0u;
   find(w.s0 + wid);
   load_k(w.s0 + wid);
   load_v();
@@ -686,23 +699,18 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
   __shared__ float2 ml[W][16 * NR];
   __shared__ __attribute__((aligned(16))) float sc[W][128];  // the scales of a wave's step
   float* btab = reinterpret_cast<float*>(lds);
-  const bool bias_in_lds = n * a.buckets <= kBiasLds;
+  const BiasTable table_of(a, btab, kvh, n);
   uint4 qa[NR][KC], qb[NR][KC], qc[NR][KC];
   float qf[NR];
-  int last[NR];
-  const float* brow[NR];
+  int last[NR], head[NR];
 #pragma unroll
   for (int t = 0; t < NR; ++t) {
     const int r = min(w.row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
     qf[t] = F::digits(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D,
                       qa[t], qb[t], qc[t]) * a.scale * kLog2e;
-    last[t] = node < fresh ? len + node : -1;
-    brow[t] = (bias_in_lds ? btab : a.bias + (size_t)kvh * n * a.buckets) + hq * a.buckets;
+    last[t] = node < fresh ? len + node : -1, head[t] = hq;
   }
-  if (a.bias != nullptr && bias_in_lds) {
-    for (int x = tid; x < n * a.buckets; x += 64 * W) btab[x] = a.bias[(size_t)kvh * n * a.buckets + x];
-    ring_barrier();
-  }
+  if (a.bias != nullptr && table_of.fill(btab, n, 64 * W)) ring_barrier();  // does not wait for the loads of the first step
 
   f32x4_t o[NR][E];
   float m[NR], l[NR];
@@ -713,11 +721,21 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
     for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
   }
   const i32x4_t zero = {0, 0, 0, 0};
+  // Keys at distances beyond the table's have its last value, unless that is a mask.
+  float far[NR];
+  bool plain = true;
+#pragma unroll
+  for (int t = 0; t < NR; ++t) {
+    far[t] = 0.f;
+    if (a.bias != nullptr) table_of.template each<1>(head[t], INT_MAX, [](int) { return 0; }, [&](int, float by) { far[t] = by; });
+    plain = plain && far[t] >= kNone;
+  }
+  const int near = a.bias == nullptr ? INT_MAX : __all(plain) ? len - a.buckets + 2 : 0;  // from here on the table is read
 
   for (int st = w.s0 + wid; st < w.s1; st += W) {
     const int base = st * KEYS;
     const bool there = page[0] >= 0 && page[1] >= 0 && page[2] >= 0 && page[3] >= 0;
-    const bool masks = a.bias != nullptr || !there || fresh == 0 || base + KEYS > len + 1;
+    const bool masks = !there || fresh == 0 || base + KEYS > min(near, len + 1);
     const bool in[4] = {page[0] >= 0, page[1] >= 0, page[2] >= 0, page[3] >= 0};
     const bool more = st + W < w.s1;
     sc[wid][lane] = ks, sc[wid][64 + lane] = vs;  // read by the wave's lanes alone, in order
@@ -737,7 +755,11 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
         const float4 s = *reinterpret_cast<const float4*>(&sc[wid][k * 16 + 4 * g]);
         const float by_key[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-        for (int r = 0; r < 4; ++r) p[t][4 * k + r] = join_digits(x[r], y[r], z[r]) * qf[t] * by_key[r];
+        for (int r = 0; r < 4; ++r) {
+          p[t][4 * k + r] = join_digits(x[r], y[r], z[r]) * qf[t] * by_key[r];
+          asm volatile("" : "+v"(p[t][4 * k + r]));  // here: the sums of all tiles do not fit the registers
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if (more) {
@@ -759,22 +781,27 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
         sv[4 * k] = s.x, sv[4 * k + 1] = s.y, sv[4 * k + 2] = s.z, sv[4 * k + 3] = s.w;
       }
       if (masks) {
+        const int upto = last[t] - base - 4 * g;  // the row's newest key, from the lane's first on
+        auto key = [](int j) { return (j >> 2) * 16 + (j & 3); };
+        if (a.bias != nullptr)
+          table_of.template each<16>(head[t], upto, key, [&](int j, float by) { p[t][j] = by < kNone ? -INFINITY : p[t][j] + by; });
+        const int most[4] = {in[0] ? upto : -1, in[1] ? upto : -1, in[2] ? upto : -1, in[3] ? upto : -1};
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const int key = base + (j >> 2) * 16 + 4 * g + (j & 3);
-          float by = 0.f;
-          if (a.bias != nullptr) by = brow[t][bucket(last[t], key, a.buckets)] * kLog2e;
-          const float x = p[t][j] + by;
-          const bool out = by < kNone || x < kNone || !in[j >> 2] || key > last[t];
-          p[t][j] = out ? -INFINITY : x;
+          const bool out = key(j) > most[j >> 2] || p[t][j] < kNone;
+          p[t][j] = out ? -INFINITY : p[t][j];
           sv[j] = out ? 0.f : sv[j];  // a masked entry's scale may be NaN
         }
+      } else if (a.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) p[t][j] += far[t];
       }
       float top = p[t][0];
 #pragma unroll
       for (int j = 1; j < 16; ++j) top = fmaxf(top, p[t][j]);
       top = max_over_groups(top);
       if (__any(top > m[t])) {
+        asm volatile("");  // a branch: most steps leave the output alone
         const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
         m[t] = mn;
         l[t] *= f;
@@ -798,13 +825,16 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
       uint4 op[4];
       F::transpose(vf, x, op);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
+      for (int e = 0; e < 4; ++e) {
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
           const i32x4_t u = mma8(op[e], wa[t], zero), v = mma8(op[e], wb[t], zero), y = mma8(op[e], wc[t], zero);
 #pragma unroll
           for (int r = 0; r < 4; ++r) o[t][4 * x + e][r] = fmaf(join_digits(u[r], v[r], y[r]), wf[t], o[t][4 * x + e][r]);
+          asm volatile("" : "+v"(o[t][4 * x + e]));
         }
+        if (e & 1) __builtin_amdgcn_sched_barrier(0);
+      }
     }
     if (more) load_v();
   }
