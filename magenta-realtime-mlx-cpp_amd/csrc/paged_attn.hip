@@ -23,9 +23,12 @@
 // dimension, transposed in registers by byte permutations, are its operand of
 // O^T = V^T P^T.
 //
-// A unit's steps are cut into parts of equal size where the card needs more blocks, on the
-// device, from the lengths, which the host never sees; parts leave (maximum, sum, output)
-// in fp32 and k_paged_join sums them in order, so a result does not depend on timing.
+// As many blocks run as the card holds.  Long caches: the units' steps, one after the other,
+// are cut into equal shares, on the device, from the lengths, which the host never sees; a
+// share may end and begin inside units, whose parts leave (maximum, sum, output) in fp32, and
+// k_paged_join sums them in order, so a result does not depend on timing.  Short ones: a block
+// takes whole units in turn.  Either way the next unit's first keys are requested before
+// this one's waves join.
 #include <algorithm>
 #include <climits>
 #include <type_traits>
@@ -38,6 +41,18 @@ namespace mrt {
 namespace {
 
 constexpr int kBiasLds = 4096;  // floats of the bias by distance kept in LDS
+
+// Row tiles a wave holds at most: what one more takes in registers costs more than reading
+// the keys again from the L2.
+constexpr int row_tiles(size_t elt, int dp) { return elt == 2 && dp <= 64 ? 2 : 1; }
+// Waves of a block, and blocks that a CU holds (by their registers).
+constexpr int waves_of(size_t elt, int dp) { return elt == 2 && dp == 128 ? 8 : 4; }
+constexpr int blocks_of_cu(size_t elt, int dp, int nr) {
+  return elt == 1 ? (dp == 256 ? 1 : 2) : elt == 4 ? (dp == 32 ? 4 : dp == 64 ? 2 : 1)
+                                                   : dp == 32 ? 4 / nr : dp == 64 ? (nr == 1 ? 3 : 2) : 1;
+}
+#define MRT_ATTN_BOUNDS(elt) \
+  __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(blocks_of_cu(elt, DP, NR) * W / 4)))
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 struct PageArgs {
@@ -51,8 +66,9 @@ struct PageArgs {
   int64_t q_row, q_node, q_head, o_row, o_node, o_head, page_stride, head_stride, slot_stride, table_stride;
   Divide by_tiles;  // 16-key tiles of a page
   int page_tiles, row_pages, pages, rows, kv_heads, heads, tokens, D, buckets;
-  int parts;   // wanted of the whole work; 0: units are not cut
-  int least;   // steps that a part has at least
+  int teams;   // blocks that take a share each
+  int least;   // steps that a share has at least
+  int unit;    // steps that beginning and ending a unit counts as; 0: units are not cut
   int row_blocks;
   float scale;
 };
@@ -75,40 +91,110 @@ __device__ __forceinline__ int steps_of(const PageArgs& a, int b) {
   return n == 0 ? 0 : (min(length_of(a, b) + n, capacity_of(a)) + KEYS - 1) / KEYS;
 }
 
-// Steps of a part, the same for all units: ceil(total / parts), at least `least`; the
-// last part of a unit may have fewer.  At most parts + units parts then.
-template <int KEYS>
-__device__ __forceinline__ int chunk_of(const PageArgs& a, int lane) {
-  int64_t sum = 0;
-  for (int b = lane; b < a.rows; b += 64) sum += steps_of<KEYS>(a, b);
+// Positions of all units' steps in a row, each unit's after `unit` of its own, cut into `teams`
+// shares of `total`: share t is [t total / teams, (t + 1) total / teams), rounded down.
+struct Shares {
+  int64_t total;
+  int teams;
+  __device__ __forceinline__ int64_t begin(int t) const { return t * total / teams; }
+  __device__ __forceinline__ int of(int64_t at) const { return (int)(((at + 1) * teams + total - 1) / total) - 1; }
+};
+__device__ __forceinline__ int64_t wave_sum64(int64_t v) {
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, 64);
-  const int64_t total = uniform(sum) * a.kv_heads;
-  return max(a.least, (int)((total + a.parts - 1) / a.parts));
+  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+  return uniform(v);
 }
-__device__ __forceinline__ int parts_of(int steps, int chunk) { return max(1, (steps + chunk - 1) / chunk); }
-
-// The sequence whose units hold part `at` of all, and the parts before it; rows if none.
 template <int KEYS>
-__device__ __forceinline__ int find_row(const PageArgs& a, int lane, int chunk, int64_t at, int64_t* before) {
-  int64_t base = 0;
-  for (int b0 = 0; b0 < a.rows; b0 += 64) {
-    const int64_t own = b0 + lane < a.rows ? (int64_t)parts_of(steps_of<KEYS>(a, b0 + lane), chunk) * a.kv_heads : 0;
-    int64_t incl = own;
+__device__ __forceinline__ Shares shares_of(const PageArgs& a, int lane) {
+  int64_t steps = 0;
+  for (int b = lane; b < a.rows; b += 64) steps += steps_of<KEYS>(a, b);
+  steps = wave_sum64(steps) * a.kv_heads;
+  Shares s;
+  s.total = steps + (int64_t)a.unit * a.rows * a.kv_heads;
+  s.teams = (int)max((int64_t)1, min((int64_t)a.teams, s.total / a.least));
+  return s;
+}
+
+// One unit's part: steps s0 .. s1 - 1 of its `steps`.  Whole units of short caches leave s1
+// and steps open, so that no key waits for the length.
+struct Part {
+  int b, kvh, s0, s1, steps;
+  int64_t slot;  // of its result, if the unit is cut: unit + team, which are all different
+  bool open, all;
+};
+
+// The parts of a team, one after the other.
+template <int KEYS>
+struct Walk {
+  int64_t at, from, to;  // cut: where the next unit begins, the share
+  int team, b, kvh, steps;
+  __device__ __forceinline__ Walk(const PageArgs& a, int lane, int team_) : at(0), from(0), to(0), team(team_), b(0), kvh(0), steps(0) {
+    if (a.unit == 0) {
+      b = team / a.kv_heads, kvh = team - b * a.kv_heads;
+      return;
+    }
+    const Shares s = shares_of<KEYS>(a, lane);
+    if (team >= s.teams) return;
+    from = s.begin(team), to = s.begin(team + 1);
+    int64_t base = 0;
+    for (int b0 = 0; b0 < a.rows; b0 += 64) {  // the row that holds position `from`
+      const int own_steps = b0 + lane < a.rows ? steps_of<KEYS>(a, b0 + lane) : 0;
+      const int64_t own = b0 + lane < a.rows ? (int64_t)(own_steps + a.unit) * a.kv_heads : 0;
+      int64_t incl = own;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const int64_t x = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += x;
+      for (int o = 1; o < 64; o <<= 1) {
+        const int64_t x = __shfl_up(incl, o, 64);
+        if (lane >= o) incl += x;
+      }
+      const uint64_t past = __ballot(base + incl > from);
+      if (past != 0) {
+        const int l = __ffsll((unsigned long long)past) - 1;
+        base += uniform((int64_t)__shfl(incl - own, l, 64));
+        b = b0 + l, steps = uniform(__shfl(own_steps, l, 64));
+        kvh = (int)((from - base) / (steps + a.unit));
+        at = base + (int64_t)kvh * (steps + a.unit);
+        return;
+      }
+      base += uniform((int64_t)__shfl(incl, 63, 64));
     }
-    const uint64_t past = __ballot(base + incl > at);
-    if (past != 0) {
-      const int l = __ffsll((unsigned long long)past) - 1;
-      *before = uniform((int64_t)(base + __shfl(incl - own, l, 64)));
-      return uniform(b0 + l);
-    }
-    base += uniform((int64_t)__shfl(incl, 63, 64));
   }
-  return a.rows;
+  __device__ __forceinline__ bool next(const PageArgs& a, Part& w) {
+    if (a.unit == 0) {
+      if (b >= a.rows) return false;
+      w.b = b, w.kvh = kvh, w.s0 = 0, w.s1 = w.steps = 0, w.slot = 0, w.open = w.all = true;
+      const int64_t u = (int64_t)b * a.kv_heads + kvh + a.teams;
+      b = (int)(u / a.kv_heads), kvh = (int)(u - (int64_t)b * a.kv_heads);
+      return true;
+    }
+    while (at < to) {
+      const int64_t first = at + a.unit;  // of the unit's steps
+      w.b = b, w.kvh = kvh, w.steps = steps, w.open = false;
+      w.s0 = (int)max((int64_t)0, from - first), w.s1 = (int)min((int64_t)steps, to - first);
+      w.slot = (int64_t)b * a.kv_heads + kvh + team;
+      w.all = w.s0 == 0 && w.s1 == steps;
+      // a unit without steps, whose outputs are zeros, falls to the share with its beginning
+      const bool mine = steps == 0 ? at >= from : w.s0 < w.s1;
+      at = first + steps;
+      if (++kvh == a.kv_heads) {
+        kvh = 0, ++b;
+        steps = b < a.rows ? uniform(steps_of<KEYS>(a, b)) : 0;
+      }
+      if (mine) return true;
+    }
+    return false;
+  }
+};
+
+// The team of this block, and its first query row; row blocks of a team share keys and follow
+// each other on one XCD.
+__device__ __forceinline__ int team_of(const PageArgs& a, int rows_of_block, int& row0) {
+  if (a.row_blocks == 1) {
+    row0 = 0;
+    return blockIdx.x;
+  }
+  const int x = blockIdx.x >> 3, rb = x % a.row_blocks;
+  row0 = rb * rows_of_block;
+  return (x / a.row_blocks) * 8 + (blockIdx.x & 7);
 }
 
 // The page and place in it of a wave's next tiles, one a lane.
@@ -358,45 +444,11 @@ struct BiasTable {
   }
 };
 
-struct Work {
-  int b, kvh, row0, s0, s1, steps, id;
-  bool all;
-};
-
-// The block's part; false: none.  Where units are not cut, s1 and steps are left for later,
-// since they depend on the length.
-template <int KEYS, int NR>
-__device__ __forceinline__ bool find_work(const PageArgs& a, int lane, Work& w) {
-  int64_t id = blockIdx.x;
-  int rb = 0;
-  if (a.row_blocks > 1) {  // the row blocks of a part share keys: they follow each other on one XCD
-    const int x = blockIdx.x >> 3;
-    rb = x % a.row_blocks;
-    id = (int64_t)(x / a.row_blocks) * 8 + (blockIdx.x & 7);
-  }
-  w.row0 = rb * (16 * NR);
-  w.id = (int)id;
-  if (a.parts == 0) {
-    if (id >= (int64_t)a.rows * a.kv_heads) return false;
-    w.b = w.id / a.kv_heads, w.kvh = w.id - w.b * a.kv_heads, w.s0 = 0, w.s1 = w.steps = 0, w.all = true;
-    return true;
-  }
-  const int chunk = chunk_of<KEYS>(a, lane);
-  int64_t before = 0;
-  w.b = find_row<KEYS>(a, lane, chunk, id, &before);
-  if (w.b >= a.rows) return false;
-  w.steps = steps_of<KEYS>(a, w.b);
-  const int n = parts_of(w.steps, chunk), at = (int)(id - before);
-  w.kvh = at / n;
-  w.s0 = (at - w.kvh * n) * chunk, w.s1 = min(w.steps, w.s0 + chunk);
-  w.all = n == 1;
-  return true;
-}
-
 // Joins the waves' outputs at the common maximum and stores the rows.  l: the lane's own
-// sums.  In two halves, so that the buffer holds half of the waves' outputs.
+// sums.  In two halves, so that the buffer holds half of the waves' outputs.  No barrier
+// waits for loads: those of the next part are on their way.
 template <typename T, int W, int NR, int E>
-__device__ __forceinline__ void join_waves(const PageArgs& a, const Work& w, int there_rows, char* lds, float2 (*ml)[16 * NR],
+__device__ __forceinline__ void join_waves(const PageArgs& a, const Part& w, int row0, int there_rows, char* lds, float2 (*ml)[16 * NR],
                                            const float (&m)[NR], float (&l)[NR], f32x4_t (&o)[NR][E]) {
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   constexpr int H = W / 2;
@@ -406,7 +458,7 @@ __device__ __forceinline__ void join_waves(const PageArgs& a, const Work& w, int
     l[t] = sum_over_groups(l[t]);
     if (g == 0) ml[wid][t * 16 + i] = make_float2(m[t], l[t]);
   }
-  __syncthreads();  // and the bias in LDS has been read
+  ring_barrier();  // and the bias in LDS has been read
   float top[NR], sum[NR];
 #pragma unroll
   for (int t = 0; t < NR; ++t) {
@@ -422,19 +474,19 @@ __device__ __forceinline__ void join_waves(const PageArgs& a, const Work& w, int
       if (wid >= H) buf[((wid - H) * NR * E + t * E + e) * 64 + lane] = o[t][e];
     }
   }
-  __syncthreads();
+  ring_barrier();
   if (wid < H) {
 #pragma unroll
     for (int t = 0; t < NR; ++t)
 #pragma unroll
       for (int e = 0; e < E; ++e) buf[(wid * NR * E + t * E + e) * 64 + lane] += o[t][e];
   }
-  __syncthreads();
+  ring_barrier();
   const int R = a.tokens * (a.heads / a.kv_heads);
 #pragma unroll
   for (int t = 0; t < NR; ++t) {
     if (wid / 4 != t % (W / 4)) continue;  // wave x: register x % 4 of every W / 4 th row tile
-    const int r = w.row0 + t * 16 + i, reg = wid & 3, d = (4 * g + reg) * E;
+    const int r = row0 + t * 16 + i, reg = wid & 3, d = (4 * g + reg) * E;
     if (r >= R) continue;
     float v[E];
 #pragma unroll
@@ -443,29 +495,30 @@ __device__ __forceinline__ void join_waves(const PageArgs& a, const Work& w, int
 #pragma unroll
       for (int x = 0; x < H; ++x) v[e] += reinterpret_cast<const float*>(&buf[(x * NR * E + t * E + e) * 64 + lane])[reg];
     }
-    emit<T, E>(a, w.all, w.id, w.b, w.kvh, r, d, v, top[t], sum[t], r < there_rows);
+    emit<T, E>(a, w.all, w.slot, w.b, w.kvh, r, d, v, top[t], sum[t], r < there_rows);
   }
+  ring_barrier();  // the buffer is free
 }
 
 template <typename T, int DP, int NR, int W>
-__global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
+__global__ MRT_ATTN_BOUNDS(sizeof(T)) void k_paged(const PageArgs a) {
   using F = AttnFrag<T, DP>;
   constexpr int E = F::E, VW = F::VW, KC = F::KC, KEYS = 32;
   using Lookup = TileLookup<2>;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, D = a.D;
-  Work w;
-  if (!find_work<KEYS, NR>(a, lane, w)) return;
-  const int b = w.b, kvh = w.kvh, n = a.heads / a.kv_heads, R = a.tokens * n;
-  const int* table = a.table + b * a.table_stride;
-  const T* kc = static_cast<const T*>(a.k) + kvh * a.head_stride;
-  const T* vc = static_cast<const T*>(a.v) + kvh * a.head_stride;
+  int row0;
+  Walk<KEYS> walk(a, lane, team_of(a, 16 * NR, row0));
+  Part w;
+  if (!walk.next(a, w)) return;
+  const int n = a.heads / a.kv_heads, R = a.tokens * n;
+  const int* table;
+  const T *kc, *vc;
 
   // Nothing here needs the length: what lies past it is masked, and so is what has no page,
   // which is read from page 0.
   Lookup look;
-  int looked = w.s0 + wid;  // the step of the lookup's first tile
-  look.fetch(a, table, looked, W, lane);
+  int looked;  // the step of the lookup's first tile
   uint4 kf[2][KC];
   uint32_t vf[8][VW];
   int page[2], place[2];
@@ -490,12 +543,22 @@ __global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
       for (int j = 0; j < 4; ++j) F::load_v(base + (4 * g + j) * a.slot_stride, i, D, vf[h * 4 + j]);
     }
   };
-  find(w.s0 + wid);
-  load_k();
-  load_v();
+  auto request = [&] {  // the first keys of part w
+    table = a.table + w.b * a.table_stride;
+    kc = static_cast<const T*>(a.k) + w.kvh * a.head_stride;
+    vc = static_cast<const T*>(a.v) + w.kvh * a.head_stride;
+    looked = w.s0 + wid;
+    look.fetch(a, table, looked, W, lane);
+    find(looked);
+    load_k();
+    load_v();
+  };
+  request();
 
+  for (;;) {
+  const int b = w.b, kvh = w.kvh;
   const int len = length_of(a, b), fresh = fresh_of(a, b), end = min(len + fresh, capacity_of(a));
-  if (a.parts == 0) w.s1 = w.steps = steps_of<KEYS>(a, b);
+  if (w.open) w.s1 = w.steps = steps_of<KEYS>(a, b);
 
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float2 ml[W][16 * NR];
@@ -505,7 +568,7 @@ __global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
   int last[NR], head[NR];  // the newest entry that the row sees, -1: the row is not there; its query head of the K/V head's
 #pragma unroll
   for (int t = 0; t < NR; ++t) {
-    const int r = min(w.row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
+    const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
     F::load_row(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D, q[t]);
     last[t] = node < fresh ? len + node : -1, head[t] = hq;
   }
@@ -630,33 +693,34 @@ __global__ __launch_bounds__(64 * W) void k_paged(const PageArgs a) {
   for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]) && last[t] >= 0;
   if (__builtin_expect(__any(odd), 0)) {  // rare: this wave's steps once more
     begin();
-    looked = w.s0 + wid;
-    look.fetch(a, table, looked, W, lane);
-    find(looked);
-    load_k();
-    load_v();
+    request();
     steps(std::true_type{});
   }
-  join_waves<T, W, NR, E>(a, w, fresh * n, lds, ml, m, l, o);
+  const Part done = w;
+  const bool more = walk.next(a, w);
+  if (more) request();
+  join_waves<T, W, NR, E>(a, done, row0, fresh * n, lds, ml, m, l, o);
+  if (!more) break;
+  }
 }
 
 template <typename T, int DP, int NR, int W>
-__global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
+__global__ MRT_ATTN_BOUNDS(1) void k_paged_codes(const PageArgs a) {
   using F = CodeFrag<DP>;
   constexpr int E = F::E, VW = F::VW, KC = F::KC, KEYS = 64;
   using Lookup = TileLookup<4>;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, D = a.D;
-  Work w;
-  if (!find_work<KEYS, NR>(a, lane, w)) return;
-  const int b = w.b, kvh = w.kvh, n = a.heads / a.kv_heads, R = a.tokens * n, page_size = a.page_tiles * kPageUnit;
-  const int* table = a.table + b * a.table_stride;
-  const char* kc = static_cast<const char*>(a.k) + kvh * a.head_stride;
-  const char* vc = static_cast<const char*>(a.v) + kvh * a.head_stride;
+  int row0;
+  Walk<KEYS> walk(a, lane, team_of(a, 16 * NR, row0));
+  Part w;
+  if (!walk.next(a, w)) return;
+  const int n = a.heads / a.kv_heads, R = a.tokens * n, page_size = a.page_tiles * kPageUnit;
+  const int* table;
+  const char *kc, *vc;
 
   Lookup look;
-  int looked = w.s0 + wid;
-  look.fetch(a, table, looked, W, lane);
+  int looked;
   uint4 kf[4][KC];
   uint32_t vf[16][VW];
   float ks, vs;  // the scales of key `lane` of the step, of K and of V
@@ -674,7 +738,7 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
   auto load_k = [&](int st) {
     const int x = (st - looked) / W * 4 + g;  // of the lane's own key, 16 g + i
     const int pg = __shfl(look.page, x, 64), pl = __shfl(look.place, x, 64);
-    const int64_t own = ((int64_t)max(pg, 0) * a.kv_heads + kvh) * page_size + pl + i;
+    const int64_t own = ((int64_t)max(pg, 0) * a.kv_heads + w.kvh) * page_size + pl + i;
     ks = ld_g(a.k_scale + own);
     vs = ld_g(a.v_scale + own);
 #pragma unroll
@@ -688,12 +752,22 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
       for (int j = 0; j < 4; ++j) F::load_v(base, at.v[j], vf[4 * t + j]);
     }
   };
-  find(w.s0 + wid);
-  load_k(w.s0 + wid);
-  load_v();
+  auto request = [&] {
+    table = a.table + w.b * a.table_stride;
+    kc = static_cast<const char*>(a.k) + w.kvh * a.head_stride;
+    vc = static_cast<const char*>(a.v) + w.kvh * a.head_stride;
+    looked = w.s0 + wid;
+    look.fetch(a, table, looked, W, lane);
+    find(looked);
+    load_k(looked);
+    load_v();
+  };
+  request();
 
+  for (;;) {
+  const int b = w.b, kvh = w.kvh;
   const int len = length_of(a, b), fresh = fresh_of(a, b);
-  if (a.parts == 0) w.s1 = w.steps = steps_of<KEYS>(a, b);
+  if (w.open) w.s1 = w.steps = steps_of<KEYS>(a, b);
 
   extern __shared__ __attribute__((aligned(16))) char lds[];
   __shared__ float2 ml[W][16 * NR];
@@ -705,7 +779,7 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
   int last[NR], head[NR];
 #pragma unroll
   for (int t = 0; t < NR; ++t) {
-    const int r = min(w.row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
+    const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
     qf[t] = F::digits(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D,
                       qa[t], qb[t], qc[t]) * a.scale * kLog2e;
     last[t] = node < fresh ? len + node : -1, head[t] = hq;
@@ -838,7 +912,12 @@ __global__ __launch_bounds__(64 * W) void k_paged_codes(const PageArgs a) {
     }
     if (more) load_v();
   }
-  join_waves<T, W, NR, E>(a, w, fresh * n, lds, ml, m, l, o);
+  const Part done = w;
+  const bool again = walk.next(a, w);
+  if (again) request();
+  join_waves<T, W, NR, E>(a, done, row0, fresh * n, lds, ml, m, l, o);
+  if (!again) break;
+  }
 }
 
 // ---- joining parts ------------------------------------------------------------------------
@@ -852,13 +931,14 @@ __global__ __launch_bounds__(256) void k_paged_join(const PageArgs a, int cols) 
   const int r = (blockIdx.x - unit * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (r >= R) return;
   const int b = unit / a.kv_heads, kvh = unit - b * a.kv_heads, steps = steps_of<KEYS>(a, b);
-  const int chunk = chunk_of<KEYS>(a, lane), parts = parts_of(steps, chunk);
-  if (parts == 1) return;  // written by its block
+  if (steps == 0) return;
+  const Shares sh = shares_of<KEYS>(a, lane);
   int64_t first = 0;
-  for (int x = lane; x < b; x += 64) first += parts_of(steps_of<KEYS>(a, x), chunk);
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) first += __shfl_xor(first, o, 64);
-  first = uniform(first) * a.kv_heads + (int64_t)kvh * parts;
+  for (int x = lane; x < b; x += 64) first += a.unit + steps_of<KEYS>(a, x);
+  first = wave_sum64(first) * a.kv_heads + (int64_t)kvh * (a.unit + steps) + a.unit;  // the unit's first step
+  const int t0 = sh.of(first), parts = sh.of(first + steps - 1) - t0 + 1;
+  if (parts == 1) return;  // written by its block
+  first = unit + t0;
   const int d = lane % cols * 4, from = lane / cols, every = 64 / cols;
   const float2* ml = a.part_ml + first * R + r;
   const float* part = a.part + (first * R + r) * a.D;
@@ -890,16 +970,11 @@ __global__ __launch_bounds__(256) void k_paged_join(const PageArgs a, int cols) 
 // ---- host -----------------------------------------------------------------------------------
 
 struct Plan {
-  int keys, tiles, row_blocks, parts, least;
+  int keys, tiles, row_blocks, teams, least, unit;
 };
 
-// Row tiles a wave holds at most, and waves of a block: registers allow two tiles and
-// eight waves (two a SIMD), of wide heads or fp32 values less.
-constexpr int row_tiles(size_t elt, int dp) { return dp == 256 ? 1 : 2; }
-constexpr int waves_of(size_t elt, int dp) { return dp == 256 || (elt == 4 && dp == 128) ? 4 : 8; }
-
 Plan plan(const PagedCache& c, int heads, int tokens) {
-  const int R = tokens * (heads / c.kv_heads), dp = c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
+  const int R = tokens * (heads / c.kv_heads), dp = c.d <= 32 && !c.codes ? 32 : c.d <= 64 ? 64 : c.d <= 128 ? 128 : 256;
   const size_t elt = c.codes ? 1 : dtype_size(c.dt);
   Plan p;
   p.keys = c.codes ? 64 : 32;
@@ -907,33 +982,33 @@ Plan plan(const PagedCache& c, int heads, int tokens) {
   p.row_blocks = (R + 16 * p.tiles - 1) / (16 * p.tiles);
   const int64_t units = std::max<int64_t>(1, (int64_t)c.rows * c.kv_heads);
   const int64_t steps = ((int64_t)c.capacity() + p.keys - 1) / p.keys;
-  p.least = 2 * waves_of(elt, dp);
-  p.parts = std::max(8, 1024 / p.row_blocks);
-  if (steps <= p.least || units >= 4096) p.parts = 0;
+  const int waves = waves_of(elt, dp), teams = std::max(8, 256 * blocks_of_cu(elt, dp, p.tiles) / p.row_blocks / 8 * 8);
+  p.least = 2 * waves;
+  p.unit = steps <= 2 * p.least || units >= 8 * teams ? 0 : 2 * waves;
+  p.teams = p.unit == 0 ? (int)std::min<int64_t>((units + 7) / 8 * 8, teams) : teams;
   return p;
 }
 
-size_t blocks_of(const PagedCache& c, const Plan& p) { return (size_t)p.parts + (size_t)c.rows * c.kv_heads; }
+size_t slots_of(const PagedCache& c, const Plan& p) { return (size_t)p.teams + (size_t)c.rows * c.kv_heads; }
 
 template <typename K>
-void start(K kernel, int threads, size_t lds, const PageArgs& a, size_t blocks, hipStream_t s) {
+void start(K kernel, int threads, size_t lds, const PageArgs& a, hipStream_t s) {
   lds = std::max(lds, a.bias != nullptr ? (size_t)kBiasLds * 4 : size_t{0});
   allow_dynamic_lds(reinterpret_cast<const void*>(kernel), 96 * 1024);
-  const size_t grid = a.row_blocks > 1 ? (blocks + 7) / 8 * 8 * a.row_blocks : blocks;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(threads), lds, s, a);
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(a.teams * a.row_blocks)), dim3(threads), lds, s, a);
 }
 
 template <typename T, int DP, int NR>
-void launch(const PageArgs& a, bool codes, size_t blocks, hipStream_t s) {
+void launch(const PageArgs& a, bool codes, hipStream_t s) {
   if constexpr (NR <= row_tiles(sizeof(T), DP)) {
     if (codes) {
       if constexpr (DP >= 64) {
         constexpr int W = waves_of(1, DP);
-        start(&k_paged_codes<T, DP, NR, W>, 64 * W, (size_t)W / 2 * NR * (DP / 16) * 1024, a, blocks, s);
+        start(&k_paged_codes<T, DP, NR, W>, 64 * W, (size_t)W / 2 * NR * (DP / 16) * 1024, a, s);
       }
     } else {
       constexpr int W = waves_of(sizeof(T), DP);
-      start(&k_paged<T, DP, NR, W>, 64 * W, (size_t)W / 2 * NR * (DP / 16) * 1024, a, blocks, s);
+      start(&k_paged<T, DP, NR, W>, 64 * W, (size_t)W / 2 * NR * (DP / 16) * 1024, a, s);
     }
   }
 }
@@ -944,12 +1019,12 @@ bool paged_attention_fits(const PagedCache& c, int heads, int tokens) {
   const Plan p = plan(c, heads, tokens);
   const int64_t units = (int64_t)c.rows * c.kv_heads, most = (1ll << 32) - 1;  // threads of a launch
   const int R = tokens * (heads / c.kv_heads);
-  return ((int64_t)blocks_of(c, p) + 7) / 8 * 8 * p.row_blocks * 512 <= most && units * ((R + 3) / 4) * 256 <= most;
+  return (int64_t)p.teams * p.row_blocks * 512 <= most && units * ((R + 3) / 4) * 256 <= most;
 }
 
 size_t paged_attention_workspace(const PagedCache& c, int heads, int tokens) {
   const Plan p = plan(c, heads, tokens);
-  return p.parts == 0 ? 0 : blocks_of(c, p) * (size_t)(heads / c.kv_heads * tokens) * (c.d + 2) * 4;
+  return p.unit == 0 ? 0 : slots_of(c, p) * (size_t)(heads / c.kv_heads * tokens) * (c.d + 2) * 4;
 }
 
 void paged_attention(const PagedCache& c, const PagedAttnArgs& t, void* ws, hipStream_t s) {
@@ -962,18 +1037,17 @@ void paged_attention(const PagedCache& c, const PagedAttnArgs& t, void* ws, hipS
   a.page_stride = c.page_stride, a.head_stride = c.head_stride, a.slot_stride = c.slot_stride, a.table_stride = c.table_stride;
   a.page_tiles = c.page_size / kPageUnit, a.by_tiles = Divide(a.page_tiles), a.row_pages = c.row_pages, a.pages = c.pages;
   a.rows = c.rows, a.kv_heads = c.kv_heads, a.heads = t.heads, a.tokens = t.tokens, a.D = c.d, a.buckets = t.buckets;
-  a.parts = p.parts, a.least = p.least, a.row_blocks = p.row_blocks, a.scale = t.scale;
+  a.teams = p.teams, a.unit = p.unit, a.least = p.least, a.row_blocks = p.row_blocks, a.scale = t.scale;
   const int R = t.tokens * (t.heads / c.kv_heads);
-  const size_t blocks = blocks_of(c, p);
-  if (p.parts > 0) {
+  if (p.unit > 0) {
     a.part = static_cast<float*>(ws);
-    a.part_ml = reinterpret_cast<float2*>(a.part + blocks * R * c.d);
+    a.part_ml = reinterpret_cast<float2*>(a.part + slots_of(c, p) * R * c.d);
   }
   MRT_DTYPE_DISPATCH(t.dt, {
     auto tiles = [&](auto width) {
       constexpr int DP = decltype(width)::value;
-      if (p.tiles == 1) launch<T, DP, 1>(a, c.codes, blocks, s);
-      else launch<T, DP, 2>(a, c.codes, blocks, s);
+      if (p.tiles == 1) launch<T, DP, 1>(a, c.codes, s);
+      else launch<T, DP, 2>(a, c.codes, s);
     };
     if (c.d <= 32 && !c.codes) tiles(std::integral_constant<int, 32>{});
     else if (c.d <= 64) tiles(std::integral_constant<int, 64>{});
@@ -981,7 +1055,7 @@ void paged_attention(const PagedCache& c, const PagedAttnArgs& t, void* ws, hipS
     else tiles(std::integral_constant<int, 256>{});
   });
   MRT_HIP_CHECK(hipGetLastError());
-  if (p.parts > 0) {
+  if (p.unit > 0) {
     const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64;
     const dim3 grid((unsigned)((size_t)c.rows * c.kv_heads * ((R + 3) / 4)));
     MRT_DTYPE_DISPATCH(t.dt, {
