@@ -880,8 +880,12 @@ typedef struct mrt_draft_verify_args {
  * the target's own draws.  Without draft: uniforms[child] * Z < r[x], else r[x] = 0
  * and Z = Z - r[x].  In 64 bits; probabilities that are not positive finite
  * numbers count as 0, nodes with a token outside the vocabulary as absent.
- * accepted: the path's ids, ascending, then -1. */
-int mrt_draft_verify(const mrt_draft_verify_args* args, int device, void* hip_stream);
+ * accepted: the path's ids, ascending, then -1.
+ * mrt_draft_verify_workspace gives the workspace bytes (0: none; workspace may then be
+ * NULL); it goes by rows, vocab and whether there are draft and parents. */
+int mrt_draft_verify_workspace(const mrt_draft_verify_args* args, size_t* bytes);
+int mrt_draft_verify(const mrt_draft_verify_args* args, void* workspace, size_t workspace_bytes, int device,
+                     void* hip_stream);
 
 /* 8-bit codes of the rows of src (rows, k), row stride ld, in `dtype`: scales (rows)
  * and codes (rows, k), row stride ldc, as mrt_paged_write makes them; a row that

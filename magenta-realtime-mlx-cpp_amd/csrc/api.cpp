@@ -386,6 +386,25 @@ void check_i8(int rows, int k) {
   require(k >= 16 && k % 16 == 0 && k < (1 << 17), "8-bit products: k must be a multiple of 16, below 2^17");
 }
 
+// Sizes and strides checked; the pointers are not looked at.
+mrt::VerifyArgs to_verify(const mrt_draft_verify_args* args) {
+  to_dtype(args->dtype);
+  require(args->rows >= 0 && args->rows <= (1 << 20), "draft_verify: rows must be in 0..2^20");
+  mrt::VerifyArgs a;
+  a.rows = args->rows, a.nodes = args->nodes, a.vocab = args->vocab;
+  if (a.rows == 0) return a;
+  require(a.nodes >= 1 && a.nodes <= mrt::kMaxNodes, "draft_verify: nodes must be in 1..64");
+  require(a.vocab >= 1 && a.vocab <= (1 << 24), "draft_verify: vocab must be in 1..2^24");
+  require(args->target_row_stride >= 0 && args->target_slot_stride >= 0 && args->draft_row_stride >= 0 &&
+              args->draft_slot_stride >= 0 && args->parents_stride >= 0,
+          "draft_verify: negative stride");
+  a.target = args->target, a.draft = args->draft, a.t_row = args->target_row_stride, a.t_slot = args->target_slot_stride;
+  a.d_row = args->draft_row_stride, a.d_slot = args->draft_slot_stride, a.tokens = args->tokens;
+  a.parents = args->parents, a.parents_stride = args->parents_stride, a.uniforms = args->uniforms;
+  a.accepted = args->accepted, a.count = args->count, a.token = args->token;
+  return a;
+}
+
 mrt::CodecConfig to_codec_config(const mrt_codec_config* c, int* max_frames) {
   mrt::CodecConfig k;
   k.embedding_dim = c->embedding_dim;
@@ -1308,33 +1327,31 @@ int mrt_paged_attention(const mrt_paged_cache* cache, const mrt_paged_attention_
   });
 }
 
-int mrt_draft_verify(const mrt_draft_verify_args* args, int device, void* hip_stream) {
+int mrt_draft_verify_workspace(const mrt_draft_verify_args* args, size_t* bytes) {
+  return guarded([&] {
+    require(args != nullptr && bytes != nullptr, "null argument");
+    *bytes = mrt::draft_verify_workspace(to_verify(args));
+  });
+}
+
+int mrt_draft_verify(const mrt_draft_verify_args* args, void* workspace, size_t workspace_bytes, int device, void* hip_stream) {
   return guarded([&] {
     require(args != nullptr, "null argument");
     const mrt::DType dt = to_dtype(args->dtype);
-    require(args->rows >= 0 && args->rows <= (1 << 20), "draft_verify: rows must be in 0..2^20");
-    if (args->rows == 0) return;
-    require(args->nodes >= 1 && args->nodes <= mrt::kMaxNodes, "draft_verify: nodes must be in 1..64");
-    require(args->vocab >= 1 && args->vocab <= (1 << 24), "draft_verify: vocab must be in 1..2^24");
-    require(args->target && args->tokens && args->uniforms && args->accepted && args->count && args->token,
-            "draft_verify: null argument");
+    const mrt::VerifyArgs a = to_verify(args);
+    if (a.rows == 0) return;
+    require(a.target && a.tokens && a.uniforms && a.accepted && a.count && a.token, "draft_verify: null argument");
     const size_t size = mrt::dtype_size(dt);
-    require(aligned(args->target, size) && aligned(args->draft, size), "draft_verify: target and draft must be aligned to their elements");
-    require(args->target_row_stride >= 0 && args->target_slot_stride >= 0 && args->draft_row_stride >= 0 &&
-                args->draft_slot_stride >= 0 && args->parents_stride >= 0,
-            "draft_verify: negative stride");
-    require(aligned4({args->tokens, args->parents, args->uniforms, args->accepted, args->count, args->token}),
+    require(aligned(a.target, size) && aligned(a.draft, size), "draft_verify: target and draft must be aligned to their elements");
+    require(aligned4({a.tokens, a.parents, a.uniforms, a.accepted, a.count, a.token}),
             "draft_verify: int32 and fp32 arrays must be 4-byte aligned");
-    require(args->accepted != args->count && args->accepted != args->token && args->count != args->token,
+    require(a.accepted != a.count && a.accepted != a.token && a.count != a.token,
             "draft_verify: outputs must be arrays of their own");
-    mrt::VerifyArgs a;
-    a.target = args->target, a.draft = args->draft, a.t_row = args->target_row_stride, a.t_slot = args->target_slot_stride;
-    a.d_row = args->draft_row_stride, a.d_slot = args->draft_slot_stride, a.tokens = args->tokens;
-    a.parents = args->parents, a.parents_stride = args->parents_stride, a.uniforms = args->uniforms;
-    a.accepted = args->accepted, a.count = args->count, a.token = args->token;
-    a.rows = args->rows, a.nodes = args->nodes, a.vocab = args->vocab;
+    const size_t want = mrt::draft_verify_workspace(a);
+    require(want == 0 || (workspace != nullptr && workspace_bytes >= want && aligned(workspace, 16)),
+            "draft_verify: workspace too small, misaligned or null");
     OnDevice on(device);
-    mrt::draft_verify(dt, a, static_cast<hipStream_t>(hip_stream));
+    mrt::draft_verify(dt, a, workspace, static_cast<hipStream_t>(hip_stream));
   });
 }
 

@@ -104,10 +104,11 @@ __device__ __forceinline__ int64_t wave_sum64(int64_t v) {
   for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return uniform(v);
 }
+// first: the steps of a unit of row `lane`.
 template <int KEYS>
-__device__ __forceinline__ Shares shares_of(const PageArgs& a, int lane) {
-  int64_t steps = 0;
-  for (int b = lane; b < a.rows; b += 64) steps += steps_of<KEYS>(a, b);
+__device__ __forceinline__ Shares shares_of(const PageArgs& a, int lane, int first) {
+  int64_t steps = first;
+  for (int b = lane + 64; b < a.rows; b += 64) steps += steps_of<KEYS>(a, b);
   steps = wave_sum64(steps) * a.kv_heads;
   Shares s;
   s.total = steps + (int64_t)a.unit * a.rows * a.kv_heads;
@@ -133,12 +134,13 @@ struct Walk {
       b = team / a.kv_heads, kvh = team - b * a.kv_heads;
       return;
     }
-    const Shares s = shares_of<KEYS>(a, lane);
+    int own_steps = lane < a.rows ? steps_of<KEYS>(a, lane) : 0;
+    const Shares s = shares_of<KEYS>(a, lane, own_steps);
     if (team >= s.teams) return;
     from = s.begin(team), to = s.begin(team + 1);
     int64_t base = 0;
     for (int b0 = 0; b0 < a.rows; b0 += 64) {  // the row that holds position `from`
-      const int own_steps = b0 + lane < a.rows ? steps_of<KEYS>(a, b0 + lane) : 0;
+      if (b0 > 0) own_steps = b0 + lane < a.rows ? steps_of<KEYS>(a, b0 + lane) : 0;
       const int64_t own = b0 + lane < a.rows ? (int64_t)(own_steps + a.unit) * a.kv_heads : 0;
       int64_t incl = own;
 #pragma unroll
@@ -922,49 +924,52 @@ __global__ MRT_ATTN_BOUNDS(1) void k_paged_codes(const PageArgs a) {
 
 // ---- joining parts ------------------------------------------------------------------------
 
-// A wave a row: the row's parts at their common maximum, in order.  `cols` lanes (a power of
-// two, 4 cols >= D) take a part's outputs, four each, 64 / cols parts at a time.
+// A block a row: the row's parts at their common maximum.  `cols` lanes (a power of two, 4
+// cols >= D) take a part's outputs, four each; groups of lanes take parts in turn, and are
+// summed in order.
 template <typename T, int KEYS>
 __global__ __launch_bounds__(256) void k_paged_join(const PageArgs a, int cols) {
-  const int lane = threadIdx.x & 63, n = a.heads / a.kv_heads, R = a.tokens * n;
-  const int blocks = (R + 3) / 4, unit = blockIdx.x / blocks;
-  const int r = (blockIdx.x - unit * blocks) * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (r >= R) return;
-  const int b = unit / a.kv_heads, kvh = unit - b * a.kv_heads, steps = steps_of<KEYS>(a, b);
+  const int tid = threadIdx.x, lane = tid & 63, n = a.heads / a.kv_heads, R = a.tokens * n;
+  const int unit = blockIdx.x / R, r = blockIdx.x - unit * R, b = unit / a.kv_heads, kvh = unit - b * a.kv_heads;
+  // steps of the units of this row, and of all and those before it
+  const int own = lane < a.rows ? steps_of<KEYS>(a, lane) : 0, steps = steps_of<KEYS>(a, b);
   if (steps == 0) return;
-  const Shares sh = shares_of<KEYS>(a, lane);
-  int64_t first = 0;
-  for (int x = lane; x < b; x += 64) first += a.unit + steps_of<KEYS>(a, x);
+  const Shares sh = shares_of<KEYS>(a, lane, own);
+  int64_t first = lane < b ? a.unit + own : 0;
+  for (int x = lane + 64; x < b; x += 64) first += a.unit + steps_of<KEYS>(a, x);
   first = wave_sum64(first) * a.kv_heads + (int64_t)kvh * (a.unit + steps) + a.unit;  // the unit's first step
   const int t0 = sh.of(first), parts = sh.of(first + steps - 1) - t0 + 1;
   if (parts == 1) return;  // written by its block
   first = unit + t0;
-  const int d = lane % cols * 4, from = lane / cols, every = 64 / cols;
   const float2* ml = a.part_ml + first * R + r;
-  const float* part = a.part + (first * R + r) * a.D;
-  float top = kNone, sum = 0.f, v[4] = {0.f, 0.f, 0.f, 0.f};
+  const int groups = 256 / cols, group = tid / cols, d = tid % cols * 4;
+  const float* part = a.part + (first * R + r) * a.D + min(d, a.D - 4);
+  float top = kNone;
+  for (int s = lane; s < parts; s += 64) top = fmaxf(top, ml[(size_t)s * R].x);
+  top = wave_max(top);
+  float sum = 0.f;
   for (int s0 = 0; s0 < parts; s0 += 64) {
     const float2 y = s0 + lane < parts ? ml[(size_t)(s0 + lane) * R] : make_float2(kNone, 0.f);
-    const float to = fmaxf(top, wave_max(y.x)), f = fade(top - to);
-    top = to;
-    const float w = s0 + lane < parts ? fade(y.x - top) : 0.f;
-    sum = fmaf(sum, f, wave_sum(y.y * w));
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] *= f;
-    const int end = min(64, parts - s0);
-    for (int s = from; s < (end + every - 1) / every * every; s += every) {
-      const float ws = __shfl(w, s, 64);
-      if (s < end && d < a.D) {
-        const float4 z = *reinterpret_cast<const float4*>(part + (size_t)(s0 + s) * R * a.D + d);
-        v[0] = fmaf(z.x, ws, v[0]), v[1] = fmaf(z.y, ws, v[1]), v[2] = fmaf(z.z, ws, v[2]), v[3] = fmaf(z.w, ws, v[3]);
-      }
-    }
+    sum += wave_sum(y.y * fade(y.x - top));
   }
-  for (int o = cols; o < 64; o <<= 1) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] += __shfl_xor(v[e], o, 64);
+  float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = group; s < parts; s += groups) {
+    const float w = fade(ml[(size_t)s * R].x - top);
+    const float4 z = *reinterpret_cast<const float4*>(part + (size_t)s * R * a.D);
+    v[0] = fmaf(z.x, w, v[0]), v[1] = fmaf(z.y, w, v[1]), v[2] = fmaf(z.z, w, v[2]), v[3] = fmaf(z.w, w, v[3]);
   }
-  if (from == 0 && d < a.D) emit<T, 4>(a, true, 0, b, kvh, r, d, v, top, sum, r / n < fresh_of(a, b));
+  __shared__ float4 sums[256];
+  sums[tid] = make_float4(v[0], v[1], v[2], v[3]);
+  __syncthreads();
+  if (tid >= cols) return;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = 0.f;
+  for (int x = 0; x < groups; ++x) {
+    const float4 z = sums[x * cols + tid];
+    v[0] += z.x, v[1] += z.y, v[2] += z.z, v[3] += z.w;
+  }
+  if (d < a.D) emit<T, 4>(a, true, 0, b, kvh, r, d, v, top, sum, r / n < fresh_of(a, b));
 }
 
 // ---- host -----------------------------------------------------------------------------------
@@ -984,7 +989,7 @@ Plan plan(const PagedCache& c, int heads, int tokens) {
   const int64_t steps = ((int64_t)c.capacity() + p.keys - 1) / p.keys;
   const int waves = waves_of(elt, dp), teams = std::max(8, 256 * blocks_of_cu(elt, dp, p.tiles) / p.row_blocks / 8 * 8);
   p.least = 2 * waves;
-  p.unit = steps <= 2 * p.least || units >= 8 * teams ? 0 : 2 * waves;
+  p.unit = steps <= 10 * waves || units >= 8 * teams ? 0 : 2 * waves;
   p.teams = p.unit == 0 ? (int)std::min<int64_t>((units + 7) / 8 * 8, teams) : teams;
   return p;
 }
@@ -1019,7 +1024,7 @@ bool paged_attention_fits(const PagedCache& c, int heads, int tokens) {
   const Plan p = plan(c, heads, tokens);
   const int64_t units = (int64_t)c.rows * c.kv_heads, most = (1ll << 32) - 1;  // threads of a launch
   const int R = tokens * (heads / c.kv_heads);
-  return (int64_t)p.teams * p.row_blocks * 512 <= most && units * ((R + 3) / 4) * 256 <= most;
+  return (int64_t)p.teams * p.row_blocks * 512 <= most && units * R * 256 <= most;
 }
 
 size_t paged_attention_workspace(const PagedCache& c, int heads, int tokens) {
@@ -1057,7 +1062,7 @@ void paged_attention(const PagedCache& c, const PagedAttnArgs& t, void* ws, hipS
   MRT_HIP_CHECK(hipGetLastError());
   if (p.unit > 0) {
     const int cols = c.d <= 32 ? 8 : c.d <= 64 ? 16 : c.d <= 128 ? 32 : 64;
-    const dim3 grid((unsigned)((size_t)c.rows * c.kv_heads * ((R + 3) / 4)));
+    const dim3 grid((unsigned)((size_t)c.rows * c.kv_heads * R));
     MRT_DTYPE_DISPATCH(t.dt, {
       if (c.codes) hipLaunchKernelGGL((k_paged_join<T, 64>), grid, dim3(256), 0, s, a, cols);
       else hipLaunchKernelGGL((k_paged_join<T, 32>), grid, dim3(256), 0, s, a, cols);

@@ -10,10 +10,16 @@
 // All of it in 64 bits: a drawn token is a comparison of sums over the vocabulary, and with sums
 // in 32 bits it would depend on their order.
 //
-// A block a sequence.  Each node's own p(x) and q(x) are gathered at once, so tests need no
-// memory; a rejection costs one pass over the slot's rows, in which wave w sums segments w,
-// w + 16, ..; the drawn token's segment is the only one looked at again.
+// Each node's own p(x) and q(x) are gathered at once, so tests need no memory; a rejection
+// costs one pass over the slot's rows.  Sums are taken by segments of the vocabulary, a wave
+// each, and the drawn token's segment is the only one looked at again.  k_verify does all of
+// it, a block a sequence.  What bounds that is one CU's share of arithmetic in 64 bits, so over
+// large vocabularies the first passes are made by many blocks, a launch each (k_verify_pass):
+// every block walks the tree as far as the sums of the launches before go, which takes no
+// memory, and sums its segments of the pass that is needed next.  Passes beyond those launches
+// are k_verify's own.  Sums are the same either way, bit for bit.
 #include <algorithm>
+#include <type_traits>
 
 #include "device_utils.hpp"
 #include "verify.hpp"
@@ -23,9 +29,13 @@ namespace {
 
 constexpr int kWaves = 16;
 constexpr int kSegments = 256;
+constexpr int kAhead = 4;
+constexpr int kManyVocab = 16384;
 
 // What is not a positive finite number counts as 0.
-__device__ __forceinline__ float counted(float p) { return p > 0.f && p < INFINITY ? p : 0.f; }
+__device__ __forceinline__ float counted(float p) {
+  return __builtin_amdgcn_classf(p, 0x180) ? p : 0.f;  // positive, normal or not
+}
 
 // VEC consecutive probabilities; 0 past the end.
 template <typename T, int VEC>
@@ -56,142 +66,279 @@ __device__ __forceinline__ double wave_sum(double v) {
   return v;
 }
 
+__device__ __forceinline__ double lane_of(double v, int lane) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float lane_of(float v, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), lane));
+}
+__device__ __forceinline__ int lane_of(int v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
+
+// The rejections at a slot, the k-th in lane k of every wave: Z before it, the token.
 struct Rejections {
-  double z[kMaxNodes + 1];  // Z before each rejection
-  int token[kMaxNodes];     // the rejected tokens
+  double z;
+  int token;
 };
 
-// r of element `at` after n rejections.
-template <bool DRAFT>
-__device__ __forceinline__ double rest(double p, double q, int at, const Rejections& j, int n) {
-  for (int k = 0; k < n; ++k) {
-    if constexpr (DRAFT) p = fmax(p - j.z[k] * q, 0.0);
-    else p = at == j.token[k] ? 0.0 : p;
+// r of element `at` after n rejections, at most M of them in registers (absent ones change
+// nothing); M -1: any number.
+template <bool DRAFT, int M>
+struct Rest {
+  double z[M > 0 ? M : 1];
+  int token[M > 0 ? M : 1];
+  const Rejections& rej;
+  int n;
+  __device__ __forceinline__ Rest(const Rejections& r, int n_) : rej(r), n(n_) {
+#pragma unroll
+    for (int k = 0; k < M; ++k) z[k] = k < n ? lane_of(rej.z, k) : 0.0, token[k] = k < n ? lane_of(rej.token, k) : -1;
   }
-  return p;
+  __device__ __forceinline__ double operator()(float p, float q, int at) const {
+    double r = (double)p;
+    auto fold = [&](double zk, int tk) {
+      if constexpr (DRAFT) r = fmax(fma(-zk, (double)q, r), 0.0);
+      else r = at == tk ? 0.0 : r;
+    };
+    if constexpr (M < 0) {
+      for (int k = 0; k < n; ++k) fold(lane_of(rej.z, k), lane_of(rej.token, k));
+    } else {
+#pragma unroll
+      for (int k = 0; k < M; ++k) fold(z[k], token[k]);
+    }
+    return r;
+  }
+};
+
+// A sequence's nodes, node t in lane t of every wave.
+struct Nodes {
+  int parent, token;  // -2, -1: not there
+  float p, q, u;      // of its token at its slot, its random number
+};
+
+// Sums over a slot, by segments, in LDS.
+struct Sums {
+  double seg[kSegments];  // running over the segments
+  double total;
+};
+
+// How the vocabulary is cut: chunks of 64 lanes, `per` of them a segment.
+template <typename T>
+struct Cut {
+  static constexpr int VEC = 16 / sizeof(T), CHUNK = 64 * VEC;
+  int chunks, per, segments;
+  __host__ __device__ explicit Cut(int V)
+      : chunks((V + CHUNK - 1) / CHUNK), per((chunks + kSegments - 1) / kSegments), segments((chunks + per - 1) / per) {}
+};
+
+template <typename T, bool DRAFT>
+__device__ __forceinline__ Nodes gather(const VerifyArgs& a, int b, int lane) {
+  const int N = a.nodes, t = min(lane, N - 1);
+  const T* target = static_cast<const T*>(a.target) + b * a.t_row;
+  const T* draft = static_cast<const T*>(a.draft) + b * a.d_row;
+  const int up = a.parents != nullptr ? a.parents[b * a.parents_stride + t] : t - 1;
+  const int x = a.tokens[(int64_t)b * N + t];
+  Nodes s;
+  s.u = a.uniforms[(int64_t)b * (N + 1) + t];
+  const bool there = lane < N && up >= -1 && up < t, known = x >= 0 && x < a.vocab;
+  s.parent = there ? up : -2;
+  s.token = known ? x : -1;
+  const int slot = there ? up + 1 : 0, at = known ? x : 0;
+  s.p = counted(St<T>::ld(ld_g(target + slot * a.t_slot + at)));
+  s.q = DRAFT ? counted(St<T>::ld(ld_g(draft + slot * a.d_slot + at))) : 1.f;
+  return s;
+}
+
+// Sums of r after n rejections at slot `at`, of the segments first, first + W, .. below
+// `last`, by W waves: put(segment, sum).
+template <typename T, bool DRAFT, int W, int M, class Put>
+__device__ __forceinline__ void sum_segments_of(const VerifyArgs& a, const Cut<T>& cut, bool wide, int b, int at, int n,
+                                                const Rejections& rej, int first, int last, Put&& put) {
+  constexpr int VEC = Cut<T>::VEC, CHUNK = Cut<T>::CHUNK;
+  const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const T* p = static_cast<const T*>(a.target) + b * a.t_row + at * a.t_slot;
+  const T* q = static_cast<const T*>(a.draft) + b * a.d_row + at * a.d_slot;
+  constexpr bool both = DRAFT && M != 0;
+  const Rest<DRAFT, M> r(rej, n);
+  // A wave's chunks, kAhead of them on their way.
+  const int from = first + wid, mine = from < last ? ((last - 1 - from) / W + 1) * cut.per : 0;
+  auto chunk_of = [&](int k) { return (from + k / cut.per * W) * cut.per + k % cut.per; };
+  uint4 pr[kAhead], qr[kAhead];
+  auto load = [&](int k, int j) {
+    const int x = chunk_of(min(k, mine - 1)) * CHUNK + lane * VEC;
+    pr[j] = load_raw<T, VEC>(p, x, a.vocab, wide);
+    if constexpr (both) qr[j] = load_raw<T, VEC>(q, x, a.vocab, wide);
+  };
+  if (mine > 0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) load(j, j);
+  }
+  double sum = 0.0;
+  for (int k0 = 0; k0 < mine; k0 += kAhead) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int k = k0 + j;
+      if (k >= mine) break;
+      const int x = chunk_of(k) * CHUNK + lane * VEC;
+      float pv[VEC], qv[VEC] = {};
+      unpack<T, VEC>(pr[j], pv);
+      if constexpr (both) unpack<T, VEC>(qr[j], qv);
+      if (k + kAhead < mine) load(k + kAhead, j);
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sum += r(pv[e], qv[e], x + e);
+      if ((k + 1) % cut.per == 0) {
+        sum = wave_sum(sum);
+        if (lane == 0) put(from + k / cut.per * W, sum);
+        sum = 0.0;
+      }
+    }
+  }
+}
+
+template <typename T, bool DRAFT, int W, class Put>
+__device__ __forceinline__ void sum_segments(const VerifyArgs& a, const Cut<T>& cut, bool wide, int b, int at, int n,
+                                             const Rejections& rej, int first, int last, Put&& put) {
+  if (n == 0) sum_segments_of<T, DRAFT, W, 0>(a, cut, wide, b, at, n, rej, first, last, put);
+  else if (n <= 2) sum_segments_of<T, DRAFT, W, 2>(a, cut, wide, b, at, n, rej, first, last, put);
+  else sum_segments_of<T, DRAFT, W, -1>(a, cut, wide, b, at, n, rej, first, last, put);
+}
+
+// s.seg from the segments' sums to running ones, and s.total; by the whole block.
+__device__ __forceinline__ void run_sums(Sums& s, int segments) {
+  const int lane = threadIdx.x & 63;
+  __syncthreads();
+  if (threadIdx.x < 64) {  // four segments a lane
+    double v[4], run = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      run += lane * 4 + k < segments ? s.seg[lane * 4 + k] : 0.0;
+      v[k] = run;
+    }
+    double incl = run;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double y = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += y;
+    }
+    double before = __shfl_up(incl, 1, 64);
+    if (lane == 0) before = 0.0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (lane * 4 + k < segments) s.seg[lane * 4 + k] = before + v[k];
+    if (lane == 63) s.total = incl;
+  }
+  __syncthreads();
+}
+
+struct End {
+  int slot, rejected, accepted;  // where the walk ended, rejections there, nodes accepted
+  int path;                      // lane k: the k-th accepted node
+  Rejections rej;
+};
+
+// The walk, the same in every wave.  pass(slot, n, rejections) leaves the sums of r after n
+// rejections in s, or returns false where the walk is to stop.
+template <bool DRAFT, class Pass>
+__device__ __forceinline__ bool walk(const Nodes& node, int lane, const Sums& s, End& end, Pass&& pass) {
+  int here = 0, n = 0, count = 0, path = -1;
+  double z = 1.0;
+  Rejections rej = {0.0, -1};
+  // the children of `here`, in order; nothing was drawn for what is not a token
+  uint64_t kids = __ballot(node.parent == -1 && node.token >= 0);
+  while (kids != 0) {
+    const int t = __ffsll((unsigned long long)kids) - 1;
+    kids &= kids - 1;
+    if (DRAFT && n > 0) {
+      if (!pass(here, n, rej)) return false;
+      z = s.total;
+    }
+    const int x = lane_of(node.token, t);
+    const float q = lane_of(node.q, t);
+    const double r = Rest<DRAFT, -1>(rej, n)(lane_of(node.p, t), q, x);
+    if ((double)lane_of(node.u, t) * z * (double)q < r) {
+      path = lane == count ? t : path;
+      ++count;
+      here = t + 1, n = 0, z = 1.0;
+      kids = __ballot(node.parent == t && node.token >= 0);
+    } else {
+      rej.z = lane == n ? z : rej.z, rej.token = lane == n ? x : rej.token;
+      if (!DRAFT) z -= r;
+      ++n;
+    }
+  }
+  if (!pass(here, n, rej)) return false;
+  if (!(s.total > 0.0) && n > 0) {  // nothing left: the target itself
+    n = 0;
+    if (!pass(here, 0, rej)) return false;
+  }
+  end = {here, n, count, path, rej};
+  return true;
+}
+
+// Pass `round` of each sequence, if it has as many: block (x, b) sums segments x share ..
+// of sequence b.  sums (rounds, rows, kSegments).
+template <typename T, bool DRAFT>
+__global__ __launch_bounds__(256) void k_verify_pass(const VerifyArgs a, bool wide, int round, int share, double* sums) {
+  const Cut<T> cut(a.vocab);
+  const int b = blockIdx.y, first = blockIdx.x * share, last = min(first + share, cut.segments), lane = threadIdx.x & 63;
+  __shared__ Sums s;
+  int done = 0;
+  End end;
+  walk<DRAFT>(gather<T, DRAFT>(a, b, lane), lane, s, end, [&](int at, int n, const Rejections& rej) {
+    double* of = sums + ((int64_t)done * a.rows + b) * kSegments;
+    if (done == round) {
+      sum_segments<T, DRAFT, 4>(a, cut, wide, b, at, n, rej, first, last, [&](int x, double v) { of[x] = v; });
+      return false;
+    }
+    __syncthreads();  // the pass before has been read
+    if ((int)threadIdx.x < cut.segments) s.seg[threadIdx.x] = of[threadIdx.x];
+    run_sums(s, cut.segments);
+    ++done;
+    return true;
+  });
 }
 
 template <typename T, bool DRAFT>
-__global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool wide) {
-  constexpr int VEC = 16 / sizeof(T), CHUNK = 64 * VEC;
+__global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool wide, int rounds, const double* sums) {
+  constexpr int VEC = Cut<T>::VEC, CHUNK = Cut<T>::CHUNK;
+  const Cut<T> cut(a.vocab);
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int N = a.nodes, V = a.vocab;
-  __shared__ double own_p[kMaxNodes], own_q[kMaxNodes], own_u[kMaxNodes + 1];
-  __shared__ int parent[kMaxNodes], token[kMaxNodes], path[kMaxNodes];
-  __shared__ Rejections rej;
-  __shared__ double seg[kSegments];
-  __shared__ double total;
-  const T* target = static_cast<const T*>(a.target) + b * a.t_row;
-  const T* draft = static_cast<const T*>(a.draft) + b * a.d_row;
-  if (tid < N) {
-    const int up = a.parents != nullptr ? a.parents[b * a.parents_stride + tid] : tid - 1;
-    const int x = a.tokens[(int64_t)b * N + tid];
-    const bool there = up >= -1 && up < tid, known = x >= 0 && x < V;
-    parent[tid] = there ? up : -2;
-    token[tid] = known ? x : -1;
-    own_p[tid] = there && known ? (double)counted(St<T>::ld(target[(up + 1) * a.t_slot + x])) : 0.0;
-    own_q[tid] = DRAFT && there && known ? (double)counted(St<T>::ld(draft[(up + 1) * a.d_slot + x])) : 1.0;
-  }
-  if (tid <= N) own_u[tid] = a.uniforms[(int64_t)b * (N + 1) + tid];
-  __syncthreads();
-
-  const int chunks = (V + CHUNK - 1) / CHUNK, per = (chunks + kSegments - 1) / kSegments;
-  const int segments = (chunks + per - 1) / per;
-  // The sums of r after n rejections at slot s: of each segment, running, and of all.
-  auto pass = [&](int s, int n) {
-    const T* p = target + s * a.t_slot;
-    const T* q = draft + s * a.d_slot;
-    const bool both = DRAFT && n > 0;
-    for (int x = wid; x < segments; x += kWaves) {
-      double sum = 0.0;
-      const int end = min((x + 1) * per, chunks);
-      for (int c = x * per; c < end; ++c) {
-        const int at = c * CHUNK + lane * VEC;
-        float pv[VEC], qv[VEC];
-        unpack<T, VEC>(load_raw<T, VEC>(p, at, V, wide), pv);
-        if (both) unpack<T, VEC>(load_raw<T, VEC>(q, at, V, wide), qv);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum += rest<DRAFT>((double)pv[e], both ? (double)qv[e] : 0.0, at + e, rej, n);
-      }
-      sum = wave_sum(sum);
-      if (lane == 0) seg[x] = sum;
-    }
-    __syncthreads();
-    if (wid == 0) {  // running sums, four segments a lane
-      double v[4], run = 0.0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        run += lane * 4 + k < segments ? seg[lane * 4 + k] : 0.0;
-        v[k] = run;
-      }
-      double incl = run;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double y = __shfl_up(incl, o, 64);
-        if (lane >= o) incl += y;
-      }
-      double before = __shfl_up(incl, 1, 64);
-      if (lane == 0) before = 0.0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (lane * 4 + k < segments) seg[lane * 4 + k] = before + v[k];
-      if (lane == 63) total = incl;
-    }
-    __syncthreads();
-  };
-
-  // The path, the same in every thread.
-  int here = 0, n = 0, count = 0;  // slot, rejections there, accepted nodes
-  bool summed = false;             // the last pass was of this slot and n
-  double z = 1.0;
-  for (int t = 0; t < N; ++t) {
-    if (parent[t] + 1 != here) continue;
-    const int x = token[t];
-    if (x < 0) continue;  // not a token: nothing was drawn
-    if (DRAFT && n > 0 && !summed) {
-      pass(here, n);
-      summed = true;
-      z = total;
-    }
-    const double r = rest<DRAFT>(own_p[t], own_q[t], x, rej, n);
-    if (own_u[t] * z * own_q[t] < r) {
-      if (tid == 0) path[count] = t;
-      ++count;
-      here = t + 1, n = 0, z = 1.0, summed = false;
+  const int N = a.nodes, V = a.vocab, per = cut.per, chunks = cut.chunks, segments = cut.segments;
+  __shared__ Sums s;
+  int done = 0;
+  End reached;
+  walk<DRAFT>(gather<T, DRAFT>(a, b, lane), lane, s, reached, [&](int at, int n, const Rejections& rej) {
+    __syncthreads();  // the pass before has been read
+    if (done < rounds) {
+      if (tid < segments) s.seg[tid] = sums[((int64_t)done * a.rows + b) * kSegments + tid];
     } else {
-      __syncthreads();  // everyone has read what is there
-      if (tid == 0) rej.z[n] = z, rej.token[n] = x;
-      __syncthreads();
-      if (!DRAFT) z -= r;
-      ++n;
-      summed = false;
+      sum_segments<T, DRAFT, kWaves>(a, cut, wide, b, at, n, rej, 0, segments, [&](int x, double v) { s.seg[x] = v; });
     }
-  }
-  if (!summed) pass(here, n);
-  if (!(total > 0.0) && n > 0) {  // nothing left: the target itself
-    __syncthreads();
-    n = 0;
-    pass(here, 0);
-  }
-  if (tid < N) a.accepted[(int64_t)b * N + tid] = tid < count ? path[tid] : -1;
-  if (tid == 0) a.count[b] = count;
+    run_sums(s, segments);
+    ++done;
+    return true;
+  });
+  const int here = reached.slot, n = reached.rejected;
+  const Rest<DRAFT, -1> rest(reached.rej, n);
+  if (tid < N) a.accepted[(int64_t)b * N + tid] = tid < reached.accepted ? reached.path : -1;
+  if (tid == 0) a.count[b] = reached.accepted;
   if (wid != 0) return;
 
   // The first segment that exceeds the threshold, then its first chunk, lane, token.
-  const double sum = total, want = fmax(own_u[N] * sum, 0.0);
+  const double sum = s.total, want = fmax(a.uniforms[(int64_t)b * (N + 1) + N] * sum, 0.0);
   int found = -1;
   for (int s0 = 0; s0 < segments && found < 0; s0 += 64) {
-    const uint64_t past = __ballot(s0 + lane < segments && seg[s0 + lane] > want);
+    const uint64_t past = __ballot(s0 + lane < segments && s.seg[s0 + lane] > want);
     if (past != 0) found = s0 + __ffsll((unsigned long long)past) - 1;
   }
   int drawn = -1, latest = -1;  // latest: the last token with a positive r seen
-  const T* p = target + here * a.t_slot;
-  const T* q = draft + here * a.d_slot;
+  const T* p = static_cast<const T*>(a.target) + b * a.t_row + here * a.t_slot;
+  const T* q = static_cast<const T*>(a.draft) + b * a.d_row + here * a.d_slot;
   const bool both = DRAFT && n > 0;
   // Without one (a random number of 1): the last token with any weight, over all segments.
   int c = found < 0 ? 0 : found * per;
   const int end = found < 0 ? chunks : min((found + 1) * per, chunks);
-  double before = found > 0 ? seg[found - 1] : 0.0;
+  double before = found > 0 ? s.seg[found - 1] : 0.0;
   for (; c < end && sum > 0.0; ++c) {
     const int at = c * CHUNK + lane * VEC;
     float pv[VEC], qv[VEC];
@@ -200,7 +347,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool
     double v[VEC], run = 0.0;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
-      v[e] = rest<DRAFT>((double)pv[e], both ? (double)qv[e] : 0.0, at + e, rej, n);
+      v[e] = rest(pv[e], both ? qv[e] : 0.f, at + e);
       run += v[e];
     }
     double incl = run;
@@ -232,17 +379,38 @@ __global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool
   if (lane == 0) a.token[b] = drawn >= 0 ? drawn : latest;
 }
 
+// Passes made by many blocks, a launch each.
+int rounds_of(const VerifyArgs& a) {
+  if (a.vocab < kManyVocab || a.rows >= 256) return 0;
+  return a.draft == nullptr || a.parents == nullptr ? 1 : 3;  // a chain has one, as have drafts that were not drawn
+}
+
 }  // namespace
 
-void draft_verify(DType dt, const VerifyArgs& a, hipStream_t s) {
+size_t draft_verify_workspace(const VerifyArgs& a) { return (size_t)rounds_of(a) * a.rows * kSegments * 8; }
+
+void draft_verify(DType dt, const VerifyArgs& a, void* ws, hipStream_t s) {
   const int64_t unit = 16 / (int64_t)dtype_size(dt);
   auto whole = [&](const void* p, int64_t row, int64_t slot) {
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % unit == 0 && slot % unit == 0;
   };
   const bool wide = whole(a.target, a.t_row, a.t_slot) && (a.draft == nullptr || whole(a.draft, a.d_row, a.d_slot));
+  const int rounds = rounds_of(a);
+  double* sums = static_cast<double*>(ws);
   MRT_DTYPE_DISPATCH(dt, {
-    if (a.draft != nullptr) hipLaunchKernelGGL((k_verify<T, true>), dim3(a.rows), dim3(64 * kWaves), 0, s, a, wide);
-    else hipLaunchKernelGGL((k_verify<T, false>), dim3(a.rows), dim3(64 * kWaves), 0, s, a, wide);
+    auto go = [&](auto drawn) {
+      constexpr bool DRAFT = decltype(drawn)::value;
+      const Cut<T> cut(a.vocab);
+      // four segments a block, a wave each, or as many as give the card two blocks a CU
+      const int blocks = std::max(1, std::min((cut.segments + 3) / 4, 512 / a.rows));
+      const int share = (cut.segments + blocks - 1) / blocks;
+      const dim3 grid((cut.segments + share - 1) / share, a.rows);
+      for (int r = 0; r < rounds; ++r)
+        hipLaunchKernelGGL((k_verify_pass<T, DRAFT>), grid, dim3(256), 0, s, a, wide, r, share, sums);
+      hipLaunchKernelGGL((k_verify<T, DRAFT>), dim3(a.rows), dim3(64 * kWaves), 0, s, a, wide, rounds, sums);
+    };
+    if (a.draft != nullptr) go(std::true_type{});
+    else go(std::false_type{});
   });
   MRT_HIP_CHECK(hipGetLastError());
 }

@@ -21,6 +21,8 @@ struct VerifyArgs {
   int* token = nullptr;             // (rows)
   int rows = 0, nodes = 0, vocab = 0;
 };
-void draft_verify(DType dt, const VerifyArgs& a, hipStream_t s);
+// Bytes of workspace that draft_verify wants (0: none).
+size_t draft_verify_workspace(const VerifyArgs& a);
+void draft_verify(DType dt, const VerifyArgs& a, void* ws, hipStream_t s);
 
 }  // namespace mrt

@@ -324,7 +324,8 @@ def load_library(path: Optional[os.PathLike] = None) -> ctypes.CDLL:
         "mrt_paged_read": (i32, [vp, vp, i32, vp]),
         "mrt_paged_attention_workspace": (i32, [vp, i32, i32, ctypes.POINTER(sz)]),
         "mrt_paged_attention": (i32, [vp, vp, vp, sz, i32, vp]),
-        "mrt_draft_verify": (i32, [vp, i32, vp]),
+        "mrt_draft_verify_workspace": (i32, [vp, ctypes.POINTER(sz)]),
+        "mrt_draft_verify": (i32, [vp, vp, sz, i32, vp]),
         "mrt_i8_quantize": (i32, [vp, ctypes.c_int64, i32, i32, i32, vp, ctypes.c_int64, vp, i32, vp]),
         "mrt_i8_matmul": (i32, [vp, i32, vp]),
         "mrt_codec_config_default": (None, [ctypes.POINTER(_CodecConfig)]),
@@ -1522,6 +1523,14 @@ def paged_attention(q, cache: PagedCache, fresh=None, scale: float = 1.0, bias=N
     return out, lse
 
 
+@functools.lru_cache(maxsize=1024)
+def _verify_workspace(rows, nodes, vocab, drawn, tree) -> int:
+    lib, size = load_library(), ctypes.c_size_t()
+    c = _VERIFY_STRUCT.pack(0, int(drawn), 0, 0, 0, 0, 0, int(tree), 0, 0, 0, 0, 0, rows, nodes, vocab, DTYPE_F32)
+    _check(lib, lib.mrt_draft_verify_workspace(c, ctypes.byref(size)))
+    return size.value
+
+
 def draft_verify(target, draft, tokens, uniforms, parents=None):
     """Which drafted tokens stand against the target's probabilities (mrt_draft_verify).
 
@@ -1552,7 +1561,9 @@ def draft_verify(target, draft, tokens, uniforms, parents=None):
                                _ints(tokens, (rows, nodes), index, "tokens"), tp, pstride,
                                _floats(uniforms, (rows, nodes + 1), index, "uniforms"), ap, ap + 4 * rows * nodes,
                                ap + 4 * rows * (nodes + 1), rows, nodes, vocab, _dtype_code(target.dtype))
-    code = lib.mrt_draft_verify(args, index, _raw_stream(index))
+    size = _verify_workspace(rows, nodes, vocab, draft is not None, parents is not None)
+    ws = torch.empty(size, dtype=torch.uint8, device=target.device) if size else None
+    code = lib.mrt_draft_verify(args, ws.data_ptr() if size else None, size, index, _raw_stream(index))
     if code:
         _check(lib, code)
     return got[:rows * nodes].view(rows, nodes), got[rows * nodes:rows * (nodes + 1)], got[rows * (nodes + 1):]

@@ -135,7 +135,7 @@ def test_workspaces_and_null_arguments(lib):
     refused(lib, lib.mrt_paged_attention(pages(), None, None, 0, 0, None))
     refused(lib, lib.mrt_paged_write(pages(), None, 0, None))
     refused(lib, lib.mrt_paged_read(None, store(), 0, None))
-    refused(lib, lib.mrt_draft_verify(None, 0, None))
+    refused(lib, lib.mrt_draft_verify(None, P, 1 << 30, 0, None))
     refused(lib, lib.mrt_i8_matmul(None, 0, None))
     size = ctypes.c_size_t()
     refused(lib, lib.mrt_paged_attention_workspace(pages(), 4, 4, None))
@@ -154,7 +154,20 @@ def test_workspaces_and_null_arguments(lib):
 
 @pytest.mark.parametrize("bad", BAD_VERIFY)
 def test_verify(lib, bad):
-    refused(lib, lib.mrt_draft_verify(verify(**BAD_VERIFY[bad]), 0, None))
+    refused(lib, lib.mrt_draft_verify(verify(**BAD_VERIFY[bad]), P, 1 << 30, 0, None))
+
+
+def test_verify_workspace(lib):
+    size = ctypes.c_size_t()
+    refused(lib, lib.mrt_draft_verify_workspace(None, ctypes.byref(size)))
+    refused(lib, lib.mrt_draft_verify_workspace(verify(), None))
+    refused(lib, lib.mrt_draft_verify_workspace(verify(nodes=65), ctypes.byref(size)))
+    assert lib.mrt_draft_verify_workspace(verify(), ctypes.byref(size)) == 0 and size.value == 0
+    large = verify(vocab=100000, parents=P)
+    assert lib.mrt_draft_verify_workspace(large, ctypes.byref(size)) == 0 and size.value > 0
+    refused(lib, lib.mrt_draft_verify(large, None, 0, 0, None))
+    refused(lib, lib.mrt_draft_verify(large, P, size.value - 1, 0, None))
+    refused(lib, lib.mrt_draft_verify(large, P + 8, size.value, 0, None))
 
 
 @pytest.mark.parametrize("bad", BAD_PRODUCTS)
@@ -174,7 +187,7 @@ def test_no_rows_is_no_work(lib):
     assert lib.mrt_paged_write(empty, store(k=0, v=0), 0, None) == 0
     assert lib.mrt_paged_read(empty, store(k=0, v=0), 0, None) == 0
     assert lib.mrt_paged_attention(empty, attention(q=0, out=0, lse=0), None, 0, 0, None) == 0
-    assert lib.mrt_draft_verify(verify(rows=0, target=0, tokens=0, u=0, accepted=0, count=0, token=0), 0, None) == 0
+    assert lib.mrt_draft_verify(verify(rows=0, target=0, tokens=0, u=0, accepted=0, count=0, token=0), None, 0, 0, None) == 0
     assert lib.mrt_i8_matmul(product(rows=0, x=0, xs=0, out=0), 0, None) == 0
     assert lib.mrt_i8_quantize(None, 64, 0, 64, 1, None, 64, None, 0, None) == 0
 
