@@ -182,15 +182,18 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a) {
 
 // ---- tiles -----------------------------------------------------------------------------------
 
-// 8-bit operands in the ring: a k-tile is 128 deep, in bytes the same as one of 16-bit
-// operands, and so are its places in LDS.
+// 8-bit operands in the ring: a k-tile is 16 C deep (C 4 or 8), a row of it C chunks of 16
+// bytes.  Chunk c of row r is stored at chunk c ^ swz(r), so that 16 consecutive lanes of a
+// fragment read (16 rows, one chunk) fall in distinct banks.
+template <int C>
 struct Core8 {
   typedef i32x4_t v8;
   typedef i32x16_t Acc;
-  static constexpr int kChunks = 8, kSteps = 4, kParts = 1, kDepth = 128, kProducts = 1;
+  static constexpr int kChunks = C, kSteps = C / 2, kParts = 1, kDepth = 16 * C, kProducts = 1;
   static constexpr bool kFine = false;
-  __device__ static int place(int r, int chunk) { return Core16<bf16>::place(r, chunk); }
-  __device__ static int chunk_at(int r, int pos) { return Core16<bf16>::chunk_at(r, pos); }
+  __device__ static int swz(int r) { return C == 8 ? (r ^ (r >> 3)) & 7 : (r >> 2) & 3; }
+  __device__ static int place(int r, int chunk) { return chunk ^ swz(r); }
+  __device__ static int chunk_at(int r, int pos) { return pos ^ swz(r); }
   __device__ static int chunk(int step, int, int half) { return 2 * step + half; }
   __device__ __forceinline__ static void mma(const v8 (&a)[1], const v8 (&b)[1], int, i32x16_t& c) {
     c = __builtin_amdgcn_mfma_i32_32x32x32_i8(b[0], a[0], c, 0, 0, 0);
@@ -199,68 +202,98 @@ struct Core8 {
 
 __device__ __constant__ uint4 kZeros;  // what k-tiles hold past the end of k
 
-// A wave's tile, first row mb, first column nb: a lane holds row mb + 32 i + lane % 32 of
-// tile (i, j) and four times four consecutive columns.  wide: rows of out and add take
-// vectors of four elements.
-template <typename T, int MI, int NJ>
-__device__ __forceinline__ void store_tile(const I8Args& a, const i32x16_t (&acc)[MI][NJ], int mb, int nb, bool wide) {
+// Results of a wave's tile, whose first row and column are (mb, nb) in the matrix and (mt, nt)
+// in the block's tile: a lane holds row mb + 32 i + lane % 32 of tile (i, j) and four times
+// four consecutive columns; 16-bit results swap halves between lanes l and l + 32, so that a
+// lane stores 16 bytes.  scale: the block's rows' scales, then its columns'.  wide: rows of out
+// (and add) are 16-byte aligned.
+template <typename T, int BM, int MI, int NJ>
+__device__ __forceinline__ void store_tile(const I8Args& a, const i32x16_t (&acc)[MI][NJ], const float* scale, int mb, int nb,
+                                           int mt, int nt, bool wide) {
+  constexpr bool k16 = sizeof(T) == 2;
   const int lane = threadIdx.x & 63, lh = lane >> 5;
+  const bool whole = wide && nb + 32 * NJ <= a.n;
+  float by_row[MI];
 #pragma unroll
-  for (int j = 0; j < NJ; ++j)
+  for (int i = 0; i < MI; ++i) by_row[i] = scale[mt + 32 * i + (lane & 31)];
+#pragma unroll
+  for (int j = 0; j < NJ; ++j) {
+    float by_col[4][4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      const int col = nb + 32 * j + 8 * g + 4 * lh;
-      float by_col[4];
+      const float4 v = *reinterpret_cast<const float4*>(scale + BM + nt + 32 * j + 8 * g + 4 * lh);
+      by_col[g][0] = v.x, by_col[g][1] = v.y, by_col[g][2] = v.z, by_col[g][3] = v.w;
+    }
 #pragma unroll
-      for (int r = 0; r < 4; ++r) by_col[r] = a.w_scale[min(col + r, a.n - 1)];
+    for (int i = 0; i < MI; ++i) {
+      const int row = mb + 32 * i + (lane & 31), first = nb + 32 * j + 4 * lh;
+      const bool there = row < a.rows;
+      const T* add = static_cast<const T*>(a.add) + (int64_t)min(row, a.rows - 1) * a.lda + first;
+      T* dst = static_cast<T*>(a.out) + (int64_t)row * a.ldo + nb + 32 * j;
+      if (whole) {
+        uint32_t w[4][4];  // of group g: the lane's four results, of 16 bits in two words
 #pragma unroll
-      for (int i = 0; i < MI; ++i) {
-        const int row = mb + 32 * i + (lane & 31);
-        if (row >= a.rows) continue;
-        const float by_row = a.x_scale[row];
-        const T* add = static_cast<const T*>(a.add) + row * a.lda + col;
-        T* dst = static_cast<T*>(a.out) + row * a.ldo + col;
-        union {
-          T x[4];
-          uint4 w4;
-          uint2 w2;
-        } u, old;
-        const bool whole = wide && col + 4 <= a.n;
-        if (a.add != nullptr) {
-          if (whole) {
-            if constexpr (sizeof(T) == 4) old.w4 = *reinterpret_cast<const uint4*>(add);
-            else old.w2 = *reinterpret_cast<const uint2*>(add);
+        for (int g = 0; g < 4; ++g) {
+          float y[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) y[r] = (float)acc[i][j][4 * g + r] * by_row[i] * by_col[g][r];
+          if (a.add != nullptr) {
+            union {
+              uint4 w4;
+              uint2 w2;
+              T x[4];
+            } old;
+            if constexpr (k16) old.w2 = *reinterpret_cast<const uint2*>(add + 8 * g);
+            else old.w4 = *reinterpret_cast<const uint4*>(add + 8 * g);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) y[r] += St<T>::ld(old.x[r]);
+          }
+          if constexpr (k16) {
+            w[g][0] = St<T>::bits(y[0]) | (St<T>::bits(y[1]) << 16), w[g][1] = St<T>::bits(y[2]) | (St<T>::bits(y[3]) << 16);
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) old.x[r] = col + r < a.n ? add[r] : T(0);
+            for (int r = 0; r < 4; ++r) w[g][r] = __float_as_uint(y[r]);
           }
         }
+        if constexpr (k16) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const float y = (float)acc[i][j][4 * g + r] * by_row * by_col[r];
-          u.x[r] = St<T>::st(a.add != nullptr ? y + St<T>::ld(old.x[r]) : y);
-        }
-        if (whole) {
-          if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = u.w4;
-          else *reinterpret_cast<uint2*>(dst) = u.w2;
+          for (int h = 0; h < 2; ++h) {
+            const auto s0 = __builtin_amdgcn_permlane32_swap(w[2 * h][0], w[2 * h + 1][0], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(w[2 * h][1], w[2 * h + 1][1], false, false);
+            if (there) *reinterpret_cast<uint4*>(dst + 8 * (2 * h + lh)) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
+          }
         } else {
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (col + r < a.n) dst[r] = u.x[r];
+          for (int g = 0; g < 4; ++g)
+            if (there) *reinterpret_cast<uint4*>(dst + 8 * g + 4 * lh) = make_uint4(w[g][0], w[g][1], w[g][2], w[g][3]);
         }
+      } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float y = (float)acc[i][j][4 * g + r] * by_row[i] * by_col[g][r];
+            if (there && first + 8 * g + r < a.n)
+              dst[8 * g + 4 * lh + r] = St<T>::st(a.add != nullptr ? y + St<T>::ld(add[8 * g + r]) : y);
+          }
       }
     }
+  }
 }
 
 // Block L takes tiles L, L + gridDim, .. (gridDim % 8 == 0) of the grouped_tile order.  Rows
-// and columns past the end are read from the last one and not stored.
-template <typename T, int BM, int BN, int WM, int WN, int S>
+// and columns past the end are read from the last one and not stored.  TAIL: k is no multiple
+// of a k-tile's depth, and what lies past it is read from kZeros.
+template <typename T, int C, int BM, int BN, int WM, int WN, int S, bool TAIL>
 __global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a, bool wide) {
-  using Tile = RingTile<Core8, BM, BN, WM, WN, S>;
+  using Core = Core8<C>;
+  using Tile = RingTile<Core, BM, BN, WM, WN, S>;
+  static_assert(BM + BN <= Tile::kThreads, "a scale a thread");
   extern __shared__ __align__(16) unsigned char lds[];
-  const int wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ __attribute__((aligned(16))) float scale[BM + BN];
+  const int tid = threadIdx.x, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int tm = (a.rows + BM - 1) / BM, tn = (a.n + BN - 1) / BN, tiles = tm * tn;
-  const int nk = (a.k + Core8::kDepth - 1) / Core8::kDepth;
+  const int nk = (a.k + Core::kDepth - 1) / Core::kDepth;
   const int x = blockIdx.x & 7, cnt = (tiles >> 3) + (x < (tiles & 7)), step = gridDim.x >> 3;
   auto origin = [&](int i, int& m0, int& n0) {
     int mt, nt;
@@ -271,41 +304,43 @@ __global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a, bool w
   int t = blockIdx.x >> 3;
   if (t >= cnt) return;
 
-  // the next k-tile to request: tile lt, depth lk; this thread's rows in it and chunks
+  // the next k-tile to request: tile lt, depth lk; byte offsets of this thread's chunks from
+  // the tile's first rows
   int lt = t, lk = 0;
-  const int8_t *ap[Tile::LA], *bp[Tile::LB];
-  int ac[Tile::LA], bc[Tile::LB];
+  const int8_t *ab, *bb;
+  uint32_t ao[Tile::LA], bo[Tile::LB];
   auto point = [&]() {
     int m0, n0;
     origin(lt, m0, n0);
+    ab = a.x + m0 * a.ldx, bb = a.w + n0 * a.ldw;
 #pragma unroll
     for (int q = 0; q < Tile::LA; ++q) {
       int row, chunk;
       Tile::load_pos(q, row, chunk);
-      ap[q] = a.x + (int64_t)min(m0 + row, a.rows - 1) * a.ldx, ac[q] = chunk * 16;
+      ao[q] = (uint32_t)min(row, a.rows - 1 - m0) * (uint32_t)a.ldx + chunk * 16;
     }
 #pragma unroll
     for (int q = 0; q < Tile::LB; ++q) {
       int row, chunk;
       Tile::load_pos(q, row, chunk);
-      bp[q] = a.w + (int64_t)min(n0 + row, a.n - 1) * a.ldw, bc[q] = chunk * 16;
+      bo[q] = (uint32_t)min(row, a.n - 1 - n0) * (uint32_t)a.ldw + chunk * 16;
     }
   };
   point();
-  auto issue = [&](unsigned char* stage) {
-    const int k0 = lk * Core8::kDepth;
-    if (k0 + Core8::kDepth <= a.k) {
+  auto load = [&](unsigned char* stage) {
+    const int8_t *pa = ab + lk * Core::kDepth, *pb = bb + lk * Core::kDepth;
+    auto from = [&](const int8_t* p, uint32_t at, int q) {
+      if constexpr (!TAIL) return static_cast<const void*>(p + at);
+      int row, chunk;
+      Tile::load_pos(q, row, chunk);
+      return lk * Core::kDepth + chunk * 16 < a.k ? static_cast<const void*>(p + at) : static_cast<const void*>(&kZeros);
+    };
 #pragma unroll
-      for (int q = 0; q < Tile::LA; ++q) Tile::load_a(stage, q, ap[q] + k0 + ac[q]);
+    for (int q = 0; q < Tile::LA; ++q) Tile::load_a(stage, q, from(pa, ao[q], q));
 #pragma unroll
-      for (int q = 0; q < Tile::LB; ++q) Tile::load_b(stage, q, bp[q] + k0 + bc[q]);
-    } else {
-      const int8_t* zero = reinterpret_cast<const int8_t*>(&kZeros);
-#pragma unroll
-      for (int q = 0; q < Tile::LA; ++q) Tile::load_a(stage, q, k0 + ac[q] < a.k ? ap[q] + k0 + ac[q] : zero);
-#pragma unroll
-      for (int q = 0; q < Tile::LB; ++q) Tile::load_b(stage, q, k0 + bc[q] < a.k ? bp[q] + k0 + bc[q] : zero);
-    }
+    for (int q = 0; q < Tile::LB; ++q) Tile::load_b(stage, q, from(pb, bo[q], q));
+  };
+  auto advance = [&] {
     if (++lk == nk) {
       if (lt + step < cnt) {
         lt += step;
@@ -318,27 +353,49 @@ __global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a, bool w
   };
 
   typename Tile::State s;
-  Tile::start(lds, s, issue);
+  Tile::start(lds, s, [&](unsigned char* stage) {
+    load(stage);
+    advance();
+  });
+  // store instructions of a whole tile's epilogue, 16 bytes each
+  constexpr int kStores = Tile::MI * Tile::NJ * (sizeof(T) == 2 ? 2 : 4);
+  bool stored = false;  // the previous tile's epilogue issued exactly those after the ring's loads
   for (; t < cnt; t += step) {
     int m0, n0;
     origin(t, m0, n0);
+    float own = 0.f;  // this thread's scale, which lands while the products run
+    if (tid < BM) own = ld_g(a.x_scale + min(m0 + tid, a.rows - 1));
+    else if (tid < BM + BN) own = ld_g(a.w_scale + min(n0 + tid - BM, a.n - 1));
     s.clear();
     Tile::reread(lds, s);  // the first fragments need no registers across the epilogue
-    for (int kt = 0; kt < nk; ++kt) Tile::ktile(lds, s, issue, [&] { Tile::template wait_loads<>(); });
-    store_tile<T, Tile::MI, Tile::NJ>(a, s.acc, m0 + (wid / WN) * (BM / WM), n0 + (wid % WN) * (BN / WN), wide);
+    for (int kt = 0; kt < nk; ++kt) {
+      const bool after = stored && kt == 0;
+      Tile::ktile_mixed(lds, s, load, advance, [&] {
+        if (after) Tile::template wait_loads<kStores>();
+        else Tile::template wait_loads<>();
+      });
+    }
+    if (tid < BM + BN) scale[tid] = own;
+    ring_barrier();
+    const int mt = (wid / WN) * (BM / WM), nt = (wid % WN) * (BN / WN);
+    store_tile<T, BM, Tile::MI, Tile::NJ>(a, s.acc, scale, m0 + mt, n0 + nt, mt, nt, wide);
     asm volatile("" ::: "memory");  // the stores stay ahead of the next tile's waits
+    stored = wide && a.add == nullptr && m0 + BM <= a.rows && n0 + BN <= a.n;
   }
   __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));  // no copy into LDS outlives the block
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int S>
+template <typename T, int C, int BM, int BN, int WM, int WN, int S>
 void launch_tile(const I8Args& a, bool wide, hipStream_t s) {
-  using Tile = RingTile<Core8, BM, BN, WM, WN, S>;
-  const auto kernel = &k_i8_tile<T, BM, BN, WM, WN, S>;
-  allow_dynamic_lds(reinterpret_cast<const void*>(kernel), Tile::kLds);
+  using Tile = RingTile<Core8<C>, BM, BN, WM, WN, S>;
   const int64_t tiles = (int64_t)((a.rows + BM - 1) / BM) * ((a.n + BN - 1) / BN);
   const int64_t grid = std::min<int64_t>(std::max(8, device_cus() & ~7), (tiles + 7) / 8 * 8);
-  hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(Tile::kThreads), Tile::kLds, s, a, wide);
+  auto go = [&](auto kernel) {
+    allow_dynamic_lds(reinterpret_cast<const void*>(kernel), Tile::kLds);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(Tile::kThreads), Tile::kLds, s, a, wide);
+  };
+  if (a.k % Core8<C>::kDepth == 0) go(&k_i8_tile<T, C, BM, BN, WM, WN, S, false>);
+  else go(&k_i8_tile<T, C, BM, BN, WM, WN, S, true>);
 }
 
 template <typename T, int MT>
@@ -353,18 +410,18 @@ void launch_few(const I8Args& a, hipStream_t s) {
 
 void i8_matmul(DType dt, const I8Args& a, hipStream_t s) {
   MRT_DTYPE_DISPATCH(dt, {
-    const size_t unit = 4 * sizeof(T);
-    const bool wide = reinterpret_cast<uintptr_t>(a.out) % unit == 0 && a.ldo % 4 == 0 &&
-                      (a.add == nullptr || (reinterpret_cast<uintptr_t>(a.add) % unit == 0 && a.lda % 4 == 0));
+    const int64_t unit = 16 / (int64_t)sizeof(T);
+    const bool wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo % unit == 0 &&
+                      (a.add == nullptr || (reinterpret_cast<uintptr_t>(a.add) % 16 == 0 && a.lda % unit == 0));
     if (a.rows <= 16) launch_few<T, 1>(a, s);
     else if (a.rows <= 32) launch_few<T, 2>(a, s);
     else if (a.rows <= 64) launch_few<T, 4>(a, s);
     else {
       const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.n + 255) / 256);
       const int64_t mid = (int64_t)((a.rows + 127) / 128) * ((a.n + 127) / 128);
-      if (big >= 192) launch_tile<T, 256, 256, 2, 4, 2>(a, wide, s);
-      else if (mid >= 192) launch_tile<T, 128, 128, 2, 2, 4>(a, wide, s);
-      else launch_tile<T, 64, 64, 2, 2, 6>(a, wide, s);
+      if (big >= 192) launch_tile<T, 8, 256, 256, 2, 4, 2>(a, wide, s);
+      else if (mid >= 192) launch_tile<T, 8, 128, 128, 2, 2, 4>(a, wide, s);
+      else launch_tile<T, 8, 64, 64, 2, 2, 6>(a, wide, s);
     }
   });
   MRT_HIP_CHECK(hipGetLastError());

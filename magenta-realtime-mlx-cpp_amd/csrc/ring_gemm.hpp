@@ -136,6 +136,34 @@ struct RingTile {
     interleave();
   }
 
+  // The same where a k-tile is requested without a branch: load(stage) issues exactly its
+  // loads, which then go between the last products, and advance() turns to the next one.
+  template <class Load, class Advance, class Wait>
+  __device__ static void ktile_mixed(unsigned char* lds, State& s, Load&& load, Advance&& advance, Wait&& wait) {
+    unsigned char* st = lds + s.slot * kStage;
+    s.slot = s.slot + 1 == S ? 0 : s.slot + 1;
+#pragma unroll
+    for (int t = 0; t + 1 < Core::kSteps; ++t) {
+      read(st, t + 1, (t + 1) & 1, s);
+      products(t & 1, s);
+      interleave();
+    }
+    wait();
+    ring_barrier();
+    load(st);
+    read(lds + s.slot * kStage, 0, 0, s);
+    products((Core::kSteps - 1) & 1, s);
+    constexpr int kReads = (MI + NJ) * Core::kParts, kMfma = MI * NJ * Core::kProducts;
+#pragma unroll
+    for (int r = 0; r < kMfma; ++r) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kMfma - 1) / kMfma, 0);
+      __builtin_amdgcn_sched_group_barrier(0x020, (LA + LB + kMfma - 1) / kMfma, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    advance();
+  }
+
   // The first fragments of the next k-tile again.
   __device__ static void reread(unsigned char* lds, State& s) { read(lds + s.slot * kStage, 0, 0, s); }
 
