@@ -3,8 +3,8 @@
 // The sums are whole numbers, exact in 32 bits below k = 2^17 (a term is at most 2^14), so
 // how they are cut and ordered changes no bit of a result.
 //
-// Few rows (k_i8_few): the weights' bytes bound the product.  A block takes 16 NT columns,
-// its eight waves 128-deep pieces of k in turn; weights go from memory to the matrix cores
+// Few rows (k_i8_few): the weights' bytes bound the product.  A block takes 16 columns, its
+// eight waves 128-deep pieces of k in turn; weights go from memory to the matrix cores
 // through registers, four lanes to 64 bytes of a row, and one exchange between lanes brings
 // them into operand order; the waves' sums meet in LDS.
 //
@@ -111,73 +111,63 @@ __device__ __forceinline__ float result(const I8Args& a, int sum, float by_row, 
   return a.add != nullptr ? y + St<T>::ld(static_cast<const T*>(a.add)[row * a.lda + col]) : y;
 }
 
-template <typename T, int MT, int NT>
+template <typename T, int MT>
 __global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a) {
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int i = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+  const int i = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
   const int pieces = (a.k + kPiece - 1) / kPiece;
-  __shared__ i32x4_t sums[kWaves][NT * MT][64];
-  const int8_t* wrow[NT];
-#pragma unroll
-  for (int t = 0; t < NT; ++t) wrow[t] = a.w + (int64_t)min(n0 + t * 16 + (lane >> 2), a.n - 1) * a.ldw;
+  __shared__ i32x4_t sums[kWaves][MT][64];
+  const int8_t* wrow = a.w + (int64_t)min(n0 + (lane >> 2), a.n - 1) * a.ldw;
   const int8_t* xrow[MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xrow[m] = a.x + (int64_t)min(m0 + m * 16 + i, a.rows - 1) * a.ldx;
+  for (int m = 0; m < MT; ++m) xrow[m] = a.x + (int64_t)min(m * 16 + i, a.rows - 1) * a.ldx;
   struct Piece {
-    uint4 w[NT][2], x[MT][2];
+    uint4 w[2], x[MT][2];
   };
   auto load = [&](int p) {
     Piece r;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int kw = p * kPiece + h * 64 + (lane & 3) * 16, kx = p * kPiece + h * 64 + g * 16;
-#pragma unroll
-      for (int t = 0; t < NT; ++t) r.w[t][h] = kw < a.k ? ld_nt16(wrow[t] + kw) : make_uint4(0, 0, 0, 0);
+      r.w[h] = kw < a.k ? ld_nt16(wrow + kw) : make_uint4(0, 0, 0, 0);
 #pragma unroll
       for (int m = 0; m < MT; ++m) r.x[m][h] = kx < a.k ? ld_g16(xrow[m] + kx) : make_uint4(0, 0, 0, 0);
     }
     return r;
   };
-  i32x4_t y[NT][MT];
+  i32x4_t y[MT];
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) y[t][m] = {0, 0, 0, 0};
+  for (int m = 0; m < MT; ++m) y[m] = {0, 0, 0, 0};
   const int pull = (i * 4 + g) * 4;  // the lane with row i's 16 bytes of lane group g
   Piece now = load(wid);
   for (int p = wid; p < pieces; p += kWaves) {
     Piece next = now;
     if (p + kWaves < pieces) next = load(p + kWaves);
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      const uint4 u = now.w[h];
+      const i32x4_t w = {__builtin_amdgcn_ds_bpermute(pull, u.x), __builtin_amdgcn_ds_bpermute(pull, u.y),
+                         __builtin_amdgcn_ds_bpermute(pull, u.z), __builtin_amdgcn_ds_bpermute(pull, u.w)};
 #pragma unroll
-      for (int t = 0; t < NT; ++t) {
-        const uint4 u = now.w[t][h];
-        i32x4_t w = {__builtin_amdgcn_ds_bpermute(pull, u.x), __builtin_amdgcn_ds_bpermute(pull, u.y),
-                     __builtin_amdgcn_ds_bpermute(pull, u.z), __builtin_amdgcn_ds_bpermute(pull, u.w)};
-#pragma unroll
-        for (int m = 0; m < MT; ++m)
-          y[t][m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, __builtin_bit_cast(i32x4_t, now.x[m][h]), y[t][m], 0, 0, 0);
-      }
+      for (int m = 0; m < MT; ++m)
+        y[m] = __builtin_amdgcn_mfma_i32_16x16x64_i8(w, __builtin_bit_cast(i32x4_t, now.x[m][h]), y[m], 0, 0, 0);
+    }
     now = next;
   }
 #pragma unroll
-  for (int t = 0; t < NT; ++t)
-#pragma unroll
-    for (int m = 0; m < MT; ++m) sums[wid][t * MT + m][lane] = y[t][m];
+  for (int m = 0; m < MT; ++m) sums[wid][m][lane] = y[m];
   __syncthreads();
-  for (int z = wid; z < NT * MT; z += kWaves) {
-    const int t = z / MT, m = z - t * MT, row = m0 + m * 16 + i, col = n0 + t * 16 + g * 4;
-    i32x4_t v = sums[0][z][lane];
+  if (wid >= MT) return;
+  const int row = wid * 16 + i, col = n0 + g * 4;
+  i32x4_t v = sums[0][wid][lane];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) v += sums[w][z][lane];
-    if (row >= a.rows) continue;
-    const float by_row = a.x_scale[row];
-    T* dst = static_cast<T*>(a.out) + row * a.ldo + col;
+  for (int w = 1; w < kWaves; ++w) v += sums[w][wid][lane];
+  if (row >= a.rows) return;
+  const float by_row = a.x_scale[row];
+  T* dst = static_cast<T*>(a.out) + row * a.ldo + col;
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-      if (col + r < a.n) dst[r] = St<T>::st(result<T>(a, v[r], by_row, row, col + r));
-  }
+  for (int r = 0; r < 4; ++r)
+    if (col + r < a.n) dst[r] = St<T>::st(result<T>(a, v[r], by_row, row, col + r));
 }
 
 // ---- tiles -----------------------------------------------------------------------------------
@@ -400,10 +390,31 @@ void launch_tile(const I8Args& a, bool wide, hipStream_t s) {
 
 template <typename T, int MT>
 void launch_few(const I8Args& a, hipStream_t s) {
-  const int tiles = (a.n + 15) / 16;
-  const dim3 grid((tiles + 1) / 2, (a.rows + 16 * MT - 1) / (16 * MT));
-  if (tiles < 1024) hipLaunchKernelGGL((k_i8_few<T, MT, 1>), dim3(tiles, grid.y), dim3(64 * kWaves), 0, s, a);
-  else hipLaunchKernelGGL((k_i8_few<T, MT, 2>), grid, dim3(64 * kWaves), 0, s, a);
+  hipLaunchKernelGGL((k_i8_few<T, MT>), dim3((a.n + 15) / 16), dim3(64 * kWaves), 0, s, a);
+}
+
+// Tiles to choose from: us that a k-tile and the rest of a tile take on a full card (from
+// 4096^3 and 2048 x 1024 by 3200).  Measured and chosen (us): 512 x 2816 by 1024 with 256 x 256
+// / 128 x 128 / 64 x 128 / 32 x 64 tiles 32 / 16.6 / 12.0 / 10.0, 2048 x 2816 by 1024 34 / 18.8 /
+// 13.9 / 33, 256 x 4096 by 16384 47 / 25.8 / 31.5 / 82, 4096^3 66.8 / 89 / 117 / 318.
+struct TileCost {
+  int bm, bn;
+  double ktile, rest;
+};
+constexpr TileCost kTiles[] = {{256, 256, 1.75, 4.0}, {128, 256, 1.13, 2.3}, {128, 128, 0.70, 1.9},
+                               {64, 128, 0.45, 1.0},  {32, 128, 0.35, 1.0},  {32, 64, 0.31, 0.8}};
+
+int best_tile(const I8Args& a) {
+  const int64_t nk = (a.k + 127) / 128, cus = std::max(8, device_cus() & ~7);
+  int best = 0;
+  double least = 0.;
+  for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+    const TileCost& t = kTiles[i];
+    const int64_t tiles = (int64_t)((a.rows + t.bm - 1) / t.bm) * ((a.n + t.bn - 1) / t.bn);
+    const double us = (double)((tiles + cus - 1) / cus) * (nk * t.ktile + t.rest);
+    if (i == 0 || us < least) best = i, least = us;
+  }
+  return best;
 }
 
 }  // namespace
@@ -413,15 +424,22 @@ void i8_matmul(DType dt, const I8Args& a, hipStream_t s) {
     const int64_t unit = 16 / (int64_t)sizeof(T);
     const bool wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo % unit == 0 &&
                       (a.add == nullptr || (reinterpret_cast<uintptr_t>(a.add) % 16 == 0 && a.lda % unit == 0));
-    if (a.rows <= 16) launch_few<T, 1>(a, s);
-    else if (a.rows <= 32) launch_few<T, 2>(a, s);
-    else if (a.rows <= 64) launch_few<T, 4>(a, s);
-    else {
-      const int64_t big = (int64_t)((a.rows + 255) / 256) * ((a.n + 255) / 256);
-      const int64_t mid = (int64_t)((a.rows + 127) / 128) * ((a.n + 127) / 128);
-      if (big >= 192) launch_tile<T, 8, 256, 256, 2, 4, 2>(a, wide, s);
-      else if (mid >= 192) launch_tile<T, 8, 128, 128, 2, 2, 4>(a, wide, s);
-      else launch_tile<T, 8, 64, 64, 2, 2, 6>(a, wide, s);
+    // Few columns give too few tiles to keep the card's loads out, many blocks of k_i8_few read
+    // x again (us, k_i8_few / tiles): 2 x 4096 by 4096 7.8 / 12.8, by 16384 19.4 / 14.1; 32 x
+    // 4096 by 4096 9.7 / 13.2, by 8192 16.1 / 13.3.
+    if (a.rows <= 16 && a.n <= 12288) {
+      launch_few<T, 1>(a, s);
+    } else if (a.rows <= 32 && a.n <= 6144) {
+      launch_few<T, 2>(a, s);
+    } else {
+      switch (best_tile(a)) {
+        case 0: launch_tile<T, 8, 256, 256, 2, 4, 2>(a, wide, s); break;
+        case 1: launch_tile<T, 8, 128, 256, 2, 4, 3>(a, wide, s); break;
+        case 2: launch_tile<T, 8, 128, 128, 2, 2, 4>(a, wide, s); break;
+        case 3: launch_tile<T, 8, 64, 128, 2, 2, 4>(a, wide, s); break;
+        case 4: launch_tile<T, 8, 32, 128, 1, 4, 5>(a, wide, s); break;
+        default: launch_tile<T, 8, 32, 64, 1, 2, 8>(a, wide, s);
+      }
     }
   });
   MRT_HIP_CHECK(hipGetLastError());
