@@ -770,8 +770,8 @@ int mrt_q4_quantize(const void* src, int64_t ld, int n, int k, int group, int dt
 
 /* The K/V of one layer for `rows` sequences, in pages of a pool.  k and v:
  * (pages, kv_heads, page_size, d) with element strides page_stride, head_stride
- * and slot_stride (those of both; multiples of 16 bytes) and d contiguous, in
- * `dtype`: MRT_DTYPE_*, d a multiple of 8, or MRT_PAGES_I8, d a multiple of 16;
+ * and slot_stride (those of both; multiples of 16 bytes, slot_stride at most 2^24)
+ * and d contiguous, in `dtype`: MRT_DTYPE_*, d a multiple of 8, or MRT_PAGES_I8, d a multiple of 16;
  * at most 256.  With codes also k_scale and v_scale, (pages, kv_heads, page_size)
  * fp32, 16-byte aligned, not negative.  page_size is a multiple of 16, at most
  * 2^16.  table (rows, row_pages), table_stride elements between sequences: entries
@@ -914,7 +914,7 @@ typedef struct mrt_i8_matmul_args {
 /* out = (x w^T) x_scale w_scale + add: a scale for each row and each column.  The
  * products are summed exactly; the sum is rounded to fp32, scaled and added to in
  * fp32, and rounded to `dtype`.  k is a multiple of 16, below 2^17; ldx and ldw are
- * multiples of 16, x and w 16-byte aligned. */
+ * multiples of 16 below 2^24, x and w 16-byte aligned. */
 int mrt_i8_matmul(const mrt_i8_matmul_args* args, int device, void* hip_stream);
 
 #ifdef __cplusplus

@@ -340,6 +340,7 @@ mrt::PagedCache to_pages(const mrt_paged_cache* c, bool data = true) {
     require(stride_ok(c->page_stride, c->pages, step) && stride_ok(c->head_stride, c->kv_heads, step) &&
                 stride_ok(c->slot_stride, c->page_size, step),
             "pages: strides must be multiples of 16 bytes, not negative");
+    require(c->slot_stride <= (1 << 24), "pages: slot_stride must be at most 2^24");
     require(c->table_stride >= 0, "pages: negative table_stride");
     require(aligned4({c->table, c->length}), "pages: table and length must be 4-byte aligned");
   }
@@ -1387,6 +1388,8 @@ int mrt_i8_matmul(const mrt_i8_matmul_args* args, int device, void* hip_stream) 
     require((args->rows == 1 || (args->ldx >= args->k && args->ldx % 16 == 0)) &&
                 (args->n == 1 || (args->ldw >= args->k && args->ldw % 16 == 0)),
             "i8_matmul: ldx and ldw must be >= k, multiples of 16");
+    require((args->rows == 1 || args->ldx < (1 << 24)) && (args->n == 1 || args->ldw < (1 << 24)),
+            "i8_matmul: ldx and ldw must be below 2^24");
     require(args->rows == 1 || (args->ldo >= args->n && (args->add == nullptr || args->lda >= 0)),
             "i8_matmul: ldo must be >= n, lda not negative");
     require(args->add != args->out || args->rows == 1 || args->lda == args->ldo, "i8_matmul: add in place needs out's row stride");

@@ -1382,6 +1382,27 @@ def q4_quantize(weight, group: int = 64):
 # As the operators above: the caller's tensors, torch's current stream, no gradients.
 
 PAGES_I8 = 3
+_INT32 = 4
+_KIND: Dict = {}  # of the dtypes that these operators take: MRT_DTYPE_*, PAGES_I8, _INT32
+
+
+def _kind(dtype) -> int:
+    if not _KIND:
+        torch = _torch()
+        _KIND.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.int8: PAGES_I8,
+                      torch.int32: _INT32})
+    return _KIND.get(dtype, -1)
+
+
+def _array(t, shape, kind, index, what) -> int:
+    """Pointer of a contiguous int32 or fp32 tensor of this shape on GPU ``index``; None: 0."""
+    if t is None:
+        return 0
+    if t.shape != shape or _kind(t.dtype) != kind or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{what} must be a contiguous {'int32' if kind == _INT32 else 'fp32'} {tuple(shape)} on GPU {index}")
+    return t.data_ptr()
+
+
 _PAGES_STRUCT = struct.Struct("PPPPPPqqqqiiiiiiixxxx")      # mrt_paged_cache
 _STORE_STRUCT = struct.Struct("PqqqPqqqPPPii")              # mrt_paged_store_args
 _PAGED_STRUCT = struct.Struct("PqqqPqqqPPPiiiifxxxx")       # mrt_paged_attention_args
@@ -1400,41 +1421,34 @@ class PagedCache:
     tensors are kept, not copied.
     """
 
-    __slots__ = ("k", "v", "table", "length", "k_scale", "v_scale", "index", "dtype", "codes", "shape", "rows", "row_pages",
-                 "_c")
+    __slots__ = ("k", "v", "table", "length", "k_scale", "v_scale", "index", "kind", "shape", "rows", "row_pages", "_c")
 
     def __init__(self, k, v, table, length, k_scale=None, v_scale=None):
-        torch = _torch()
-        shape, stride, index, self.codes = k.shape, k.stride(), k.get_device(), k.dtype is torch.int8
-        code = PAGES_I8 if self.codes else _dtype_code(k.dtype)
-        if code < 0 or len(shape) != 4 or stride[3] != 1:
+        shape, stride, index, kind = k.shape, k.stride(), k.get_device(), _kind(k.dtype)
+        if not 0 <= kind <= PAGES_I8 or len(shape) != 4 or stride[3] != 1:
             raise ValueError("pages: k must be (pages, kv_heads, page_size, d) fp32, bf16, fp16 or int8, d contiguous")
         if v.shape != shape or v.dtype is not k.dtype or v.stride() != stride or v.get_device() != index:
             raise ValueError("pages: v must have k's shape, dtype, strides and device")
         if index < 0:
             raise ValueError("pages: the tensors must be on a GPU")
-        if table.dim() != 2 or table.dtype is not torch.int32 or table.get_device() != index or table.stride(1) != 1:
+        where = table.shape
+        if len(where) != 2 or _kind(table.dtype) != _INT32 or table.get_device() != index or table.stride(1) != 1:
             raise ValueError("pages: table must be int32 (rows, row_pages) on k's GPU, rows contiguous")
-        rows, row_pages = table.shape
-        lp, ks, vs = _ints(length, (rows,), index, "length"), 0, 0
-        if self.codes:
-            if k_scale is None or v_scale is None:
-                raise ValueError("pages: int8 codes need k_scale and v_scale")
-            ks, vs = _floats(k_scale, shape[:3], index, "k_scale"), _floats(v_scale, shape[:3], index, "v_scale")
-        elif k_scale is not None or v_scale is not None:
+        if (kind == PAGES_I8) != (k_scale is not None and v_scale is not None) or (k_scale is None) != (v_scale is None):
             raise ValueError("pages: k_scale and v_scale go with int8 codes")
         self.k, self.v, self.table, self.length, self.k_scale, self.v_scale = k, v, table, length, k_scale, v_scale
-        self.index, self.dtype, self.shape, self.rows, self.row_pages = index, k.dtype, shape, rows, row_pages
-        self._c = _PAGES_STRUCT.pack(k.data_ptr(), v.data_ptr(), ks, vs, table.data_ptr(), lp, stride[0], stride[1],
-                                     stride[2], table.stride(0), shape[0], rows, row_pages, shape[1], shape[2], shape[3],
-                                     code)
+        self.index, self.kind, self.shape, (self.rows, self.row_pages) = index, kind, shape, where
+        self._c = _PAGES_STRUCT.pack(k.data_ptr(), v.data_ptr(), _array(k_scale, shape[:3], DTYPE_F32, index, "k_scale"),
+                                     _array(v_scale, shape[:3], DTYPE_F32, index, "v_scale"), table.data_ptr(),
+                                     _array(length, where[:1], _INT32, index, "length"), stride[0], stride[1], stride[2],
+                                     table.stride(0), shape[0], where[0], where[1], shape[1], shape[2], shape[3], kind)
 
 
-def _page_rows(t, shape, dtype, cache, what):
-    """Pointer and strides of a 4-d operand of ``dtype``, which goes with the cache's pages."""
+def _page_rows(t, shape, kind, cache, what):
+    """Pointer and strides of a 4-d operand of the dtype ``kind``, which goes with the cache's pages."""
     s = t.stride()
-    if t.shape != shape or t.dtype is not dtype or t.get_device() != cache.index or s[3] != 1 or _dtype_code(dtype) < 0 or (
-            not cache.codes and dtype is not cache.dtype):
+    if t.shape != shape or _kind(t.dtype) != kind or t.get_device() != cache.index or s[3] != 1 or (
+            kind != cache.kind if cache.kind != PAGES_I8 else not 0 <= kind < PAGES_I8):
         raise ValueError(f"{what} must be {tuple(shape)} of the pages' dtype, with int8 pages fp32, bf16 or fp16, on their GPU, "
                          "d contiguous")
     return t.data_ptr(), s[0], s[1], s[2]
@@ -1448,15 +1462,14 @@ def paged_write(cache: PagedCache, k_new, v_new, fresh=None, length_out=None) ->
     where the pages hold codes.  length_out, a tensor of its own, receives the
     new lengths.
     """
-    lib, index = load_library(), cache.index
+    lib, index, rows = load_library(), cache.index, cache.rows
     if k_new.dim() != 4:
         raise ValueError("k_new must be (rows, tokens, kv_heads, d)")
-    tokens, dtype = k_new.shape[1], k_new.dtype
-    shape = (cache.rows, tokens, cache.shape[1], cache.shape[3])
-    args = _STORE_STRUCT.pack(*_page_rows(k_new, shape, dtype, cache, "k_new"), *_page_rows(v_new, shape, dtype, cache, "v_new"),
-                              0 if fresh is None else _ints(fresh, (cache.rows,), index, "fresh"), 0,
-                              0 if length_out is None else _ints(length_out, (cache.rows,), index, "length_out"), tokens,
-                              _dtype_code(dtype))
+    tokens, kind = k_new.shape[1], _kind(k_new.dtype)
+    shape = (rows, tokens, cache.shape[1], cache.shape[3])
+    args = _STORE_STRUCT.pack(*_page_rows(k_new, shape, kind, cache, "k_new"), *_page_rows(v_new, shape, kind, cache, "v_new"),
+                              _array(fresh, (rows,), _INT32, index, "fresh"), 0,
+                              _array(length_out, (rows,), _INT32, index, "length_out"), tokens, kind)
     code = lib.mrt_paged_write(cache._c, args, index, _raw_stream(index))
     if code:
         _check(lib, code)
@@ -1468,14 +1481,14 @@ def paged_read(cache: PagedCache, k_out, v_out, start=None) -> None:
     k_out, v_out (rows, kv_heads, tokens, d), the layout of ``KVCache``; start
     int32 (rows), None: 0.  Entries past a sequence's length are left as they are.
     """
-    lib, index = load_library(), cache.index
+    lib, index, rows = load_library(), cache.index, cache.rows
     if k_out.dim() != 4:
         raise ValueError("k_out must be (rows, kv_heads, tokens, d)")
-    tokens, dtype = k_out.shape[2], k_out.dtype
-    shape = (cache.rows, cache.shape[1], tokens, cache.shape[3])
-    kp, vp = _page_rows(k_out, shape, dtype, cache, "k_out"), _page_rows(v_out, shape, dtype, cache, "v_out")
-    args = _STORE_STRUCT.pack(kp[0], kp[1], kp[3], kp[2], vp[0], vp[1], vp[3], vp[2], 0,
-                              0 if start is None else _ints(start, (cache.rows,), index, "start"), 0, tokens, _dtype_code(dtype))
+    tokens, kind = k_out.shape[2], _kind(k_out.dtype)
+    shape = (rows, cache.shape[1], tokens, cache.shape[3])
+    k, v = _page_rows(k_out, shape, kind, cache, "k_out"), _page_rows(v_out, shape, kind, cache, "v_out")
+    args = _STORE_STRUCT.pack(k[0], k[1], k[3], k[2], v[0], v[1], v[3], v[2], 0, _array(start, (rows,), _INT32, index, "start"), 0,
+                              tokens, kind)
     code = lib.mrt_paged_read(cache._c, args, index, _raw_stream(index))
     if code:
         _check(lib, code)
@@ -1498,25 +1511,21 @@ def paged_attention(q, cache: PagedCache, fresh=None, scale: float = 1.0, bias=N
     (out (rows, tokens, heads, d), lse (rows, tokens, heads) fp32), new tensors
     unless given; tokens past fresh[b] get 0 and -inf.
     """
-    torch, lib, index = _torch(), load_library(), cache.index
-    shape, dtype = q.shape, q.dtype
-    if len(shape) != 4 or shape[0] != cache.rows or shape[3] != cache.shape[3]:
+    lib, index, shape, kind = load_library(), cache.index, q.shape, _kind(q.dtype)
+    pages, kv_heads, page_size, d = cache.shape
+    if len(shape) != 4 or shape[0] != cache.rows or shape[3] != d:
         raise ValueError("q must be (rows, tokens, heads, d) with the cache's rows and d")
-    rows, tokens, heads, d = shape
-    qp = _page_rows(q, shape, dtype, cache, "q")
+    rows, tokens, heads, _ = shape
     if out is None:
-        out = torch.empty(shape, dtype=dtype, device=q.device)
-    op = _page_rows(out, shape, dtype, cache, "out")
+        out = q.new_empty(shape)
     if lse is None:
-        lse = torch.empty((rows, tokens, heads), dtype=torch.float32, device=q.device)
+        lse = q.new_empty(shape[:3], dtype=_torch().float32)
     table, buckets = _bias_table(bias, heads, cache)
-    args = _PAGED_STRUCT.pack(*qp, *op, 0 if fresh is None else _ints(fresh, (rows,), index, "fresh"),
-                              _floats(lse, (rows, tokens, heads), index, "lse"), table, buckets, tokens, heads,
-                              _dtype_code(dtype), scale)
-    pages, kv_heads, page_size, _ = cache.shape
-    size = _paged_workspace(rows, cache.row_pages, pages, kv_heads, page_size, d,
-                            PAGES_I8 if cache.codes else _dtype_code(dtype), heads, tokens)
-    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    args = _PAGED_STRUCT.pack(*_page_rows(q, shape, kind, cache, "q"), *_page_rows(out, shape, kind, cache, "out"),
+                              _array(fresh, shape[:1], _INT32, index, "fresh"), _array(lse, shape[:3], DTYPE_F32, index, "lse"),
+                              table, buckets, tokens, heads, kind, scale)
+    size = _paged_workspace(rows, cache.row_pages, pages, kv_heads, page_size, d, cache.kind, heads, tokens)
+    ws = q.new_empty(size, dtype=_torch().uint8) if size else None
     code = lib.mrt_paged_attention(cache._c, args, ws.data_ptr() if size else None, size, index, _raw_stream(index))
     if code:
         _check(lib, code)
@@ -1541,10 +1550,10 @@ def draft_verify(target, draft, tokens, uniforms, parents=None):
     ``tree_attention``, None: a chain.  Returns int32 (accepted (rows, nodes), as
     ``cache_commit`` takes it, count (rows), token (rows): the one that follows).
     """
-    torch, lib, index = _torch(), load_library(), target.get_device()
-    if target.dim() != 3 or index < 0 or target.shape[1] < 2 or target.stride(2) != 1 or _dtype_code(target.dtype) < 0:
+    lib, index, shape, kind = load_library(), target.get_device(), target.shape, _kind(target.dtype)
+    if len(shape) != 3 or index < 0 or shape[1] < 2 or target.stride(2) != 1 or not 0 <= kind < PAGES_I8:
         raise ValueError("target must be (rows, nodes + 1, vocab) fp32, bf16 or fp16 on a GPU, the vocabulary contiguous")
-    rows, nodes, vocab = target.shape[0], target.shape[1] - 1, target.shape[2]
+    rows, nodes, vocab = shape[0], shape[1] - 1, shape[2]
     dp = d_row = d_slot = 0
     if draft is not None:
         if draft.shape != (rows, nodes, vocab) or draft.dtype is not target.dtype or draft.get_device() != index or (
@@ -1554,31 +1563,31 @@ def draft_verify(target, draft, tokens, uniforms, parents=None):
     tp = pstride = 0
     if parents is not None:
         one = parents.dim() == 1
-        tp, pstride = _ints(parents, (nodes,) if one else (rows, nodes), index, "parents"), 0 if one else nodes
-    got = torch.empty(rows * (nodes + 2), dtype=torch.int32, device=target.device)
+        tp, pstride = _array(parents, (nodes,) if one else (rows, nodes), _INT32, index, "parents"), 0 if one else nodes
+    got = tokens.new_empty(rows * (nodes + 2))
     ap = got.data_ptr()
     args = _VERIFY_STRUCT.pack(target.data_ptr(), dp, target.stride(0), target.stride(1), d_row, d_slot,
-                               _ints(tokens, (rows, nodes), index, "tokens"), tp, pstride,
-                               _floats(uniforms, (rows, nodes + 1), index, "uniforms"), ap, ap + 4 * rows * nodes,
-                               ap + 4 * rows * (nodes + 1), rows, nodes, vocab, _dtype_code(target.dtype))
+                               _array(tokens, (rows, nodes), _INT32, index, "tokens"), tp, pstride,
+                               _array(uniforms, (rows, nodes + 1), DTYPE_F32, index, "uniforms"), ap, ap + 4 * rows * nodes,
+                               ap + 4 * rows * (nodes + 1), rows, nodes, vocab, kind)
     size = _verify_workspace(rows, nodes, vocab, draft is not None, parents is not None)
-    ws = torch.empty(size, dtype=torch.uint8, device=target.device) if size else None
+    ws = target.new_empty(size, dtype=_torch().uint8) if size else None
     code = lib.mrt_draft_verify(args, ws.data_ptr() if size else None, size, index, _raw_stream(index))
     if code:
         _check(lib, code)
-    return got[:rows * nodes].view(rows, nodes), got[rows * nodes:rows * (nodes + 1)], got[rows * (nodes + 1):]
+    accepted, count, token = got.split((rows * nodes, rows, rows))
+    return accepted.view(rows, nodes), count, token
 
 
 def i8_quantize(x):
     """8-bit codes of the rows of x (rows, k), k a multiple of 16 (mrt_i8_quantize): (int8 (rows, k), fp32 scales (rows))."""
-    lib, torch, index = load_library(), _torch(), x.get_device()
-    if x.dim() != 2 or index < 0 or x.stride(1) != 1 or _dtype_code(x.dtype) < 0:
+    lib, torch, index, kind, shape = load_library(), _torch(), x.get_device(), _kind(x.dtype), x.shape
+    if len(shape) != 2 or index < 0 or x.stride(1) != 1 or not 0 <= kind < PAGES_I8:
         raise ValueError("x must be (rows, k) fp32, bf16 or fp16 on a GPU, rows contiguous")
-    rows, k = x.shape
-    codes = torch.empty((rows, k), dtype=torch.int8, device=x.device)
-    scales = torch.empty(rows, dtype=torch.float32, device=x.device)
-    code = lib.mrt_i8_quantize(x.data_ptr(), x.stride(0), rows, k, _dtype_code(x.dtype), codes.data_ptr(), k,
-                               scales.data_ptr(), index, _raw_stream(index))
+    rows, k = shape
+    codes, scales = x.new_empty(shape, dtype=torch.int8), x.new_empty(rows, dtype=torch.float32)
+    code = lib.mrt_i8_quantize(x.data_ptr(), x.stride(0), rows, k, kind, codes.data_ptr(), k, scales.data_ptr(), index,
+                               _raw_stream(index))
     if code:
         _check(lib, code)
     return codes, scales
@@ -1591,23 +1600,26 @@ def i8_matmul(x, x_scale, w, w_scale, dtype=None, add=None, out=None):
     ``i8_quantize`` makes them: out = (x w^T) x_scale w_scale + add, add (rows,
     n) or None, which may be out.  dtype: that of out or add where given, else bf16.
     """
-    lib, torch, index = load_library(), _torch(), x.get_device()
-    if x.dim() != 2 or w.dim() != 2 or x.shape[1] != w.shape[1] or x.dtype is not torch.int8 or w.dtype is not torch.int8:
+    lib, index, shape, (n, k) = load_library(), x.get_device(), x.shape, w.shape
+    if len(shape) != 2 or shape[1] != k or _kind(x.dtype) != PAGES_I8 or _kind(w.dtype) != PAGES_I8:
         raise ValueError("x and w must be int8 (rows, k) and (n, k)")
-    (rows, k), n = x.shape, w.shape[0]
     if index < 0 or w.get_device() != index or x.stride(1) != 1 or w.stride(1) != 1:
         raise ValueError("x and w must be on one GPU, rows contiguous")
     if dtype is None:
-        dtype = out.dtype if out is not None else add.dtype if add is not None else torch.bfloat16
+        dtype = out.dtype if out is not None else add.dtype if add is not None else _torch().bfloat16
+    kind, rows = _kind(dtype), shape[0]
     if out is None:
-        out = torch.empty((rows, n), dtype=dtype, device=x.device)
-    for t, what in ((out, "out"), (add, "add")):
-        if t is not None and (t.shape != (rows, n) or t.dtype is not dtype or t.get_device() != index or t.stride(1) != 1):
-            raise ValueError(f"{what} must be (rows, n) in dtype, on x's GPU, rows contiguous")
-    args = _I8_STRUCT.pack(x.data_ptr(), _floats(x_scale, (rows,), index, "x_scale"), w.data_ptr(),
-                           _floats(w_scale, (n,), index, "w_scale"), 0 if add is None else add.data_ptr(), out.data_ptr(),
-                           x.stride(0), w.stride(0), 0 if add is None else add.stride(0), out.stride(0), rows, n, k,
-                           _dtype_code(dtype))
+        out = x.new_empty((rows, n), dtype=dtype)
+    elif out.shape != (rows, n) or out.dtype is not dtype or out.get_device() != index or out.stride(1) != 1:
+        raise ValueError("out must be (rows, n) in dtype, on x's GPU, rows contiguous")
+    ap = lda = 0
+    if add is not None:
+        if add.shape != (rows, n) or add.dtype is not dtype or add.get_device() != index or add.stride(1) != 1:
+            raise ValueError("add must be (rows, n) in dtype, on x's GPU, rows contiguous")
+        ap, lda = add.data_ptr(), add.stride(0)
+    args = _I8_STRUCT.pack(x.data_ptr(), _array(x_scale, shape[:1], DTYPE_F32, index, "x_scale"), w.data_ptr(),
+                           _array(w_scale, (n,), DTYPE_F32, index, "w_scale"), ap, out.data_ptr(), x.stride(0), w.stride(0), lda,
+                           out.stride(0), rows, n, k, kind)
     code = lib.mrt_i8_matmul(args, index, _raw_stream(index))
     if code:
         _check(lib, code)

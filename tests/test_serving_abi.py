@@ -38,7 +38,7 @@ BAD_PAGES = {
     "large page size": dict(size=(1 << 16) + 16), "odd d": dict(d=60), "wide d": dict(d=264), "no d": dict(d=0),
     "dtype": dict(dtype=4), "stride": dict(ss=68), "negative stride": dict(hs=-1024), "table stride": dict(ts=-1),
     "too long": dict(rp=1 << 20, size=1 << 11), "too many heads": dict(rows=1 << 12, kv=1 << 9),
-    "codes without scales": dict(dtype=3), "codes with one scale": dict(dtype=3, ks=P), "misaligned scales": dict(I8, ks=P + 4),
+    "wide slots": dict(ss=(1 << 24) + 64), "codes without scales": dict(dtype=3), "codes with one scale": dict(dtype=3, ks=P), "misaligned scales": dict(I8, ks=P + 4),
     "d of codes": dict(I8, d=72), "stride of codes": dict(I8, ss=72),
 }
 
@@ -97,6 +97,7 @@ BAD_PRODUCTS = {
     "large n": dict(n=(1 << 26) + 1), "odd k": dict(k=24), "no k": dict(k=0), "large k": dict(k=1 << 17, ld=(1 << 17, 1 << 17, 32, 32)),
     "short ldx": dict(ld=(48, 64, 32, 32)), "odd ldx": dict(ld=(72, 64, 32, 32)), "short ldw": dict(ld=(64, 48, 32, 32)),
     "odd ldw": dict(ld=(64, 72, 32, 32)), "short ldo": dict(ld=(64, 64, 32, 31)), "negative lda": dict(add=P, ld=(64, 64, -32, 32)),
+    "long ldx": dict(ld=(1 << 24, 64, 32, 32)), "long ldw": dict(ld=(64, 1 << 24, 32, 32)),
     "in place with another stride": dict(add=V, ld=(64, 64, 0, 32)), "dtype": dict(dtype=3),
     "too many tiles": dict(rows=1 << 24, n=1 << 26, ld=(64, 64, 1 << 26, 1 << 26)),
 }
