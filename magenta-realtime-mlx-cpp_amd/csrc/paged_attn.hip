@@ -173,8 +173,8 @@ struct Walk {
       w.b = b, w.kvh = kvh, w.steps = steps, w.open = false;
       w.s0 = (int)max((int64_t)0, from - first), w.s1 = (int)min((int64_t)steps, to - first);
       w.slot = (int64_t)b * a.kv_heads + kvh + team;
-      w.all = w.s0 == 0 && w.s1 == steps;
       // a unit without steps, whose outputs are zeros, falls to the share with its beginning
+      w.all = steps == 0 || (w.s0 == 0 && w.s1 == steps);
       const bool mine = steps == 0 ? at >= from : w.s0 < w.s1;
       at = first + steps;
       if (++kvh == a.kv_heads) {

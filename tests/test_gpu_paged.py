@@ -88,6 +88,12 @@ def call(c, s, **kw):
     return out.cpu(), lse.cpu()
 
 
+def workspace(c, s):
+    """Bytes; none where a block takes whole sequences' heads."""
+    n, kv, page, d = c["k"].shape
+    return mrt_df._paged_workspace(*c["table"].shape, n, kv, page, d, mrt_df._kind(c["k"].dtype), s["q"].shape[2], s["q"].shape[1])
+
+
 def size_of(c, x, norm):
     """The largest norm of an entry's finite values."""
     v = c[x].double()
@@ -411,3 +417,48 @@ def test_write_from_wider_rows(store):
     wide[..., 256:384], wide[..., 384:] = new[0].flatten(2), new[1].flatten(2)
     g = wide.to(DEV)
     check_write(c, new, None, g[..., 256:384].unflatten(-1, (2, 64)), g[..., 384:].unflatten(-1, (2, 64)))
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("rows", [30, 150])
+def test_sequences_without_new_tokens_among_long_ones(rows, store):
+    """Wherever a share of the keys ends among them, their outputs are zeros."""
+    lengths = [(4000 if b % 37 == 0 else 60 * (b % 5)) for b in range(rows)]
+    fresh = [1 if b % 37 == 0 or b % 11 == 0 else 0 for b in range(rows)]
+    c, s = make(17, store, rows, 2, 1, 64, 1, lengths, fresh=fresh)
+    assert workspace(c, s) > 0  # shared out by length
+    g, h = on_gpu(c), on_gpu(s)
+    out = torch.full(s["q"].shape, 9.0, dtype=s["q"].dtype, device=DEV)
+    lse = torch.full(s["q"].shape[:3], 9.0, device=DEV)
+    mrt_df.paged_attention(h["q"], pages(g), fresh=h["fresh"], scale=s["scale"], out=out, lse=lse)
+    torch.cuda.synchronize()
+    check(c, s, store, (out.cpu(), lse.cpu()))
+
+
+SHARED = [
+    # rows heads kv d tokens lengths page                           shares end
+    (70, 2, 1, 64, 1, [(37 * b * b) % 2900 for b in range(70)], 16),  # inside and between more sequences than lanes
+    (3, 4, 2, 64, 2, [2700, 1, 900], 32),                           # across a sequence that is one step
+    (2, 8, 1, 64, 9, [3000, 1700], 16),                             # for several row blocks alike
+    (1, 14, 2, 128, 11, [5500], 64),
+    (2, 2, 1, 256, 33, [2900, 2700], 128),
+    (3, 2, 2, 32, 5, [5000, 17, 1300], 16),
+]
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("case", SHARED, ids=[f"r{c[0]}h{c[1]}kv{c[2]}d{c[3]}t{c[4]}" for c in SHARED])
+def test_keys_shared_out(case, store):
+    c, s = make(18, store, *case)
+    assert workspace(c, s) > 0
+    check(c, s, store, call(c, s))
+
+
+@pytest.mark.parametrize("store", STORES)
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_several_heads_a_block(tokens, store):
+    """More sequences and heads than blocks: a block takes them in turn, the bias of each."""
+    fresh = [b % (tokens + 1) for b in range(160)]
+    c, s = make(19, store, 160, 8, 8, 64, tokens, [(7 * b) % 40 for b in range(160)], buckets=20, fresh=fresh)
+    assert workspace(c, s) == 0
+    check(c, s, store, call(c, s))
