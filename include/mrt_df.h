@@ -826,7 +826,7 @@ typedef struct mrt_paged_attention_args {
   const int32_t* fresh;  /* (rows) new tokens that are there; NULL: all */
   float* lse;            /* (rows, tokens, heads) fp32 log-sum-exp of the logits, or NULL */
   const float* bias;     /* (heads, buckets) fp32 logit bias by distance, or NULL */
-  int32_t buckets;       /* with bias: 1 .. 2^18 */
+  int32_t buckets;       /* with bias: 1 .. 2^18, heads * buckets below 2^31 */
   int32_t tokens;        /* 1 .. MRT_MAX_NODES */
   int32_t heads;         /* a multiple of kv_heads */
   int32_t dtype;         /* of q and out: the pages' own, any of the three for codes */
@@ -913,7 +913,7 @@ typedef struct mrt_i8_matmul_args {
 
 /* out = (x w^T) x_scale w_scale + add: a scale for each row and each column.  The
  * products are summed exactly; the sum is rounded to fp32, scaled and added to in
- * fp32, and rounded to `dtype`.  k is a multiple of 16, below 2^17; ldx and ldw are
+ * fp32, and rounded to `dtype`.  rows is below 2^24, k a multiple of 16, below 2^17; ldx and ldw are
  * multiples of 16 below 2^24, x and w 16-byte aligned. */
 int mrt_i8_matmul(const mrt_i8_matmul_args* args, int device, void* hip_stream);
 

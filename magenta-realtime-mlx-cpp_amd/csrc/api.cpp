@@ -383,7 +383,7 @@ void check_apart(const Vectors& x, const Vectors& y, const void* px, const void*
 constexpr char kPagedTooLarge[] = "paged_attention: too many sequences, heads and tokens for one call";
 
 void check_i8(int rows, int k) {
-  require(rows >= 0 && rows <= (1 << 24), "8-bit products: rows must be in 0..2^24");
+  require(rows >= 0 && rows < (1 << 24), "8-bit products: rows must be in 0..2^24 - 1");
   require(k >= 16 && k % 16 == 0 && k < (1 << 17), "8-bit products: k must be a multiple of 16, below 2^17");
 }
 
@@ -1310,6 +1310,8 @@ int mrt_paged_attention(const mrt_paged_cache* cache, const mrt_paged_attention_
     if (c.rows == 0) return;
     check_heads(c.rows, c.kv_heads, args->heads, args->tokens);
     check_bias(args->bias, args->buckets);
+    require(args->bias == nullptr || static_cast<int64_t>(args->heads) * args->buckets < (1ll << 31),
+            "paged_attention: heads * buckets must be below 2^31");
     mrt::PagedAttnArgs a;
     a.dt = operand_type(c, args->dtype);
     a.q = to_nodes(args->q, a.dt, c.rows, args->tokens, args->heads, "paged_attention: null q");
@@ -1378,7 +1380,7 @@ int mrt_i8_matmul(const mrt_i8_matmul_args* args, int device, void* hip_stream) 
     const mrt::DType dt = to_dtype(args->dtype);
     check_i8(args->rows, args->k);
     require(args->n >= 1 && args->n <= (1 << 26), "i8_matmul: n must be in 1..2^26");
-    require((static_cast<int64_t>(args->rows) / 64 + 1) * (args->n / 64 + 1) < (1ll << 31), "i8_matmul: too many rows and columns");
+    require((static_cast<int64_t>(args->rows) / 32 + 1) * (args->n / 64 + 1) < (1ll << 31), "i8_matmul: too many rows and columns");
     if (args->rows == 0) return;
     require(args->x && args->x_scale && args->w && args->w_scale && args->out, "i8_matmul: null argument");
     require(aligned(args->x, 16) && aligned(args->w, 16), "i8_matmul: x and w must be 16-byte aligned");

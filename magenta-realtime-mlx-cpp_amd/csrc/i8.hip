@@ -172,16 +172,15 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a) {
 
 // ---- tiles -----------------------------------------------------------------------------------
 
-// 8-bit operands in the ring: a k-tile is 16 C deep (C 4 or 8), a row of it C chunks of 16
-// bytes.  Chunk c of row r is stored at chunk c ^ swz(r), so that 16 consecutive lanes of a
-// fragment read (16 rows, one chunk) fall in distinct banks.
-template <int C>
+// 8-bit operands in the ring: a k-tile is 128 deep, a row of it 8 chunks of 16 bytes.  Chunk c
+// of row r is stored at chunk c ^ swz(r), so that 16 consecutive lanes of a fragment read (16
+// rows, one chunk) fall in distinct banks.
 struct Core8 {
   typedef i32x4_t v8;
   typedef i32x16_t Acc;
-  static constexpr int kChunks = C, kSteps = C / 2, kParts = 1, kDepth = 16 * C, kProducts = 1;
+  static constexpr int kChunks = 8, kSteps = 4, kParts = 1, kDepth = 128, kProducts = 1;
   static constexpr bool kFine = false;
-  __device__ static int swz(int r) { return C == 8 ? (r ^ (r >> 3)) & 7 : (r >> 2) & 3; }
+  __device__ static int swz(int r) { return (r ^ (r >> 3)) & 7; }
   __device__ static int place(int r, int chunk) { return chunk ^ swz(r); }
   __device__ static int chunk_at(int r, int pos) { return pos ^ swz(r); }
   __device__ static int chunk(int step, int, int half) { return 2 * step + half; }
@@ -274,9 +273,9 @@ __device__ __forceinline__ void store_tile(const I8Args& a, const i32x16_t (&acc
 // Block L takes tiles L, L + gridDim, .. (gridDim % 8 == 0) of the grouped_tile order.  Rows
 // and columns past the end are read from the last one and not stored.  TAIL: k is no multiple
 // of a k-tile's depth, and what lies past it is read from kZeros.
-template <typename T, int C, int BM, int BN, int WM, int WN, int S, bool TAIL>
+template <typename T, int BM, int BN, int WM, int WN, int S, bool TAIL>
 __global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a, bool wide) {
-  using Core = Core8<C>;
+  using Core = Core8;
   using Tile = RingTile<Core, BM, BN, WM, WN, S>;
   static_assert(BM + BN <= Tile::kThreads, "a scale a thread");
   extern __shared__ __align__(16) unsigned char lds[];
@@ -375,17 +374,17 @@ __global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a, bool w
   __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));  // no copy into LDS outlives the block
 }
 
-template <typename T, int C, int BM, int BN, int WM, int WN, int S>
+template <typename T, int BM, int BN, int WM, int WN, int S>
 void launch_tile(const I8Args& a, bool wide, hipStream_t s) {
-  using Tile = RingTile<Core8<C>, BM, BN, WM, WN, S>;
+  using Tile = RingTile<Core8, BM, BN, WM, WN, S>;
   const int64_t tiles = (int64_t)((a.rows + BM - 1) / BM) * ((a.n + BN - 1) / BN);
   const int64_t grid = std::min<int64_t>(std::max(8, device_cus() & ~7), (tiles + 7) / 8 * 8);
   auto go = [&](auto kernel) {
     allow_dynamic_lds(reinterpret_cast<const void*>(kernel), Tile::kLds);
     hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(Tile::kThreads), Tile::kLds, s, a, wide);
   };
-  if (a.k % Core8<C>::kDepth == 0) go(&k_i8_tile<T, C, BM, BN, WM, WN, S, false>);
-  else go(&k_i8_tile<T, C, BM, BN, WM, WN, S, true>);
+  if (a.k % Core8::kDepth == 0) go(&k_i8_tile<T, BM, BN, WM, WN, S, false>);
+  else go(&k_i8_tile<T, BM, BN, WM, WN, S, true>);
 }
 
 template <typename T, int MT>
@@ -433,12 +432,12 @@ void i8_matmul(DType dt, const I8Args& a, hipStream_t s) {
       launch_few<T, 2>(a, s);
     } else {
       switch (best_tile(a)) {
-        case 0: launch_tile<T, 8, 256, 256, 2, 4, 2>(a, wide, s); break;
-        case 1: launch_tile<T, 8, 128, 256, 2, 4, 3>(a, wide, s); break;
-        case 2: launch_tile<T, 8, 128, 128, 2, 2, 4>(a, wide, s); break;
-        case 3: launch_tile<T, 8, 64, 128, 2, 2, 4>(a, wide, s); break;
-        case 4: launch_tile<T, 8, 32, 128, 1, 4, 5>(a, wide, s); break;
-        default: launch_tile<T, 8, 32, 64, 1, 2, 8>(a, wide, s);
+        case 0: launch_tile<T, 256, 256, 2, 4, 2>(a, wide, s); break;
+        case 1: launch_tile<T, 128, 256, 2, 4, 3>(a, wide, s); break;
+        case 2: launch_tile<T, 128, 128, 2, 2, 4>(a, wide, s); break;
+        case 3: launch_tile<T, 64, 128, 2, 2, 4>(a, wide, s); break;
+        case 4: launch_tile<T, 32, 128, 1, 4, 5>(a, wide, s); break;
+        default: launch_tile<T, 32, 64, 1, 2, 8>(a, wide, s);
       }
     }
   });

@@ -51,8 +51,8 @@ constexpr int blocks_of_cu(size_t elt, int dp, int nr) {
   return elt == 1 ? (dp == 256 ? 1 : 2) : elt == 4 ? (dp == 32 ? 4 : dp == 64 ? 2 : 1)
                                                    : dp == 32 ? 4 / nr : dp == 64 ? (nr == 1 ? 3 : 2) : 1;
 }
-#define MRT_ATTN_BOUNDS(elt) \
-  __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(blocks_of_cu(elt, DP, NR) * W / 4)))
+#define MRT_ATTN_BOUNDS(elt, nr) \
+  __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(blocks_of_cu(elt, DP, nr) * W / 4)))
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
 struct PageArgs {
@@ -129,7 +129,8 @@ template <int KEYS>
 struct Walk {
   int64_t at, from, to;  // cut: where the next unit begins, the share
   int team, b, kvh, steps;
-  __device__ __forceinline__ Walk(const PageArgs& a, int lane, int team_) : at(0), from(0), to(0), team(team_), b(0), kvh(0), steps(0) {
+  __device__ __forceinline__ Walk(const PageArgs& a, int lane, int team_)
+      : at(0), from(0), to(0), team(team_), b(0), kvh(0), steps(0) {
     if (a.unit == 0) {
       b = team / a.kv_heads, kvh = team - b * a.kv_heads;
       return;
@@ -450,8 +451,8 @@ struct BiasTable {
 // sums.  In two halves, so that the buffer holds half of the waves' outputs.  No barrier
 // waits for loads: those of the next part are on their way.
 template <typename T, int W, int NR, int E>
-__device__ __forceinline__ void join_waves(const PageArgs& a, const Part& w, int row0, int there_rows, char* lds, float2 (*ml)[16 * NR],
-                                           const float (&m)[NR], float (&l)[NR], f32x4_t (&o)[NR][E]) {
+__device__ __forceinline__ void join_waves(const PageArgs& a, const Part& w, int row0, int there_rows, char* lds,
+                                           float2 (*ml)[16 * NR], const float (&m)[NR], float (&l)[NR], f32x4_t (&o)[NR][E]) {
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15, g = lane >> 4;
   constexpr int H = W / 2;
   f32x4_t* buf = reinterpret_cast<f32x4_t*>(lds);
@@ -503,7 +504,7 @@ __device__ __forceinline__ void join_waves(const PageArgs& a, const Part& w, int
 }
 
 template <typename T, int DP, int NR, int W>
-__global__ MRT_ATTN_BOUNDS(sizeof(T)) void k_paged(const PageArgs a) {
+__global__ MRT_ATTN_BOUNDS(sizeof(T), NR) void k_paged(const PageArgs a) {
   using F = AttnFrag<T, DP>;
   constexpr int E = F::E, VW = F::VW, KC = F::KC, KEYS = 32;
   using Lookup = TileLookup<2>;
@@ -558,158 +559,158 @@ __global__ MRT_ATTN_BOUNDS(sizeof(T)) void k_paged(const PageArgs a) {
   request();
 
   for (;;) {
-  const int b = w.b, kvh = w.kvh;
-  const int len = length_of(a, b), fresh = fresh_of(a, b), end = min(len + fresh, capacity_of(a));
-  if (w.open) w.s1 = w.steps = steps_of<KEYS>(a, b);
+    const int b = w.b, kvh = w.kvh;
+    const int len = length_of(a, b), fresh = fresh_of(a, b), end = min(len + fresh, capacity_of(a));
+    if (w.open) w.s1 = w.steps = steps_of<KEYS>(a, b);
 
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ float2 ml[W][16 * NR];
-  float* btab = reinterpret_cast<float*>(lds);  // the bias of this K/V head's heads, until the waves join
-  const BiasTable table_of(a, btab, kvh, n);
-  uint4 q[NR][KC];
-  int last[NR], head[NR];  // the newest entry that the row sees, -1: the row is not there; its query head of the K/V head's
-#pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
-    F::load_row(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D, q[t]);
-    last[t] = node < fresh ? len + node : -1, head[t] = hq;
-  }
-  if (a.bias != nullptr && table_of.fill(btab, n, 64 * W)) ring_barrier();  // does not wait for the loads of the first step
-
-  f32x4_t o[NR][E];
-  float m[NR], l[NR];
-  auto begin = [&] {
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float2 ml[W][16 * NR];
+    float* btab = reinterpret_cast<float*>(lds);  // the bias of this K/V head's heads, until the waves join
+    const BiasTable table_of(a, btab, kvh, n);
+    uint4 q[NR][KC];
+    int last[NR], head[NR];  // the newest entry that the row sees, -1: the row is not there; its query head of the K/V head's
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
-      m[t] = kNone, l[t] = 0.f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
+      const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
+      F::load_row(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D, q[t]);
+      last[t] = node < fresh ? len + node : -1, head[t] = hq;
     }
-  };
-  begin();
-  const float scale2 = a.scale * kLog2e;
-  // fp16 weights reach up to 2^15, so that those far below the maximum keep their bits.
-  constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;
+    if (a.bias != nullptr && table_of.fill(btab, n, 64 * W)) ring_barrier();  // does not wait for the loads of the first step
 
-  // One step; next() requests the keys of the wave's next one.  A matrix product makes NaN
-  // of 0 * inf: infinities and NaN in values that some rows do not see (the new tokens', and
-  // with `exact` all) are left out of it and added by class.
-  auto step = [&](int st, auto exact, auto&& next) {
-    const int base = st * KEYS;
-    const bool in[2] = {page[0] >= 0, page[1] >= 0};
-    const bool whole = base + KEYS <= len + 1 && fresh > 0 && in[0] && in[1];
-    const bool apart = exact.value || (fresh > 1 && base + KEYS > len + 1);
-    const int page_v[2] = {page[0], page[1]}, place_v[2] = {place[0], place[1]};
-    if (!whole) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-#pragma unroll
-        for (int x = 0; x < VW; ++x) vf[j][x] = in[j >> 2] && base + lane_key(g, j) < end ? vf[j][x] : 0u;
-    }
-    float p[NR][8];
-#pragma unroll
-    for (int t = 0; t < NR; ++t) {
-      const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
-      const float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
-      if (a.bias != nullptr) {
-        table_of.template each<8>(head[t], last[t] - base - 4 * g, [](int j) { return lane_key(0, j); }, [&](int j, float by) {
-          p[t][j] = by < kNone ? -INFINITY : fmaf(s[j], scale2, by);  // a masked key may hold anything
-        });
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[t][j] = s[j] * scale2;
-      }
-      if (!whole) {
-        const int most[2] = {in[0] ? last[t] - base - 4 * g : -1, in[1] ? last[t] - base - 4 * g : -1};
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[t][j] = lane_key(0, j) <= most[j >> 2] ? p[t][j] : -INFINITY;
-      }
-    }
-    next();
-    uint32_t seen[NR];  // the keys that the row does not mask, a bit each
-    if (apart) {
+    f32x4_t o[NR][E];
+    float m[NR], l[NR];
+    auto begin = [&] {
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
-        seen[t] = 0;
+        m[t] = kNone, l[t] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) seen[t] |= p[t][j] < kNone ? 0u : 1u << j;
+        for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
       }
-    }
-    running_softmax<NR, E>(p, m, l, o, kShift);
-    if (!apart) {
-      F::template add_pv<NR>(vf, p, o);
-    } else {
-      uint32_t diff = 0;
+    };
+    begin();
+    const float scale2 = a.scale * kLog2e;
+    // fp16 weights reach up to 2^15, so that those far below the maximum keep their bits.
+    constexpr float kShift = std::is_same_v<T, f16> ? 15.f : 0.f;
+
+    // One step; next() requests the keys of the wave's next one.  A matrix product makes NaN
+    // of 0 * inf: infinities and NaN in values that some rows do not see (the new tokens', and
+    // with `exact` all) are left out of it and added by class.
+    auto step = [&](int st, auto exact, auto&& next) {
+      const int base = st * KEYS;
+      const bool in[2] = {page[0] >= 0, page[1] >= 0};
+      const bool whole = base + KEYS <= len + 1 && fresh > 0 && in[0] && in[1];
+      const bool apart = exact.value || (fresh > 1 && base + KEYS > len + 1);
+      const int page_v[2] = {page[0], page[1]}, place_v[2] = {place[0], place[1]};
+      if (!whole) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-        for (int x = 0; x < VW; ++x) {
-          const uint32_t y = F::finite_part(vf[j][x]);
-          diff |= y ^ vf[j][x];
-          vf[j][x] = y;
+          for (int x = 0; x < VW; ++x) vf[j][x] = in[j >> 2] && base + lane_key(g, j) < end ? vf[j][x] : 0u;
+      }
+      float p[NR][8];
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        const f32x4_t x = F::scores(kf[0], q[t]), y = F::scores(kf[1], q[t]);
+        const float s[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+        if (a.bias != nullptr) {
+          table_of.template each<8>(head[t], last[t] - base - 4 * g, [](int j) { return lane_key(0, j); }, [&](int j, float by) {
+            p[t][j] = by < kNone ? -INFINITY : fmaf(s[j], scale2, by);  // a masked key may hold anything
+          });
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) p[t][j] = s[j] * scale2;
         }
-      F::template add_pv<NR>(vf, p, o);
-      if (__builtin_expect(__any(diff != 0), 0)) {
+        if (!whole) {
+          const int most[2] = {in[0] ? last[t] - base - 4 * g : -1, in[1] ? last[t] - base - 4 * g : -1};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int h = j >> 2;
-          const bool have = page_v[h] >= 0 && base + lane_key(g, j) < end;
-          if (page_v[h] >= 0)
-            F::load_v(vc + page_v[h] * a.page_stride + (int64_t)(place_v[h] + 4 * g + (j & 3)) * a.slot_stride, i, D, vf[j]);
-#pragma unroll
-          for (int x = 0; x < VW; ++x) vf[j][x] = have ? F::classes(vf[j][x]) : 0u;
+          for (int j = 0; j < 8; ++j) p[t][j] = lane_key(0, j) <= most[j >> 2] ? p[t][j] : -INFINITY;
         }
+      }
+      next();
+      uint32_t seen[NR];  // the keys that the row does not mask, a bit each
+      if (apart) {
 #pragma unroll
         for (int t = 0; t < NR; ++t) {
-          float one[8];
+          seen[t] = 0;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) one[j] = (seen[t] >> j) & 1 ? 1.f : 0.f;
+          for (int j = 0; j < 8; ++j) seen[t] |= p[t][j] < kNone ? 0u : 1u << j;
+        }
+      }
+      running_softmax<NR, E>(p, m, l, o, kShift);
+      if (!apart) {
+        F::template add_pv<NR>(vf, p, o);
+      } else {
+        uint32_t diff = 0;
 #pragma unroll
-          for (int e = 0; e < E; ++e) {
-            const f32x4_t c = F::count(vf, one, e);
+        for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(c[r]);
+          for (int x = 0; x < VW; ++x) {
+            const uint32_t y = F::finite_part(vf[j][x]);
+            diff |= y ^ vf[j][x];
+            vf[j][x] = y;
+          }
+        F::template add_pv<NR>(vf, p, o);
+        if (__builtin_expect(__any(diff != 0), 0)) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int h = j >> 2;
+            const bool have = page_v[h] >= 0 && base + lane_key(g, j) < end;
+            if (page_v[h] >= 0)
+              F::load_v(vc + page_v[h] * a.page_stride + (int64_t)(place_v[h] + 4 * g + (j & 3)) * a.slot_stride, i, D, vf[j]);
+#pragma unroll
+            for (int x = 0; x < VW; ++x) vf[j][x] = have ? F::classes(vf[j][x]) : 0u;
+          }
+#pragma unroll
+          for (int t = 0; t < NR; ++t) {
+            float one[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) one[j] = (seen[t] >> j) & 1 ? 1.f : 0.f;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const f32x4_t c = F::count(vf, one, e);
+#pragma unroll
+              for (int r = 0; r < 4; ++r) o[t][e][r] += F::class_value(c[r]);
+            }
           }
         }
       }
-    }
-  };
-  auto steps = [&](auto exact) {
-    for (int st = w.s0 + wid; st < w.s1; st += W) {
-      const bool more = st + W < w.s1;
-      step(st, exact, [&] {
-        if (!more) return;
-        if (st + W - looked >= Lookup::kSteps * W) {
-          looked = st + W;
-          look.fetch(a, table, looked, W, lane);
-        }
-        find(st + W);
-        load_k();
-      });
-      if (more) load_v();
-    }
-  };
-  steps(std::false_type{});
-  bool odd = false;
+    };
+    auto steps = [&](auto exact) {
+      for (int st = w.s0 + wid; st < w.s1; st += W) {
+        const bool more = st + W < w.s1;
+        step(st, exact, [&] {
+          if (!more) return;
+          if (st + W - looked >= Lookup::kSteps * W) {
+            looked = st + W;
+            look.fetch(a, table, looked, W, lane);
+          }
+          find(st + W);
+          load_k();
+        });
+        if (more) load_v();
+      }
+    };
+    steps(std::false_type{});
+    bool odd = false;
 #pragma unroll
-  for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]) && last[t] >= 0;
-  if (__builtin_expect(__any(odd), 0)) {  // rare: this wave's steps once more
-    begin();
-    request();
-    steps(std::true_type{});
-  }
-  const Part done = w;
-  const bool more = walk.next(a, w);
-  if (more) request();
-  join_waves<T, W, NR, E>(a, done, row0, fresh * n, lds, ml, m, l, o);
-  if (!more) break;
+    for (int t = 0; t < NR; ++t) odd |= !all_finite<E>(l[t], o[t]) && last[t] >= 0;
+    if (__builtin_expect(__any(odd), 0)) {  // rare: this wave's steps once more
+      begin();
+      request();
+      steps(std::true_type{});
+    }
+    const Part done = w;
+    const bool more = walk.next(a, w);
+    if (more) request();
+    join_waves<T, W, NR, E>(a, done, row0, fresh * n, lds, ml, m, l, o);
+    if (!more) break;
   }
 }
 
-template <typename T, int DP, int NR, int W>
-__global__ MRT_ATTN_BOUNDS(1) void k_paged_codes(const PageArgs a) {
+template <typename T, int DP, int W>
+__global__ MRT_ATTN_BOUNDS(1, 1) void k_paged_codes(const PageArgs a) {
   using F = CodeFrag<DP>;
-  constexpr int E = F::E, VW = F::VW, KC = F::KC, KEYS = 64;
+  constexpr int E = F::E, VW = F::VW, KC = F::KC, KEYS = 64, NR = row_tiles(1, DP);
   using Lookup = TileLookup<4>;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, D = a.D;
@@ -767,158 +768,161 @@ __global__ MRT_ATTN_BOUNDS(1) void k_paged_codes(const PageArgs a) {
   request();
 
   for (;;) {
-  const int b = w.b, kvh = w.kvh;
-  const int len = length_of(a, b), fresh = fresh_of(a, b);
-  if (w.open) w.s1 = w.steps = steps_of<KEYS>(a, b);
+    const int b = w.b, kvh = w.kvh;
+    const int len = length_of(a, b), fresh = fresh_of(a, b);
+    if (w.open) w.s1 = w.steps = steps_of<KEYS>(a, b);
 
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  __shared__ float2 ml[W][16 * NR];
-  __shared__ __attribute__((aligned(16))) float sc[W][128];  // the scales of a wave's step
-  float* btab = reinterpret_cast<float*>(lds);
-  const BiasTable table_of(a, btab, kvh, n);
-  uint4 qa[NR][KC], qb[NR][KC], qc[NR][KC];
-  float qf[NR];
-  int last[NR], head[NR];
-#pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
-    qf[t] = F::digits(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D,
-                      qa[t], qb[t], qc[t]) * a.scale * kLog2e;
-    last[t] = node < fresh ? len + node : -1, head[t] = hq;
-  }
-  if (a.bias != nullptr && table_of.fill(btab, n, 64 * W)) ring_barrier();  // does not wait for the loads of the first step
-
-  f32x4_t o[NR][E];
-  float m[NR], l[NR];
-#pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    m[t] = kNone, l[t] = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
-  }
-  const i32x4_t zero = {0, 0, 0, 0};
-  // Keys at distances beyond the table's have its last value, unless that is a mask.
-  float far[NR];
-  bool plain = true;
-#pragma unroll
-  for (int t = 0; t < NR; ++t) {
-    far[t] = 0.f;
-    if (a.bias != nullptr) table_of.template each<1>(head[t], INT_MAX, [](int) { return 0; }, [&](int, float by) { far[t] = by; });
-    plain = plain && far[t] >= kNone;
-  }
-  const int near = a.bias == nullptr ? INT_MAX : __all(plain) ? len - a.buckets + 2 : 0;  // from here on the table is read
-
-  for (int st = w.s0 + wid; st < w.s1; st += W) {
-    const int base = st * KEYS;
-    const bool there = page[0] >= 0 && page[1] >= 0 && page[2] >= 0 && page[3] >= 0;
-    const bool masks = !there || fresh == 0 || base + KEYS > min(near, len + 1);
-    const bool in[4] = {page[0] >= 0, page[1] >= 0, page[2] >= 0, page[3] >= 0};
-    const bool more = st + W < w.s1;
-    sc[wid][lane] = ks, sc[wid][64 + lane] = vs;  // read by the wave's lanes alone, in order
-    __builtin_amdgcn_wave_barrier();
-    float p[NR][16];
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    __shared__ float2 ml[W][16 * NR];
+    __shared__ __attribute__((aligned(16))) float sc[W][128];  // the scales of a wave's step
+    float* btab = reinterpret_cast<float*>(lds);
+    const BiasTable table_of(a, btab, kvh, n);
+    uint4 qa[NR][KC], qb[NR][KC], qc[NR][KC];
+    float qf[NR];
+    int last[NR], head[NR];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        i32x4_t x = zero, y = zero, z = zero;
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          x = mma8(kf[k][c], qa[t][c], x);
-          y = mma8(kf[k][c], qb[t][c], y);
-          z = mma8(kf[k][c], qc[t][c], z);
-        }
-        const float4 s = *reinterpret_cast<const float4*>(&sc[wid][k * 16 + 4 * g]);
-        const float by_key[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          p[t][4 * k + r] = join_digits(x[r], y[r], z[r]) * qf[t] * by_key[r];
-          asm volatile("" : "+v"(p[t][4 * k + r]));  // here: the sums of all tiles do not fit the registers
-        }
-        __builtin_amdgcn_sched_barrier(0);
-      }
+      const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
+      qf[t] = F::digits(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D,
+                        qa[t], qb[t], qc[t]) * a.scale * kLog2e;
+      last[t] = node < fresh ? len + node : -1, head[t] = hq;
     }
-    if (more) {
-      if (st + W - looked >= Lookup::kSteps * W) {
-        looked = st + W;
-        look.fetch(a, table, looked, W, lane);
-      }
-      find(st + W);
-      load_k(st + W);
-    }
-    uint4 wa[NR], wb[NR], wc[NR];
-    float wf[NR];
+    if (a.bias != nullptr && table_of.fill(btab, n, 64 * W)) ring_barrier();  // does not wait for the loads of the first step
+
+    f32x4_t o[NR][E];
+    float m[NR], l[NR];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
-      float sv[16];
+      m[t] = kNone, l[t] = 0.f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float4 s = *reinterpret_cast<const float4*>(&sc[wid][64 + k * 16 + 4 * g]);
-        sv[4 * k] = s.x, sv[4 * k + 1] = s.y, sv[4 * k + 2] = s.z, sv[4 * k + 3] = s.w;
+      for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
+    }
+    const i32x4_t zero = {0, 0, 0, 0};
+    // Keys at distances beyond the table's have its last value, unless that is a mask.
+    float far[NR];
+    bool plain = true;
+#pragma unroll
+    for (int t = 0; t < NR; ++t) {
+      far[t] = 0.f;
+      if (a.bias != nullptr)
+        table_of.template each<1>(head[t], INT_MAX, [](int) { return 0; }, [&](int, float by) { far[t] = by; });
+      plain = plain && far[t] >= kNone;
+    }
+    const int near = a.bias == nullptr ? INT_MAX : __all(plain) ? len - a.buckets + 2 : 0;  // from here on the table is read
+
+    for (int st = w.s0 + wid; st < w.s1; st += W) {
+      const int base = st * KEYS;
+      const bool there = page[0] >= 0 && page[1] >= 0 && page[2] >= 0 && page[3] >= 0;
+      const bool masks = !there || fresh == 0 || base + KEYS > min(near, len + 1);
+      const bool in[4] = {page[0] >= 0, page[1] >= 0, page[2] >= 0, page[3] >= 0};
+      const bool more = st + W < w.s1;
+      sc[wid][lane] = ks, sc[wid][64 + lane] = vs;  // read by the wave's lanes alone, in order
+      __builtin_amdgcn_wave_barrier();
+      float p[NR][16];
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          i32x4_t x = zero, y = zero, z = zero;
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            x = mma8(kf[k][c], qa[t][c], x);
+            y = mma8(kf[k][c], qb[t][c], y);
+            z = mma8(kf[k][c], qc[t][c], z);
+          }
+          const float4 s = *reinterpret_cast<const float4*>(&sc[wid][k * 16 + 4 * g]);
+          const float by_key[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            p[t][4 * k + r] = join_digits(x[r], y[r], z[r]) * qf[t] * by_key[r];
+            asm volatile("" : "+v"(p[t][4 * k + r]));  // here: the sums of all tiles do not fit the registers
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
-      if (masks) {
-        const int upto = last[t] - base - 4 * g;  // the row's newest key, from the lane's first on
-        auto key = [](int j) { return (j >> 2) * 16 + (j & 3); };
-        if (a.bias != nullptr)
-          table_of.template each<16>(head[t], upto, key, [&](int j, float by) { p[t][j] = by < kNone ? -INFINITY : p[t][j] + by; });
-        const int most[4] = {in[0] ? upto : -1, in[1] ? upto : -1, in[2] ? upto : -1, in[3] ? upto : -1};
+      if (more) {
+        if (st + W - looked >= Lookup::kSteps * W) {
+          looked = st + W;
+          look.fetch(a, table, looked, W, lane);
+        }
+        find(st + W);
+        load_k(st + W);
+      }
+      uint4 wa[NR], wb[NR], wc[NR];
+      float wf[NR];
+#pragma unroll
+      for (int t = 0; t < NR; ++t) {
+        float sv[16];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float4 s = *reinterpret_cast<const float4*>(&sc[wid][64 + k * 16 + 4 * g]);
+          sv[4 * k] = s.x, sv[4 * k + 1] = s.y, sv[4 * k + 2] = s.z, sv[4 * k + 3] = s.w;
+        }
+        if (masks) {
+          const int upto = last[t] - base - 4 * g;  // the row's newest key, from the lane's first on
+          auto key = [](int j) { return (j >> 2) * 16 + (j & 3); };
+          if (a.bias != nullptr)
+            table_of.template each<16>(head[t], upto, key, [&](int j, float by) {
+              p[t][j] = by < kNone ? -INFINITY : p[t][j] + by;
+            });
+          const int most[4] = {in[0] ? upto : -1, in[1] ? upto : -1, in[2] ? upto : -1, in[3] ? upto : -1};
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const bool out = key(j) > most[j >> 2] || p[t][j] < kNone;
+            p[t][j] = out ? -INFINITY : p[t][j];
+            sv[j] = out ? 0.f : sv[j];  // a masked entry's scale may be NaN
+          }
+        } else if (a.bias != nullptr) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) p[t][j] += far[t];
+        }
+        float top = p[t][0];
+#pragma unroll
+        for (int j = 1; j < 16; ++j) top = fmaxf(top, p[t][j]);
+        top = max_over_groups(top);
+        if (__any(top > m[t])) {
+          asm volatile("");  // a branch: most steps leave the output alone
+          const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
+          m[t] = mn;
+          l[t] *= f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[t][e] *= f;
+        }
+        uint32_t size = 0;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const bool out = key(j) > most[j >> 2] || p[t][j] < kNone;
-          p[t][j] = out ? -INFINITY : p[t][j];
-          sv[j] = out ? 0.f : sv[j];  // a masked entry's scale may be NaN
+          const float x = __builtin_amdgcn_exp2f(p[t][j] - m[t]);
+          l[t] += x;
+          p[t][j] = x * sv[j];
+          size = max(size, __float_as_uint(p[t][j]));  // bits of what is not negative order as the values do, NaN above all
         }
-      } else if (a.bias != nullptr) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) p[t][j] += far[t];
+        size = max_bits_over_groups(size);
+        F::digits(p[t], to_digits(size), wa[t], wb[t], wc[t]);
+        wf[t] = from_digits(size);
       }
-      float top = p[t][0];
 #pragma unroll
-      for (int j = 1; j < 16; ++j) top = fmaxf(top, p[t][j]);
-      top = max_over_groups(top);
-      if (__any(top > m[t])) {
-        asm volatile("");  // a branch: most steps leave the output alone
-        const float mn = fmaxf(m[t], top), f = __builtin_amdgcn_exp2f(m[t] - mn);
-        m[t] = mn;
-        l[t] *= f;
+      for (int x = 0; x < VW; ++x) {
+        uint4 op[4];
+        F::transpose(vf, x, op);
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[t][e] *= f;
-      }
-      uint32_t size = 0;
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float x = __builtin_amdgcn_exp2f(p[t][j] - m[t]);
-        l[t] += x;
-        p[t][j] = x * sv[j];
-        size = max(size, __float_as_uint(p[t][j]));  // bits of what is not negative order as the values do, NaN above all
-      }
-      size = max_bits_over_groups(size);
-      F::digits(p[t], to_digits(size), wa[t], wb[t], wc[t]);
-      wf[t] = from_digits(size);
-    }
+          for (int t = 0; t < NR; ++t) {
+            const i32x4_t u = mma8(op[e], wa[t], zero), v = mma8(op[e], wb[t], zero), y = mma8(op[e], wc[t], zero);
 #pragma unroll
-    for (int x = 0; x < VW; ++x) {
-      uint4 op[4];
-      F::transpose(vf, x, op);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-#pragma unroll
-        for (int t = 0; t < NR; ++t) {
-          const i32x4_t u = mma8(op[e], wa[t], zero), v = mma8(op[e], wb[t], zero), y = mma8(op[e], wc[t], zero);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[t][4 * x + e][r] = fmaf(join_digits(u[r], v[r], y[r]), wf[t], o[t][4 * x + e][r]);
-          asm volatile("" : "+v"(o[t][4 * x + e]));
+            for (int r = 0; r < 4; ++r) o[t][4 * x + e][r] = fmaf(join_digits(u[r], v[r], y[r]), wf[t], o[t][4 * x + e][r]);
+            asm volatile("" : "+v"(o[t][4 * x + e]));
+          }
+          if (e & 1) __builtin_amdgcn_sched_barrier(0);
         }
-        if (e & 1) __builtin_amdgcn_sched_barrier(0);
       }
+      if (more) load_v();
     }
-    if (more) load_v();
-  }
-  const Part done = w;
-  const bool again = walk.next(a, w);
-  if (again) request();
-  join_waves<T, W, NR, E>(a, done, row0, fresh * n, lds, ml, m, l, o);
-  if (!again) break;
+    const Part done = w;
+    const bool again = walk.next(a, w);
+    if (again) request();
+    join_waves<T, W, NR, E>(a, done, row0, fresh * n, lds, ml, m, l, o);
+    if (!again) break;
   }
 }
 
@@ -1007,9 +1011,9 @@ template <typename T, int DP, int NR>
 void launch(const PageArgs& a, bool codes, hipStream_t s) {
   if constexpr (NR <= row_tiles(sizeof(T), DP)) {
     if (codes) {
-      if constexpr (DP >= 64) {
+      if constexpr (DP >= 64 && NR <= row_tiles(1, DP)) {
         constexpr int W = waves_of(1, DP);
-        start(&k_paged_codes<T, DP, NR, W>, 64 * W, (size_t)W / 2 * NR * (DP / 16) * 1024, a, s);
+        start(&k_paged_codes<T, DP, W>, 64 * W, (size_t)W / 2 * NR * (DP / 16) * 1024, a, s);
       }
     } else {
       constexpr int W = waves_of(sizeof(T), DP);

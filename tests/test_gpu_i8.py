@@ -127,3 +127,27 @@ def test_products_of_quantised_operands(dtype):
     hx, hw = ax.amax(1, keepdim=True) / 254 * 1.0001, aw.amax(1, keepdim=True) / 254 * 1.0001
     lim = hx * aw.sum(1) + ax.sum(1, keepdim=True) * hw.T + 512 * hx * hw.T
     assert ((y - x.double() @ w.double().T).abs() <= lim).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("aligned", [True, False], ids=["whole", "odd"])
+@pytest.mark.parametrize("rows,k,n", [
+    (520, 144, 13057), (520, 128, 13056), (4100, 128, 5891), (4100, 32, 5888),  # tiles of 256 x 256, one a block and several
+    (257, 128, 13060), (1030, 160, 13056), (1024, 256, 13056),                  # 128 x 256
+    (70, 128, 16385), (4100, 48, 1794), (4096, 384, 1792),                      # 128 x 128
+    (4100, 128, 133), (130, 400, 16384), (128, 256, 16384),                     # 64 x 128
+    (40, 128, 8198), (40, 1040, 8200), (40, 128, 102), (300, 640, 500),         # 32 rows
+])
+def test_one_and_several_tiles_a_block(rows, k, n, aligned, dtype):
+    """With and without a residual; results in 16-byte stores or one by one; nothing past the edges."""
+    x, xs, w, ws = (t.to(DEV) for t in make(7, rows, k, n))
+    sums = x.double() @ w.double().T.contiguous()
+    want = sums * xs.double()[:, None] * ws.double()
+    pad = 8 if aligned else 3
+    out = torch.full((rows + 1, -(-n // 8) * 8 + pad), 7.0, dtype=DT[dtype], device=DEV)
+    got = mrt_df.i8_matmul(x, xs, w, ws, dtype=DT[dtype], out=out[:rows, :n])
+    check(got, want)
+    assert (out[rows] == 7).all() and (out[:, n:] == 7).all()
+    add = torch.randn((rows, out.shape[1]), generator=torch.Generator().manual_seed(8)).to(DEV, DT[dtype])[:, :n]
+    check(mrt_df.i8_matmul(x, xs, w, ws, add=add, out=out[:rows, :n]), want + add.double(), add)
+    assert (out[rows] == 7).all() and (out[:, n:] == 7).all()

@@ -147,3 +147,34 @@ def test_draws_follow_the_target():
     chi = float(((seen - want) ** 2 / want).sum())
     assert chi < 31.3  # 11 degrees of freedom: 1 in 1000
     assert (count > 0).float().mean() > 0.5
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("sure", [False, True], ids=["drawn", "sure"])
+def test_many_rejections_over_a_large_vocabulary(sure, dtype):
+    """Up to 20 children of one slot rejected, then some of the next: more passes than are
+    made ahead of the last launch, beside sequences that end at once."""
+    s = make(11, dtype, 5, 30, 50001, True, sure, near=2.0)
+    s["parents"][:] = torch.tensor([-1] * 20 + [19] * 10)
+    s["uniforms"][:, :30] = 1.0 - 2.0 ** -24
+    s["uniforms"][0, 0] = 0  # its first child, which has none
+    s["uniforms"][1, 19] = 0
+    s["uniforms"][2, 4] = 0.3
+    paths, _ = check(s)
+    assert paths[0] == [0] and any(not p or p[0] > 6 for p in paths)
+
+
+def test_many_sequences_over_a_large_vocabulary():
+    """As many as there are CUs: a block each, whatever the vocabulary."""
+    s = make(12, "bf16", 257, 1, 40009, False, False)
+    check(s)
+
+
+def test_passes_do_not_depend_on_how_many_blocks_make_them():
+    """The same sequence among few, many blocks each, and among so many that one block makes all."""
+    s = make(13, "fp32", 2, 9, 40960, True, False, near=2.0)
+    few = mrt_df.draft_verify(*(s[n].to(DEV) for n in ("target", "draft", "tokens", "uniforms")), parents=s["parents"].to(DEV))
+    many = {n: x.to(DEV).repeat(128, *[1] * (x.dim() - 1)) for n, x in s.items()}
+    got = mrt_df.draft_verify(many["target"], many["draft"], many["tokens"], many["uniforms"], parents=many["parents"])
+    for x, y in zip(few, got):
+        assert torch.equal(x.repeat(128, *[1] * (x.dim() - 1)), y)

@@ -65,7 +65,7 @@ BAD_ATTENTION = {
     "negative stride": dict(os=(4096, 1024, -64)), "overlapping out": dict(os=(4096, 0, 64)), "no tokens": dict(tokens=0),
     "many tokens": dict(tokens=65), "heads": dict(heads=3), "no heads": dict(heads=0), "bias without buckets": dict(bias=P),
     "too many buckets": dict(bias=P, buckets=(1 << 18) + 1), "misaligned bias": dict(bias=P + 2, buckets=4),
-    "another dtype": dict(dtype=0), "dtype": dict(dtype=3), "misaligned lse": dict(lse=P + 1), "misaligned fresh": dict(fresh=P + 2),
+    "large bias": dict(bias=P, heads=1 << 14, buckets=1 << 17), "another dtype": dict(dtype=0), "dtype": dict(dtype=3), "misaligned lse": dict(lse=P + 1), "misaligned fresh": dict(fresh=P + 2),
 }
 
 
@@ -93,13 +93,13 @@ def product(x=P, xs=P, w=P, ws=P, add=0, out=V, ld=(64, 64, 32, 32), rows=4, n=3
 BAD_PRODUCTS = {
     "null x": dict(x=0), "null x_scale": dict(xs=0), "null w": dict(w=0), "null w_scale": dict(ws=0), "null out": dict(out=0),
     "misaligned x": dict(x=P + 8), "misaligned w": dict(w=P + 8), "misaligned scale": dict(xs=P + 2), "misaligned out": dict(out=V + 1),
-    "misaligned add": dict(add=P + 1), "negative rows": dict(rows=-1), "many rows": dict(rows=(1 << 24) + 1), "no n": dict(n=0),
+    "misaligned add": dict(add=P + 1), "negative rows": dict(rows=-1), "many rows": dict(rows=1 << 24), "no n": dict(n=0),
     "large n": dict(n=(1 << 26) + 1), "odd k": dict(k=24), "no k": dict(k=0), "large k": dict(k=1 << 17, ld=(1 << 17, 1 << 17, 32, 32)),
     "short ldx": dict(ld=(48, 64, 32, 32)), "odd ldx": dict(ld=(72, 64, 32, 32)), "short ldw": dict(ld=(64, 48, 32, 32)),
     "odd ldw": dict(ld=(64, 72, 32, 32)), "short ldo": dict(ld=(64, 64, 32, 31)), "negative lda": dict(add=P, ld=(64, 64, -32, 32)),
     "long ldx": dict(ld=(1 << 24, 64, 32, 32)), "long ldw": dict(ld=(64, 1 << 24, 32, 32)),
     "in place with another stride": dict(add=V, ld=(64, 64, 0, 32)), "dtype": dict(dtype=3),
-    "too many tiles": dict(rows=1 << 24, n=1 << 26, ld=(64, 64, 1 << 26, 1 << 26)),
+    "too many tiles": dict(rows=(1 << 24) - 1, n=1 << 26, ld=(64, 64, 1 << 26, 1 << 26)),
 }
 
 
@@ -179,7 +179,7 @@ def test_products(lib, bad):
 def test_quantize(lib):
     good = dict(src=P, ld=64, rows=4, k=64, dtype=1, codes=V, ldc=64, scales=P)
     for bad in (dict(src=0), dict(codes=0), dict(scales=0), dict(src=P + 8), dict(codes=V + 8), dict(scales=P + 2), dict(ld=56),
-                dict(ld=68), dict(ldc=48), dict(ldc=72), dict(k=24), dict(k=0), dict(k=1 << 17), dict(rows=-1), dict(dtype=7)):
+                dict(ld=68), dict(ldc=48), dict(ldc=72), dict(k=24), dict(k=0), dict(k=1 << 17), dict(rows=-1), dict(rows=1 << 24), dict(dtype=7)):
         refused(lib, lib.mrt_i8_quantize(*dict(good, **bad).values(), 0, None))
 
 
