@@ -978,6 +978,16 @@ __global__ __launch_bounds__(256) void k_paged_join(const PageArgs a, int cols) 
 
 // ---- host -----------------------------------------------------------------------------------
 
+// Cutting units costs 4 to 8 us: the walk over the lengths, a second join in most blocks, the
+// launch of k_paged_join.  Whole units leave a wave up to (rounds of units over the blocks less
+// units a block) x steps / waves more steps to read, one after the other, about 10 us for 84 KB.
+// So units are cut where it is more than that (codes of d 64 take as long as those of d 128), by
+// the table's room, as lengths are not known here.  One token, whole / cut (us): 16 heads of
+// d 64 in bf16, 2 sequences of 1000 entries 13.0 / 15.0, of 2400 26.9 / 15.5; 24 of 2400 45.8 /
+// 54.0; 8-bit pages, 2 of 1000 12.5 / 15.3, of 2400 24.2 / 15.7; 24 of 2400 33.9 / 39.1.  With
+// many units a block they even out: 100 x 16 heads of up to 2400 114.1 / 115.2.
+constexpr int64_t kMoreBytes = 84000;
+
 struct Plan {
   int keys, tiles, row_blocks, teams, least, unit;
 };
@@ -993,7 +1003,9 @@ Plan plan(const PagedCache& c, int heads, int tokens) {
   const int64_t steps = ((int64_t)c.capacity() + p.keys - 1) / p.keys;
   const int waves = waves_of(elt, dp), teams = std::max(8, 256 * blocks_of_cu(elt, dp, p.tiles) / p.row_blocks / 8 * 8);
   p.least = 2 * waves;
-  p.unit = steps <= 10 * waves || units >= 8 * teams ? 0 : 2 * waves;
+  const int64_t rounds = (units + teams - 1) / teams, bytes = (int64_t)p.keys * (c.codes ? std::max(dp, 128) : dp) * (int)elt * 2;
+  const bool whole = (rounds * steps * teams - units * steps) * bytes <= kMoreBytes * waves * teams || units >= 8 * teams;
+  p.unit = whole ? 0 : 2 * waves;
   p.teams = p.unit == 0 ? (int)std::min<int64_t>((units + 7) / 8 * 8, teams) : teams;
   return p;
 }
