@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "codes8.hpp"
 #include "i8.hpp"
 #include "ring_gemm.hpp"
 
@@ -75,19 +76,9 @@ __global__ __launch_bounds__(256) void k_i8_quantize(const T* src, int64_t ld, i
     for (int w = 0; w < TH / 64; ++w) top = max(top, red[w]);
   }
   if (!there) return;
-  const float s = top >= 0x7f800000u ? NAN : __uint_as_float(top) * (1.f / 127.f);
+  const float s = codes_scale(top);
   auto put = [&](const float (&x)[16], int p) {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[j] = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float q = s > 0.f ? fminf(fmaxf(rintf(x[4 * j + e] / s), -127.f), 127.f) : 0.f;
-        w[j] |= ((uint32_t)(int)q & 0xffu) << (8 * e);
-      }
-    }
-    *reinterpret_cast<uint4*>(codes + (int64_t)row * ldc + (int64_t)p * 16) = make_uint4(w[0], w[1], w[2], w[3]);
+    *reinterpret_cast<uint4*>(codes + (int64_t)row * ldc + (int64_t)p * 16) = codes16(x, s);
   };
 #pragma unroll
   for (int h = 0; h < HOLD; ++h)

@@ -1,17 +1,17 @@
 // Entries of a paged cache: written, quantised to 8 bits on the way where the pages hold
 // codes, and read back.
 //
-// A vector is one entry's d values of one K/V head, of K or of V.  Quantised: scale s =
-// max |x| (1 / 127) in fp32, codes the whole numbers nearest to the fp32 quotients x / s
-// (ties to even); it stands for code s.  Every vector has its own scale, so a new entry
-// never changes what others stand for.  A vector with an infinity or NaN has scale NaN: 8
-// bits cannot hold what it was, and nothing that reads it may pass it off as finite.
+// A vector is one entry's d values of one K/V head, of K or of V; codes8.hpp says how it is
+// quantised.  Every vector has its own scale, so a new entry never changes what others stand
+// for.  A vector with an infinity or NaN has scale NaN: 8 bits cannot hold what it was, and
+// nothing that reads it may pass it off as finite.
 //
 // LP lanes (the power of two from d / 16 on) take a vector, 16 elements each, so that
 // codes move in 16-byte pieces and the maximum needs log2 LP exchanges.  Bound by bytes;
 // consecutive vectors are consecutive entries of a head, which lie together in a page.
 #include <algorithm>
 
+#include "codes8.hpp"
 #include "device_utils.hpp"
 #include "paged.hpp"
 
@@ -33,7 +33,7 @@ struct MoveArgs {
 };
 
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
+__device__ __forceinline__ void load8(const T* p, float* v) {
   if constexpr (sizeof(T) == 4) {
     const uint4 a = ld_g16(p), b = ld_g16(p + 4);
     v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
@@ -46,7 +46,7 @@ __device__ __forceinline__ void load8(const T* p, float (&v)[8]) {
   }
 }
 template <typename T>
-__device__ __forceinline__ void store8(T* p, const float (&v)[8]) {
+__device__ __forceinline__ void store8(T* p, const float* v) {
   if constexpr (sizeof(T) == 4) {
     reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
     reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
@@ -69,11 +69,11 @@ __global__ __launch_bounds__(256) void k_paged_move(const MoveArgs a) {
   const int len = min(max(a.length[b], 0), a.capacity);
   T* row = reinterpret_cast<T*>(a.rows_p[x]) + b * a.r_row[x] + t * a.r_node[x] + h * a.r_head[x];
   const int d0 = part * 16;
-  float v[2][8] = {};
+  float v[16] = {};
   if constexpr (WRITE) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      if (d0 + c * 8 < a.D) load8(row + d0 + c * 8, v[c]);
+      if (d0 + c * 8 < a.D) load8(row + d0 + c * 8, v + c * 8);
   }
   int entry;
   bool there;
@@ -96,29 +96,16 @@ __global__ __launch_bounds__(256) void k_paged_move(const MoveArgs a) {
   if constexpr (WRITE && CODES) {
     uint32_t top = 0;  // bits of |x| order as the values do, NaN above all
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(v[c][j]) & 0x7fffffffu);
+    for (int j = 0; j < 16; ++j) top = max(top, __float_as_uint(v[j]) & 0x7fffffffu);
 #pragma unroll
     for (int o = 1; o < LP; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-    const float s = top >= 0x7f800000u ? NAN : __uint_as_float(top) * (1.f / 127.f);
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      w[j] = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        // beyond 127 only where s is so small that it was rounded down by much
-        const float q = s > 0.f ? fminf(fmaxf(rintf(v[j / 2][(j % 2) * 4 + k] / s), -127.f), 127.f) : 0.f;
-        w[j] |= ((uint32_t)(int)q & 0xffu) << (8 * k);
-      }
-    }
-    if (d0 < a.D) *reinterpret_cast<uint4*>(a.pool[x] + to + d0) = make_uint4(w[0], w[1], w[2], w[3]);
+    const float s = codes_scale(top);
+    if (d0 < a.D) *reinterpret_cast<uint4*>(a.pool[x] + to + d0) = codes16(v, s);
     if (part == 0) *scale = s;
   } else if constexpr (WRITE) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      if (d0 + c * 8 < a.D) store8(reinterpret_cast<T*>(a.pool[x]) + to + d0 + c * 8, v[c]);
+      if (d0 + c * 8 < a.D) store8(reinterpret_cast<T*>(a.pool[x]) + to + d0 + c * 8, v + c * 8);
   } else {
     if constexpr (CODES) {
       if (d0 >= a.D) return;
@@ -128,15 +115,15 @@ __global__ __launch_bounds__(256) void k_paged_move(const MoveArgs a) {
 #pragma unroll
       for (int j = 0; j < 4; ++j)
 #pragma unroll
-        for (int k = 0; k < 4; ++k) v[j / 2][(j % 2) * 4 + k] = (float)(int8_t)(w[j] >> (8 * k)) * s;
+        for (int k = 0; k < 4; ++k) v[4 * j + k] = (float)(int8_t)(w[j] >> (8 * k)) * s;
     } else {
 #pragma unroll
       for (int c = 0; c < 2; ++c)
-        if (d0 + c * 8 < a.D) load8(reinterpret_cast<const T*>(a.pool[x]) + to + d0 + c * 8, v[c]);
+        if (d0 + c * 8 < a.D) load8(reinterpret_cast<const T*>(a.pool[x]) + to + d0 + c * 8, v + c * 8);
     }
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      if (d0 + c * 8 < a.D) store8(row + d0 + c * 8, v[c]);
+      if (d0 + c * 8 < a.D) store8(row + d0 + c * 8, v + c * 8);
   }
 }
 

@@ -151,3 +151,23 @@ def test_one_and_several_tiles_a_block(rows, k, n, aligned, dtype):
     add = torch.randn((rows, out.shape[1]), generator=torch.Generator().manual_seed(8)).to(DEV, DT[dtype])[:, :n]
     check(mrt_df.i8_matmul(x, xs, w, ws, add=add, out=out[:rows, :n]), want + add.double(), add)
     assert (out[rows] == 7).all() and (out[:, n:] == 7).all()
+
+
+def near_ties(rows, k, seed=9):
+    """Rows of fp32 whose values are within four steps of a half of their row's scale, of all sizes."""
+    g = torch.Generator().manual_seed(seed)
+    most = (torch.rand(rows, generator=g) + 1) * torch.exp2(torch.randint(-118, 120, (rows,), generator=g).float())
+    scale = most * (torch.tensor(1.0) / 127)
+    half = torch.randint(-126, 126, (rows, k), generator=g).float() + 0.5
+    x = (scale.double()[:, None] * half.double()).float().contiguous()
+    x = (x.view(torch.int32) + torch.randint(-4, 5, (rows, k), generator=g, dtype=torch.int32)).view(torch.float32)
+    x[:, 5] = most
+    return x
+
+
+def test_codes_near_ties():
+    """The quotient's rounding decides: equal to the definition in every code."""
+    x = near_ties(20000, 128)
+    want, ws = O.quantise(x)
+    codes, scale = mrt_df.i8_quantize(x.to(DEV))
+    assert torch.equal(scale.cpu(), ws) and torch.equal(codes.cpu(), want)

@@ -23,6 +23,7 @@ import torch
 
 import mrt_df
 from oracle import serving_oracle as O
+from test_gpu_i8 import near_ties
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -406,6 +407,12 @@ def test_codes_of_odd_entries(dtype):
     k[0, 6] = (torch.arange(64) - 31.5)   # ties where the scale is 1/2
     k[0, 6, :, 0] = 63.5
     k[0, 7, :, 1:] = 0
+    check_write(c, new, None)
+
+
+def test_codes_near_ties():
+    c, new, _ = store_case(26, "i8-fp32", 2, 3, 128, 200, [0, 7], 64)
+    new = [near_ties(1200, 128, seed).view(new[0].shape) for seed in (1, 2)]
     check_write(c, new, None)
 
 
