@@ -21,7 +21,7 @@ __device__ __forceinline__ float codes_scale(uint32_t top) {
 // y + (x - y s) r in fused steps corrects it: to less than one, then, by Markstein's theorem
 // (Computation of elementary functions on the IBM RISC System/6000 processor, 1990), to the
 // quotient rounded to nearest.  That takes 5 instructions of a division's 10: 16 x 4001 tokens
-// of 8 heads of d 128 in fp16 are written in 83 us, not 97.  Where s is below 2^-60 remainders
+// of 8 heads of d 128 in fp16 are written in 80 us, not 97.  Where s is below 2^-60 remainders
 // may lose bits and the division itself is used; the least scales are rounded down by so much
 // that quotients are beyond 127.
 __device__ __forceinline__ uint4 codes16(const float (&x)[16], float s) {

@@ -6,9 +6,14 @@
 // for.  A vector with an infinity or NaN has scale NaN: 8 bits cannot hold what it was, and
 // nothing that reads it may pass it off as finite.
 //
-// LP lanes (the power of two from d / 16 on) take a vector, 16 elements each, so that
-// codes move in 16-byte pieces and the maximum needs log2 LP exchanges.  Bound by bytes;
-// consecutive vectors are consecutive entries of a head, which lie together in a page.
+// LP lanes (the power of two from d / 16 on) take a vector, 16 elements each: to quantise, 16
+// in a row, so that codes move in 16-byte pieces and the maximum needs log2 LP exchanges; else
+// 16-byte pieces of the values, LP in a row, so that what a store covers is contiguous (codes
+// to fp32, 16 x 2000 tokens of 8 heads of d 128: 96 us with 64 bytes a lane, 63 so).  Bound by
+// bytes; consecutive vectors are consecutive entries of a head, which lie together in a page.
+// 16 x 4001 tokens in fp16: written in 80 us, read in 84, 4.9 and 4.7 TB/s, as a large copy.
+// Several vectors a lane group do not help: 97, 106 and 124 us with one, two and four (when a
+// write took 97).
 #include <algorithm>
 
 #include "codes8.hpp"
@@ -32,29 +37,19 @@ struct MoveArgs {
   bool tokens_inner;
 };
 
+// 16 values.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v) {
-  if constexpr (sizeof(T) == 4) {
-    const uint4 a = ld_g16(p), b = ld_g16(p + 4);
-    v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z), v[3] = __uint_as_float(a.w);
-    v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y), v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
-  } else {
-    const uint4 a = ld_g16(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
+  constexpr int kPer = 16 / sizeof(T);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[2 * j] = St<T>::unbits(w[j] & 0xffffu), v[2 * j + 1] = St<T>::unbits(w[j] >> 16);
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* v) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint32_t w[4];
+  for (int x = 0; x < 16 / kPer; ++x) {
+    union {
+      uint4 w;
+      T e[kPer];
+    } u;
+    u.w = ld_g16(p + x * kPer);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = St<T>::bits(v[2 * j]) | (St<T>::bits(v[2 * j + 1]) << 16);
-    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < kPer; ++j) v[x * kPer + j] = St<T>::ld(u.e[j]);
   }
 }
 
@@ -68,12 +63,16 @@ __global__ __launch_bounds__(256) void k_paged_move(const MoveArgs a) {
   const int t = a.tokens_inner ? y : z, h = a.tokens_inner ? z : y;
   const int len = min(max(a.length[b], 0), a.capacity);
   T* row = reinterpret_cast<T*>(a.rows_p[x]) + b * a.r_row[x] + t * a.r_node[x] + h * a.r_head[x];
-  const int d0 = part * 16;
-  float v[16] = {};
-  if constexpr (WRITE) {
+  constexpr int kPer = 16 / sizeof(T), kPieces = 16 / kPer;  // elements of 16 bytes
+  [[maybe_unused]] float v[16] = {};
+  [[maybe_unused]] uint4 piece[kPieces];
+  auto at_of = [&](int p) { return (p * LP + part) * kPer; };  // first element of the lane's piece p
+  if constexpr (WRITE && CODES) {
+    if (part * 16 < a.D) load16(row + part * 16, v);
+  } else if constexpr (WRITE) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-      if (d0 + c * 8 < a.D) load8(row + d0 + c * 8, v + c * 8);
+    for (int p = 0; p < kPieces; ++p)
+      if (at_of(p) < a.D) piece[p] = ld_g16(row + at_of(p));
   }
   int entry;
   bool there;
@@ -100,30 +99,42 @@ __global__ __launch_bounds__(256) void k_paged_move(const MoveArgs a) {
 #pragma unroll
     for (int o = 1; o < LP; o <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, o, 64));
     const float s = codes_scale(top);
-    if (d0 < a.D) *reinterpret_cast<uint4*>(a.pool[x] + to + d0) = codes16(v, s);
+    if (part * 16 < a.D) *reinterpret_cast<uint4*>(a.pool[x] + to + part * 16) = codes16(v, s);
     if (part == 0) *scale = s;
   } else if constexpr (WRITE) {
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-      if (d0 + c * 8 < a.D) store8(reinterpret_cast<T*>(a.pool[x]) + to + d0 + c * 8, v + c * 8);
-  } else {
-    if constexpr (CODES) {
-      if (d0 >= a.D) return;
-      const float s = ld_g(scale);
-      const uint4 c = ld_g16(a.pool[x] + to + d0);
-      const uint32_t w[4] = {c.x, c.y, c.z, c.w};
+    for (int p = 0; p < kPieces; ++p)
+      if (at_of(p) < a.D) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(a.pool[x]) + to + at_of(p)) = piece[p];
+  } else if constexpr (CODES) {
+    const float s = ld_g(scale);
+    uint32_t w[kPieces][kPer / 4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[4 * j + k] = (float)(int8_t)(w[j] >> (8 * k)) * s;
-    } else {
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-        if (d0 + c * 8 < a.D) load8(reinterpret_cast<const T*>(a.pool[x]) + to + d0 + c * 8, v + c * 8);
+    for (int p = 0; p < kPieces; ++p) {
+      const char* from = a.pool[x] + to + min(at_of(p), a.D - kPer);
+      if constexpr (kPer == 8) {
+        const uint64_t u = ld_g(reinterpret_cast<const uint64_t*>(from));
+        w[p][0] = (uint32_t)u, w[p][1] = (uint32_t)(u >> 32);
+      } else {
+        w[p][0] = ld_g(reinterpret_cast<const uint32_t*>(from));
+      }
     }
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
-      if (d0 + c * 8 < a.D) store8(row + d0 + c * 8, v + c * 8);
+    for (int p = 0; p < kPieces; ++p) {
+      union {
+        T e[kPer];
+        uint4 w4;
+      } u;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) u.e[j] = St<T>::st((float)(int8_t)(w[p][j / 4] >> (8 * (j % 4))) * s);
+      if (at_of(p) < a.D) *reinterpret_cast<uint4*>(row + at_of(p)) = u.w4;
+    }
+  } else {
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+      if (at_of(p) < a.D) piece[p] = ld_g16(reinterpret_cast<const T*>(a.pool[x]) + to + at_of(p));
+#pragma unroll
+    for (int p = 0; p < kPieces; ++p)
+      if (at_of(p) < a.D) *reinterpret_cast<uint4*>(row + at_of(p)) = piece[p];
   }
 }
 
