@@ -1383,22 +1383,31 @@ def q4_quantize(weight, group: int = 64):
 
 PAGES_I8 = 3
 _INT32 = 4
-_KIND: Dict = {}  # of the dtypes that these operators take: MRT_DTYPE_*, PAGES_I8, _INT32
 
 
-def _kind(dtype) -> int:
-    if not _KIND:
-        torch = _torch()
-        _KIND.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.int8: PAGES_I8,
-                      torch.int32: _INT32})
-    return _KIND.get(dtype, -1)
+class _Kinds(dict):
+    """Of a dtype: MRT_DTYPE_*, PAGES_I8, _INT32, or -1.  What these calls need of torch is looked up once."""
+
+    f32 = i8 = u8 = bf16 = stream = None
+
+    def __missing__(self, dtype) -> int:
+        if not self:
+            torch = _torch()
+            self.f32, self.i8, self.u8, self.bf16 = torch.float32, torch.int8, torch.uint8, torch.bfloat16
+            self.stream = torch._C._cuda_getCurrentRawStream
+            self.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16, torch.float16: DTYPE_F16, torch.int8: PAGES_I8,
+                         torch.int32: _INT32})
+        return self.get(dtype, -1)
+
+
+_KIND = _Kinds()
 
 
 def _array(t, shape, kind, index, what) -> int:
     """Pointer of a contiguous int32 or fp32 tensor of this shape on GPU ``index``; None: 0."""
     if t is None:
         return 0
-    if t.shape != shape or _kind(t.dtype) != kind or t.get_device() != index or not t.is_contiguous():
+    if t.shape != shape or _KIND[t.dtype] != kind or t.get_device() != index or not t.is_contiguous():
         raise ValueError(f"{what} must be a contiguous {'int32' if kind == _INT32 else 'fp32'} {tuple(shape)} on GPU {index}")
     return t.data_ptr()
 
@@ -1424,7 +1433,7 @@ class PagedCache:
     __slots__ = ("k", "v", "table", "length", "k_scale", "v_scale", "index", "kind", "shape", "rows", "row_pages", "_c")
 
     def __init__(self, k, v, table, length, k_scale=None, v_scale=None):
-        shape, stride, index, kind = k.shape, k.stride(), k.get_device(), _kind(k.dtype)
+        shape, stride, index, kind = k.shape, k.stride(), k.get_device(), _KIND[k.dtype]
         if not 0 <= kind <= PAGES_I8 or len(shape) != 4 or stride[3] != 1:
             raise ValueError("pages: k must be (pages, kv_heads, page_size, d) fp32, bf16, fp16 or int8, d contiguous")
         if v.shape != shape or v.dtype is not k.dtype or v.stride() != stride or v.get_device() != index:
@@ -1432,14 +1441,17 @@ class PagedCache:
         if index < 0:
             raise ValueError("pages: the tensors must be on a GPU")
         where = table.shape
-        if len(where) != 2 or _kind(table.dtype) != _INT32 or table.get_device() != index or table.stride(1) != 1:
+        if len(where) != 2 or _KIND[table.dtype] != _INT32 or table.get_device() != index or table.stride(1) != 1:
             raise ValueError("pages: table must be int32 (rows, row_pages) on k's GPU, rows contiguous")
         if (kind == PAGES_I8) != (k_scale is not None and v_scale is not None) or (k_scale is None) != (v_scale is None):
             raise ValueError("pages: k_scale and v_scale go with int8 codes")
         self.k, self.v, self.table, self.length, self.k_scale, self.v_scale = k, v, table, length, k_scale, v_scale
         self.index, self.kind, self.shape, (self.rows, self.row_pages) = index, kind, shape, where
-        self._c = _PAGES_STRUCT.pack(k.data_ptr(), v.data_ptr(), _array(k_scale, shape[:3], DTYPE_F32, index, "k_scale"),
-                                     _array(v_scale, shape[:3], DTYPE_F32, index, "v_scale"), table.data_ptr(),
+        ks = vs = 0
+        if k_scale is not None:
+            ks = _array(k_scale, shape[:3], DTYPE_F32, index, "k_scale")
+            vs = _array(v_scale, shape[:3], DTYPE_F32, index, "v_scale")
+        self._c = _PAGES_STRUCT.pack(k.data_ptr(), v.data_ptr(), ks, vs, table.data_ptr(),
                                      _array(length, where[:1], _INT32, index, "length"), stride[0], stride[1], stride[2],
                                      table.stride(0), shape[0], where[0], where[1], shape[1], shape[2], shape[3], kind)
 
@@ -1447,7 +1459,7 @@ class PagedCache:
 def _page_rows(t, shape, kind, cache, what):
     """Pointer and strides of a 4-d operand of the dtype ``kind``, which goes with the cache's pages."""
     s = t.stride()
-    if t.shape != shape or _kind(t.dtype) != kind or t.get_device() != cache.index or s[3] != 1 or (
+    if t.shape != shape or _KIND[t.dtype] != kind or t.get_device() != cache.index or s[3] != 1 or (
             kind != cache.kind if cache.kind != PAGES_I8 else not 0 <= kind < PAGES_I8):
         raise ValueError(f"{what} must be {tuple(shape)} of the pages' dtype, with int8 pages fp32, bf16 or fp16, on their GPU, "
                          "d contiguous")
@@ -1465,12 +1477,12 @@ def paged_write(cache: PagedCache, k_new, v_new, fresh=None, length_out=None) ->
     lib, index, rows = load_library(), cache.index, cache.rows
     if k_new.dim() != 4:
         raise ValueError("k_new must be (rows, tokens, kv_heads, d)")
-    tokens, kind = k_new.shape[1], _kind(k_new.dtype)
+    tokens, kind = k_new.shape[1], _KIND[k_new.dtype]
     shape = (rows, tokens, cache.shape[1], cache.shape[3])
     args = _STORE_STRUCT.pack(*_page_rows(k_new, shape, kind, cache, "k_new"), *_page_rows(v_new, shape, kind, cache, "v_new"),
                               _array(fresh, (rows,), _INT32, index, "fresh"), 0,
                               _array(length_out, (rows,), _INT32, index, "length_out"), tokens, kind)
-    code = lib.mrt_paged_write(cache._c, args, index, _raw_stream(index))
+    code = lib.mrt_paged_write(cache._c, args, index, _KIND.stream(index))
     if code:
         _check(lib, code)
 
@@ -1484,12 +1496,12 @@ def paged_read(cache: PagedCache, k_out, v_out, start=None) -> None:
     lib, index, rows = load_library(), cache.index, cache.rows
     if k_out.dim() != 4:
         raise ValueError("k_out must be (rows, kv_heads, tokens, d)")
-    tokens, kind = k_out.shape[2], _kind(k_out.dtype)
+    tokens, kind = k_out.shape[2], _KIND[k_out.dtype]
     shape = (rows, cache.shape[1], tokens, cache.shape[3])
     k, v = _page_rows(k_out, shape, kind, cache, "k_out"), _page_rows(v_out, shape, kind, cache, "v_out")
     args = _STORE_STRUCT.pack(k[0], k[1], k[3], k[2], v[0], v[1], v[3], v[2], 0, _array(start, (rows,), _INT32, index, "start"), 0,
                               tokens, kind)
-    code = lib.mrt_paged_read(cache._c, args, index, _raw_stream(index))
+    code = lib.mrt_paged_read(cache._c, args, index, _KIND.stream(index))
     if code:
         _check(lib, code)
 
@@ -1511,22 +1523,31 @@ def paged_attention(q, cache: PagedCache, fresh=None, scale: float = 1.0, bias=N
     (out (rows, tokens, heads, d), lse (rows, tokens, heads) fp32), new tensors
     unless given; tokens past fresh[b] get 0 and -inf.
     """
-    lib, index, shape, kind = load_library(), cache.index, q.shape, _kind(q.dtype)
+    lib, index, shape, kind = load_library(), cache.index, q.shape, _KIND[q.dtype]
     pages, kv_heads, page_size, d = cache.shape
     if len(shape) != 4 or shape[0] != cache.rows or shape[3] != d:
         raise ValueError("q must be (rows, tokens, heads, d) with the cache's rows and d")
     rows, tokens, heads, _ = shape
+    rows_of_q = _page_rows(q, shape, kind, cache, "q")
     if out is None:
         out = q.new_empty(shape)
+        rows_of_out = out.data_ptr(), tokens * heads * d, heads * d, d
+    else:
+        rows_of_out = _page_rows(out, shape, kind, cache, "out")
     if lse is None:
-        lse = q.new_empty(shape[:3], dtype=_torch().float32)
-    table, buckets = _bias_table(bias, heads, cache)
-    args = _PAGED_STRUCT.pack(*_page_rows(q, shape, kind, cache, "q"), *_page_rows(out, shape, kind, cache, "out"),
-                              _array(fresh, shape[:1], _INT32, index, "fresh"), _array(lse, shape[:3], DTYPE_F32, index, "lse"),
-                              table, buckets, tokens, heads, kind, scale)
+        lse = q.new_empty(shape[:3], dtype=_KIND.f32)
+        lp = lse.data_ptr()
+    else:
+        lp = _array(lse, shape[:3], DTYPE_F32, index, "lse")
+    table = buckets = 0
+    if bias is not None:
+        buckets = bias.shape[-1]
+        table = _array(bias, (heads, buckets), DTYPE_F32, index, "bias")
+    args = _PAGED_STRUCT.pack(*rows_of_q, *rows_of_out, _array(fresh, shape[:1], _INT32, index, "fresh"), lp, table, buckets,
+                              tokens, heads, kind, scale)
     size = _paged_workspace(rows, cache.row_pages, pages, kv_heads, page_size, d, cache.kind, heads, tokens)
-    ws = q.new_empty(size, dtype=_torch().uint8) if size else None
-    code = lib.mrt_paged_attention(cache._c, args, ws.data_ptr() if size else None, size, index, _raw_stream(index))
+    ws = q.new_empty(size, dtype=_KIND.u8) if size else None
+    code = lib.mrt_paged_attention(cache._c, args, ws.data_ptr() if size else None, size, index, _KIND.stream(index))
     if code:
         _check(lib, code)
     return out, lse
@@ -1550,7 +1571,7 @@ def draft_verify(target, draft, tokens, uniforms, parents=None):
     ``tree_attention``, None: a chain.  Returns int32 (accepted (rows, nodes), as
     ``cache_commit`` takes it, count (rows), token (rows): the one that follows).
     """
-    lib, index, shape, kind = load_library(), target.get_device(), target.shape, _kind(target.dtype)
+    lib, index, shape, kind = load_library(), target.get_device(), target.shape, _KIND[target.dtype]
     if len(shape) != 3 or index < 0 or shape[1] < 2 or target.stride(2) != 1 or not 0 <= kind < PAGES_I8:
         raise ValueError("target must be (rows, nodes + 1, vocab) fp32, bf16 or fp16 on a GPU, the vocabulary contiguous")
     rows, nodes, vocab = shape[0], shape[1] - 1, shape[2]
@@ -1571,8 +1592,8 @@ def draft_verify(target, draft, tokens, uniforms, parents=None):
                                _array(uniforms, (rows, nodes + 1), DTYPE_F32, index, "uniforms"), ap, ap + 4 * rows * nodes,
                                ap + 4 * rows * (nodes + 1), rows, nodes, vocab, kind)
     size = _verify_workspace(rows, nodes, vocab, draft is not None, parents is not None)
-    ws = target.new_empty(size, dtype=_torch().uint8) if size else None
-    code = lib.mrt_draft_verify(args, ws.data_ptr() if size else None, size, index, _raw_stream(index))
+    ws = target.new_empty(size, dtype=_KIND.u8) if size else None
+    code = lib.mrt_draft_verify(args, ws.data_ptr() if size else None, size, index, _KIND.stream(index))
     if code:
         _check(lib, code)
     accepted, count, token = got.split((rows * nodes, rows, rows))
@@ -1581,13 +1602,13 @@ def draft_verify(target, draft, tokens, uniforms, parents=None):
 
 def i8_quantize(x):
     """8-bit codes of the rows of x (rows, k), k a multiple of 16 (mrt_i8_quantize): (int8 (rows, k), fp32 scales (rows))."""
-    lib, torch, index, kind, shape = load_library(), _torch(), x.get_device(), _kind(x.dtype), x.shape
+    lib, index, kind, shape = load_library(), x.get_device(), _KIND[x.dtype], x.shape
     if len(shape) != 2 or index < 0 or x.stride(1) != 1 or not 0 <= kind < PAGES_I8:
         raise ValueError("x must be (rows, k) fp32, bf16 or fp16 on a GPU, rows contiguous")
     rows, k = shape
-    codes, scales = x.new_empty(shape, dtype=torch.int8), x.new_empty(rows, dtype=torch.float32)
+    codes, scales = x.new_empty(shape, dtype=_KIND.i8), x.new_empty(rows, dtype=_KIND.f32)
     code = lib.mrt_i8_quantize(x.data_ptr(), x.stride(0), rows, k, kind, codes.data_ptr(), k, scales.data_ptr(), index,
-                               _raw_stream(index))
+                               _KIND.stream(index))
     if code:
         _check(lib, code)
     return codes, scales
@@ -1601,13 +1622,13 @@ def i8_matmul(x, x_scale, w, w_scale, dtype=None, add=None, out=None):
     n) or None, which may be out.  dtype: that of out or add where given, else bf16.
     """
     lib, index, shape, (n, k) = load_library(), x.get_device(), x.shape, w.shape
-    if len(shape) != 2 or shape[1] != k or _kind(x.dtype) != PAGES_I8 or _kind(w.dtype) != PAGES_I8:
+    if len(shape) != 2 or shape[1] != k or _KIND[x.dtype] != PAGES_I8 or _KIND[w.dtype] != PAGES_I8:
         raise ValueError("x and w must be int8 (rows, k) and (n, k)")
     if index < 0 or w.get_device() != index or x.stride(1) != 1 or w.stride(1) != 1:
         raise ValueError("x and w must be on one GPU, rows contiguous")
     if dtype is None:
-        dtype = out.dtype if out is not None else add.dtype if add is not None else _torch().bfloat16
-    kind, rows = _kind(dtype), shape[0]
+        dtype = out.dtype if out is not None else add.dtype if add is not None else _KIND.bf16
+    kind, rows = _KIND[dtype], shape[0]
     if out is None:
         out = x.new_empty((rows, n), dtype=dtype)
     elif out.shape != (rows, n) or out.dtype is not dtype or out.get_device() != index or out.stride(1) != 1:
@@ -1620,7 +1641,7 @@ def i8_matmul(x, x_scale, w, w_scale, dtype=None, add=None, out=None):
     args = _I8_STRUCT.pack(x.data_ptr(), _array(x_scale, shape[:1], DTYPE_F32, index, "x_scale"), w.data_ptr(),
                            _array(w_scale, (n,), DTYPE_F32, index, "w_scale"), ap, out.data_ptr(), x.stride(0), w.stride(0), lda,
                            out.stride(0), rows, n, k, kind)
-    code = lib.mrt_i8_matmul(args, index, _raw_stream(index))
+    code = lib.mrt_i8_matmul(args, index, _KIND.stream(index))
     if code:
         _check(lib, code)
     return out

@@ -92,7 +92,7 @@ def call(c, s, **kw):
 def workspace(c, s):
     """Bytes; none where a block takes whole sequences' heads."""
     n, kv, page, d = c["k"].shape
-    return mrt_df._paged_workspace(*c["table"].shape, n, kv, page, d, mrt_df._kind(c["k"].dtype), s["q"].shape[2], s["q"].shape[1])
+    return mrt_df._paged_workspace(*c["table"].shape, n, kv, page, d, mrt_df._KIND[c["k"].dtype], s["q"].shape[2], s["q"].shape[1])
 
 
 def size_of(c, x, norm):
