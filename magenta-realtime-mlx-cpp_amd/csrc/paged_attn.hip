@@ -23,6 +23,14 @@
 // dimension, transposed in registers by byte permutations, are its operand of
 // O^T = V^T P^T.
 //
+// Bound by bytes but for many rows a K/V head (16 new tokens of 4 heads on one over 8-bit pages
+// of 4 x 32000 entries, d 128: 127 us for 63 with 4, by vector instructions on the digits and the
+// softmax).  One pass, us (bytes at the rate of a large copy): 64 x 16 heads of 1006 entries of
+// d 64 in 8 bits 37 (30), 48 x 8 heads of up to 8191 of d 128 in bf16 156 (172), 3 x 8 heads of
+// up to 131000 in 8 bits, 4 tokens of 4 heads each, 99 (101).  Vector instructions take 42, 19
+// and 36 % of the SIMDs' cycles there, the matrix cores 5 to 9 %, and waves wait for 35 to 47 %
+// of theirs.
+//
 // As many blocks run as the card holds.  Long caches: the units' steps, one after the other,
 // are cut into equal shares, on the device, from the lengths, which the host never sees; a
 // share may end and begin inside units, whose parts leave (maximum, sum, output) in fp32, and
@@ -43,7 +51,7 @@ namespace {
 constexpr int kBiasLds = 4096;  // floats of the bias by distance kept in LDS
 
 // Row tiles a wave holds at most: what one more takes in registers costs more than reading
-// the keys again from the L2.
+// the keys again from the L2.  With 16 rows or fewer there is one.
 constexpr int row_tiles(size_t elt, int dp) { return elt == 2 && dp <= 64 ? 2 : 1; }
 // Waves of a block, and blocks that a CU holds (by their registers).
 constexpr int waves_of(size_t elt, int dp) { return elt == 2 && dp == 128 ? 8 : 4; }
@@ -986,6 +994,10 @@ __global__ __launch_bounds__(256) void k_paged_join(const PageArgs a, int cols) 
 // d 64 in bf16, 2 sequences of 1000 entries 13.0 / 15.0, of 2400 26.9 / 15.5; 24 of 2400 45.8 /
 // 54.0; 8-bit pages, 2 of 1000 12.5 / 15.3, of 2400 24.2 / 15.7; 24 of 2400 33.9 / 39.1.  With
 // many units a block they even out: 100 x 16 heads of up to 2400 114.1 / 115.2.
+//
+// A share has a step a wave at least (two: 2 sequences of 2400, 8 heads of d 128, 8-bit pages,
+// 17.8 us for 15.9; 8 of 5000 23.7 for 25.2), and a unit counts as two more (one: 24 sequences of
+// up to 8000 62 us, two 54, four 56; in bf16 105, 86, 86).
 constexpr int64_t kMoreBytes = 84000;
 
 struct Plan {
@@ -1002,7 +1014,7 @@ Plan plan(const PagedCache& c, int heads, int tokens) {
   const int64_t units = std::max<int64_t>(1, (int64_t)c.rows * c.kv_heads);
   const int64_t steps = ((int64_t)c.capacity() + p.keys - 1) / p.keys;
   const int waves = waves_of(elt, dp), teams = std::max(8, 256 * blocks_of_cu(elt, dp, p.tiles) / p.row_blocks / 8 * 8);
-  p.least = 2 * waves;
+  p.least = waves;
   const int64_t rounds = (units + teams - 1) / teams, bytes = (int64_t)p.keys * (c.codes ? std::max(dp, 128) : dp) * (int)elt * 2;
   const bool whole = (rounds * steps * teams - units * steps) * bytes <= kMoreBytes * waves * teams || units >= 8 * teams;
   p.unit = whole ? 0 : 2 * waves;
