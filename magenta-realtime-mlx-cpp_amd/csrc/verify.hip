@@ -15,9 +15,12 @@
 // each, and the drawn token's segment is the only one looked at again.  k_verify does all of
 // it, a block a sequence.  What bounds that is one CU's share of arithmetic in 64 bits, so over
 // large vocabularies the first passes are made by many blocks, a launch each (k_verify_pass):
-// every block walks the tree as far as the sums of the launches before go, which takes no
-// memory, and sums its segments of the pass that is needed next.  Passes beyond those launches
-// are k_verify's own.  Sums are the same either way, bit for bit.
+// every block takes the walk up where the launch before stopped, goes on by that one's sums as
+// far as they reach, which takes no memory, and sums its segments of the pass that is needed
+// next.  Passes beyond those launches are k_verify's own.  Sums are the same either way, bit
+// for bit.  Bound by launches then, which follow each other: 16 trees of 31 nodes over 131072
+// tokens in fp32 take 38 us in seven of them for 17 MB that they have to read (4 us at the rate
+// of a large copy); a chain of 16 nodes over 1024 tokens is one of 6 us, and 9 from Python.
 #include <algorithm>
 #include <type_traits>
 
@@ -30,12 +33,14 @@ namespace {
 constexpr int kWaves = 16;
 constexpr int kSegments = 256;
 constexpr int kAhead = 4;  // loads of a wave that are on their way: a pass by one block 43 us with one, 35 with four
-// Vocabulary from which passes are made by many blocks.  Chains of 16, drawn (us, one block /
-// many): 32 x 29824 in bf16 13.6 / 16.0, 16 x 131072 in fp32 32.9 / 15.9.
-constexpr int kManyVocab = 40000;
-// Launches of passes for a tree, of 31 nodes with 1.6 passes on average: the most among 16
-// sequences is three to five.  16 x 131072 with 0 / 3 / 5: 152 / 92 / 56 us.
-constexpr int kTreeRounds = 5;
+// Vocabulary from which passes are made by many blocks.  32 chains of 16, drawn (us, one block /
+// many): 16000 in fp32 11.6 / 12.4, 29824 in fp32 15.6 / 12.6, in bf16 13.7 / 12.8; 16 of 131072
+// in fp32 32.9 / 13.2.
+constexpr int kManyVocab = 24000;
+// Launches of passes for trees, of 31 nodes with 1.6 passes on average; the most among 16
+// sequences is three to six, a launch that nobody needs takes 2 to 3 us, a pass by one block 35.
+// 16 x 131072 with 0 / 5 / 7 / 9: 152 / 43 / 42 / 45 us, 2 x 131072 with 4 / 6: 21 / 25.
+constexpr int tree_rounds(int rows) { return rows <= 4 ? 4 : 6; }
 
 // What is not a positive finite number counts as 0.
 __device__ __forceinline__ float counted(float p) {
@@ -235,98 +240,178 @@ __device__ __forceinline__ void run_sums(Sums& s, int segments) {
   __syncthreads();
 }
 
-struct End {
-  int slot, rejected, accepted;  // where the walk ended, rejections there, nodes accepted
-  int path;                      // lane k: the k-th accepted node
+// The walk, the same in every wave of a sequence's blocks: it stops where it needs the sums of a
+// pass, and goes on from there, in the same launch or the next.
+struct Walk {
+  enum { kTest = -1, kLast = -2, kBare = -3 };
+  int here, n, count;  // the slot, rejections there, nodes accepted
+  int wait;            // what the sums are for: the test of a node (its id), the last draw, that from the target itself
+  uint64_t kids;       // children of `here` that are left
+  double z;
+  int path;            // lane k: the k-th accepted node
   Rejections rej;
-};
 
-// The walk, the same in every wave.  pass(slot, n, rejections) leaves the sums of r after n
-// rejections in s, or returns false where the walk is to stop.
-template <bool DRAFT, class Pass>
-__device__ __forceinline__ bool walk(const Nodes& node, int lane, const Sums& s, End& end, Pass&& pass) {
-  int here = 0, n = 0, count = 0, path = -1;
-  double z = 1.0;
-  Rejections rej = {0.0, -1};
-  // the children of `here`, in order; nothing was drawn for what is not a token
-  uint64_t kids = __ballot(node.parent == -1 && node.token >= 0);
-  while (kids != 0) {
-    const int t = __ffsll((unsigned long long)kids) - 1;
-    kids &= kids - 1;
-    if (DRAFT && n > 0) {
-      if (!pass(here, n, rej)) return false;
-      z = s.total;
-    }
-    const int x = lane_of(node.token, t);
-    const float q = lane_of(node.q, t);
-    const double r = Rest<DRAFT, -1>(rej, n)(lane_of(node.p, t), q, x);
-    if ((double)lane_of(node.u, t) * z * (double)q < r) {
-      path = lane == count ? t : path;
-      ++count;
-      here = t + 1, n = 0, z = 1.0;
-      kids = __ballot(node.parent == t && node.token >= 0);
-    } else {
-      rej.z = lane == n ? z : rej.z, rej.token = lane == n ? x : rej.token;
-      if (!DRAFT) z -= r;
-      ++n;
-    }
+  // The children of a node, in order; nothing was drawn for what is not a token.
+  __device__ __forceinline__ static uint64_t children(const Nodes& node, int parent) {
+    return __ballot(node.parent == parent && node.token >= 0);
   }
-  if (!pass(here, n, rej)) return false;
-  if (!(s.total > 0.0) && n > 0) {  // nothing left: the target itself
-    n = 0;
-    if (!pass(here, 0, rej)) return false;
+  __device__ __forceinline__ void begin(const Nodes& node) {
+    here = n = count = 0, wait = kTest, z = 1.0, path = -1, rej = {0.0, -1};
+    kids = children(node, -1);
   }
-  end = {here, n, count, path, rej};
-  return true;
-}
-
-// Pass `round` of each sequence, if it has as many: block (x, b) sums segments x share ..
-// of sequence b.  sums (rounds, rows, kSegments).
-template <typename T, bool DRAFT>
-__global__ __launch_bounds__(256) void k_verify_pass(const VerifyArgs a, bool wide, int round, int share, double* sums) {
-  const Cut<T> cut(a.vocab);
-  const int b = blockIdx.y, first = blockIdx.x * share, last = min(first + share, cut.segments), lane = threadIdx.x & 63;
-  __shared__ Sums s;
-  int done = 0;
-  End end;
-  walk<DRAFT>(gather<T, DRAFT>(a, b, lane), lane, s, end, [&](int at, int n, const Rejections& rej) {
-    double* of = sums + ((int64_t)done * a.rows + b) * kSegments;
-    if (done == round) {
-      sum_segments<T, DRAFT, 4>(a, cut, wide, b, at, n, rej, first, last, [&](int x, double v) { of[x] = v; });
+  // Goes on, with the sum of the pass that it stopped for.  True: the walk has ended, and the
+  // last sums are those of its draw; else it needs those of r at slot `here` after n rejections.
+  template <bool DRAFT>
+  __device__ __forceinline__ bool go(const Nodes& node, int lane, double total) {
+    if (wait == kBare) return true;
+    if (wait == kLast) {
+      if (total > 0.0 || n == 0) return true;
+      n = 0, wait = kBare;  // nothing left: the target itself
       return false;
     }
-    __syncthreads();  // the pass before has been read
-    if ((int)threadIdx.x < cut.segments) s.seg[threadIdx.x] = of[threadIdx.x];
+    if (wait >= 0) z = total;
+    for (;;) {
+      int t = wait;
+      wait = kTest;
+      if (t < 0) {
+        if (kids == 0) {
+          wait = kLast;
+          return false;
+        }
+        t = __ffsll((unsigned long long)kids) - 1;
+        kids &= kids - 1;
+        if (DRAFT && n > 0) {
+          wait = t;
+          return false;
+        }
+      }
+      const int x = lane_of(node.token, t);
+      const float q = lane_of(node.q, t);
+      const double r = Rest<DRAFT, -1>(rej, n)(lane_of(node.p, t), q, x);
+      if ((double)lane_of(node.u, t) * z * (double)q < r) {
+        path = lane == count ? t : path;
+        ++count;
+        here = t + 1, n = 0, z = 1.0;
+        kids = children(node, t);
+      } else {
+        rej.z = lane == n ? z : rej.z, rej.token = lane == n ? x : rej.token;
+        if (!DRAFT) z -= r;
+        ++n;
+      }
+    }
+  }
+};
+
+// A walk between two launches, and its nodes.
+struct Saved {
+  double z, rej_z[64];
+  uint64_t kids;
+  int here, n, count, wait;
+  int rej_token[64], path[64], parent[64], token[64];
+  float p[64], q[64], u[64];
+
+  __device__ __forceinline__ void put(const Walk& w, const Nodes& x, int lane) {
+    rej_z[lane] = w.rej.z, rej_token[lane] = w.rej.token, path[lane] = w.path;
+    parent[lane] = x.parent, token[lane] = x.token, p[lane] = x.p, q[lane] = x.q, u[lane] = x.u;
+    if (lane == 0) z = w.z, kids = w.kids, here = w.here, n = w.n, count = w.count, wait = w.wait;
+  }
+  __device__ __forceinline__ void get(Walk& w, Nodes& x, int lane) const {
+    w.rej = {ld_g(rej_z + lane), ld_g(rej_token + lane)}, w.path = ld_g(path + lane);
+    x.parent = ld_g(parent + lane), x.token = ld_g(token + lane), x.p = ld_g(p + lane), x.q = ld_g(q + lane);
+    x.u = ld_g(u + lane);
+    const double z0 = ld_g(&z);
+    const uint64_t k0 = ld_g(&kids);
+    const int h0 = ld_g(&here), n0 = ld_g(&n), c0 = ld_g(&count), w0 = ld_g(&wait);
+    w.z = lane_of(z0, 0);
+    w.kids = (uint64_t)(uint32_t)lane_of((int)(k0 >> 32), 0) << 32 | (uint32_t)lane_of((int)k0, 0);
+    w.here = lane_of(h0, 0), w.n = lane_of(n0, 0), w.count = lane_of(c0, 0), w.wait = lane_of(w0, 0);
+  }
+};
+
+// What goes from launch to launch.  A launch reads what the one before wrote and writes the
+// other of two halves; the walk and sums of a sequence whose walk has ended stay.
+struct Between {
+  Saved* saved;  // (2, rows)
+  double* sums;  // (2, rows, kSegments)
+  int* ended;    // (2, rows) 0, or the launch that found it ended
+  static size_t bytes(int rows) { return (size_t)rows * (2 * sizeof(Saved) + 2 * kSegments * 8 + 8); }
+  Between(void* ws, int rows)
+      : saved(static_cast<Saved*>(ws)),
+        sums(reinterpret_cast<double*>(saved + 2 * (size_t)rows)),
+        ended(reinterpret_cast<int*>(sums + 2 * (size_t)rows * kSegments)) {}
+  __device__ __forceinline__ Saved& walk_of(int launch, int rows, int b) const { return saved[(int64_t)(launch & 1) * rows + b]; }
+  __device__ __forceinline__ int& ended_of(int launch, int rows, int b) const { return ended[(int64_t)(launch & 1) * rows + b]; }
+  __device__ __forceinline__ double* sums_of(int launch, int rows, int b) const {
+    return sums + ((int64_t)(launch & 1) * rows + b) * kSegments;
+  }
+};
+
+// Launch `round` of passes: block (x, b) sums segments x share .. of sequence b.
+template <typename T, bool DRAFT>
+__global__ __launch_bounds__(256) void k_verify_pass(const VerifyArgs a, bool wide, int round, int share, const Between mem) {
+  const Cut<T> cut(a.vocab);
+  const int b = blockIdx.y, first = blockIdx.x * share, last = min(first + share, cut.segments);
+  const int tid = threadIdx.x, lane = tid & 63;
+  __shared__ Sums s;
+  Nodes node;
+  Walk walk;
+  bool ended = false;
+  if (round == 0) {
+    node = gather<T, DRAFT>(a, b, lane);
+    walk.begin(node);
+    walk.go<DRAFT>(node, lane, 0.0);
+  } else {
+    const int over = ld_g(&mem.ended_of(round - 1, a.rows, b));
+    if (over != 0) {
+      if (blockIdx.x == 0 && tid == 0) mem.ended_of(round, a.rows, b) = over;
+      return;
+    }
+    if (tid < cut.segments) s.seg[tid] = ld_g(mem.sums_of(round - 1, a.rows, b) + tid);
+    mem.walk_of(round - 1, a.rows, b).get(walk, node, lane);
     run_sums(s, cut.segments);
-    ++done;
-    return true;
-  });
+    ended = walk.go<DRAFT>(node, lane, s.total);
+  }
+  if (blockIdx.x == 0 && tid < 64) {
+    mem.walk_of(round, a.rows, b).put(walk, node, lane);
+    if (lane == 0) mem.ended_of(round, a.rows, b) = ended ? round : 0;
+  }
+  if (ended) return;
+  double* to = mem.sums_of(round, a.rows, b);
+  sum_segments<T, DRAFT, 4>(a, cut, wide, b, walk.here, walk.n, walk.rej, first, last, [&](int x, double v) { to[x] = v; });
 }
 
+// The rest, a block a sequence, after `rounds` launches of passes.
 template <typename T, bool DRAFT>
-__global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool wide, int rounds, const double* sums) {
+__global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool wide, int rounds, const Between mem) {
   constexpr int VEC = Cut<T>::VEC, CHUNK = Cut<T>::CHUNK;
   const Cut<T> cut(a.vocab);
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int N = a.nodes, V = a.vocab, per = cut.per, chunks = cut.chunks, segments = cut.segments;
   __shared__ Sums s;
-  int done = 0;
-  End reached;
-  walk<DRAFT>(gather<T, DRAFT>(a, b, lane), lane, s, reached, [&](int at, int n, const Rejections& rej) {
-    __syncthreads();  // the pass before has been read
-    if (done < rounds) {
-      if (tid < segments) s.seg[tid] = sums[((int64_t)done * a.rows + b) * kSegments + tid];
-    } else {
-      sum_segments<T, DRAFT, kWaves>(a, cut, wide, b, at, n, rej, 0, segments, [&](int x, double v) { s.seg[x] = v; });
-    }
+  Nodes node;
+  Walk walk;
+  bool ended = false;
+  if (rounds == 0) {
+    node = gather<T, DRAFT>(a, b, lane);
+    walk.begin(node);
+    walk.go<DRAFT>(node, lane, 0.0);
+  } else {
+    const int at = __builtin_amdgcn_readfirstlane(ld_g(&mem.ended_of(rounds - 1, a.rows, b)));
+    if (tid < segments) s.seg[tid] = ld_g(mem.sums_of(at != 0 ? at - 1 : rounds - 1, a.rows, b) + tid);
+    mem.walk_of(at != 0 ? at : rounds - 1, a.rows, b).get(walk, node, lane);
     run_sums(s, segments);
-    ++done;
-    return true;
-  });
-  const int here = reached.slot, n = reached.rejected;
-  const Rest<DRAFT, -1> rest(reached.rej, n);
-  if (tid < N) a.accepted[(int64_t)b * N + tid] = tid < reached.accepted ? reached.path : -1;
-  if (tid == 0) a.count[b] = reached.accepted;
+    ended = at != 0 || walk.go<DRAFT>(node, lane, s.total);
+  }
+  while (!ended) {
+    __syncthreads();  // the pass before has been read
+    sum_segments<T, DRAFT, kWaves>(a, cut, wide, b, walk.here, walk.n, walk.rej, 0, segments, [&](int x, double v) { s.seg[x] = v; });
+    run_sums(s, segments);
+    ended = walk.go<DRAFT>(node, lane, s.total);
+  }
+  const int here = walk.here, n = walk.n;
+  const Rest<DRAFT, -1> rest(walk.rej, n);
+  if (tid < N) a.accepted[(int64_t)b * N + tid] = tid < walk.count ? walk.path : -1;
+  if (tid == 0) a.count[b] = walk.count;
   if (wid != 0) return;
 
   // The first segment that exceeds the threshold, then its first chunk, lane, token.
@@ -387,12 +472,12 @@ __global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool
 // Passes made by many blocks, a launch each.
 int rounds_of(const VerifyArgs& a) {
   if (a.vocab < kManyVocab || a.rows >= 256) return 0;
-  return a.draft == nullptr || a.parents == nullptr ? 1 : kTreeRounds;  // a chain has one, as have drafts that were not drawn
+  return a.draft == nullptr || a.parents == nullptr ? 1 : tree_rounds(a.rows);  // a chain has one, as have drafts that were not drawn
 }
 
 }  // namespace
 
-size_t draft_verify_workspace(const VerifyArgs& a) { return (size_t)rounds_of(a) * a.rows * kSegments * 8; }
+size_t draft_verify_workspace(const VerifyArgs& a) { return rounds_of(a) > 0 ? Between::bytes(a.rows) : 0; }
 
 void draft_verify(DType dt, const VerifyArgs& a, void* ws, hipStream_t s) {
   const int64_t unit = 16 / (int64_t)dtype_size(dt);
@@ -401,7 +486,7 @@ void draft_verify(DType dt, const VerifyArgs& a, void* ws, hipStream_t s) {
   };
   const bool wide = whole(a.target, a.t_row, a.t_slot) && (a.draft == nullptr || whole(a.draft, a.d_row, a.d_slot));
   const int rounds = rounds_of(a);
-  double* sums = static_cast<double*>(ws);
+  const Between mem(ws, a.rows);
   MRT_DTYPE_DISPATCH(dt, {
     auto go = [&](auto drawn) {
       constexpr bool DRAFT = decltype(drawn)::value;
@@ -411,8 +496,8 @@ void draft_verify(DType dt, const VerifyArgs& a, void* ws, hipStream_t s) {
       const int share = (cut.segments + blocks - 1) / blocks;
       const dim3 grid((cut.segments + share - 1) / share, a.rows);
       for (int r = 0; r < rounds; ++r)
-        hipLaunchKernelGGL((k_verify_pass<T, DRAFT>), grid, dim3(256), 0, s, a, wide, r, share, sums);
-      hipLaunchKernelGGL((k_verify<T, DRAFT>), dim3(a.rows), dim3(64 * kWaves), 0, s, a, wide, rounds, sums);
+        hipLaunchKernelGGL((k_verify_pass<T, DRAFT>), grid, dim3(256), 0, s, a, wide, r, share, mem);
+      hipLaunchKernelGGL((k_verify<T, DRAFT>), dim3(a.rows), dim3(64 * kWaves), 0, s, a, wide, rounds, mem);
     };
     if (a.draft != nullptr) go(std::true_type{});
     else go(std::false_type{});
