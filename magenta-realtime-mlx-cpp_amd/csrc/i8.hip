@@ -6,11 +6,16 @@
 // Few rows (k_i8_few): the weights' bytes bound the product.  A block takes 16 columns, its
 // eight waves 128-deep pieces of k in turn; weights go from memory to the matrix cores
 // through registers, four lanes to 64 bytes of a row, and one exchange between lanes brings
-// them into operand order; the waves' sums meet in LDS.
+// them into operand order; the waves' sums meet in LDS.  2 x 1024 by 5632 takes 3.6 us on the
+// GPU (1.2 at the rate of a large copy), 16 x 8192 by 8192 21 (14).
+//
+// Few tiles (k_i8_cut): as above, tiles of 32 x 32, one for each CU at most.
 //
 // More rows (k_i8_tile): tiles through the LDS ring of ring_gemm.hpp, a k-tile 128 deep, by
 // persistent blocks: the k-tiles of all tiles of a block are one stream, so the next tile's
-// first k-tiles land while this tile's results are stored.
+// first k-tiles land while this tile's results are stored.  8192^3 in bf16 takes 505 us, 2180
+// TOP/s (a library's product 2004), the matrix cores busy for 67 % of the cycles; 4096^3 67.5.
+// 64 x 8192 by 28672, bound by bytes, 54 us, 4.5 TB/s.
 #include <algorithm>
 #include <type_traits>
 
@@ -42,7 +47,8 @@ __device__ __forceinline__ void load16(const T* p, float (&v)[16]) {
 }
 
 // TH threads a row, 16 values of it each at a time; the first HOLD of a thread's pieces stay
-// in registers between the maximum and the codes, longer rows are read again.
+// in registers between the maximum and the codes, longer rows are read again.  Bound by bytes:
+// 8192 x 8192 in bf16 takes 38 us, 5.3 TB/s.
 template <typename T, int TH, int HOLD>
 __global__ __launch_bounds__(256) void k_i8_quantize(const T* src, int64_t ld, int rows, int k, int8_t* codes, int64_t ldc,
                                                      float* scales) {
@@ -96,14 +102,53 @@ __global__ __launch_bounds__(256) void k_i8_quantize(const T* src, int64_t ld, i
 constexpr int kWaves = 8;
 constexpr int kPiece = 128;  // k of a wave at a time
 
+// Four consecutive results of a row: what goes with their sums, requested before those are
+// there.  wide: rows of out (and add) are aligned to four results.
 template <typename T>
-__device__ __forceinline__ float result(const I8Args& a, int sum, float by_row, int64_t row, int col) {
-  const float y = (float)sum * by_row * a.w_scale[col];
-  return a.add != nullptr ? y + St<T>::ld(static_cast<const T*>(a.add)[row * a.lda + col]) : y;
-}
+struct Four {
+  union Packed {
+    T x[4];
+    uint2 w2;
+    uint4 w4;
+  };
+  float by_row, by_col[4];
+  Packed old;
+  __device__ __forceinline__ void request(const I8Args& a, bool wide, int row, int col) {
+    by_row = ld_g(a.x_scale + min(row, a.rows - 1));
+#pragma unroll
+    for (int r = 0; r < 4; ++r) by_col[r] = ld_g(a.w_scale + min(col + r, a.n - 1));
+    if (a.add == nullptr || row >= a.rows || col >= a.n) return;
+    const T* add = static_cast<const T*>(a.add) + row * a.lda + col;
+    if (wide && col + 4 <= a.n) {
+      if constexpr (sizeof(T) == 2) old.w2 = *reinterpret_cast<const uint2*>(add);
+      else old.w4 = *reinterpret_cast<const uint4*>(add);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) old.x[r] = add[min(r, a.n - 1 - col)];
+    }
+  }
+  __device__ __forceinline__ void store(const I8Args& a, bool wide, int row, int col, const i32x4_t& sum) {
+    if (row >= a.rows || col >= a.n) return;
+    T* dst = static_cast<T*>(a.out) + row * a.ldo + col;
+    Packed u;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const float y = (float)sum[r] * by_row * by_col[r];
+      u.x[r] = St<T>::st(a.add != nullptr ? y + St<T>::ld(old.x[r]) : y);
+    }
+    if (wide && col + 4 <= a.n) {
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = u.w2;
+      else *reinterpret_cast<uint4*>(dst) = u.w4;
+    } else {
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (col + r < a.n) dst[r] = u.x[r];
+    }
+  }
+};
 
 template <typename T, int MT>
-__global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a) {
+__global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a, bool wide) {
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
   const int pieces = (a.k + kPiece - 1) / kPiece;
@@ -126,6 +171,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a) {
     }
     return r;
   };
+  const int row = wid * 16 + i, col = n0 + g * 4;  // of the results that this wave stores
+  Four<T> four;
+  if (wid < MT) four.request(a, wide, row, col);
   i32x4_t y[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) y[m] = {0, 0, 0, 0};
@@ -149,16 +197,80 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a) {
   for (int m = 0; m < MT; ++m) sums[wid][m][lane] = y[m];
   __syncthreads();
   if (wid >= MT) return;
-  const int row = wid * 16 + i, col = n0 + g * 4;
   i32x4_t v = sums[0][wid][lane];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) v += sums[w][wid][lane];
-  if (row >= a.rows) return;
-  const float by_row = a.x_scale[row];
-  T* dst = static_cast<T*>(a.out) + row * a.ldo + col;
+  four.store(a, wide, row, col, v);
+}
+
+// ---- tiles cut along k -----------------------------------------------------------------------
+
+// Tiles of 32 x 32 whose k eight waves take in turn, 128 at a time, straight from memory: where
+// tiles are fewer than CUs, a product takes as long as one tile does, and this one's k-tiles are
+// 0.21 us each, those of a 32 x 64 tile through LDS 0.31.  The waves' sums meet in LDS.  More
+// pieces on their way (four) or wider tiles (32 x 64) are slower: 33 x 4096 by 4096 10.4 us, 11.2
+// and 14.5, through LDS 12.9.
+template <typename T>
+__global__ __launch_bounds__(64 * kWaves) void k_i8_cut(const I8Args a, bool wide) {
+  constexpr int MT = 2, NT = 2;
+  const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
+  const int pieces = (a.k + kPiece - 1) / kPiece;
+  __shared__ i32x4_t sums[kWaves][MT * NT][64];
+  const int8_t *wrow[NT], *xrow[MT];
 #pragma unroll
-  for (int r = 0; r < 4; ++r)
-    if (col + r < a.n) dst[r] = St<T>::st(result<T>(a, v[r], by_row, row, col + r));
+  for (int n = 0; n < NT; ++n) wrow[n] = a.w + (int64_t)min(n0 + n * 16 + i, a.n - 1) * a.ldw + g * 16;
+#pragma unroll
+  for (int m = 0; m < MT; ++m) xrow[m] = a.x + (int64_t)min(m0 + m * 16 + i, a.rows - 1) * a.ldx + g * 16;
+  struct Piece {
+    uint4 w[NT][2], x[MT][2];
+  };
+  auto load = [&](int p) {
+    Piece r;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int k = p * kPiece + h * 64;
+      const bool there = k + g * 16 < a.k;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) r.x[m][h] = there ? ld_g16(xrow[m] + k) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NT; ++n) r.w[n][h] = there ? ld_g16(wrow[n] + k) : make_uint4(0, 0, 0, 0);
+    }
+    return r;
+  };
+  static_assert(MT * NT <= kWaves, "a wave stores one tile of 16 x 16");
+  const int row = m0 + wid / NT * 16 + i, col = n0 + wid % NT * 16 + g * 4;
+  Four<T> four;
+  if (wid < MT * NT) four.request(a, wide, row, col);
+  i32x4_t y[MT][NT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) y[m][n] = {0, 0, 0, 0};
+  Piece now = load(wid);
+  for (int p = wid; p < pieces; p += kWaves) {
+    Piece next = now;
+    if (p + kWaves < pieces) next = load(p + kWaves);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+          y[m][n] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4_t, now.w[n][h]),
+                                                          __builtin_bit_cast(i32x4_t, now.x[m][h]), y[m][n], 0, 0, 0);
+    now = next;
+  }
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) sums[wid][m * NT + n][lane] = y[m][n];
+  __syncthreads();
+  i32x4_t v = {0, 0, 0, 0};
+  if (wid >= MT * NT) return;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) v += sums[w][wid][lane];
+  four.store(a, wide, row, col, v);
 }
 
 // ---- tiles -----------------------------------------------------------------------------------
@@ -379,28 +491,33 @@ void launch_tile(const I8Args& a, bool wide, hipStream_t s) {
 }
 
 template <typename T, int MT>
-void launch_few(const I8Args& a, hipStream_t s) {
-  hipLaunchKernelGGL((k_i8_few<T, MT>), dim3((a.n + 15) / 16), dim3(64 * kWaves), 0, s, a);
+void launch_few(const I8Args& a, bool wide, hipStream_t s) {
+  hipLaunchKernelGGL((k_i8_few<T, MT>), dim3((a.n + 15) / 16), dim3(64 * kWaves), 0, s, a, wide);
 }
 
-// Tiles to choose from: us that a k-tile and the rest of a tile take on a full card (from
-// 4096^3 and 2048 x 1024 by 3200).  Measured and chosen (us): 512 x 2816 by 1024 with 256 x 256
-// / 128 x 128 / 64 x 128 / 32 x 64 tiles 32 / 16.6 / 12.0 / 10.0, 2048 x 2816 by 1024 34 / 18.8 /
-// 13.9 / 33, 256 x 4096 by 16384 47 / 25.8 / 31.5 / 82, 4096^3 66.8 / 89 / 117 / 318.
+// Tiles to choose from, the last, k_i8_cut's, where each has a CU of its own: us that a k-tile
+// and the rest of a tile take on a full card (from 4096^3 and 2048 x 1024 by 3200).  Measured and
+// chosen (us): 512 x 2816 by 1024 with 256 x 256 / 128 x 128 / 64 x 128 / 32 x 64 tiles 32 / 16.6 /
+// 12.0 / 10.0, 2048 x 2816 by 1024 34 / 18.8 / 13.9 / 33, 256 x 4096 by 16384 47 / 25.8 / 31.5 /
+// 82, 4096^3 66.8 / 89 / 117 / 318; with 32 x 64 tiles / cut along k 64 x 2816 by 1024 9.7 / 7.3,
+// 64 x 8192 by 2048 21.5 / 16.6.
 struct TileCost {
   int bm, bn;
   double ktile, rest;
 };
 constexpr TileCost kTiles[] = {{256, 256, 1.75, 4.0}, {128, 256, 1.13, 2.3}, {128, 128, 0.70, 1.9},
-                               {64, 128, 0.45, 1.0},  {32, 128, 0.35, 1.0},  {32, 64, 0.31, 0.8}};
+                               {64, 128, 0.45, 1.0},  {32, 128, 0.35, 1.0},  {32, 64, 0.31, 0.8},
+                               {32, 32, 0.21, 1.5}};
+constexpr int kCut = sizeof(kTiles) / sizeof(kTiles[0]) - 1;
 
 int best_tile(const I8Args& a) {
   const int64_t nk = (a.k + 127) / 128, cus = std::max(8, device_cus() & ~7);
   int best = 0;
   double least = 0.;
-  for (int i = 0; i < (int)(sizeof(kTiles) / sizeof(kTiles[0])); ++i) {
+  for (int i = 0; i <= kCut; ++i) {
     const TileCost& t = kTiles[i];
     const int64_t tiles = (int64_t)((a.rows + t.bm - 1) / t.bm) * ((a.n + t.bn - 1) / t.bn);
+    if (i == kCut && tiles > cus) break;
     const double us = (double)((tiles + cus - 1) / cus) * (nk * t.ktile + t.rest);
     if (i == 0 || us < least) best = i, least = us;
   }
@@ -418,9 +535,9 @@ void i8_matmul(DType dt, const I8Args& a, hipStream_t s) {
     // x again (us, k_i8_few / tiles): 2 x 4096 by 4096 7.8 / 12.8, by 16384 19.4 / 14.1; 32 x
     // 4096 by 4096 9.7 / 13.2, by 8192 16.1 / 13.3.
     if (a.rows <= 16 && a.n <= 12288) {
-      launch_few<T, 1>(a, s);
+      launch_few<T, 1>(a, wide, s);
     } else if (a.rows <= 32 && a.n <= 6144) {
-      launch_few<T, 2>(a, s);
+      launch_few<T, 2>(a, wide, s);
     } else {
       switch (best_tile(a)) {
         case 0: launch_tile<T, 256, 256, 2, 4, 2>(a, wide, s); break;
@@ -428,7 +545,9 @@ void i8_matmul(DType dt, const I8Args& a, hipStream_t s) {
         case 2: launch_tile<T, 128, 128, 2, 2, 4>(a, wide, s); break;
         case 3: launch_tile<T, 64, 128, 2, 2, 4>(a, wide, s); break;
         case 4: launch_tile<T, 32, 128, 1, 4, 5>(a, wide, s); break;
-        default: launch_tile<T, 32, 64, 1, 2, 8>(a, wide, s);
+        case 5: launch_tile<T, 32, 64, 1, 2, 8>(a, wide, s); break;
+        default:
+          hipLaunchKernelGGL((k_i8_cut<T>), dim3((a.n + 31) / 32, (a.rows + 31) / 32), dim3(64 * kWaves), 0, s, a, wide);
       }
     }
   });

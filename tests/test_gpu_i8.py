@@ -137,6 +137,7 @@ def test_products_of_quantised_operands(dtype):
     (70, 128, 16385), (4100, 48, 1794), (4096, 384, 1792),                      # 128 x 128
     (4100, 128, 133), (130, 400, 16384), (128, 256, 16384),                     # 64 x 128
     (40, 128, 8198), (40, 1040, 8200), (40, 128, 102), (300, 640, 500),         # 32 rows
+    (40, 1024, 100), (33, 4096, 999), (256, 2832, 1000), (64, 16384, 2000),     # 32 x 32, cut along k
 ])
 def test_one_and_several_tiles_a_block(rows, k, n, aligned, dtype):
     """With and without a residual; results in 16-byte stores or one by one; nothing past the edges."""
