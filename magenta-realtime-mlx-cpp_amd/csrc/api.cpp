@@ -1318,6 +1318,7 @@ int mrt_paged_attention(const mrt_paged_cache* cache, const mrt_paged_attention_
     a.out = to_nodes(args->out, a.dt, c.rows, args->tokens, args->heads, "paged_attention: null out");
     require(Vectors(c.d, {c.rows, a.out.row_stride}, {args->tokens, a.out.node_stride}, {args->heads, a.out.head_stride}).apart(),
             "paged_attention: out overlaps itself");
+    require(a.q.p != a.out.p, "paged_attention: out must be memory of its own");
     require(aligned4({args->fresh, args->lse}), "paged_attention: fresh and lse must be 4-byte aligned");
     a.fresh = args->fresh, a.lse = args->lse, a.bias = args->bias, a.buckets = args->bias ? args->buckets : 0;
     a.tokens = args->tokens, a.heads = args->heads, a.scale = args->scale;

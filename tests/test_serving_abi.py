@@ -62,7 +62,7 @@ def attention(q=P, out=V, qs=(4096, 1024, 64), os=(4096, 1024, 64), fresh=0, lse
 
 BAD_ATTENTION = {
     "null q": dict(q=0), "null out": dict(out=0), "misaligned q": dict(q=P + 4), "stride": dict(qs=(4096, 1020, 64)),
-    "negative stride": dict(os=(4096, 1024, -64)), "overlapping out": dict(os=(4096, 0, 64)), "no tokens": dict(tokens=0),
+    "negative stride": dict(os=(4096, 1024, -64)), "out in place": dict(out=P), "overlapping out": dict(os=(4096, 0, 64)), "no tokens": dict(tokens=0),
     "many tokens": dict(tokens=65), "heads": dict(heads=3), "no heads": dict(heads=0), "bias without buckets": dict(bias=P),
     "too many buckets": dict(bias=P, buckets=(1 << 18) + 1), "misaligned bias": dict(bias=P + 2, buckets=4),
     "large bias": dict(bias=P, heads=1 << 14, buckets=1 << 17), "another dtype": dict(dtype=0), "dtype": dict(dtype=3), "misaligned lse": dict(lse=P + 1), "misaligned fresh": dict(fresh=P + 2),
