@@ -21,6 +21,7 @@
 
 #include "codes8.hpp"
 #include "i8.hpp"
+#include "loose.hpp"
 #include "ring_gemm.hpp"
 
 namespace mrt {
@@ -103,31 +104,30 @@ constexpr int kWaves = 8;
 constexpr int kPiece = 128;  // k of a wave at a time
 
 // Four consecutive results of a row: what goes with their sums, requested before those are
-// there.  wide: rows of out (and add) are aligned to four results.
+// there.
 template <typename T>
 struct Four {
+  typedef Loose<T, sizeof(T)> Mem;
   union Packed {
     T x[4];
-    uint2 w2;
-    uint4 w4;
+    typename Mem::Word w;
   };
   float by_row, by_col[4];
   Packed old;
-  __device__ __forceinline__ void request(const I8Args& a, bool wide, int row, int col) {
+  __device__ __forceinline__ void request(const I8Args& a, int row, int col) {
     by_row = ld_g(a.x_scale + min(row, a.rows - 1));
 #pragma unroll
     for (int r = 0; r < 4; ++r) by_col[r] = ld_g(a.w_scale + min(col + r, a.n - 1));
     if (a.add == nullptr || row >= a.rows || col >= a.n) return;
     const T* add = static_cast<const T*>(a.add) + row * a.lda + col;
-    if (wide && col + 4 <= a.n) {
-      if constexpr (sizeof(T) == 2) old.w2 = *reinterpret_cast<const uint2*>(add);
-      else old.w4 = *reinterpret_cast<const uint4*>(add);
+    if (col + 4 <= a.n) {
+      old.w = Mem::load(add);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r) old.x[r] = add[min(r, a.n - 1 - col)];
     }
   }
-  __device__ __forceinline__ void store(const I8Args& a, bool wide, int row, int col, const i32x4_t& sum) {
+  __device__ __forceinline__ void store(const I8Args& a, int row, int col, const i32x4_t& sum) {
     if (row >= a.rows || col >= a.n) return;
     T* dst = static_cast<T*>(a.out) + row * a.ldo + col;
     Packed u;
@@ -136,9 +136,8 @@ struct Four {
       const float y = (float)sum[r] * by_row * by_col[r];
       u.x[r] = St<T>::st(a.add != nullptr ? y + St<T>::ld(old.x[r]) : y);
     }
-    if (wide && col + 4 <= a.n) {
-      if constexpr (sizeof(T) == 2) *reinterpret_cast<uint2*>(dst) = u.w2;
-      else *reinterpret_cast<uint4*>(dst) = u.w4;
+    if (col + 4 <= a.n) {
+      Mem::store(dst, u.w);
     } else {
 #pragma unroll
       for (int r = 0; r < 4; ++r)
@@ -148,7 +147,7 @@ struct Four {
 };
 
 template <typename T, int MT>
-__global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a, bool wide) {
+__global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a) {
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
   const int pieces = (a.k + kPiece - 1) / kPiece;
@@ -173,7 +172,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a, bool wid
   };
   const int row = wid * 16 + i, col = n0 + g * 4;  // of the results that this wave stores
   Four<T> four;
-  if (wid < MT) four.request(a, wide, row, col);
+  if (wid < MT) four.request(a, row, col);
   i32x4_t y[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) y[m] = {0, 0, 0, 0};
@@ -200,7 +199,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a, bool wid
   i32x4_t v = sums[0][wid][lane];
 #pragma unroll
   for (int w = 1; w < kWaves; ++w) v += sums[w][wid][lane];
-  four.store(a, wide, row, col, v);
+  four.store(a, row, col, v);
 }
 
 // ---- tiles cut along k -----------------------------------------------------------------------
@@ -211,7 +210,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_few(const I8Args a, bool wid
 // pieces on their way (four) or wider tiles (32 x 64) are slower: 33 x 4096 by 4096 10.4 us, 11.2
 // and 14.5, through LDS 12.9.
 template <typename T>
-__global__ __launch_bounds__(64 * kWaves) void k_i8_cut(const I8Args a, bool wide) {
+__global__ __launch_bounds__(64 * kWaves) void k_i8_cut(const I8Args a) {
   constexpr int MT = 2, NT = 2;
   const int tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int i = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16 * NT, m0 = blockIdx.y * 16 * MT;
@@ -241,7 +240,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_cut(const I8Args a, bool wid
   static_assert(MT * NT <= kWaves, "a wave stores one tile of 16 x 16");
   const int row = m0 + wid / NT * 16 + i, col = n0 + wid % NT * 16 + g * 4;
   Four<T> four;
-  if (wid < MT * NT) four.request(a, wide, row, col);
+  if (wid < MT * NT) four.request(a, row, col);
   i32x4_t y[MT][NT];
 #pragma unroll
   for (int m = 0; m < MT; ++m)
@@ -270,7 +269,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_i8_cut(const I8Args a, bool wid
   if (wid >= MT * NT) return;
 #pragma unroll
   for (int w = 0; w < kWaves; ++w) v += sums[w][wid][lane];
-  four.store(a, wide, row, col, v);
+  four.store(a, row, col, v);
 }
 
 // ---- tiles -----------------------------------------------------------------------------------
@@ -297,78 +296,90 @@ __device__ __constant__ uint4 kZeros;  // what k-tiles hold past the end of k
 // Results of a wave's tile, whose first row and column are (mb, nb) in the matrix and (mt, nt)
 // in the block's tile: a lane holds row mb + 32 i + lane % 32 of tile (i, j) and four times
 // four consecutive columns; 16-bit results swap halves between lanes l and l + 32, so that a
-// lane stores 16 bytes.  scale: the block's rows' scales, then its columns'.  wide: rows of out
-// (and add) are 16-byte aligned.
+// lane stores 16 bytes, and what is added comes the same way, requested kAddAhead tiles ahead
+// (in fp32 a second one does not fit the registers).  Rows may begin anywhere: 1000 x 512 by
+// 20001 in bf16 takes 36 us, 68 with results stored one by one; by 20000 26.  scale: the block's
+// rows' scales, then its columns'.
 template <typename T, int BM, int MI, int NJ>
 __device__ __forceinline__ void store_tile(const I8Args& a, const i32x16_t (&acc)[MI][NJ], const float* scale, int mb, int nb,
-                                           int mt, int nt, bool wide) {
+                                           int mt, int nt) {
   constexpr bool k16 = sizeof(T) == 2;
+  constexpr int kAccesses = k16 ? 2 : 4;  // of 16 bytes, a lane and tile
+  constexpr int kAddAhead = k16 ? 2 : 1;
+  typedef Loose<T, 4> Mem;
+  typedef typename Mem::Word Word;
   const int lane = threadIdx.x & 63, lh = lane >> 5;
-  const bool whole = wide && nb + 32 * NJ <= a.n;
-  float by_row[MI];
+  auto column = [&](int h) { return k16 ? 8 * (2 * h + lh) : 8 * h + 4 * lh; };  // of the lane's access h
+  const T* add = static_cast<const T*>(a.add);
+  Word old[kAddAhead][kAccesses];
+  auto request = [&](int x) {  // for tile x % MI, x / MI
+    const int row = min(mb + 32 * (x % MI) + (lane & 31), a.rows - 1), first = nb + 32 * (x / MI);
+    if (first + 32 > a.n) return;
 #pragma unroll
-  for (int i = 0; i < MI; ++i) by_row[i] = scale[mt + 32 * i + (lane & 31)];
+    for (int h = 0; h < kAccesses; ++h) old[x % kAddAhead][h] = Mem::load(add + (int64_t)row * a.lda + first + column(h));
+  };
+  if (add != nullptr) {
 #pragma unroll
-  for (int j = 0; j < NJ; ++j) {
-    float by_col[4][4];
+    for (int x = 0; x < kAddAhead && x < MI * NJ; ++x) request(x);
+  }
+#pragma unroll
+  for (int x = 0; x < MI * NJ; ++x) {
+    const int i = x % MI, j = x / MI;
+    const float by_row = scale[mt + 32 * i + (lane & 31)];
+    float y[4][4];
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
       const float4 v = *reinterpret_cast<const float4*>(scale + BM + nt + 32 * j + 8 * g + 4 * lh);
-      by_col[g][0] = v.x, by_col[g][1] = v.y, by_col[g][2] = v.z, by_col[g][3] = v.w;
+      const float by_col[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r) y[g][r] = (float)acc[i][j][4 * g + r] * by_row * by_col[r];
     }
+    const int row = mb + 32 * i + (lane & 31), first = nb + 32 * j;
+    const bool there = row < a.rows;
+    T* dst = static_cast<T*>(a.out) + (int64_t)row * a.ldo + first;
+    if (first + 32 <= a.n) {
+      if (add != nullptr) {
 #pragma unroll
-    for (int i = 0; i < MI; ++i) {
-      const int row = mb + 32 * i + (lane & 31), first = nb + 32 * j + 4 * lh;
-      const bool there = row < a.rows;
-      const T* add = static_cast<const T*>(a.add) + (int64_t)min(row, a.rows - 1) * a.lda + first;
-      T* dst = static_cast<T*>(a.out) + (int64_t)row * a.ldo + nb + 32 * j;
-      if (whole) {
-        uint32_t w[4][4];  // of group g: the lane's four results, of 16 bits in two words
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float y[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) y[r] = (float)acc[i][j][4 * g + r] * by_row[i] * by_col[g][r];
-          if (a.add != nullptr) {
-            union {
-              uint4 w4;
-              uint2 w2;
-              T x[4];
-            } old;
-            if constexpr (k16) old.w2 = *reinterpret_cast<const uint2*>(add + 8 * g);
-            else old.w4 = *reinterpret_cast<const uint4*>(add + 8 * g);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) y[r] += St<T>::ld(old.x[r]);
-          }
+        for (int h = 0; h < kAccesses; ++h) {
+          const Word w = old[x % kAddAhead][h];
           if constexpr (k16) {
-            w[g][0] = St<T>::bits(y[0]) | (St<T>::bits(y[1]) << 16), w[g][1] = St<T>::bits(y[2]) | (St<T>::bits(y[3]) << 16);
+            const auto s0 = __builtin_amdgcn_permlane32_swap(w[0], w[2], false, false);
+            const auto s1 = __builtin_amdgcn_permlane32_swap(w[1], w[3], false, false);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t p[2] = {s0[e], s1[e]};
+#pragma unroll
+              for (int r = 0; r < 4; ++r) y[2 * h + e][r] += St<T>::unbits((p[r >> 1] >> (16 * (r & 1))) & 0xffffu);
+            }
           } else {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) w[g][r] = __float_as_uint(y[r]);
+            for (int r = 0; r < 4; ++r) y[h][r] += __uint_as_float(w[r]);
           }
         }
-        if constexpr (k16) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const auto s0 = __builtin_amdgcn_permlane32_swap(w[2 * h][0], w[2 * h + 1][0], false, false);
-            const auto s1 = __builtin_amdgcn_permlane32_swap(w[2 * h][1], w[2 * h + 1][1], false, false);
-            if (there) *reinterpret_cast<uint4*>(dst + 8 * (2 * h + lh)) = make_uint4(s0[0], s1[0], s0[1], s1[1]);
-          }
-        } else {
-#pragma unroll
-          for (int g = 0; g < 4; ++g)
-            if (there) *reinterpret_cast<uint4*>(dst + 8 * g + 4 * lh) = make_uint4(w[g][0], w[g][1], w[g][2], w[g][3]);
-        }
-      } else {
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float y = (float)acc[i][j][4 * g + r] * by_row[i] * by_col[g][r];
-            if (there && first + 8 * g + r < a.n)
-              dst[8 * g + 4 * lh + r] = St<T>::st(a.add != nullptr ? y + St<T>::ld(add[8 * g + r]) : y);
-          }
+        if (x + kAddAhead < MI * NJ) request(x + kAddAhead);
       }
+#pragma unroll
+      for (int h = 0; h < kAccesses; ++h) {
+        Word w;
+        if constexpr (k16) {
+          auto pack = [&](int g, int r) { return St<T>::bits(y[g][r]) | (St<T>::bits(y[g][r + 1]) << 16); };
+          const auto s0 = __builtin_amdgcn_permlane32_swap(pack(2 * h, 0), pack(2 * h + 1, 0), false, false);
+          const auto s1 = __builtin_amdgcn_permlane32_swap(pack(2 * h, 2), pack(2 * h + 1, 2), false, false);
+          w = {s0[0], s1[0], s0[1], s1[1]};
+        } else {
+          w = {__float_as_uint(y[h][0]), __float_as_uint(y[h][1]), __float_as_uint(y[h][2]), __float_as_uint(y[h][3])};
+        }
+        if (there) Mem::store(dst + column(h), w);
+      }
+    } else {
+#pragma unroll
+      for (int g = 0; g < 4; ++g)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int col = 8 * g + 4 * lh + r;
+          if (there && first + col < a.n)
+            dst[col] = St<T>::st(add != nullptr ? y[g][r] + St<T>::ld(add[(int64_t)row * a.lda + first + col]) : y[g][r]);
+        }
     }
   }
 }
@@ -377,7 +388,7 @@ __device__ __forceinline__ void store_tile(const I8Args& a, const i32x16_t (&acc
 // and columns past the end are read from the last one and not stored.  TAIL: k is no multiple
 // of a k-tile's depth, and what lies past it is read from kZeros.
 template <typename T, int BM, int BN, int WM, int WN, int S, bool TAIL>
-__global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a, bool wide) {
+__global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a) {
   using Core = Core8;
   using Tile = RingTile<Core, BM, BN, WM, WN, S>;
   static_assert(BM + BN <= Tile::kThreads, "a scale a thread");
@@ -451,7 +462,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a, bool w
   });
   // store instructions of a whole tile's epilogue, 16 bytes each
   constexpr int kStores = Tile::MI * Tile::NJ * (sizeof(T) == 2 ? 2 : 4);
-  bool stored = false;  // the previous tile's epilogue issued exactly those after the ring's loads
+  bool stored = false;  // the previous tile's epilogue issued those, if not more, after the ring's loads
   for (; t < cnt; t += step) {
     int m0, n0;
     origin(t, m0, n0);
@@ -470,29 +481,29 @@ __global__ __launch_bounds__(64 * WM * WN) void k_i8_tile(const I8Args a, bool w
     if (tid < BM + BN) scale[tid] = own;
     ring_barrier();
     const int mt = (wid / WN) * (BM / WM), nt = (wid % WN) * (BN / WN);
-    store_tile<T, BM, Tile::MI, Tile::NJ>(a, s.acc, scale, m0 + mt, n0 + nt, mt, nt, wide);
+    store_tile<T, BM, Tile::MI, Tile::NJ>(a, s.acc, scale, m0 + mt, n0 + nt, mt, nt);
     asm volatile("" ::: "memory");  // the stores stay ahead of the next tile's waits
-    stored = wide && a.add == nullptr && m0 + BM <= a.rows && n0 + BN <= a.n;
+    stored = m0 + BM <= a.rows && n0 + BN <= a.n;
   }
   __builtin_amdgcn_s_waitcnt(vm_wait_imm(0));  // no copy into LDS outlives the block
 }
 
 template <typename T, int BM, int BN, int WM, int WN, int S>
-void launch_tile(const I8Args& a, bool wide, hipStream_t s) {
+void launch_tile(const I8Args& a, hipStream_t s) {
   using Tile = RingTile<Core8, BM, BN, WM, WN, S>;
   const int64_t tiles = (int64_t)((a.rows + BM - 1) / BM) * ((a.n + BN - 1) / BN);
   const int64_t grid = std::min<int64_t>(std::max(8, device_cus() & ~7), (tiles + 7) / 8 * 8);
   auto go = [&](auto kernel) {
     allow_dynamic_lds(reinterpret_cast<const void*>(kernel), Tile::kLds);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(Tile::kThreads), Tile::kLds, s, a, wide);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(Tile::kThreads), Tile::kLds, s, a);
   };
   if (a.k % Core8::kDepth == 0) go(&k_i8_tile<T, BM, BN, WM, WN, S, false>);
   else go(&k_i8_tile<T, BM, BN, WM, WN, S, true>);
 }
 
 template <typename T, int MT>
-void launch_few(const I8Args& a, bool wide, hipStream_t s) {
-  hipLaunchKernelGGL((k_i8_few<T, MT>), dim3((a.n + 15) / 16), dim3(64 * kWaves), 0, s, a, wide);
+void launch_few(const I8Args& a, hipStream_t s) {
+  hipLaunchKernelGGL((k_i8_few<T, MT>), dim3((a.n + 15) / 16), dim3(64 * kWaves), 0, s, a);
 }
 
 // Tiles to choose from, the last, k_i8_cut's, where each has a CU of its own: us that a k-tile
@@ -528,26 +539,23 @@ int best_tile(const I8Args& a) {
 
 void i8_matmul(DType dt, const I8Args& a, hipStream_t s) {
   MRT_DTYPE_DISPATCH(dt, {
-    const int64_t unit = 16 / (int64_t)sizeof(T);
-    const bool wide = reinterpret_cast<uintptr_t>(a.out) % 16 == 0 && a.ldo % unit == 0 &&
-                      (a.add == nullptr || (reinterpret_cast<uintptr_t>(a.add) % 16 == 0 && a.lda % unit == 0));
     // Few columns give too few tiles to keep the card's loads out, many blocks of k_i8_few read
     // x again (us, k_i8_few / tiles): 2 x 4096 by 4096 7.8 / 12.8, by 16384 19.4 / 14.1; 32 x
     // 4096 by 4096 9.7 / 13.2, by 8192 16.1 / 13.3.
     if (a.rows <= 16 && a.n <= 12288) {
-      launch_few<T, 1>(a, wide, s);
+      launch_few<T, 1>(a, s);
     } else if (a.rows <= 32 && a.n <= 6144) {
-      launch_few<T, 2>(a, wide, s);
+      launch_few<T, 2>(a, s);
     } else {
       switch (best_tile(a)) {
-        case 0: launch_tile<T, 256, 256, 2, 4, 2>(a, wide, s); break;
-        case 1: launch_tile<T, 128, 256, 2, 4, 3>(a, wide, s); break;
-        case 2: launch_tile<T, 128, 128, 2, 2, 4>(a, wide, s); break;
-        case 3: launch_tile<T, 64, 128, 2, 2, 4>(a, wide, s); break;
-        case 4: launch_tile<T, 32, 128, 1, 4, 5>(a, wide, s); break;
-        case 5: launch_tile<T, 32, 64, 1, 2, 8>(a, wide, s); break;
+        case 0: launch_tile<T, 256, 256, 2, 4, 2>(a, s); break;
+        case 1: launch_tile<T, 128, 256, 2, 4, 3>(a, s); break;
+        case 2: launch_tile<T, 128, 128, 2, 2, 4>(a, s); break;
+        case 3: launch_tile<T, 64, 128, 2, 2, 4>(a, s); break;
+        case 4: launch_tile<T, 32, 128, 1, 4, 5>(a, s); break;
+        case 5: launch_tile<T, 32, 64, 1, 2, 8>(a, s); break;
         default:
-          hipLaunchKernelGGL((k_i8_cut<T>), dim3((a.n + 31) / 32, (a.rows + 31) / 32), dim3(64 * kWaves), 0, s, a, wide);
+          hipLaunchKernelGGL((k_i8_cut<T>), dim3((a.n + 31) / 32, (a.rows + 31) / 32), dim3(64 * kWaves), 0, s, a);
       }
     }
   });

@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "device_utils.hpp"
+#include "loose.hpp"
 #include "verify.hpp"
 
 namespace mrt {
@@ -47,16 +48,20 @@ __device__ __forceinline__ float counted(float p) {
   return __builtin_amdgcn_classf(p, 0x180) ? p : 0.f;  // positive, normal or not
 }
 
-// VEC consecutive probabilities; 0 past the end.
+// VEC consecutive probabilities; 0 past the end.  Rows may begin anywhere.
 template <typename T, int VEC>
-__device__ __forceinline__ uint4 load_raw(const T* row, int at, int V, bool wide) {
-  if (wide && at + VEC <= V) return ld_g16(row + at);
+__device__ __forceinline__ uint4 load_raw(const T* row, int at, int V) {
   union {
     T x[VEC];
     uint4 w;
+    typename Loose<T, 4>::Word v;
   } u;
+  if (at + VEC <= V) {
+    u.v = Loose<T, 4>::load(row + at);
+  } else {
 #pragma unroll
-  for (int e = 0; e < VEC; ++e) u.x[e] = at + e < V ? ld_g(row + at + e) : T(0);
+    for (int e = 0; e < VEC; ++e) u.x[e] = at + e < V ? ld_g(row + at + e) : T(0);
+  }
   return u.w;
 }
 template <typename T, int VEC>
@@ -162,7 +167,7 @@ __device__ __forceinline__ Nodes gather(const VerifyArgs& a, int b, int lane) {
 // Sums of r after n rejections at slot `at`, of the segments first, first + W, .. below
 // `last`, by W waves: put(segment, sum).
 template <typename T, bool DRAFT, int W, int M, class Put>
-__device__ __forceinline__ void sum_segments_of(const VerifyArgs& a, const Cut<T>& cut, bool wide, int b, int at, int n,
+__device__ __forceinline__ void sum_segments_of(const VerifyArgs& a, const Cut<T>& cut, int b, int at, int n,
                                                 const Rejections& rej, int first, int last, Put&& put) {
   constexpr int VEC = Cut<T>::VEC, CHUNK = Cut<T>::CHUNK;
   const int lane = threadIdx.x & 63, wid = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -176,8 +181,8 @@ __device__ __forceinline__ void sum_segments_of(const VerifyArgs& a, const Cut<T
   uint4 pr[kAhead], qr[kAhead];
   auto load = [&](int k, int j) {
     const int x = chunk_of(min(k, mine - 1)) * CHUNK + lane * VEC;
-    pr[j] = load_raw<T, VEC>(p, x, a.vocab, wide);
-    if constexpr (both) qr[j] = load_raw<T, VEC>(q, x, a.vocab, wide);
+    pr[j] = load_raw<T, VEC>(p, x, a.vocab);
+    if constexpr (both) qr[j] = load_raw<T, VEC>(q, x, a.vocab);
   };
   if (mine > 0) {
 #pragma unroll
@@ -206,11 +211,11 @@ __device__ __forceinline__ void sum_segments_of(const VerifyArgs& a, const Cut<T
 }
 
 template <typename T, bool DRAFT, int W, class Put>
-__device__ __forceinline__ void sum_segments(const VerifyArgs& a, const Cut<T>& cut, bool wide, int b, int at, int n,
+__device__ __forceinline__ void sum_segments(const VerifyArgs& a, const Cut<T>& cut, int b, int at, int n,
                                              const Rejections& rej, int first, int last, Put&& put) {
-  if (n == 0) sum_segments_of<T, DRAFT, W, 0>(a, cut, wide, b, at, n, rej, first, last, put);
-  else if (n <= 2) sum_segments_of<T, DRAFT, W, 2>(a, cut, wide, b, at, n, rej, first, last, put);
-  else sum_segments_of<T, DRAFT, W, -1>(a, cut, wide, b, at, n, rej, first, last, put);
+  if (n == 0) sum_segments_of<T, DRAFT, W, 0>(a, cut, b, at, n, rej, first, last, put);
+  else if (n <= 2) sum_segments_of<T, DRAFT, W, 2>(a, cut, b, at, n, rej, first, last, put);
+  else sum_segments_of<T, DRAFT, W, -1>(a, cut, b, at, n, rej, first, last, put);
 }
 
 // s.seg from the segments' sums to running ones, and s.total; by the whole block.
@@ -348,7 +353,7 @@ struct Between {
 
 // Launch `round` of passes: block (x, b) sums segments x share .. of sequence b.
 template <typename T, bool DRAFT>
-__global__ __launch_bounds__(256) void k_verify_pass(const VerifyArgs a, bool wide, int round, int share, const Between mem) {
+__global__ __launch_bounds__(256) void k_verify_pass(const VerifyArgs a, int round, int share, const Between mem) {
   const Cut<T> cut(a.vocab);
   const int b = blockIdx.y, first = blockIdx.x * share, last = min(first + share, cut.segments);
   const int tid = threadIdx.x, lane = tid & 63;
@@ -377,12 +382,12 @@ __global__ __launch_bounds__(256) void k_verify_pass(const VerifyArgs a, bool wi
   }
   if (ended) return;
   double* to = mem.sums_of(round, a.rows, b);
-  sum_segments<T, DRAFT, 4>(a, cut, wide, b, walk.here, walk.n, walk.rej, first, last, [&](int x, double v) { to[x] = v; });
+  sum_segments<T, DRAFT, 4>(a, cut, b, walk.here, walk.n, walk.rej, first, last, [&](int x, double v) { to[x] = v; });
 }
 
 // The rest, a block a sequence, after `rounds` launches of passes.
 template <typename T, bool DRAFT>
-__global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool wide, int rounds, const Between mem) {
+__global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, int rounds, const Between mem) {
   constexpr int VEC = Cut<T>::VEC, CHUNK = Cut<T>::CHUNK;
   const Cut<T> cut(a.vocab);
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wid = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -404,7 +409,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool
   }
   while (!ended) {
     __syncthreads();  // the pass before has been read
-    sum_segments<T, DRAFT, kWaves>(a, cut, wide, b, walk.here, walk.n, walk.rej, 0, segments, [&](int x, double v) { s.seg[x] = v; });
+    sum_segments<T, DRAFT, kWaves>(a, cut, b, walk.here, walk.n, walk.rej, 0, segments, [&](int x, double v) { s.seg[x] = v; });
     run_sums(s, segments);
     ended = walk.go<DRAFT>(node, lane, s.total);
   }
@@ -432,8 +437,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_verify(const VerifyArgs a, bool
   for (; c < end && sum > 0.0; ++c) {
     const int at = c * CHUNK + lane * VEC;
     float pv[VEC], qv[VEC];
-    unpack<T, VEC>(load_raw<T, VEC>(p, at, V, wide), pv);
-    if (both) unpack<T, VEC>(load_raw<T, VEC>(q, at, V, wide), qv);
+    unpack<T, VEC>(load_raw<T, VEC>(p, at, V), pv);
+    if (both) unpack<T, VEC>(load_raw<T, VEC>(q, at, V), qv);
     double v[VEC], run = 0.0;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) {
@@ -480,11 +485,6 @@ int rounds_of(const VerifyArgs& a) {
 size_t draft_verify_workspace(const VerifyArgs& a) { return rounds_of(a) > 0 ? Between::bytes(a.rows) : 0; }
 
 void draft_verify(DType dt, const VerifyArgs& a, void* ws, hipStream_t s) {
-  const int64_t unit = 16 / (int64_t)dtype_size(dt);
-  auto whole = [&](const void* p, int64_t row, int64_t slot) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && row % unit == 0 && slot % unit == 0;
-  };
-  const bool wide = whole(a.target, a.t_row, a.t_slot) && (a.draft == nullptr || whole(a.draft, a.d_row, a.d_slot));
   const int rounds = rounds_of(a);
   const Between mem(ws, a.rows);
   MRT_DTYPE_DISPATCH(dt, {
@@ -496,8 +496,8 @@ void draft_verify(DType dt, const VerifyArgs& a, void* ws, hipStream_t s) {
       const int share = (cut.segments + blocks - 1) / blocks;
       const dim3 grid((cut.segments + share - 1) / share, a.rows);
       for (int r = 0; r < rounds; ++r)
-        hipLaunchKernelGGL((k_verify_pass<T, DRAFT>), grid, dim3(256), 0, s, a, wide, r, share, mem);
-      hipLaunchKernelGGL((k_verify<T, DRAFT>), dim3(a.rows), dim3(64 * kWaves), 0, s, a, wide, rounds, mem);
+        hipLaunchKernelGGL((k_verify_pass<T, DRAFT>), grid, dim3(256), 0, s, a, r, share, mem);
+      hipLaunchKernelGGL((k_verify<T, DRAFT>), dim3(a.rows), dim3(64 * kWaves), 0, s, a, rounds, mem);
     };
     if (a.draft != nullptr) go(std::true_type{});
     else go(std::false_type{});
