@@ -1603,11 +1603,12 @@ def draft_verify(target, draft, tokens, uniforms, parents=None):
 def i8_quantize(x):
     """8-bit codes of the rows of x (rows, k), k a multiple of 16 (mrt_i8_quantize): (int8 (rows, k), fp32 scales (rows))."""
     lib, index, kind, shape = load_library(), x.get_device(), _KIND[x.dtype], x.shape
-    if len(shape) != 2 or index < 0 or x.stride(1) != 1 or not 0 <= kind < PAGES_I8:
+    stride = x.stride()
+    if len(shape) != 2 or index < 0 or stride[1] != 1 or not 0 <= kind < PAGES_I8:
         raise ValueError("x must be (rows, k) fp32, bf16 or fp16 on a GPU, rows contiguous")
     rows, k = shape
     codes, scales = x.new_empty(shape, dtype=_KIND.i8), x.new_empty(rows, dtype=_KIND.f32)
-    code = lib.mrt_i8_quantize(x.data_ptr(), x.stride(0), rows, k, kind, codes.data_ptr(), k, scales.data_ptr(), index,
+    code = lib.mrt_i8_quantize(x.data_ptr(), stride[0], rows, k, kind, codes.data_ptr(), k, scales.data_ptr(), index,
                                _KIND.stream(index))
     if code:
         _check(lib, code)
@@ -1624,23 +1625,25 @@ def i8_matmul(x, x_scale, w, w_scale, dtype=None, add=None, out=None):
     lib, index, shape, (n, k) = load_library(), x.get_device(), x.shape, w.shape
     if len(shape) != 2 or shape[1] != k or _KIND[x.dtype] != PAGES_I8 or _KIND[w.dtype] != PAGES_I8:
         raise ValueError("x and w must be int8 (rows, k) and (n, k)")
-    if index < 0 or w.get_device() != index or x.stride(1) != 1 or w.stride(1) != 1:
+    (ldx, xs), (ldw, ws) = x.stride(), w.stride()
+    if index < 0 or w.get_device() != index or xs != 1 or ws != 1:
         raise ValueError("x and w must be on one GPU, rows contiguous")
     if dtype is None:
         dtype = out.dtype if out is not None else add.dtype if add is not None else _KIND.bf16
-    kind, rows = _KIND[dtype], shape[0]
+    rows, ap, lda, ldo = shape[0], 0, 0, n
     if out is None:
         out = x.new_empty((rows, n), dtype=dtype)
-    elif out.shape != (rows, n) or out.dtype is not dtype or out.get_device() != index or out.stride(1) != 1:
-        raise ValueError("out must be (rows, n) in dtype, on x's GPU, rows contiguous")
-    ap = lda = 0
+    else:
+        if out.shape != (rows, n) or out.dtype is not dtype or out.get_device() != index or out.stride(1) != 1:
+            raise ValueError("out must be (rows, n) in dtype, on x's GPU, rows contiguous")
+        ldo = out.stride(0)
     if add is not None:
         if add.shape != (rows, n) or add.dtype is not dtype or add.get_device() != index or add.stride(1) != 1:
             raise ValueError("add must be (rows, n) in dtype, on x's GPU, rows contiguous")
         ap, lda = add.data_ptr(), add.stride(0)
     args = _I8_STRUCT.pack(x.data_ptr(), _array(x_scale, shape[:1], DTYPE_F32, index, "x_scale"), w.data_ptr(),
-                           _array(w_scale, (n,), DTYPE_F32, index, "w_scale"), ap, out.data_ptr(), x.stride(0), w.stride(0), lda,
-                           out.stride(0), rows, n, k, kind)
+                           _array(w_scale, (n,), DTYPE_F32, index, "w_scale"), ap, out.data_ptr(), ldx, ldw, lda, ldo, rows, n, k,
+                           _KIND[dtype])
     code = lib.mrt_i8_matmul(args, index, _KIND.stream(index))
     if code:
         _check(lib, code)
