@@ -912,8 +912,9 @@ typedef struct mrt_i8_matmul_args {
 } mrt_i8_matmul_args;
 
 /* out = (x w^T) x_scale w_scale + add: a scale for each row and each column.  The
- * products are summed exactly; the sum is rounded to fp32, scaled and added to in
- * fp32, and rounded to `dtype`.  rows is below 2^24, k a multiple of 16, below 2^17; ldx and ldw are
+ * products are summed exactly; the sum is rounded to fp32, multiplied by x_scale, then
+ * by w_scale, and added to, each step rounded to fp32, and rounded to `dtype`: a row's
+ * bits do not depend on the others.  rows is below 2^24, k a multiple of 16, below 2^17; ldx and ldw are
  * multiples of 16 below 2^24, x and w 16-byte aligned. */
 int mrt_i8_matmul(const mrt_i8_matmul_args* args, int device, void* hip_stream);
 

@@ -1,7 +1,8 @@
 // Products in 8-bit integers with a scale for each row (token) and each column (channel):
 //   out[m][n] = x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + add[m][n].
 // The sums are whole numbers, exact in 32 bits below k = 2^17 (a term is at most 2^14), so
-// how they are cut and ordered changes no bit of a result.
+// how they are cut and ordered changes no bit of a result; a sum is rounded to fp32, and each of
+// the two products and the addition by itself, in every kernel.
 //
 // Few rows (k_i8_few): the weights' bytes bound the product.  A block takes 16 columns, its
 // eight waves 128-deep pieces of k in turn; weights go from memory to the matrix cores
@@ -127,7 +128,10 @@ struct Four {
       for (int r = 0; r < 4; ++r) old.x[r] = add[min(r, a.n - 1 - col)];
     }
   }
+  // Scaled and added to step by step, as store_tile does, never in one fused step: which kernel
+  // a batch leads to changes no bit of a row.
   __device__ __forceinline__ void store(const I8Args& a, int row, int col, const i32x4_t& sum) {
+#pragma clang fp contract(off)
     if (row >= a.rows || col >= a.n) return;
     T* dst = static_cast<T*>(a.out) + row * a.ldo + col;
     Packed u;
@@ -303,6 +307,7 @@ __device__ __constant__ uint4 kZeros;  // what k-tiles hold past the end of k
 template <typename T, int BM, int MI, int NJ>
 __device__ __forceinline__ void store_tile(const I8Args& a, const i32x16_t (&acc)[MI][NJ], const float* scale, int mb, int nb,
                                            int mt, int nt) {
+#pragma clang fp contract(off)
   constexpr bool k16 = sizeof(T) == 2;
   constexpr int kAccesses = k16 ? 2 : 4;  // of 16 bytes, a lane and tile
   constexpr int kAddAhead = k16 ? 2 : 1;
