@@ -218,7 +218,11 @@ __device__ __forceinline__ void sum_segments(const VerifyArgs& a, const Cut<T>& 
   else sum_segments_of<T, DRAFT, W, -1>(a, cut, b, at, n, rej, first, last, put);
 }
 
-// s.seg from the segments' sums to running ones, and s.total; by the whole block.
+// s.seg from the segments' sums to running ones, and s.total; by the whole block.  Running
+// sums never fall, a segment without weight adds nothing to them, and the last one is the total,
+// whatever the roundings: at each level of the scan the right half's lanes add the left half's
+// last sum to their own, and a lane's last segment takes the lane's sum itself.  So the first
+// that exceeds a threshold is of a segment with weight, and none exceeds the total.
 __device__ __forceinline__ void run_sums(Sums& s, int segments) {
   const int lane = threadIdx.x & 63;
   __syncthreads();
@@ -232,14 +236,14 @@ __device__ __forceinline__ void run_sums(Sums& s, int segments) {
     double incl = run;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const double y = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += y;
+      const double y = __shfl(incl, (lane & -o) - 1, 64);  // of the right half's lanes: the left half's last
+      if (lane & o) incl += y;
     }
     double before = __shfl_up(incl, 1, 64);
     if (lane == 0) before = 0.0;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      if (lane * 4 + k < segments) s.seg[lane * 4 + k] = before + v[k];
+      if (lane * 4 + k < segments) s.seg[lane * 4 + k] = v[k] == run ? incl : fmin(before + v[k], incl);
     if (lane == 63) s.total = incl;
   }
   __syncthreads();
