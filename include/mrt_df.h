@@ -822,7 +822,8 @@ int mrt_paged_read(const mrt_paged_cache* cache, const mrt_paged_store_args* arg
 
 typedef struct mrt_paged_attention_args {
   mrt_node_rows q;       /* (rows, tokens, heads, d) of `dtype` */
-  mrt_node_rows out;     /* the same, memory of its own: several blocks read a row of q */
+  mrt_node_rows out;     /* the same, memory of its own: several blocks read a row of q.  Laid out */
+                         /*   alike the two may lie between each other, else their ranges are apart */
   const int32_t* fresh;  /* (rows) new tokens that are there; NULL: all */
   float* lse;            /* (rows, tokens, heads) fp32 log-sum-exp of the logits, or NULL */
   const float* bias;     /* (heads, buckets) fp32 logit bias by distance, or NULL */

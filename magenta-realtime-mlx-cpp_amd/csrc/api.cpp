@@ -276,6 +276,17 @@ struct Vectors {
     }
     return true;
   }
+  // Elements from the first to the last.
+  __int128 extent() const {
+    __int128 n = d;
+    for (const Dim& x : dims) n += static_cast<__int128>(x.size - 1) * x.stride;
+    return n;
+  }
+  bool alike(const Vectors& y) const {
+    bool same = d == y.d;
+    for (int i = 0; i < 3; ++i) same = same && dims[i].size == y.dims[i].size && dims[i].stride == y.dims[i].stride;
+    return same;
+  }
   // Whether one of these vectors shares elements with one of the same array `by` elements on.
   bool meets(__int128 by, int i = 0) const {
     if (i == 3) return by > -d && by < d;
@@ -285,6 +296,21 @@ struct Vectors {
     return false;
   }
 };
+
+// Whether [p, p + n) and [q, q + m) (bytes) meet.
+bool ranges_meet(const void* p, __int128 n, const void* q, __int128 m) {
+  const __int128 a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+  return a < b + m && b < a + n;
+}
+
+// Whether x at px and y at py, of elements of `size` bytes, share memory.  Laid out alike, and
+// each apart in itself, they may lie between each other; else their whole ranges count.
+bool share(const Vectors& x, const void* px, const Vectors& y, const void* py, size_t size) {
+  const __int128 e = static_cast<__int128>(size);
+  if (!ranges_meet(px, x.extent() * e, py, y.extent() * e)) return false;
+  const __int128 by = static_cast<__int128>(reinterpret_cast<uintptr_t>(py)) - reinterpret_cast<uintptr_t>(px);
+  return !x.alike(y) || by % e != 0 || x.meets(by / e);
+}
 
 // Of a cache that is written.
 void check_own_slots(const mrt::KvCache& c) {
@@ -1316,9 +1342,16 @@ int mrt_paged_attention(const mrt_paged_cache* cache, const mrt_paged_attention_
     a.dt = operand_type(c, args->dtype);
     a.q = to_nodes(args->q, a.dt, c.rows, args->tokens, args->heads, "paged_attention: null q");
     a.out = to_nodes(args->out, a.dt, c.rows, args->tokens, args->heads, "paged_attention: null out");
-    require(Vectors(c.d, {c.rows, a.out.row_stride}, {args->tokens, a.out.node_stride}, {args->heads, a.out.head_stride}).apart(),
-            "paged_attention: out overlaps itself");
-    require(a.q.p != a.out.p, "paged_attention: out must be memory of its own");
+    auto vectors = [&](const mrt::NodeRows& r) {
+      return Vectors(c.d, {c.rows, r.row_stride}, {args->tokens, r.node_stride}, {args->heads, r.head_stride});
+    };
+    const Vectors q = vectors(a.q), out = vectors(a.out);
+    const size_t size = mrt::dtype_size(a.dt);
+    require(out.apart(), "paged_attention: out overlaps itself");
+    require(!share(q, a.q.p, out, a.out.p, size), "paged_attention: out must be memory of its own");
+    require(args->lse == nullptr || !ranges_meet(args->lse, static_cast<__int128>(c.rows) * args->tokens * args->heads * 4, a.out.p,
+                                                 out.extent() * static_cast<__int128>(size)),
+            "paged_attention: lse overlaps out");
     require(aligned4({args->fresh, args->lse}), "paged_attention: fresh and lse must be 4-byte aligned");
     a.fresh = args->fresh, a.lse = args->lse, a.bias = args->bias, a.buckets = args->bias ? args->buckets : 0;
     a.tokens = args->tokens, a.heads = args->heads, a.scale = args->scale;

@@ -1,0 +1,57 @@
+"""Outputs of a server's operators that overlap in part, at an offset: refused without a GPU, each with
+its own message; operands that only lie between each other's rows are not."""
+
+from __future__ import annotations
+
+import pytest
+
+import mrt_df
+from test_serving_abi import INVALID, P, V, attention, pages
+
+pytestmark = pytest.mark.filterwarnings("ignore")
+
+
+@pytest.fixture(scope="module")
+def lib():
+    return mrt_df.load_library()
+
+
+def says(lib, code, text):
+    return code == INVALID and text in lib.mrt_last_error().decode()
+
+
+# q (2, 4, 4, 64) bf16 at P, rows of 4 x 1024 elements
+OUTS = {
+    "a head on": dict(out=P + 128), "a token on": dict(out=P + 2048), "a row on": dict(out=P + 8192),
+    "a token before": dict(out=P + 65536 - 2048, q=P + 65536),
+    "the last vector": dict(out=P + 2 * (4096 + 3 * 1024 + 3 * 64)),
+    "another layout": dict(out=P + 2048, os=(1024, 256, 64)),
+    "heads first": dict(out=P + 16, os=(1024, 64, 256)),
+    "one q for all": dict(out=P + 64, qs=(0, 0, 64)),
+}
+APART = {
+    "behind it": dict(out=P + 2 * 8192), "right before it": dict(q=P + 16384, out=P),
+    "heads side by side": dict(qs=(4096, 1024, 128), os=(4096, 1024, 128), out=P + 128),
+    "in one product's rows": dict(out=P + 512),
+    "another layout behind it": dict(out=P + 2 * 8192, os=(1024, 64, 256)),
+}
+
+
+def paged(lib, **kw):
+    return lib.mrt_paged_attention(pages(), attention(**dict(dict(lse=0), **kw)), None, 0, 0, None)
+
+
+@pytest.mark.parametrize("case", OUTS)
+def test_attention_out_of_q(lib, case):
+    assert says(lib, paged(lib, **OUTS[case]), "memory of its own")
+
+
+@pytest.mark.parametrize("case", APART)
+def test_attention_beside_q(lib, case):
+    """Gets past the checks of q and out, to the last of all: a bias with no table."""
+    assert says(lib, paged(lib, fresh=P + 2, **APART[case]), "fresh and lse must be 4-byte aligned")
+
+
+def test_attention_lse(lib):
+    assert says(lib, paged(lib, lse=V + 4), "lse overlaps out")
+    assert says(lib, paged(lib, lse=V - 4), "lse overlaps out")
