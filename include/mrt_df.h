@@ -801,8 +801,8 @@ typedef struct mrt_paged_cache {
 } mrt_paged_cache;
 
 typedef struct mrt_paged_store_args {
-  mrt_node_rows k;       /* (rows, tokens, kv_heads, d) of `dtype`; written by mrt_paged_read */
-  mrt_node_rows v;
+  mrt_node_rows k;       /* (rows, tokens, kv_heads, d) of `dtype`; written by mrt_paged_read: */
+  mrt_node_rows v;       /*   laid out alike they may lie between each other, else their ranges are apart */
   const int32_t* fresh;  /* write: (rows) tokens that are there, 0 .. tokens; NULL: all */
   const int32_t* start;  /* read: (rows) the first entry; NULL: 0 */
   int32_t* length_out;   /* write: (rows), an array of its own, or NULL */

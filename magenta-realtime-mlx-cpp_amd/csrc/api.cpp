@@ -396,14 +396,9 @@ mrt::PagedStoreArgs to_store(const mrt::PagedCache& c, const mrt_paged_store_arg
   return a;
 }
 
-// Two arrays of vectors that are written: neither overlaps itself, nor, where they are
-// laid out alike, the other.
+// Two arrays of vectors that are written: neither overlaps itself or the other.
 void check_apart(const Vectors& x, const Vectors& y, const void* px, const void* py, size_t size, const char* msg) {
-  require(x.apart() && y.apart(), msg);
-  bool alike = true;
-  for (int i = 0; i < 3; ++i) alike = alike && x.dims[i].size == y.dims[i].size && x.dims[i].stride == y.dims[i].stride;
-  const __int128 bytes = static_cast<__int128>(reinterpret_cast<uintptr_t>(py)) - reinterpret_cast<uintptr_t>(px);
-  require(alike ? !x.meets(bytes / static_cast<int64_t>(size)) : px != py, msg);
+  require(x.apart() && y.apart() && !share(x, px, y, py, size), msg);
 }
 
 constexpr char kPagedTooLarge[] = "paged_attention: too many sequences, heads and tokens for one call";

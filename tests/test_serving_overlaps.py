@@ -55,3 +55,14 @@ def test_attention_beside_q(lib, case):
 def test_attention_lse(lib):
     assert says(lib, paged(lib, lse=V + 4), "lse overlaps out")
     assert says(lib, paged(lib, lse=V - 4), "lse overlaps out")
+
+
+# k and v (2, 2, 2, 64) bf16 of paged_read: rows of 1024, tokens of 512, heads of 128 elements
+
+def store_of(k=P, v=V, kst=(1024, 512, 128), vst=(1024, 512, 128), start=0):
+    return mrt_df._STORE_STRUCT.pack(k, *kst, v, *vst, 0, start, 0, 2, 1)
+
+
+def test_read_into_rows_laid_out_otherwise(lib):
+    for kw in (dict(v=P + 256, vst=(1024, 256, 512)), dict(v=P + 1024, vst=(512, 256, 64)), dict(k=P + 2048, v=P, vst=(2048, 1024, 64))):
+        assert says(lib, lib.mrt_paged_read(pages(), store_of(**kw), 0, None), "overlaps itself or the other")
