@@ -1288,11 +1288,13 @@ int mrt_paged_write(const mrt_paged_cache* cache, const mrt_paged_store_args* ar
     const mrt::PagedCache c = to_pages(cache);
     if (c.rows == 0) return;
     const mrt::PagedStoreArgs a = to_store(c, args);
-    require(a.length_out == nullptr || (a.length_out != c.length && a.length_out != a.fresh),
+    const __int128 counts = static_cast<__int128>(c.rows) * 4, scales = static_cast<__int128>(c.pages) * c.kv_heads * c.page_size * 4;
+    require(a.length_out == nullptr || (!ranges_meet(a.length_out, counts, c.length, counts) &&
+                                        (a.fresh == nullptr || !ranges_meet(a.length_out, counts, a.fresh, counts))),
             "paged_write: length_out must be an array of its own");
     const Vectors slots(c.d, {c.pages, c.page_stride}, {c.kv_heads, c.head_stride}, {c.page_size, c.slot_stride});
     check_apart(slots, slots, c.k, c.v, c.codes ? 1 : mrt::dtype_size(c.dt), "pages: pages, heads, slots or k and v overlap");
-    require(!c.codes || c.k_scale != c.v_scale, "pages: k_scale and v_scale overlap");
+    require(!c.codes || !ranges_meet(c.k_scale, scales, c.v_scale, scales), "pages: k_scale and v_scale overlap");
     OnDevice on(device);
     mrt::paged_write(c, a, static_cast<hipStream_t>(hip_stream));
   });

@@ -66,3 +66,19 @@ def store_of(k=P, v=V, kst=(1024, 512, 128), vst=(1024, 512, 128), start=0):
 def test_read_into_rows_laid_out_otherwise(lib):
     for kw in (dict(v=P + 256, vst=(1024, 256, 512)), dict(v=P + 1024, vst=(512, 256, 64)), dict(k=P + 2048, v=P, vst=(2048, 1024, 64))):
         assert says(lib, lib.mrt_paged_read(pages(), store_of(**kw), 0, None), "overlaps itself or the other")
+
+
+def test_written_lengths(lib):
+    """length_out (2) int32 against the lengths and counts that other blocks read."""
+    def write(length=P, fresh=0, out=0):
+        return lib.mrt_paged_write(pages(length=length), store_of(k=V, v=V + (1 << 20))[:64] +
+                                   mrt_df.struct.pack("PPPii", fresh, 0, out, 2, 1), 0, None)
+    for kw in (dict(out=P + 4), dict(out=P - 4), dict(out=P), dict(out=V + 4, fresh=V), dict(out=V - 4, fresh=V)):
+        assert says(lib, write(**kw), "array of its own")
+
+
+def test_written_scales(lib):
+    """(8, 2, 16) fp32 each."""
+    for vs in (P + 16, P - 16, P + 1024 - 16):
+        c = pages(dtype=3, ks=P, vs=vs, k=V, v=V + (1 << 20))
+        assert says(lib, lib.mrt_paged_write(c, store_of(), 0, None), "k_scale and v_scale overlap")
