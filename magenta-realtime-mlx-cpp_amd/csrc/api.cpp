@@ -1379,7 +1379,9 @@ int mrt_draft_verify(const mrt_draft_verify_args* args, void* workspace, size_t 
     require(aligned(a.target, size) && aligned(a.draft, size), "draft_verify: target and draft must be aligned to their elements");
     require(aligned4({a.tokens, a.parents, a.uniforms, a.accepted, a.count, a.token}),
             "draft_verify: int32 and fp32 arrays must be 4-byte aligned");
-    require(a.accepted != a.count && a.accepted != a.token && a.count != a.token,
+    const int64_t counts = static_cast<int64_t>(a.rows) * 4, paths = counts * a.nodes;
+    require(!ranges_meet(a.accepted, paths, a.count, counts) && !ranges_meet(a.accepted, paths, a.token, counts) &&
+                !ranges_meet(a.count, counts, a.token, counts),
             "draft_verify: outputs must be arrays of their own");
     const size_t want = mrt::draft_verify_workspace(a);
     require(want == 0 || (workspace != nullptr && workspace_bytes >= want && aligned(workspace, 16)),

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 
 import mrt_df
-from test_serving_abi import INVALID, P, V, attention, pages
+from test_serving_abi import INVALID, P, V, attention, pages, product, verify
 
 pytestmark = pytest.mark.filterwarnings("ignore")
 
@@ -82,3 +82,10 @@ def test_written_scales(lib):
     for vs in (P + 16, P - 16, P + 1024 - 16):
         c = pages(dtype=3, ks=P, vs=vs, k=V, v=V + (1 << 20))
         assert says(lib, lib.mrt_paged_write(c, store_of(), 0, None), "k_scale and v_scale overlap")
+
+
+def test_outputs_of_the_verification(lib):
+    """accepted (2, 2), count (2) and token (2) int32."""
+    for kw in (dict(accepted=P, count=P + 12, token=V), dict(accepted=P + 4, count=P, token=V), dict(accepted=P, count=V, token=P + 8),
+               dict(accepted=P, count=V, token=V + 4), dict(accepted=P, count=V + 4, token=V)):
+        assert says(lib, lib.mrt_draft_verify(verify(target=V << 4, draft=V << 5, **kw), None, 0, 0, None), "arrays of their own")
