@@ -900,7 +900,8 @@ typedef struct mrt_i8_matmul_args {
   const float* x_scale;  /* (rows) */
   const int8_t* w;       /* (n, k), row stride ldw */
   const float* w_scale;  /* (n) */
-  const void* add;       /* (rows, n) of `dtype`, row stride lda, or NULL; may be out itself */
+  const void* add;       /* (rows, n) of `dtype`, row stride lda, or NULL; may be out itself, with its row */
+                         /*   stride; with that stride the two may lie between each other, else their ranges are apart */
   void* out;             /* (rows, n) of `dtype`, row stride ldo */
   int64_t ldx;
   int64_t ldw;

@@ -51,3 +51,21 @@ def test_a_row_does_not_depend_on_its_batch(dtype):
         for n in (33, 1000, 6144, 12288, 13059):
             got = mrt_df.i8_matmul(x[:rows], xs[:rows], w[:n], ws[:n], add=add[:rows, :n])
             assert torch.equal(got, whole[:rows, :n]), (rows, n)
+
+
+@pytest.mark.parametrize("rows,k,n", [(1, 64, 40), (5, 64, 40), (64, 512, 500), (300, 640, 500), (520, 144, 13056)])
+def test_residuals_beside_the_output(rows, k, n):
+    """What is added lies between the output's rows, before it, or is the output itself."""
+    x, xs, w, ws = (t.to(DEV) for t in make(25, rows, k, n))
+    add = torch.randn((rows, n), generator=torch.Generator().manual_seed(26)).to(DEV)
+    want = mrt_df.i8_matmul(x, xs, w, ws, add=add)
+    both = torch.zeros((rows, 2 * n), device=DEV)
+    both[:, :n] = add
+    mrt_df.i8_matmul(x, xs, w, ws, add=both[:, :n], out=both[:, n:])
+    assert torch.equal(both[:, n:], want) and torch.equal(both[:, :n], add)
+    line = torch.zeros((2 * rows, n), device=DEV)
+    line[:rows] = add
+    mrt_df.i8_matmul(x, xs, w, ws, add=line[:rows], out=line[rows:])
+    assert torch.equal(line[rows:], want) and torch.equal(line[:rows], add)
+    mrt_df.i8_matmul(x, xs, w, ws, add=line[:rows], out=line[:rows])
+    assert torch.equal(line[:rows], want)

@@ -89,3 +89,10 @@ def test_outputs_of_the_verification(lib):
     for kw in (dict(accepted=P, count=P + 12, token=V), dict(accepted=P + 4, count=P, token=V), dict(accepted=P, count=V, token=P + 8),
                dict(accepted=P, count=V, token=V + 4), dict(accepted=P, count=V + 4, token=V)):
         assert says(lib, lib.mrt_draft_verify(verify(target=V << 4, draft=V << 5, **kw), None, 0, 0, None), "arrays of their own")
+
+
+def test_residuals(lib):
+    """add and out (4, 32) bf16, out at V: the very same, or apart."""
+    for kw in (dict(add=V + 8), dict(add=V + 64), dict(add=V - 2), dict(add=V + 64, ld=(64, 64, 0, 32)),
+               dict(add=V + 16, ld=(64, 64, 64, 64)), dict(add=V + 2, rows=1), dict(add=V + 128, ld=(64, 64, 64, 32))):
+        assert says(lib, lib.mrt_i8_matmul(product(**kw), 0, None), "add overlaps out")
