@@ -1427,10 +1427,13 @@ class PagedCache:
     k_scale, v_scale (pages, kv_heads, page_size) fp32.  table int32 (rows,
     row_pages): the page of each page_size entries of a sequence, an id outside
     the pool where there is none; length int32 (rows), the entries in use.  The
-    tensors are kept, not copied.
+    tensors are kept, not copied: what they hold may change between calls, which
+    they are may not (a cache with other lengths is a new object).
     """
 
-    __slots__ = ("k", "v", "table", "length", "k_scale", "v_scale", "index", "kind", "shape", "rows", "row_pages", "_c")
+    __slots__ = ("_tensors", "_index", "_kind", "_shape", "_rows", "_row_pages", "_c")
+    k, v, table, length, k_scale, v_scale = (property(lambda self, i=i: self._tensors[i]) for i in range(6))
+    index, kind, shape, rows, row_pages = (property(lambda self, n=n: getattr(self, n)) for n in __slots__[1:6])
 
     def __init__(self, k, v, table, length, k_scale=None, v_scale=None):
         shape, stride, index, kind = k.shape, k.stride(), k.get_device(), _KIND[k.dtype]
@@ -1445,8 +1448,8 @@ class PagedCache:
             raise ValueError("pages: table must be int32 (rows, row_pages) on k's GPU, rows contiguous")
         if (kind == PAGES_I8) != (k_scale is not None and v_scale is not None) or (k_scale is None) != (v_scale is None):
             raise ValueError("pages: k_scale and v_scale go with int8 codes")
-        self.k, self.v, self.table, self.length, self.k_scale, self.v_scale = k, v, table, length, k_scale, v_scale
-        self.index, self.kind, self.shape, (self.rows, self.row_pages) = index, kind, shape, where
+        self._tensors = k, v, table, length, k_scale, v_scale
+        self._index, self._kind, self._shape, (self._rows, self._row_pages) = index, kind, shape, where
         ks = vs = 0
         if k_scale is not None:
             ks = _array(k_scale, shape[:3], DTYPE_F32, index, "k_scale")
@@ -1459,8 +1462,8 @@ class PagedCache:
 def _page_rows(t, shape, kind, cache, what):
     """Pointer and strides of a 4-d operand of the dtype ``kind``, which goes with the cache's pages."""
     s = t.stride()
-    if t.shape != shape or _KIND[t.dtype] != kind or t.get_device() != cache.index or s[3] != 1 or (
-            kind != cache.kind if cache.kind != PAGES_I8 else not 0 <= kind < PAGES_I8):
+    if t.shape != shape or _KIND[t.dtype] != kind or t.get_device() != cache._index or s[3] != 1 or (
+            kind != cache._kind if cache._kind != PAGES_I8 else not 0 <= kind < PAGES_I8):
         raise ValueError(f"{what} must be {tuple(shape)} of the pages' dtype, with int8 pages fp32, bf16 or fp16, on their GPU, "
                          "d contiguous")
     return t.data_ptr(), s[0], s[1], s[2]
@@ -1474,11 +1477,11 @@ def paged_write(cache: PagedCache, k_new, v_new, fresh=None, length_out=None) ->
     where the pages hold codes.  length_out, a tensor of its own, receives the
     new lengths.
     """
-    lib, index, rows = load_library(), cache.index, cache.rows
+    lib, index, rows = load_library(), cache._index, cache._rows
     if k_new.dim() != 4:
         raise ValueError("k_new must be (rows, tokens, kv_heads, d)")
     tokens, kind = k_new.shape[1], _KIND[k_new.dtype]
-    shape = (rows, tokens, cache.shape[1], cache.shape[3])
+    shape = (rows, tokens, cache._shape[1], cache._shape[3])
     args = _STORE_STRUCT.pack(*_page_rows(k_new, shape, kind, cache, "k_new"), *_page_rows(v_new, shape, kind, cache, "v_new"),
                               _array(fresh, (rows,), _INT32, index, "fresh"), 0,
                               _array(length_out, (rows,), _INT32, index, "length_out"), tokens, kind)
@@ -1493,11 +1496,11 @@ def paged_read(cache: PagedCache, k_out, v_out, start=None) -> None:
     k_out, v_out (rows, kv_heads, tokens, d), the layout of ``KVCache``; start
     int32 (rows), None: 0.  Entries past a sequence's length are left as they are.
     """
-    lib, index, rows = load_library(), cache.index, cache.rows
+    lib, index, rows = load_library(), cache._index, cache._rows
     if k_out.dim() != 4:
         raise ValueError("k_out must be (rows, kv_heads, tokens, d)")
     tokens, kind = k_out.shape[2], _KIND[k_out.dtype]
-    shape = (rows, cache.shape[1], tokens, cache.shape[3])
+    shape = (rows, cache._shape[1], tokens, cache._shape[3])
     k, v = _page_rows(k_out, shape, kind, cache, "k_out"), _page_rows(v_out, shape, kind, cache, "v_out")
     args = _STORE_STRUCT.pack(k[0], k[1], k[3], k[2], v[0], v[1], v[3], v[2], 0, _array(start, (rows,), _INT32, index, "start"), 0,
                               tokens, kind)
@@ -1523,9 +1526,9 @@ def paged_attention(q, cache: PagedCache, fresh=None, scale: float = 1.0, bias=N
     (out (rows, tokens, heads, d), lse (rows, tokens, heads) fp32), new tensors
     unless given; tokens past fresh[b] get 0 and -inf.
     """
-    lib, index, shape, kind = load_library(), cache.index, q.shape, _KIND[q.dtype]
-    pages, kv_heads, page_size, d = cache.shape
-    if len(shape) != 4 or shape[0] != cache.rows or shape[3] != d:
+    lib, index, shape, kind = load_library(), cache._index, q.shape, _KIND[q.dtype]
+    pages, kv_heads, page_size, d = cache._shape
+    if len(shape) != 4 or shape[0] != cache._rows or shape[3] != d:
         raise ValueError("q must be (rows, tokens, heads, d) with the cache's rows and d")
     rows, tokens, heads, _ = shape
     rows_of_q = _page_rows(q, shape, kind, cache, "q")
@@ -1545,7 +1548,7 @@ def paged_attention(q, cache: PagedCache, fresh=None, scale: float = 1.0, bias=N
         table = _array(bias, (heads, buckets), DTYPE_F32, index, "bias")
     args = _PAGED_STRUCT.pack(*rows_of_q, *rows_of_out, _array(fresh, shape[:1], _INT32, index, "fresh"), lp, table, buckets,
                               tokens, heads, kind, scale)
-    size = _paged_workspace(rows, cache.row_pages, pages, kv_heads, page_size, d, cache.kind, heads, tokens)
+    size = _paged_workspace(rows, cache._row_pages, pages, kv_heads, page_size, d, cache._kind, heads, tokens)
     ws = q.new_empty(size, dtype=_KIND.u8) if size else None
     code = lib.mrt_paged_attention(cache._c, args, ws.data_ptr() if size else None, size, index, _KIND.stream(index))
     if code:
