@@ -1428,8 +1428,9 @@ int mrt_i8_matmul(const mrt_i8_matmul_args* args, int device, void* hip_stream) 
     require(args->rows == 1 || (args->ldo >= args->n && (args->add == nullptr || args->lda >= 0)),
             "i8_matmul: ldo must be >= n, lda not negative");
     require(args->add != args->out || args->rows == 1 || args->lda == args->ldo, "i8_matmul: add in place needs out's row stride");
-    const Vectors add(args->n, {args->rows, args->lda}, {1, 0}, {1, 0}), out(args->n, {args->rows, args->ldo}, {1, 0}, {1, 0});
-    require(args->add == nullptr || args->add == args->out || !share(add, args->add, out, args->out, size),
+    auto matrix = [&](int64_t ld) { return Vectors(args->n, {args->rows, ld}, {1, 0}, {1, 0}); };
+    require(args->add == nullptr || args->add == args->out ||
+                !share(matrix(args->lda), args->add, matrix(args->ldo), args->out, size),
             "i8_matmul: add overlaps out");
     mrt::I8Args a;
     a.x = args->x, a.x_scale = args->x_scale, a.w = args->w, a.w_scale = args->w_scale, a.add = args->add, a.out = args->out;
