@@ -12,9 +12,9 @@
 //
 // Pages of the operands' type: the fragments of attn_frag.hpp, 32 keys a step.
 //
-// Pages of 8-bit codes: 64 keys a step, and both products in integers.  Converting codes to
-// 16 bits would cost a vector instruction for two of them; instead the few query rows and
-// weights become three digits of 8 bits,
+// Pages of 8-bit codes: 64 keys a step.  For operands of 16 bits both products are in integers:
+// converting codes to 16 bits would cost a vector instruction for two of them; instead the few
+// query rows and weights become three digits of 8 bits,
 //   x = f (65536 a + 256 b + c),  a, b, c in [-128, 127],
 // f a power of two for the row (of weights: for the row and step) by which its largest
 // magnitude is in [2^21, 2^22), so that x is within 2^-22 of that magnitude; sums of products
@@ -22,6 +22,15 @@
 // lane (i, g) with keys 16 t + 4 g + r of the four tiles, just the 16 keys whose codes of one
 // dimension, transposed in registers by byte permutations, are its operand of
 // O^T = V^T P^T.
+//
+// Digits are relative to a row's largest magnitude.  Beside a channel of q 1000 times the others,
+// in which keys have little, the others keep 12 bits: enough for operands of 16 bits, which have
+// no more than 11.  Outputs of fp32 operands were 1.5e-4 off there, 5e-7 with plain fp32
+// products.  So q and the weights of fp32 are three bf16 parts each, which hold any value whole,
+// and codes become bf16, which holds them exactly: every product is exact in fp32, as over fp32
+// pages.  It costs the conversion, one and a half vector instructions a code: 48 x 8 heads of up
+// to 8191 of d 128 111 us (digits 96, the fp32 matrix instruction 172), 4 x 32000 of d 128 with 4
+// tokens of 4 heads 72 (63, 108), with 16 161 (131, 363), 16 x 16000 of d 256 51 (44, 83).
 //
 // Bound by bytes but for many rows a K/V head (16 new tokens of 4 heads on one over 8-bit pages
 // of 4 x 32000 entries, d 128: 127 us for 63 with 4, by vector instructions on the digits and the
@@ -350,9 +359,27 @@ struct CodeFrag {
       f[0] = ld_g(reinterpret_cast<const uint32_t*>(base + at));
     }
   }
-  // One query row: the digits of lane group g's 16 KC values, and f.
+  // Operands of 16 values: three digits, of fp32 three bf16 parts of each eight.
   template <typename T>
-  __device__ __forceinline__ static float digits(const T* row, int g, int D, uint4 (&a)[KC], uint4 (&b)[KC], uint4 (&c)[KC]) {
+  static constexpr int kParts = sizeof(T) == 4 ? 6 : 3;
+  // Eight fp32 values as three bf16 operands, whose sum they are (bits below 2^-133 are lost).
+  __device__ __forceinline__ static void split(const float* x, uint4 (&p)[3]) {
+    uint32_t w[3][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float a = x[2 * j], b = x[2 * j + 1];
+#pragma unroll
+      for (int e = 0; e < 3; ++e) {
+        w[e][j] = Mma<bf16>::pack(a, b);
+        a -= Mma<bf16>::low(w[e][j]), b -= Mma<bf16>::high(w[e][j]);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 3; ++e) p[e] = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
+  }
+  // One query row: lane group g's 16 KC values in units of f, as digits or in parts, and f.
+  template <typename T>
+  __device__ __forceinline__ static float query(const T* row, int g, int D, uint4 (&q)[KC][kParts<T>]) {
     float x[KC][16];
     uint32_t top = 0;
 #pragma unroll
@@ -376,21 +403,81 @@ struct CodeFrag {
     const float up = top < 0x7f800000u ? to_digits(top) : 0.f;
 #pragma unroll
     for (int k = 0; k < KC; ++k) {
-      uint32_t q[3][4];
 #pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        uint32_t y[4];
+      for (int j = 0; j < 16; ++j) x[k][j] *= up;
+      if constexpr (sizeof(T) == 4) {
+        uint4 p[3];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          y[j] = (uint32_t)((int)rintf(x[k][w * 4 + j] * up) + 0x808080);  // each digit and 128
+        for (int h = 0; h < 2; ++h) {
+          split(x[k] + 8 * h, p);
+#pragma unroll
+          for (int e = 0; e < 3; ++e) q[k][3 * h + e] = p[e];
         }
-        bytes_of(y, q[2][w], q[1][w], q[0][w]);
+      } else {
+        uint32_t p[3][4];
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t y[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) y[j] = (uint32_t)((int)rintf(x[k][w * 4 + j]) + 0x808080);  // each digit and 128
+          bytes_of(y, p[2][w], p[1][w], p[0][w]);
+        }
+#pragma unroll
+        for (int e = 0; e < 3; ++e)
+          q[k][e] = make_uint4(p[e][0] ^ 0x80808080u, p[e][1] ^ 0x80808080u, p[e][2] ^ 0x80808080u, p[e][3] ^ 0x80808080u);
       }
-      a[k] = make_uint4(q[0][0] ^ 0x80808080u, q[0][1] ^ 0x80808080u, q[0][2] ^ 0x80808080u, q[0][3] ^ 0x80808080u);
-      b[k] = make_uint4(q[1][0] ^ 0x80808080u, q[1][1] ^ 0x80808080u, q[1][2] ^ 0x80808080u, q[1][3] ^ 0x80808080u);
-      c[k] = make_uint4(q[2][0] ^ 0x80808080u, q[2][1] ^ 0x80808080u, q[2][2] ^ 0x80808080u, q[2][3] ^ 0x80808080u);
     }
     return from_digits(top);
+  }
+  // Two codes, byte ea of a and byte eb of b, in bf16, which holds them exactly: the upper halves
+  // of their fp32 values.
+  __device__ __forceinline__ static uint32_t pair(uint32_t a, int ea, uint32_t b, int eb) {
+    const float x = (float)(int8_t)(a >> (8 * ea)), y = (float)(int8_t)(b >> (8 * eb));
+    return __builtin_amdgcn_perm(__float_as_uint(y), __float_as_uint(x), 0x07060302u);
+  }
+  __device__ __forceinline__ static uint4 codes8(uint32_t a, uint32_t b) {
+    return make_uint4(pair(a, 0, a, 1), pair(a, 2, a, 3), pair(b, 0, b, 1), pair(b, 2, b, 3));
+  }
+  // Products of 16 keys with a query row, in units of f.
+  __device__ __forceinline__ static f32x4_t scores(const uint4 (&k)[KC], const uint4 (&q)[KC][3]) {
+    i32x4_t x = {0, 0, 0, 0}, y = x, z = x;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      x = mma8(k[c], q[c][0], x);
+      y = mma8(k[c], q[c][1], y);
+      z = mma8(k[c], q[c][2], z);
+    }
+    f32x4_t s;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) s[r] = join_digits(x[r], y[r], z[r]);
+    return s;
+  }
+  // Of the step's four tiles of keys with a row in parts, the lane's operand x at parts[64 x].
+  // Products of parts are exact in fp32; the small ones, below 2^-8 of the others, have sums of
+  // their own.
+  __device__ __forceinline__ static void scores(const uint4 (&k)[4][KC], const uint4* parts, f32x4_t (&s)[4]) {
+    f32x4_t low[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s[t] = low[t] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint4 q[3];
+#pragma unroll
+        for (int e = 0; e < 3; ++e) q[e] = parts[(c * 6 + 3 * h + e) * 64];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const uint4 x = h == 0 ? codes8(k[t][c].x, k[t][c].y) : codes8(k[t][c].z, k[t][c].w);
+          s[t] = Mma<bf16>::mma(x, q[0], s[t]);
+          low[t] = Mma<bf16>::mma(x, q[1], low[t]);
+          low[t] = Mma<bf16>::mma(x, q[2], low[t]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t) s[t] += low[t];
   }
   // 16 weights, not negative and below 2^22 by `up`: the digits, in the order of the
   // keys.  In [2^23, 2^24) a float's low bits count ones; 0x8080 adds 128 to two digits.
@@ -406,6 +493,29 @@ struct CodeFrag {
     a = make_uint4(q[0][0], q[0][1], q[0][2], q[0][3]);
     b = make_uint4(q[1][0] ^ 0x80808080u, q[1][1] ^ 0x80808080u, q[1][2] ^ 0x80808080u, q[1][3] ^ 0x80808080u);
     c = make_uint4(q[2][0] ^ 0x80808080u, q[2][1] ^ 0x80808080u, q[2][2] ^ 0x80808080u, q[2][3] ^ 0x80808080u);
+  }
+  // o += V^T P^T of fp32 weights: 16 keys of the lane's dimensions, v[4 t + j] and p[4 t + j] of
+  // key 16 t + 4 g + j.
+  __device__ __forceinline__ static void add_pv(const uint32_t (&v)[16][VW], const float (&p)[16], f32x4_t (&o)[E]) {
+    uint4 w[2][3];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) split(p + 8 * h, w[h]);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      f32x4_t low = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint32_t x[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] = pair(v[8 * h + 2 * j][e / 4], e % 4, v[8 * h + 2 * j + 1][e / 4], e % 4);
+        const uint4 a = make_uint4(x[0], x[1], x[2], x[3]);
+        o[e] = Mma<bf16>::mma(a, w[h][0], o[e]);
+        low = Mma<bf16>::mma(a, w[h][1], low);
+        low = Mma<bf16>::mma(a, w[h][2], low);
+      }
+      o[e] += low;
+      if (e & 1) __builtin_amdgcn_sched_barrier(0);  // values of all dimensions do not fit the registers
+    }
   }
   // Codes of dimensions 4 w .. 4 w + 3 of the lane, all 16 keys: operands of the four
   // output tiles.  v[4 t + j]: key 16 t + 4 g + j.
@@ -785,17 +895,26 @@ __global__ MRT_ATTN_BOUNDS(1, 1) void k_paged_codes(const PageArgs a) {
     __shared__ __attribute__((aligned(16))) float sc[W][128];  // the scales of a wave's step
     float* btab = reinterpret_cast<float*>(lds);
     const BiasTable table_of(a, btab, kvh, n);
-    uint4 qa[NR][KC], qb[NR][KC], qc[NR][KC];
+    constexpr int kParts = F::template kParts<T>;
+    uint4 q[NR][KC][kParts];
+    [[maybe_unused]] __shared__ uint4 parts[sizeof(T) == 4 ? NR * KC * kParts * 64 : 1];  // q of fp32, for all waves
     float qf[NR];
     int last[NR], head[NR];
 #pragma unroll
     for (int t = 0; t < NR; ++t) {
       const int r = min(row0 + t * 16 + i, R - 1), node = r / n, hq = r - node * n;
-      qf[t] = F::digits(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D,
-                        qa[t], qb[t], qc[t]) * a.scale * kLog2e;
+      qf[t] = F::query(static_cast<const T*>(a.q) + b * a.q_row + node * a.q_node + (int64_t)(kvh * n + hq) * a.q_head, g, D,
+                       q[t]) * a.scale * kLog2e;
       last[t] = node < fresh ? len + node : -1, head[t] = hq;
     }
-    if (a.bias != nullptr && table_of.fill(btab, n, 64 * W)) ring_barrier();  // does not wait for the loads of the first step
+    bool wrote = sizeof(T) == 4;
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int x = 0; x < NR * KC * kParts; ++x)
+        if (x % W == wid) parts[x * 64 + lane] = q[x / (KC * kParts)][x / kParts % KC][x % kParts];
+    }
+    if (a.bias != nullptr) wrote |= table_of.fill(btab, n, 64 * W);
+    if (wrote) ring_barrier();  // does not wait for the loads of the first step
 
     f32x4_t o[NR][E];
     float m[NR], l[NR];
@@ -805,7 +924,7 @@ __global__ MRT_ATTN_BOUNDS(1, 1) void k_paged_codes(const PageArgs a) {
 #pragma unroll
       for (int e = 0; e < E; ++e) o[t][e] = {0.f, 0.f, 0.f, 0.f};
     }
-    const i32x4_t zero = {0, 0, 0, 0};
+    [[maybe_unused]] const i32x4_t zero = {0, 0, 0, 0};
     // Keys at distances beyond the table's have its last value, unless that is a mask.
     float far[NR];
     bool plain = true;
@@ -829,20 +948,18 @@ __global__ MRT_ATTN_BOUNDS(1, 1) void k_paged_codes(const PageArgs a) {
       float p[NR][16];
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
+        [[maybe_unused]] f32x4_t all[4];
+        if constexpr (sizeof(T) == 4) F::scores(kf, parts + t * KC * kParts * 64 + lane, all);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          i32x4_t x = zero, y = zero, z = zero;
-#pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            x = mma8(kf[k][c], qa[t][c], x);
-            y = mma8(kf[k][c], qb[t][c], y);
-            z = mma8(kf[k][c], qc[t][c], z);
-          }
+          f32x4_t x;
+          if constexpr (sizeof(T) == 4) x = all[k];
+          else x = F::scores(kf[k], q[t]);
           const float4 s = *reinterpret_cast<const float4*>(&sc[wid][k * 16 + 4 * g]);
           const float by_key[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            p[t][4 * k + r] = join_digits(x[r], y[r], z[r]) * qf[t] * by_key[r];
+            p[t][4 * k + r] = x[r] * qf[t] * by_key[r];
             asm volatile("" : "+v"(p[t][4 * k + r]));  // here: the sums of all tiles do not fit the registers
           }
           __builtin_amdgcn_sched_barrier(0);
@@ -856,8 +973,8 @@ __global__ MRT_ATTN_BOUNDS(1, 1) void k_paged_codes(const PageArgs a) {
         find(st + W);
         load_k(st + W);
       }
-      uint4 wa[NR], wb[NR], wc[NR];
-      float wf[NR];
+      [[maybe_unused]] uint4 wa[NR], wb[NR], wc[NR];
+      [[maybe_unused]] float wf[NR];
 #pragma unroll
       for (int t = 0; t < NR; ++t) {
         float sv[16];
@@ -904,24 +1021,30 @@ __global__ MRT_ATTN_BOUNDS(1, 1) void k_paged_codes(const PageArgs a) {
           p[t][j] = x * sv[j];
           size = max(size, __float_as_uint(p[t][j]));  // bits of what is not negative order as the values do, NaN above all
         }
-        size = max_bits_over_groups(size);
-        F::digits(p[t], to_digits(size), wa[t], wb[t], wc[t]);
-        wf[t] = from_digits(size);
+        if constexpr (sizeof(T) == 4) {
+          F::add_pv(vf, p[t], o[t]);
+        } else {
+          size = max_bits_over_groups(size);
+          F::digits(p[t], to_digits(size), wa[t], wb[t], wc[t]);
+          wf[t] = from_digits(size);
+        }
       }
+      if constexpr (sizeof(T) != 4) {
 #pragma unroll
-      for (int x = 0; x < VW; ++x) {
-        uint4 op[4];
-        F::transpose(vf, x, op);
+        for (int x = 0; x < VW; ++x) {
+          uint4 op[4];
+          F::transpose(vf, x, op);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
+          for (int e = 0; e < 4; ++e) {
 #pragma unroll
-          for (int t = 0; t < NR; ++t) {
-            const i32x4_t u = mma8(op[e], wa[t], zero), v = mma8(op[e], wb[t], zero), y = mma8(op[e], wc[t], zero);
+            for (int t = 0; t < NR; ++t) {
+              const i32x4_t u = mma8(op[e], wa[t], zero), v = mma8(op[e], wb[t], zero), y = mma8(op[e], wc[t], zero);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) o[t][4 * x + e][r] = fmaf(join_digits(u[r], v[r], y[r]), wf[t], o[t][4 * x + e][r]);
-            asm volatile("" : "+v"(o[t][4 * x + e]));
+              for (int r = 0; r < 4; ++r) o[t][4 * x + e][r] = fmaf(join_digits(u[r], v[r], y[r]), wf[t], o[t][4 * x + e][r]);
+              asm volatile("" : "+v"(o[t][4 * x + e]));
+            }
+            if (e & 1) __builtin_amdgcn_sched_barrier(0);
           }
-          if (e & 1) __builtin_amdgcn_sched_barrier(0);
         }
       }
       if (more) load_v();
