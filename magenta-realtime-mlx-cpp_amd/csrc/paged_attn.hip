@@ -403,9 +403,9 @@ struct CodeFrag {
     const float up = top < 0x7f800000u ? to_digits(top) : 0.f;
 #pragma unroll
     for (int k = 0; k < KC; ++k) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) x[k][j] *= up;
       if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) x[k][j] *= up;
         uint4 p[3];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -419,7 +419,7 @@ struct CodeFrag {
         for (int w = 0; w < 4; ++w) {
           uint32_t y[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) y[j] = (uint32_t)((int)rintf(x[k][w * 4 + j]) + 0x808080);  // each digit and 128
+          for (int j = 0; j < 4; ++j) y[j] = (uint32_t)((int)rintf(x[k][w * 4 + j] * up) + 0x808080);  // each digit and 128
           bytes_of(y, p[2][w], p[1][w], p[0][w]);
         }
 #pragma unroll
@@ -438,22 +438,8 @@ struct CodeFrag {
   __device__ __forceinline__ static uint4 codes8(uint32_t a, uint32_t b) {
     return make_uint4(pair(a, 0, a, 1), pair(a, 2, a, 3), pair(b, 0, b, 1), pair(b, 2, b, 3));
   }
-  // Products of 16 keys with a query row, in units of f.
-  __device__ __forceinline__ static f32x4_t scores(const uint4 (&k)[KC], const uint4 (&q)[KC][3]) {
-    i32x4_t x = {0, 0, 0, 0}, y = x, z = x;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      x = mma8(k[c], q[c][0], x);
-      y = mma8(k[c], q[c][1], y);
-      z = mma8(k[c], q[c][2], z);
-    }
-    f32x4_t s;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) s[r] = join_digits(x[r], y[r], z[r]);
-    return s;
-  }
-  // Of the step's four tiles of keys with a row in parts, the lane's operand x at parts[64 x].
-  // Products of parts are exact in fp32; the small ones, below 2^-8 of the others, have sums of
+  // Products of the step's four tiles of keys with a row in parts, in units of f; the lane's operand
+  // x is at parts[64 x].  Products of parts are exact in fp32; the small ones, below 2^-8 of the others, have sums of
   // their own.
   __device__ __forceinline__ static void scores(const uint4 (&k)[4][KC], const uint4* parts, f32x4_t (&s)[4]) {
     f32x4_t low[4];
@@ -907,14 +893,13 @@ __global__ MRT_ATTN_BOUNDS(1, 1) void k_paged_codes(const PageArgs a) {
                        q[t]) * a.scale * kLog2e;
       last[t] = node < fresh ? len + node : -1, head[t] = hq;
     }
-    bool wrote = sizeof(T) == 4;
     if constexpr (sizeof(T) == 4) {
 #pragma unroll
       for (int x = 0; x < NR * KC * kParts; ++x)
         if (x % W == wid) parts[x * 64 + lane] = q[x / (KC * kParts)][x / kParts % KC][x % kParts];
     }
-    if (a.bias != nullptr) wrote |= table_of.fill(btab, n, 64 * W);
-    if (wrote) ring_barrier();  // does not wait for the loads of the first step
+    // does not wait for the loads of the first step
+    if ((a.bias != nullptr && table_of.fill(btab, n, 64 * W)) || sizeof(T) == 4) ring_barrier();
 
     f32x4_t o[NR][E];
     float m[NR], l[NR];
@@ -952,14 +937,21 @@ __global__ MRT_ATTN_BOUNDS(1, 1) void k_paged_codes(const PageArgs a) {
         if constexpr (sizeof(T) == 4) F::scores(kf, parts + t * KC * kParts * 64 + lane, all);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          f32x4_t x;
-          if constexpr (sizeof(T) == 4) x = all[k];
-          else x = F::scores(kf[k], q[t]);
+          [[maybe_unused]] i32x4_t x = zero, y = zero, z = zero;
+          if constexpr (sizeof(T) != 4) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+              x = mma8(kf[k][c], q[t][c][0], x);
+              y = mma8(kf[k][c], q[t][c][1], y);
+              z = mma8(kf[k][c], q[t][c][2], z);
+            }
+          }
           const float4 s = *reinterpret_cast<const float4*>(&sc[wid][k * 16 + 4 * g]);
           const float by_key[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            p[t][4 * k + r] = x[r] * qf[t] * by_key[r];
+            if constexpr (sizeof(T) == 4) p[t][4 * k + r] = all[k][r] * qf[t] * by_key[r];
+            else p[t][4 * k + r] = join_digits(x[r], y[r], z[r]) * qf[t] * by_key[r];
             asm volatile("" : "+v"(p[t][4 * k + r]));  // here: the sums of all tiles do not fit the registers
           }
           __builtin_amdgcn_sched_barrier(0);
