@@ -843,7 +843,7 @@ typedef struct mrt_paged_attention_args {
  * see, are treated as in mrt_tree_attention.  Over codes a row of q that holds an
  * infinity or NaN gives NaN, and one whose largest magnitude is below 2^-104 counts as 0.
  * With fp32 operands products with codes are exact and summed in fp32, whatever the
- * magnitudes beside them.  With operands of 16 bits q is taken as whole multiples of 2^-22
+ * magnitudes beside them (what weights times scales have below 2^-126 may be lost).  With operands of 16 bits q is taken as whole multiples of 2^-22
  * (or up to 2^-21) of its largest magnitude, and weights times scales likewise among 64
  * entries; where those are below 2^-104 they count as 0. */
 int mrt_paged_attention_workspace(const mrt_paged_cache* cache, int heads, int tokens, size_t* bytes);
